@@ -172,7 +172,7 @@ def _norm_inputs(case, gen):
         w = 1 + _normal(gen, d, by=0.2)
         return (w, _normal(gen, d, by=0.2)) if layer else (w, None)
 
-    shape = {"none": None, "vector": (d,), "image": (b, 1, d), "row": (b, t, d)}[case["gate"]]
+    shape = {"none": None, "vector": (d,), "image": (b, d), "row": (b, t, d)}[case["gate"]]
     s = dict(x=_normal(gen, b, t, d, type=x, by=3.0), z=_normal(gen, b, t, d, type=z),
              gate=None if shape is None else _normal(gen, *shape, type=z),
              scale=_normal(gen, d, by=0.5) if case["scale"] else None, post=weights(case["post"]),
@@ -271,13 +271,18 @@ def _normed(v, w, layer):
     return hat, r, hat * w[0] + w[1] if layer else hat * w[0]
 
 
+def _gate(case, s):
+    """The gate as fp32 factors of [B, T, D] rows; [B, D] holds one an image."""
+    return s["gate"].float()[:, None] if case["gate"] == "image" else s["gate"].float()
+
+
 def _norm_parts(case, s):
     layer = case["kind"] == "layer"
     z = s["z"].float()
     zhat, zr, n = _normed(z, s["post"], layer) if s["post"] else (None, None, z)
     factor = 1.0
     if s["gate"] is not None:
-        factor = s["gate"].float()
+        factor = _gate(case, s)
     if s["scale"] is not None:
         factor = factor * s["scale"]
     y = s["x"].float() + factor * n
@@ -308,11 +313,11 @@ def _norm_back(case, s):
     out["dx"] = dy.to(s["x"].dtype)
     dn = dy * factor
     if s["scale"] is not None:
-        out["scale"] = (dy * n * (1.0 if s["gate"] is None else s["gate"].float())).sum((0, 1))
+        out["scale"] = (dy * n * (1.0 if s["gate"] is None else _gate(case, s))).sum((0, 1))
     if s["gate"] is not None:
         dg = dy * n * (1.0 if s["scale"] is None else s["scale"])
         # a gate of a whole image or of all rows gets its sum in fp32, one of each row its own type
-        out["gate"] = {"vector": lambda: dg.sum((0, 1)), "image": lambda: dg.sum(1, keepdim=True),
+        out["gate"] = {"vector": lambda: dg.sum((0, 1)), "image": lambda: dg.sum(1),
                        "row": lambda: dg.to(s["gate"].dtype)}[case["gate"]]()
     if s["post"]:
         out["post_w"], out["post_b"] = (dn * zhat).sum((0, 1)), dn.sum((0, 1)) if layer else None
@@ -409,8 +414,10 @@ def _exact_norm(case, s, grads):
     x, z, gate, scale = (wide(s[n]) for n in ("x", "z", "gate", "scale"))
     post, pre = (tuple(wide(w) for w in s[n]) if s[n] else None for n in ("post", "pre"))
     part = norm(z, post) if post else z
-    for factor in (gate, scale):
-        part = part if factor is None else part * factor
+    if gate is not None:
+        part = part * (gate[:, None] if case["gate"] == "image" else gate)
+    if scale is not None:
+        part = part * scale
     y = x + part
     h = norm(y, pre) if pre else None
     if not grads:
