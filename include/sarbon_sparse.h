@@ -48,6 +48,7 @@ extern "C" {
 #define SB_F16 0
 #define SB_F32 1
 #define SB_F8  2
+#define SB_BF16 3  /* operands of the memory-reading block (sb_cross_attention and after) only */
 
 /* step modes (fused_engine.py:230-237) */
 #define SB_MODE_SKIP   0
@@ -447,6 +448,86 @@ SB_API int sb_box_dec(int first, const void* prebox, long long ldp, const void* 
 
 /* F.normalize(x.float(), dim=-1) of fp16 rows into fp32 rows (sarbon_det.py:359-360). */
 SB_API int sb_l2norm_rows(const void* x, long long ldx, int rows, int D, float* out, long long ldo, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * A transformer block that reads an encoder's memory, forward and backward, beside the
+ * detector's own kernels.  No reference counterpart.  Rows are addressed in elements: element
+ * (b, t, c) of a [B][T][C] operand is at ptr[b * img + t * row + c]; `row` may exceed C (a slice
+ * of a wider projection) and `img` may be 0 for inputs (one memory for every item).  Each call
+ * launches on `stream`, allocates nothing and may be captured in a CUDA graph after a first call
+ * outside capture on the device.  dtype codes: SB_F16, SB_BF16 and, where said, SB_F32. */
+
+/* Attention of Tq queries to an encoder's Tk states, out = softmax(scale q k^T) v per head.
+ * H query heads of dh = 32, 64 or 128 channels (head h = columns h*dh ..), Hkv key / value heads,
+ * H % Hkv == 0, query head h reads key head h / (H / Hkv).  q, k, v, out have one dtype (SB_F16 or
+ * SB_BF16), 16-byte aligned bases, row and img multiples of 8.  Key j of item b takes part when
+ * j < lens[b] (int32 [B], NULL: Tk; values outside [0, Tk] are clamped) and valid[b * valid_img + j]
+ * != 0 (uint8, NULL: all).  Keys that do not take part may hold anything, NaN included.  A query
+ * without keys gets a zero row.  lse (fp32 [B][H][Tq], NULL: none): natural log of the sum of the
+ * exponentials, -inf without keys.  scale > 0.  work: sb_cross_attention_work bytes (16-byte
+ * aligned), not shared by calls that may overlap.  Scores, statistics and sums are fp32; the
+ * probabilities are rounded to dtype before they meet v. */
+SB_API int sb_cross_attention(const void* q, long long q_row, long long q_img, const void* k, long long k_row,
+                              long long k_img, const void* v, long long v_row, long long v_img, int dtype, int B, int H,
+                              int Hkv, int dh, int Tq, int Tk, float scale, const int* lens, const void* valid,
+                              long long valid_img, void* out, long long o_row, long long o_img, float* lse, void* work,
+                              long long work_bytes, void* stream);
+
+/* Bytes of workspace that sb_cross_attention (backward = 0) or sb_cross_attention_backward
+ * (backward = 1) needs for these sizes on the current device (0: work may be NULL). */
+SB_API int sb_cross_attention_work(int backward, int B, int H, int Hkv, int dh, int Tq, int Tk, long long* bytes);
+
+/* Gradients of sb_cross_attention: dq [B][Tq][H*dh], dk, dv [B][Tk][Hkv*dh] (every element is
+ * written; keys that take no part get zeros) from dout and the forward pass's out and lse. Sums
+ * over queries, keys and the query heads of a key head are fp32 and in a fixed order: the same
+ * inputs give the same bits. */
+SB_API int sb_cross_attention_backward(const void* dout, long long do_row, long long do_img, const void* q, long long q_row,
+                                       long long q_img, const void* k, long long k_row, long long k_img, const void* v,
+                                       long long v_row, long long v_img, const void* out, long long o_row,
+                                       long long o_img, const float* lse, int dtype, int B, int H, int Hkv, int dh, int Tq,
+                                       int Tk, float scale, const int* lens, const void* valid, long long valid_img,
+                                       void* dq, long long dq_row, long long dq_img, void* dk, long long dk_row,
+                                       long long dk_img, void* dv, long long dv_row, long long dv_img, void* work,
+                                       long long work_bytes, void* stream);
+
+/* Rotary positions with several axes: pair p < R of every head is turned by the angle
+ * pos[b, t, axis[p]] * freq[p] (inverse != 0: by its negative, the gradient).  The pair is
+ * channels (p, p + R) of the head (pairs = 0) or (2p, 2p + 1) (pairs = 1); channels from 2R on are
+ * copied.  x, out: SB_F16, SB_BF16 or SB_F32 [B][T][H*dh], may be the same rows; pos int32
+ * (pos_f32 = 0) or fp32 [B][T][A] at pos[b * pos_img + t * A + a]; freq fp64 [R] radians a
+ * position, axis int32 [R] (an axis outside [0, A) leaves its pair as it is). */
+SB_API int sb_rope_axes(const void* x, long long x_row, long long x_img, int dtype, int B, int T, int H, int dh,
+                        const void* pos, int pos_f32, long long pos_img, int A, const double* freq, const int* axis, int R,
+                        int pairs, int inverse, void* out, long long o_row, long long o_img, void* stream);
+
+/* The end of one block and the start of the next:
+ *   n = Npost(z) (or z),  y = x + scale * gate * n,  h = Npre(y) (or absent)
+ * over B x T rows of D <= 8192 channels.  Norms: layer = 0 RMS, 1 layer norm, each with weights w
+ * [D] and (layer norm) biases b [D] or NULL, fp32; post_w / pre_w NULL: no such norm.  scale fp32
+ * [D] or NULL.  gate: elements gate[b * gate_img + t * gate_row + c] of z's dtype or NULL; strides 0
+ * broadcast it.  x, y: x_dtype, z, h, gate: z_dtype (SB_F16, SB_BF16, SB_F32).  Statistics are fp32
+ * and h comes from y before its rounding. */
+SB_API int sb_gated_norm(const void* x, long long x_row, long long x_img, int x_dtype, const void* z, long long z_row,
+                         long long z_img, int z_dtype, const void* gate, long long gate_row, long long gate_img,
+                         const float* scale, const float* post_w, const float* post_b, const float* pre_w,
+                         const float* pre_b, int layer, float eps, int B, int T, int D, void* y, long long y_row,
+                         long long y_img, void* h, long long h_row, long long h_img, void* stream);
+
+/* Bytes of workspace that sb_gated_norm_backward needs for these sizes on the current device. */
+SB_API int sb_gated_norm_work(int B, int T, int D, long long* bytes);
+
+/* Gradients of sb_gated_norm from dy (x_dtype, NULL: 0) and dh (z_dtype, NULL: 0): dx (x_dtype) and
+ * dz (z_dtype) contiguous [B][T][D]; fp32 [D] dscale, dpost_w, dpost_b, dpre_w, dpre_b (each may be
+ * NULL); dgate: mode 0 none, 1 fp32 [D] (one gate for all rows), 2 fp32 [B][D] (one an item), 3
+ * z_dtype [B][T][D] (one a row).  Column sums are fp32 in a fixed order. */
+SB_API int sb_gated_norm_backward(const void* dy, long long dy_row, long long dy_img, const void* dh, long long dh_row,
+                                  long long dh_img, const void* x, long long x_row, long long x_img, int x_dtype,
+                                  const void* z, long long z_row, long long z_img, int z_dtype, const void* gate,
+                                  long long gate_row, long long gate_img, const float* scale, const float* post_w,
+                                  const float* post_b, const float* pre_w, const float* pre_b, int layer, float eps, int B,
+                                  int T, int D, void* dx, void* dz, float* dscale, void* dgate, int dgate_mode,
+                                  float* dpost_w, float* dpost_b, float* dpre_w, float* dpre_b, void* work,
+                                  long long work_bytes, void* stream);
 
 /* Counters (fused_engine.py:92,239) and sticky device errors (synchronises). */
 SB_API int sb_stats(sb_engine* e, void* stream, sb_stats_t* out);

@@ -11,7 +11,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libsarbon_sparse.so"
 
 SB_OK, SB_EINVAL, SB_EOVERFLOW, SB_ETIMEOUT, SB_ECUDA, SB_ENOMEM = range(6)
-SB_F16, SB_F32, SB_F8 = 0, 1, 2
+SB_F16, SB_F32, SB_F8, SB_BF16 = 0, 1, 2, 3
 SB_MODE_SKIP, SB_MODE_SPARSE, SB_MODE_DENSE = 0, 1, 2
 MODE_NAMES = ("skip", "sparse", "dense")
 SB_CREATE_BLOCK_UNITS = 1
@@ -107,6 +107,16 @@ PROTOTYPES = {
     "sb_box_enc": (_I, [_P, _LL, _P, _I, _P, _I, _I, _P, _P, _LL, _P]),
     "sb_box_dec": (_I, [_I, _P, _LL, _P, _P, _LL, _P, _LL, _I, _P, C.c_float, _P, _P, _P, _LL, _I, _P]),
     "sb_l2norm_rows": (_I, [_P, _LL, _I, _I, _P, _LL, _P]),
+    "sb_cross_attention": (_I, [_P, _LL, _LL] * 3 + [_I] * 7 + [C.c_float, _P, _P, _LL, _P, _LL, _LL, _P, _P, _LL, _P]),
+    "sb_cross_attention_work": (_I, [_I] * 7 + [C.POINTER(_LL)]),
+    "sb_cross_attention_backward": (_I, [_P, _LL, _LL] * 5 + [_P] + [_I] * 7 + [C.c_float, _P, _P, _LL]
+                                    + [_P, _LL, _LL] * 3 + [_P, _LL, _P]),
+    "sb_rope_axes": (_I, [_P, _LL, _LL, _I, _I, _I, _I, _I, _P, _I, _LL, _I, _P, _P, _I, _I, _I, _P, _LL, _LL, _P]),
+    "sb_gated_norm": (_I, [_P, _LL, _LL, _I] * 2 + [_P, _LL, _LL] + [_P] * 5 + [_I, C.c_float, _I, _I, _I]
+                      + [_P, _LL, _LL] * 2 + [_P]),
+    "sb_gated_norm_work": (_I, [_I, _I, _I, C.POINTER(_LL)]),
+    "sb_gated_norm_backward": (_I, [_P, _LL, _LL] * 2 + [_P, _LL, _LL, _I] * 2 + [_P, _LL, _LL] + [_P] * 5
+                               + [_I, C.c_float, _I, _I, _I] + [_P] * 4 + [_I] + [_P] * 5 + [_LL, _P]),
     "sb_stats": (_I, [_P, _P, C.POINTER(Stats)]),
     "sb_last_launch_count": (_I, [_P]),
     "sb_destroy": (_I, [_P]),

@@ -1,0 +1,584 @@
+"""The memory-reading block's operators against their formulas in 64 bits.
+
+Bounds: a value rounded to type t is off by at most u = eps(t) / 2 of itself.  Attention rounds its
+probabilities (and dS in the backward pass) once to the inputs' type before the second product, so an
+output sum_j p_j v_j is off by at most u (|out| + sum_j p_j |v_j|); fp16 probabilities below 2^-14 are
+rounded by at most 2^-25 absolutely.  Everything else is fp32: scores are off by at most
+(dim + 2) 2^-24 sum |q||k| scale, the exponential by a few 2^-22, sums by a few 2^-22 of their
+absolute terms; ``FP32`` = 2^-18 of the absolute terms covers these."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+FP32 = 2.0 ** -18
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU tests need CUDA")
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rand(g, *shape, dtype=torch.float32, by=1.0):
+    return (torch.randn(*shape, device="cuda", generator=g) * by).to(dtype)
+
+
+def unit(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def heads_of(x, heads, groups):
+    """[B, T, heads * dim] -> fp64 [B, groups, heads / groups, T, dim]."""
+    return x.double().unflatten(-1, (groups, heads // groups, -1)).permute(0, 2, 3, 1, 4)
+
+
+def rows_of(x):
+    return x.permute(0, 3, 1, 2, 4).flatten(2)
+
+
+def keep_of(b, tk, lens, valid):
+    keep = torch.ones(b, tk, dtype=torch.bool, device="cuda")
+    if lens is not None:
+        keep &= torch.arange(tk, device="cuda") < lens[:, None]
+    return keep if valid is None else keep & (valid != 0)
+
+
+def formula(q, k, v, heads, kv_heads, lens, valid, scale=None):
+    """(out, lse, P, q, k, v) in fp64, keys that take no part left out of every sum."""
+    q, k, v = heads_of(q, heads, kv_heads), heads_of(k, kv_heads, kv_heads), heads_of(v, kv_heads, kv_heads)
+    keep = keep_of(q.shape[0], k.shape[3], lens, valid)
+    k, v = (x.masked_fill(~keep[:, None, None, :, None], 0) for x in (k, v))
+    s = q @ k.transpose(-1, -2) * (scale or q.shape[-1] ** -0.5)
+    s = s.masked_fill(~keep[:, None, None, None], -math.inf)
+    lse = torch.logsumexp(s, -1) if s.shape[-1] else s.new_full(s.shape[:-1], -math.inf)
+    p = torch.where(lse[..., None] == -math.inf, 0.0, torch.exp(s - lse[..., None]))
+    return p @ v, lse, p, q, k, v
+
+
+def slack_of(q, k, scale=None):
+    """Relative error of a probability from the fp32 scores."""
+    s = q.abs() @ k.abs().transpose(-1, -2) * (scale or q.shape[-1] ** -0.5)
+    return FP32 + 2 * (q.shape[-1] + 2) * 2.0 ** -24 * (s.amax().item() if s.numel() else 0.0)
+
+
+def check_forward(out, lse, q, k, v, heads, kv_heads, lens, valid, scale=None):
+    ref, ref_lse, p, qd, kd, vd = formula(q, k, v, heads, kv_heads, lens, valid, scale)
+    u, e = unit(q.dtype), slack_of(qd, kd, scale)
+    tol = u * ref.abs() + (u + e) * (p @ vd.abs()) + 1e-30
+    if q.dtype == torch.float16:
+        tol = tol + 2.0 ** -25 * (2 + vd.abs().sum(-2, keepdim=True))
+    err = (out.double() - rows_of(ref)).abs()
+    assert out.isfinite().all()
+    assert (err <= 1.02 * rows_of(tol)).all(), (err / rows_of(tol)).max().item()
+    if lse is not None:
+        ref_lse = ref_lse.flatten(1, 2)
+        none = ref_lse == -math.inf
+        assert torch.equal(lse == -math.inf, none)
+        assert ((lse.double() - ref_lse).abs()[~none] <= e * (1 + ref_lse.abs()[~none])).all()
+    return ref, p
+
+
+TYPES = [torch.float16, torch.bfloat16]
+
+
+# one key, a full tile of 128 and its neighbours, several tiles, more query rows than a tile
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,tq,tk,heads,kv_heads,dim", [
+    (2, 300, 240, 8, 8, 32), (1, 1, 1, 1, 1, 64), (2, 5, 77, 4, 2, 128), (1, 128, 128, 2, 1, 64),
+    (3, 129, 127, 3, 3, 32), (2, 257, 385, 6, 2, 128), (1, 130, 129, 7, 1, 64), (4, 1, 2040, 8, 2, 128),
+    (1, 1, 4097, 5, 1, 32), (2, 33, 1000, 12, 4, 64), (1, 513, 64, 2, 2, 128), (1, 3, 9001, 1, 1, 128),
+])
+def test_cross_attention(b, tq, tk, heads, kv_heads, dim, dtype):
+    import sarbon_b200 as sb
+    g = gen(tq * 7 + tk)
+    q = rand(g, b, tq, heads * dim, dtype=dtype)
+    k, v = rand(g, b, tk, kv_heads * dim, dtype=dtype), rand(g, b, tk, kv_heads * dim, dtype=dtype)
+    lse = torch.empty(b, heads, tq, device="cuda")
+    out = sb.cross_attention(q, k, v, heads, kv_heads=kv_heads, lse=lse)
+    check_forward(out, lse, q, k, v, heads, kv_heads, None, None)
+    assert torch.equal(out, sb.cross_attention(q, k, v, heads, kv_heads=kv_heads))  # with and without lse, twice
+
+
+MASKS = ["lens", "valid", "both", "none_left", "ends", "holes"]
+
+
+def masks_of(kind, b, tk, g):
+    lens = valid = None
+    if kind in ("lens", "both"):
+        lens = torch.tensor([(tk * (i + 1)) // b - (i == 0) for i in range(b)], dtype=torch.int32, device="cuda")
+    if kind in ("valid", "both"):
+        valid = (torch.rand(b, tk, device="cuda", generator=g) < 0.6).to(torch.uint8)
+    if kind == "none_left":
+        lens = torch.tensor([0, tk] + [-5] * (b - 2), dtype=torch.int32, device="cuda")[:b]
+        valid = torch.ones(b, tk, dtype=torch.bool, device="cuda")
+        valid[min(1, b - 1)] = False
+    if kind == "ends":  # outside [0, Tk]: clamped
+        lens = torch.tensor([1, tk + 1000, 2 ** 31 - 1, 128][:b], dtype=torch.int32, device="cuda")
+    if kind == "holes":  # whole tiles without a key between tiles with some
+        valid = torch.zeros(b, tk, dtype=torch.uint8, device="cuda")
+        valid[:, tk // 2] = 1
+        valid[0, -1] = 255
+    return lens, valid
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", MASKS)
+@pytest.mark.parametrize("tq,tk,heads,kv_heads,dim", [(70, 300, 4, 2, 64), (1, 700, 4, 1, 128), (150, 129, 2, 2, 32),
+                                                      (260, 520, 2, 1, 128)])
+def test_cross_attention_masks(kind, tq, tk, heads, kv_heads, dim, dtype):
+    """Masked places hold NaN and infinities; a row without keys gives zeros."""
+    import sarbon_b200 as sb
+    g = gen(tk + len(kind))
+    b = 4
+    q = rand(g, b, tq, heads * dim, dtype=dtype)
+    kv = rand(g, b, tk, 2 * kv_heads * dim, dtype=dtype)
+    lens, valid = masks_of(kind, b, tk, g)
+    away = ~keep_of(b, tk, lens, valid)
+    kv[away] = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(dtype).min], device="cuda", dtype=dtype).repeat(
+        kv.shape[-1] // 4)
+    k, v = kv[..., :kv_heads * dim], kv[..., kv_heads * dim:]
+    lse = torch.empty(b, heads, tq, device="cuda")
+    out = sb.cross_attention(q, k, v, heads, kv_heads=kv_heads, lens=lens, valid=valid, lse=lse)
+    check_forward(out, lse, q, k, v, heads, kv_heads, lens, valid)
+    if kind == "none_left":
+        assert not out[0].any() and not out[1].any()
+
+
+def test_cross_attention_strides_and_scale():
+    """Sequence-first rows, a slice of a wider projection, one memory for all items, out in place of a
+    slice; what lies around out stays as it was."""
+    import sarbon_b200 as sb
+    g = gen(5)
+    b, tq, tk, heads, dim = 3, 45, 200, 4, 64
+    q = rand(g, tq, b, heads * dim, dtype=torch.bfloat16).transpose(0, 1)
+    wide = rand(g, 1, tk, 3 * heads * dim, dtype=torch.bfloat16)
+    k = wide[..., :heads * dim].expand(b, -1, -1)
+    v = wide[..., 2 * heads * dim:].expand(b, -1, -1)
+    hold = torch.full((b, tq + 2, heads * dim + 8), 7.0, device="cuda", dtype=torch.bfloat16)
+    out = hold[:, 1:-1, 8:]
+    assert sb.cross_attention(q, k, v, heads, scale=0.3, out=out) is out
+    check_forward(out, None, q, k, v, heads, heads, None, None, scale=0.3)
+    assert (hold[:, 0] == 7).all() and (hold[:, -1] == 7).all() and (hold[..., :8] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_cross_attention_large_scores(dtype):
+    """Scores that grow from tile to tile and differ by hundreds: the running maximum moves often."""
+    import sarbon_b200 as sb
+    g = gen(6)
+    b, tq, tk, heads, dim = 1, 140, 1500, 2, 64
+    q = rand(g, b, tq, heads * dim, dtype=dtype)
+    ramp = torch.linspace(0.1, 6.0, tk, device="cuda")[None, :, None]
+    k = (rand(g, b, tk, heads * dim) * ramp).to(dtype)
+    v = rand(g, b, tk, heads * dim, dtype=dtype)
+    lse = torch.empty(b, heads, tq, device="cuda")
+    out = sb.cross_attention(q, k, v, heads, scale=1.0, lse=lse)
+    check_forward(out, lse, q, k, v, heads, heads, None, None, scale=1.0)
+
+
+def test_cross_attention_empty_sizes():
+    import sarbon_b200 as sb
+    z = dict(device="cuda", dtype=torch.float16)
+    assert sb.cross_attention(torch.zeros(0, 3, 64, **z), torch.zeros(0, 5, 64, **z), torch.zeros(0, 5, 64, **z), 1).shape == (0, 3, 64)
+    assert sb.cross_attention(torch.zeros(2, 0, 64, **z), torch.zeros(2, 5, 64, **z), torch.zeros(2, 5, 64, **z), 1).shape == (2, 0, 64)
+    lse = torch.zeros(2, 2, 3, device="cuda")
+    q, none = torch.ones(2, 3, 64, **z), torch.zeros(2, 0, 64, **z)
+    out = sb.cross_attention(q, none, none, 2, lse=lse)
+    assert not out.any() and (lse == -math.inf).all()
+    dq, dk, dv = sb.cross_attention_backward(q, q, none, none, out, lse, 2)
+    assert not dq.any() and dk.shape == dv.shape == (2, 0, 64)
+    k = torch.ones(2, 5, 64, **z)
+    empty = torch.zeros(2, 0, 64, **z)
+    dq, dk, dv = sb.cross_attention_backward(empty, empty, k, k, empty, torch.zeros(2, 2, 0, device="cuda"), 2)
+    assert dq.shape == (2, 0, 64) and not dk.any() and not dv.any()
+
+
+def check_backward(grads, dout, q, k, v, heads, kv_heads, lens, valid, out16, scale=None):
+    ref, lse, p, qd, kd, vd = formula(q, k, v, heads, kv_heads, lens, valid, scale)
+    scale = scale or qd.shape[-1] ** -0.5
+    g, o = heads_of(dout, heads, kv_heads), heads_of(out16, heads, kv_heads)
+    u, e = unit(q.dtype), slack_of(qd, kd, scale)
+    dp, d = g @ vd.transpose(-1, -2), (g * ref).sum(-1, keepdim=True)
+    ds = p * (dp - d)
+    # dS is off by its rounding, by D from the rounded out, by P and by the fp32 products
+    absd = (g.abs() * ref.abs()).sum(-1, keepdim=True)
+    sub = 2.0 ** -25 if q.dtype == torch.float16 else 0.0  # fp16 values below 2^-14
+    ds_tol = u * ds.abs() + p * ((g * (o - ref)).abs().sum(-1, keepdim=True) + e * (g.abs() @ vd.abs().transpose(-1, -2) + absd)) + sub
+    p_tol = (u + e) * p + sub
+    want = {"dq": (ds @ kd * scale, ds_tol @ kd.abs() * scale),
+            "dk": ((ds.transpose(-1, -2) @ qd * scale).sum(2, keepdim=True),
+                   (ds_tol.transpose(-1, -2) @ qd.abs() * scale).sum(2, keepdim=True)),
+            "dv": ((p.transpose(-1, -2) @ g).sum(2, keepdim=True), (p_tol.transpose(-1, -2) @ g.abs()).sum(2, keepdim=True))}
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        r, t = (rows_of(x) for x in want[name])
+        t = t + u * r.abs() + sub
+        err = (got.double() - r).abs()
+        assert got.isfinite().all(), name
+        assert (err <= 1.02 * t + 1e-30).all(), (name, (err / (t + 1e-30)).max().item())
+    return {n: rows_of(w[0]) for n, w in want.items()}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,tq,tk,heads,kv_heads,dim,kind", [
+    (2, 300, 240, 8, 8, 32, None), (1, 1, 1, 1, 1, 64, None), (2, 5, 77, 4, 2, 128, None), (1, 64, 128, 2, 1, 64, None),
+    (3, 65, 129, 6, 2, 64, "lens"), (4, 130, 200, 4, 4, 32, "none_left"), (4, 257, 130, 4, 1, 128, "both"),
+    (4, 1, 700, 4, 2, 128, "valid"), (2, 40, 385, 3, 1, 64, "holes"), (4, 33, 260, 2, 2, 128, "ends"),
+    (1, 700, 3, 2, 1, 128, None),
+])
+def test_cross_attention_backward(b, tq, tk, heads, kv_heads, dim, kind, dtype):
+    import sarbon_b200 as sb
+    g = gen(tq * 3 + tk)
+    q, dout = rand(g, b, tq, heads * dim, dtype=dtype), rand(g, b, tq, heads * dim, dtype=dtype)
+    kv = rand(g, b, tk, 2 * kv_heads * dim, dtype=dtype)
+    lens, valid = masks_of(kind, b, tk, g) if kind else (None, None)
+    kv[~keep_of(b, tk, lens, valid)] = math.nan
+    k, v = kv[..., :kv_heads * dim], kv[..., kv_heads * dim:]
+    ref, lse, *_ = formula(q, k, v, heads, kv_heads, lens, valid)
+    out, lse = rows_of(ref).to(dtype), lse.flatten(1, 2).float().contiguous()
+    call = lambda: sb.cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=kv_heads, lens=lens, valid=valid)  # noqa: E731
+    grads = call()
+    check_backward(grads, dout, q, k, v, heads, kv_heads, lens, valid, out)
+    assert all(torch.equal(x, y) for x, y in zip(grads, call()))  # the same bits again
+    away = ~keep_of(b, tk, lens, valid)
+    assert not grads[1][away].any() and not grads[2][away].any()
+
+
+def test_cross_attention_backward_strides():
+    """Gradients written into slices of one projection's gradient; a memory shared by the items."""
+    import sarbon_b200 as sb
+    g = gen(9)
+    b, tq, tk, heads, dim = 3, 50, 140, 2, 64
+    q, dout = (rand(g, tq, b, heads * dim, dtype=torch.float16).transpose(0, 1) for _ in range(2))
+    kv = rand(g, 1, tk, 2 * heads * dim, dtype=torch.float16).expand(b, -1, -1)
+    k, v = kv[..., :heads * dim], kv[..., heads * dim:]
+    lse = torch.empty(b, heads, tq, device="cuda")
+    out = sb.cross_attention(q, k, v, heads, lse=lse)
+    both = torch.full((b, tk, 2 * heads * dim + 16), 3.0, device="cuda", dtype=torch.float16)
+    dk, dv = both[..., 8:8 + heads * dim], both[..., 8 + heads * dim:-8]
+    grads = sb.cross_attention_backward(dout, q, k, v, out, lse, heads, dk=dk, dv=dv)
+    assert grads[1] is dk and grads[2] is dv
+    check_backward(grads, dout, q, k, v, heads, heads, None, None, out)
+    assert (both[..., :8] == 3).all() and (both[..., -8:] == 3).all()
+
+
+def test_cross_attention_gradient_against_differences():
+    """<gradient, direction> against the central difference of the 64-bit formula, whose own error at
+    step 1e-4 is of order 1e-8; the gradients carry roundings of u to each of their many terms."""
+    import sarbon_b200 as sb
+    g = gen(10)
+    b, tq, tk, heads, kv_heads, dim = 2, 40, 70, 4, 2, 64
+    x = [rand(g, b, n, h * dim, dtype=torch.float16) for n, h in ((tq, heads), (tk, kv_heads), (tk, kv_heads))]
+    dout = rand(g, b, tq, heads * dim, dtype=torch.float16)
+    lens = torch.tensor([70, 33], dtype=torch.int32, device="cuda")
+    lse = torch.empty(b, heads, tq, device="cuda")
+    out = sb.cross_attention(*x, heads, kv_heads=kv_heads, lens=lens, lse=lse)
+    grads = sb.cross_attention_backward(dout, *x, out, lse, heads, kv_heads=kv_heads, lens=lens)
+
+    def loss(y):
+        return (rows_of(formula(*y, heads, kv_heads, lens, None)[0]) * dout.double()).sum().item()
+
+    for i in range(3):
+        d = rand(g, *x[i].shape).double()
+        up, down = ([y.double() + s * 1e-4 * d if j == i else y for j, y in enumerate(x)] for s in (1, -1))
+        want = (loss(up) - loss(down)) / 2e-4
+        got = (grads[i].double() * d).sum().item()
+        # n roundings of relative size <= 4 u (P, dS, out, the result), of random sign
+        tol = 4 * 4 * unit(torch.float16) * (grads[i].double() * d).square().sum().sqrt().item() + 1e-5 * abs(want)
+        assert abs(got - want) <= tol, (i, got, want, tol)
+
+
+# ---------------------------------------------------------------- rotary positions
+def rope_formula(x, pos, heads, freq, axis, layout, inverse):
+    b, t, width = x.shape
+    y = x.double().view(b, t, heads, -1).clone()
+    n = freq.numel()
+    pos = pos.double().expand(b, t, -1)
+    ok = (axis >= 0) & (axis < pos.shape[-1])
+    angle = pos[..., axis.long().clamp(0, pos.shape[-1] - 1)] * freq * ok
+    cos, sin = angle.cos()[:, :, None], angle.sin()[:, :, None] * (-1 if inverse else 1)
+    at = (slice(0, n), slice(n, 2 * n)) if layout == "half" else (slice(0, 2 * n, 2), slice(1, 2 * n, 2))
+    u, v = y[..., at[0]].clone(), y[..., at[1]].clone()
+    y[..., at[0]], y[..., at[1]] = u * cos - v * sin, u * sin + v * cos
+    size = torch.zeros_like(y)  # |u| + |v| of each channel's pair
+    size[..., at[0]] = size[..., at[1]] = u.abs() + v.abs()
+    return y.flatten(2), size.flatten(2)
+
+
+def check_rope(out, x, *args):
+    ref, size = rope_formula(x, *args)
+    # sines and cosines off by about 2^-22, fp32 products and sums, one rounding to the type
+    tol = unit(x.dtype) * ref.abs() + 2.0 ** -21 * size + (2.0 ** -25 if x.dtype == torch.float16 else 0)
+    assert ((out.double() - ref).abs() <= 1.01 * tol).all(), ((out.double() - ref).abs() - tol).max().item()
+
+
+@pytest.mark.parametrize("dtype", TYPES + [torch.float32])
+@pytest.mark.parametrize("layout", ["half", "pairs"])
+@pytest.mark.parametrize("b,t,heads,dim,sections,pos32", [
+    (2, 300, 8, 32, (8, 8), True), (1, 1, 1, 64, (32,), False), (3, 77, 4, 128, (16, 24, 24), False),
+    (2, 33, 3, 80, (4, 6, 6), False), (1, 50, 2, 20, (3, 4), True), (2, 9, 40, 64, (8, 12, 12), False),
+])
+def test_rope(b, t, heads, dim, sections, pos32, layout, dtype):
+    import sarbon_b200 as sb
+    g = gen(t + dim)
+    freq, axis = sb.rope_table(sections)
+    pos = torch.randint(-50, 5_000_000, (b, t, len(sections)), device="cuda", generator=g)
+    pos = pos.float() + 0.25 if pos32 else pos.to(torch.int32)
+    x = rand(g, b, t, heads * dim, dtype=dtype)
+    for inverse in (False, True):
+        out = sb.rope_axes(x, pos, heads, freq, axis, layout=layout, inverse=inverse)
+        check_rope(out, x, pos, heads, freq, axis, layout, inverse)
+    same = x.clone()
+    assert sb.rope_axes(same, pos, heads, freq, axis, layout=layout, inverse=True, out=same) is same
+    assert torch.equal(same, out)
+
+
+def test_rope_views():
+    """Positions shared by the items, odd offsets (no vector loads), an axis that pos lacks, a slice as
+    output whose surroundings stay, no pairs at all."""
+    import sarbon_b200 as sb
+    g = gen(3)
+    freq, axis = sb.rope_table((6, 5, 5))
+    axis = axis.clone()
+    axis[3], axis[4] = 7, -1
+    pos = sb.grid_positions(3, 5, 7)
+    wide = rand(g, 2, 105, 3 * 64 + 1, dtype=torch.bfloat16)
+    x = wide[..., 1:129]
+    hold = torch.full_like(wide, 9.0)
+    out = sb.rope_axes(x, pos, 2, freq, axis, out=hold[..., 3:131])
+    check_rope(out, x, pos[None], 2, freq, axis, "half", False)
+    assert (hold[..., :3] == 9).all() and (hold[..., 131:] == 9).all()
+    first = rand(g, 105, 2, 128).transpose(0, 1)
+    check_rope(sb.rope_axes(first, pos, 2, freq, axis), first, pos[None], 2, freq, axis, "half", False)
+    assert torch.equal(sb.rope_axes(x, pos, 2, freq[:0], axis[:0]), x)
+    assert sb.rope_axes(x[:0], pos, 2, freq, axis).shape == (0, 105, 128)
+
+
+# ---------------------------------------------------------------- gated residual and norms
+def norm_formula(x, z, gate, scale, post, pre, kind, eps):
+    def norm(v, w):
+        m = v.mean(-1, keepdim=True) if kind == "layer" else 0
+        r = ((v - m).square().mean(-1, keepdim=True) + eps).rsqrt()
+        return (v - m) * r * w[0] + (0 if w[1] is None else w[1])
+
+    n = norm(z, post) if post else z
+    f = 1.0 if gate is None else gate[:, None] if gate.dim() == 2 else gate
+    y = x + f * n * (1.0 if scale is None else scale)
+    return y, norm(y, pre) if pre else None
+
+
+def norm_case(g, b, t, d, xt, zt, kind, gate, scale, post, pre):
+    def w(on):
+        return None if not on else (1 + rand(g, d, by=0.3), rand(g, d, by=0.3) if kind == "layer" else None)
+
+    shape = {None: None, "vector": (d,), "image": (b, d), "row": (b, t, d)}[gate]
+    return dict(x=rand(g, b, t, d, dtype=xt, by=2.0), z=rand(g, b, t, d, dtype=zt),
+                gate=None if shape is None else rand(g, *shape, dtype=zt), scale=rand(g, d) if scale else None,
+                post=w(post), pre=w(pre), kind=kind, eps=1e-5)
+
+
+def wide(s, grad=False):
+    """The case's tensors in fp64."""
+    f = lambda t: None if t is None else t.double().requires_grad_(grad)  # noqa: E731
+    return {k: tuple(f(t) for t in v) if isinstance(v, tuple) else f(v) if torch.is_tensor(v) or v is None else v
+            for k, v in s.items()}
+
+
+NORMS = [
+    (2, 300, 256, torch.float32, torch.float16, "layer", None, True, True, True),
+    (1, 1, 8, torch.bfloat16, torch.bfloat16, "rms", "vector", False, True, True),
+    (3, 17, 100, torch.float16, torch.float16, "layer", "image", True, False, True),
+    (2, 40, 255, torch.float32, torch.bfloat16, "rms", "row", True, True, True),
+    (2, 9, 1152, torch.bfloat16, torch.bfloat16, "layer", "image", True, True, True),
+    (5, 3, 2048, torch.float32, torch.float32, "rms", "image", False, True, False),
+    (1, 70, 64, torch.bfloat16, torch.float16, "layer", "row", False, True, True),
+    (2, 5, 4104, torch.float32, torch.bfloat16, "layer", "vector", True, True, True),
+    (1, 3, 8192, torch.bfloat16, torch.bfloat16, "rms", None, False, False, True),
+    (4, 33, 768, torch.float32, torch.float16, "rms", None, True, False, False),
+    (1, 1, 1, torch.float32, torch.float32, "rms", "row", True, True, True),
+]
+
+
+@pytest.mark.parametrize("case", NORMS, ids=lambda c: "x".join(map(str, c[:3])) + "-" + c[5])
+def test_gated_norm(case):
+    import sarbon_b200 as sb
+    s = norm_case(gen(case[2]), *case)
+    y, h = sb.gated_norm(**s)
+    ry, rh = norm_formula(**wide(s))
+    # fp32: products and sums of the terms of y; the norm's statistics are sums of D terms by trees
+    d = wide(s)
+    size = d["x"].abs() + (ry - d["x"]).abs() * 2 + 1
+    assert ((y.double() - ry).abs() <= unit(y.dtype) * ry.abs() + FP32 * size + 2.0 ** -25).all()
+    assert (h is None) == (s["pre"] is None)
+    if h is not None:
+        spread = (ry.abs().mean(-1, keepdim=True) + size) * (ry.square().mean(-1, keepdim=True) if case[5] == "rms" else
+                                                             ry.var(-1, keepdim=True, unbiased=False)).add(s["eps"]).rsqrt()
+        tol = unit(h.dtype) * rh.abs() + 2 * FP32 * (spread * d["pre"][0].abs() + 1) + 2.0 ** -25
+        assert ((h.double() - rh).abs() <= tol).all(), ((h.double() - rh).abs() / tol).max().item()
+    again = dict(s, x=s["x"].clone(), z=s["z"].clone())
+    y2, h2 = sb.gated_norm(**again, y=again["x"], h=again["z"] if s["pre"] else None)  # in place
+    assert torch.equal(y2, y) and (h is None or torch.equal(h2, h))
+
+
+@pytest.mark.parametrize("missing", [None, "dy", "dh"])
+@pytest.mark.parametrize("case", NORMS, ids=lambda c: "x".join(map(str, c[:3])) + "-" + c[5])
+def test_gated_norm_backward(case, missing):
+    import sarbon_b200 as sb
+    g = gen(case[2] + 1)
+    s = norm_case(g, *case)
+    b, t, d = case[:3]
+    dy = None if missing == "dy" else rand(g, b, t, d, dtype=case[3])
+    dh = None if missing == "dh" or s["pre"] is None else rand(g, b, t, d, dtype=case[4])
+    got = sb.gated_norm_backward(dy, dh, **s)
+    w = wide(s, grad=True)
+    y, h = norm_formula(**w)
+    total = (y * (0 if dy is None else dy.double())).sum() + (0 if dh is None else (h * dh.double()).sum())
+    total.backward()
+    want = dict(dx=w["x"], dz=w["z"], gate=w["gate"], scale=w["scale"])
+    for name in ("post", "pre"):
+        want[name + "_w"], want[name + "_b"] = w[name] if w[name] else (None, None)
+    for name, leaf in want.items():
+        if leaf is None:
+            assert got[name] is None
+            continue
+        r = torch.zeros_like(leaf) if leaf.grad is None else leaf.grad
+        x = got[name].double()
+        # one rounding to the type; fp32 chains of about ten operations on terms that may cancel
+        # (measured by the gradient's own size), sums over rows by trees of chunks
+        size = r.abs() + r.square().mean().sqrt() + (1 if name in ("dx", "dz") else math.sqrt(b * t))
+        tol = unit(got[name].dtype) * r.abs() + 16 * FP32 * size + 2.0 ** -25
+        assert ((x - r).abs() <= tol).all(), (name, ((x - r).abs() / tol).max().item())
+    again = sb.gated_norm_backward(dy, dh, **s)
+    assert all(v is None or torch.equal(v, again[k]) for k, v in got.items())
+
+
+def test_gated_norm_views_and_offset_rows():
+    """Slices, an image's gate as an expanded row, rows whose mean is far from zero."""
+    import sarbon_b200 as sb
+    g = gen(21)
+    b, t, d = 2, 30, 96
+    s = norm_case(g, b, t, d, torch.float32, torch.bfloat16, "layer", None, True, True, True)
+    s["x"] = (rand(g, b, t, 3 * d + 1) + 1000.0)[..., 1:d + 1]
+    s["z"] = rand(g, t, b, d, dtype=torch.bfloat16).transpose(0, 1)
+    s["gate"] = rand(g, b, 1, d, dtype=torch.bfloat16).expand(b, t, d)
+    y, h = sb.gated_norm(**s)
+    ry, rh = norm_formula(**wide(s))
+    assert ((y.double() - ry).abs() <= 2.0 ** -23 * 1010).all()
+    # fp32 rows around 1000 with deviations around 1: each value is known to 2^-24 * 1000
+    assert ((h.double() - rh).abs() <= unit(torch.bfloat16) * rh.abs() + 8 * 2.0 ** -24 * 1000 * (1 + rh.abs())).all()
+    got = sb.gated_norm_backward(y, h, **s)
+    assert got["gate"].shape == (b, t, d) and got["gate"].dtype == torch.bfloat16
+    none = {k: (v[:, :0] if k in ("x", "z", "gate") else v) for k, v in s.items()}
+    y, h = sb.gated_norm(**none)
+    assert y.shape == h.shape == (b, 0, d)
+    got = sb.gated_norm_backward(y, h, **none)
+    assert got["dx"].shape == (b, 0, d) and not got["post_w"].any() and not got["scale"].any()
+
+
+# ---------------------------------------------------------------- together
+def block(sb, g, heads, kv_heads, dim):
+    """One block that reads a memory: positions, attention, gated residual and norms."""
+    d = heads * dim
+    freq, axis = sb.rope_table((dim // 8, dim // 8, dim // 4))
+    return dict(d=d, freq=freq, axis=axis, w0=1 + rand(g, d, by=0.1), w1=1 + rand(g, d, by=0.1), heads=heads, kv=kv_heads)
+
+
+def run_block(sb, p, x, q, k, v, qpos, kpos, gate, lens, lse):
+    qr = sb.rope_axes(q, qpos, p["heads"], p["freq"], p["axis"])
+    kr = sb.rope_axes(k, kpos, p["kv"], p["freq"], p["axis"])
+    o = sb.cross_attention(qr, kr, v, p["heads"], kv_heads=p["kv"], lens=lens, lse=lse)
+    y, h = sb.gated_norm(x, o, gate=gate, post=p["w0"], pre=p["w1"])
+    return qr, kr, o, y, h
+
+
+def back_block(sb, p, x, q, k, v, qpos, kpos, gate, lens, lse, qr, kr, o, dy, dh):
+    g = sb.gated_norm_backward(dy, dh, x, o, gate=gate, post=p["w0"], pre=p["w1"])
+    dqr, dkr, dv = sb.cross_attention_backward(g["dz"], qr, kr, v, o, lse, p["heads"], kv_heads=p["kv"], lens=lens)
+    dq = sb.rope_axes(dqr, qpos, p["heads"], p["freq"], p["axis"], inverse=True)
+    dk = sb.rope_axes(dkr, kpos, p["kv"], p["freq"], p["axis"], inverse=True)
+    return g["dx"], dq, dk, dv, g["gate"], g["post_w"], g["pre_w"]
+
+
+def block_inputs(g, p, b, tq, clip, dim):
+    t = clip[0] * clip[1] * clip[2]
+    z = dict(dtype=torch.bfloat16)
+    return dict(x=rand(g, b, tq, p["d"]), q=rand(g, b, tq, p["d"], **z), k=rand(g, b, t, p["kv"] * dim, **z),
+                v=rand(g, b, t, p["kv"] * dim, **z), gate=rand(g, b, p["d"], **z),
+                qpos=torch.randint(0, 9, (b, tq, 3), device="cuda", generator=g, dtype=torch.int32),
+                lens=torch.tensor([t, t // 2 + 1, 1][:b], dtype=torch.int32, device="cuda"),
+                lse=torch.empty(b, p["heads"], tq, device="cuda"))
+
+
+def test_block_forward_backward():
+    """The operators one after the other against fp64 with autograd; each bf16 tensor on the way adds
+    a rounding of u, and the chain multiplies them by a modest factor."""
+    import sarbon_b200 as sb
+    g = gen(30)
+    b, tq, heads, kv_heads, dim, clip = 3, 60, 4, 2, 64, (2, 6, 10)
+    p = block(sb, g, heads, kv_heads, dim)
+    s = block_inputs(g, p, b, tq, clip, dim)
+    kpos = sb.grid_positions(*clip)
+    qr, kr, o, y, h = run_block(sb, p, kpos=kpos, **s)
+    dy, dh = rand(g, *y.shape), rand(g, *h.shape, dtype=h.dtype)
+    got = back_block(sb, p, kpos=kpos, **s, qr=qr, kr=kr, o=o, dy=dy, dh=dh)
+
+    leaf = {n: s[n].double().requires_grad_(True) for n in ("x", "q", "k", "v", "gate")}
+    w0, w1 = (p[n].double().requires_grad_(True) for n in ("w0", "w1"))
+
+    def rot(x, pos, n):
+        xx = x.view(b, -1, n, dim)
+        a = pos.double().expand(b, -1, -1)[..., p["axis"].long()] * p["freq"]
+        c, sn = a.cos()[:, :, None], a.sin()[:, :, None]
+        u, v = xx[..., :dim // 2], xx[..., dim // 2:]
+        return torch.cat([u * c - v * sn, u * sn + v * c], -1).flatten(2)
+
+    ro = rows_of(formula(rot(leaf["q"], s["qpos"], heads), rot(leaf["k"], kpos, kv_heads), leaf["v"], heads, kv_heads,
+                         s["lens"], None)[0])
+    ry, rh = norm_formula(leaf["x"], ro, leaf["gate"], None, (w0, None), (w1, None), "rms", 1e-6)
+    ((ry * dy.double()).sum() + (rh * dh.double()).sum()).backward()
+    pairs = [(y, ry), (h, rh)] + list(zip(got, [t.grad for t in (*(leaf[n] for n in ("x", "q", "k", "v", "gate")), w0, w1)]))
+    u = unit(torch.bfloat16)
+    for i, (a, r) in enumerate(pairs):
+        rel = ((a.double() - r).norm() / r.norm()).item()
+        assert rel <= 6 * u, (i, rel, 6 * u)
+
+
+def test_block_in_graphs_and_on_streams():
+    """Two captured graphs and eager calls on a second stream, all in flight together, give the eager
+    results: no workspace is shared."""
+    import sarbon_b200 as sb
+    b, tq, heads, kv_heads, dim, clip = 2, 3, 4, 1, 128, (4, 16, 30)
+    kpos = sb.grid_positions(*clip)
+    p = block(sb, gen(40), heads, kv_heads, dim)
+    sets = [block_inputs(gen(41 + i), p, b, tq, clip, dim) for i in range(3)]
+
+    def both(s):
+        qr, kr, o, y, h = run_block(sb, p, kpos=kpos, **s)
+        return (o, y, h) + back_block(sb, p, kpos=kpos, **s, qr=qr, kr=kr, o=o, dy=y, dh=h)
+
+    want = [[t.clone() for t in both(s)] for s in sets]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in sets[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(both(s))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(3):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            third = both(sets[2])
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs + [third]):
+        assert all(torch.equal(x, y) for x, y in zip(w, o))
+    from sarbon_b200 import det_ops
+    assert det_ops.kernels_error() == 0
