@@ -35,6 +35,7 @@
 
 #include "sb_internal.cuh"
 #include "sb_ptx.cuh"
+#include "sb_xattn.cuh"
 
 namespace sb {
 namespace {
@@ -571,5 +572,8 @@ extern "C" int sb_kernels_error(int clear, int* flags) {
     if (cudaMemcpyToSymbol(g_kernel_error, &zero, sizeof(int)) != cudaSuccess)
       return record_error(SB_ECUDA, "sb_kernels_error: clear");
   }
+  int attn = 0;
+  if (xattn_error(clear, &attn) != 0) return record_error(SB_ECUDA, "sb_kernels_error: attention");
+  *flags |= attn;
   return SB_OK;
 }
