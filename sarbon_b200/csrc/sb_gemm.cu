@@ -572,8 +572,9 @@ extern "C" int sb_kernels_error(int clear, int* flags) {
     if (cudaMemcpyToSymbol(g_kernel_error, &zero, sizeof(int)) != cudaSuccess)
       return record_error(SB_ECUDA, "sb_kernels_error: clear");
   }
-  int attn = 0;
-  if (xattn_error(clear, &attn) != 0) return record_error(SB_ECUDA, "sb_kernels_error: attention");
-  *flags |= attn;
+  int fwd = 0, bwd = 0;
+  if (xattn_error(clear, &fwd) != 0 || xattn_back_error(clear, &bwd) != 0)
+    return record_error(SB_ECUDA, "sb_kernels_error: cross attention");
+  *flags |= fwd | bwd;
   return SB_OK;
 }

@@ -519,9 +519,13 @@ extern "C" int sb_cross_attention_work(int backward, int B, int H, int Hkv, int 
   if (!bytes || !xattn_sizes_ok(SB_F16, B, H, Hkv, dh, Tq, Tk))
     return record_error(SB_EINVAL, "sb_cross_attention_work: arguments");
   *bytes = 0;
-  if (backward || B == 0 || Tq == 0 || Tk == 0) return SB_OK;
+  if (B == 0 || Tq == 0 || Tk == 0) return SB_OK;
   const int sms = xattn_sms();
   if (sms == 0) return record_error(SB_ECUDA, "sb_cross_attention_work: device");
+  if (backward) {
+    *bytes = xattn_back_work(B, H, Hkv, dh, Tq, Tk, sms);
+    return SB_OK;
+  }
   const FwdPlan p = fwd_plan(B, H, Hkv, Tq, Tk, sms);
   if (p.splits > 1) *bytes = (long long)p.splits * B * H * Tq * (dh + 1) * 4;
   return SB_OK;

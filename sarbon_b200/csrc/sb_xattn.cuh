@@ -146,6 +146,8 @@ bool xattn_sizes_ok(int dtype, int B, int H, int Hkv, int dh, int Tq, int Tk);
 bool xattn_view_ok(const void* p, long long row, long long img);
 // Sticky SB_ERR_* flags of the attention kernels, cleared on request.
 int xattn_error(int clear, int* flags);  // 0, or -1 when the device could not be read
+int xattn_back_error(int clear, int* flags);
+long long xattn_back_work(int B, int H, int Hkv, int dh, int Tq, int Tk, int sms);
 // SMs of the current device, 0 on error
 int xattn_sms();
 
