@@ -19,9 +19,10 @@
 // Each CTA keeps its columns' sums in registers over its rows and writes them once; a second
 // kernel adds the CTAs' sums in a fixed order (no atomics: the same inputs give the same bits).
 //
-// A row belongs to `tpr` threads (a multiple of a warp, eight columns each), a CTA of at least
-// 256 threads handles several short rows at once, and the next rows' loads are issued before the
-// current rows' reductions.
+// A row belongs to one warp, or to all of a CTA's threads, NV vectors of eight columns each; a
+// CTA walks its rows with the next row's loads issued before the current row's reductions.  Element
+// types are compile-time for the usual pairs (DT of the template), so a row costs few registers
+// and no selects.
 #include <algorithm>
 
 #include "sb_rows.cuh"
@@ -43,8 +44,10 @@ struct NormArgs {
   const float *scale, *post_w, *post_b, *pre_w, *pre_b;
   int layer;
   float eps;
-  int T, D, tpr, per;  // threads a row, rows a CTA takes at once
+  int T, D, tpr, per;  // threads a row, rows a CTA takes at once (several: a warp each)
   long long rows;      // B * T
+  long long step_b;    // a CTA's step from row to row as (items, rows): no division in the loop
+  int step_t;
   void *y, *h;         // forward
   long long y_row, y_img, h_row, h_img;
   void *dx, *dz, *dgate_rows;  // backward
@@ -53,10 +56,10 @@ struct NormArgs {
   int chunks, gate_is_row;     // CTAs a group
 };
 
-// Sums of two values over the threads of a row; `slot` alternates between two halves of the
-// buffer, so one barrier a reduction is enough.
+// Sum of a pair of values over the threads of a row; the two halves of the buffer alternate, so one
+// barrier a reduction is enough.
 struct RowSum {
-  float2* buf;  // [2][per * warps a row]
+  float2* buf;  // [2][32]
   int warps, half;
   SB_DEV float2 operator()(float a, float b) {
 #pragma unroll
@@ -67,18 +70,36 @@ struct RowSum {
     if (warps == 1) return make_float2(a, b);
     float2* mine = buf + half * 32;
     half ^= 1;
-    const int w = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) mine[w] = make_float2(a, b);
+    if ((threadIdx.x & 31) == 0) mine[threadIdx.x >> 5] = make_float2(a, b);
     __syncthreads();
-    const int w0 = w / warps * warps;
     float2 s = make_float2(0.f, 0.f);
     for (int i = 0; i < warps; ++i) {
-      const float2 t = mine[w0 + i];
+      const float2 t = mine[i];
       s.x += t.x;
       s.y += t.y;
     }
     return s;
   }
+  SB_DEV float operator()(float a) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+    if (warps == 1) return a;
+    float2* mine = buf + half * 32;
+    half ^= 1;
+    if ((threadIdx.x & 31) == 0) mine[threadIdx.x >> 5].x = a;
+    __syncthreads();
+    float s = 0.f;
+    for (int i = 0; i < warps; ++i) s += mine[i].x;
+    return s;
+  }
+};
+
+// A thread's columns: vector j begins at c0 + j * pitch; n(j) of its eight columns exist.
+template <int NV>
+struct Cols {
+  int c0, pitch, D;
+  SB_DEV int at(int j) const { return c0 + j * pitch; }
+  SB_DEV int n(int j) const { return max(0, min(8, D - at(j))); }
 };
 
 template <bool VEC>
@@ -104,195 +125,281 @@ SB_DEV void columns(const float* w, int c, int n, float other, float (&v)[8]) {
   unpack8(fetch<VEC>(w, SB_F32, c, n), SB_F32, v);
 }
 
-// mean and 1 / deviation of a row; columns from n on do not count
-SB_DEV void stats_of(const float (&v)[8], int n, int layer, float inv_d, float eps, RowSum& sum, float& mean, float& r) {
-  float s = 0.f, q = 0.f;
+// mean and 1 / deviation of a row whose columns past D hold zeros
+template <int NV>
+SB_DEV void stats_of(const float (&v)[NV][8], const Cols<NV>& cols, int layer, float inv_d, float eps, RowSum& sum,
+                     float& mean, float& r) {
+  mean = 0.f;
   if (layer) {
+    float s = 0.f;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) s += v[u];  // zero from n on
-    mean = sum(s, 0.f).x * inv_d;
-  } else {
-    mean = 0.f;
-  }
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const float d = v[u] - mean;
-    q += u < n ? d * d : 0.f;
+      for (int u = 0; u < 8; ++u) s += v[j][u];
+    mean = sum(s) * inv_d;
   }
-  r = rsqrtf(sum(q, 0.f).x * inv_d + eps);
+  float q = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int n = cols.n(j);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float d = v[j][u] - mean;
+      q += u < n ? d * d : 0.f;
+    }
+  }
+  r = rsqrtf(sum(q) * inv_d + eps);
 }
 
-template <bool VEC, int MAXT>
+// XD, ZD: dtype codes of x and z, -1: as the arguments say
+template <int XD, int ZD, bool VEC, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float2 buf[64];
+  const int xdt = XD < 0 ? a.xdt : XD, zdt = ZD < 0 ? a.zdt : ZD;
   RowSum sum{buf, a.tpr >> 5, 0};
-  const int sub = threadIdx.x / a.tpr;
-  const int c = (threadIdx.x - sub * a.tpr) * 8;
-  const int n = max(0, min(8, a.D - c));
+  const int sub = a.per > 1 ? threadIdx.x >> 5 : 0;
+  const Cols<NV> cols{(int)(a.per > 1 ? threadIdx.x & 31 : threadIdx.x) * 8, a.tpr * 8, a.D};
   const float inv_d = 1.f / (float)a.D;
   const long long step = (long long)gridDim.x * a.per;
-  Raw8 rx, rz, rg;
-  auto load = [&](long long r) {
-    const bool ok = r < a.rows;
-    const long long b = ok ? r / a.T : 0, t = ok ? r - b * a.T : 0;
-    const int m = ok ? n : 0;
-    rx = fetch<VEC>(a.x.p, a.xdt, b * a.x.img + t * a.x.row + c, m);
-    rz = fetch<VEC>(a.z.p, a.zdt, b * a.z.img + t * a.z.row + c, m);
-    if (a.gate.p) rg = fetch<VEC>(a.gate.p, a.zdt, b * a.gate.img + t * a.gate.row + c, m);
+  long long r = (long long)blockIdx.x * a.per + sub;
+  long long b = r / a.T;
+  int t = (int)(r - b * a.T);
+  Raw8 rx[NV], rz[NV], rg[NV];
+  auto load = [&](bool ok, long long bb, int tt) {
+    const long long xo = bb * a.x.img + tt * a.x.row, zo = bb * a.z.img + tt * a.z.row;
+    const long long go = bb * a.gate.img + tt * a.gate.row;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = cols.at(j), m = ok ? cols.n(j) : 0;
+      rx[j] = fetch<VEC>(a.x.p, xdt, xo + c, m);
+      rz[j] = fetch<VEC>(a.z.p, zdt, zo + c, m);
+      if (a.gate.p) rg[j] = fetch<VEC>(a.gate.p, zdt, go + c, m);
+    }
   };
-  float scale[8], post_w[8], pre_w[8];
-  columns<VEC>(a.scale, c, n, 1.f, scale);
-  columns<VEC>(a.post_w, c, n, 1.f, post_w);
-  columns<VEC>(a.pre_w, c, n, 1.f, pre_w);
-  long long r0 = (long long)blockIdx.x * a.per;
-  load(r0 + sub);
-  for (; r0 < a.rows; r0 += step) {
-    const long long r = r0 + sub;
-    const bool ok = r < a.rows;
-    float v[8], y[8], g[8];
-    unpack8(rz, a.zdt, v);
-    unpack8(rx, a.xdt, y);
-    if (a.gate.p) {
-      unpack8(rg, a.zdt, g);
-    } else {
+  load(r < a.rows, b, t);
+  // every warp of a row's CTA walks the same rows; with a warp a row there is no barrier
+  for (; r < a.rows; r += step) {
+    float v[NV][8], y[NV][8], g[NV][8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) g[u] = 1.f;
+    for (int j = 0; j < NV; ++j) {
+      unpack8(rz[j], zdt, v[j]);
+      unpack8(rx[j], xdt, y[j]);
+      if (a.gate.p) {
+        unpack8(rg[j], zdt, g[j]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) g[j][u] = 1.f;
+      }
     }
-    load(r + step);
-    if (a.post_w) {
-      float mean, rs, post_b[8];
-      stats_of(v, n, a.layer, inv_d, a.eps, sum, mean, rs);
-      columns<VEC>(a.post_b, c, n, 0.f, post_b);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = (v[u] - mean) * rs * post_w[u] + post_b[u];
+    long long nb = b + a.step_b;
+    int nt = t + a.step_t;
+    if (nt >= a.T) {
+      nt -= a.T;
+      ++nb;
     }
+    load(r + step < a.rows, nb, nt);
+    float mean = 0.f, rs = 1.f;
+    if (a.post_w) stats_of(v, cols, a.layer, inv_d, a.eps, sum, mean, rs);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) y[u] = u < n ? fmaf(scale[u] * g[u], v[u], y[u]) : 0.f;
-    const long long b = r / a.T, t = r - b * a.T;
-    if (ok) put<VEC>(a.y, a.xdt, b * a.y_img + t * a.y_row + c, y, n);
+    for (int j = 0; j < NV; ++j) {
+      const int c = cols.at(j), n = cols.n(j);
+      float s[8], w[8], o[8];
+      columns<VEC>(a.scale, c, n, 1.f, s);
+      if (a.post_w) {
+        columns<VEC>(a.post_w, c, n, 1.f, w);
+        columns<VEC>(a.post_b, c, n, 0.f, o);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[j][u] = fmaf((v[j][u] - mean) * rs, w[u], o[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) y[j][u] = u < n ? fmaf(s[u] * g[j][u], v[j][u], y[j][u]) : 0.f;
+      put<VEC>(a.y, xdt, b * a.y_img + t * a.y_row + c, y[j], n);
+    }
     if (a.h) {
-      float mean, rs, pre_b[8];
-      stats_of(y, n, a.layer, inv_d, a.eps, sum, mean, rs);
-      columns<VEC>(a.pre_b, c, n, 0.f, pre_b);
+      stats_of(y, cols, a.layer, inv_d, a.eps, sum, mean, rs);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) y[u] = (y[u] - mean) * rs * pre_w[u] + pre_b[u];
-      if (ok) put<VEC>(a.h, a.zdt, b * a.h_img + t * a.h_row + c, y, n);
+      for (int j = 0; j < NV; ++j) {
+        const int c = cols.at(j), n = cols.n(j);
+        float w[8], o[8];
+        columns<VEC>(a.pre_w, c, n, 1.f, w);
+        columns<VEC>(a.pre_b, c, n, 0.f, o);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) y[j][u] = fmaf((y[j][u] - mean) * rs, w[u], o[u]);
+        put<VEC>(a.h, zdt, b * a.h_img + t * a.h_row + c, y[j], n);
+      }
     }
+    b = nb;
+    t = nt;
   }
 }
 
-template <bool VEC, int MAXT>
-__global__ void __launch_bounds__(MAXT) gated_norm_back_kernel(const __grid_constant__ NormArgs a) {
+template <int XD, int ZD, bool VEC, int NV, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float2 buf[64];
-  extern __shared__ float fold[];  // [per][kSums][tpr * 8] sums of the rows a CTA takes at once
+  extern __shared__ float fold[];  // [per][kSums][D padded]: several rows' warps meet here
+  const int xdt = XD < 0 ? a.xdt : XD, zdt = ZD < 0 ? a.zdt : ZD;
   RowSum sum{buf, a.tpr >> 5, 0};
-  const int sub = threadIdx.x / a.tpr;
-  const int c = (threadIdx.x - sub * a.tpr) * 8;
-  const int n = max(0, min(8, a.D - c));
+  const int sub = a.per > 1 ? threadIdx.x >> 5 : 0;
+  const Cols<NV> cols{(int)(a.per > 1 ? threadIdx.x & 31 : threadIdx.x) * 8, a.tpr * 8, a.D};
   const float inv_d = 1.f / (float)a.D;
   const long long group = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
   const long long each = (a.group_rows + a.chunks - 1) / a.chunks;
   const long long first = group * a.group_rows + min(chunk * each, a.group_rows);
   const long long last = group * a.group_rows + min((chunk + 1) * each, a.group_rows);
-  float acc[kSums][8];
+  float acc[kSums][NV][8];
 #pragma unroll
   for (int k = 0; k < kSums; ++k)
 #pragma unroll
-    for (int u = 0; u < 8; ++u) acc[k][u] = 0.f;
-  Raw8 rx, rz, rg, rdy, rdh;
-  auto load = [&](long long r) {
-    const bool ok = r < last;
-    const long long b = ok ? r / a.T : 0, t = ok ? r - b * a.T : 0;
-    const int m = ok ? n : 0;
-    rx = fetch<VEC>(a.x.p, a.xdt, b * a.x.img + t * a.x.row + c, a.dh.p ? m : 0);
-    rz = fetch<VEC>(a.z.p, a.zdt, b * a.z.img + t * a.z.row + c, m);
-    rg = fetch<VEC>(a.gate.p, a.zdt, b * a.gate.img + t * a.gate.row + c, a.gate.p ? m : 0);
-    rdy = fetch<VEC>(a.dy.p, a.xdt, b * a.dy.img + t * a.dy.row + c, a.dy.p ? m : 0);
-    rdh = fetch<VEC>(a.dh.p, a.zdt, b * a.dh.img + t * a.dh.row + c, a.dh.p ? m : 0);
-  };
-  load(first + sub);
-  for (long long r0 = first; r0 < last; r0 += a.per) {
-    const long long r = r0 + sub;
-    const bool ok = r < last;
-    float zh[8], g[8], d[8], y[8], dh[8];
-    unpack8(rz, a.zdt, zh);
-    unpack8(rx, a.xdt, y);
-    unpack8(rdy, a.xdt, d);
-    unpack8(rdh, a.zdt, dh);
-    if (a.gate.p) {
-      unpack8(rg, a.zdt, g);
-    } else {
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int u = 0; u < 8; ++u) g[u] = 1.f;
+      for (int u = 0; u < 8; ++u) acc[k][j][u] = 0.f;
+  long long r = first + sub, b = r / a.T;
+  int t = (int)(r - b * a.T);
+  Raw8 rx[NV], rz[NV], rg[NV], rdy[NV], rdh[NV];
+  auto load = [&](bool ok, long long bb, int tt) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = cols.at(j), m = ok ? cols.n(j) : 0;
+      rz[j] = fetch<VEC>(a.z.p, zdt, bb * a.z.img + tt * a.z.row + c, m);
+      rdy[j] = fetch<VEC>(a.dy.p, xdt, bb * a.dy.img + tt * a.dy.row + c, a.dy.p ? m : 0);
+      if (a.dh.p) {
+        rx[j] = fetch<VEC>(a.x.p, xdt, bb * a.x.img + tt * a.x.row + c, m);
+        rdh[j] = fetch<VEC>(a.dh.p, zdt, bb * a.dh.img + tt * a.dh.row + c, m);
+      }
+      if (a.gate.p) rg[j] = fetch<VEC>(a.gate.p, zdt, bb * a.gate.img + tt * a.gate.row + c, m);
     }
-    load(r + a.per);
-    float zr = 1.f, w[8], bb[8], s[8];
-    columns<VEC>(a.scale, c, n, 1.f, s);
+  };
+  load(r < last, b, t);
+  for (; r < last; r += a.per) {
+    float zh[NV][8], g[NV][8], d[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      unpack8(rz[j], zdt, zh[j]);
+      unpack8(rdy[j], xdt, d[j]);
+      if (a.gate.p) {
+        unpack8(rg[j], zdt, g[j]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) g[j][u] = 1.f;
+      }
+    }
+    float y[NV][8], dh[NV][8];
+    if (a.dh.p) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        unpack8(rx[j], xdt, y[j]);
+        unpack8(rdh[j], zdt, dh[j]);
+      }
+    }
+    t += a.per;
+    if (t >= a.T) {  // T < per: the division below
+      const int over = t / a.T;
+      t -= over * a.T;
+      b += over;
+    }
+    load(r + a.per < last, b, t);
+    float zr = 1.f;
     if (a.post_w) {
       float mean;
-      stats_of(zh, n, a.layer, inv_d, a.eps, sum, mean, zr);
+      stats_of(zh, cols, a.layer, inv_d, a.eps, sum, mean, zr);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) zh[u] = u < n ? (zh[u] - mean) * zr : 0.f;
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) zh[j][u] = u < cols.n(j) ? (zh[j][u] - mean) * zr : 0.f;
     }
-    columns<VEC>(a.post_w, c, n, 1.f, w);
     if (a.dh.p) {
-      columns<VEC>(a.post_b, c, n, 0.f, bb);
-      float mean, rs;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) y[u] = u < n ? fmaf(s[u] * g[u], zh[u] * w[u] + bb[u], y[u]) : 0.f;
-      stats_of(y, n, a.layer, inv_d, a.eps, sum, mean, rs);
-      float pw[8], e0 = 0.f, e1 = 0.f;
-      columns<VEC>(a.pre_w, c, n, 1.f, pw);
+      for (int j = 0; j < NV; ++j) {
+        const int c = cols.at(j), n = cols.n(j);
+        float s[8], w[8], o[8];
+        columns<VEC>(a.scale, c, n, 1.f, s);
+        columns<VEC>(a.post_w, c, n, 1.f, w);
+        columns<VEC>(a.post_b, c, n, 0.f, o);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        y[u] = u < n ? (y[u] - mean) * rs : 0.f;
-        acc[2][u] += ok ? dh[u] * y[u] : 0.f;
-        acc[3][u] += dh[u];
-        dh[u] *= pw[u];
-        e0 += dh[u];
-        e1 += dh[u] * y[u];
+        for (int u = 0; u < 8; ++u)
+          y[j][u] = u < n ? fmaf(s[u] * g[j][u], fmaf(zh[j][u], w[u], o[u]), y[j][u]) : 0.f;
+      }
+      float mean, rs, e0 = 0.f, e1 = 0.f;
+      stats_of(y, cols, a.layer, inv_d, a.eps, sum, mean, rs);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float w[8];
+        columns<VEC>(a.pre_w, cols.at(j), cols.n(j), 1.f, w);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          y[j][u] = u < cols.n(j) ? (y[j][u] - mean) * rs : 0.f;
+          acc[2][j][u] = fmaf(dh[j][u], y[j][u], acc[2][j][u]);
+          acc[3][j][u] += dh[j][u];
+          dh[j][u] *= w[u];
+          e0 += dh[j][u];
+          e1 = fmaf(dh[j][u], y[j][u], e1);
+        }
       }
       const float2 m = sum(e0, e1);
       const float m0 = a.layer ? m.x * inv_d : 0.f, m1 = m.y * inv_d;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) d[u] += rs * (dh[u] - y[u] * m1 - m0);
-    }
-    if (ok) put<VEC>(a.dx, a.xdt, r * a.D + c, d, n);
-    if (a.dgate_rows) {
-      float dg[8];
-      columns<VEC>(a.post_b, c, n, 0.f, bb);
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int u = 0; u < 8; ++u) dg[u] = d[u] * s[u] * (zh[u] * w[u] + bb[u]);
-      if (ok) put<VEC>(a.dgate_rows, a.zdt, r * a.D + c, dg, n);
+        for (int u = 0; u < 8; ++u) d[j][u] += rs * (dh[j][u] - y[j][u] * m1 - m0);
     }
     float e0 = 0.f, e1 = 0.f;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      // rows past the CTA's last hold zeros in d and zh
-      const float f = a.gate_is_row ? d[u] * g[u] : d[u];
-      acc[0][u] += ok ? f * zh[u] : 0.f;
-      acc[1][u] += ok ? f : 0.f;
-      d[u] = u < n ? d[u] * s[u] * g[u] * w[u] : 0.f;
-      e0 += d[u];
-      e1 += d[u] * zh[u];
+    for (int j = 0; j < NV; ++j) {
+      const int c = cols.at(j), n = cols.n(j);
+      put<VEC>(a.dx, xdt, r * a.D + c, d[j], n);
+      float s[8], w[8];
+      columns<VEC>(a.scale, c, n, 1.f, s);
+      columns<VEC>(a.post_w, c, n, 1.f, w);
+      if (a.dgate_rows) {
+        float o[8], dg[8];
+        columns<VEC>(a.post_b, c, n, 0.f, o);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) dg[u] = d[j][u] * s[u] * fmaf(zh[j][u], w[u], o[u]);
+        put<VEC>(a.dgate_rows, zdt, r * a.D + c, dg, n);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float f = a.gate_is_row ? d[j][u] * g[j][u] : d[j][u];
+        acc[0][j][u] = fmaf(f, zh[j][u], acc[0][j][u]);
+        acc[1][j][u] += f;
+        d[j][u] = u < n ? d[j][u] * s[u] * g[j][u] * w[u] : 0.f;
+        e0 += d[j][u];
+        e1 = fmaf(d[j][u], zh[j][u], e1);
+      }
     }
+    float m0 = 0.f, m1 = 0.f;
     if (a.post_w) {
       const float2 m = sum(e0, e1);
-      const float m0 = a.layer ? m.x * inv_d : 0.f, m1 = m.y * inv_d;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) d[u] = zr * (d[u] - zh[u] * m1 - m0);
+      m0 = a.layer ? m.x * inv_d : 0.f;
+      m1 = m.y * inv_d;
     }
-    if (ok) put<VEC>(a.dz, a.zdt, r * a.D + c, d, n);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (a.post_w) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) d[j][u] = zr * (d[j][u] - zh[j][u] * m1 - m0);
+      }
+      put<VEC>(a.dz, zdt, r * a.D + cols.at(j), d[j], cols.n(j));
+    }
   }
   if (!a.part) return;
-  // the CTA's sums: over its row groups in order, one group of threads after the other
-  const int width = a.tpr * 8;
+  float* mine = a.part + (long long)blockIdx.x * kSums * a.D;
+  if (a.per == 1) {
+#pragma unroll
+    for (int k = 0; k < kSums; ++k)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) put<VEC>(mine, SB_F32, (long long)k * a.D + cols.at(j), acc[k][j], cols.n(j));
+    return;
+  }
+  // the CTA's warps one after the other
+  const int width = a.tpr * 8 * NV;
 #pragma unroll
   for (int k = 0; k < kSums; ++k)
 #pragma unroll
-    for (int u = 0; u < 8; ++u) fold[(sub * kSums + k) * width + c + u] = acc[k][u];
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) fold[(sub * kSums + k) * width + cols.at(j) + u] = acc[k][j][u];
   __syncthreads();
-  float* mine = a.part + (long long)blockIdx.x * kSums * a.D;
   for (int i = threadIdx.x; i < kSums * a.D; i += blockDim.x) {
     const int k = i / a.D, col = i - k * a.D;
     float s = 0.f;
@@ -367,20 +474,58 @@ int sm_count() {
   return n;
 }
 
+// Up to 256 channels a warp takes a row with one vector a lane, eight (backward: four) rows a CTA;
+// above, a CTA takes a row: two vectors a thread forward and, with its column sums in registers, one
+// backward up to 2048 channels and two above.
 struct Plan {
+  int kind;  // of the launch tables
   int tpr, per, threads;
 };
-Plan plan_of(int D) {
+Plan plan_of(int D, bool back) {
   Plan p;
-  p.tpr = ((D + 7) / 8 + 31) / 32 * 32;
-  p.per = std::max(1, 256 / p.tpr);
+  const int vecs = (D + 7) / 8;
+  if (vecs <= 32) {
+    p = {0, 32, back ? 4 : 8, 0};
+  } else if (!back) {
+    p.tpr = ((vecs + 1) / 2 + 31) / 32 * 32;
+    p.kind = p.tpr <= 128 ? 1 : 2;
+    p.per = 1;
+  } else {
+    p.kind = vecs <= 256 ? 1 : 2;
+    p.tpr = (p.kind == 1 ? vecs + 31 : (vecs + 1) / 2 + 31) / 32 * 32;
+    p.per = 1;
+  }
   p.threads = p.tpr * p.per;
   return p;
 }
 
-// CTAs a group of rows: about two a SM over all groups, at least eight rows each
+using NormKernel = void (*)(const NormArgs);
+
+template <int XD, int ZD, bool VEC>
+NormKernel norm_kernel(int kind) {
+  return kind == 0 ? gated_norm_kernel<XD, ZD, VEC, 1, 256> : kind == 1 ? gated_norm_kernel<XD, ZD, VEC, 2, 128>
+                                                                        : gated_norm_kernel<XD, ZD, VEC, 2, 512>;
+}
+template <int XD, int ZD, bool VEC>
+NormKernel back_kernel(int kind) {
+  return kind == 0 ? gated_norm_back_kernel<XD, ZD, VEC, 1, 128> : kind == 1 ? gated_norm_back_kernel<XD, ZD, VEC, 1, 256>
+                                                                             : gated_norm_back_kernel<XD, ZD, VEC, 2, 512>;
+}
+NormKernel pick(bool back, int xdt, int zdt, bool vec, int kind) {
+#define SB_PICK(X, Z, V) (back ? back_kernel<X, Z, V>(kind) : norm_kernel<X, Z, V>(kind))
+  if (!vec) return SB_PICK(-1, -1, false);
+  if (xdt == SB_F32 && zdt == SB_F16) return SB_PICK(SB_F32, SB_F16, true);
+  if (xdt == SB_F32 && zdt == SB_BF16) return SB_PICK(SB_F32, SB_BF16, true);
+  if (xdt == SB_F16 && zdt == SB_F16) return SB_PICK(SB_F16, SB_F16, true);
+  if (xdt == SB_BF16 && zdt == SB_BF16) return SB_PICK(SB_BF16, SB_BF16, true);
+  return SB_PICK(-1, -1, true);
+#undef SB_PICK
+}
+
+// CTAs a group of rows: about `kBackCtas` a SM over all groups, at least eight rows a warp or CTA
+constexpr int kBackCtas = 3;
 int chunks_of(int groups, long long group_rows, const Plan& p, int sms) {
-  const long long want = std::max(1, 2 * sms / groups);
+  const long long want = std::max(1, kBackCtas * sms / groups);
   return (int)std::max(1ll, std::min(want, (group_rows + 8 * p.per - 1) / (8 * p.per)));
 }
 
@@ -405,7 +550,7 @@ extern "C" int sb_gated_norm(const void* x, long long x_row, long long x_img, in
   if (B == 0 || T == 0) return SB_OK;
   if (!x || !z || !y || (pre_w != nullptr) != (h != nullptr) || (post_b && !post_w) || (pre_b && !pre_w))
     return record_error(SB_EINVAL, "sb_gated_norm: null argument (h with pre_w, biases with their weights)");
-  const Plan p = plan_of(D);
+  const Plan p = plan_of(D, false);
   NormArgs a{};
   a.x = {x, x_row, x_img};
   a.z = {z, z_row, z_img};
@@ -423,10 +568,14 @@ extern "C" int sb_gated_norm(const void* x, long long x_row, long long x_img, in
                    cols_aligned(pre_b);
   const int sms = sm_count();
   if (sms == 0) return record_error(SB_ECUDA, "sb_gated_norm: device");
-  const long long grid = std::min((a.rows + p.per - 1) / p.per, (long long)sms * std::max(1, 1536 / p.threads));
-  auto kernel = p.threads <= 256   ? vec ? gated_norm_kernel<true, 256> : gated_norm_kernel<false, 256>
-                : p.threads <= 512 ? vec ? gated_norm_kernel<true, 512> : gated_norm_kernel<false, 512>
-                                   : vec ? gated_norm_kernel<true, 1024> : gated_norm_kernel<false, 1024>;
+  const NormKernel kernel = pick(false, x_dtype, z_dtype, vec, p.kind);
+  int ctas = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, p.threads, 0) != cudaSuccess || ctas < 1)
+    return record_error(SB_ECUDA, "sb_gated_norm: occupancy");
+  const long long grid = std::min((a.rows + p.per - 1) / p.per, (long long)sms * ctas);
+  const long long step = grid * p.per;
+  a.step_b = step / T;
+  a.step_t = (int)(step % T);
   kernel<<<(unsigned)grid, p.threads, 0, (cudaStream_t)stream>>>(a);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return record_error(SB_ECUDA, cudaGetErrorString(e));
@@ -437,7 +586,7 @@ extern "C" int sb_gated_norm_work(int B, int T, int D, long long* bytes) {
   if (!bytes || B < 0 || T < 0 || D < 1 || D > kMaxD) return record_error(SB_EINVAL, "sb_gated_norm_work: arguments");
   const int sms = sm_count();
   if (sms == 0) return record_error(SB_ECUDA, "sb_gated_norm_work: device");
-  const Plan p = plan_of(D);
+  const Plan p = plan_of(D, true);
   // enough for one group of all rows and for a group an item
   const long long one = chunks_of(1, (long long)B * T, p, sms), each = (long long)B * chunks_of(std::max(1, B), T, p, sms);
   *bytes = std::max(one, each) * kSums * D * 4;
@@ -462,7 +611,7 @@ extern "C" int sb_gated_norm_backward(const void* dy, long long dy_row, long lon
   const bool by_img = gate && gate_img != 0 && B > 1;
   if ((dgate_mode == 1 && (by_row || by_img)) || (dgate_mode == 2 && by_row))
     return record_error(SB_EINVAL, "sb_gated_norm_backward: dgate_mode does not fit the gate's strides");
-  const Plan p = plan_of(D);
+  const Plan p = plan_of(D, true);
   NormArgs a{};
   a.x = {x, x_row, x_img};
   a.z = {z, z_row, z_img};
@@ -495,13 +644,8 @@ extern "C" int sb_gated_norm_backward(const void* dy, long long dy_row, long lon
                    rows_aligned(dz, z_dtype, 0, 0) && (dgate_mode != 3 || rows_aligned(dgate, z_dtype, 0, 0)) &&
                    cols_aligned(scale) && cols_aligned(post_w) && cols_aligned(post_b) && cols_aligned(pre_w) &&
                    cols_aligned(pre_b);
-  auto kernel = p.threads <= 256   ? vec ? gated_norm_back_kernel<true, 256> : gated_norm_back_kernel<false, 256>
-                : p.threads <= 512 ? vec ? gated_norm_back_kernel<true, 512> : gated_norm_back_kernel<false, 512>
-                                   : vec ? gated_norm_back_kernel<true, 1024> : gated_norm_back_kernel<false, 1024>;
-  const int smem = sums ? p.per * kSums * p.tpr * 8 * 4 : 0;
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return record_error(SB_ECUDA, "sb_gated_norm_backward: shared memory");
+  const NormKernel kernel = pick(true, x_dtype, z_dtype, vec, p.kind);
+  const int smem = sums && p.per > 1 ? p.per * kSums * p.tpr * 8 * 4 : 0;
   if ((long long)groups * a.chunks > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_gated_norm_backward: too many items");
   kernel<<<(unsigned)(groups * a.chunks), p.threads, smem, (cudaStream_t)stream>>>(a);
   if (sums) {

@@ -23,6 +23,7 @@ calls record no graph and refuse tensors that would need one.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -30,98 +31,128 @@ from . import _lib
 from ._lib import check, lib
 
 DTYPES = {torch.float16: _lib.SB_F16, torch.bfloat16: _lib.SB_BF16, torch.float32: _lib.SB_F32}
+_HALVES = (torch.float16, torch.bfloat16)
 
 # library calls made through this module
 CALLS = [0]
 
-
-def _require(ok, what):
-    if not ok:
-        raise ValueError(what)
+# A call's host time is what a small call costs, so the checks below format their messages only
+# when they fail and read each tensor's attributes once.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _ready(*tensors):
-    """All tensors on one CUDA device and none that autograd would have to follow."""
-    tensors = [t for t in tensors if t is not None]
-    dev = tensors[0].device
+    """All tensors on one CUDA device and none that autograd would have to follow; its index."""
+    index = tensors[0].get_device()
+    grad = torch.is_grad_enabled()
     for t in tensors:
-        _require(t.is_cuda and t.device == dev, "tensors of one CUDA device")
-        _require(not (t.requires_grad and torch.is_grad_enabled()),
-                 "no autograd graph is recorded: call under torch.no_grad() or from an autograd.Function")
-    return dev
+        if t is not None:
+            if t.get_device() != index or not t.is_cuda:
+                raise ValueError("tensors of one CUDA device")
+            if grad and t.requires_grad:
+                raise ValueError("no autograd graph is recorded: call under torch.no_grad() or from an autograd.Function")
+    return index
 
 
-def _launch(name, dev, *args):
+def _launch(name, index, *args):
     CALLS[0] += 1
-    if dev.index == torch.cuda.current_device():
-        status = getattr(lib(), name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if index == torch.cuda.current_device():
+        status = getattr(lib(), name)(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            status = getattr(lib(), name)(*args, torch.cuda.current_stream(dev).cuda_stream)
-    check(status, name)
+        with torch.cuda.device(index):
+            status = getattr(lib(), name)(*args, _raw_stream(index))
+    if status:
+        check(status, name)
 
 
-def _work(name, dev, *args):
-    """Workspace of a call: (tensor or None, pointer, bytes)."""
+@functools.lru_cache(maxsize=4096)
+def _work_bytes(name, index, *args):
+    """Workspace bytes of a call with these sizes on this device."""
     n = C.c_longlong(0)
-    with torch.cuda.device(dev):
+    with torch.cuda.device(index):
         check(getattr(lib(), name)(*args, C.byref(n)), name)
-    if n.value == 0:
+    return n.value
+
+
+def _work(name, index, *args):
+    """Workspace of a call: (tensor or None, pointer, bytes)."""
+    n = _work_bytes(name, index, *args)
+    if n == 0:
         return None, None, 0
-    w = torch.empty(n.value, device=dev, dtype=torch.uint8)
-    return w, w.data_ptr(), n.value
+    w = torch.empty(n, device=torch.device("cuda", index), dtype=torch.uint8)
+    return w, w.data_ptr(), n
 
 
-def _rows(t, what, shape, dtype=None, out=False):
+def _rows(t, what, shape, dtype, out=False):
     """(pointer, row stride, item stride) in elements of [B, T, C] rows."""
-    _require(t.dim() == 3 and tuple(t.shape) == tuple(shape), f"{what}: expected {tuple(shape)}, got {tuple(t.shape)}")
-    _require(dtype is None or t.dtype == dtype, f"{what}: expected {dtype}, got {t.dtype}")
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{what}: expected {tuple(shape)} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
     b, n, c = shape
-    _require(c <= 1 or t.stride(2) == 1, f"{what}: channels must be contiguous")
+    img, row, one = t.stride()
+    if one != 1 and c > 1:
+        raise ValueError(f"{what}: channels must be contiguous")
     # the stride of a dimension of one element is arbitrary and never used
-    row = t.stride(1) if n > 1 else c
-    img = t.stride(0) if b > 1 else n * row
-    if out and t.numel():
+    if n <= 1:
+        row = c
+    if b <= 1:
+        img = n * row
+    if out and (row < c or img < row * (n - 1) + c) and t.numel():
         apart = (n == 1 or row >= c) and (b == 1 or img >= c) and \
             (n == 1 or b == 1 or img >= row * (n - 1) + c or row >= img * (b - 1) + c)
-        _require(apart, f"{what}: rows overlap")
+        if not apart:
+            raise ValueError(f"{what}: rows overlap")
     return t.data_ptr(), row, img
 
 
+def _dense(t, shape):
+    """_rows of a new tensor."""
+    return t.data_ptr(), shape[2], shape[1] * shape[2]
+
+
 # ---------------------------------------------------------------- attention
-def _attention_sizes(q, k, v, heads, kv_heads, scale):
-    _require(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k, v: [B, T, heads * dim] rows")
-    _require(q.dtype in (torch.float16, torch.bfloat16), "q: fp16 or bf16")
-    kv_heads = heads if kv_heads is None else kv_heads
-    _require(heads >= 1 and kv_heads >= 1 and heads % kv_heads == 0, "heads: a multiple of kv_heads")
+def _attention_sizes(q, k, heads, kv_heads, scale):
+    if q.dim() != 3 or k.dim() != 3 or q.dtype not in _HALVES:
+        raise ValueError("q, k, v: [B, T, heads * dim] rows of fp16 or bf16")
+    if kv_heads is None:
+        kv_heads = heads
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError("heads: a multiple of kv_heads")
     b, tq, width = q.shape
     dim = width // heads
-    _require(width == heads * dim and dim in (32, 64, 128), "heads of 32, 64 or 128 channels")
-    tk = k.shape[1]
+    if dim not in (32, 64, 128) or width != heads * dim:
+        raise ValueError("heads of 32, 64 or 128 channels")
     if scale is None:
         scale = dim ** -0.5
-    _require(0.0 < scale < float("inf"), "scale: a positive number")
-    return kv_heads, b, tq, tk, dim, float(scale)
+    if not 0.0 < scale < _INF:
+        raise ValueError("scale: a positive number")
+    return kv_heads, b, tq, k.shape[1], dim, scale
+
+
+_INF = float("inf")
+_NO_MASK = (None, None, 0)
 
 
 def _masks(lens, valid, b, tk):
     """Pointers of the masks: (lens, valid, valid's item stride)."""
+    if lens is None and valid is None:
+        return _NO_MASK
     p_lens = p_valid = None
     img = 0
     if lens is not None:
-        _require(lens.dtype == torch.int32 and tuple(lens.shape) == (b,) and (b <= 1 or lens.stride(0) == 1),
-                 "lens: contiguous int32 [B]")
+        if lens.dtype != torch.int32 or lens.shape != (b,) or (b > 1 and lens.stride(0) != 1):
+            raise ValueError("lens: contiguous int32 [B]")
         p_lens = lens.data_ptr()
     if valid is not None:
-        _require(valid.dtype in (torch.uint8, torch.bool) and tuple(valid.shape) == (b, tk) and
-                 (tk <= 1 or valid.stride(1) == 1), "valid: uint8 or bool [B, Tk] with contiguous rows")
+        if valid.dtype not in (torch.uint8, torch.bool) or valid.shape != (b, tk) or (tk > 1 and valid.stride(1) != 1):
+            raise ValueError("valid: uint8 or bool [B, Tk] with contiguous rows")
         p_valid, img = valid.data_ptr(), valid.stride(0) if b > 1 else tk
     return p_lens, p_valid, img
 
 
 def _statistics(lse, b, heads, tq):
-    _require(lse.dtype == torch.float32 and tuple(lse.shape) == (b, heads, tq) and lse.is_contiguous(),
-             "lse: contiguous fp32 [B, heads, Tq]")
+    if lse.dtype != torch.float32 or lse.shape != (b, heads, tq) or not lse.is_contiguous():
+        raise ValueError("lse: contiguous fp32 [B, heads, Tq]")
 
 
 def cross_attention(q, k, v, heads, kv_heads=None, lens=None, valid=None, scale=None, out=None, lse=None):
@@ -134,23 +165,22 @@ def cross_attention(q, k, v, heads, kv_heads=None, lens=None, valid=None, scale=
     (allocated if None; it must not share memory with q, k or v) and, if given, lse (fp32 [B, heads,
     Tq], the log-sum-exp of the scaled scores, -inf without states), which the backward pass reads.  Few
     queries on many states (single tokens) are split over the states."""
-    kv_heads, b, tq, tk, dim, scale = _attention_sizes(q, k, v, heads, kv_heads, scale)
-    qp = _rows(q, "q", (b, tq, heads * dim))
-    kp = _rows(k, "k", (b, tk, kv_heads * dim), q.dtype)
-    vp = _rows(v, "v", (b, tk, kv_heads * dim), q.dtype)
+    kv_heads, b, tq, tk, dim, scale = _attention_sizes(q, k, heads, kv_heads, scale)
+    dtype, qs, ks = q.dtype, (b, tq, heads * dim), (b, tk, kv_heads * dim)
+    qp, kp, vp = _rows(q, "q", qs, dtype), _rows(k, "k", ks, dtype), _rows(v, "v", ks, dtype)
     masks = _masks(lens, valid, b, tk)
     if lse is not None:
         _statistics(lse, b, heads, tq)
     if out is not None:
-        op = _rows(out, "out", (b, tq, heads * dim), q.dtype, out=True)
-    dev = _ready(q, k, v, lens, valid, out, lse)
+        op = _rows(out, "out", qs, dtype, out=True)
+    index = _ready(q, k, v, lens, valid, out, lse)
     if out is None:
-        out = torch.empty(b, tq, heads * dim, device=dev, dtype=q.dtype)
-        op = (out.data_ptr(), heads * dim, tq * heads * dim)
-    if out.numel() == 0:
+        out = torch.empty(qs, device=q.device, dtype=dtype)
+        op = _dense(out, qs)
+    if b == 0 or tq == 0:
         return out
-    hold, work, size = _work("sb_cross_attention_work", dev, 0, b, heads, kv_heads, dim, tq, tk)
-    _launch("sb_cross_attention", dev, *qp, *kp, *vp, DTYPES[q.dtype], b, heads, kv_heads, dim, tq, tk, scale, *masks,
+    hold, work, size = _work("sb_cross_attention_work", index, 0, b, heads, kv_heads, dim, tq, tk)
+    _launch("sb_cross_attention", index, *qp, *kp, *vp, DTYPES[dtype], b, heads, kv_heads, dim, tq, tk, scale, *masks,
             *op, None if lse is None else lse.data_ptr(), work, size)
     return out
 
@@ -162,25 +192,25 @@ def cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=None, lens
     The same sizes, masks and scale as forward.  dk and dv have one row for every item's state, also
     where k and v are shared by the items (sum them over the batch then); states that take no part
     get zeros.  The sums have a fixed order: the same inputs give the same bits."""
-    kv_heads, b, tq, tk, dim, scale = _attention_sizes(q, k, v, heads, kv_heads, scale)
-    qs, ks = (b, tq, heads * dim), (b, tk, kv_heads * dim)
-    views = [_rows(dout, "dout", qs, q.dtype), _rows(q, "q", qs), _rows(k, "k", ks, q.dtype),
-             _rows(v, "v", ks, q.dtype), _rows(out, "out", qs, q.dtype)]
+    kv_heads, b, tq, tk, dim, scale = _attention_sizes(q, k, heads, kv_heads, scale)
+    dtype, qs, ks = q.dtype, (b, tq, heads * dim), (b, tk, kv_heads * dim)
+    views = _rows(dout, "dout", qs, dtype) + _rows(q, "q", qs, dtype) + _rows(k, "k", ks, dtype) + \
+        _rows(v, "v", ks, dtype) + _rows(out, "out", qs, dtype)
     masks = _masks(lens, valid, b, tk)
     _statistics(lse, b, heads, tq)
-    for name, t, s in (("dq", dq, qs), ("dk", dk, ks), ("dv", dv, ks)):
+    for what, t, shape in (("dq", dq, qs), ("dk", dk, ks), ("dv", dv, ks)):
         if t is not None:
-            _rows(t, name, s, q.dtype, out=True)
-    dev = _ready(dout, q, k, v, out, lse, lens, valid, dq, dk, dv)
-    dq = torch.empty(qs, device=dev, dtype=q.dtype) if dq is None else dq
-    dk = torch.empty(ks, device=dev, dtype=q.dtype) if dk is None else dk
-    dv = torch.empty(ks, device=dev, dtype=q.dtype) if dv is None else dv
+            _rows(t, what, shape, dtype, out=True)
+    index = _ready(dout, q, k, v, out, lse, lens, valid, dq, dk, dv)
+    dq = torch.empty(qs, device=q.device, dtype=dtype) if dq is None else dq
+    dk = torch.empty(ks, device=q.device, dtype=dtype) if dk is None else dk
+    dv = torch.empty(ks, device=q.device, dtype=dtype) if dv is None else dv
     if dq.numel() == 0 and dk.numel() == 0:
         return dq, dk, dv
-    grads = [_rows(t, name, s) for name, t, s in (("dq", dq, qs), ("dk", dk, ks), ("dv", dv, ks))]
-    hold, work, size = _work("sb_cross_attention_work", dev, 1, b, heads, kv_heads, dim, tq, tk)
-    _launch("sb_cross_attention_backward", dev, *(x for t in views for x in t), lse.data_ptr(), DTYPES[q.dtype], b, heads,
-            kv_heads, dim, tq, tk, scale, *masks, *(x for t in grads for x in t), work, size)
+    grads = _rows(dq, "dq", qs, dtype) + _rows(dk, "dk", ks, dtype) + _rows(dv, "dv", ks, dtype)
+    hold, work, size = _work("sb_cross_attention_work", index, 1, b, heads, kv_heads, dim, tq, tk)
+    _launch("sb_cross_attention_backward", index, *views, lse.data_ptr(), DTYPES[dtype], b, heads, kv_heads, dim, tq, tk,
+            scale, *masks, *grads, work, size)
     return dq, dk, dv
 
 
@@ -188,7 +218,8 @@ def cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=None, lens
 def rope_table(sections, theta=10000.0, per_axis=True, device="cuda"):
     """(freq fp64 [R], axis int32 [R]) of :func:`rope_axes`: ``sections[a]`` pairs turn with axis a, in
     this order.  Frequencies theta ** (-i / n): i counts an axis's own n pairs (per_axis), or all R."""
-    _require(len(sections) >= 1 and all(int(n) == n and n >= 0 for n in sections) and theta > 0, "sections of pairs")
+    if len(sections) < 1 or any(int(n) != n or n < 0 for n in sections) or not theta > 0:
+        raise ValueError("sections: numbers of pairs; theta > 0")
     total = sum(sections)
     i = [torch.arange(n, dtype=torch.float64) / max(n, 1) for n in sections]
     i = torch.cat(i) if per_axis else torch.arange(total, dtype=torch.float64) / max(total, 1)
@@ -210,62 +241,74 @@ def rope_axes(x, pos, heads, freq, axis, layout="half", inverse=False, out=None)
     (:func:`rope_table`; an axis outside pos's leaves its pair).  Pairs are channels (p, p + R) of a
     head ("half") or (2p, 2p + 1) ("pairs"); channels from 2R on stay as they are.  Angles are formed in
     fp64, so positions in the millions keep their fraction of a turn.  out may be x itself."""
-    _require(x.dim() == 3 and x.dtype in DTYPES, "x: [B, T, heads * dim] of fp16, bf16 or fp32")
-    b, t, width = x.shape
-    _require(heads >= 1 and width % heads == 0 and width > 0, "x: a multiple of heads channels")
-    dim = width // heads
-    _require(layout in ("half", "pairs"), "layout: 'half' or 'pairs'")
-    _require(freq.dtype == torch.float64 and axis.dtype == torch.int32 and freq.dim() == 1 and
-             freq.shape == axis.shape and freq.is_contiguous() and axis.is_contiguous(), "freq fp64 [R], axis int32 [R]")
-    _require(2 * freq.numel() <= dim, "pairs: at most half of a head's channels")
-    _require(pos.dtype in (torch.int32, torch.float32) and pos.dim() in (2, 3) and
-             tuple(pos.shape[:-1]) in ((t,), (b, t)) and pos.shape[-1] >= 1, "pos: int32 or fp32 [B, T, A] or [T, A]")
-    a = pos.shape[-1]
-    _require((a == 1 or pos.stride(-1) == 1) and (t <= 1 or pos.stride(-2) == a), "pos: contiguous rows")
-    pos_img = pos.stride(0) if pos.dim() == 3 and b > 1 else 0
-    xp = _rows(x, "x", (b, t, width))
+    dtype = x.dtype
+    if x.dim() != 3 or dtype not in DTYPES:
+        raise ValueError("x: [B, T, heads * dim] of fp16, bf16 or fp32")
+    shape = b, t, width = x.shape
+    if heads < 1 or width == 0 or width % heads:
+        raise ValueError("x: a multiple of heads channels")
+    dim, r = width // heads, freq.numel()
+    if layout not in ("half", "pairs"):
+        raise ValueError("layout: 'half' or 'pairs'")
+    if freq.dtype != torch.float64 or axis.dtype != torch.int32 or freq.dim() != 1 or axis.shape != freq.shape or \
+            not freq.is_contiguous() or not axis.is_contiguous():
+        raise ValueError("freq: fp64 [R], axis: int32 [R]")
+    if 2 * r > dim:
+        raise ValueError("pairs: at most half of a head's channels")
+    at, ps = pos.shape, pos.stride()
+    if pos.dtype not in (torch.int32, torch.float32) or at[:-1] not in ((t,), (b, t)) or at[-1] < 1:
+        raise ValueError("pos: int32 or fp32 [B, T, A] or [T, A]")
+    if (at[-1] > 1 and ps[-1] != 1) or (t > 1 and ps[-2] != at[-1]):
+        raise ValueError("pos: contiguous rows")
+    xp = _rows(x, "x", shape, dtype)
     if out is not None:
-        op = _rows(out, "out", (b, t, width), x.dtype, out=True)
-    dev = _ready(x, pos, freq, axis, out)
+        op = _rows(out, "out", shape, dtype, out=True)
+    index = _ready(x, pos, freq, axis, out)
     if out is None:
-        out = torch.empty(b, t, width, device=dev, dtype=x.dtype)
-        op = (out.data_ptr(), width, t * width)
-    if out.numel() == 0:
+        out = torch.empty(shape, device=x.device, dtype=dtype)
+        op = _dense(out, shape)
+    if b == 0 or t == 0:
         return out
-    _launch("sb_rope_axes", dev, *xp, DTYPES[x.dtype], b, t, heads, dim, pos.data_ptr(), int(pos.dtype == torch.float32),
-            pos_img, a, freq.data_ptr(), axis.data_ptr(), freq.numel(), int(layout == "pairs"), int(inverse), *op)
+    _launch("sb_rope_axes", index, *xp, DTYPES[dtype], b, t, heads, dim, pos.data_ptr(), pos.dtype == torch.float32,
+            ps[0] if len(at) == 3 and b > 1 else 0, at[-1], freq.data_ptr(), axis.data_ptr(), r, layout == "pairs",
+            bool(inverse), *op)
     return out
 
 
 # ---------------------------------------------------------------- gated residual and norms
+def _columns(t, what, d):
+    if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.numel() != d or not t.is_contiguous()):
+        raise ValueError(f"{what}: contiguous fp32 [D]")
+    return t
+
+
 def _norm_weights(w, what, d, kind):
-    """A norm's (weight, bias) or None -> (weight, bias) tensors or None."""
+    """A norm's weight, (weight, bias) or None -> (weight, bias)."""
     if w is None:
         return None, None
     w, b = w if isinstance(w, (tuple, list)) else (w, None)
-    for t in (w, b):
-        _require(t is None or (t.dtype == torch.float32 and tuple(t.shape) == (d,) and t.is_contiguous()),
-                 f"{what}: contiguous fp32 [D] weight and bias")
-    _require(w is not None and (b is None or kind == "layer"), f"{what}: a weight, and a bias for layer norms only")
-    return w, b
+    if w is None or (b is not None and kind != "layer"):
+        raise ValueError(f"{what}: a weight, and a bias for layer norms only")
+    return _columns(w, what, d), _columns(b, what, d)
 
 
 def _norm_inputs(x, z, gate, scale, post, pre, kind, eps):
-    _require(x.dim() == 3 and x.dtype in DTYPES and z.dtype in DTYPES, "x, z: [B, T, D] of fp16, bf16 or fp32")
-    _require(kind in ("rms", "layer") and eps >= 0, "kind: 'rms' or 'layer', eps >= 0")
-    b, t, d = x.shape
-    _require(1 <= d <= 8192, "1 to 8192 channels")
+    if x.dim() != 3 or x.dtype not in DTYPES or z.dtype not in DTYPES:
+        raise ValueError("x, z: [B, T, D] of fp16, bf16 or fp32")
+    if kind not in ("rms", "layer") or not eps >= 0:
+        raise ValueError("kind: 'rms' or 'layer', eps >= 0")
+    shape = b, t, d = x.shape
+    if not 1 <= d <= 8192:
+        raise ValueError("1 to 8192 channels")
     gp = (None, 0, 0)
     if gate is not None:
-        _require(gate.dtype == z.dtype, "gate: z's type")
-        _require(tuple(gate.shape) in ((d,), (b, d), (b, t, d)), "gate: [D], [B, D] or [B, T, D]")
-        _require(d == 1 or gate.stride(-1) == 1, "gate: channels must be contiguous")
-        row = gate.stride(1) if gate.dim() == 3 and t > 1 else 0
-        gp = (gate.data_ptr(), row, gate.stride(0) if gate.dim() > 1 and b > 1 else 0)
-    _require(scale is None or (scale.dtype == torch.float32 and tuple(scale.shape) == (d,) and scale.is_contiguous()),
-             "scale: contiguous fp32 [D]")
+        n, s = gate.dim(), gate.stride()
+        if gate.dtype != z.dtype or gate.shape not in ((d,), (b, d), (b, t, d)) or (d > 1 and s[-1] != 1):
+            raise ValueError("gate: [D], [B, D] or [B, T, D] of z's type with contiguous channels")
+        gp = (gate.data_ptr(), s[1] if n == 3 and t > 1 else 0, s[0] if n > 1 and b > 1 else 0)
+    _columns(scale, "scale", d)
     weights = _norm_weights(post, "post", d, kind) + _norm_weights(pre, "pre", d, kind)
-    return (b, t, d), _rows(x, "x", (b, t, d)), _rows(z, "z", (b, t, d)), gp, weights
+    return shape, _rows(x, "x", shape, x.dtype), _rows(z, "z", shape, z.dtype), gp, weights
 
 
 def _ptr(t):
@@ -279,20 +322,24 @@ def gated_norm(x, z, gate=None, scale=None, post=None, pre=None, kind="rms", eps
     norm's fp32 [D] weight or (weight, bias), None for no norm there (without pre, h is None).  kind:
     "rms" or "layer".  gate: z's type, [D], [B, D] (one an item) or [B, T, D].  scale: fp32 [D].  h comes
     from y before its rounding.  y may be x and h may be z.  Returns (y, h)."""
-    (b, t, d), xp, zp, gp, weights = _norm_inputs(x, z, gate, scale, post, pre, kind, eps)
-    _require(h is None or pre is not None, "h needs the norm pre")
-    yp = _rows(y, "y", (b, t, d), x.dtype, out=True) if y is not None else None
-    hp = _rows(h, "h", (b, t, d), z.dtype, out=True) if h is not None else (None, 0, 0)
-    dev = _ready(x, z, gate, scale, *weights, y, h)
+    shape, xp, zp, gp, weights = _norm_inputs(x, z, gate, scale, post, pre, kind, eps)
+    hp = (None, 0, 0)
+    if y is not None:
+        yp = _rows(y, "y", shape, x.dtype, out=True)
+    if h is not None:
+        if pre is None:
+            raise ValueError("h needs the norm pre")
+        hp = _rows(h, "h", shape, z.dtype, out=True)
+    index = _ready(x, z, gate, scale, *weights, y, h)
     if y is None:
-        y = torch.empty(b, t, d, device=dev, dtype=x.dtype)
-        yp = (y.data_ptr(), d, t * d)
+        y = torch.empty(shape, device=x.device, dtype=x.dtype)
+        yp = _dense(y, shape)
     if h is None and pre is not None:
-        h = torch.empty(b, t, d, device=dev, dtype=z.dtype)
-        hp = (h.data_ptr(), d, t * d)
-    if y.numel():
-        _launch("sb_gated_norm", dev, *xp, DTYPES[x.dtype], *zp, DTYPES[z.dtype], *gp, _ptr(scale), *map(_ptr, weights),
-                int(kind == "layer"), eps, b, t, d, *yp, *hp)
+        h = torch.empty(shape, device=x.device, dtype=z.dtype)
+        hp = _dense(h, shape)
+    if shape[0] and shape[1]:
+        _launch("sb_gated_norm", index, *xp, DTYPES[x.dtype], *zp, DTYPES[z.dtype], *gp, _ptr(scale), *map(_ptr, weights),
+                kind == "layer", eps, *shape, *yp, *hp)
     return y, h
 
 
@@ -302,21 +349,23 @@ def gated_norm_backward(dy, dh, x, z, gate=None, scale=None, post=None, pre=None
     Returns a dict of dx (x's type), dz (z's type) and, where there is such an input, fp32 scale,
     post_w, post_b, pre_w, pre_b [D] and gate: fp32 [D] or [B, D] sums for a gate of that shape, z's
     type for one of [B, T, D]; None otherwise.  The sums over rows have a fixed order."""
-    (b, t, d), xp, zp, gp, weights = _norm_inputs(x, z, gate, scale, post, pre, kind, eps)
-    _require(dh is None or pre is not None, "dh needs the norm pre")
-    dyp = _rows(dy, "dy", (b, t, d), x.dtype) if dy is not None else (None, 0, 0)
-    dhp = _rows(dh, "dh", (b, t, d), z.dtype) if dh is not None else (None, 0, 0)
-    dev = _ready(x, z, gate, scale, *weights, dy, dh)
-    g = {"dx": torch.empty(b, t, d, device=dev, dtype=x.dtype), "dz": torch.empty(b, t, d, device=dev, dtype=z.dtype)}
+    shape, xp, zp, gp, weights = _norm_inputs(x, z, gate, scale, post, pre, kind, eps)
+    b, t, d = shape
+    if dh is not None and pre is None:
+        raise ValueError("dh needs the norm pre")
+    dyp = (None, 0, 0) if dy is None else _rows(dy, "dy", shape, x.dtype)
+    dhp = (None, 0, 0) if dh is None else _rows(dh, "dh", shape, z.dtype)
+    index = _ready(x, z, gate, scale, *weights, dy, dh)
+    g = {"dx": torch.empty(shape, device=x.device, dtype=x.dtype), "dz": torch.empty(shape, device=x.device, dtype=z.dtype)}
     make = torch.empty if b * t else torch.zeros  # no rows: every sum is zero
     for name, w in zip(("scale", "post_w", "post_b", "pre_w", "pre_b"), (scale,) + weights):
-        g[name] = None if w is None else make(d, device=dev, dtype=torch.float32)
+        g[name] = None if w is None else make(d, device=x.device, dtype=torch.float32)
     mode = 0 if gate is None else gate.dim()
-    g["gate"] = None if gate is None else make(gate.shape, device=dev, dtype=z.dtype if mode == 3 else torch.float32)
+    g["gate"] = None if gate is None else make(gate.shape, device=x.device, dtype=z.dtype if mode == 3 else torch.float32)
     if b * t == 0:
         return g
-    hold, work, size = _work("sb_gated_norm_work", dev, b, t, d)
-    _launch("sb_gated_norm_backward", dev, *dyp, *dhp, *xp, DTYPES[x.dtype], *zp, DTYPES[z.dtype], *gp, _ptr(scale),
-            *map(_ptr, weights), int(kind == "layer"), eps, b, t, d, _ptr(g["dx"]), _ptr(g["dz"]), _ptr(g["scale"]),
+    hold, work, size = _work("sb_gated_norm_work", index, b, t, d)
+    _launch("sb_gated_norm_backward", index, *dyp, *dhp, *xp, DTYPES[x.dtype], *zp, DTYPES[z.dtype], *gp, _ptr(scale),
+            *map(_ptr, weights), kind == "layer", eps, b, t, d, _ptr(g["dx"]), _ptr(g["dz"]), _ptr(g["scale"]),
             _ptr(g["gate"]), mode, _ptr(g["post_w"]), _ptr(g["post_b"]), _ptr(g["pre_w"]), _ptr(g["pre_b"]), work, size)
     return g

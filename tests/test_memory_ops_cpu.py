@@ -8,6 +8,7 @@ import torch
 import sarbon_b200 as sb
 from sarbon_b200 import _lib, memory_ops as mo
 
+F32 = torch.float32
 H16 = dict(dtype=torch.float16)
 
 
@@ -78,14 +79,14 @@ def test_gated_norm_refuses():
 
 def test_strides_of_views():
     wide = torch.zeros(2, 5, 192)
-    assert mo._rows(wide[..., 64:128], "x", (2, 5, 64))[1:] == (192, 960)
+    assert mo._rows(wide[..., 64:128], "x", (2, 5, 64), F32)[1:] == (192, 960)
     first = torch.zeros(5, 2, 64).transpose(0, 1)  # sequence first
-    assert mo._rows(first, "x", (2, 5, 64), out=True)[1:] == (128, 64)
+    assert mo._rows(first, "x", (2, 5, 64), F32, out=True)[1:] == (128, 64)
     shared = torch.zeros(1, 5, 64).expand(3, 5, 64)
-    assert mo._rows(shared, "x", (3, 5, 64))[1:] == (64, 0)
+    assert mo._rows(shared, "x", (3, 5, 64), F32)[1:] == (64, 0)
     one = torch.zeros(3, 9, 64)[:, 4:5]
-    assert mo._rows(one, "x", (3, 1, 64), out=True)[1:] == (64, 576)
-    assert mo._rows(torch.zeros(3, 9, 64)[:, ::3], "x", (3, 3, 64), out=True)[1:] == (192, 576)
+    assert mo._rows(one, "x", (3, 1, 64), F32, out=True)[1:] == (64, 576)
+    assert mo._rows(torch.zeros(3, 9, 64)[:, ::3], "x", (3, 3, 64), F32, out=True)[1:] == (192, 576)
 
 
 def test_library_refuses():
