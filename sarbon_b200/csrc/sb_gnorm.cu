@@ -19,13 +19,14 @@
 // Each CTA keeps its columns' sums in registers over its rows and writes them once; a second
 // kernel adds the CTAs' sums in a fixed order (no atomics: the same inputs give the same bits).
 //
-// A row belongs to one warp, or to all of a CTA's threads, NV vectors of eight columns each; a
-// CTA walks its rows with the next row's loads issued before the current row's reductions.  Element
-// types are compile-time for the usual pairs (DT of the template), so a row costs few registers
-// and no selects.
+// A row belongs to a team: one warp, or all of a CTA's threads; a thread has NV vectors of eight
+// columns.  Rows reach shared memory by bulk copies (x, z, dy, dh and a row's own gate), several rows
+// ahead, so what is in flight does not cost registers and the reductions' latency is hidden.
+// Element types are compile-time for the usual pairs.  Rows that are not 16-byte aligned or not a
+// multiple of eight columns take plain loads, one row ahead (the kernels named `_any`).
 #include <algorithm>
 
-#include "sb_rows.cuh"
+#include "sb_xattn.cuh"
 
 namespace sb {
 namespace {
@@ -46,7 +47,7 @@ struct NormArgs {
   float eps;
   int T, D, tpr, per;  // threads a row, rows a CTA takes at once (several: a warp each)
   long long rows;      // B * T
-  long long step_b;    // a CTA's step from row to row as (items, rows): no division in the loop
+  long long step_b;    // a team's step from row to row as (items, rows): no division in the loop
   int step_t;
   void *y, *h;         // forward
   long long y_row, y_img, h_row, h_img;
@@ -54,6 +55,8 @@ struct NormArgs {
   float* part;                 // [groups * chunks][kSums][D]
   long long group_rows;        // rows that share their column sums (T for an image's gate, B * T else)
   int chunks, gate_is_row;     // CTAs a group
+  int stages, stage_bytes;     // rows in a team's ring, bytes of one
+  long long team_rows;         // forward: rows of a team
 };
 
 // Sum of a pair of values over the threads of a row; the two halves of the buffer alternate, so one
@@ -102,27 +105,13 @@ struct Cols {
   SB_DEV int n(int j) const { return max(0, min(8, D - at(j))); }
 };
 
-template <bool VEC>
-SB_DEV Raw8 fetch(const void* p, int dt, long long i, int n) {
-  if constexpr (VEC) return n > 0 ? load_raw8(p, dt, i) : Raw8{};
-  else return load_raw8_tail(p, dt, i, n);
-}
-template <bool VEC>
-SB_DEV void put(void* p, int dt, long long i, const float (&v)[8], int n) {
-  if constexpr (VEC) {
-    if (n > 0) store8(p, dt, i, v);
-  } else {
-    store8_tail(p, dt, i, v, n);
-  }
-}
-template <bool VEC>
 SB_DEV void columns(const float* w, int c, int n, float other, float (&v)[8]) {
   if (!w) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) v[u] = other;
     return;
   }
-  unpack8(fetch<VEC>(w, SB_F32, c, n), SB_F32, v);
+  unpack8(load_raw8_tail(w, SB_F32, c, n), SB_F32, v);
 }
 
 // mean and 1 / deviation of a row whose columns past D hold zeros
@@ -151,11 +140,451 @@ SB_DEV void stats_of(const float (&v)[NV][8], const Cols<NV>& cols, int layer, f
   r = rsqrtf(sum(q) * inv_d + eps);
 }
 
-// XD, ZD: dtype codes of x and z, -1: as the arguments say
-template <int XD, int ZD, bool VEC, int NV, int MAXT>
+// ---------------------------------------------------------------- rows through shared memory
+// The same value in every lane: whether all of the team's threads say yes (a barrier of the team).
+SB_DEV bool team_all(bool yes, int warps) {
+  return warps == 1 ? __all_sync(0xFFFFFFFFu, yes) : __syncthreads_and(yes) != 0;
+}
+// 8 fp32 column weights (16-byte aligned, read-only), `other` without any
+SB_DEV void weights8(const float* w, int c, bool on, float other, float (&v)[8]) {
+  if (w && on) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(w + c)), y = __ldg(reinterpret_cast<const float4*>(w + c) + 1);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = other;
+  }
+}
+template <int DT>
+SB_DEV void from_smem(const uint8_t* row, int dt, int c, bool on, float (&v)[8]) {
+  if (on) {
+    unpack8(load_raw8(row, DT < 0 ? dt : DT, c), DT < 0 ? dt : DT, v);
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = 0.f;
+  }
+}
+// 1 / deviation r and -mean r of a row, so that its hats are v r + shift; `on[j]`: vector j exists
+// (the others hold zeros)
+template <bool LAYER, int NV>
+SB_DEV void stats8(const float (&v)[NV][8], const bool (&on)[NV], float inv_d, float eps, RowSum& sum, float& r,
+                   float& shift) {
+  float mean = 0.f, q = 0.f;
+  if (LAYER) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[j][u];
+    mean = sum(s) * inv_d;
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if (on[j]) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float d = LAYER ? v[j][u] - mean : v[j][u];
+        q = fmaf(d, d, q);
+      }
+    }
+  r = rsqrtf(sum(q) * inv_d + eps);
+  shift = LAYER ? -mean * r : 0.f;
+}
+
+// A team's ring of rows.  Operand o of a row lies `off[o]` bytes into its stage; an operand that is
+// not streamed has no bytes.
+struct Ring {
+  uint8_t* base;
+  uint64_t* full;
+  int stages, stage_bytes;
+};
+// A place in the ring: stage and the parity of its use.
+struct Place {
+  int st = 0;
+  uint32_t parity = 0;
+  SB_DEV void next(const Ring& r) {
+    if (++st == r.stages) {
+      st = 0;
+      parity ^= 1u;
+    }
+  }
+};
+constexpr int kMaxStages = 8;
+
+// The copies of row (b, t) into stage st, by the team's first thread.
+template <bool BACK>
+SB_DEV void fill(const NormArgs& a, const Ring& ring, int st, long long b, int t) {
+  uint64_t* bar = &ring.full[st];
+  uint8_t* dst = ring.base + st * ring.stage_bytes;
+  mbar_arrive_expect_tx(bar, (uint32_t)ring.stage_bytes);
+  const int xs = a.xdt == SB_F32 ? 4 : 2, zs = a.zdt == SB_F32 ? 4 : 2;
+  const uint32_t xb = a.D * xs, zb = a.D * zs;
+  auto copy = [&](const Rows& r, int size, uint32_t bytes) {
+    bulk_load(dst, static_cast<const uint8_t*>(r.p) + (b * r.img + t * r.row) * size, bytes, bar);
+    dst += bytes;
+  };
+  copy(a.z, zs, zb);
+  if (a.gate_is_row) copy(a.gate, zs, zb);
+  if (BACK ? a.dh.p != nullptr : true) copy(a.x, xs, xb);
+  if (BACK && a.dy.p) copy(a.dy, xs, xb);
+  if (BACK && a.dh.p) copy(a.dh, zs, zb);
+}
+
+// A row as (b, t); the team's rows follow each other.
+struct Walk {
+  long long b;
+  int t, T;
+  SB_DEV void next() {
+    if (++t == T) {
+      t = 0;
+      ++b;
+    }
+  }
+};
+
+__device__ int g_gnorm_error;
+
+// A copy did not come: note it, and wait (bounded too) for those in flight before the CTA ends.
+SB_DEV void give_up(const Ring& ring, Place at, int left, int me) {
+  if (me != 0) return;
+  atomicOr(&g_gnorm_error, SB_ERR_TIMEOUT_FULL);
+  for (; left > 0; --left, at.next(ring)) bounded_wait(&ring.full[at.st], at.parity);
+}
+
+// XD, ZD: dtype codes of x and z, -1: as the arguments say.  Each team walks rows that follow each
+// other, so that what depends on the columns alone (and an image's gate) stays in registers:
+// y = x + hat A + B with A = scale gate post_w, B = scale gate post_b.
+template <int XD, int ZD, bool LAYER, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float2 buf[64];
+  __shared__ uint64_t bars[8 * kMaxStages];
+  extern __shared__ __align__(16) uint8_t rows_smem[];
   const int xdt = XD < 0 ? a.xdt : XD, zdt = ZD < 0 ? a.zdt : ZD;
+  const int warps = a.tpr >> 5;
+  RowSum sum{buf, warps, 0};
+  const int sub = a.per > 1 ? threadIdx.x >> 5 : 0, me = a.per > 1 ? threadIdx.x & 31 : threadIdx.x;
+  const Ring ring{rows_smem + (size_t)sub * a.stages * a.stage_bytes, bars + sub * a.stages, a.stages, a.stage_bytes};
+  const float inv_d = 1.f / (float)a.D;
+  int c[NV];
+  bool on[NV];
+  float w[NV][8], o[NV][8];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    c[j] = (me + j * a.tpr) * 8;
+    on[j] = c[j] < a.D;
+    weights8(a.pre_w, c[j], on[j], 1.f, w[j]);
+    if (LAYER) weights8(a.pre_b, c[j], on[j], 0.f, o[j]);
+  }
+  if (me == 0)
+    for (int i = 0; i < a.stages; ++i) mbar_init(&ring.full[i], 1);
+  fence_mbar_init();
+  __syncthreads();
+  const long long begin = min(((long long)blockIdx.x * a.per + sub) * a.team_rows, a.rows);
+  const int n = (int)(min(begin + a.team_rows, a.rows) - begin);
+  Walk at{begin / a.T, (int)(begin % a.T), a.T}, ahead = at;
+  Place here, there;
+  int filled = 0;
+  if (me == 0)
+    for (; filled < min(n, a.stages); ++filled, ahead.next(), there.next(ring))
+      fill<false>(a, ring, there.st, ahead.b, ahead.t);
+  const int go = a.D * (zdt == SB_F32 ? 4 : 2), xo = a.gate_is_row ? 2 * go : go;  // places in a stage: z, gate, x
+  float A[NV][8], B[NV][8];
+  long long gate_of = -1;
+  for (int i = 0; i < n; ++i, at.next(), here.next(ring)) {
+    if (!team_all(bounded_wait(&ring.full[here.st], here.parity), warps)) {
+      give_up(ring, here, filled - i, me);
+      break;
+    }
+    // the team has left row i - 1: its stage is free
+    if (me == 0 && i > 0 && filled < n) {
+      fill<false>(a, ring, there.st, ahead.b, ahead.t);
+      ++filled;
+      ahead.next();
+      there.next(ring);
+    }
+    if (at.b != gate_of) {
+      gate_of = at.b;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        weights8(a.scale, c[j], on[j], 1.f, A[j]);
+        if (a.gate.p && !a.gate_is_row && on[j]) {
+          float g[8];
+          unpack8(load_raw8(a.gate.p, zdt, at.b * a.gate.img + c[j]), zdt, g);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) A[j][u] *= g[u];
+        }
+        if (LAYER) {
+          weights8(a.post_b, c[j], on[j], 0.f, B[j]);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) B[j][u] *= A[j][u];
+        }
+        float pw[8];
+        weights8(a.post_w, c[j], on[j], 1.f, pw);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) A[j][u] *= pw[u];
+      }
+    }
+    const uint8_t* row = ring.base + here.st * a.stage_bytes;
+    float v[NV][8], y[NV][8], r = 1.f, shift = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) from_smem<ZD>(row, zdt, c[j], on[j], v[j]);
+    if (a.post_w) stats8<LAYER>(v, on, inv_d, a.eps, sum, r, shift);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      from_smem<XD>(row + xo, xdt, c[j], on[j], y[j]);
+      if (!on[j]) continue;
+      if (a.gate_is_row) {
+        float g[8];
+        from_smem<ZD>(row + go, zdt, c[j], true, g);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float hat = fmaf(v[j][u], r, shift);
+          y[j][u] = fmaf(g[u], LAYER ? fmaf(hat, A[j][u], B[j][u]) : hat * A[j][u], y[j][u]);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float hat = LAYER ? fmaf(v[j][u], r, shift) : v[j][u] * r;
+          y[j][u] = fmaf(hat, A[j][u], LAYER ? y[j][u] + B[j][u] : y[j][u]);
+        }
+      }
+      store8(a.y, xdt, at.b * a.y_img + at.t * a.y_row + c[j], y[j]);
+    }
+    if (a.h) {
+      stats8<LAYER>(y, on, inv_d, a.eps, sum, r, shift);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (!on[j]) continue;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          y[j][u] = LAYER ? fmaf(fmaf(y[j][u], r, shift), w[j][u], o[j][u]) : y[j][u] * r * w[j][u];
+        store8(a.h, zdt, at.b * a.h_img + at.t * a.h_row + c[j], y[j]);
+      }
+    }
+  }
+}
+
+template <int XD, int ZD, bool LAYER, int NV, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float2 buf[64];
+  __shared__ uint64_t bars[8 * kMaxStages];
+  extern __shared__ __align__(16) uint8_t rows_smem[];
+  const int xdt = XD < 0 ? a.xdt : XD, zdt = ZD < 0 ? a.zdt : ZD;
+  const int warps = a.tpr >> 5;
+  RowSum sum{buf, warps, 0};
+  const int sub = a.per > 1 ? threadIdx.x >> 5 : 0, me = a.per > 1 ? threadIdx.x & 31 : threadIdx.x;
+  const Ring ring{rows_smem + (size_t)sub * a.stages * a.stage_bytes, bars + sub * a.stages, a.stages, a.stage_bytes};
+  const float inv_d = 1.f / (float)a.D;
+  int c[NV];
+  bool on[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    c[j] = (me + j * a.tpr) * 8;
+    on[j] = c[j] < a.D;
+  }
+  if (me == 0)
+    for (int i = 0; i < a.stages; ++i) mbar_init(&ring.full[i], 1);
+  fence_mbar_init();
+  __syncthreads();
+  const long long group = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+  const long long each = (a.group_rows + a.chunks - 1) / a.chunks;
+  const long long last = group * a.group_rows + min((chunk + 1) * each, a.group_rows);
+  const long long part = (each + a.per - 1) / a.per;  // a team's rows
+  const long long begin = min(group * a.group_rows + min(chunk * each, a.group_rows) + sub * part, last);
+  const int n = (int)(min(begin + part, last) - begin);
+  Walk at{begin / a.T, (int)(begin % a.T), a.T}, ahead = at;
+  Place here, there;
+  int filled = 0;
+  if (me == 0)
+    for (; filled < min(n, a.stages); ++filled, ahead.next(), there.next(ring))
+      fill<true>(a, ring, there.st, ahead.b, ahead.t);
+  // places in a stage: z, gate, x, dy, dh
+  const int zb = a.D * (zdt == SB_F32 ? 4 : 2), xb = a.D * (xdt == SB_F32 ? 4 : 2);
+  const int xo = a.gate_is_row ? 2 * zb : zb, dyo = a.dh.p ? xo + xb : xo, dho = a.dy.p ? dyo + xb : dyo;
+  // scale x gate of the CTA's rows (scale alone where every row has its gate)
+  float sg[NV][8], acc[kSums][NV][8];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    weights8(a.scale, c[j], on[j], 1.f, sg[j]);
+    if (a.gate.p && !a.gate_is_row && on[j]) {
+      float g[8];
+      unpack8(load_raw8(a.gate.p, zdt, group * a.gate.img + c[j]), zdt, g);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sg[j][u] *= g[u];
+    }
+#pragma unroll
+    for (int k = 0; k < kSums; ++k)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) acc[k][j][u] = 0.f;
+  }
+  long long out = begin * a.D;
+  for (int i = 0; i < n; ++i, out += a.D, here.next(ring)) {
+    if (!team_all(bounded_wait(&ring.full[here.st], here.parity), warps)) {
+      give_up(ring, here, filled - i, me);
+      break;
+    }
+    if (me == 0 && i > 0 && filled < n) {
+      fill<true>(a, ring, there.st, ahead.b, ahead.t);
+      ++filled;
+      ahead.next();
+      there.next(ring);
+    }
+    const uint8_t* row = ring.base + here.st * a.stage_bytes;
+    float zh[NV][8], d[NV][8], zr = 1.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      from_smem<ZD>(row, zdt, c[j], on[j], zh[j]);
+      from_smem<XD>(row + dyo, xdt, c[j], on[j] && a.dy.p, d[j]);
+    }
+    if (a.post_w) {
+      float shift;
+      stats8<LAYER>(zh, on, inv_d, a.eps, sum, zr, shift);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (on[j]) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) zh[j][u] = LAYER ? fmaf(zh[j][u], zr, shift) : zh[j][u] * zr;
+        }
+    }
+    if (a.dh.p) {
+      float y[NV][8], dh[NV][8];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        from_smem<XD>(row + xo, xdt, c[j], on[j], y[j]);
+        if (!on[j]) continue;
+        float w[8], o[8], f[8];
+        weights8(a.post_w, c[j], true, 1.f, w);
+        if (LAYER) weights8(a.post_b, c[j], true, 0.f, o);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) f[u] = sg[j][u];
+        if (a.gate_is_row) {
+          float g[8];
+          from_smem<ZD>(row + zb, zdt, c[j], true, g);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) f[u] *= g[u];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          y[j][u] = fmaf(f[u], LAYER ? fmaf(zh[j][u], w[u], o[u]) : zh[j][u] * w[u], y[j][u]);
+      }
+      float rs, shift, e0 = 0.f, e1 = 0.f;
+      stats8<LAYER>(y, on, inv_d, a.eps, sum, rs, shift);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float w[8];
+        weights8(a.pre_w, c[j], on[j], 1.f, w);
+        from_smem<ZD>(row + dho, zdt, c[j], on[j], dh[j]);
+        if (!on[j]) continue;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          y[j][u] = LAYER ? fmaf(y[j][u], rs, shift) : y[j][u] * rs;
+          acc[2][j][u] = fmaf(dh[j][u], y[j][u], acc[2][j][u]);
+          if (LAYER) acc[3][j][u] += dh[j][u];
+          dh[j][u] *= w[u];
+          if (LAYER) e0 += dh[j][u];
+          e1 = fmaf(dh[j][u], y[j][u], e1);
+        }
+      }
+      float2 m;
+      if (LAYER) m = sum(e0, e1);
+      else m = make_float2(0.f, sum(e1));
+      const float m0 = -m.x * inv_d * rs, m1 = -m.y * inv_d;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (!on[j]) continue;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          d[j][u] = fmaf(rs, fmaf(y[j][u], m1, dh[j][u]), d[j][u]);
+          if (LAYER) d[j][u] += m0;
+        }
+      }
+    }
+    float e0 = 0.f, e1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (!on[j]) continue;
+      store8(a.dx, xdt, out + c[j], d[j]);
+      float w[8];
+      weights8(a.post_w, c[j], true, 1.f, w);
+      if (a.gate_is_row) {
+        float g[8];
+        from_smem<ZD>(row + zb, zdt, c[j], true, g);
+        if (a.dgate_rows) {
+          float o[8], dg[8];
+          weights8(a.post_b, c[j], true, 0.f, o);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) dg[u] = d[j][u] * sg[j][u] * fmaf(zh[j][u], w[u], o[u]);
+          store8(a.dgate_rows, zdt, out + c[j], dg);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) d[j][u] *= g[u];
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        acc[0][j][u] = fmaf(d[j][u], zh[j][u], acc[0][j][u]);
+        if (LAYER) acc[1][j][u] += d[j][u];
+        d[j][u] *= sg[j][u] * w[u];
+        if (LAYER) e0 += d[j][u];
+        e1 = fmaf(d[j][u], zh[j][u], e1);
+      }
+    }
+    float m0 = 0.f, m1 = 0.f;
+    if (a.post_w) {
+      float2 m;
+      if (LAYER) m = sum(e0, e1);
+      else m = make_float2(0.f, sum(e1));
+      m0 = -m.x * inv_d;
+      m1 = -m.y * inv_d;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (!on[j]) continue;
+      if (a.post_w) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          d[j][u] = fmaf(zh[j][u], m1, d[j][u]);
+          if (LAYER) d[j][u] += m0;
+          d[j][u] *= zr;
+        }
+      }
+      store8(a.dz, zdt, out + c[j], d[j]);
+    }
+  }
+  if (!a.part) return;
+  float* mine = a.part + (long long)blockIdx.x * kSums * a.D;
+  if (a.per == 1) {
+#pragma unroll
+    for (int k = 0; k < kSums; ++k)
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (on[j]) store8(mine, SB_F32, (long long)k * a.D + c[j], acc[k][j]);
+    return;
+  }
+  // the CTA's warps one after the other, over the rings (every copy has been waited for)
+  float* fold = reinterpret_cast<float*>(rows_smem);
+  const int width = a.tpr * 8 * NV;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kSums; ++k)
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) fold[(sub * kSums + k) * width + c[j] + u] = acc[k][j][u];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kSums * a.D; i += blockDim.x) {
+    const int k = i / a.D, col = i - k * a.D;
+    float s = 0.f;
+    for (int q = 0; q < a.per; ++q) s += fold[(q * kSums + k) * width + col];
+    mine[i] = s;
+  }
+}
+
+// ---------------------------------------------------------------- any alignment, any D
+template <int NV, int MAXT>
+__global__ void __launch_bounds__(MAXT) gated_norm_any_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float2 buf[64];
+  const int xdt = a.xdt, zdt = a.zdt;
   RowSum sum{buf, a.tpr >> 5, 0};
   const int sub = a.per > 1 ? threadIdx.x >> 5 : 0;
   const Cols<NV> cols{(int)(a.per > 1 ? threadIdx.x & 31 : threadIdx.x) * 8, a.tpr * 8, a.D};
@@ -171,9 +600,9 @@ __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant_
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = cols.at(j), m = ok ? cols.n(j) : 0;
-      rx[j] = fetch<VEC>(a.x.p, xdt, xo + c, m);
-      rz[j] = fetch<VEC>(a.z.p, zdt, zo + c, m);
-      if (a.gate.p) rg[j] = fetch<VEC>(a.gate.p, zdt, go + c, m);
+      rx[j] = load_raw8_tail(a.x.p, xdt, xo + c, m);
+      rz[j] = load_raw8_tail(a.z.p, zdt, zo + c, m);
+      if (a.gate.p) rg[j] = load_raw8_tail(a.gate.p, zdt, go + c, m);
     }
   };
   load(r < a.rows, b, t);
@@ -204,16 +633,16 @@ __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant_
     for (int j = 0; j < NV; ++j) {
       const int c = cols.at(j), n = cols.n(j);
       float s[8], w[8], o[8];
-      columns<VEC>(a.scale, c, n, 1.f, s);
+      columns(a.scale, c, n, 1.f, s);
       if (a.post_w) {
-        columns<VEC>(a.post_w, c, n, 1.f, w);
-        columns<VEC>(a.post_b, c, n, 0.f, o);
+        columns(a.post_w, c, n, 1.f, w);
+        columns(a.post_b, c, n, 0.f, o);
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[j][u] = fmaf((v[j][u] - mean) * rs, w[u], o[u]);
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u) y[j][u] = u < n ? fmaf(s[u] * g[j][u], v[j][u], y[j][u]) : 0.f;
-      put<VEC>(a.y, xdt, b * a.y_img + t * a.y_row + c, y[j], n);
+      store8_tail(a.y, xdt, b * a.y_img + t * a.y_row + c, y[j], n);
     }
     if (a.h) {
       stats_of(y, cols, a.layer, inv_d, a.eps, sum, mean, rs);
@@ -221,11 +650,11 @@ __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant_
       for (int j = 0; j < NV; ++j) {
         const int c = cols.at(j), n = cols.n(j);
         float w[8], o[8];
-        columns<VEC>(a.pre_w, c, n, 1.f, w);
-        columns<VEC>(a.pre_b, c, n, 0.f, o);
+        columns(a.pre_w, c, n, 1.f, w);
+        columns(a.pre_b, c, n, 0.f, o);
 #pragma unroll
         for (int u = 0; u < 8; ++u) y[j][u] = fmaf((y[j][u] - mean) * rs, w[u], o[u]);
-        put<VEC>(a.h, zdt, b * a.h_img + t * a.h_row + c, y[j], n);
+        store8_tail(a.h, zdt, b * a.h_img + t * a.h_row + c, y[j], n);
       }
     }
     b = nb;
@@ -233,11 +662,11 @@ __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant_
   }
 }
 
-template <int XD, int ZD, bool VEC, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_constant__ NormArgs a) {
+template <int NV, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) gated_norm_back_any_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float2 buf[64];
   extern __shared__ float fold[];  // [per][kSums][D padded]: several rows' warps meet here
-  const int xdt = XD < 0 ? a.xdt : XD, zdt = ZD < 0 ? a.zdt : ZD;
+  const int xdt = a.xdt, zdt = a.zdt;
   RowSum sum{buf, a.tpr >> 5, 0};
   const int sub = a.per > 1 ? threadIdx.x >> 5 : 0;
   const Cols<NV> cols{(int)(a.per > 1 ? threadIdx.x & 31 : threadIdx.x) * 8, a.tpr * 8, a.D};
@@ -260,13 +689,13 @@ __global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_c
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = cols.at(j), m = ok ? cols.n(j) : 0;
-      rz[j] = fetch<VEC>(a.z.p, zdt, bb * a.z.img + tt * a.z.row + c, m);
-      rdy[j] = fetch<VEC>(a.dy.p, xdt, bb * a.dy.img + tt * a.dy.row + c, a.dy.p ? m : 0);
+      rz[j] = load_raw8_tail(a.z.p, zdt, bb * a.z.img + tt * a.z.row + c, m);
+      rdy[j] = load_raw8_tail(a.dy.p, xdt, bb * a.dy.img + tt * a.dy.row + c, a.dy.p ? m : 0);
       if (a.dh.p) {
-        rx[j] = fetch<VEC>(a.x.p, xdt, bb * a.x.img + tt * a.x.row + c, m);
-        rdh[j] = fetch<VEC>(a.dh.p, zdt, bb * a.dh.img + tt * a.dh.row + c, m);
+        rx[j] = load_raw8_tail(a.x.p, xdt, bb * a.x.img + tt * a.x.row + c, m);
+        rdh[j] = load_raw8_tail(a.dh.p, zdt, bb * a.dh.img + tt * a.dh.row + c, m);
       }
-      if (a.gate.p) rg[j] = fetch<VEC>(a.gate.p, zdt, bb * a.gate.img + tt * a.gate.row + c, m);
+      if (a.gate.p) rg[j] = load_raw8_tail(a.gate.p, zdt, bb * a.gate.img + tt * a.gate.row + c, m);
     }
   };
   load(r < last, b, t);
@@ -312,9 +741,9 @@ __global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_c
       for (int j = 0; j < NV; ++j) {
         const int c = cols.at(j), n = cols.n(j);
         float s[8], w[8], o[8];
-        columns<VEC>(a.scale, c, n, 1.f, s);
-        columns<VEC>(a.post_w, c, n, 1.f, w);
-        columns<VEC>(a.post_b, c, n, 0.f, o);
+        columns(a.scale, c, n, 1.f, s);
+        columns(a.post_w, c, n, 1.f, w);
+        columns(a.post_b, c, n, 0.f, o);
 #pragma unroll
         for (int u = 0; u < 8; ++u)
           y[j][u] = u < n ? fmaf(s[u] * g[j][u], fmaf(zh[j][u], w[u], o[u]), y[j][u]) : 0.f;
@@ -324,7 +753,7 @@ __global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_c
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         float w[8];
-        columns<VEC>(a.pre_w, cols.at(j), cols.n(j), 1.f, w);
+        columns(a.pre_w, cols.at(j), cols.n(j), 1.f, w);
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
           y[j][u] = u < cols.n(j) ? (y[j][u] - mean) * rs : 0.f;
@@ -346,16 +775,16 @@ __global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_c
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = cols.at(j), n = cols.n(j);
-      put<VEC>(a.dx, xdt, r * a.D + c, d[j], n);
+      store8_tail(a.dx, xdt, r * a.D + c, d[j], n);
       float s[8], w[8];
-      columns<VEC>(a.scale, c, n, 1.f, s);
-      columns<VEC>(a.post_w, c, n, 1.f, w);
+      columns(a.scale, c, n, 1.f, s);
+      columns(a.post_w, c, n, 1.f, w);
       if (a.dgate_rows) {
         float o[8], dg[8];
-        columns<VEC>(a.post_b, c, n, 0.f, o);
+        columns(a.post_b, c, n, 0.f, o);
 #pragma unroll
         for (int u = 0; u < 8; ++u) dg[u] = d[j][u] * s[u] * fmaf(zh[j][u], w[u], o[u]);
-        put<VEC>(a.dgate_rows, zdt, r * a.D + c, dg, n);
+        store8_tail(a.dgate_rows, zdt, r * a.D + c, dg, n);
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
@@ -379,7 +808,7 @@ __global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_c
 #pragma unroll
         for (int u = 0; u < 8; ++u) d[j][u] = zr * (d[j][u] - zh[j][u] * m1 - m0);
       }
-      put<VEC>(a.dz, zdt, r * a.D + cols.at(j), d[j], cols.n(j));
+      store8_tail(a.dz, zdt, r * a.D + cols.at(j), d[j], cols.n(j));
     }
   }
   if (!a.part) return;
@@ -388,7 +817,7 @@ __global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_c
 #pragma unroll
     for (int k = 0; k < kSums; ++k)
 #pragma unroll
-      for (int j = 0; j < NV; ++j) put<VEC>(mine, SB_F32, (long long)k * a.D + cols.at(j), acc[k][j], cols.n(j));
+      for (int j = 0; j < NV; ++j) store8_tail(mine, SB_F32, (long long)k * a.D + cols.at(j), acc[k][j], cols.n(j));
     return;
   }
   // the CTA's warps one after the other
@@ -475,8 +904,7 @@ int sm_count() {
 }
 
 // Up to 256 channels a warp takes a row with one vector a lane, eight (backward: four) rows a CTA;
-// above, a CTA takes a row: two vectors a thread forward and, with its column sums in registers, one
-// backward up to 2048 channels and two above.
+// above, a CTA takes a row with two vectors a thread.
 struct Plan {
   int kind;  // of the launch tables
   int tpr, per, threads;
@@ -486,13 +914,9 @@ Plan plan_of(int D, bool back) {
   const int vecs = (D + 7) / 8;
   if (vecs <= 32) {
     p = {0, 32, back ? 4 : 8, 0};
-  } else if (!back) {
-    p.tpr = ((vecs + 1) / 2 + 31) / 32 * 32;
-    p.kind = p.tpr <= 128 ? 1 : 2;
-    p.per = 1;
   } else {
-    p.kind = vecs <= 256 ? 1 : 2;
-    p.tpr = (p.kind == 1 ? vecs + 31 : (vecs + 1) / 2 + 31) / 32 * 32;
+    p.tpr = ((vecs + 1) / 2 + 31) / 32 * 32;
+    p.kind = p.tpr <= 128 ? 1 : p.tpr <= 256 ? 2 : 3;
     p.per = 1;
   }
   p.threads = p.tpr * p.per;
@@ -501,29 +925,55 @@ Plan plan_of(int D, bool back) {
 
 using NormKernel = void (*)(const NormArgs);
 
-template <int XD, int ZD, bool VEC>
-NormKernel norm_kernel(int kind) {
-  return kind == 0 ? gated_norm_kernel<XD, ZD, VEC, 1, 256> : kind == 1 ? gated_norm_kernel<XD, ZD, VEC, 2, 128>
-                                                                        : gated_norm_kernel<XD, ZD, VEC, 2, 512>;
+template <int XD, int ZD, bool LAYER>
+NormKernel ring_kernel(bool back, int kind) {
+  if (kind == 0) return back ? gated_norm_back_kernel<XD, ZD, LAYER, 1, 128> : gated_norm_kernel<XD, ZD, LAYER, 1, 256>;
+  if (kind == 1) return back ? gated_norm_back_kernel<XD, ZD, LAYER, 2, 128> : gated_norm_kernel<XD, ZD, LAYER, 2, 128>;
+  if (kind == 2) return back ? gated_norm_back_kernel<XD, ZD, LAYER, 2, 256> : gated_norm_kernel<XD, ZD, LAYER, 2, 256>;
+  return back ? gated_norm_back_kernel<-1, -1, LAYER, 2, 512> : gated_norm_kernel<-1, -1, LAYER, 2, 512>;
 }
-template <int XD, int ZD, bool VEC>
-NormKernel back_kernel(int kind) {
-  return kind == 0 ? gated_norm_back_kernel<XD, ZD, VEC, 1, 128> : kind == 1 ? gated_norm_back_kernel<XD, ZD, VEC, 1, 256>
-                                                                             : gated_norm_back_kernel<XD, ZD, VEC, 2, 512>;
+template <int XD, int ZD>
+NormKernel ring_kernel(bool back, int kind, bool layer) {
+  return layer ? ring_kernel<XD, ZD, true>(back, kind) : ring_kernel<XD, ZD, false>(back, kind);
 }
-NormKernel pick(bool back, int xdt, int zdt, bool vec, int kind) {
-#define SB_PICK(X, Z, V) (back ? back_kernel<X, Z, V>(kind) : norm_kernel<X, Z, V>(kind))
-  if (!vec) return SB_PICK(-1, -1, false);
-  if (xdt == SB_F32 && zdt == SB_F16) return SB_PICK(SB_F32, SB_F16, true);
-  if (xdt == SB_F32 && zdt == SB_BF16) return SB_PICK(SB_F32, SB_BF16, true);
-  if (xdt == SB_F16 && zdt == SB_F16) return SB_PICK(SB_F16, SB_F16, true);
-  if (xdt == SB_BF16 && zdt == SB_BF16) return SB_PICK(SB_BF16, SB_BF16, true);
-  return SB_PICK(-1, -1, true);
-#undef SB_PICK
+NormKernel pick(bool back, int xdt, int zdt, bool vec, int kind, bool layer) {
+  if (!vec) {
+    if (kind == 0) return back ? gated_norm_back_any_kernel<1, 128> : gated_norm_any_kernel<1, 256>;
+    if (kind <= 2) return back ? gated_norm_back_any_kernel<2, 256> : gated_norm_any_kernel<2, 256>;
+    return back ? gated_norm_back_any_kernel<2, 512> : gated_norm_any_kernel<2, 512>;
+  }
+  if (xdt == SB_F32 && zdt == SB_F16) return ring_kernel<SB_F32, SB_F16>(back, kind, layer);
+  if (xdt == SB_F32 && zdt == SB_BF16) return ring_kernel<SB_F32, SB_BF16>(back, kind, layer);
+  if (xdt == SB_F16 && zdt == SB_F16) return ring_kernel<SB_F16, SB_F16>(back, kind, layer);
+  if (xdt == SB_BF16 && zdt == SB_BF16) return ring_kernel<SB_BF16, SB_BF16>(back, kind, layer);
+  return ring_kernel<-1, -1>(back, kind, layer);
+}
+
+// The ring of each team (as many rows as kRing bytes a CTA hold, two to eight) and a CTA's shared
+// memory, which the backward kernels' last sums share.
+constexpr int kRing = 46 * 1024;
+int ring_of(NormArgs& a, const Plan& p, bool back, bool& vec) {
+  const int xs = dtype_bytes(a.xdt), zs = dtype_bytes(a.zdt);
+  a.stage_bytes = a.D * (zs + (a.gate_is_row ? zs : 0));
+  if (back) a.stage_bytes += a.D * ((a.dh.p ? xs + zs : 0) + (a.dy.p ? xs : 0));
+  else a.stage_bytes += a.D * xs;
+  a.stages = std::max(2, std::min(kMaxStages, kRing / (p.per * a.stage_bytes)));
+  vec = vec && 2 * p.per * a.stage_bytes <= 200 * 1024;  // else the widest fp32 rows: no room for two
+  const int ring = vec ? p.per * a.stages * a.stage_bytes : 0;
+  const int fold = back && p.per > 1 ? p.per * kSums * p.tpr * 8 * 4 : 0;
+  return std::max(ring, fold);
+}
+cudaError_t launch_norm(NormKernel kernel, unsigned grid, int threads, int smem, const NormArgs& a, cudaStream_t st) {
+  if (smem > 46 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
+  kernel<<<grid, threads, smem, st>>>(a);
+  return cudaGetLastError();
 }
 
 // CTAs a group of rows: about `kBackCtas` a SM over all groups, at least eight rows a warp or CTA
-constexpr int kBackCtas = 3;
+constexpr int kBackCtas = 4, kNormCtas = 4;
 int chunks_of(int groups, long long group_rows, const Plan& p, int sms) {
   const long long want = std::max(1, kBackCtas * sms / groups);
   return (int)std::max(1ll, std::min(want, (group_rows + 8 * p.per - 1) / (8 * p.per)));
@@ -536,6 +986,13 @@ bool rows_aligned(const void* p, int dt, long long row, long long img) {
 bool cols_aligned(const float* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
+
+int gnorm_error(int clear, int* flags) {
+  const int zero = 0;
+  if (cudaMemcpyFromSymbol(flags, g_gnorm_error, sizeof(int)) != cudaSuccess) return -1;
+  return clear && cudaMemcpyToSymbol(g_gnorm_error, &zero, sizeof(int)) != cudaSuccess ? -1 : 0;
+}
+
 }  // namespace sb
 
 using namespace sb;
@@ -561,23 +1018,22 @@ extern "C" int sb_gated_norm(const void* x, long long x_row, long long x_img, in
   a.rows = (long long)B * T;
   a.y = y; a.y_row = y_row; a.y_img = y_img;
   a.h = h; a.h_row = h_row; a.h_img = h_img;
-  const bool vec = D % 8 == 0 && rows_aligned(x, x_dtype, x_row, x_img) && rows_aligned(z, z_dtype, z_row, z_img) &&
+  bool vec = D % 8 == 0 && rows_aligned(x, x_dtype, x_row, x_img) && rows_aligned(z, z_dtype, z_row, z_img) &&
                    (!gate || rows_aligned(gate, z_dtype, gate_row, gate_img)) &&
                    rows_aligned(y, x_dtype, y_row, y_img) && (!h || rows_aligned(h, z_dtype, h_row, h_img)) &&
                    cols_aligned(scale) && cols_aligned(post_w) && cols_aligned(post_b) && cols_aligned(pre_w) &&
                    cols_aligned(pre_b);
   const int sms = sm_count();
   if (sms == 0) return record_error(SB_ECUDA, "sb_gated_norm: device");
-  const NormKernel kernel = pick(false, x_dtype, z_dtype, vec, p.kind);
-  int ctas = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, p.threads, 0) != cudaSuccess || ctas < 1)
-    return record_error(SB_ECUDA, "sb_gated_norm: occupancy");
-  const long long grid = std::min((a.rows + p.per - 1) / p.per, (long long)sms * ctas);
+  a.gate_is_row = gate && gate_row != 0;
+  const int smem = ring_of(a, p, false, vec);
+  const NormKernel kernel = pick(false, x_dtype, z_dtype, vec, p.kind, layer != 0);
+  const long long grid = std::min((a.rows + p.per - 1) / p.per, (long long)sms * kNormCtas);
   const long long step = grid * p.per;
   a.step_b = step / T;
   a.step_t = (int)(step % T);
-  kernel<<<(unsigned)grid, p.threads, 0, (cudaStream_t)stream>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  a.team_rows = (a.rows + step - 1) / step;
+  const cudaError_t e = launch_norm(kernel, (unsigned)grid, p.threads, smem, a, (cudaStream_t)stream);
   if (e != cudaSuccess) return record_error(SB_ECUDA, cudaGetErrorString(e));
   return SB_OK;
 }
@@ -637,18 +1093,20 @@ extern "C" int sb_gated_norm_backward(const void* dy, long long dy_row, long lon
       return record_error(SB_EINVAL, "sb_gated_norm_backward: workspace (sb_gated_norm_work bytes, 16-byte aligned)");
     a.part = static_cast<float*>(work);
   }
-  const bool vec = D % 8 == 0 && rows_aligned(x, x_dtype, x_row, x_img) && rows_aligned(z, z_dtype, z_row, z_img) &&
+  bool vec = D % 8 == 0 && rows_aligned(x, x_dtype, x_row, x_img) && rows_aligned(z, z_dtype, z_row, z_img) &&
                    (!gate || rows_aligned(gate, z_dtype, gate_row, gate_img)) &&
                    (!dy || rows_aligned(dy, x_dtype, dy_row, dy_img)) &&
                    (!dh || rows_aligned(dh, z_dtype, dh_row, dh_img)) && rows_aligned(dx, x_dtype, 0, 0) &&
                    rows_aligned(dz, z_dtype, 0, 0) && (dgate_mode != 3 || rows_aligned(dgate, z_dtype, 0, 0)) &&
                    cols_aligned(scale) && cols_aligned(post_w) && cols_aligned(post_b) && cols_aligned(pre_w) &&
                    cols_aligned(pre_b);
-  const NormKernel kernel = pick(true, x_dtype, z_dtype, vec, p.kind);
-  const int smem = sums && p.per > 1 ? p.per * kSums * p.tpr * 8 * 4 : 0;
+  const int smem = ring_of(a, p, true, vec);
+  const NormKernel kernel = pick(true, x_dtype, z_dtype, vec, p.kind, layer != 0);
+  a.step_b = p.per / T;
+  a.step_t = p.per % T;
   if ((long long)groups * a.chunks > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_gated_norm_backward: too many items");
-  kernel<<<(unsigned)(groups * a.chunks), p.threads, smem, (cudaStream_t)stream>>>(a);
-  if (sums) {
+  cudaError_t e = launch_norm(kernel, (unsigned)(groups * a.chunks), p.threads, smem, a, (cudaStream_t)stream);
+  if (e == cudaSuccess && sums) {
     FoldArgs f{};
     f.part = a.part;
     f.groups = groups; f.chunks = a.chunks; f.D = D; f.gate_mode = dgate_mode;
@@ -657,8 +1115,8 @@ extern "C" int sb_gated_norm_backward(const void* dy, long long dy_row, long lon
     f.dscale = dscale; f.dgate = static_cast<float*>(dgate);
     f.dpost_w = dpost_w; f.dpost_b = dpost_b; f.dpre_w = dpre_w; f.dpre_b = dpre_b;
     gated_norm_fold_kernel<<<(unsigned)((D + 31) / 32), 512, 0, (cudaStream_t)stream>>>(f);
+    e = cudaGetLastError();
   }
-  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return record_error(SB_ECUDA, cudaGetErrorString(e));
   return SB_OK;
 }

@@ -108,4 +108,13 @@ SB_DEV void store8_tail(void* p, int dt, long long i, const float (&v)[8], int n
     if (u < n) put_one(p, dt, i + u, v[u]);
 }
 
+// A bounded wait for an mbarrier's phase that no flag cuts short; false when it ran out.
+SB_DEV bool bounded_wait(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (global_ns() - t0 > SB_WAIT_NS) return false;
+  return true;
+}
+
 }  // namespace sb

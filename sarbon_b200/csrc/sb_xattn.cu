@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
                       item);
       }
       if (*abort_flag)
-        for (int i = max(0, p - ST); i < p; ++i) drain_wait(&full[i % ST], (i / ST) & 1);
+        for (int i = max(0, p - ST); i < p; ++i) bounded_wait(&full[i % ST], (i / ST) & 1);
     }
   } else if (warp == NT * 4) {
     if (lane == 0 && n > 0) {  // MMA
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
       if (!ok) {
         give_up(SB_ERR_TIMEOUT_FULL);
         mma_commit(dbar);
-        drain_wait(dbar, 0);
+        bounded_wait(dbar, 0);
       }
     }
   } else if (warp == NT * 4 + 2) {

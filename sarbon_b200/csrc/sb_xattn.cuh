@@ -130,13 +130,6 @@ SB_DEV uint32_t pack16(float lo, float hi) {
   return pack_pair(lo, hi, BF16 ? SB_BF16 : SB_F16);
 }
 
-// A wait that no abort flag cuts short: for copies in flight before a CTA gives up.
-SB_DEV void drain_wait(uint64_t* bar, uint32_t parity) {
-  const uint64_t t0 = global_ns();
-  while (!mbar_try_wait(bar, parity))
-    if (global_ns() - t0 > SB_WAIT_NS) return;
-}
-
 // ---------------------------------------------------------------- host
 // One [B][T][heads * dh] operand as a 4-D tensor map; its box is `rows` rows of one head of one item, and rows past T arrive as zeros.  img = 0 (one memory for
 // every item) makes the item dimension 1: kernels multiply the item by 0 then.
@@ -147,6 +140,7 @@ bool xattn_view_ok(const void* p, long long row, long long img);
 // Sticky SB_ERR_* flags of the attention kernels, cleared on request.
 int xattn_error(int clear, int* flags);  // 0, or -1 when the device could not be read
 int xattn_back_error(int clear, int* flags);
+int gnorm_error(int clear, int* flags);  // of the gated norms
 long long xattn_back_work(int B, int H, int Hkv, int dh, int Tq, int Tk, int sms);
 // SMs of the current device, 0 on error
 int xattn_sms();

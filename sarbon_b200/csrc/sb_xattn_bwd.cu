@@ -212,8 +212,8 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
         }
       }
       if (*abort_flag) {
-        for (int i = max(0, p - ST); i < p; ++i) drain_wait(&full[i % ST], (i / ST) & 1);
-        if (SIDE == 1) drain_wait(x_full, 0);
+        for (int i = max(0, p - ST); i < p; ++i) bounded_wait(&full[i % ST], (i / ST) & 1);
+        if (SIDE == 1) bounded_wait(x_full, 0);
       }
     }
   } else if (warp == 8) {
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
       } else {
         give_up(SB_ERR_TIMEOUT_FULL);
         mma_commit(dbar);
-        drain_wait(dbar, 0);
+        bounded_wait(dbar, 0);
       }
     }
   } else if (warp == 10) {
