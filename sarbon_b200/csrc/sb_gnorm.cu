@@ -55,14 +55,16 @@ struct NormArgs {
   float* part;                 // [groups * chunks][kSums][D]
   long long group_rows;        // rows that share their column sums (T for an image's gate, B * T else)
   int chunks, gate_is_row;     // CTAs a group
-  int stages, stage_bytes;     // rows in a team's ring, bytes of one
+  int stages, stage_bytes;     // of a team's ring
+  int row_bytes, copy_bytes;   // room of a row in it, what is copied of one
+  int pitch;                   // columns that a row has room for
   long long team_rows;         // forward: rows of a team
 };
 
 // Sum of a pair of values over the threads of a row; the two halves of the buffer alternate, so one
 // barrier a reduction is enough.
 struct RowSum {
-  float2* buf;  // [2][32]
+  float2* buf;  // [2][32], with four sums at once [2][16] of them
   int warps, half;
   SB_DEV float2 operator()(float a, float b) {
 #pragma unroll
@@ -157,6 +159,10 @@ SB_DEV void weights8(const float* w, int c, bool on, float other, float (&v)[8])
   }
 }
 template <int DT>
+SB_DEV void from_smem(const uint8_t* row, int dt, int c, float (&v)[8]) {
+  unpack8(load_raw8(row, DT < 0 ? dt : DT, c), DT < 0 ? dt : DT, v);
+}
+template <int DT>
 SB_DEV void from_smem(const uint8_t* row, int dt, int c, bool on, float (&v)[8]) {
   if (on) {
     unpack8(load_raw8(row, DT < 0 ? dt : DT, c), DT < 0 ? dt : DT, v);
@@ -165,31 +171,87 @@ SB_DEV void from_smem(const uint8_t* row, int dt, int c, bool on, float (&v)[8])
     for (int u = 0; u < 8; ++u) v[u] = 0.f;
   }
 }
-// 1 / deviation r and -mean r of a row, so that its hats are v r + shift; `on[j]`: vector j exists
-// (the others hold zeros)
-template <bool LAYER, int NV>
-SB_DEV void stats8(const float (&v)[NV][8], const bool (&on)[NV], float inv_d, float eps, RowSum& sum, float& r,
-                   float& shift) {
-  float mean = 0.f, q = 0.f;
-  if (LAYER) {
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int u = 0; u < 8; ++u) s += v[j][u];
-    mean = sum(s) * inv_d;
+// Sums of K = 1, 2 or 4 values over a team, in every thread.  A warp halves the values with its lanes
+// (each half of the lanes goes on with half of the values), so K values take 5 or 6 shuffles, not 5 K.
+template <int K>
+SB_DEV void team_sum(float (&v)[K], RowSum& sum) {
+  static_assert(K == 1 || K == 2 || K == 4, "values");
+  const int lane = threadIdx.x & 31;
+  float x;
+  if constexpr (K == 4) {
+    const bool up = lane & 16, odd = lane & 8;
+    const float k0 = up ? v[2] : v[0], k1 = up ? v[3] : v[1], s0 = up ? v[0] : v[2], s1 = up ? v[1] : v[3];
+    const float a0 = k0 + __shfl_xor_sync(0xFFFFFFFFu, s0, 16), a1 = k1 + __shfl_xor_sync(0xFFFFFFFFu, s1, 16);
+    x = (odd ? a1 : a0) + __shfl_xor_sync(0xFFFFFFFFu, odd ? a0 : a1, 8);
+  } else if constexpr (K == 2) {
+    const bool up = lane & 16;
+    x = (up ? v[1] : v[0]) + __shfl_xor_sync(0xFFFFFFFFu, up ? v[0] : v[1], 16);
+  } else {
+    x = v[0] + __shfl_xor_sync(0xFFFFFFFFu, v[0], 16);
   }
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-    if (on[j]) {
+  for (int o = K == 4 ? 4 : 8; o; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
+  constexpr int per = 32 / K;  // lanes that hold the same value: value k in lanes k * per ..
+  if (sum.warps == 1) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float d = LAYER ? v[j][u] - mean : v[j][u];
-        q = fmaf(d, d, q);
-      }
+    for (int k = 0; k < K; ++k) v[k] = K == 1 ? x : __shfl_sync(0xFFFFFFFFu, x, k * per);
+    return;
+  }
+  float* mine = reinterpret_cast<float*>(sum.buf) + sum.half * 64;
+  sum.half ^= 1;
+  if (lane % per == 0) mine[(threadIdx.x >> 5) * K + lane / per] = x;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = 0.f;
+  for (int i = 0; i < sum.warps; ++i) {
+    if constexpr (K == 4) {
+      const float4 t = reinterpret_cast<const float4*>(mine)[i];
+      v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+    } else if constexpr (K == 2) {
+      const float2 t = reinterpret_cast<const float2*>(mine)[i];
+      v[0] += t.x; v[1] += t.y;
+    } else {
+      v[0] += mine[i];
     }
-  r = rsqrtf(sum(q) * inv_d + eps);
-  shift = LAYER ? -mean * r : 0.f;
+  }
+}
+
+// 1 / deviation r and -mean r of R rows, so that their hats are v r + shift; `on[j]`: vector j of a row
+// exists (the others hold zeros)
+template <bool LAYER, int R, int NV>
+SB_DEV void stats8(const float (&v)[R][NV][8], const bool (&on)[NV], float inv_d, float eps, RowSum& sum, float (&r)[R],
+                   float (&shift)[R]) {
+  float mean[R], q[R];
+#pragma unroll
+  for (int x = 0; x < R; ++x) mean[x] = q[x] = 0.f;
+  if (LAYER) {
+#pragma unroll
+    for (int x = 0; x < R; ++x)
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) mean[x] += v[x][j][u];
+    team_sum(mean, sum);
+#pragma unroll
+    for (int x = 0; x < R; ++x) mean[x] *= inv_d;
+  }
+#pragma unroll
+  for (int x = 0; x < R; ++x)
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (on[j]) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float d = LAYER ? v[x][j][u] - mean[x] : v[x][j][u];
+          q[x] = fmaf(d, d, q[x]);
+        }
+      }
+  team_sum(q, sum);
+#pragma unroll
+  for (int x = 0; x < R; ++x) {
+    r[x] = rsqrtf(q[x] * inv_d + eps);
+    shift[x] = LAYER ? -mean[x] * r[x] : 0.f;
+  }
 }
 
 // A team's ring of rows.  Operand o of a row lies `off[o]` bytes into its stage; an operand that is
@@ -212,25 +274,6 @@ struct Place {
 };
 constexpr int kMaxStages = 8;
 
-// The copies of row (b, t) into stage st, by the team's first thread.
-template <bool BACK>
-SB_DEV void fill(const NormArgs& a, const Ring& ring, int st, long long b, int t) {
-  uint64_t* bar = &ring.full[st];
-  uint8_t* dst = ring.base + st * ring.stage_bytes;
-  mbar_arrive_expect_tx(bar, (uint32_t)ring.stage_bytes);
-  const int xs = a.xdt == SB_F32 ? 4 : 2, zs = a.zdt == SB_F32 ? 4 : 2;
-  const uint32_t xb = a.D * xs, zb = a.D * zs;
-  auto copy = [&](const Rows& r, int size, uint32_t bytes) {
-    bulk_load(dst, static_cast<const uint8_t*>(r.p) + (b * r.img + t * r.row) * size, bytes, bar);
-    dst += bytes;
-  };
-  copy(a.z, zs, zb);
-  if (a.gate_is_row) copy(a.gate, zs, zb);
-  if (BACK ? a.dh.p != nullptr : true) copy(a.x, xs, xb);
-  if (BACK && a.dy.p) copy(a.dy, xs, xb);
-  if (BACK && a.dh.p) copy(a.dh, zs, zb);
-}
-
 // A row as (b, t); the team's rows follow each other.
 struct Walk {
   long long b;
@@ -242,6 +285,26 @@ struct Walk {
     }
   }
 };
+
+// The copies of `rows` rows from `ahead` on into stage st, by the team's first thread.
+template <bool BACK>
+SB_DEV void fill(const NormArgs& a, const Ring& ring, int st, Walk& ahead, int rows) {
+  uint64_t* bar = &ring.full[st];
+  mbar_arrive_expect_tx(bar, (uint32_t)(rows * a.copy_bytes));
+  const int xs = a.xdt == SB_F32 ? 4 : 2, zs = a.zdt == SB_F32 ? 4 : 2;
+  for (int i = 0; i < rows; ++i, ahead.next()) {
+    uint8_t* dst = ring.base + st * ring.stage_bytes + i * a.row_bytes;
+    auto copy = [&](const Rows& r, int size) {
+      bulk_load(dst, static_cast<const uint8_t*>(r.p) + (ahead.b * r.img + ahead.t * r.row) * size, a.D * size, bar);
+      dst += a.pitch * size;
+    };
+    copy(a.z, zs);
+    if (a.gate_is_row) copy(a.gate, zs);
+    if (BACK ? a.dh.p != nullptr : true) copy(a.x, xs);
+    if (BACK && a.dy.p) copy(a.dy, xs);
+    if (BACK && a.dh.p) copy(a.dh, zs);
+  }
+}
 
 __device__ int g_gnorm_error;
 
@@ -257,7 +320,7 @@ SB_DEV void give_up(const Ring& ring, Place at, int left, int me) {
 // y = x + hat A + B with A = scale gate post_w, B = scale gate post_b.
 template <int XD, int ZD, bool LAYER, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float2 buf[64];
+  __shared__ __align__(16) float2 buf[64];
   __shared__ uint64_t bars[8 * kMaxStages];
   extern __shared__ __align__(16) uint8_t rows_smem[];
   const int xdt = XD < 0 ? a.xdt : XD, zdt = ZD < 0 ? a.zdt : ZD;
@@ -286,9 +349,8 @@ __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant_
   Place here, there;
   int filled = 0;
   if (me == 0)
-    for (; filled < min(n, a.stages); ++filled, ahead.next(), there.next(ring))
-      fill<false>(a, ring, there.st, ahead.b, ahead.t);
-  const int go = a.D * (zdt == SB_F32 ? 4 : 2), xo = a.gate_is_row ? 2 * go : go;  // places in a stage: z, gate, x
+    for (; filled < min(n, a.stages); ++filled, there.next(ring)) fill<false>(a, ring, there.st, ahead, 1);
+  const int go = a.pitch * (zdt == SB_F32 ? 4 : 2), xo = a.gate_is_row ? 2 * go : go;  // places in a stage: z, gate, x
   float A[NV][8], B[NV][8];
   long long gate_of = -1;
   for (int i = 0; i < n; ++i, at.next(), here.next(ring)) {
@@ -298,9 +360,8 @@ __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant_
     }
     // the team has left row i - 1: its stage is free
     if (me == 0 && i > 0 && filled < n) {
-      fill<false>(a, ring, there.st, ahead.b, ahead.t);
+      fill<false>(a, ring, there.st, ahead, 1);
       ++filled;
-      ahead.next();
       there.next(ring);
     }
     if (at.b != gate_of) {
@@ -326,10 +387,13 @@ __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant_
       }
     }
     const uint8_t* row = ring.base + here.st * a.stage_bytes;
-    float v[NV][8], y[NV][8], r = 1.f, shift = 0.f;
+    float v1[1][NV][8], y1[1][NV][8], r1[1] = {1.f}, shift1[1] = {0.f};
+    float(&v)[NV][8] = v1[0];
+    float(&y)[NV][8] = y1[0];
+    float &r = r1[0], &shift = shift1[0];
 #pragma unroll
     for (int j = 0; j < NV; ++j) from_smem<ZD>(row, zdt, c[j], on[j], v[j]);
-    if (a.post_w) stats8<LAYER>(v, on, inv_d, a.eps, sum, r, shift);
+    if (a.post_w) stats8<LAYER>(v1, on, inv_d, a.eps, sum, r1, shift1);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       from_smem<XD>(row + xo, xdt, c[j], on[j], y[j]);
@@ -352,7 +416,7 @@ __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant_
       store8(a.y, xdt, at.b * a.y_img + at.t * a.y_row + c[j], y[j]);
     }
     if (a.h) {
-      stats8<LAYER>(y, on, inv_d, a.eps, sum, r, shift);
+      stats8<LAYER>(y1, on, inv_d, a.eps, sum, r1, shift1);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (!on[j]) continue;
@@ -365,9 +429,13 @@ __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant_
   }
 }
 
-template <int XD, int ZD, bool LAYER, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float2 buf[64];
+// R rows of a team at once: their reductions share barriers and overlap.  A row in shared memory has
+// room for all of the team's columns, zero past D, and a row past the team's last is zeroed before its
+// step, so the loop has no selects: lanes past D hold zeros in x, z, dy, dh and in scale x gate, which
+// makes every term they add zero but the squares around the mean (left out by `in`).
+template <int XD, int ZD, bool LAYER, int R, int NV, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) gated_norm_back_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ __align__(16) float2 buf[64];
   __shared__ uint64_t bars[8 * kMaxStages];
   extern __shared__ __align__(16) uint8_t rows_smem[];
   const int xdt = XD < 0 ? a.xdt : XD, zdt = ZD < 0 ? a.zdt : ZD;
@@ -376,37 +444,41 @@ __global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_c
   const int sub = a.per > 1 ? threadIdx.x >> 5 : 0, me = a.per > 1 ? threadIdx.x & 31 : threadIdx.x;
   const Ring ring{rows_smem + (size_t)sub * a.stages * a.stage_bytes, bars + sub * a.stages, a.stages, a.stage_bytes};
   const float inv_d = 1.f / (float)a.D;
-  int c[NV];
+  int c[NV], cw[NV];  // columns; of the weights (any for a lane past D)
   bool on[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     c[j] = (me + j * a.tpr) * 8;
     on[j] = c[j] < a.D;
+    cw[j] = on[j] ? c[j] : 0;
   }
   if (me == 0)
     for (int i = 0; i < a.stages; ++i) mbar_init(&ring.full[i], 1);
   fence_mbar_init();
+  for (int i = threadIdx.x; i < a.per * a.stages * a.stage_bytes / 16; i += blockDim.x)
+    reinterpret_cast<uint4*>(rows_smem)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
   __syncthreads();
   const long long group = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
   const long long each = (a.group_rows + a.chunks - 1) / a.chunks;
   const long long last = group * a.group_rows + min((chunk + 1) * each, a.group_rows);
   const long long part = (each + a.per - 1) / a.per;  // a team's rows
   const long long begin = min(group * a.group_rows + min(chunk * each, a.group_rows) + sub * part, last);
-  const int n = (int)(min(begin + part, last) - begin);
-  Walk at{begin / a.T, (int)(begin % a.T), a.T}, ahead = at;
+  const int rows = (int)(min(begin + part, last) - begin), n = (rows + R - 1) / R;
+  Walk ahead{begin / a.T, (int)(begin % a.T), a.T};
   Place here, there;
   int filled = 0;
   if (me == 0)
-    for (; filled < min(n, a.stages); ++filled, ahead.next(), there.next(ring))
-      fill<true>(a, ring, there.st, ahead.b, ahead.t);
-  // places in a stage: z, gate, x, dy, dh
-  const int zb = a.D * (zdt == SB_F32 ? 4 : 2), xb = a.D * (xdt == SB_F32 ? 4 : 2);
+    for (; filled < min(n, a.stages); ++filled, there.next(ring))
+      fill<true>(a, ring, there.st, ahead, min(R, rows - filled * R));
+  // places in a row of a stage: z, gate, x, dy, dh
+  const int zb = a.pitch * (zdt == SB_F32 ? 4 : 2), xb = a.pitch * (xdt == SB_F32 ? 4 : 2);
   const int xo = a.gate_is_row ? 2 * zb : zb, dyo = a.dh.p ? xo + xb : xo, dho = a.dy.p ? dyo + xb : dyo;
   // scale x gate of the CTA's rows (scale alone where every row has its gate)
   float sg[NV][8], acc[kSums][NV][8];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    weights8(a.scale, c[j], on[j], 1.f, sg[j]);
+    weights8(a.scale, c[j], on[j], on[j] ? 1.f : 0.f, sg[j]);
     if (a.gate.p && !a.gate_is_row && on[j]) {
       float g[8];
       unpack8(load_raw8(a.gate.p, zdt, group * a.gate.img + c[j]), zdt, g);
@@ -419,137 +491,179 @@ __global__ void __launch_bounds__(MAXT, 1) gated_norm_back_kernel(const __grid_c
       for (int u = 0; u < 8; ++u) acc[k][j][u] = 0.f;
   }
   long long out = begin * a.D;
-  for (int i = 0; i < n; ++i, out += a.D, here.next(ring)) {
+  for (int i = 0; i < n; ++i, out += R * a.D, here.next(ring)) {
     if (!team_all(bounded_wait(&ring.full[here.st], here.parity), warps)) {
       give_up(ring, here, filled - i, me);
       break;
     }
+    // the team has left step i - 1: its stage is free
     if (me == 0 && i > 0 && filled < n) {
-      fill<true>(a, ring, there.st, ahead.b, ahead.t);
+      fill<true>(a, ring, there.st, ahead, min(R, rows - filled * R));
       ++filled;
-      ahead.next();
       there.next(ring);
     }
-    const uint8_t* row = ring.base + here.st * a.stage_bytes;
-    float zh[NV][8], d[NV][8], zr = 1.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      from_smem<ZD>(row, zdt, c[j], on[j], zh[j]);
-      from_smem<XD>(row + dyo, xdt, c[j], on[j] && a.dy.p, d[j]);
+    uint8_t* row = ring.base + here.st * a.stage_bytes;
+    const bool odd = R > 1 && (i + 1) * R > rows;  // the last row of this step does not exist
+    if (odd) {
+      for (int o = 0; o < a.row_bytes; o += 16 * a.tpr)
+        if (o + 16 * me < a.row_bytes) *reinterpret_cast<uint4*>(row + a.row_bytes + o + 16 * me) = make_uint4(0, 0, 0, 0);
+      team_all(true, warps);
     }
-    if (a.post_w) {
-      float shift;
-      stats8<LAYER>(zh, on, inv_d, a.eps, sum, zr, shift);
+    float zh[R][NV][8], d[R][NV][8], zr[R], shift[R];
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (on[j]) {
-#pragma unroll
-          for (int u = 0; u < 8; ++u) zh[j][u] = LAYER ? fmaf(zh[j][u], zr, shift) : zh[j][u] * zr;
-        }
-    }
-    if (a.dh.p) {
-      float y[NV][8], dh[NV][8];
+    for (int x = 0; x < R; ++x) {
+      zr[x] = 1.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        from_smem<XD>(row + xo, xdt, c[j], on[j], y[j]);
-        if (!on[j]) continue;
-        float w[8], o[8], f[8];
-        weights8(a.post_w, c[j], true, 1.f, w);
-        if (LAYER) weights8(a.post_b, c[j], true, 0.f, o);
+        from_smem<ZD>(row + x * a.row_bytes, zdt, c[j], zh[x][j]);
+        if (a.dy.p) {
+          from_smem<XD>(row + x * a.row_bytes + dyo, xdt, c[j], d[x][j]);
+        } else {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) f[u] = sg[j][u];
-        if (a.gate_is_row) {
-          float g[8];
-          from_smem<ZD>(row + zb, zdt, c[j], true, g);
-#pragma unroll
-          for (int u = 0; u < 8; ++u) f[u] *= g[u];
+          for (int u = 0; u < 8; ++u) d[x][j][u] = 0.f;
         }
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          y[j][u] = fmaf(f[u], LAYER ? fmaf(zh[j][u], w[u], o[u]) : zh[j][u] * w[u], y[j][u]);
       }
-      float rs, shift, e0 = 0.f, e1 = 0.f;
+    }
+    if (a.post_w) {
+      stats8<LAYER>(zh, on, inv_d, a.eps, sum, zr, shift);
+      if (odd) zr[R - 1] = shift[R - 1] = 0.f;
+#pragma unroll
+      for (int x = 0; x < R; ++x)
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int u = 0; u < 8; ++u) zh[x][j][u] = LAYER ? fmaf(zh[x][j][u], zr[x], shift[x]) : zh[x][j][u] * zr[x];
+    }
+    if (a.dh.p) {
+      float y[R][NV][8], dh[R][NV][8], rs[R];
+#pragma unroll
+      for (int x = 0; x < R; ++x)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          float n8[8];  // Npost(z)
+          if (a.post_w) {
+            float w[8];
+            weights8(a.post_w, cw[j], true, 1.f, w);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) n8[u] = zh[x][j][u] * w[u];
+            if (LAYER && a.post_b) {
+              weights8(a.post_b, cw[j], true, 0.f, w);
+#pragma unroll
+              for (int u = 0; u < 8; ++u) n8[u] += w[u];
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) n8[u] = zh[x][j][u];
+          }
+          if (a.gate_is_row) {
+            float g[8];
+            from_smem<ZD>(row + x * a.row_bytes + zb, zdt, c[j], g);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) n8[u] *= g[u];
+          }
+          from_smem<XD>(row + x * a.row_bytes + xo, xdt, c[j], y[x][j]);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) y[x][j][u] = fmaf(sg[j][u], n8[u], y[x][j][u]);
+        }
       stats8<LAYER>(y, on, inv_d, a.eps, sum, rs, shift);
+      if (odd) rs[R - 1] = shift[R - 1] = 0.f;
+      float e[LAYER ? 2 * R : R];  // sums of e yhat, then (layer norm) of e
+#pragma unroll
+      for (int x = 0; x < (LAYER ? 2 * R : R); ++x) e[x] = 0.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         float w[8];
-        weights8(a.pre_w, c[j], on[j], 1.f, w);
-        from_smem<ZD>(row + dho, zdt, c[j], on[j], dh[j]);
-        if (!on[j]) continue;
+        weights8(a.pre_w, cw[j], true, 1.f, w);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          y[j][u] = LAYER ? fmaf(y[j][u], rs, shift) : y[j][u] * rs;
-          acc[2][j][u] = fmaf(dh[j][u], y[j][u], acc[2][j][u]);
-          if (LAYER) acc[3][j][u] += dh[j][u];
-          dh[j][u] *= w[u];
-          if (LAYER) e0 += dh[j][u];
-          e1 = fmaf(dh[j][u], y[j][u], e1);
+        for (int x = 0; x < R; ++x) {
+          from_smem<ZD>(row + x * a.row_bytes + dho, zdt, c[j], dh[x][j]);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            float& yy = y[x][j][u];
+            float& dd = dh[x][j][u];
+            yy = LAYER ? fmaf(yy, rs[x], shift[x]) : yy * rs[x];
+            acc[2][j][u] = fmaf(dd, yy, acc[2][j][u]);
+            if (LAYER) acc[3][j][u] += dd;
+            dd *= w[u];
+            e[x] = fmaf(dd, yy, e[x]);
+            if (LAYER) e[R + x] += dd;
+          }
         }
       }
-      float2 m;
-      if (LAYER) m = sum(e0, e1);
-      else m = make_float2(0.f, sum(e1));
-      const float m0 = -m.x * inv_d * rs, m1 = -m.y * inv_d;
+      team_sum(e, sum);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (!on[j]) continue;
+      for (int x = 0; x < R; ++x) {
+        const float m1 = -e[x] * inv_d, m0 = LAYER ? -e[R + x] * inv_d * rs[x] : 0.f;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          d[j][u] = fmaf(rs, fmaf(y[j][u], m1, dh[j][u]), d[j][u]);
-          if (LAYER) d[j][u] += m0;
-        }
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            d[x][j][u] = fmaf(rs[x], fmaf(y[x][j][u], m1, dh[x][j][u]), d[x][j][u]);
+            if (LAYER) d[x][j][u] += m0;
+          }
       }
     }
-    float e0 = 0.f, e1 = 0.f;
+    float e[LAYER ? 2 * R : R];
+#pragma unroll
+    for (int x = 0; x < (LAYER ? 2 * R : R); ++x) e[x] = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (!on[j]) continue;
-      store8(a.dx, xdt, out + c[j], d[j]);
-      float w[8];
-      weights8(a.post_w, c[j], true, 1.f, w);
-      if (a.gate_is_row) {
-        float g[8];
-        from_smem<ZD>(row + zb, zdt, c[j], true, g);
-        if (a.dgate_rows) {
-          float o[8], dg[8];
-          weights8(a.post_b, c[j], true, 0.f, o);
-#pragma unroll
-          for (int u = 0; u < 8; ++u) dg[u] = d[j][u] * sg[j][u] * fmaf(zh[j][u], w[u], o[u]);
-          store8(a.dgate_rows, zdt, out + c[j], dg);
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) d[j][u] *= g[u];
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        acc[0][j][u] = fmaf(d[j][u], zh[j][u], acc[0][j][u]);
-        if (LAYER) acc[1][j][u] += d[j][u];
-        d[j][u] *= sg[j][u] * w[u];
-        if (LAYER) e0 += d[j][u];
-        e1 = fmaf(d[j][u], zh[j][u], e1);
-      }
-    }
-    float m0 = 0.f, m1 = 0.f;
-    if (a.post_w) {
-      float2 m;
-      if (LAYER) m = sum(e0, e1);
-      else m = make_float2(0.f, sum(e1));
-      m0 = -m.x * inv_d;
-      m1 = -m.y * inv_d;
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (!on[j]) continue;
+      float w[8];  // scale x gate x post_w
       if (a.post_w) {
+        weights8(a.post_w, cw[j], true, 1.f, w);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) w[u] *= sg[j][u];
+      } else {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) w[u] = sg[j][u];
+      }
+#pragma unroll
+      for (int x = 0; x < R; ++x) {
+        const bool there_is = on[j] && !(x == R - 1 && odd);
+        if (there_is) store8(a.dx, xdt, out + x * a.D + c[j], d[x][j]);
+        if (a.gate_is_row) {
+          float g[8];
+          from_smem<ZD>(row + x * a.row_bytes + zb, zdt, c[j], g);
+          if (a.dgate_rows && there_is) {
+            float o[8], dg[8];
+            weights8(LAYER ? a.post_b : nullptr, c[j], true, 0.f, o);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) dg[u] = d[x][j][u] * fmaf(zh[x][j][u], w[u], sg[j][u] * o[u]);
+            store8(a.dgate_rows, zdt, out + x * a.D + c[j], dg);
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) d[x][j][u] *= g[u];
+        }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          d[j][u] = fmaf(zh[j][u], m1, d[j][u]);
-          if (LAYER) d[j][u] += m0;
-          d[j][u] *= zr;
+          float& dd = d[x][j][u];
+          acc[0][j][u] = fmaf(dd, zh[x][j][u], acc[0][j][u]);
+          if (LAYER) acc[1][j][u] += dd;
+          dd *= w[u];
+          e[x] = fmaf(dd, zh[x][j][u], e[x]);
+          if (LAYER) e[R + x] += dd;
         }
       }
-      store8(a.dz, zdt, out + c[j], d[j]);
     }
+    if (a.post_w) {
+      team_sum(e, sum);
+#pragma unroll
+      for (int x = 0; x < R; ++x) {
+        const float m1 = -e[x] * inv_d * zr[x], m0 = LAYER ? -e[R + x] * inv_d * zr[x] : 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const float t = LAYER ? fmaf(zh[x][j][u], m1, m0) : zh[x][j][u] * m1;
+            d[x][j][u] = fmaf(d[x][j][u], zr[x], t);
+          }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < R; ++x)
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (on[j] && !(x == R - 1 && odd)) store8(a.dz, zdt, out + x * a.D + c[j], d[x][j]);
   }
   if (!a.part) return;
   float* mine = a.part + (long long)blockIdx.x * kSums * a.D;
@@ -903,21 +1017,30 @@ int sm_count() {
   return n;
 }
 
-// Up to 256 channels a warp takes a row with one vector a lane, eight (backward: four) rows a CTA;
-// above, a CTA takes a row with two vectors a thread.
+// Up to 256 channels a warp takes a row with one vector a lane, eight (backward: four) teams a CTA;
+// above, a CTA is a team: forward with two vectors a thread, backward with two rows of one vector
+// (twice the independent work of a row, half the registers that two vectors' column sums take) up to
+// 2048 channels, and one row of two vectors above.
 struct Plan {
   int kind;  // of the launch tables
-  int tpr, per, threads;
+  int tpr, per, threads, at_once;
 };
 Plan plan_of(int D, bool back) {
   Plan p;
   const int vecs = (D + 7) / 8;
+  p.at_once = back && vecs <= 256 ? 2 : 1;
+  p.per = 1;
   if (vecs <= 32) {
-    p = {0, 32, back ? 4 : 8, 0};
+    p.kind = 0;
+    p.tpr = 32;
+    p.per = back ? 4 : 8;
+  } else if (p.at_once == 2) {
+    p.tpr = (vecs + 31) / 32 * 32;
+    p.kind = p.tpr <= 128 ? 1 : 2;
   } else {
     p.tpr = ((vecs + 1) / 2 + 31) / 32 * 32;
     p.kind = p.tpr <= 128 ? 1 : p.tpr <= 256 ? 2 : 3;
-    p.per = 1;
+    if (back) p.kind += 1;  // 3, 4
   }
   p.threads = p.tpr * p.per;
   return p;
@@ -927,10 +1050,15 @@ using NormKernel = void (*)(const NormArgs);
 
 template <int XD, int ZD, bool LAYER>
 NormKernel ring_kernel(bool back, int kind) {
-  if (kind == 0) return back ? gated_norm_back_kernel<XD, ZD, LAYER, 1, 128> : gated_norm_kernel<XD, ZD, LAYER, 1, 256>;
-  if (kind == 1) return back ? gated_norm_back_kernel<XD, ZD, LAYER, 2, 128> : gated_norm_kernel<XD, ZD, LAYER, 2, 128>;
-  if (kind == 2) return back ? gated_norm_back_kernel<XD, ZD, LAYER, 2, 256> : gated_norm_kernel<XD, ZD, LAYER, 2, 256>;
-  return back ? gated_norm_back_kernel<-1, -1, LAYER, 2, 512> : gated_norm_kernel<-1, -1, LAYER, 2, 512>;
+  if (back) {
+    if (kind == 0) return gated_norm_back_kernel<XD, ZD, LAYER, 2, 1, 128>;
+    if (kind == 1) return gated_norm_back_kernel<XD, ZD, LAYER, 2, 1, 128>;
+    if (kind == 2) return gated_norm_back_kernel<XD, ZD, LAYER, 2, 1, 256>;
+    return kind == 3 ? gated_norm_back_kernel<-1, -1, LAYER, 1, 2, 256> : gated_norm_back_kernel<-1, -1, LAYER, 1, 2, 512>;
+  }
+  if (kind == 0) return gated_norm_kernel<XD, ZD, LAYER, 1, 256>;
+  if (kind == 1) return gated_norm_kernel<XD, ZD, LAYER, 2, 128>;
+  return kind == 2 ? gated_norm_kernel<XD, ZD, LAYER, 2, 256> : gated_norm_kernel<-1, -1, LAYER, 2, 512>;
 }
 template <int XD, int ZD>
 NormKernel ring_kernel(bool back, int kind, bool layer) {
@@ -938,9 +1066,8 @@ NormKernel ring_kernel(bool back, int kind, bool layer) {
 }
 NormKernel pick(bool back, int xdt, int zdt, bool vec, int kind, bool layer) {
   if (!vec) {
-    if (kind == 0) return back ? gated_norm_back_any_kernel<1, 128> : gated_norm_any_kernel<1, 256>;
-    if (kind <= 2) return back ? gated_norm_back_any_kernel<2, 256> : gated_norm_any_kernel<2, 256>;
-    return back ? gated_norm_back_any_kernel<2, 512> : gated_norm_any_kernel<2, 512>;
+    if (back) return kind <= 2 ? gated_norm_back_any_kernel<1, 256> : gated_norm_back_any_kernel<2, 512>;
+    return kind == 0 ? gated_norm_any_kernel<1, 256> : gated_norm_any_kernel<2, 512>;
   }
   if (xdt == SB_F32 && zdt == SB_F16) return ring_kernel<SB_F32, SB_F16>(back, kind, layer);
   if (xdt == SB_F32 && zdt == SB_BF16) return ring_kernel<SB_F32, SB_BF16>(back, kind, layer);
@@ -954,9 +1081,11 @@ NormKernel pick(bool back, int xdt, int zdt, bool vec, int kind, bool layer) {
 constexpr int kRing = 46 * 1024;
 int ring_of(NormArgs& a, const Plan& p, bool back, bool& vec) {
   const int xs = dtype_bytes(a.xdt), zs = dtype_bytes(a.zdt);
-  a.stage_bytes = a.D * (zs + (a.gate_is_row ? zs : 0));
-  if (back) a.stage_bytes += a.D * ((a.dh.p ? xs + zs : 0) + (a.dy.p ? xs : 0));
-  else a.stage_bytes += a.D * xs;
+  a.pitch = back ? p.tpr * 8 * (p.at_once == 2 || p.kind == 0 ? 1 : 2) : a.D;
+  const int elem = zs + (a.gate_is_row ? zs : 0) + (back ? (a.dh.p ? xs + zs : 0) + (a.dy.p ? xs : 0) : xs);
+  a.copy_bytes = a.D * elem;
+  a.row_bytes = a.pitch * elem;
+  a.stage_bytes = a.row_bytes * p.at_once;
   a.stages = std::max(2, std::min(kMaxStages, kRing / (p.per * a.stage_bytes)));
   vec = vec && 2 * p.per * a.stage_bytes <= 200 * 1024;  // else the widest fp32 rows: no room for two
   const int ring = vec ? p.per * a.stages * a.stage_bytes : 0;
@@ -973,7 +1102,7 @@ cudaError_t launch_norm(NormKernel kernel, unsigned grid, int threads, int smem,
 }
 
 // CTAs a group of rows: about `kBackCtas` a SM over all groups, at least eight rows a warp or CTA
-constexpr int kBackCtas = 4, kNormCtas = 4;
+constexpr int kBackCtas = 3, kNormCtas = 4;
 int chunks_of(int groups, long long group_rows, const Plan& p, int sms) {
   const long long want = std::max(1, kBackCtas * sms / groups);
   return (int)std::max(1ll, std::min(want, (group_rows + 8 * p.per - 1) / (8 * p.per)));
@@ -1005,7 +1134,7 @@ extern "C" int sb_gated_norm(const void* x, long long x_row, long long x_img, in
   if (B < 0 || T < 0 || D < 1 || D > kMaxD || !rows_dtype_ok(x_dtype) || !rows_dtype_ok(z_dtype) || !(eps >= 0.f))
     return record_error(SB_EINVAL, "sb_gated_norm: sizes (1 <= D <= 8192), dtype or eps");
   if (B == 0 || T == 0) return SB_OK;
-  if (!x || !z || !y || (pre_w != nullptr) != (h != nullptr) || (post_b && !post_w) || (pre_b && !pre_w))
+  if (!x || !z || !y || (pre_w != nullptr) != (h != nullptr) || (post_b && !(post_w && layer)) || (pre_b && !(pre_w && layer)))
     return record_error(SB_EINVAL, "sb_gated_norm: null argument (h with pre_w, biases with their weights)");
   const Plan p = plan_of(D, false);
   NormArgs a{};
@@ -1059,7 +1188,7 @@ extern "C" int sb_gated_norm_backward(const void* dy, long long dy_row, long lon
                                       long long work_bytes, void* stream) {
   if (B < 1 || T < 1 || D < 1 || D > kMaxD || !rows_dtype_ok(x_dtype) || !rows_dtype_ok(z_dtype) || !(eps >= 0.f))
     return record_error(SB_EINVAL, "sb_gated_norm_backward: sizes (1 <= D <= 8192), dtype or eps");
-  if (!x || !z || !dx || !dz || (dh && !pre_w) || (post_b && !post_w) || (pre_b && !pre_w) || dgate_mode < 0 ||
+  if (!x || !z || !dx || !dz || (dh && !pre_w) || (post_b && !(post_w && layer)) || (pre_b && !(pre_w && layer)) || dgate_mode < 0 ||
       dgate_mode > 3 || (dgate_mode != 0 && (!dgate || !gate)) || (dscale && !scale) || ((dpost_w || dpost_b) && !post_w) ||
       ((dpre_w || dpre_b) && !pre_w))
     return record_error(SB_EINVAL, "sb_gated_norm_backward: null argument or a gradient without its input");
