@@ -4,20 +4,24 @@
 // out_i = sum_j exp(s_ij - L_i) v_j; a query without keys gets zeros and L_i = -inf.
 //
 // The query heads that share a key head are one list of rows (token-major, head-minor): a tile is
-// 128 of them, whatever the group's size.  A CTA takes NT tiles of one (item, key head) and a range
-// of key tiles (KT keys), walked once with the softmax's running maximum and sum:
-//   loader warp   K and V tiles by TMA into one ring, in the order K0 V0 K1 V1 ...
+// 128 of them, whatever the group's size.  A CTA has two streams of 128-row tiles, each with its scores,
+// accumulator and four softmax warps, over a range of 128-key tiles:
+//   two tiles of rows left   a tile a stream, both over every key tile
+//   one                      both streams on it, over alternate key tiles, joined at the end (a token
+//                            a stream, and the last tile of an odd number)
+//   loader warp   K and V tiles by TMA into one ring, in the order in which they are used
 //   MMA warp      S_t = Q_t K^T (operands in shared memory), O_t += P_t V with P_t in TMEM as the A
-//                 operand; the NT tiles alternate, so one tile's products run while the other's
-//                 softmax does
-//   4 warps/tile  thread = query row: reads its scores from TMEM, 2^(s scale log2 e - m), rounds P to
-//                 the operands' type and writes it over the scores.  O is rescaled only when the
+//                 operand; the streams alternate, so one's products run while the other's softmax does
+//   4 warps a stream  thread = query row: reads its scores from TMEM, 2^(s scale log2 e - m), rounds P
+//                 to the operands' type and writes it over the scores.  O is rescaled only when the
 //                 maximum grew by more than 2^8 since the last time (P stays below 2^8, far from
 //                 fp16's limit; the reference point cancels in O / l)
 //   cleaner warp  with masks: zeroes V's rows of keys that take no part (0 x NaN is NaN), before
 //                 the product reads them
-// Few rows (a token a stream, NT = 1) leave SMs idle: the key range is split over CTAs, which write
-// fp32 partial rows with their L, and a second kernel joins them.
+// The exponentials bound the softmax (16 a clock and SM): part of them runs as a polynomial on the FMA
+// pipe, and the rest of a row's arithmetic works on pairs.
+// The key range is split over CTAs where the rows alone leave SMs idle: these write fp32 partial rows
+// with their L, and a second kernel joins them.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -45,41 +49,63 @@ struct FwdArgs {
   long long all_rows;
 };
 
-template <int DH, int NT>
-struct Fwd {
-  static constexpr int KT = NT == 2 ? 128 : 64;
-  static constexpr int QB = Tile<DH>::bytes(128);  // one tile of queries
-  static constexpr int SB = Tile<DH>::bytes(KT);   // a stage: one K or V tile
-  static constexpr int ROOM = (NT == 2 ? 224 : 109) * 1024 - NT * QB;
-  static constexpr int STAGES = ROOM / SB < 8 ? ROOM / SB : 8;
-  static constexpr int SMEM = 1024 + NT * QB + STAGES * SB + 512;
-  static constexpr int THREADS = (NT * 4 + 3) * 32;
-  static constexpr uint32_t TMEM = NT == 2 ? 512 : 256;
-  static constexpr int O0 = NT * KT;  // TMEM column of the first accumulator
-  static_assert(STAGES >= 3 && NT * (KT + DH) <= (int)TMEM, "ring and TMEM");
-};
-constexpr int kClean = 8;  // more V tiles than the ring can hold at once
+constexpr int KT = 128;      // keys a tile
+constexpr int kClean = 8;    // more V tiles than the ring can hold at once
+constexpr int kThreads = 11 * 32;
 
-template <int DH, bool BF16, int NT>
-__global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
+template <int DH>
+struct Fwd {
+  static constexpr int QB = Tile<DH>::bytes(128);  // a tile of queries
+  static constexpr int SB = Tile<DH>::bytes(KT);   // a stage: one K or V tile
+  static constexpr int ROOM = 224 * 1024 - 2 * QB;
+  static constexpr int STAGES = ROOM / SB < 8 ? ROOM / SB : 8;
+  static constexpr int SMEM = 1024 + 2 * QB + STAGES * SB + 512 + 1024;
+  static constexpr int O0 = 2 * KT;  // TMEM column of the first accumulator
+  static_assert(STAGES >= 3 && 2 * (KT + DH) <= 512, "ring and TMEM");
+  // pairs of exponentials out of 16 that take the polynomial: more where the products are short
+  static constexpr int POLY = DH == 128 ? 4 : 5;
+};
+
+// P of 32 columns: 2^(s sl - ms), their sum added to `sum`, rounded into 16 words
+template <int DH, bool BF16, bool POLY>
+SB_DEV void probabilities(const uint32_t* s, uint64_t sl, uint64_t ms, uint64_t (&sum)[2], uint32_t (&pk)[16]) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const uint64_t x = fma2(pair2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), sl, ms);
+    float a, b;
+    if (POLY && (j * Fwd<DH>::POLY) % 16 < Fwd<DH>::POLY) {
+      exp2_poly(x, a, b);
+    } else {
+      split2(x, a, b);
+      a = exp2_hw(a);
+      b = exp2_hw(b);
+    }
+    sum[j & 1] = add2(sum[j & 1], pair2(a, b));
+    pk[j] = pack16<BF16>(a, b);
+  }
+}
+
+template <int DH, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
     attend_kernel(const __grid_constant__ FwdArgs a, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap) {
-  using C = Fwd<DH, NT>;
+  using C = Fwd<DH>;
   using T = Tile<DH>;
-  constexpr int KT = C::KT, ST = C::STAGES;
+  constexpr int ST = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = smem + NT * C::QB;
+  uint8_t* ring = smem + 2 * C::QB;
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + ST * C::SB);
   uint64_t* empty = full + ST;
-  uint64_t* clean = empty + ST;     // [kClean]
-  uint64_t* q_full = clean + kClean;  // [NT] each
-  uint64_t* s_full = q_full + NT;
-  uint64_t* p_full = s_full + NT;
-  uint64_t* o_full = p_full + NT;
-  uint64_t* dbar = o_full + NT;
+  uint64_t* clean = empty + ST;       // [kClean]
+  uint64_t* q_full = clean + kClean;  // [2] each
+  uint64_t* s_full = q_full + 2;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* dbar = o_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dbar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  float2* ml = reinterpret_cast<float2*>(ring + ST * C::SB + 512);  // [128] maximum and sum of the second stream
   const int warp = warp_id(), lane = lane_id();
 
   int idx = blockIdx.x;
@@ -88,12 +114,14 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
   const int split = idx % a.splits;
   idx /= a.splits;
   const int kvh = idx % a.Hkv, b = idx / a.Hkv;
-  const int tiles = (a.rows + 127) / 128;
-  const int na = min(NT, tiles - pair * NT);  // tiles of this CTA
+  const bool two = pair * 256 + 128 < a.rows;  // two tiles of rows
   const int count = a.mask.count(b);
   const int each = (a.key_tiles + a.splits - 1) / a.splits;
   const int first = split * each;
   const int n = max(0, min(min(first + each, a.key_tiles), (count + KT - 1) / KT) - first);
+  // places of K and V tile i in the ring: K0 V0 K1 V1 ..., or with alternate tiles K0 K1 V0 K2 V1 ...
+  auto k_at = [&](int i) { return two ? 2 * i : max(0, 2 * i - 1); };
+  auto v_at = [&](int i) { return two ? 2 * i + 1 : min(2 * i + 2, 2 * n - 1); };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
@@ -101,7 +129,7 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < kClean; ++i) mbar_init(&clean[i], 1);
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 4);
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[t], 4);
@@ -111,8 +139,8 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == NT * 4) {
-    tmem_alloc(tmem_holder, C::TMEM);
+  if (warp == 8) {
+    tmem_alloc(tmem_holder, 512);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -124,7 +152,20 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
     atomicOr(&g_xattn_error, code);
   };
 
-  if (warp == NT * 4 + 1) {
+  // softmax threads: their row, running maximum (of the raw scores) and sum
+  const int t = warp >> 2, quad = warp & 3;  // stream, TMEM lane quadrant
+  const int tile = pair * 2 + (two ? t : 0);
+  const int r = tile * 128 + quad * 32 + lane;
+  const bool some = warp < 8 && tile * 128 + quad * 32 < a.rows;  // the warp has rows
+  const int tq = r / a.group, h = kvh * a.group + (r - tq * a.group);
+  const int mine = two ? n : (n - t + 1) / 2;  // key tiles of the stream
+  const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+  const uint32_t s_at = tmem + lanes + t * KT, o_at = tmem + lanes + C::O0 + t * DH;
+  const float sl = a.scale_log2;
+  float m = -INFINITY, l = 0.f;
+  bool ok = true;
+
+  if (warp == 9) {
     if (lane == 0) {  // loader
       prefetch_tmap(&kmap);
       prefetch_tmap(&vmap);
@@ -136,55 +177,90 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
           break;
         }
         mbar_arrive_expect_tx(&full[st], C::SB);
-        const CUtensorMap* map = p & 1 ? &vmap : &kmap;
-        const int item = b * (p & 1 ? a.v_item : a.k_item);
+        bool v;
+        int i;
+        if (two) {
+          v = p & 1;
+          i = p / 2;
+        } else if (p == 2 * n - 1) {
+          v = true;
+          i = n - 1;
+        } else {
+          v = p > 0 && !(p & 1);
+          i = v ? p / 2 - 1 : (p + 1) / 2;
+        }
+        const CUtensorMap* map = v ? &vmap : &kmap;
+        const int item = b * (v ? a.v_item : a.k_item);
         for (int x = 0; x < T::BOXES; ++x)
-          tma_load_4d(ring + st * C::SB + x * T::box_bytes(KT), map, &full[st], x * T::COLS, (first + p / 2) * KT, kvh,
-                      item);
+          tma_load_4d(ring + st * C::SB + x * T::box_bytes(KT), map, &full[st], x * T::COLS, (first + i) * KT, kvh, item);
       }
       if (*abort_flag)
         for (int i = max(0, p - ST); i < p; ++i) bounded_wait(&full[i % ST], (i / ST) & 1);
     }
-  } else if (warp == NT * 4) {
+  } else if (warp == 8) {
     if (lane == 0 && n > 0) {  // MMA
       const uint32_t qb = smem_u32(smem), rb = smem_u32(ring);
       constexpr uint32_t id_s = idesc_16bit(BF16, 128, KT, false), id_o = idesc_16bit(BF16, 128, DH, true);
-      auto scores = [&](int t, int st) {
+      auto landed = [&](int p) { return mbar_wait(&full[p % ST], (p / ST) & 1, abort_flag); };
+      auto scores = [&](int u, int i) {  // stream u, key tile i
+        const uint32_t k = rb + k_at(i) % ST * C::SB, q = qb + (two ? u * C::QB : 0);
 #pragma unroll
         for (int ks = 0; ks < T::KSTEPS; ++ks)
-          mma_f16_ss(tmem + t * KT, T::k_major(qb + t * C::QB, 128, ks), T::k_major(rb + st * C::SB, KT, ks), id_s, ks > 0);
-        mma_commit(&s_full[t]);
+          mma_f16_ss(tmem + u * KT, T::k_major(q, 128, ks), T::k_major(k, KT, ks), id_s, ks > 0);
+        mma_commit(&s_full[u]);
       };
-      bool ok = true;
-      for (int t = 0; t < na && ok; ++t) ok = mbar_wait(&q_full[t], 0, abort_flag);
-      ok = ok && mbar_wait(&full[0], 0, abort_flag);
-      if (ok) {
-        tc_fence_after();
-        for (int t = 0; t < na; ++t) scores(t, 0);
-        mma_commit(&empty[0]);
-      }
-      for (int i = 0; i < n && ok; ++i) {
-        const int vp = 2 * i + 1, vs = vp % ST, kp = 2 * i + 2, ks = kp % ST;
-        for (int t = 0; t < na; ++t) {
-          ok = mbar_wait(&p_full[t], i & 1, abort_flag);
-          if (t == 0 && ok)
-            ok = mbar_wait(&full[vs], (vp / ST) & 1, abort_flag) &&
-                 (!a.masked || mbar_wait(&clean[i % kClean], (i / kClean) & 1, abort_flag));
-          if (!ok) break;
-          tc_fence_after();
+      auto values = [&](int u, int i, bool add) {
+        const uint32_t v = rb + v_at(i) % ST * C::SB;
 #pragma unroll
-          for (int k = 0; k < KT / 16; ++k)
-            mma_f16_ts(tmem + C::O0 + t * DH, tmem + t * KT + k * 8, T::mn_major(rb + vs * C::SB, KT, k), id_o,
-                       i > 0 || k > 0);
-          mma_commit(&o_full[t]);
-          if (t == na - 1) mma_commit(&empty[vs]);
-          if (i + 1 < n) {
-            if (t == 0) ok = mbar_wait(&full[ks], (kp / ST) & 1, abort_flag);
+        for (int k = 0; k < KT / 16; ++k)
+          mma_f16_ts(tmem + C::O0 + u * DH, tmem + u * KT + k * 8, T::mn_major(v, KT, k), id_o, add || k > 0);
+        mma_commit(&o_full[u]);
+      };
+      auto clean_v = [&](int i) {
+        return landed(v_at(i)) && (!a.masked || mbar_wait(&clean[i % kClean], (i / kClean) & 1, abort_flag));
+      };
+      ok = mbar_wait(&q_full[0], 0, abort_flag) && (!two || mbar_wait(&q_full[1], 0, abort_flag));
+      if (two) {
+        ok = ok && landed(0);
+        if (ok) {
+          tc_fence_after();
+          scores(0, 0);
+          scores(1, 0);
+          mma_commit(&empty[0]);
+        }
+        for (int i = 0; i < n && ok; ++i)
+          for (int u = 0; u < 2 && ok; ++u) {
+            ok = mbar_wait(&p_full[u], i & 1, abort_flag) && (u > 0 || clean_v(i));
             if (!ok) break;
             tc_fence_after();
-            scores(t, ks);
-            if (t == na - 1) mma_commit(&empty[ks]);
+            values(u, i, i > 0);
+            if (u == 1) mma_commit(&empty[v_at(i) % ST]);
+            if (i + 1 < n) {
+              ok = u > 0 || landed(k_at(i + 1));
+              if (!ok) break;
+              tc_fence_after();
+              scores(u, i + 1);
+              if (u == 1) mma_commit(&empty[k_at(i + 1) % ST]);
+            }
           }
+      } else {
+        auto next = [&](int i) {
+          ok = ok && landed(k_at(i));
+          if (!ok) return;
+          tc_fence_after();
+          scores(i & 1, i);
+          mma_commit(&empty[k_at(i) % ST]);
+        };
+        next(0);
+        if (n > 1) next(1);
+        for (int i = 0; i < n && ok; ++i) {
+          const int u = i & 1;
+          ok = mbar_wait(&p_full[u], (i >> 1) & 1, abort_flag) && clean_v(i);
+          if (!ok) break;
+          tc_fence_after();
+          values(u, i, i > 1);
+          mma_commit(&empty[v_at(i) % ST]);
+          if (i + 2 < n) next(i + 2);
         }
       }
       if (!ok) {
@@ -193,11 +269,12 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
         bounded_wait(dbar, 0);
       }
     }
-  } else if (warp == NT * 4 + 2) {
+  } else if (warp == 10) {
     if (a.masked) {  // cleaner
       for (int i = 0; i < n; ++i) {
-        const int vp = 2 * i + 1, vs = vp % ST, j0 = (first + i) * KT;
-        if (!warp_wait(&full[vs], (vp / ST) & 1, abort_flag)) {
+        const int p = v_at(i), j0 = (first + i) * KT;
+        uint8_t* v = ring + p % ST * C::SB;
+        if (!warp_wait(&full[p % ST], (p / ST) & 1, abort_flag)) {
           if (lane == 0) give_up(SB_ERR_TIMEOUT_FULL);
           break;
         }
@@ -209,21 +286,15 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
           touched = true;
           if (!(w >> lane & 1u))
             for (int c = 0; c < DH / 8; ++c)
-              *reinterpret_cast<uint4*>(ring + vs * C::SB + T::chunk(KT, 32 * x + lane, c)) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(v + T::chunk(KT, 32 * x + lane, c)) = make_uint4(0, 0, 0, 0);
         }
         if (touched) fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&clean[i % kClean]);
       }
     }
-  } else if (warp < na * 4) {
-    const int t = warp >> 2, quad = warp & 3;
-    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const uint32_t s_at = tmem + lanes + t * KT, o_at = tmem + lanes + C::O0 + t * DH;
-    const int r = (pair * NT + t) * 128 + quad * 32 + lane;  // row of the (item, key head)
-    const bool some = (pair * NT + t) * 128 + quad * 32 < a.rows;  // the warp has rows
-    const int tq = r / a.group, h = kvh * a.group + (r - tq * a.group);
-    {
+  } else {
+    if (two || t == 0) {
       const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __half*>(a.q.p) + b * a.q.img + tq * a.q.row +
                                                         (long long)h * DH);
       uint8_t* dst = smem + t * C::QB;
@@ -235,15 +306,15 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[t]);
     }
-    const float sl = a.scale_log2, slack = 8.f / sl;
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
+    const float slack = 8.f / sl;
+    const uint64_t sl2 = pair2(sl, sl);
+    for (int i = 0; i < mine; ++i) {
+      const int j0 = (first + (two ? i : 2 * i + t)) * KT;
       uint32_t w[KT / 32];
       bool all = true;
 #pragma unroll
       for (int x = 0; x < KT / 32; ++x) {
-        w[x] = a.mask.word(b, (first + i) * KT + 32 * x, count);
+        w[x] = a.mask.word(b, j0 + 32 * x, count);
         all = all && w[x] == 0xFFFFFFFFu;
       }
       ok = warp_wait(&s_full[t], i & 1, abort_flag);
@@ -261,15 +332,16 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < KT; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        for (int j = 0; j < KT; j += 2)
+          mx[j / 2 & 3] = max3(mx[j / 2 & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+        const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
         if (i == 0) {
           m = top;  // nothing accumulated yet
-        } else if (__any_sync(0xFFFFFFFFu, top > m + slack)) {
+        } else if (__any_sync(0xFFFFFFFFu, !(top <= m + slack))) {  // also for NaN
           ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          const float mn = fmaxf(m, top);
+          const float mn = max3(m, top, top);
           const float c = m == mn ? 1.f : exp2_hw((m - mn) * sl);
           m = mn;
           l *= c;
@@ -283,72 +355,123 @@ __global__ void __launch_bounds__(Fwd<DH, NT>::THREADS, NT == 2 ? 1 : 2)
             tmem_st16(o_at + 16 * x, o);
           }
         }
-        const float ms = m == -INFINITY ? 0.f : m * sl;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float ms = m == -INFINITY ? 0.f : -m * sl;
+        const uint64_t ms2 = pair2(ms, ms);
+        uint64_t sum[2] = {0, 0};
+        if (all) {
 #pragma unroll
-        for (int x = 0; x < KT / 32; ++x) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float p0 = exp2_hw(fmaf(__uint_as_float(s[32 * x + 2 * j]), sl, -ms));
-            const float p1 = exp2_hw(fmaf(__uint_as_float(s[32 * x + 2 * j + 1]), sl, -ms));
-            sum[j & 3] += p0 + p1;
-            pk[j] = pack16<BF16>(p0, p1);
+          for (int x = 0; x < KT / 32; ++x) {
+            uint32_t pk[16];
+            probabilities<DH, BF16, true>(s + 32 * x, sl2, ms2, sum, pk);
+            tmem_st16(s_at + 16 * x, pk);
           }
-          tmem_st16(s_at + 16 * x, pk);
+        } else {  // -inf in masked places must give an exact zero: no polynomial
+#pragma unroll
+          for (int x = 0; x < KT / 32; ++x) {
+            uint32_t pk[16];
+            probabilities<DH, BF16, false>(s + 32 * x, sl2, ms2, sum, pk);
+            tmem_st16(s_at + 16 * x, pk);
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float s0, s1;
+        split2(add2(sum[0], sum[1]), s0, s1);
+        l += s0 + s1;
         tmem_st_wait();
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[t]);
     }
-    if (ok && n > 0) ok = warp_wait(&o_full[t], (n - 1) & 1, abort_flag);
-    if (!ok) {
-      if (lane == 0) give_up(SB_ERR_TIMEOUT_ACC);
-    } else if (some) {
-      tc_fence_after();
-      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
-      const float lse = l == 0.f ? -INFINITY : m * sl * 0.69314718055994531f + logf(l);
-      const long long rr = ((long long)b * a.H + h) * a.Tq + tq;
-      const bool live = r < a.rows;
+    if (ok && mine > 0) ok = warp_wait(&o_full[t], (mine - 1) & 1, abort_flag);
+    if (!ok && lane == 0) give_up(SB_ERR_TIMEOUT_ACC);
+    tc_fence_after();
+  }
+
+  float m1 = -INFINITY, l1 = 0.f;  // of the other stream on the same rows
+  float4* other = reinterpret_cast<float4*>(smem);  // [128][DH / 4] its O, in the queries' place
+  constexpr int per = DH / 4;
+  const int lr = quad * 32 + lane;
+  const bool join = !two && n > 1;
+  if (join) {
+    __syncthreads();  // both streams' products are done: the queries are no longer read
+    if (warp >= 4 && warp < 8 && some && ok) {
+      ml[lr] = make_float2(m, l);
 #pragma unroll
-      for (int x = 0; x < DH / 32; ++x) {
-        uint32_t o[32];
-        __syncwarp();
-        if (n > 0) {
-          tmem_ld32(o_at + 32 * x, o);
-          tmem_ld_wait();
-        }
-        if (!live || (a.splits > 1 && n == 0)) continue;
-        float f[32];
+      for (int x = 0; x < DH / 16; ++x) {
+        uint32_t o[16];
+        tmem_ld16(o_at + 16 * x, o);
+        tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = n > 0 && l != 0.f ? __uint_as_float(o[j]) * inv : 0.f;
-        if (a.splits > 1) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + (split * a.all_rows + rr) * DH + 32 * x);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) dst[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(a.o.p) + b * a.o.img + tq * a.o.row +
-                                                (long long)h * DH + 32 * x);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            dst[j] = make_uint4(pack16<BF16>(f[8 * j], f[8 * j + 1]), pack16<BF16>(f[8 * j + 2], f[8 * j + 3]),
-                                pack16<BF16>(f[8 * j + 4], f[8 * j + 5]), pack16<BF16>(f[8 * j + 6], f[8 * j + 7]));
-        }
-      }
-      if (live) {
-        if (a.splits > 1) a.part_l[split * a.all_rows + rr] = n > 0 ? lse : -INFINITY;
-        else if (a.lse) a.lse[rr] = n > 0 ? lse : -INFINITY;
+        for (int c = 0; c < 4; ++c)
+          other[lr * per + ((4 * x + c) ^ (lr & 7))] =
+              make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
+                          __uint_as_float(o[4 * c + 3]));
       }
     }
-    tc_fence_before();
+    __syncthreads();
   }
+  if (warp < (two ? 8 : 4) && some && !*abort_flag) {
+    float w0 = 1.f, w1 = 0.f;
+    if (join) {
+      m1 = ml[lr].x;
+      l1 = ml[lr].y;
+      const float top = max3(m, m1, m1);
+      w0 = m == top ? 1.f : exp2_hw((m - top) * sl);
+      w1 = m1 == top ? 1.f : exp2_hw((m1 - top) * sl);
+      m = top;
+      l = l * w0 + l1 * w1;
+    }
+    const float lse = l == 0.f ? -INFINITY : m * sl * 0.69314718055994531f + logf(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    w0 *= inv;
+    w1 *= inv;
+    const long long rr = ((long long)b * a.H + h) * a.Tq + tq;
+    const bool live = r < a.rows;
+#pragma unroll
+    for (int x = 0; x < DH / 16; ++x) {
+      uint32_t o[16];
+      float f[16];
+      __syncwarp();
+      if (mine > 0) {
+        tmem_ld16(o_at + 16 * x, o);
+        tmem_ld_wait();
+      }
+      if (!live || (a.splits > 1 && n == 0)) continue;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) f[j] = mine > 0 ? __uint_as_float(o[j]) * w0 : 0.f;
+      if (join) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float4 e = other[lr * per + ((4 * x + c) ^ (lr & 7))];
+          f[4 * c] = fmaf(e.x, w1, f[4 * c]);
+          f[4 * c + 1] = fmaf(e.y, w1, f[4 * c + 1]);
+          f[4 * c + 2] = fmaf(e.z, w1, f[4 * c + 2]);
+          f[4 * c + 3] = fmaf(e.w, w1, f[4 * c + 3]);
+        }
+      }
+      if (a.splits > 1) {
+        float4* dst = reinterpret_cast<float4*>(a.part_o + (split * a.all_rows + rr) * DH + 16 * x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dst[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+      } else {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(a.o.p) + b * a.o.img + tq * a.o.row +
+                                              (long long)h * DH + 16 * x);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          dst[j] = make_uint4(pack16<BF16>(f[8 * j], f[8 * j + 1]), pack16<BF16>(f[8 * j + 2], f[8 * j + 3]),
+                              pack16<BF16>(f[8 * j + 4], f[8 * j + 5]), pack16<BF16>(f[8 * j + 6], f[8 * j + 7]));
+      }
+    }
+    if (live) {
+      if (a.splits > 1) a.part_l[split * a.all_rows + rr] = n > 0 ? lse : -INFINITY;
+      else if (a.lse) a.lse[rr] = n > 0 ? lse : -INFINITY;
+    }
+  }
+  tc_fence_before();
   __syncthreads();
-  if (warp == NT * 4) {
+  if (warp == 8) {
     tc_fence_after();
-    tmem_dealloc(tmem, C::TMEM);
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -397,29 +520,31 @@ __global__ void attend_none_kernel(OutView o, float* lse, int H, int Tq, int dh,
 }
 
 struct FwdPlan {
-  int nt, kt, pairs, splits, key_tiles;
+  int pairs, splits, key_tiles;
   long long units;
 };
 
-// Two tiles of rows a CTA where there are two (one CTA an SM), one otherwise (two CTAs an SM).  The
-// key range is split where the CTAs' last wave would leave more SMs idle than the splits cost: a CTA
-// spends about `kStart` key tiles on starting and ending, and joining costs about as much again.
+// CTAs take two tiles of rows each; a last single tile takes half of a CTA's time (its streams share
+// the key tiles).  The key range is split where that shortens the longest CTA or evens out the SMs by
+// more than it costs: a CTA spends about `kStart` key tiles on starting and ending, and joining costs
+// about as much again.
 FwdPlan fwd_plan(int B, int H, int Hkv, int Tq, int Tk, int sms) {
   constexpr int kStart = 4, kMost = 64;
   FwdPlan p;
-  const int rows_tiles = (int)(((long long)(H / Hkv) * Tq + 127) / 128);
-  p.nt = rows_tiles >= 2 ? 2 : 1;
-  p.kt = p.nt == 2 ? 128 : 64;
-  p.pairs = (rows_tiles + p.nt - 1) / p.nt;
-  p.key_tiles = (Tk + p.kt - 1) / p.kt;
+  const long long tiles = ((long long)(H / Hkv) * Tq + 127) / 128;
+  p.pairs = (int)((tiles + 1) / 2);
+  p.key_tiles = (Tk + KT - 1) / KT;
   p.units = (long long)B * Hkv * p.pairs;
-  const long long slots = (long long)sms * (p.nt == 2 ? 1 : 2);
+  const double twos = (double)B * Hkv * (tiles / 2), ones = (double)B * Hkv * (tiles % 2);
   p.splits = 1;
   double best = 1e300;
   for (int s = 1; s <= std::min(kMost, p.key_tiles); ++s) {
-    const long long each = (p.key_tiles + s - 1) / s;
+    const int each = (p.key_tiles + s - 1) / s;
     if ((p.key_tiles + each - 1) / each != s) continue;  // some split would be empty
-    const double cost = (double)((p.units * s + slots - 1) / slots) * (each + kStart) + (s > 1 ? kStart : 0);
+    const double t2 = each + kStart, t1 = 0.5 * each + kStart, longest = tiles > 1 ? t2 : t1;
+    // SMs take CTAs as they come: the even share, and about half of a CTA's time until the last ends
+    const double share = s * (twos * t2 + ones * t1) / sms;
+    const double cost = std::max(longest, share + 0.5 * longest) + (s > 1 ? kStart : 0);
     if (cost < 0.97 * best) {
       best = cost;
       p.splits = s;
@@ -445,12 +570,13 @@ PFN_encodeTiled encode_fn() {
   return fn;
 }
 
-template <int DH, bool BF16, int NT>
-cudaError_t launch_fwd(const FwdArgs& a, long long grid, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
-  using C = Fwd<DH, NT>;
-  cudaError_t e = cudaFuncSetAttribute(attend_kernel<DH, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+template <int DH, bool BF16>
+cudaError_t launch_fwd(const FwdArgs& a, const FwdPlan& p, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+  using C = Fwd<DH>;
+  static bool ready[64];
+  cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&attend_kernel<DH, BF16>), C::SMEM, ready);
   if (e != cudaSuccess) return e;
-  attend_kernel<DH, BF16, NT><<<(unsigned)grid, C::THREADS, C::SMEM, st>>>(a, k, v);
+  attend_kernel<DH, BF16><<<(unsigned)(p.units * p.splits), kThreads, C::SMEM, st>>>(a, k, v);
   e = cudaGetLastError();
   if (e != cudaSuccess || a.splits == 1) return e;
   const long long threads = a.all_rows * (DH / 8);
@@ -460,9 +586,7 @@ cudaError_t launch_fwd(const FwdArgs& a, long long grid, const CUtensorMap& k, c
 template <int DH>
 cudaError_t launch_fwd(const FwdArgs& a, const FwdPlan& p, bool bf16, const CUtensorMap& k, const CUtensorMap& v,
                        cudaStream_t st) {
-  const long long grid = p.units * p.splits;
-  if (p.nt == 2) return bf16 ? launch_fwd<DH, true, 2>(a, grid, k, v, st) : launch_fwd<DH, false, 2>(a, grid, k, v, st);
-  return bf16 ? launch_fwd<DH, true, 1>(a, grid, k, v, st) : launch_fwd<DH, false, 1>(a, grid, k, v, st);
+  return bf16 ? launch_fwd<DH, true>(a, p, k, v, st) : launch_fwd<DH, false>(a, p, k, v, st);
 }
 
 }  // namespace
@@ -497,6 +621,15 @@ int xattn_error(int clear, int* flags) {
   const int zero = 0;
   if (cudaMemcpyFromSymbol(flags, g_xattn_error, sizeof(int)) != cudaSuccess) return -1;
   return clear && cudaMemcpyToSymbol(g_xattn_error, &zero, sizeof(int)) != cudaSuccess ? -1 : 0;
+}
+
+cudaError_t xattn_smem(const void* kernel, int bytes, bool (&ready)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || ready[dev & 63]) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  ready[dev & 63] = e == cudaSuccess;
+  return e;
 }
 
 int xattn_sms() {
@@ -570,8 +703,8 @@ extern "C" int sb_cross_attention(const void* q, long long q_row, long long q_im
   a.part_o = static_cast<float*>(work);
   a.part_l = a.part_o + (long long)p.splits * a.all_rows * dh;
   CUtensorMap km, vm;
-  if (!xattn_tensor_map(&km, {k, k_row, k_img}, dtype, B, Tk, Hkv, dh, p.kt) ||
-      !xattn_tensor_map(&vm, {v, v_row, v_img}, dtype, B, Tk, Hkv, dh, p.kt))
+  if (!xattn_tensor_map(&km, {k, k_row, k_img}, dtype, B, Tk, Hkv, dh, KT) ||
+      !xattn_tensor_map(&vm, {v, v_row, v_img}, dtype, B, Tk, Hkv, dh, KT))
     return record_error(SB_EINVAL, "sb_cross_attention: tensor map of k or v");
   const bool bf16 = dtype == SB_BF16;
   const cudaError_t e = dh == 32 ? launch_fwd<32>(a, p, bf16, km, vm, st)

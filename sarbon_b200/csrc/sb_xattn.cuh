@@ -77,6 +77,49 @@ SB_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 SB_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two fp32 values in one register pair: one instruction works on both.
+SB_DEV uint64_t pair2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+SB_DEV void split2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+SB_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+SB_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// The largest of three; NaN if one is.
+SB_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of a pair on the FMA pipe, beside the special-function unit that bounds a softmax: x = j + f with
+// the integer j nearest to x (added to 1.5 2^23, whose low bits then hold it; Cody and Waite's
+// reduction), a polynomial for 2^f on [-1/2, 1/2] (least relative error at degree four, fitted by Remez
+// exchange: 2.7e-6), and j added to its exponent.  x >= -126 (raised to it).
+SB_DEV void exp2_poly(uint64_t x, float& lo, float& hi) {
+  float a, b, ta, tb;
+  split2(x, a, b);
+  x = pair2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t t = add2(x, pair2(12582912.f, 12582912.f));
+  const uint64_t f = fma2(add2(t, pair2(-12582912.f, -12582912.f)), pair2(-1.f, -1.f), x);
+  uint64_t r = fma2(f, pair2(0.009570101276f, 0.009570101276f), pair2(0.05591786280f, 0.05591786280f));
+  r = fma2(r, f, pair2(0.2402474433f, 0.2402474433f));
+  r = fma2(r, f, pair2(0.6931217909f, 0.6931217909f));
+  r = fma2(r, f, pair2(0.9999992847f, 0.9999992847f));
+  split2(r, a, b);
+  split2(t, ta, tb);
+  lo = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
+  hi = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
+}
+
 SB_DEV float exp2_hw(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -144,5 +187,7 @@ int gnorm_error(int clear, int* flags);  // of the gated norms
 long long xattn_back_work(int B, int H, int Hkv, int dh, int Tq, int Tk, int sms);
 // SMs of the current device, 0 on error
 int xattn_sms();
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device, once a device (`ready`).
+cudaError_t xattn_smem(const void* kernel, int bytes, bool (&ready)[64]);
 
 }  // namespace sb

@@ -502,8 +502,8 @@ BackPlan back_plan(int B, int H, int Hkv, int dh, int Tq, int Tk, int sms) {
 template <int DH, bool BF16, int SIDE>
 cudaError_t launch_side(BackArgs a, const SidePlan& p, const CUtensorMap (&m)[4], cudaStream_t st) {
   using C = Back<DH, SIDE>;
-  cudaError_t e =
-      cudaFuncSetAttribute(attend_back_kernel<DH, BF16, SIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  static bool ready[64];
+  cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&attend_back_kernel<DH, BF16, SIDE>), C::SMEM, ready);
   if (e != cudaSuccess) return e;
   a.x_tiles = p.x_tiles;
   a.splits = p.splits;

@@ -41,6 +41,8 @@ CALLS = [0]
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
 
 def _ready(*tensors):
     """All tensors on one CUDA device and none that autograd would have to follow; its index."""
@@ -57,7 +59,7 @@ def _ready(*tensors):
 
 def _launch(name, index, *args):
     CALLS[0] += 1
-    if index == torch.cuda.current_device():
+    if index == _device():
         status = getattr(lib(), name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -105,9 +107,11 @@ def _rows(t, what, shape, dtype, out=False):
     return t.data_ptr(), row, img
 
 
-def _dense(t, shape):
-    """_rows of a new tensor."""
-    return t.data_ptr(), shape[2], shape[1] * shape[2]
+def _new(like, shape, dtype):
+    """A contiguous tensor, (pointer, row stride, item stride); empty_like is the cheapest allocation."""
+    t = torch.empty_like(like) if like.dtype == dtype and like.is_contiguous() and like.shape == shape else \
+        torch.empty(shape, device=like.device, dtype=dtype)
+    return t, (t.data_ptr(), shape[2], shape[1] * shape[2])
 
 
 # ---------------------------------------------------------------- attention
@@ -175,8 +179,7 @@ def cross_attention(q, k, v, heads, kv_heads=None, lens=None, valid=None, scale=
         op = _rows(out, "out", qs, dtype, out=True)
     index = _ready(q, k, v, lens, valid, out, lse)
     if out is None:
-        out = torch.empty(qs, device=q.device, dtype=dtype)
-        op = _dense(out, qs)
+        out, op = _new(q, qs, dtype)
     if b == 0 or tq == 0:
         return out
     hold, work, size = _work("sb_cross_attention_work", index, 0, b, heads, kv_heads, dim, tq, tk)
@@ -202,15 +205,14 @@ def cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=None, lens
         if t is not None:
             _rows(t, what, shape, dtype, out=True)
     index = _ready(dout, q, k, v, out, lse, lens, valid, dq, dk, dv)
-    dq = torch.empty(qs, device=q.device, dtype=dtype) if dq is None else dq
-    dk = torch.empty(ks, device=q.device, dtype=dtype) if dk is None else dk
-    dv = torch.empty(ks, device=q.device, dtype=dtype) if dv is None else dv
-    if dq.numel() == 0 and dk.numel() == 0:
+    dq, dqp = _new(q, qs, dtype) if dq is None else (dq, _rows(dq, "dq", qs, dtype))
+    dk, dkp = _new(k, ks, dtype) if dk is None else (dk, _rows(dk, "dk", ks, dtype))
+    dv, dvp = _new(v, ks, dtype) if dv is None else (dv, _rows(dv, "dv", ks, dtype))
+    if b == 0 or (tq == 0 and tk == 0):
         return dq, dk, dv
-    grads = _rows(dq, "dq", qs, dtype) + _rows(dk, "dk", ks, dtype) + _rows(dv, "dv", ks, dtype)
     hold, work, size = _work("sb_cross_attention_work", index, 1, b, heads, kv_heads, dim, tq, tk)
     _launch("sb_cross_attention_backward", index, *views, lse.data_ptr(), DTYPES[dtype], b, heads, kv_heads, dim, tq, tk,
-            scale, *masks, *grads, work, size)
+            scale, *masks, *dqp, *dkp, *dvp, work, size)
     return dq, dk, dv
 
 
@@ -265,8 +267,7 @@ def rope_axes(x, pos, heads, freq, axis, layout="half", inverse=False, out=None)
         op = _rows(out, "out", shape, dtype, out=True)
     index = _ready(x, pos, freq, axis, out)
     if out is None:
-        out = torch.empty(shape, device=x.device, dtype=dtype)
-        op = _dense(out, shape)
+        out, op = _new(x, shape, dtype)
     if b == 0 or t == 0:
         return out
     _launch("sb_rope_axes", index, *xp, DTYPES[dtype], b, t, heads, dim, pos.data_ptr(), pos.dtype == torch.float32,
@@ -276,20 +277,14 @@ def rope_axes(x, pos, heads, freq, axis, layout="half", inverse=False, out=None)
 
 
 # ---------------------------------------------------------------- gated residual and norms
-def _columns(t, what, d):
-    if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.numel() != d or not t.is_contiguous()):
-        raise ValueError(f"{what}: contiguous fp32 [D]")
-    return t
-
-
-def _norm_weights(w, what, d, kind):
+def _norm_weights(w, what, kind):
     """A norm's weight, (weight, bias) or None -> (weight, bias)."""
     if w is None:
         return None, None
     w, b = w if isinstance(w, (tuple, list)) else (w, None)
     if w is None or (b is not None and kind != "layer"):
         raise ValueError(f"{what}: a weight, and a bias for layer norms only")
-    return _columns(w, what, d), _columns(b, what, d)
+    return w, b
 
 
 def _norm_inputs(x, z, gate, scale, post, pre, kind, eps):
@@ -297,7 +292,7 @@ def _norm_inputs(x, z, gate, scale, post, pre, kind, eps):
         raise ValueError("x, z: [B, T, D] of fp16, bf16 or fp32")
     if kind not in ("rms", "layer") or not eps >= 0:
         raise ValueError("kind: 'rms' or 'layer', eps >= 0")
-    shape = b, t, d = x.shape
+    b, t, d = shape = x.shape
     if not 1 <= d <= 8192:
         raise ValueError("1 to 8192 channels")
     gp = (None, 0, 0)
@@ -306,8 +301,10 @@ def _norm_inputs(x, z, gate, scale, post, pre, kind, eps):
         if gate.dtype != z.dtype or gate.shape not in ((d,), (b, d), (b, t, d)) or (d > 1 and s[-1] != 1):
             raise ValueError("gate: [D], [B, D] or [B, T, D] of z's type with contiguous channels")
         gp = (gate.data_ptr(), s[1] if n == 3 and t > 1 else 0, s[0] if n > 1 and b > 1 else 0)
-    _columns(scale, "scale", d)
-    weights = _norm_weights(post, "post", d, kind) + _norm_weights(pre, "pre", d, kind)
+    weights = _norm_weights(post, "post", kind) + _norm_weights(pre, "pre", kind)
+    for t in (scale,) + weights:
+        if t is not None and (t.dtype != torch.float32 or t.numel() != d or t.dim() != 1 or not t.is_contiguous()):
+            raise ValueError("scale, weights and biases: contiguous fp32 [D]")
     return shape, _rows(x, "x", shape, x.dtype), _rows(z, "z", shape, z.dtype), gp, weights
 
 
@@ -332,13 +329,11 @@ def gated_norm(x, z, gate=None, scale=None, post=None, pre=None, kind="rms", eps
         hp = _rows(h, "h", shape, z.dtype, out=True)
     index = _ready(x, z, gate, scale, *weights, y, h)
     if y is None:
-        y = torch.empty(shape, device=x.device, dtype=x.dtype)
-        yp = _dense(y, shape)
+        y, yp = _new(x, shape, x.dtype)
     if h is None and pre is not None:
-        h = torch.empty(shape, device=x.device, dtype=z.dtype)
-        hp = _dense(h, shape)
+        h, hp = _new(z, shape, z.dtype)
     if shape[0] and shape[1]:
-        _launch("sb_gated_norm", index, *xp, DTYPES[x.dtype], *zp, DTYPES[z.dtype], *gp, _ptr(scale), *map(_ptr, weights),
+        _launch("sb_gated_norm", index, *xp, DTYPES[x.dtype], *zp, DTYPES[z.dtype], *gp, *[None if w is None else w.data_ptr() for w in (scale,) + weights],
                 kind == "layer", eps, *shape, *yp, *hp)
     return y, h
 
@@ -356,7 +351,7 @@ def gated_norm_backward(dy, dh, x, z, gate=None, scale=None, post=None, pre=None
     dyp = (None, 0, 0) if dy is None else _rows(dy, "dy", shape, x.dtype)
     dhp = (None, 0, 0) if dh is None else _rows(dh, "dh", shape, z.dtype)
     index = _ready(x, z, gate, scale, *weights, dy, dh)
-    g = {"dx": torch.empty(shape, device=x.device, dtype=x.dtype), "dz": torch.empty(shape, device=x.device, dtype=z.dtype)}
+    g = {"dx": _new(x, shape, x.dtype)[0], "dz": _new(z, shape, z.dtype)[0]}
     make = torch.empty if b * t else torch.zeros  # no rows: every sum is zero
     for name, w in zip(("scale", "post_w", "post_b", "pre_w", "pre_b"), (scale,) + weights):
         g[name] = None if w is None else make(d, device=x.device, dtype=torch.float32)
