@@ -4,22 +4,28 @@
 // out_i = sum_j exp(s_ij - L_i) v_j; a query without keys gets zeros and L_i = -inf.
 //
 // The query heads that share a key head are one list of rows (token-major, head-minor): a tile is
-// 128 of them, whatever the group's size.  A CTA has two streams of 128-row tiles, each with its scores,
-// accumulator and four softmax warps, over a range of 128-key tiles:
+// 128 of them, whatever the group's size.  A CTA has two streams of 128-row tiles, each with an
+// accumulator, eight softmax warps and a warp that issues its products, over a range of 128-key tiles:
 //   two tiles of rows left   a tile a stream, both over every key tile
 //   one                      both streams on it, over alternate key tiles, joined at the end (a token
 //                            a stream, and the last tile of an odd number)
 //   loader warp   K and V tiles by TMA into one ring, in the order in which they are used
-//   MMA warp      S_t = Q_t K^T (operands in shared memory), O_t += P_t V with P_t in TMEM as the A
-//                 operand; the streams alternate, so one's products run while the other's softmax does
-//   4 warps a stream  thread = query row: reads its scores from TMEM, 2^(s scale log2 e - m), rounds P
-//                 to the operands' type and writes it over the scores.  O is rescaled only when the
-//                 maximum grew by more than 2^8 since the last time (P stays below 2^8, far from
-//                 fp16's limit; the reference point cancels in O / l)
+//   issuer warps  S_t = Q_t K^T (operands in shared memory); O_t += P_t V with P_t in TMEM as the A
+//                 operand.  One a stream: a wait on a barrier costs an issuer a few hundred clocks, in
+//                 which the other one keeps the tensor pipe fed
+//   8 warps a stream  two threads a query row, 64 keys each (one thread a row left two warps a
+//                 scheduler, too few to cover the arithmetic's latency): scores from TMEM into registers
+//                 at once, so that the next tile's are computed meanwhile (one buffer for both
+//                 streams with 128 channels, which the accumulators leave no room beside; one each
+//                 below); P = 2^(s scale log2 e - m), rounded to the operands' type, back to TMEM.  The
+//                 reference point m moves, and O is rescaled, only when a row's maximum grew by more
+//                 than 2^8 since the last time (P stays below 2^8, far from fp16's limit; m cancels in
+//                 O / l), so the two threads need each other's maximum only then: otherwise one barrier
+//                 with the OR of "grew" is all that a tile costs them
 //   cleaner warp  with masks: zeroes V's rows of keys that take no part (0 x NaN is NaN), before
 //                 the product reads them
-// The exponentials bound the softmax (16 a clock and SM): part of them runs as a polynomial on the FMA
-// pipe, and the rest of a row's arithmetic works on pairs.
+// The exponentials bound heads of few channels (16 a clock and SM): there, part of them runs as a
+// polynomial on the FMA pipe.  The rest of a row's arithmetic works on pairs.
 // The key range is split over CTAs where the rows alone leave SMs idle: these write fp32 partial rows
 // with their L, and a second kernel joins them.
 #include <algorithm>
@@ -51,7 +57,8 @@ struct FwdArgs {
 
 constexpr int KT = 128;      // keys a tile
 constexpr int kClean = 8;    // more V tiles than the ring can hold at once
-constexpr int kThreads = 11 * 32;
+constexpr int kSoft = 16;     // softmax warps: stream (w / 8), half of a tile's keys (w / 4 % 2), TMEM lanes (w % 4)
+constexpr int kThreads = (kSoft + 4) * 32;
 
 template <int DH>
 struct Fwd {
@@ -60,20 +67,22 @@ struct Fwd {
   static constexpr int ROOM = 224 * 1024 - 2 * QB;
   static constexpr int STAGES = ROOM / SB < 8 ? ROOM / SB : 8;
   static constexpr int SMEM = 1024 + 2 * QB + STAGES * SB + 512 + 1024;
-  static constexpr int O0 = 2 * KT;  // TMEM column of the first accumulator
-  static_assert(STAGES >= 3 && 2 * (KT + DH) <= 512, "ring and TMEM");
-  // pairs of exponentials out of 16 that take the polynomial: more where the products are short
-  static constexpr int POLY = DH == 128 ? 4 : 5;
+  // TMEM columns: scores (shared by the streams or one each), P, accumulators
+  static constexpr bool SHARED = DH == 128;
+  static constexpr int P0 = SHARED ? KT : 2 * KT, O0 = P0 + KT;
+  static_assert(STAGES >= 5 && O0 + 2 * DH <= 512, "ring and TMEM");
+  // pairs of exponentials out of 16 that take the polynomial
+  static constexpr int POLY = DH == 128 ? 0 : 5;
 };
 
 // P of 32 columns: 2^(s sl - ms), their sum added to `sum`, rounded into 16 words
-template <int DH, bool BF16, bool POLY>
+template <int DH, bool BF16>
 SB_DEV void probabilities(const uint32_t* s, uint64_t sl, uint64_t ms, uint64_t (&sum)[2], uint32_t (&pk)[16]) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     const uint64_t x = fma2(pair2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), sl, ms);
     float a, b;
-    if (POLY && (j * Fwd<DH>::POLY) % 16 < Fwd<DH>::POLY) {
+    if ((j * Fwd<DH>::POLY) % 16 < Fwd<DH>::POLY) {
       exp2_poly(x, a, b);
     } else {
       split2(x, a, b);
@@ -98,14 +107,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + ST * C::SB);
   uint64_t* empty = full + ST;
   uint64_t* clean = empty + ST;       // [kClean]
-  uint64_t* q_full = clean + kClean;  // [2] each
-  uint64_t* s_full = q_full + 2;
-  uint64_t* p_full = s_full + 2;
+  uint64_t* q_full = clean + kClean;  // [2] each, a stream
+  uint64_t* s_full = q_full + 2;      // scores computed
+  uint64_t* s_free = s_full + 2;      // scores taken into registers
+  uint64_t* p_full = s_free + 2;
   uint64_t* o_full = p_full + 2;
-  uint64_t* dbar = o_full + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dbar + 1);
+  uint64_t* dbar = o_full + 2;        // [2]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dbar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  float2* ml = reinterpret_cast<float2*>(ring + ST * C::SB + 512);  // [128] maximum and sum of the second stream
+  // what threads of a row tell each other: [stream][row] a maximum or a sum; at the end [row] both of the
+  // second stream's
+  float* told = reinterpret_cast<float*>(ring + ST * C::SB + 512);
+  float2* ml = reinterpret_cast<float2*>(told);
   const int warp = warp_id(), lane = lane_id();
 
   int idx = blockIdx.x;
@@ -119,27 +132,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int each = (a.key_tiles + a.splits - 1) / a.splits;
   const int first = split * each;
   const int n = max(0, min(min(first + each, a.key_tiles), (count + KT - 1) / KT) - first);
-  // places of K and V tile i in the ring: K0 V0 K1 V1 ..., or with alternate tiles K0 K1 V0 K2 V1 ...
-  auto k_at = [&](int i) { return two ? 2 * i : max(0, 2 * i - 1); };
-  auto v_at = [&](int i) { return two ? 2 * i + 1 : min(2 * i + 2, 2 * n - 1); };
+  // a stream's scores are a tile before its values: the ring holds K0 .. K(ahead - 1) V0 K(ahead) V1 ...;
+  // the places of K and V tile i
+  const int ahead = two ? 2 : 4;
+  auto k_at = [&](int i) { return i + max(0, i - ahead + 1); };
+  auto v_at = [&](int i) { return i + min(n, i + ahead); };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&empty[i], two ? 2 : 1);  // the streams that read a tile
     }
     for (int i = 0; i < kClean; ++i) mbar_init(&clean[i], 1);
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&q_full[t], 4);
+      mbar_init(&q_full[t], kSoft / 2);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
+      mbar_init(&s_free[t], kSoft / 2);
+      mbar_init(&p_full[t], kSoft / 2);
       mbar_init(&o_full[t], 1);
+      mbar_init(&dbar[t], 1);
     }
-    mbar_init(dbar, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == kSoft) {
     tmem_alloc(tmem_holder, 512);
     tmem_relinquish();
   }
@@ -152,24 +168,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     atomicOr(&g_xattn_error, code);
   };
 
-  // softmax threads: their row, running maximum (of the raw scores) and sum
-  const int t = warp >> 2, quad = warp & 3;  // stream, TMEM lane quadrant
+  // softmax threads: their row, reference point (of the raw scores) and sum over their half of the keys
+  const int t = warp >> 3, hf = warp >> 2 & 1, quad = warp & 3;
+  const int lr = quad * 32 + lane;
   const int tile = pair * 2 + (two ? t : 0);
-  const int r = tile * 128 + quad * 32 + lane;
-  const bool some = warp < 8 && tile * 128 + quad * 32 < a.rows;  // the warp has rows
+  const int r = tile * 128 + lr;
+  const bool some = warp < kSoft && tile * 128 + quad * 32 < a.rows;  // the warp has rows
   const int tq = r / a.group, h = kvh * a.group + (r - tq * a.group);
   const int mine = two ? n : (n - t + 1) / 2;  // key tiles of the stream
   const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-  const uint32_t s_at = tmem + lanes + t * KT, o_at = tmem + lanes + C::O0 + t * DH;
+  const uint32_t s_at = tmem + lanes + (C::SHARED ? 0 : t * KT) + hf * 64, p_at = tmem + lanes + C::P0 + t * (KT / 2) + hf * 32;
+  const uint32_t o_at = tmem + lanes + C::O0 + t * DH + hf * (DH / 2);
+  const int bar_id = 1 + t * 4 + quad;  // of the two warps of these rows
+  float* tell = told + t * 128 + lr;
   const float sl = a.scale_log2;
   float m = -INFINITY, l = 0.f;
   bool ok = true;
 
-  if (warp == 9) {
+  if (warp == kSoft + 2) {
     if (lane == 0) {  // loader
       prefetch_tmap(&kmap);
       prefetch_tmap(&vmap);
-      int p = 0;
+      int p = 0, ki = 0, vi = 0;
       for (; p < 2 * n; ++p) {
         const int st = p % ST;
         if (p >= ST && !mbar_wait(&empty[st], ((p / ST) - 1) & 1, abort_flag)) {
@@ -177,18 +197,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         mbar_arrive_expect_tx(&full[st], C::SB);
-        bool v;
-        int i;
-        if (two) {
-          v = p & 1;
-          i = p / 2;
-        } else if (p == 2 * n - 1) {
-          v = true;
-          i = n - 1;
-        } else {
-          v = p > 0 && !(p & 1);
-          i = v ? p / 2 - 1 : (p + 1) / 2;
-        }
+        const bool v = ki == min(n, vi + ahead);
+        const int i = v ? vi++ : ki++;
         const CUtensorMap* map = v ? &vmap : &kmap;
         const int item = b * (v ? a.v_item : a.k_item);
         for (int x = 0; x < T::BOXES; ++x)
@@ -197,100 +207,86 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (*abort_flag)
         for (int i = max(0, p - ST); i < p; ++i) bounded_wait(&full[i % ST], (i / ST) & 1);
     }
-  } else if (warp == 8) {
-    if (lane == 0 && n > 0) {  // MMA
-      const uint32_t qb = smem_u32(smem), rb = smem_u32(ring);
+  } else if (warp == kSoft || warp == kSoft + 1) {
+    const int u = warp - kSoft, tiles = two ? n : (n - u + 1) / 2;
+    if (lane == 0 && tiles > 0) {  // issuer of stream u
+      const uint32_t rb = smem_u32(ring), q = smem_u32(smem) + (two ? u * C::QB : 0);
+      const uint32_t s_to = tmem + (C::SHARED ? 0 : u * KT), p_from = tmem + C::P0 + u * (KT / 2), o_to = tmem + C::O0 + u * DH;
       constexpr uint32_t id_s = idesc_16bit(BF16, 128, KT, false), id_o = idesc_16bit(BF16, 128, DH, true);
       auto landed = [&](int p) { return mbar_wait(&full[p % ST], (p / ST) & 1, abort_flag); };
-      auto scores = [&](int u, int i) {  // stream u, key tile i
-        const uint32_t k = rb + k_at(i) % ST * C::SB, q = qb + (two ? u * C::QB : 0);
+      auto tile_of = [&](int c) { return two ? c : 2 * c + u; };
+      auto scores = [&](int c) {
+        const int p = k_at(tile_of(c));
+        ok = ok && landed(p);
+        // the buffer: the other stream took its scores before (this tile's, or the last one's), or this one
+        if (C::SHARED) {
+          if (c + u > 0) ok = ok && mbar_wait(&s_free[1 - u], (c - 1 + u) & 1, abort_flag);
+        } else if (c > 0) {
+          ok = ok && mbar_wait(&s_free[u], (c - 1) & 1, abort_flag);
+        }
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t k = rb + p % ST * C::SB;
 #pragma unroll
         for (int ks = 0; ks < T::KSTEPS; ++ks)
-          mma_f16_ss(tmem + u * KT, T::k_major(q, 128, ks), T::k_major(k, KT, ks), id_s, ks > 0);
+          mma_f16_ss(s_to, T::k_major(q, 128, ks), T::k_major(k, KT, ks), id_s, ks > 0);
         mma_commit(&s_full[u]);
+        mma_commit(&empty[p % ST]);
       };
-      auto values = [&](int u, int i, bool add) {
-        const uint32_t v = rb + v_at(i) % ST * C::SB;
+      ok = mbar_wait(&q_full[two ? u : 0], 0, abort_flag);
+      scores(0);
+      for (int c = 0; c < tiles && ok; ++c) {
+        if (c + 1 < tiles) scores(c + 1);
+        const int i = tile_of(c), p = v_at(i);
+        ok = ok && landed(p) && (!a.masked || mbar_wait(&clean[i % kClean], (i / kClean) & 1, abort_flag)) &&
+             mbar_wait(&p_full[u], c & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t v = rb + p % ST * C::SB;
 #pragma unroll
         for (int k = 0; k < KT / 16; ++k)
-          mma_f16_ts(tmem + C::O0 + u * DH, tmem + u * KT + k * 8, T::mn_major(v, KT, k), id_o, add || k > 0);
+          mma_f16_ts(o_to, p_from + k * 8, T::mn_major(v, KT, k), id_o, c > 0 || k > 0);
         mma_commit(&o_full[u]);
-      };
-      auto clean_v = [&](int i) {
-        return landed(v_at(i)) && (!a.masked || mbar_wait(&clean[i % kClean], (i / kClean) & 1, abort_flag));
-      };
-      ok = mbar_wait(&q_full[0], 0, abort_flag) && (!two || mbar_wait(&q_full[1], 0, abort_flag));
-      if (two) {
-        ok = ok && landed(0);
-        if (ok) {
-          tc_fence_after();
-          scores(0, 0);
-          scores(1, 0);
-          mma_commit(&empty[0]);
-        }
-        for (int i = 0; i < n && ok; ++i)
-          for (int u = 0; u < 2 && ok; ++u) {
-            ok = mbar_wait(&p_full[u], i & 1, abort_flag) && (u > 0 || clean_v(i));
-            if (!ok) break;
-            tc_fence_after();
-            values(u, i, i > 0);
-            if (u == 1) mma_commit(&empty[v_at(i) % ST]);
-            if (i + 1 < n) {
-              ok = u > 0 || landed(k_at(i + 1));
-              if (!ok) break;
-              tc_fence_after();
-              scores(u, i + 1);
-              if (u == 1) mma_commit(&empty[k_at(i + 1) % ST]);
-            }
-          }
-      } else {
-        auto next = [&](int i) {
-          ok = ok && landed(k_at(i));
-          if (!ok) return;
-          tc_fence_after();
-          scores(i & 1, i);
-          mma_commit(&empty[k_at(i) % ST]);
-        };
-        next(0);
-        if (n > 1) next(1);
-        for (int i = 0; i < n && ok; ++i) {
-          const int u = i & 1;
-          ok = mbar_wait(&p_full[u], (i >> 1) & 1, abort_flag) && clean_v(i);
-          if (!ok) break;
-          tc_fence_after();
-          values(u, i, i > 1);
-          mma_commit(&empty[v_at(i) % ST]);
-          if (i + 2 < n) next(i + 2);
-        }
+        mma_commit(&empty[p % ST]);
       }
       if (!ok) {
         give_up(SB_ERR_TIMEOUT_FULL);
-        mma_commit(dbar);
-        bounded_wait(dbar, 0);
+        mma_commit(&dbar[u]);
+        bounded_wait(&dbar[u], 0);
       }
     }
-  } else if (warp == 10) {
-    if (a.masked) {  // cleaner
+  } else if (warp == kSoft + 3) {
+    if (a.masked) {  // cleaner, its mask bytes two tiles ahead
+      uint32_t next[2][KT / 32];
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int x = 0; x < KT / 32; ++x) next[y][x] = a.mask.ask(b, (first + y) * KT + 32 * x, count);
+#pragma unroll 2
       for (int i = 0; i < n; ++i) {
         const int p = v_at(i), j0 = (first + i) * KT;
         uint8_t* v = ring + p % ST * C::SB;
+        uint32_t w[KT / 32];
+#pragma unroll
+        for (int x = 0; x < KT / 32; ++x) {
+          w[x] = a.mask.told(next[i & 1][x], j0 + 32 * x, count);
+          next[i & 1][x] = a.mask.ask(b, j0 + 2 * KT + 32 * x, count);
+        }
         if (!warp_wait(&full[p % ST], (p / ST) & 1, abort_flag)) {
           if (lane == 0) give_up(SB_ERR_TIMEOUT_FULL);
           break;
         }
         bool touched = false;
-#pragma unroll 1
+#pragma unroll
         for (int x = 0; x < KT / 32; ++x) {
-          const uint32_t w = a.mask.word(b, j0 + 32 * x, count);
-          if (w == 0xFFFFFFFFu) continue;
+          if (w[x] == 0xFFFFFFFFu) continue;
           touched = true;
-          if (!(w >> lane & 1u))
+          if (!(w[x] >> lane & 1u))
             for (int c = 0; c < DH / 8; ++c)
               *reinterpret_cast<uint4*>(v + T::chunk(KT, 32 * x + lane, c)) = make_uint4(0, 0, 0, 0);
         }
         if (touched) fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&clean[i % kClean]);
+        warp_arrive(&clean[i % kClean]);
       }
     }
   } else {
@@ -298,119 +294,132 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __half*>(a.q.p) + b * a.q.img + tq * a.q.row +
                                                         (long long)h * DH);
       uint8_t* dst = smem + t * C::QB;
-#pragma unroll 8
-      for (int c = 0; c < DH / 8; ++c)
-        *reinterpret_cast<uint4*>(dst + T::chunk(128, quad * 32 + lane, c)) =
-            r < a.rows ? src[c] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = hf * (DH / 16); c < (hf + 1) * (DH / 16); ++c)
+        *reinterpret_cast<uint4*>(dst + T::chunk(128, lr, c)) = r < a.rows ? src[c] : make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[t]);
+      warp_arrive(&q_full[t]);
     }
     const float slack = 8.f / sl;
     const uint64_t sl2 = pair2(sl, sl);
-    for (int i = 0; i < mine; ++i) {
-      const int j0 = (first + (two ? i : 2 * i + t)) * KT;
-      uint32_t w[KT / 32];
-      bool all = true;
-#pragma unroll
-      for (int x = 0; x < KT / 32; ++x) {
-        w[x] = a.mask.word(b, j0 + 32 * x, count);
-        all = all && w[x] == 0xFFFFFFFFu;
+    const int jstep = two ? KT : 2 * KT;
+    int j0 = (first + (two ? 0 : t)) * KT + hf * 64;
+    uint32_t b0 = a.mask.ask(b, j0, count), b1 = a.mask.ask(b, j0 + 32, count);
+    // A warp whose wait failed goes on to the next barrier with its partner, which then leaves too.
+    for (int i = 0; i < mine; ++i, j0 += jstep) {
+      const uint32_t w0 = a.mask.told(b0, j0, count), w1 = a.mask.told(b1, j0 + 32, count);
+      b0 = a.mask.ask(b, j0 + jstep, count);
+      b1 = a.mask.ask(b, j0 + jstep + 32, count);
+      ok = ok && warp_wait(&s_full[t], i & 1, abort_flag);
+      if (!some) {  // P of lanes without rows is never looked at
+        if (!ok) break;
+        warp_arrive(&s_free[t]);
+        ok = i == 0 || warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
+        if (!ok) break;
+        warp_arrive(&p_full[t]);
+        continue;
       }
-      ok = warp_wait(&s_full[t], i & 1, abort_flag);
-      if (!ok) break;
       tc_fence_after();
-      if (some) {
-        uint32_t s[KT];
-#pragma unroll
-        for (int x = 0; x < KT / 32; ++x) tmem_ld32(s_at + 32 * x, s + 32 * x);
-        tmem_ld_wait();
-        if (!all) {
-#pragma unroll
-          for (int j = 0; j < KT; ++j)
-            if (!(w[j >> 5] >> (j & 31) & 1u)) s[j] = 0xFF800000u;  // -inf
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int j = 0; j < KT; j += 2)
-          mx[j / 2 & 3] = max3(mx[j / 2 & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-        const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-        if (i == 0) {
-          m = top;  // nothing accumulated yet
-        } else if (__any_sync(0xFFFFFFFFu, !(top <= m + slack))) {  // also for NaN
-          ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const float mn = max3(m, top, top);
-          const float c = m == mn ? 1.f : exp2_hw((m - mn) * sl);
-          m = mn;
-          l *= c;
-#pragma unroll
-          for (int x = 0; x < DH / 16; ++x) {
-            uint32_t o[16];
-            tmem_ld16(o_at + 16 * x, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * c);
-            tmem_st16(o_at + 16 * x, o);
-          }
-        }
-        const float ms = m == -INFINITY ? 0.f : -m * sl;
-        const uint64_t ms2 = pair2(ms, ms);
-        uint64_t sum[2] = {0, 0};
-        if (all) {
-#pragma unroll
-          for (int x = 0; x < KT / 32; ++x) {
-            uint32_t pk[16];
-            probabilities<DH, BF16, true>(s + 32 * x, sl2, ms2, sum, pk);
-            tmem_st16(s_at + 16 * x, pk);
-          }
-        } else {  // -inf in masked places must give an exact zero: no polynomial
-#pragma unroll
-          for (int x = 0; x < KT / 32; ++x) {
-            uint32_t pk[16];
-            probabilities<DH, BF16, false>(s + 32 * x, sl2, ms2, sum, pk);
-            tmem_st16(s_at + 16 * x, pk);
-          }
-        }
-        float s0, s1;
-        split2(add2(sum[0], sum[1]), s0, s1);
-        l += s0 + s1;
-        tmem_st_wait();
-      }
+      uint32_t s[64];
+      tmem_ld32(s_at, s);
+      tmem_ld32(s_at + 32, s + 32);
+      tmem_ld_wait();
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
+      warp_arrive(&s_free[t]);
+      if ((w0 & w1) != 0xFFFFFFFFu) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+          if (!((j < 32 ? w0 : w1) >> (j & 31) & 1u)) s[j] = 0xFF800000u;  // -inf
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < 64; j += 2)
+        mx[j / 2 & 3] = max3(mx[j / 2 & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+      float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+      // a new reference point: with the first tile, and where the maximum grew (or is NaN)
+      const bool grew = pair_or(bar_id, !ok || i == 0 || !(top <= m + slack));
+      float c = 1.f;
+      if (grew) {
+        if (hf == 1) *tell = top;
+        if (pair_or(bar_id, !ok)) {
+          ok = false;
+          break;
+        }
+        if (hf == 0) *tell = top = max3(top, *tell, m);
+        pair_or(bar_id, false);
+        if (hf == 1) top = *tell;
+        c = m == top ? 1.f : exp2_hw((m - top) * sl);
+        m = top;
+        l *= c;
+      }
+      // masked scores give 2^-126 at most on the polynomial path: their V is zero, and a row whose
+      // reference is still -inf at the end has no keys
+      const float ms = m == -INFINITY ? 0.f : -m * sl;
+      const uint64_t ms2 = pair2(ms, ms);
+      uint64_t sum[2] = {0, 0};
+      uint32_t pk[16];
+      probabilities<DH, BF16>(s, sl2, ms2, sum, pk);
+      // the last tile's product has read its P and added to O
+      if (i > 0) ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
+      tc_fence_after();
+      if (grew && i > 0) {
+#pragma unroll
+        for (int y = 0; y < DH / 32; ++y) {
+          uint32_t o[16];
+          tmem_ld16(o_at + 16 * y, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * c);
+          tmem_st16(o_at + 16 * y, o);
+        }
+      }
+      tmem_st16(p_at, pk);
+      probabilities<DH, BF16>(s + 32, sl2, ms2, sum, pk);
+      tmem_st16(p_at + 16, pk);
+      float s0, s1;
+      split2(add2(sum[0], sum[1]), s0, s1);
+      l += s0 + s1;
+      tmem_st_wait();
+      tc_fence_before();
+      if (ok) warp_arrive(&p_full[t]);
     }
     if (ok && mine > 0) ok = warp_wait(&o_full[t], (mine - 1) & 1, abort_flag);
     if (!ok && lane == 0) give_up(SB_ERR_TIMEOUT_ACC);
     tc_fence_after();
+    if (some) {  // the row's sum
+      pair_or(bar_id, false);
+      if (hf == 1) *tell = l;
+      pair_or(bar_id, false);
+      if (hf == 0) *tell = l += *tell;
+      pair_or(bar_id, false);
+      if (hf == 1) l = *tell;
+      if (m == -INFINITY) l = 0.f;
+    }
   }
 
   float m1 = -INFINITY, l1 = 0.f;  // of the other stream on the same rows
   float4* other = reinterpret_cast<float4*>(smem);  // [128][DH / 4] its O, in the queries' place
   constexpr int per = DH / 4;
-  const int lr = quad * 32 + lane;
   const bool join = !two && n > 1;
   if (join) {
     __syncthreads();  // both streams' products are done: the queries are no longer read
-    if (warp >= 4 && warp < 8 && some && ok) {
-      ml[lr] = make_float2(m, l);
+    if (t == 1 && some && !*abort_flag) {
+      if (hf == 0) ml[lr] = make_float2(m, l);
 #pragma unroll
-      for (int x = 0; x < DH / 16; ++x) {
+      for (int x = 0; x < DH / 32; ++x) {
         uint32_t o[16];
         tmem_ld16(o_at + 16 * x, o);
         tmem_ld_wait();
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          other[lr * per + ((4 * x + c) ^ (lr & 7))] =
+          other[lr * per + ((hf * (DH / 8) + 4 * x + c) ^ (lr & 7))] =
               make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
                           __uint_as_float(o[4 * c + 3]));
       }
     }
     __syncthreads();
   }
-  if (warp < (two ? 8 : 4) && some && !*abort_flag) {
+  if (some && (two || t == 0) && !*abort_flag) {
     float w0 = 1.f, w1 = 0.f;
     if (join) {
       m1 = ml[lr].x;
@@ -428,7 +437,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const long long rr = ((long long)b * a.H + h) * a.Tq + tq;
     const bool live = r < a.rows;
 #pragma unroll
-    for (int x = 0; x < DH / 16; ++x) {
+    for (int x = 0; x < DH / 32; ++x) {
+      const int col = hf * (DH / 2) + 16 * x;
       uint32_t o[16];
       float f[16];
       __syncwarp();
@@ -442,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (join) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float4 e = other[lr * per + ((4 * x + c) ^ (lr & 7))];
+          const float4 e = other[lr * per + ((hf * (DH / 8) + 4 * x + c) ^ (lr & 7))];
           f[4 * c] = fmaf(e.x, w1, f[4 * c]);
           f[4 * c + 1] = fmaf(e.y, w1, f[4 * c + 1]);
           f[4 * c + 2] = fmaf(e.z, w1, f[4 * c + 2]);
@@ -450,26 +460,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (a.splits > 1) {
-        float4* dst = reinterpret_cast<float4*>(a.part_o + (split * a.all_rows + rr) * DH + 16 * x);
+        float4* dst = reinterpret_cast<float4*>(a.part_o + (split * a.all_rows + rr) * DH + col);
 #pragma unroll
         for (int j = 0; j < 4; ++j) dst[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
       } else {
         uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(a.o.p) + b * a.o.img + tq * a.o.row +
-                                              (long long)h * DH + 16 * x);
+                                              (long long)h * DH + col);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           dst[j] = make_uint4(pack16<BF16>(f[8 * j], f[8 * j + 1]), pack16<BF16>(f[8 * j + 2], f[8 * j + 3]),
                               pack16<BF16>(f[8 * j + 4], f[8 * j + 5]), pack16<BF16>(f[8 * j + 6], f[8 * j + 7]));
       }
     }
-    if (live) {
+    if (live && hf == 0) {
       if (a.splits > 1) a.part_l[split * a.all_rows + rr] = n > 0 ? lse : -INFINITY;
       else if (a.lse) a.lse[rr] = n > 0 ? lse : -INFINITY;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kSoft) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

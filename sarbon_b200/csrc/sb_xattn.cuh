@@ -21,15 +21,19 @@ struct KeyMask {
   long long valid_img;
   int Tk;
   SB_DEV int count(int b) const { return lens ? min(max(lens[b], 0), Tk) : Tk; }
+  // word() in two steps, so that a tile's bytes are on their way while another tile is worked on
+  SB_DEV uint32_t ask(int b, int j0, int n) const {
+    const int j = j0 + (int)lane_id();
+    return valid && j < n ? valid[b * valid_img + j] : 1u;
+  }
+  SB_DEV uint32_t told(uint32_t byte, int j0, int n) const {
+    const int left = n - j0;
+    const uint32_t w = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
+    return valid ? w & __ballot_sync(0xFFFFFFFFu, byte != 0) : w;
+  }
   // bit i of the result: key j0 + i takes part (whole warp; n = count(b))
   SB_DEV uint32_t word(int b, int j0, int n) const {
-    const int left = n - j0;
-    uint32_t w = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
-    if (valid) {
-      const int j = j0 + (int)lane_id();
-      w &= __ballot_sync(0xFFFFFFFFu, j < n && valid[b * valid_img + j] != 0);
-    }
-    return w;
+    return told(ask(b, j0, n), j0, n);
   }
 };
 
@@ -124,6 +128,28 @@ SB_DEV float exp2_hw(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// One arrival for a warp.  The barrier after it matters: without it lanes 1 .. 31 may run ahead into the
+// next wait, which suspends the warp for its whole time limit before lane 0 gets to arrive.
+SB_DEV void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if (lane_id() == 0) mbar_arrive(bar);
+  __syncwarp();
+}
+
+// Barrier `id` (1 ..) of 64 threads, two warps, with the OR of their predicates.
+SB_DEV bool pair_or(int id, bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred.aligned q, %2, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)p), "r"(id)
+      : "memory");
+  return r != 0;
 }
 
 // ---------------------------------------------------------------- operand tiles in shared memory

@@ -282,8 +282,7 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
               *reinterpret_cast<uint4*>(ring + st * C::SB + T::chunk(kStep, 32 * x + lane, c)) = make_uint4(0, 0, 0, 0);
         }
         if (touched) fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&clean[st]);
+        warp_arrive(&clean[st]);
       }
     }
   } else {
@@ -305,8 +304,7 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
         *reinterpret_cast<uint4*>(smem + u * C::XB + T::chunk(128, quad * 32 + lane, c)) =
             live ? from[c] : make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(x_full);
+      warp_arrive(x_full);
     }
     // P is held as 2^lift P, dS as F dS with F = f 2^lift
     constexpr float lift = BF16 ? 0.f : 14.f;
@@ -382,8 +380,7 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
       }
       tmem_st_wait();
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[u]);
+      warp_arrive(&p_full[u]);
     }
     if (ok && n > 0) ok = warp_wait(acc_full, 0, abort_flag);
     if (!ok) {
