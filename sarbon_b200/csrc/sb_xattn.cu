@@ -9,23 +9,26 @@
 //   two tiles of rows left   a tile a stream, both over every key tile
 //   one                      both streams on it, over alternate key tiles, joined at the end (a token
 //                            a stream, and the last tile of an odd number)
-//   loader warp   K and V tiles by TMA into one ring, in the order in which they are used
+//   loader warp   K and V tiles by TMA into a ring each, in the order in which they are used.  A stage's
+//                 barrier is only ever waited for by roles that see each of its uses (a parity says
+//                 nothing about a use before the last): K apart from V, and an even number of
+//                 stages, so that alternate tiles keep to their stream's
 //   issuer warps  S_t = Q_t K^T (operands in shared memory); O_t += P_t V with P_t in TMEM as the A
 //                 operand.  One a stream: a wait on a barrier costs an issuer a few hundred clocks, in
 //                 which the other one keeps the tensor pipe fed
 //   8 warps a stream  two threads a query row, 64 keys each (one thread a row left two warps a
 //                 scheduler, too few to cover the arithmetic's latency): scores from TMEM into registers
-//                 at once, so that the next tile's are computed meanwhile (one buffer for both
-//                 streams with 128 channels, which the accumulators leave no room beside; one each
-//                 below); P = 2^(s scale log2 e - m), rounded to the operands' type, back to TMEM.  The
+//                 at once; P = 2^(s scale log2 e - m), rounded to the operands' type, back to TMEM.  Below
+//                 128 channels P has its own columns, so that the next tile's scores are computed
+//                 meanwhile; with 128 the accumulators leave room for P over the scores only.  The
 //                 reference point m moves, and O is rescaled, only when a row's maximum grew by more
 //                 than 2^8 since the last time (P stays below 2^8, far from fp16's limit; m cancels in
 //                 O / l), so the two threads need each other's maximum only then: otherwise one barrier
 //                 with the OR of "grew" is all that a tile costs them
 //   cleaner warp  with masks: zeroes V's rows of keys that take no part (0 x NaN is NaN), before
 //                 the product reads them
-// The exponentials bound heads of few channels (16 a clock and SM): there, part of them runs as a
-// polynomial on the FMA pipe.  The rest of a row's arithmetic works on pairs.
+// The exponentials (16 a clock and SM) are the floor of heads of few channels; the rest of a row's
+// arithmetic works on pairs.  A polynomial for part of them was slower: the issue slots are as scarce.
 // The key range is split over CTAs where the rows alone leave SMs idle: these write fp32 partial rows
 // with their L, and a second kernel joins them.
 #include <algorithm>
@@ -56,7 +59,6 @@ struct FwdArgs {
 };
 
 constexpr int KT = 128;      // keys a tile
-constexpr int kClean = 8;    // more V tiles than the ring can hold at once
 constexpr int kSoft = 16;     // softmax warps: stream (w / 8), half of a tile's keys (w / 4 % 2), TMEM lanes (w % 4)
 constexpr int kThreads = (kSoft + 4) * 32;
 
@@ -65,30 +67,23 @@ struct Fwd {
   static constexpr int QB = Tile<DH>::bytes(128);  // a tile of queries
   static constexpr int SB = Tile<DH>::bytes(KT);   // a stage: one K or V tile
   static constexpr int ROOM = 224 * 1024 - 2 * QB;
-  static constexpr int STAGES = ROOM / SB < 8 ? ROOM / SB : 8;
-  static constexpr int SMEM = 1024 + 2 * QB + STAGES * SB + 512 + 1024;
-  // TMEM columns: scores (shared by the streams or one each), P, accumulators
-  static constexpr bool SHARED = DH == 128;
-  static constexpr int P0 = SHARED ? KT : 2 * KT, O0 = P0 + KT;
-  static_assert(STAGES >= 5 && O0 + 2 * DH <= 512, "ring and TMEM");
-  // pairs of exponentials out of 16 that take the polynomial
-  static constexpr int POLY = DH == 128 ? 0 : 5;
+  static constexpr int STAGES = ROOM / (2 * SB) < 6 ? ROOM / (2 * SB) / 2 * 2 : 6;  // of each ring
+  static constexpr int SMEM = 1024 + 2 * QB + 2 * STAGES * SB + 512 + 1024;
+  // TMEM columns: scores of the streams, P (over the scores or after them), accumulators
+  static constexpr bool OVER = DH == 128;
+  static constexpr int P0 = OVER ? 0 : 2 * KT, PSTEP = OVER ? KT : KT / 2, O0 = OVER ? 2 * KT : 3 * KT;
+  static_assert(STAGES >= 2 && STAGES % 2 == 0 && O0 + 2 * DH <= 512, "rings and TMEM");
 };
 
-// P of 32 columns: 2^(s sl - ms), their sum added to `sum`, rounded into 16 words
-template <int DH, bool BF16>
+// P of 32 columns: 2^(s sl + ms), their sum added to `sum`, rounded into 16 words
+template <bool BF16>
 SB_DEV void probabilities(const uint32_t* s, uint64_t sl, uint64_t ms, uint64_t (&sum)[2], uint32_t (&pk)[16]) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
-    const uint64_t x = fma2(pair2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), sl, ms);
     float a, b;
-    if ((j * Fwd<DH>::POLY) % 16 < Fwd<DH>::POLY) {
-      exp2_poly(x, a, b);
-    } else {
-      split2(x, a, b);
-      a = exp2_hw(a);
-      b = exp2_hw(b);
-    }
+    split2(fma2(pair2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), sl, ms), a, b);
+    a = exp2_hw(a);
+    b = exp2_hw(b);
     sum[j & 1] = add2(sum[j & 1], pair2(a, b));
     pk[j] = pack16<BF16>(a, b);
   }
@@ -104,10 +99,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + 2 * C::QB;
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + ST * C::SB);
-  uint64_t* empty = full + ST;
-  uint64_t* clean = empty + ST;       // [kClean]
-  uint64_t* q_full = clean + kClean;  // [2] each, a stream
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(ring + 2 * ST * C::SB);  // [ST] each, K stages before V stages
+  uint64_t* v_full = k_full + ST;
+  uint64_t* k_empty = v_full + ST;
+  uint64_t* v_empty = k_empty + ST;
+  uint64_t* clean = v_empty + ST;  // V tile ready for its product (with masks)
+  uint64_t* q_full = clean + ST;   // [2] each, a stream
   uint64_t* s_full = q_full + 2;      // scores computed
   uint64_t* s_free = s_full + 2;      // scores taken into registers
   uint64_t* p_full = s_free + 2;
@@ -117,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   // what threads of a row tell each other: [stream][row] a maximum or a sum; at the end [row] both of the
   // second stream's
-  float* told = reinterpret_cast<float*>(ring + ST * C::SB + 512);
+  float* told = reinterpret_cast<float*>(ring + 2 * ST * C::SB + 512);
   float2* ml = reinterpret_cast<float2*>(told);
   const int warp = warp_id(), lane = lane_id();
 
@@ -132,18 +129,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int each = (a.key_tiles + a.splits - 1) / a.splits;
   const int first = split * each;
   const int n = max(0, min(min(first + each, a.key_tiles), (count + KT - 1) / KT) - first);
-  // a stream's scores are a tile before its values: the ring holds K0 .. K(ahead - 1) V0 K(ahead) V1 ...;
-  // the places of K and V tile i
-  const int ahead = two ? 2 : 4;
-  auto k_at = [&](int i) { return i + max(0, i - ahead + 1); };
-  auto v_at = [&](int i) { return i + min(n, i + ahead); };
+  // a stream's scores are a tile before its values, or follow the last tile's: tiles are loaded in the
+  // order K0 .. K(ahead - 1) V0 K(ahead) V1 ...
+  const int ahead = (C::OVER ? 1 : 2) * (two ? 1 : 2);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], two ? 2 : 1);  // the streams that read a tile
+      mbar_init(&k_full[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&k_empty[i], two ? 2 : 1);  // the streams that read a tile
+      mbar_init(&v_empty[i], two ? 2 : 1);
+      mbar_init(&clean[i], 1);
     }
-    for (int i = 0; i < kClean; ++i) mbar_init(&clean[i], 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], kSoft / 2);
       mbar_init(&s_full[t], 1);
@@ -177,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tq = r / a.group, h = kvh * a.group + (r - tq * a.group);
   const int mine = two ? n : (n - t + 1) / 2;  // key tiles of the stream
   const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-  const uint32_t s_at = tmem + lanes + (C::SHARED ? 0 : t * KT) + hf * 64, p_at = tmem + lanes + C::P0 + t * (KT / 2) + hf * 32;
+  const uint32_t s_at = tmem + lanes + t * KT + hf * 64, p_at = tmem + lanes + C::P0 + t * C::PSTEP + hf * 32;
   const uint32_t o_at = tmem + lanes + C::O0 + t * DH + hf * (DH / 2);
   const int bar_id = 1 + t * 4 + quad;  // of the two warps of these rows
   float* tell = told + t * 128 + lr;
@@ -189,65 +186,66 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {  // loader
       prefetch_tmap(&kmap);
       prefetch_tmap(&vmap);
-      int p = 0, ki = 0, vi = 0;
-      for (; p < 2 * n; ++p) {
-        const int st = p % ST;
-        if (p >= ST && !mbar_wait(&empty[st], ((p / ST) - 1) & 1, abort_flag)) {
+      int ki = 0, vi = 0;
+      while (vi < n) {
+        const bool v = ki == min(n, vi + ahead);
+        const int i = v ? vi : ki, st = i % ST;
+        if (i >= ST && !mbar_wait(v ? &v_empty[st] : &k_empty[st], ((i / ST) - 1) & 1, abort_flag)) {
           give_up(SB_ERR_TIMEOUT_EMPTY);
           break;
         }
-        mbar_arrive_expect_tx(&full[st], C::SB);
-        const bool v = ki == min(n, vi + ahead);
-        const int i = v ? vi++ : ki++;
+        uint64_t* bar = v ? &v_full[st] : &k_full[st];
+        mbar_arrive_expect_tx(bar, C::SB);
         const CUtensorMap* map = v ? &vmap : &kmap;
+        uint8_t* dst = ring + (v ? ST + st : st) * C::SB;
         const int item = b * (v ? a.v_item : a.k_item);
         for (int x = 0; x < T::BOXES; ++x)
-          tma_load_4d(ring + st * C::SB + x * T::box_bytes(KT), map, &full[st], x * T::COLS, (first + i) * KT, kvh, item);
+          tma_load_4d(dst + x * T::box_bytes(KT), map, bar, x * T::COLS, (first + i) * KT, kvh, item);
+        if (v) ++vi;
+        else ++ki;
       }
-      if (*abort_flag)
-        for (int i = max(0, p - ST); i < p; ++i) bounded_wait(&full[i % ST], (i / ST) & 1);
+      if (*abort_flag) {
+        for (int i = max(0, ki - ST); i < ki; ++i) bounded_wait(&k_full[i % ST], (i / ST) & 1);
+        for (int i = max(0, vi - ST); i < vi; ++i) bounded_wait(&v_full[i % ST], (i / ST) & 1);
+      }
     }
   } else if (warp == kSoft || warp == kSoft + 1) {
     const int u = warp - kSoft, tiles = two ? n : (n - u + 1) / 2;
     if (lane == 0 && tiles > 0) {  // issuer of stream u
       const uint32_t rb = smem_u32(ring), q = smem_u32(smem) + (two ? u * C::QB : 0);
-      const uint32_t s_to = tmem + (C::SHARED ? 0 : u * KT), p_from = tmem + C::P0 + u * (KT / 2), o_to = tmem + C::O0 + u * DH;
+      const uint32_t s_to = tmem + u * KT, p_from = tmem + C::P0 + u * C::PSTEP, o_to = tmem + C::O0 + u * DH;
       constexpr uint32_t id_s = idesc_16bit(BF16, 128, KT, false), id_o = idesc_16bit(BF16, 128, DH, true);
-      auto landed = [&](int p) { return mbar_wait(&full[p % ST], (p / ST) & 1, abort_flag); };
+      auto ready = [&](uint64_t* bars, int i) { return mbar_wait(&bars[i % ST], (i / ST) & 1, abort_flag); };
       auto tile_of = [&](int c) { return two ? c : 2 * c + u; };
       auto scores = [&](int c) {
-        const int p = k_at(tile_of(c));
-        ok = ok && landed(p);
-        // the buffer: the other stream took its scores before (this tile's, or the last one's), or this one
-        if (C::SHARED) {
-          if (c + u > 0) ok = ok && mbar_wait(&s_free[1 - u], (c - 1 + u) & 1, abort_flag);
-        } else if (c > 0) {
-          ok = ok && mbar_wait(&s_free[u], (c - 1) & 1, abort_flag);
-        }
+        const int i = tile_of(c);
+        ok = ok && ready(k_full, i);
+        // the last tile's scores have been taken (P over them: and its values are issued)
+        if (!C::OVER && c > 0) ok = ok && mbar_wait(&s_free[u], (c - 1) & 1, abort_flag);
         if (!ok) return;
         tc_fence_after();
-        const uint32_t k = rb + p % ST * C::SB;
+        const uint32_t k = rb + i % ST * C::SB;
 #pragma unroll
         for (int ks = 0; ks < T::KSTEPS; ++ks)
           mma_f16_ss(s_to, T::k_major(q, 128, ks), T::k_major(k, KT, ks), id_s, ks > 0);
         mma_commit(&s_full[u]);
-        mma_commit(&empty[p % ST]);
+        mma_commit(&k_empty[i % ST]);
       };
       ok = mbar_wait(&q_full[two ? u : 0], 0, abort_flag);
       scores(0);
       for (int c = 0; c < tiles && ok; ++c) {
-        if (c + 1 < tiles) scores(c + 1);
-        const int i = tile_of(c), p = v_at(i);
-        ok = ok && landed(p) && (!a.masked || mbar_wait(&clean[i % kClean], (i / kClean) & 1, abort_flag)) &&
-             mbar_wait(&p_full[u], c & 1, abort_flag);
+        if (!C::OVER && c + 1 < tiles) scores(c + 1);
+        const int i = tile_of(c);
+        ok = ok && ready(v_full, i) && (!a.masked || ready(clean, i)) && mbar_wait(&p_full[u], c & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t v = rb + p % ST * C::SB;
+        const uint32_t v = rb + (ST + i % ST) * C::SB;
 #pragma unroll
         for (int k = 0; k < KT / 16; ++k)
           mma_f16_ts(o_to, p_from + k * 8, T::mn_major(v, KT, k), id_o, c > 0 || k > 0);
-        mma_commit(&o_full[u]);
-        mma_commit(&empty[p % ST]);
+        if (!C::OVER || c + 1 == tiles) mma_commit(&o_full[u]);  // OVER: the next scores say it of the others
+        mma_commit(&v_empty[i % ST]);
+        if (C::OVER && c + 1 < tiles) scores(c + 1);
       }
       if (!ok) {
         give_up(SB_ERR_TIMEOUT_FULL);
@@ -264,15 +262,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int x = 0; x < KT / 32; ++x) next[y][x] = a.mask.ask(b, (first + y) * KT + 32 * x, count);
 #pragma unroll 2
       for (int i = 0; i < n; ++i) {
-        const int p = v_at(i), j0 = (first + i) * KT;
-        uint8_t* v = ring + p % ST * C::SB;
+        const int j0 = (first + i) * KT;
+        uint8_t* v = ring + (ST + i % ST) * C::SB;
         uint32_t w[KT / 32];
 #pragma unroll
         for (int x = 0; x < KT / 32; ++x) {
           w[x] = a.mask.told(next[i & 1][x], j0 + 32 * x, count);
           next[i & 1][x] = a.mask.ask(b, j0 + 2 * KT + 32 * x, count);
         }
-        if (!warp_wait(&full[p % ST], (p / ST) & 1, abort_flag)) {
+        if (!warp_wait(&v_full[i % ST], (i / ST) & 1, abort_flag)) {
           if (lane == 0) give_up(SB_ERR_TIMEOUT_FULL);
           break;
         }
@@ -286,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               *reinterpret_cast<uint4*>(v + T::chunk(KT, 32 * x + lane, c)) = make_uint4(0, 0, 0, 0);
         }
         if (touched) fence_proxy_async_smem();
-        warp_arrive(&clean[i % kClean]);
+        warp_arrive(&clean[i % ST]);
       }
     }
   } else {
@@ -313,8 +311,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && warp_wait(&s_full[t], i & 1, abort_flag);
       if (!some) {  // P of lanes without rows is never looked at
         if (!ok) break;
-        warp_arrive(&s_free[t]);
-        ok = i == 0 || warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
+        if (!C::OVER) warp_arrive(&s_free[t]);
+        ok = C::OVER || i == 0 || warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
         if (!ok) break;
         warp_arrive(&p_full[t]);
         continue;
@@ -325,11 +323,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld32(s_at + 32, s + 32);
       tmem_ld_wait();
       tc_fence_before();
-      warp_arrive(&s_free[t]);
+      if (!C::OVER) warp_arrive(&s_free[t]);
       if ((w0 & w1) != 0xFFFFFFFFu) {
+        // 16 keys at a time: masks of images and lengths leave most groups whole
 #pragma unroll
-        for (int j = 0; j < 64; ++j)
-          if (!((j < 32 ? w0 : w1) >> (j & 31) & 1u)) s[j] = 0xFF800000u;  // -inf
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t g = (x < 2 ? w0 : w1) >> (16 * (x & 1)) & 0xFFFFu;
+          if (g == 0xFFFFu) continue;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (!(g >> j & 1u)) s[16 * x + j] = 0xFF800000u;  // -inf
+        }
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -352,16 +356,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         m = top;
         l *= c;
       }
-      // masked scores give 2^-126 at most on the polynomial path: their V is zero, and a row whose
-      // reference is still -inf at the end has no keys
+      // masked scores give 0; a row whose reference is still -inf has had no keys
       const float ms = m == -INFINITY ? 0.f : -m * sl;
       const uint64_t ms2 = pair2(ms, ms);
       uint64_t sum[2] = {0, 0};
       uint32_t pk[16];
-      probabilities<DH, BF16>(s, sl2, ms2, sum, pk);
-      // the last tile's product has read its P and added to O
-      if (i > 0) ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
-      tc_fence_after();
+      probabilities<BF16>(s, sl2, ms2, sum, pk);
+      // the last tile's product has read its P and added to O (OVER: this tile's scores came after it)
+      if (!C::OVER && i > 0) {
+        ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
+        tc_fence_after();
+      }
       if (grew && i > 0) {
 #pragma unroll
         for (int y = 0; y < DH / 32; ++y) {
@@ -374,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       tmem_st16(p_at, pk);
-      probabilities<DH, BF16>(s + 32, sl2, ms2, sum, pk);
+      probabilities<BF16>(s + 32, sl2, ms2, sum, pk);
       tmem_st16(p_at + 16, pk);
       float s0, s1;
       split2(add2(sum[0], sum[1]), s0, s1);
@@ -383,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       if (ok) warp_arrive(&p_full[t]);
     }
-    if (ok && mine > 0) ok = warp_wait(&o_full[t], (mine - 1) & 1, abort_flag);
+    if (ok && mine > 0) ok = warp_wait(&o_full[t], C::OVER ? 0 : (mine - 1) & 1, abort_flag);
     if (!ok && lane == 0) give_up(SB_ERR_TIMEOUT_ACC);
     tc_fence_after();
     if (some) {  // the row's sum

@@ -104,26 +104,6 @@ SB_DEV float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x of a pair on the FMA pipe, beside the special-function unit that bounds a softmax: x = j + f with
-// the integer j nearest to x (added to 1.5 2^23, whose low bits then hold it; Cody and Waite's
-// reduction), a polynomial for 2^f on [-1/2, 1/2] (least relative error at degree four, fitted by Remez
-// exchange: 2.7e-6), and j added to its exponent.  x >= -126 (raised to it).
-SB_DEV void exp2_poly(uint64_t x, float& lo, float& hi) {
-  float a, b, ta, tb;
-  split2(x, a, b);
-  x = pair2(fmaxf(a, -126.f), fmaxf(b, -126.f));
-  const uint64_t t = add2(x, pair2(12582912.f, 12582912.f));
-  const uint64_t f = fma2(add2(t, pair2(-12582912.f, -12582912.f)), pair2(-1.f, -1.f), x);
-  uint64_t r = fma2(f, pair2(0.009570101276f, 0.009570101276f), pair2(0.05591786280f, 0.05591786280f));
-  r = fma2(r, f, pair2(0.2402474433f, 0.2402474433f));
-  r = fma2(r, f, pair2(0.6931217909f, 0.6931217909f));
-  r = fma2(r, f, pair2(0.9999992847f, 0.9999992847f));
-  split2(r, a, b);
-  split2(t, ta, tb);
-  lo = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
-  hi = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
-}
-
 SB_DEV float exp2_hw(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

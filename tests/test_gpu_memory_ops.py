@@ -94,6 +94,7 @@ TYPES = [torch.float16, torch.bfloat16]
     (2, 300, 240, 8, 8, 32), (1, 1, 1, 1, 1, 64), (2, 5, 77, 4, 2, 128), (1, 128, 128, 2, 1, 64),
     (3, 129, 127, 3, 3, 32), (2, 257, 385, 6, 2, 128), (1, 130, 129, 7, 1, 64), (4, 1, 2040, 8, 2, 128),
     (1, 1, 4097, 5, 1, 32), (2, 33, 1000, 12, 4, 64), (1, 513, 64, 2, 2, 128), (1, 3, 9001, 1, 1, 128),
+    (160, 1, 8160, 4, 1, 128), (160, 1, 8160, 1, 1, 64), (80, 300, 5000, 2, 2, 32), (80, 300, 4100, 2, 2, 128),
 ])
 def test_cross_attention(b, tq, tk, heads, kv_heads, dim, dtype):
     import sarbon_b200 as sb
@@ -149,6 +150,27 @@ def test_cross_attention_masks(kind, tq, tk, heads, kv_heads, dim, dtype):
     check_forward(out, lse, q, k, v, heads, kv_heads, lens, valid)
     if kind == "none_left":
         assert not out[0].any() and not out[1].any()
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("tq", [1, 300])
+def test_cross_attention_long_ragged(tq, dim):
+    """Many key tiles a CTA of ragged, masked items: every stage of the rings is used many times."""
+    import sarbon_b200 as sb
+    g = gen(77)
+    b, tk, heads, kv_heads = 160, 6000, 2, 1
+    q = rand(g, b, tq, heads * dim, dtype=torch.bfloat16)
+    kv = rand(g, b, tk, 2 * dim, dtype=torch.bfloat16)
+    lens = torch.randint(0, tk + 1, (b,), device="cuda", generator=g, dtype=torch.int32)
+    valid = torch.rand(b, tk, device="cuda", generator=g) < 0.8
+    lse = torch.empty(b, heads, tq, device="cuda")
+    for masks in ((lens, None), (None, valid), (lens, valid)):
+        out = sb.cross_attention(q, kv[..., :dim], kv[..., dim:], heads, kv_heads=kv_heads, lens=masks[0], valid=masks[1],
+                                 lse=lse)
+        for i in range(0, b, 40):  # forty items at a time
+            at = slice(i, i + 40)
+            check_forward(out[at], lse[at], q[at], kv[at, :, :dim], kv[at, :, dim:], heads, kv_heads,
+                          None if masks[0] is None else masks[0][at], None if masks[1] is None else masks[1][at])
 
 
 def test_cross_attention_strides_and_scale():
