@@ -10,17 +10,17 @@
 //   one                      both streams on it, over alternate key tiles, joined at the end (a token
 //                            a stream, and the last tile of an odd number)
 //   loader warp   K and V tiles by TMA into a ring each, in the order in which they are used.  A stage's
-//                 barrier is only ever waited for by roles that see each of its uses (a parity says
-//                 nothing about a use before the last): K apart from V, and an even number of
-//                 stages, so that alternate tiles keep to their stream's
+//                 barrier is only waited for by roles that see each of its uses (a parity says
+//                 nothing about a use before the last)
 //   issuer warps  S_t = Q_t K^T (operands in shared memory); O_t += P_t V with P_t in TMEM as the A
-//                 operand.  One a stream: a wait on a barrier costs an issuer a few hundred clocks, in
-//                 which the other one keeps the tensor pipe fed
+//                 operand.  With a tile a stream there is an issuer a stream: a wait on a barrier costs
+//                 one a few hundred clocks, in which the other keeps the tensor pipe fed.  Alternate
+//                 tiles have one issuer
 //   8 warps a stream  two threads a query row, 64 keys each (one thread a row left two warps a
 //                 scheduler, too few to cover the arithmetic's latency): scores from TMEM into registers
-//                 at once; P = 2^(s scale log2 e - m), rounded to the operands' type, back to TMEM.  Below
-//                 128 channels P has its own columns, so that the next tile's scores are computed
-//                 meanwhile; with 128 the accumulators leave room for P over the scores only.  The
+//                 at once, so that the next tile's are computed meanwhile (one buffer for both
+//                 streams with 128 channels, which the accumulators leave no room beside; one each
+//                 below); P = 2^(s scale log2 e - m), rounded to the operands' type, back to TMEM.  The
 //                 reference point m moves, and O is rescaled, only when a row's maximum grew by more
 //                 than 2^8 since the last time (P stays below 2^8, far from fp16's limit; m cancels in
 //                 O / l), so the two threads need each other's maximum only then: otherwise one barrier
@@ -66,13 +66,28 @@ template <int DH>
 struct Fwd {
   static constexpr int QB = Tile<DH>::bytes(128);  // a tile of queries
   static constexpr int SB = Tile<DH>::bytes(KT);   // a stage: one K or V tile
-  static constexpr int ROOM = 224 * 1024 - 2 * QB;
-  static constexpr int STAGES = ROOM / (2 * SB) < 6 ? ROOM / (2 * SB) / 2 * 2 : 6;  // of each ring
-  static constexpr int SMEM = 1024 + 2 * QB + 2 * STAGES * SB + 512 + 1024;
-  // TMEM columns: scores of the streams, P (over the scores or after them), accumulators
-  static constexpr bool OVER = DH == 128;
-  static constexpr int P0 = OVER ? 0 : 2 * KT, PSTEP = OVER ? KT : KT / 2, O0 = OVER ? 2 * KT : 3 * KT;
-  static_assert(STAGES >= 2 && STAGES % 2 == 0 && O0 + 2 * DH <= 512, "rings and TMEM");
+  // K and V stages with two tiles of queries and with one
+  static constexpr int ROOM2 = (224 * 1024 - 2 * QB) / SB, ROOM1 = (224 * 1024 - QB) / SB;
+  static constexpr int K2 = ROOM2 < 12 ? (ROOM2 + 1) / 2 : 6, V2 = ROOM2 < 12 ? ROOM2 / 2 : 6;
+  static constexpr int K1 = ROOM1 < 12 ? (ROOM1 + 1) / 2 : 6, V1 = ROOM1 < 12 ? ROOM1 / 2 : 6;
+  static constexpr int TILES = 224 * 1024, SMEM = 1024 + TILES + 512 + 1024;
+  // TMEM columns: scores (shared by the streams or one each), P, accumulators
+  static constexpr bool SHARED = DH == 128;
+  static constexpr int SSTEP = SHARED ? 0 : KT, P0 = SHARED ? KT : 2 * KT, O0 = P0 + KT;
+  static_assert(V2 >= 2 && K2 <= 6 && K1 <= 6 && O0 + 2 * DH <= 512, "rings and TMEM");
+};
+
+// A place in a ring of `stages`: stage and the parity of its use.
+struct Place {
+  int stages, st = 0;
+  uint32_t parity = 0;
+  SB_DEV explicit Place(int n) : stages(n) {}
+  SB_DEV void next() {
+    if (++st == stages) {
+      st = 0;
+      parity ^= 1u;
+    }
+  }
 };
 
 // P of 32 columns: 2^(s sl + ms), their sum added to `sum`, rounded into 16 words
@@ -95,26 +110,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const __grid_constant__ CUtensorMap vmap) {
   using C = Fwd<DH>;
   using T = Tile<DH>;
-  constexpr int ST = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = smem + 2 * C::QB;
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(ring + 2 * ST * C::SB);  // [ST] each, K stages before V stages
-  uint64_t* v_full = k_full + ST;
-  uint64_t* k_empty = v_full + ST;
-  uint64_t* v_empty = k_empty + ST;
-  uint64_t* clean = v_empty + ST;  // V tile ready for its product (with masks)
-  uint64_t* q_full = clean + ST;   // [2] each, a stream
-  uint64_t* s_full = q_full + 2;      // scores computed
-  uint64_t* s_free = s_full + 2;      // scores taken into registers
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + C::TILES);  // [6] each
+  uint64_t* v_full = k_full + 6;
+  uint64_t* k_empty = v_full + 6;
+  uint64_t* v_empty = k_empty + 6;
+  uint64_t* clean = v_empty + 6;  // V tile ready for its product (with masks)
+  uint64_t* q_full = clean + 6;   // [2] each, a stream
+  uint64_t* s_full = q_full + 2;  // scores computed
+  uint64_t* s_free = s_full + 2;  // scores taken into registers
   uint64_t* p_full = s_free + 2;
   uint64_t* o_full = p_full + 2;
-  uint64_t* dbar = o_full + 2;        // [2]
+  uint64_t* dbar = o_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dbar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   // what threads of a row tell each other: [stream][row] a maximum or a sum; at the end [row] both of the
   // second stream's
-  float* told = reinterpret_cast<float*>(ring + 2 * ST * C::SB + 512);
+  float* told = reinterpret_cast<float*>(smem + C::TILES + 512);
   float2* ml = reinterpret_cast<float2*>(told);
   const int warp = warp_id(), lane = lane_id();
 
@@ -129,12 +142,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int each = (a.key_tiles + a.splits - 1) / a.splits;
   const int first = split * each;
   const int n = max(0, min(min(first + each, a.key_tiles), (count + KT - 1) / KT) - first);
-  // a stream's scores are a tile before its values, or follow the last tile's: tiles are loaded in the
-  // order K0 .. K(ahead - 1) V0 K(ahead) V1 ...
-  const int ahead = (C::OVER ? 1 : 2) * (two ? 1 : 2);
+  const int KS = two ? C::K2 : C::K1, VS = two ? C::V2 : C::V1;
+  uint8_t* k_ring = smem + (two ? 2 : 1) * C::QB;
+  uint8_t* v_ring = k_ring + KS * C::SB;
+  // tiles are used, and loaded, in the order K0 .. K(ahead - 1) V0 K(ahead) V1 ...
+  const int ahead = two || C::SHARED ? 2 : 3;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < ST; ++i) {
+    for (int i = 0; i < 6; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&v_full[i], 1);
       mbar_init(&k_empty[i], two ? 2 : 1);  // the streams that read a tile
@@ -174,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tq = r / a.group, h = kvh * a.group + (r - tq * a.group);
   const int mine = two ? n : (n - t + 1) / 2;  // key tiles of the stream
   const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-  const uint32_t s_at = tmem + lanes + t * KT + hf * 64, p_at = tmem + lanes + C::P0 + t * C::PSTEP + hf * 32;
+  const uint32_t s_at = tmem + lanes + t * C::SSTEP + hf * 64, p_at = tmem + lanes + C::P0 + t * (KT / 2) + hf * 32;
   const uint32_t o_at = tmem + lanes + C::O0 + t * DH + hf * (DH / 2);
   const int bar_id = 1 + t * 4 + quad;  // of the two warps of these rows
   float* tell = told + t * 128 + lr;
@@ -187,70 +202,114 @@ __global__ void __launch_bounds__(kThreads, 1)
       prefetch_tmap(&kmap);
       prefetch_tmap(&vmap);
       int ki = 0, vi = 0;
+      Place kp(KS), vp(VS);
       while (vi < n) {
         const bool v = ki == min(n, vi + ahead);
-        const int i = v ? vi : ki, st = i % ST;
-        if (i >= ST && !mbar_wait(v ? &v_empty[st] : &k_empty[st], ((i / ST) - 1) & 1, abort_flag)) {
+        const int i = v ? vi : ki;
+        Place& at = v ? vp : kp;
+        // (the first use of a stage passes: its barrier's phase before the first counts as done)
+        if (!mbar_wait((v ? v_empty : k_empty) + at.st, at.parity ^ 1u, abort_flag)) {
           give_up(SB_ERR_TIMEOUT_EMPTY);
           break;
         }
-        uint64_t* bar = v ? &v_full[st] : &k_full[st];
+        uint64_t* bar = (v ? v_full : k_full) + at.st;
         mbar_arrive_expect_tx(bar, C::SB);
         const CUtensorMap* map = v ? &vmap : &kmap;
-        uint8_t* dst = ring + (v ? ST + st : st) * C::SB;
+        uint8_t* dst = (v ? v_ring : k_ring) + at.st * C::SB;
         const int item = b * (v ? a.v_item : a.k_item);
         for (int x = 0; x < T::BOXES; ++x)
           tma_load_4d(dst + x * T::box_bytes(KT), map, bar, x * T::COLS, (first + i) * KT, kvh, item);
         if (v) ++vi;
         else ++ki;
+        at.next();
       }
       if (*abort_flag) {
-        for (int i = max(0, ki - ST); i < ki; ++i) bounded_wait(&k_full[i % ST], (i / ST) & 1);
-        for (int i = max(0, vi - ST); i < vi; ++i) bounded_wait(&v_full[i % ST], (i / ST) & 1);
+        for (int i = max(0, ki - KS); i < ki; ++i) bounded_wait(&k_full[i % KS], (i / KS) & 1);
+        for (int i = max(0, vi - VS); i < vi; ++i) bounded_wait(&v_full[i % VS], (i / VS) & 1);
       }
     }
   } else if (warp == kSoft || warp == kSoft + 1) {
-    const int u = warp - kSoft, tiles = two ? n : (n - u + 1) / 2;
-    if (lane == 0 && tiles > 0) {  // issuer of stream u
-      const uint32_t rb = smem_u32(ring), q = smem_u32(smem) + (two ? u * C::QB : 0);
-      const uint32_t s_to = tmem + u * KT, p_from = tmem + C::P0 + u * C::PSTEP, o_to = tmem + C::O0 + u * DH;
+    const int u0 = warp - kSoft;
+    if (lane == 0 && n > 0 && (two || u0 == 0)) {  // issuer of stream u0, or of both
+      const uint32_t kb = smem_u32(k_ring), vb = smem_u32(v_ring), qb = smem_u32(smem) + u0 * C::QB;
       constexpr uint32_t id_s = idesc_16bit(BF16, 128, KT, false), id_o = idesc_16bit(BF16, 128, DH, true);
-      auto ready = [&](uint64_t* bars, int i) { return mbar_wait(&bars[i % ST], (i / ST) & 1, abort_flag); };
-      auto tile_of = [&](int c) { return two ? c : 2 * c + u; };
-      auto scores = [&](int c) {
-        const int i = tile_of(c);
-        ok = ok && ready(k_full, i);
-        // the last tile's scores have been taken (P over them: and its values are issued)
-        if (!C::OVER && c > 0) ok = ok && mbar_wait(&s_free[u], (c - 1) & 1, abort_flag);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t k = rb + i % ST * C::SB;
+      Place kp(KS), vp(VS);
+      auto k_ready = [&]() { return mbar_wait(&k_full[kp.st], kp.parity, abort_flag); };
+      auto v_ready = [&]() {
+        return mbar_wait(&v_full[vp.st], vp.parity, abort_flag) &&
+               (!a.masked || mbar_wait(&clean[vp.st], vp.parity, abort_flag));
+      };
+      auto scores = [&](int u) {  // of stream u with the next K tile
+        const uint32_t k = kb + kp.st * C::SB;
 #pragma unroll
         for (int ks = 0; ks < T::KSTEPS; ++ks)
-          mma_f16_ss(s_to, T::k_major(q, 128, ks), T::k_major(k, KT, ks), id_s, ks > 0);
+          mma_f16_ss(tmem + u * C::SSTEP, T::k_major(qb, 128, ks), T::k_major(k, KT, ks), id_s, ks > 0);
         mma_commit(&s_full[u]);
-        mma_commit(&k_empty[i % ST]);
+        mma_commit(&k_empty[kp.st]);
+        kp.next();
       };
-      ok = mbar_wait(&q_full[two ? u : 0], 0, abort_flag);
-      scores(0);
-      for (int c = 0; c < tiles && ok; ++c) {
-        if (!C::OVER && c + 1 < tiles) scores(c + 1);
-        const int i = tile_of(c);
-        ok = ok && ready(v_full, i) && (!a.masked || ready(clean, i)) && mbar_wait(&p_full[u], c & 1, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t v = rb + (ST + i % ST) * C::SB;
+      auto values = [&](int u, int c) {  // P of stream u's tile c with the next V tile
+        const uint32_t v = vb + vp.st * C::SB;
 #pragma unroll
         for (int k = 0; k < KT / 16; ++k)
-          mma_f16_ts(o_to, p_from + k * 8, T::mn_major(v, KT, k), id_o, c > 0 || k > 0);
-        if (!C::OVER || c + 1 == tiles) mma_commit(&o_full[u]);  // OVER: the next scores say it of the others
-        mma_commit(&v_empty[i % ST]);
-        if (C::OVER && c + 1 < tiles) scores(c + 1);
+          mma_f16_ts(tmem + C::O0 + u * DH, tmem + C::P0 + u * (KT / 2) + k * 8, T::mn_major(v, KT, k), id_o,
+                     c > 0 || k > 0);
+        mma_commit(&o_full[u]);
+        mma_commit(&v_empty[vp.st]);
+        vp.next();
+      };
+      auto p_ready = [&](int u, int c) { return mbar_wait(&p_full[u], c & 1, abort_flag); };
+      // stream u has taken the scores of its tile c into registers
+      auto taken = [&](int u, int c) { return mbar_wait(&s_free[u], c & 1, abort_flag); };
+      ok = mbar_wait(&q_full[u0], 0, abort_flag);
+      if (two) {
+        // the scores' buffer is free when this stream has taken its last tile's, a shared one when the other
+        // stream has taken the tile before
+        ok = ok && k_ready() && (!C::SHARED || u0 == 0 || taken(0, 0));
+        if (ok) {
+          tc_fence_after();
+          scores(u0);
+        }
+        for (int c = 0; c < n && ok; ++c) {
+          if (c + 1 < n) {
+            ok = k_ready() && (C::SHARED ? taken(1 - u0, c + u0) : taken(u0, c));
+            if (!ok) break;
+            tc_fence_after();
+            scores(u0);
+          }
+          ok = v_ready() && p_ready(u0, c);
+          if (!ok) break;
+          tc_fence_after();
+          values(u0, c);
+        }
+      } else {
+        // tile i belongs to stream i % 2; before its values come the scores of the next tile, or of the one
+        // after where the streams have a buffer each
+        constexpr int more = C::SHARED ? 1 : 2;
+        for (int i = 0; i < min(n, more) && ok; ++i) {
+          ok = k_ready();
+          if (!ok) break;
+          tc_fence_after();
+          scores(i);
+        }
+        for (int i = 0; i < n && ok; ++i) {
+          const int u = i & 1, c = i >> 1;
+          if (i + more < n) {
+            ok = k_ready() && taken(u, c);
+            if (!ok) break;
+            tc_fence_after();
+            scores((i + more) & 1);
+          }
+          ok = v_ready() && p_ready(u, c);
+          if (!ok) break;
+          tc_fence_after();
+          values(u, c);
+        }
       }
       if (!ok) {
         give_up(SB_ERR_TIMEOUT_FULL);
-        mma_commit(&dbar[u]);
-        bounded_wait(&dbar[u], 0);
+        mma_commit(&dbar[u0]);
+        bounded_wait(&dbar[u0], 0);
       }
     }
   } else if (warp == kSoft + 3) {
@@ -260,17 +319,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int y = 0; y < 2; ++y)
 #pragma unroll
         for (int x = 0; x < KT / 32; ++x) next[y][x] = a.mask.ask(b, (first + y) * KT + 32 * x, count);
+      Place vp(VS);
 #pragma unroll 2
-      for (int i = 0; i < n; ++i) {
+      for (int i = 0; i < n; ++i, vp.next()) {
         const int j0 = (first + i) * KT;
-        uint8_t* v = ring + (ST + i % ST) * C::SB;
+        uint8_t* v = v_ring + vp.st * C::SB;
         uint32_t w[KT / 32];
 #pragma unroll
         for (int x = 0; x < KT / 32; ++x) {
           w[x] = a.mask.told(next[i & 1][x], j0 + 32 * x, count);
           next[i & 1][x] = a.mask.ask(b, j0 + 2 * KT + 32 * x, count);
         }
-        if (!warp_wait(&v_full[i % ST], (i / ST) & 1, abort_flag)) {
+        if (!warp_wait(&v_full[vp.st], vp.parity, abort_flag)) {
           if (lane == 0) give_up(SB_ERR_TIMEOUT_FULL);
           break;
         }
@@ -284,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               *reinterpret_cast<uint4*>(v + T::chunk(KT, 32 * x + lane, c)) = make_uint4(0, 0, 0, 0);
         }
         if (touched) fence_proxy_async_smem();
-        warp_arrive(&clean[i % ST]);
+        warp_arrive(&clean[vp.st]);
       }
     }
   } else {
@@ -311,8 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && warp_wait(&s_full[t], i & 1, abort_flag);
       if (!some) {  // P of lanes without rows is never looked at
         if (!ok) break;
-        if (!C::OVER) warp_arrive(&s_free[t]);
-        ok = C::OVER || i == 0 || warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
+        warp_arrive(&s_free[t]);
+        ok = i == 0 || warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
         if (!ok) break;
         warp_arrive(&p_full[t]);
         continue;
@@ -323,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld32(s_at + 32, s + 32);
       tmem_ld_wait();
       tc_fence_before();
-      if (!C::OVER) warp_arrive(&s_free[t]);
+      warp_arrive(&s_free[t]);
       if ((w0 & w1) != 0xFFFFFFFFu) {
         // 16 keys at a time: masks of images and lengths leave most groups whole
 #pragma unroll
@@ -362,8 +422,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint64_t sum[2] = {0, 0};
       uint32_t pk[16];
       probabilities<BF16>(s, sl2, ms2, sum, pk);
-      // the last tile's product has read its P and added to O (OVER: this tile's scores came after it)
-      if (!C::OVER && i > 0) {
+      // the last tile's product has read its P and added to O
+      if (i > 0) {
         ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
         tc_fence_after();
       }
@@ -388,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       if (ok) warp_arrive(&p_full[t]);
     }
-    if (ok && mine > 0) ok = warp_wait(&o_full[t], C::OVER ? 0 : (mine - 1) & 1, abort_flag);
+    if (ok && mine > 0) ok = warp_wait(&o_full[t], (mine - 1) & 1, abort_flag);
     if (!ok && lane == 0) give_up(SB_ERR_TIMEOUT_ACC);
     tc_fence_after();
     if (some) {  // the row's sum
