@@ -572,9 +572,10 @@ extern "C" int sb_kernels_error(int clear, int* flags) {
     if (cudaMemcpyToSymbol(g_kernel_error, &zero, sizeof(int)) != cudaSuccess)
       return record_error(SB_ECUDA, "sb_kernels_error: clear");
   }
-  int fwd = 0, bwd = 0, norm = 0;
-  if (xattn_error(clear, &fwd) != 0 || xattn_back_error(clear, &bwd) != 0 || gnorm_error(clear, &norm) != 0)
+  int fwd = 0, few = 0, bwd = 0, norm = 0;
+  if (xattn_error(clear, &fwd) != 0 || few_error(clear, &few) != 0 || xattn_back_error(clear, &bwd) != 0 ||
+      gnorm_error(clear, &norm) != 0)
     return record_error(SB_ECUDA, "sb_kernels_error: the memory-reading block's kernels");
-  *flags |= fwd | bwd | norm;
+  *flags |= fwd | few | bwd | norm;
   return SB_OK;
 }

@@ -7,8 +7,8 @@
 // 128 of them, whatever the group's size.  A CTA has two streams of 128-row tiles, each with an
 // accumulator, eight softmax warps and a warp that issues its products, over a range of 128-key tiles:
 //   two tiles of rows left   a tile a stream, both over every key tile
-//   one                      both streams on it, over alternate key tiles, joined at the end (a token
-//                            a stream, and the last tile of an odd number)
+//   one                      both streams on it, over alternate key tiles, joined at the end (the
+//                            last tile of an odd number)
 //   loader warp   K and V tiles by TMA into a ring each, in the order in which they are used.  A stage's
 //                 barrier is only waited for by roles that see each of its uses (a parity says
 //                 nothing about a use before the last)
@@ -30,7 +30,8 @@
 // The exponentials (16 a clock and SM) are the floor of heads of few channels; the rest of a row's
 // arithmetic works on pairs.  A polynomial for part of them was slower: the issue slots are as scarce.
 // The key range is split over CTAs where the rows alone leave SMs idle: these write fp32 partial rows
-// with their L, and a second kernel joins them.
+// with their L, and a second kernel joins them.  Up to 16 rows (single tokens) have a kernel of their
+// own, which reads K and V once at memory speed.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -42,21 +43,6 @@ namespace sb {
 namespace {
 
 __device__ int g_xattn_error;
-
-struct FwdArgs {
-  View q;
-  OutView o;
-  float* lse;
-  KeyMask mask;
-  int B, H, Hkv, group, Tq, rows;  // rows = group * Tq of an (item, key head)
-  int pairs, splits, key_tiles;    // CTAs a (item, key head) and split; key tiles in all
-  int k_item, v_item;              // 0: one memory for every item
-  int masked;                      // lens or valid given: the cleaner runs
-  float scale_log2;
-  float* part_o;  // [splits][B * H * Tq][DH]
-  float* part_l;  // [splits][B * H * Tq]
-  long long all_rows;
-};
 
 constexpr int KT = 128;      // keys a tile
 constexpr int kSoft = 16;     // softmax warps: stream (w / 8), half of a tile's keys (w / 4 % 2), TMEM lanes (w % 4)
@@ -597,6 +583,7 @@ __global__ void attend_none_kernel(OutView o, float* lse, int H, int Tq, int dh,
 struct FwdPlan {
   int pairs, splits, key_tiles;
   long long units;
+  bool few;
 };
 
 // CTAs take two tiles of rows each; a last single tile takes half of a CTA's time (its streams share
@@ -607,6 +594,13 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int Tq, int Tk, int sms) {
   constexpr int kStart = 4, kMost = 64;
   FwdPlan p;
   const long long tiles = ((long long)(H / Hkv) * Tq + 127) / 128;
+  p.few = (long long)(H / Hkv) * Tq <= kFewRows;
+  if (p.few) {
+    p.pairs = p.key_tiles = 1;
+    p.units = (long long)B * Hkv;
+    p.splits = few_splits(p.units, Tk, sms);
+    return p;
+  }
   p.pairs = (int)((tiles + 1) / 2);
   p.key_tiles = (Tk + KT - 1) / KT;
   p.units = (long long)B * Hkv * p.pairs;
@@ -778,10 +772,16 @@ extern "C" int sb_cross_attention(const void* q, long long q_row, long long q_im
   a.part_o = static_cast<float*>(work);
   a.part_l = a.part_o + (long long)p.splits * a.all_rows * dh;
   CUtensorMap km, vm;
-  if (!xattn_tensor_map(&km, {k, k_row, k_img}, dtype, B, Tk, Hkv, dh, KT) ||
-      !xattn_tensor_map(&vm, {v, v_row, v_img}, dtype, B, Tk, Hkv, dh, KT))
+  const int box = p.few ? few_keys(dh) : KT;
+  if (!xattn_tensor_map(&km, {k, k_row, k_img}, dtype, B, Tk, Hkv, dh, box) ||
+      !xattn_tensor_map(&vm, {v, v_row, v_img}, dtype, B, Tk, Hkv, dh, box))
     return record_error(SB_EINVAL, "sb_cross_attention: tensor map of k or v");
   const bool bf16 = dtype == SB_BF16;
+  if (p.few) {
+    cudaError_t e = few_launch(a, dh, bf16, km, vm, st);
+    if (e == cudaSuccess && p.splits > 1) e = few_join(a, dh, bf16, st);
+    return e == cudaSuccess ? SB_OK : record_error(SB_ECUDA, cudaGetErrorString(e));
+  }
   const cudaError_t e = dh == 32 ? launch_fwd<32>(a, p, bf16, km, vm, st)
                         : dh == 64 ? launch_fwd<64>(a, p, bf16, km, vm, st) : launch_fwd<128>(a, p, bf16, km, vm, st);
   if (e != cudaSuccess) return record_error(SB_ECUDA, cudaGetErrorString(e));

@@ -37,6 +37,22 @@ struct KeyMask {
   }
 };
 
+// Arguments of the forward kernels.
+struct FwdArgs {
+  View q;
+  OutView o;
+  float* lse;
+  KeyMask mask;
+  int B, H, Hkv, group, Tq, rows;  // rows = group * Tq of an (item, key head)
+  int pairs, splits, key_tiles;    // CTAs a (item, key head) and split; key tiles in all
+  int k_item, v_item;              // 0: one memory for every item
+  int masked;                      // lens or valid given: the cleaner runs
+  float scale_log2;
+  float* part_o;  // [splits][B * H * Tq][DH]
+  float* part_l;  // [splits][B * H * Tq]
+  long long all_rows;
+};
+
 // ---------------------------------------------------------------- tcgen05 forms
 // D[tmem] (+)= A[tmem] * B[smem]: A holds 16-bit pairs, k and k + 1 in a 32-bit column.
 SB_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accum) {
@@ -186,9 +202,17 @@ bool xattn_tensor_map(CUtensorMap* map, const View& v, int dtype, int B, int T, 
 bool xattn_sizes_ok(int dtype, int B, int H, int Hkv, int dh, int Tq, int Tk);
 // 16-byte rows whose strides fit a tensor map
 bool xattn_view_ok(const void* p, long long row, long long img);
+// Few query rows an (item, key head): the key splits of its kernel, its launch (partial rows where splits
+// > 1), and the join of the partial rows.
+constexpr int kFewRows = 16;
+int few_splits(long long units, int Tk, int sms);
+cudaError_t few_launch(const FwdArgs& a, int dh, bool bf16, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st);
+int few_keys(int dh);  // rows of its tensor maps' boxes
+cudaError_t few_join(const FwdArgs& a, int dh, bool bf16, cudaStream_t st);
 // Sticky SB_ERR_* flags of the attention kernels, cleared on request.
 int xattn_error(int clear, int* flags);  // 0, or -1 when the device could not be read
 int xattn_back_error(int clear, int* flags);
+int few_error(int clear, int* flags);
 int gnorm_error(int clear, int* flags);  // of the gated norms
 long long xattn_back_work(int B, int H, int Hkv, int dh, int Tq, int Tk, int sms);
 // SMs of the current device, 0 on error
