@@ -8,10 +8,13 @@
 //   SIDE 1 (dk, dv)  a CTA holds 128 keys (k, v) and streams 64-row tiles of q, dout, head by head
 // Per step, with X the held and Y the streamed operands:
 //   S = X1 Y1^T, R = X2 Y2^T (128 x 64, operands in shared memory)
-//   thread = held row: P and dS from S and R, rounded to the operands' type, written over them
+//   thread = held row: takes S and R into registers at once (their buffer is then free for the next
+//   step's), P and dS from them, rounded to the operands' type, back to TMEM
 //   acc1 += dS Y1 (dq, dk),  SIDE 1: acc2 += P Y2 (dv)     (A in TMEM, B the rows as they lie)
-// S and R have two buffers and four softmax warps each, so the products of one step run while the
-// other's softmax does.  S and R are computed on both sides (7 products instead of 5): against
+// Steps alternate between two groups of eight softmax warps (two threads a held row, 32 streamed rows
+// each) with their own P and dS; S and R have two buffers, or one where two accumulators of 128 columns
+// leave no room.  One warp issues S and R while another issues the accumulations: the products of one step run
+// while the other's softmax does, and an issuer's waits on barriers do not idle the tensor pipe.  S and R are computed on both sides (7 products instead of 5): against
 // one kernel that adds up dq in global memory this costs 2 of 7 products and saves the atomics.
 //
 // fp16 gradients: P and dS may be far below fp16's smallest normal number (long memories, small
@@ -32,6 +35,7 @@ namespace {
 __device__ int g_xattn_bwd_error;
 
 constexpr int kStep = 64;  // streamed rows a step
+constexpr int kSoft = 16;  // softmax warps: buffer (w / 8), half of a step's rows (w / 4 % 2), TMEM lanes (w % 4)
 
 struct BackArgs {
   View q, k, v, out, dout;
@@ -110,13 +114,15 @@ struct Back {
   static constexpr int XB = Tile<DH>::bytes(128);    // a held operand
   static constexpr int YB = Tile<DH>::bytes(kStep);  // a streamed one
   static constexpr int SB = 2 * YB;                  // a stage
-  static constexpr int STAT = SIDE ? 8 * 2 * 128 * 4 : 0;  // L and D of a step's queries, a warp each
+  static constexpr int STAT = SIDE ? kSoft * 2 * 64 * 4 : 0;  // L and D of a step's queries, a warp each
   static constexpr int ROOM = 224 * 1024 - 2 * XB - STAT;
   static constexpr int STAGES = ROOM / SB < 8 ? ROOM / SB : 8;
   static constexpr int SMEM = 1024 + 2 * XB + STAGES * SB + STAT + 512;
-  static constexpr int THREADS = 11 * 32;
-  static constexpr int ACC = 256;  // TMEM column of acc1; acc2 follows
-  static_assert(STAGES >= 3 && ACC + (1 + SIDE) * DH <= 512, "ring and TMEM");
+  static constexpr int THREADS = (kSoft + 4) * 32;
+  // TMEM columns: S and R (64 + 64, NB times), P and dS of each group (32 + 32), acc1, acc2
+  static constexpr int NB = SIDE == 1 && DH == 128 ? 1 : 2;
+  static constexpr int PD = NB * 128, ACC = PD + 128;
+  static_assert(STAGES >= 4 && ACC + (1 + SIDE) * DH <= 512, "ring and TMEM");
 };
 
 template <int DH, bool BF16, int SIDE>
@@ -135,11 +141,13 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
   uint64_t* empty = full + ST;
   uint64_t* clean = empty + ST;  // [ST]
   uint64_t* x_full = clean + ST;
-  uint64_t* s_full = x_full + 1;  // [2]
-  uint64_t* p_full = s_full + 2;  // [2]
-  uint64_t* acc_full = p_full + 2;
-  uint64_t* dbar = acc_full + 1;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dbar + 1);
+  uint64_t* s_full = x_full + 1;  // [2] each, a group: S and R computed
+  uint64_t* s_free = s_full + 2;  // S and R taken into registers
+  uint64_t* p_full = s_free + 2;  // P and dS written
+  uint64_t* p_free = p_full + 2;  // and read by the accumulations
+  uint64_t* acc_full = p_free + 2;
+  uint64_t* dbar = acc_full + 1;  // [2]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dbar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   const int warp = warp_id(), lane = lane_id();
 
@@ -162,17 +170,19 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
       mbar_init(&empty[i], 1);
       mbar_init(&clean[i], 1);
     }
-    mbar_init(x_full, SIDE == 0 ? 8 : 1);
+    mbar_init(x_full, SIDE == 0 ? kSoft : 1);
     for (int u = 0; u < 2; ++u) {
       mbar_init(&s_full[u], 1);
-      mbar_init(&p_full[u], 4);
+      mbar_init(&s_free[u], kSoft / 2);
+      mbar_init(&p_full[u], kSoft / 2);
+      mbar_init(&p_free[u], 1);
+      mbar_init(&dbar[u], 1);
     }
     mbar_init(acc_full, 1);
-    mbar_init(dbar, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == kSoft) {
     tmem_alloc(tmem_holder, 512);
     tmem_relinquish();
   }
@@ -185,7 +195,7 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
     atomicOr(&g_xattn_bwd_error, code);
   };
 
-  if (warp == 9) {
+  if (warp == kSoft + 2) {
     if (lane == 0 && n > 0) {  // loader
       if constexpr (SIDE == 1) {
         mbar_arrive_expect_tx(x_full, 2 * C::XB);
@@ -216,18 +226,19 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
         if (SIDE == 1) bounded_wait(x_full, 0);
       }
     }
-  } else if (warp == 8) {
-    if (lane == 0 && n > 0) {  // MMA
+  } else if (warp == kSoft) {
+    if (lane == 0 && n > 0) {  // issuer of S and R
       const uint32_t xb = smem_u32(smem), rb = smem_u32(ring);
-      constexpr uint32_t id_s = idesc_16bit(BF16, 128, kStep, false), id_a = idesc_16bit(BF16, 128, DH, true);
+      constexpr uint32_t id_s = idesc_16bit(BF16, 128, kStep, false);
       bool ok = mbar_wait(x_full, 0, abort_flag);
-      auto scores = [&](int i) {
+      for (int i = 0; i < n && ok; ++i) {
         const int st = i % ST, u = i & 1;
-        ok = ok && mbar_wait(&full[st], (i / ST) & 1, abort_flag) &&
-             (SIDE == 1 || !a.masked || mbar_wait(&clean[st], (i / ST) & 1, abort_flag));
-        if (!ok) return;
+        ok = mbar_wait(&full[st], (i / ST) & 1, abort_flag) &&
+             (SIDE == 1 || !a.masked || mbar_wait(&clean[st], (i / ST) & 1, abort_flag)) &&
+             (i < C::NB || mbar_wait(&s_free[(i - C::NB) & 1], ((i - C::NB) >> 1) & 1, abort_flag));
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t y = rb + st * C::SB, s = tmem + u * 128;
+        const uint32_t y = rb + st * C::SB, s = tmem + (C::NB == 2 ? u * 128 : 0);
 #pragma unroll
         for (int ks = 0; ks < T::KSTEPS; ++ks)
           mma_f16_ss(s, T::k_major(xb, 128, ks), T::k_major(y, kStep, ks), id_s, ks > 0);
@@ -235,35 +246,44 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
         for (int ks = 0; ks < T::KSTEPS; ++ks)
           mma_f16_ss(s + 64, T::k_major(xb + C::XB, 128, ks), T::k_major(y + C::YB, kStep, ks), id_s, ks > 0);
         mma_commit(&s_full[u]);
-      };
-      scores(0);
-      if (n > 1) scores(1);
-      for (int i = 0; i < n && ok; ++i) {
+      }
+      if (!ok) {
+        give_up(SB_ERR_TIMEOUT_FULL);
+        mma_commit(&dbar[0]);
+        bounded_wait(&dbar[0], 0);
+      }
+    }
+  } else if (warp == kSoft + 1) {
+    if (lane == 0 && n > 0) {  // issuer of the accumulations
+      const uint32_t rb = smem_u32(ring);
+      constexpr uint32_t id_a = idesc_16bit(BF16, 128, DH, true);
+      bool ok = true;
+      for (int i = 0; i < n; ++i) {
         const int st = i % ST, u = i & 1;
         ok = mbar_wait(&p_full[u], (i >> 1) & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t y = rb + st * C::SB, s = tmem + u * 128;
+        const uint32_t y = rb + st * C::SB, p = tmem + C::PD + u * 64;
         if constexpr (SIDE == 1) {
 #pragma unroll
           for (int k = 0; k < kStep / 16; ++k)
-            mma_f16_ts(tmem + C::ACC + DH, s + k * 8, T::mn_major(y + C::YB, kStep, k), id_a, i > 0 || k > 0);
+            mma_f16_ts(tmem + C::ACC + DH, p + k * 8, T::mn_major(y + C::YB, kStep, k), id_a, i > 0 || k > 0);
         }
 #pragma unroll
         for (int k = 0; k < kStep / 16; ++k)
-          mma_f16_ts(tmem + C::ACC, s + 64 + k * 8, T::mn_major(y, kStep, k), id_a, i > 0 || k > 0);
+          mma_f16_ts(tmem + C::ACC, p + 32 + k * 8, T::mn_major(y, kStep, k), id_a, i > 0 || k > 0);
+        mma_commit(&p_free[u]);
         mma_commit(&empty[st]);
-        if (i + 2 < n) scores(i + 2);
       }
       if (ok) {
         mma_commit(acc_full);
       } else {
         give_up(SB_ERR_TIMEOUT_FULL);
-        mma_commit(dbar);
-        bounded_wait(dbar, 0);
+        mma_commit(&dbar[1]);
+        bounded_wait(&dbar[1], 0);
       }
     }
-  } else if (warp == 10) {
+  } else if (warp == kSoft + 3) {
     if (SIDE == 0 && a.masked) {  // cleaner: k's rows of keys that take no part
       for (int i = 0; i < n; ++i) {
         const int st = i % ST, j0 = (first + i) * kStep;
@@ -286,9 +306,10 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
       }
     }
   } else {
-    const int u = warp >> 2, quad = warp & 3;
+    const int u = warp >> 3, hf = warp >> 2 & 1, quad = warp & 3;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const uint32_t s_at = tmem + lanes + u * 128, r_at = s_at + 64;
+    const uint32_t s_at = tmem + lanes + (C::NB == 2 ? u * 128 : 0) + hf * 32, r_at = s_at + 64;
+    const uint32_t p_at = tmem + lanes + C::PD + u * 64 + hf * 16, d_at = p_at + 32;
     const int x = tile * 128 + quad * 32 + lane;  // held row: query row of the group, or key
     const int rows = SIDE == 0 ? a.group * a.Tq : a.Tk;
     const int tq = SIDE == 0 ? x / a.group : 0, h = kvh * a.group + (SIDE == 0 ? x - tq * a.group : 0);
@@ -299,8 +320,8 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
       const View& src = u == 0 ? a.q : a.dout;
       const uint4* from = reinterpret_cast<const uint4*>(static_cast<const __half*>(src.p) + b * src.img + tq * src.row +
                                                          (long long)h * DH);
-#pragma unroll 8
-      for (int c = 0; c < DH / 8; ++c)
+#pragma unroll
+      for (int c = hf * (DH / 16); c < (hf + 1) * (DH / 16); ++c)
         *reinterpret_cast<uint4*>(smem + u * C::XB + T::chunk(128, quad * 32 + lane, c)) =
             live ? from[c] : make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();
@@ -321,63 +342,74 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
       l2 = a.lse2[r] - lift;
       df = a.delta[r] * f;
     }
-    float* mine = stat + warp * 256;
-    float next[4];
-    auto fetch = [&](int i) {  // SIDE 1: L and D of step i's queries, two a lane
-      const int step = first + i, t0 = step % q_tiles * kStep;
-      const long long base = ((long long)b * a.H + kvh * a.group + step / q_tiles) * a.Tq;
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int t = t0 + y * 32 + lane;
-        next[y] = t < a.Tq ? a.lse2[base + t] - lift : INFINITY;
-        next[2 + y] = t < a.Tq ? a.delta[base + t] * f : 0.f;
-      }
+    float* mine = stat + warp * 128;  // [2][L, D][32]
+    float next[2];
+    auto fetch = [&](int i) {  // SIDE 1: L and D of step i's queries, one a lane
+      const int step = first + i, t = step % q_tiles * kStep + hf * 32 + lane;
+      const long long at = ((long long)b * a.H + kvh * a.group + step / q_tiles) * a.Tq + t;
+      next[0] = t < a.Tq ? a.lse2[at] - lift : INFINITY;
+      next[1] = t < a.Tq ? a.delta[at] * f : 0.f;
     };
     if (SIDE == 1 && u < n) fetch(u);
+    uint32_t byte = SIDE == 0 ? a.mask.ask(b, (first + u) * kStep + hf * 32, count) : 0u;
     bool ok = true;
     for (int i = u; i < n; i += 2) {
-      uint32_t w[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
-      const float* st = mine + ((i >> 1) & 1) * 128;
+      uint32_t w = 0xFFFFFFFFu;
+      const float* st = mine + ((i >> 1) & 1) * 64;
       if constexpr (SIDE == 0) {
-        w[0] = a.mask.word(b, (first + i) * kStep, count);
-        w[1] = a.mask.word(b, (first + i) * kStep + 32, count);
+        const int j0 = (first + i) * kStep + hf * 32;
+        w = a.mask.told(byte, j0, count);
+        byte = a.mask.ask(b, j0 + 2 * kStep, count);
       } else {
-        float* put = mine + ((i >> 1) & 1) * 128;
-#pragma unroll
-        for (int y = 0; y < 4; ++y) put[y * 32 + lane] = next[y];
+        float* put = mine + ((i >> 1) & 1) * 64;
+        put[lane] = next[0];
+        put[32 + lane] = next[1];
         __syncwarp();
         if (i + 2 < n) fetch(i + 2);
       }
       ok = warp_wait(&s_full[u], (i >> 1) & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
+      uint32_t s[2][16], r[2][16];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t s[32], r[32], pp[16], pd[16];
-        tmem_ld32(s_at + 32 * half, s);
-        tmem_ld32(r_at + 32 * half, r);
-        tmem_ld_wait();
-        float p[32], d[32];
+      for (int q = 0; q < 2; ++q) {
+        tmem_ld16(s_at + 16 * q, s[q]);
+        tmem_ld16(r_at + 16 * q, r[q]);
+      }
+      tmem_ld_wait();
+      tc_fence_before();
+      warp_arrive(&s_free[u]);
+      uint32_t pp[2][8], pd[2][8];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float lj = SIDE == 0 ? l2 : st[32 * half + j], dj = SIDE == 0 ? df : st[64 + 32 * half + j];
-          p[j] = exp2_hw(fmaf(__uint_as_float(s[j]), sl, -lj));
-          d[j] = p[j] * fmaf(__uint_as_float(r[j]), f, -dj);
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          float p[2], d[2];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int at = 16 * q + j + y;
+            const float lj = SIDE == 0 ? l2 : st[at], dj = SIDE == 0 ? df : st[32 + at];
+            p[y] = exp2_hw(fmaf(__uint_as_float(s[q][j + y]), sl, -lj));
+            d[y] = p[y] * fmaf(__uint_as_float(r[q][j + y]), f, -dj);
+          }
+          if (SIDE == 0 ? w != 0xFFFFFFFFu : !takes) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              if (SIDE == 1 || !(w >> (16 * q + j + y) & 1u)) p[y] = d[y] = 0.f;
+          }
+          if (SIDE == 1) pp[q][j / 2] = pack16<BF16>(p[0], p[1]);
+          pd[q][j / 2] = pack16<BF16>(d[0], d[1]);
         }
-        if (SIDE == 0 ? w[half] != 0xFFFFFFFFu : !takes) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (SIDE == 1 || !(w[half] >> j & 1u)) p[j] = d[j] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (SIDE == 1) pp[j] = pack16<BF16>(p[2 * j], p[2 * j + 1]);
-          pd[j] = pack16<BF16>(d[2 * j], d[2 * j + 1]);
+        if (q == 0 && i > 1) {  // the accumulations of the group's last step have read P and dS
+          ok = warp_wait(&p_free[u], ((i >> 1) - 1) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
         }
         __syncwarp();
-        if (SIDE == 1) tmem_st16(s_at + 16 * half, pp);
-        tmem_st16(r_at + 16 * half, pd);
+        if (SIDE == 1) tmem_st8(p_at + 8 * q, pp[q]);
+        tmem_st8(d_at + 8 * q, pd[q]);
       }
+      if (!ok) break;
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&p_full[u]);
@@ -387,10 +419,11 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
       if (lane == 0) give_up(SB_ERR_TIMEOUT_ACC);
     } else {
       tc_fence_after();
-      // SIDE 0: each group of warps writes half of dq's channels; SIDE 1: the first dk, the second dv
-      constexpr int cols = SIDE == 0 ? DH / 2 : DH;
-      const int c0 = SIDE == 0 ? u * cols : 0;
-      const uint32_t from = tmem + lanes + C::ACC + (SIDE == 0 ? c0 : u * DH);
+      // a warp writes half of dq's channels (SIDE 0, four of a row's warps idle) or of dk's or dv's
+      constexpr int cols = DH / 2;
+      const int c0 = (SIDE == 0 ? u : hf) * cols;
+      const bool writes = live && (SIDE == 1 || hf == 0);
+      const uint32_t from = tmem + lanes + C::ACC + (SIDE == 0 ? 0 : u * DH) + c0;
       const float by = SIDE == 1 && u == 1 ? exp2f(-lift) : a.scale * exp2f(-lift) / f;
       const OutView& o = SIDE == 0 ? a.dq : u == 0 ? a.dk : a.dv;
       const long long prow = SIDE == 0 ? ((long long)b * a.H + h) * a.Tq + tq
@@ -403,7 +436,7 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
           tmem_ld16(from + c, v);
           tmem_ld_wait();
         }
-        if (!live) continue;
+        if (!writes) continue;
         float y[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) y[j] = n > 0 && takes ? __uint_as_float(v[j]) * by : 0.f;
@@ -425,7 +458,7 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kSoft) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
