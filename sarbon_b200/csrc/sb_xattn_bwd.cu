@@ -4,18 +4,19 @@
 //   dq = scale dS k,   dk = scale dS^T q,   dv = P^T dout   (dk, dv summed over the query heads that
 // share a key head).  Two kernels of one form, each owning its results, so that no sum needs an
 // atomic and the same inputs give the same bits:
-//   SIDE 0 (dq)      a CTA holds 128 query rows (q, dout) and streams 64-row tiles of k, v
-//   SIDE 1 (dk, dv)  a CTA holds 128 keys (k, v) and streams 64-row tiles of q, dout, head by head
+//   SIDE 0 (dq)      a CTA holds 128 query rows (q, dout) and streams 128-row tiles of k, v
+//   SIDE 1 (dk, dv)  a CTA holds 128 keys (k, v) and streams 128-row tiles of q, dout, head by head
 // Per step, with X the held and Y the streamed operands:
-//   S = X1 Y1^T, R = X2 Y2^T (128 x 64, operands in shared memory)
-//   thread = held row: takes S and R into registers at once (their buffer is then free for the next
-//   step's), P and dS from them, rounded to the operands' type, back to TMEM
+//   S = X1 Y1^T, R = X2 Y2^T (128 x 128; X in TMEM where its 512 columns have room)
+//   sixteen softmax warps, four threads a held row: P from S and dS from P and R, rounded to the operands'
+//   type, to TMEM (SIDE 1: over S and R, which they replace)
 //   acc1 += dS Y1 (dq, dk),  SIDE 1: acc2 += P Y2 (dv)     (A in TMEM, B the rows as they lie)
-// Steps alternate between two groups of eight softmax warps (two threads a held row, 32 streamed rows
-// each) with their own P and dS; S and R have two buffers, or one where two accumulators of 128 columns
-// leave no room.  One warp issues S and R while another issues the accumulations: the products of one step run
-// while the other's softmax does, and an issuer's waits on barriers do not idle the tensor pipe.  S and R are computed on both sides (7 products instead of 5): against
-// one kernel that adds up dq in global memory this costs 2 of 7 products and saves the atomics.
+// Steps of 64 streamed rows (two buffers each of S and R) were half as fast: a product of 64 columns
+// takes as long as one of 128, 60 of 68 clocks.  So there is one buffer, and what overlaps is the halves
+// of a step: one warp issues S and acc2, another R and acc1 (in SIDE 1 acc2 of a step, then the next S;
+// acc1, then the next R), so P's half runs while dS is computed, and the next S while dS's half runs.
+// S and R are computed on both sides (7 products instead of 5): against one kernel that adds up dq in
+// global memory this costs 2 of 7 products and saves the atomics.
 //
 // fp16 gradients: P and dS may be far below fp16's smallest normal number (long memories, small
 // losses).  P is held as 2^14 P, and dS as F dS with F the power of two that the bound |dS| <= 2 P
@@ -34,8 +35,8 @@ namespace {
 
 __device__ int g_xattn_bwd_error;
 
-constexpr int kStep = 64;  // streamed rows a step
-constexpr int kSoft = 16;  // softmax warps: buffer (w / 8), half of a step's rows (w / 4 % 2), TMEM lanes (w % 4)
+constexpr int kStep = 128;  // streamed rows a step
+constexpr int kSoft = 16;   // softmax warps: 32 streamed rows (w / 4), TMEM lanes (w % 4)
 
 struct BackArgs {
   View q, k, v, out, dout;
@@ -44,7 +45,7 @@ struct BackArgs {
   KeyMask mask;
   int dt, B, H, Hkv, group, Tq, Tk;
   int x_tiles, splits, steps;  // held tiles of an (item, key head); splits of its steps
-  int y1_item, y2_item, x1_item, x2_item;  // 0: one memory for every item
+  int y1_item, y2_item;  // 0: one memory for every item
   int masked;
   float scale, scale_log2;
   float* lse2;   // [B][H][Tq] L log2 e, +inf for a row without keys
@@ -111,41 +112,44 @@ __global__ void __launch_bounds__(256) attend_back_rows_kernel(const __grid_cons
 // ---------------------------------------------------------------- the products
 template <int DH, int SIDE>
 struct Back {
-  static constexpr int XB = Tile<DH>::bytes(128);    // a held operand
-  static constexpr int YB = Tile<DH>::bytes(kStep);  // a streamed one
+  // TMEM columns: S, R (SIDE 1: P and dS over them), dS (SIDE 0), acc1, acc2, X1, X2 (XT of them)
+  static constexpr int R0 = kStep, D0 = 2 * kStep, ACC = D0 + (SIDE == 0 ? kStep / 2 : 0), X0 = ACC + (1 + SIDE) * DH;
+  static constexpr int XT = DH < 128 ? 2 : SIDE == 0 ? 1 : 0;
+  static constexpr int XS = Tile<DH>::bytes(128);    // a held operand in shared memory
+  static constexpr int XB = (2 - XT) * XS;
+  static constexpr int YB = Tile<DH>::bytes(kStep);  // a streamed operand
   static constexpr int SB = 2 * YB;                  // a stage
   static constexpr int STAT = SIDE ? kSoft * 2 * 64 * 4 : 0;  // L and D of a step's queries, a warp each
-  static constexpr int ROOM = 224 * 1024 - 2 * XB - STAT;
+  static constexpr int ROOM = 224 * 1024 - XB - STAT;
   static constexpr int STAGES = ROOM / SB < 8 ? ROOM / SB : 8;
-  static constexpr int SMEM = 1024 + 2 * XB + STAGES * SB + STAT + 512;
+  static constexpr int SMEM = 1024 + XB + STAGES * SB + STAT + 512;
   static constexpr int THREADS = (kSoft + 4) * 32;
-  // TMEM columns: S and R (64 + 64, NB times), P and dS of each group (32 + 32), acc1, acc2
-  static constexpr int NB = SIDE == 1 && DH == 128 ? 1 : 2;
-  static constexpr int PD = NB * 128, ACC = PD + 128;
-  static_assert(STAGES >= 4 && ACC + (1 + SIDE) * DH <= 512, "ring and TMEM");
+  static_assert(STAGES >= 2 && X0 + XT * DH / 2 <= 512, "ring and TMEM");
 };
 
 template <int DH, bool BF16, int SIDE>
 __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
-    attend_back_kernel(const __grid_constant__ BackArgs a, const __grid_constant__ CUtensorMap x1map,
-                       const __grid_constant__ CUtensorMap x2map, const __grid_constant__ CUtensorMap y1map,
+    attend_back_kernel(const __grid_constant__ BackArgs a, const __grid_constant__ CUtensorMap y1map,
                        const __grid_constant__ CUtensorMap y2map) {
   using C = Back<DH, SIDE>;
   using T = Tile<DH>;
   constexpr int ST = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = smem + 2 * C::XB;
+  uint8_t* ring = smem + C::XB;
   float* stat = reinterpret_cast<float*>(ring + ST * C::SB);
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + ST * C::SB + C::STAT);
   uint64_t* empty = full + ST;
   uint64_t* clean = empty + ST;  // [ST]
   uint64_t* x_full = clean + ST;
-  uint64_t* s_full = x_full + 1;  // [2] each, a group: S and R computed
-  uint64_t* s_free = s_full + 2;  // S and R taken into registers
-  uint64_t* p_full = s_free + 2;  // P and dS written
-  uint64_t* p_free = p_full + 2;  // and read by the accumulations
-  uint64_t* acc_full = p_free + 2;
+  uint64_t* s_full = x_full + 1;  // S computed
+  uint64_t* r_full = s_full + 1;
+  uint64_t* s_free = r_full + 1;  // SIDE 0: S taken into registers
+  uint64_t* r_free = s_free + 1;
+  uint64_t* p_full = r_free + 1;  // SIDE 1: P written
+  uint64_t* d_full = p_full + 1;  // dS written
+  uint64_t* d_free = d_full + 1;  // SIDE 0: and read by the accumulation
+  uint64_t* acc_full = d_free + 1;
   uint64_t* dbar = acc_full + 1;  // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dbar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
@@ -167,18 +171,12 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&empty[i], 2);  // both issuers
       mbar_init(&clean[i], 1);
     }
-    mbar_init(x_full, SIDE == 0 ? kSoft : 1);
-    for (int u = 0; u < 2; ++u) {
-      mbar_init(&s_full[u], 1);
-      mbar_init(&s_free[u], kSoft / 2);
-      mbar_init(&p_full[u], kSoft / 2);
-      mbar_init(&p_free[u], 1);
-      mbar_init(&dbar[u], 1);
-    }
-    mbar_init(acc_full, 1);
+    for (uint64_t* bar : {x_full, s_free, r_free, p_full, d_full}) mbar_init(bar, kSoft);
+    for (uint64_t* bar : {s_full, r_full, d_free, &dbar[0], &dbar[1]}) mbar_init(bar, 1);
+    mbar_init(acc_full, 1 + SIDE);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -197,13 +195,6 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
 
   if (warp == kSoft + 2) {
     if (lane == 0 && n > 0) {  // loader
-      if constexpr (SIDE == 1) {
-        mbar_arrive_expect_tx(x_full, 2 * C::XB);
-        for (int x = 0; x < T::BOXES; ++x) {
-          tma_load_4d(smem + x * T::box_bytes(128), &x1map, x_full, x * T::COLS, tile * 128, kvh, b * a.x1_item);
-          tma_load_4d(smem + C::XB + x * T::box_bytes(128), &x2map, x_full, x * T::COLS, tile * 128, kvh, b * a.x2_item);
-        }
-      }
       int p = 0;
       for (; p < n; ++p) {
         const int st = p % ST;
@@ -221,83 +212,104 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
           tma_load_4d(dst + C::YB, &y2map, &full[st], x * T::COLS, row, head, b * a.y2_item);
         }
       }
-      if (*abort_flag) {
+      if (*abort_flag)
         for (int i = max(0, p - ST); i < p; ++i) bounded_wait(&full[i % ST], (i / ST) & 1);
-        if (SIDE == 1) bounded_wait(x_full, 0);
-      }
     }
-  } else if (warp == kSoft) {
-    if (lane == 0 && n > 0) {  // issuer of S and R
+  } else if (warp == kSoft || warp == kSoft + 1) {
+    if (lane == 0 && n > 0) {  // issuers: of S and acc2, of R and acc1
+      const bool second = warp == kSoft + 1;
       const uint32_t xb = smem_u32(smem), rb = smem_u32(ring);
-      constexpr uint32_t id_s = idesc_16bit(BF16, 128, kStep, false);
-      bool ok = mbar_wait(x_full, 0, abort_flag);
-      for (int i = 0; i < n && ok; ++i) {
-        const int st = i % ST, u = i & 1;
-        ok = mbar_wait(&full[st], (i / ST) & 1, abort_flag) &&
-             (SIDE == 1 || !a.masked || mbar_wait(&clean[st], (i / ST) & 1, abort_flag)) &&
-             (i < C::NB || mbar_wait(&s_free[(i - C::NB) & 1], ((i - C::NB) >> 1) & 1, abort_flag));
-        if (!ok) break;
+      constexpr uint32_t id_s = idesc_16bit(BF16, 128, kStep, false), id_a = idesc_16bit(BF16, 128, DH, true);
+      auto landed = [&](int i) { return mbar_wait(&full[i % ST], (i / ST) & 1, abort_flag); };
+      // S or R of step i
+      auto scores = [&](int i) {
         tc_fence_after();
-        const uint32_t y = rb + st * C::SB, s = tmem + (C::NB == 2 ? u * 128 : 0);
+        const uint32_t y = rb + i % ST * C::SB + (second ? C::YB : 0), d = tmem + (second ? C::R0 : 0);
 #pragma unroll
-        for (int ks = 0; ks < T::KSTEPS; ++ks)
-          mma_f16_ss(s, T::k_major(xb, 128, ks), T::k_major(y, kStep, ks), id_s, ks > 0);
+        for (int ks = 0; ks < T::KSTEPS; ++ks) {
+          const uint64_t yd = T::k_major(y, kStep, ks);
+          if (C::XT == 2 || (C::XT == 1 && !second))
+            mma_f16_ts(d, tmem + C::X0 + (second ? DH / 2 : 0) + ks * 8, yd, id_s, ks > 0);
+          else
+            mma_f16_ss(d, T::k_major(xb + (second && C::XT == 0 ? C::XS : 0), 128, ks), yd, id_s, ks > 0);
+        }
+        mma_commit(second ? r_full : s_full);
+      };
+      // acc2 += P Y2 or acc1 += dS Y1 of step i; rows 16 k .. of P and dS (SIDE 1: each warp's over its scores)
+      auto accumulate = [&](int i) {
+        tc_fence_after();
+        const uint32_t y = rb + i % ST * C::SB + (second ? 0 : C::YB);
+        const uint32_t from = tmem + (second ? (SIDE == 0 ? C::D0 : C::R0) : 0), to = tmem + C::ACC + (second ? 0 : DH);
 #pragma unroll
-        for (int ks = 0; ks < T::KSTEPS; ++ks)
-          mma_f16_ss(s + 64, T::k_major(xb + C::XB, 128, ks), T::k_major(y + C::YB, kStep, ks), id_s, ks > 0);
-        mma_commit(&s_full[u]);
+        for (int k = 0; k < kStep / 16; ++k)
+          mma_f16_ts(to, from + (SIDE == 0 ? k * 8 : (k >> 1) * 32 + (k & 1) * 8), T::mn_major(y, kStep, k), id_a,
+                     i > 0 || k > 0);
+        if (SIDE == 0) mma_commit(d_free);
+        mma_commit(&empty[i % ST]);
+      };
+      bool ok = mbar_wait(x_full, 0, abort_flag) && landed(0);
+      if (ok) scores(0);
+      if (SIDE == 0 && !second) {
+        if (ok) mma_commit(&empty[0]);
+        for (int i = 1; i < n && ok; ++i) {
+          ok = landed(i) && mbar_wait(s_free, (i - 1) & 1, abort_flag);
+          if (!ok) break;
+          scores(i);
+          mma_commit(&empty[i % ST]);
+        }
+      } else if (SIDE == 0) {
+        for (int i = 0; i < n && ok; ++i) {
+          if (i + 1 < n) {
+            ok = landed(i + 1) && mbar_wait(r_free, i & 1, abort_flag);
+            if (!ok) break;
+            scores(i + 1);
+          }
+          ok = (!a.masked || mbar_wait(&clean[i % ST], (i / ST) & 1, abort_flag)) && mbar_wait(d_full, i & 1, abort_flag);
+          if (!ok) break;
+          accumulate(i);
+        }
+        if (ok) mma_commit(acc_full);
+      } else {
+        for (int i = 0; i < n && ok; ++i) {
+          ok = (i + 1 == n || ST == 1 || landed(i + 1)) && mbar_wait(second ? d_full : p_full, i & 1, abort_flag);
+          if (!ok) break;
+          accumulate(i);
+          if (i + 1 < n) scores(i + 1);
+        }
+        if (ok) mma_commit(acc_full);
       }
       if (!ok) {
         give_up(SB_ERR_TIMEOUT_FULL);
-        mma_commit(&dbar[0]);
-        bounded_wait(&dbar[0], 0);
-      }
-    }
-  } else if (warp == kSoft + 1) {
-    if (lane == 0 && n > 0) {  // issuer of the accumulations
-      const uint32_t rb = smem_u32(ring);
-      constexpr uint32_t id_a = idesc_16bit(BF16, 128, DH, true);
-      bool ok = true;
-      for (int i = 0; i < n; ++i) {
-        const int st = i % ST, u = i & 1;
-        ok = mbar_wait(&p_full[u], (i >> 1) & 1, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t y = rb + st * C::SB, p = tmem + C::PD + u * 64;
-        if constexpr (SIDE == 1) {
-#pragma unroll
-          for (int k = 0; k < kStep / 16; ++k)
-            mma_f16_ts(tmem + C::ACC + DH, p + k * 8, T::mn_major(y + C::YB, kStep, k), id_a, i > 0 || k > 0);
-        }
-#pragma unroll
-        for (int k = 0; k < kStep / 16; ++k)
-          mma_f16_ts(tmem + C::ACC, p + 32 + k * 8, T::mn_major(y, kStep, k), id_a, i > 0 || k > 0);
-        mma_commit(&p_free[u]);
-        mma_commit(&empty[st]);
-      }
-      if (ok) {
-        mma_commit(acc_full);
-      } else {
-        give_up(SB_ERR_TIMEOUT_FULL);
-        mma_commit(&dbar[1]);
-        bounded_wait(&dbar[1], 0);
+        mma_commit(&dbar[second]);
+        bounded_wait(&dbar[second], 0);
       }
     }
   } else if (warp == kSoft + 3) {
-    if (SIDE == 0 && a.masked) {  // cleaner: k's rows of keys that take no part
+    if (SIDE == 0 && a.masked) {  // cleaner: k's rows of keys that take no part, mask bytes two tiles ahead
+      uint32_t next[2][kStep / 32];
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int x = 0; x < kStep / 32; ++x) next[y][x] = a.mask.ask(b, (first + y) * kStep + 32 * x, count);
+#pragma unroll 2
       for (int i = 0; i < n; ++i) {
         const int st = i % ST, j0 = (first + i) * kStep;
+        uint32_t w[kStep / 32];
+#pragma unroll
+        for (int x = 0; x < kStep / 32; ++x) {
+          w[x] = a.mask.told(next[i & 1][x], j0 + 32 * x, count);
+          next[i & 1][x] = a.mask.ask(b, j0 + 2 * kStep + 32 * x, count);
+        }
         if (!warp_wait(&full[st], (i / ST) & 1, abort_flag)) {
           if (lane == 0) give_up(SB_ERR_TIMEOUT_FULL);
           break;
         }
         bool touched = false;
-#pragma unroll 1
+#pragma unroll
         for (int x = 0; x < kStep / 32; ++x) {
-          const uint32_t w = a.mask.word(b, j0 + 32 * x, count);
-          if (w == 0xFFFFFFFFu) continue;
+          if (w[x] == 0xFFFFFFFFu) continue;
           touched = true;
-          if (!(w >> lane & 1u))
+          if (!(w[x] >> lane & 1u))
             for (int c = 0; c < DH / 8; ++c)
               *reinterpret_cast<uint4*>(ring + st * C::SB + T::chunk(kStep, 32 * x + lane, c)) = make_uint4(0, 0, 0, 0);
         }
@@ -306,25 +318,40 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
       }
     }
   } else {
-    const int u = warp >> 3, hf = warp >> 2 & 1, quad = warp & 3;
+    const int cg = warp >> 2, quad = warp & 3;  // streamed rows 32 cg .., held rows 32 quad ..
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const uint32_t s_at = tmem + lanes + (C::NB == 2 ? u * 128 : 0) + hf * 32, r_at = s_at + 64;
-    const uint32_t p_at = tmem + lanes + C::PD + u * 64 + hf * 16, d_at = p_at + 32;
+    const uint32_t s_at = tmem + lanes + cg * 32, r_at = s_at + C::R0;
+    const uint32_t p_at = s_at, d_at = SIDE == 0 ? tmem + lanes + C::D0 + cg * 16 : r_at;
+    const int u = cg >> 1, hf = cg & 1;  // what it loads and stores: operand or accumulator, half of its channels
     const int x = tile * 128 + quad * 32 + lane;  // held row: query row of the group, or key
     const int rows = SIDE == 0 ? a.group * a.Tq : a.Tk;
     const int tq = SIDE == 0 ? x / a.group : 0, h = kvh * a.group + (SIDE == 0 ? x - tq * a.group : 0);
     const bool live = x < rows;
     bool takes = true;  // SIDE 1: this key takes part
     if (SIDE == 1) takes = x < count && (!a.mask.valid || a.mask.valid[b * a.mask.valid_img + x] != 0);
-    if constexpr (SIDE == 0) {
-      const View& src = u == 0 ? a.q : a.dout;
-      const uint4* from = reinterpret_cast<const uint4*>(static_cast<const __half*>(src.p) + b * src.img + tq * src.row +
-                                                         (long long)h * DH);
+    {  // the held rows: X1 by the first group of warps, X2 by the second, half of the channels a warp
+      const View& src = SIDE == 0 ? (u == 0 ? a.q : a.dout) : u == 0 ? a.k : a.v;
+      const long long at = SIDE == 0 ? tq * src.row + (long long)h * DH : x * src.row + (long long)kvh * DH;
+      const uint4* from = reinterpret_cast<const uint4*>(static_cast<const __half*>(src.p) + b * src.img + at) +
+                          hf * (DH / 16);
+      uint4 v[DH / 16];
 #pragma unroll
-      for (int c = hf * (DH / 16); c < (hf + 1) * (DH / 16); ++c)
-        *reinterpret_cast<uint4*>(smem + u * C::XB + T::chunk(128, quad * 32 + lane, c)) =
-            live ? from[c] : make_uint4(0, 0, 0, 0);
-      fence_proxy_async_smem();
+      for (int c = 0; c < DH / 16; ++c) v[c] = live ? from[c] : make_uint4(0, 0, 0, 0);
+      if (u < C::XT) {
+        const uint32_t to = tmem + lanes + C::X0 + u * (DH / 2) + hf * (DH / 4);
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+        __syncwarp();
+        if constexpr (DH == 128) tmem_st32(to, w);
+        else if constexpr (DH == 64) tmem_st16(to, w);
+        else tmem_st8(to, w);
+        tmem_st_wait();
+        tc_fence_before();
+      } else {
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c)
+          *reinterpret_cast<uint4*>(smem + (u - C::XT) * C::XS + T::chunk(128, quad * 32 + lane, hf * (DH / 16) + c)) = v[c];
+        fence_proxy_async_smem();
+      }
       warp_arrive(x_full);
     }
     // P is held as 2^lift P, dS as F dS with F = f 2^lift
@@ -345,74 +372,85 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
     float* mine = stat + warp * 128;  // [2][L, D][32]
     float next[2];
     auto fetch = [&](int i) {  // SIDE 1: L and D of step i's queries, one a lane
-      const int step = first + i, t = step % q_tiles * kStep + hf * 32 + lane;
+      const int step = first + i, t = step % q_tiles * kStep + cg * 32 + lane;
       const long long at = ((long long)b * a.H + kvh * a.group + step / q_tiles) * a.Tq + t;
       next[0] = t < a.Tq ? a.lse2[at] - lift : INFINITY;
       next[1] = t < a.Tq ? a.delta[at] * f : 0.f;
     };
-    if (SIDE == 1 && u < n) fetch(u);
-    uint32_t byte = SIDE == 0 ? a.mask.ask(b, (first + u) * kStep + hf * 32, count) : 0u;
+    if (SIDE == 1 && n > 0) fetch(0);
+    uint32_t byte = SIDE == 0 ? a.mask.ask(b, first * kStep + cg * 32, count) : 0u;
     bool ok = true;
-    for (int i = u; i < n; i += 2) {
-      uint32_t w = 0xFFFFFFFFu;
-      const float* st = mine + ((i >> 1) & 1) * 64;
+    for (int i = 0; i < n; ++i) {
+      uint32_t w = takes ? 0xFFFFFFFFu : 0u;
+      const float* st = mine + (i & 1) * 64;
       if constexpr (SIDE == 0) {
-        const int j0 = (first + i) * kStep + hf * 32;
+        const int j0 = (first + i) * kStep + cg * 32;
         w = a.mask.told(byte, j0, count);
-        byte = a.mask.ask(b, j0 + 2 * kStep, count);
+        byte = a.mask.ask(b, j0 + kStep, count);
       } else {
-        float* put = mine + ((i >> 1) & 1) * 64;
+        float* put = mine + (i & 1) * 64;
         put[lane] = next[0];
         put[32 + lane] = next[1];
         __syncwarp();
-        if (i + 2 < n) fetch(i + 2);
+        if (i + 1 < n) fetch(i + 1);
       }
-      ok = warp_wait(&s_full[u], (i >> 1) & 1, abort_flag);
+      ok = warp_wait(s_full, i & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      uint32_t s[2][16], r[2][16];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        tmem_ld16(s_at + 16 * q, s[q]);
-        tmem_ld16(r_at + 16 * q, r[q]);
-      }
+      uint32_t s[32];
+      tmem_ld32(s_at, s);
       tmem_ld_wait();
-      tc_fence_before();
-      warp_arrive(&s_free[u]);
-      uint32_t pp[2][8], pd[2][8];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          float p[2], d[2];
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int at = 16 * q + j + y;
-            const float lj = SIDE == 0 ? l2 : st[at], dj = SIDE == 0 ? df : st[32 + at];
-            p[y] = exp2_hw(fmaf(__uint_as_float(s[q][j + y]), sl, -lj));
-            d[y] = p[y] * fmaf(__uint_as_float(r[q][j + y]), f, -dj);
-          }
-          if (SIDE == 0 ? w != 0xFFFFFFFFu : !takes) {
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-              if (SIDE == 1 || !(w >> (16 * q + j + y) & 1u)) p[y] = d[y] = 0.f;
-          }
-          if (SIDE == 1) pp[q][j / 2] = pack16<BF16>(p[0], p[1]);
-          pd[q][j / 2] = pack16<BF16>(d[0], d[1]);
-        }
-        if (q == 0 && i > 1) {  // the accumulations of the group's last step have read P and dS
-          ok = warp_wait(&p_free[u], ((i >> 1) - 1) & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-        }
-        __syncwarp();
-        if (SIDE == 1) tmem_st8(p_at + 8 * q, pp[q]);
-        tmem_st8(d_at + 8 * q, pd[q]);
+      if (SIDE == 0) {
+        tc_fence_before();
+        warp_arrive(s_free);
       }
+      float p[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) p[j] = exp2_hw(fmaf(__uint_as_float(s[j]), sl, -(SIDE == 0 ? l2 : st[j])));
+      if (w != 0xFFFFFFFFu) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (!(w >> j & 1u)) p[j] = 0.f;
+      }
+      if (SIDE == 1) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) pk[j] = pack16<BF16>(p[2 * j], p[2 * j + 1]);
+        __syncwarp();
+        tmem_st16(p_at, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        warp_arrive(p_full);
+      }
+      ok = warp_wait(r_full, i & 1, abort_flag);
       if (!ok) break;
+      tc_fence_after();
+      tmem_ld32(r_at, s);
+      tmem_ld_wait();
+      if (SIDE == 0) {
+        tc_fence_before();
+        warp_arrive(r_free);
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) p[j] *= fmaf(__uint_as_float(s[j]), f, -(SIDE == 0 ? df : st[32 + j]));
+      if (w != 0xFFFFFFFFu) {  // R may be NaN there
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (!(w >> j & 1u)) p[j] = 0.f;
+      }
+      uint32_t pk[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) pk[j] = pack16<BF16>(p[2 * j], p[2 * j + 1]);
+      if (SIDE == 0 && i > 0) {  // the last step's accumulation has read its dS
+        ok = warp_wait(d_free, (i - 1) & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      __syncwarp();
+      tmem_st16(d_at, pk);
       tmem_st_wait();
       tc_fence_before();
-      warp_arrive(&p_full[u]);
+      warp_arrive(d_full);
     }
     if (ok && n > 0) ok = warp_wait(acc_full, 0, abort_flag);
     if (!ok) {
@@ -497,7 +535,7 @@ struct BackPlan {
 // Steps are split where the CTAs' last wave would leave more SMs idle than the splits cost (about
 // kStart steps a CTA to start and end, as much again for the join).
 SidePlan side_plan(long long items, long long x_rows, long long steps, long long part_rows, int sms) {
-  constexpr int kStart = 8, kMost = 64;
+  constexpr int kStart = 4, kMost = 64;
   SidePlan p;
   p.x_tiles = (int)((x_rows + 127) / 128);
   p.steps = (int)steps;
@@ -530,7 +568,7 @@ BackPlan back_plan(int B, int H, int Hkv, int dh, int Tq, int Tk, int sms) {
 }
 
 template <int DH, bool BF16, int SIDE>
-cudaError_t launch_side(BackArgs a, const SidePlan& p, const CUtensorMap (&m)[4], cudaStream_t st) {
+cudaError_t launch_side(BackArgs a, const SidePlan& p, const CUtensorMap& y1, const CUtensorMap& y2, cudaStream_t st) {
   using C = Back<DH, SIDE>;
   static bool ready[64];
   cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&attend_back_kernel<DH, BF16, SIDE>), C::SMEM, ready);
@@ -539,7 +577,7 @@ cudaError_t launch_side(BackArgs a, const SidePlan& p, const CUtensorMap (&m)[4]
   a.splits = p.splits;
   a.steps = p.steps;
   a.part_rows = p.part_rows;
-  attend_back_kernel<DH, BF16, SIDE><<<(unsigned)(p.units * p.splits), C::THREADS, C::SMEM, st>>>(a, m[0], m[1], m[2], m[3]);
+  attend_back_kernel<DH, BF16, SIDE><<<(unsigned)(p.units * p.splits), C::THREADS, C::SMEM, st>>>(a, y1, y2);
   e = cudaGetLastError();
   if (e != cudaSuccess || p.splits == 1) return e;
   const long long threads = p.part_rows * (DH / 8);
@@ -555,27 +593,20 @@ int launch_back(BackArgs& a, const BackPlan& p, cudaStream_t st) {
   if (!BF16 && cudaMemsetAsync(a.top, 0, (size_t)a.B * a.Hkv * 8, st) != cudaSuccess)
     return record_error(SB_ECUDA, "sb_cross_attention_backward: memset");
   attend_back_rows_kernel<DH><<<grid, 256, 0, st>>>(a);
-  CUtensorMap m[4];
-  // SIDE 0 streams k, v (its held rows are gathered by threads); SIDE 1 holds k, v and streams q, dout
-  if (!xattn_tensor_map(&m[2], a.k, a.dt, a.B, a.Tk, a.Hkv, DH, kStep) ||
-      !xattn_tensor_map(&m[3], a.v, a.dt, a.B, a.Tk, a.Hkv, DH, kStep))
+  CUtensorMap y1, y2;
+  if (!xattn_tensor_map(&y1, a.k, a.dt, a.B, a.Tk, a.Hkv, DH, kStep) ||
+      !xattn_tensor_map(&y2, a.v, a.dt, a.B, a.Tk, a.Hkv, DH, kStep))
     return record_error(SB_EINVAL, "sb_cross_attention_backward: tensor map of k or v");
-  m[0] = m[2];
-  m[1] = m[3];
   a.y1_item = a.k.img != 0;
   a.y2_item = a.v.img != 0;
-  cudaError_t e = launch_side<DH, BF16, 0>(a, p.side[0], m, st);
+  cudaError_t e = launch_side<DH, BF16, 0>(a, p.side[0], y1, y2, st);
   if (e != cudaSuccess) return record_error(SB_ECUDA, cudaGetErrorString(e));
-  if (!xattn_tensor_map(&m[0], a.k, a.dt, a.B, a.Tk, a.Hkv, DH, 128) ||
-      !xattn_tensor_map(&m[1], a.v, a.dt, a.B, a.Tk, a.Hkv, DH, 128) ||
-      !xattn_tensor_map(&m[2], a.q, a.dt, a.B, a.Tq, a.H, DH, kStep) ||
-      !xattn_tensor_map(&m[3], a.dout, a.dt, a.B, a.Tq, a.H, DH, kStep))
-    return record_error(SB_EINVAL, "sb_cross_attention_backward: tensor map of q, dout, k or v");
-  a.x1_item = a.y1_item;
-  a.x2_item = a.y2_item;
+  if (!xattn_tensor_map(&y1, a.q, a.dt, a.B, a.Tq, a.H, DH, kStep) ||
+      !xattn_tensor_map(&y2, a.dout, a.dt, a.B, a.Tq, a.H, DH, kStep))
+    return record_error(SB_EINVAL, "sb_cross_attention_backward: tensor map of q or dout");
   a.y1_item = a.q.img != 0;
   a.y2_item = a.dout.img != 0;
-  e = launch_side<DH, BF16, 1>(a, p.side[1], m, st);
+  e = launch_side<DH, BF16, 1>(a, p.side[1], y1, y2, st);
   return e == cudaSuccess ? SB_OK : record_error(SB_ECUDA, cudaGetErrorString(e));
 }
 
