@@ -46,14 +46,27 @@ SB_DEV void turn_of(const RopeArgs& a, long long at, int p, float& sn, float& cs
   if (a.inverse) sn = -sn;
 }
 
-template <bool VEC>
+constexpr int kAhead = 2;
+
+// VEC: rows in vectors of eight, of type DT; otherwise element by element
+template <bool VEC, int DT>
 __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeArgs a) {
+  const int dt = VEC ? DT : a.dt;
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= a.units) return;
-  const int slot = (int)(i % a.slots);
-  const long long token = i / a.slots;
-  const int t = (int)(token % a.T);
-  const long long b = token / a.T;
+  int slot, t;
+  long long b;
+  if (a.units <= 0x7FFFFFFF) {  // a 64-bit division costs as much as a pair's trigonometry
+    const uint32_t token = (uint32_t)i / (uint32_t)a.slots;
+    slot = (int)((uint32_t)i - token * (uint32_t)a.slots);
+    b = token / (uint32_t)a.T;
+    t = (int)(token - (uint32_t)b * (uint32_t)a.T);
+  } else {
+    const long long token = i / a.slots;
+    slot = (int)(i - token * a.slots);
+    b = token / a.T;
+    t = (int)(token - b * a.T);
+  }
   const long long xr = b * a.x_img + t * a.x_row, orow = b * a.o_img + t * a.o_row;
   const long long at = b * a.pos_img + (long long)t * a.A;
   const int h0 = blockIdx.y * a.heads_per, h1 = min(a.H, h0 + a.heads_per);
@@ -61,10 +74,14 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeA
     const int groups = a.R >> 3;
     if (slot >= groups) {  // channels that no pair covers
       const int c = 2 * a.R + (slot - groups) * 8;
-      for (int h = h0; h < h1; ++h) {
-        float v[8];
-        unpack8(load_raw8(a.x, a.dt, xr + (long long)h * a.dh + c), a.dt, v);
-        store8(a.out, a.dt, orow + (long long)h * a.dh + c, v);
+      for (int h = h0; h < h1; h += 2 * kAhead) {
+        Raw8 r[2 * kAhead];
+#pragma unroll
+        for (int y = 0; y < 2 * kAhead; ++y)
+          if (h + y < h1) r[y] = load_raw8(a.x, dt, xr + (long long)(h + y) * a.dh + c);
+#pragma unroll
+        for (int y = 0; y < 2 * kAhead; ++y)
+          if (h + y < h1) store_raw8(a.out, dt, orow + (long long)(h + y) * a.dh + c, r[y]);
       }
       return;
     }
@@ -74,30 +91,42 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeA
     for (int u = 0; u < 8; ++u) turn_of(a, at, p0 + u, sn[u], cs[u]);
     // the eight pairs' first and second vectors: (p0.., R + p0..) or the 16 channels from 2 p0 on
     const int c0 = a.pairs ? 2 * p0 : p0, c1 = a.pairs ? 2 * p0 + 8 : a.R + p0;
-#pragma unroll 4
-    for (int h = h0; h < h1; ++h) {
-      const long long xo = xr + (long long)h * a.dh, oo = orow + (long long)h * a.dh;
-      const Raw8 r0 = load_raw8(a.x, a.dt, xo + c0), r1 = load_raw8(a.x, a.dt, xo + c1);
-      float u[8], v[8], y0[8], y1[8];
-      unpack8(r0, a.dt, u);
-      unpack8(r1, a.dt, v);
-      if (a.pairs) {
+    // two heads' loads before the first store: x and out may be the same rows, so the compiler keeps
+    // the order of what is written here
+    for (int h = h0; h < h1; h += kAhead) {
+      Raw8 r0[kAhead], r1[kAhead];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          y0[2 * k] = u[2 * k] * cs[k] - u[2 * k + 1] * sn[k];
-          y0[2 * k + 1] = u[2 * k] * sn[k] + u[2 * k + 1] * cs[k];
-          y1[2 * k] = v[2 * k] * cs[4 + k] - v[2 * k + 1] * sn[4 + k];
-          y1[2 * k + 1] = v[2 * k] * sn[4 + k] + v[2 * k + 1] * cs[4 + k];
+      for (int y = 0; y < kAhead; ++y)
+        if (h + y < h1) {
+          const long long xo = xr + (long long)(h + y) * a.dh;
+          r0[y] = load_raw8(a.x, dt, xo + c0);
+          r1[y] = load_raw8(a.x, dt, xo + c1);
         }
-      } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          y0[k] = u[k] * cs[k] - v[k] * sn[k];
-          y1[k] = u[k] * sn[k] + v[k] * cs[k];
+      for (int y = 0; y < kAhead; ++y) {
+        if (h + y >= h1) break;
+        const long long oo = orow + (long long)(h + y) * a.dh;
+        float u[8], v[8], y0[8], y1[8];
+        unpack8(r0[y], dt, u);
+        unpack8(r1[y], dt, v);
+        if (a.pairs) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            y0[2 * k] = u[2 * k] * cs[k] - u[2 * k + 1] * sn[k];
+            y0[2 * k + 1] = u[2 * k] * sn[k] + u[2 * k + 1] * cs[k];
+            y1[2 * k] = v[2 * k] * cs[4 + k] - v[2 * k + 1] * sn[4 + k];
+            y1[2 * k + 1] = v[2 * k] * sn[4 + k] + v[2 * k + 1] * cs[4 + k];
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            y0[k] = u[k] * cs[k] - v[k] * sn[k];
+            y1[k] = u[k] * sn[k] + v[k] * cs[k];
+          }
         }
+        store8(a.out, dt, oo + c0, y0);
+        store8(a.out, dt, oo + c1, y1);
       }
-      store8(a.out, a.dt, oo + c0, y0);
-      store8(a.out, a.dt, oo + c1, y1);
     }
   } else {
     if (slot >= a.R) {
@@ -151,15 +180,15 @@ extern "C" int sb_rope_axes(const void* x, long long x_row, long long x_img, int
   a.units = (long long)B * T * a.slots;
   const long long blocks = (a.units + 255) / 256;
   if (blocks > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_rope_axes: too many rows");
-  // split the heads until every SM has about two blocks
+  // split the heads until every SM has about eight blocks
   int parts = 1;
-  while (parts < H && parts < 32 && blocks * parts < 296) ++parts;
+  while (parts < H && parts < 32 && blocks * parts < 1184) ++parts;
   a.heads_per = (H + parts - 1) / parts;
   const dim3 grid((unsigned)blocks, (unsigned)((H + a.heads_per - 1) / a.heads_per));
-  if (vec)
-    rope_kernel<true><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
-  else
-    rope_kernel<false><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
+  auto kernel = !vec               ? rope_kernel<false, 0>
+                : dtype == SB_F32 ? rope_kernel<true, SB_F32>
+                : dtype == SB_F16 ? rope_kernel<true, SB_F16> : rope_kernel<true, SB_BF16>;
+  kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(a);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return record_error(SB_ECUDA, cudaGetErrorString(e));
   return SB_OK;

@@ -102,6 +102,15 @@ SB_DEV void store8(void* p, int dt, long long i, const float (&v)[8]) {
                    pack_pair(v[6], v[7], dt));
   }
 }
+SB_DEV void store_raw8(void* p, int dt, long long i, const Raw8& r) {
+  if (dt == SB_F32) {
+    uint4* q = reinterpret_cast<uint4*>(static_cast<float*>(p) + i);
+    q[0] = r.lo;
+    q[1] = r.hi;
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<__half*>(p) + i) = r.lo;
+  }
+}
 SB_DEV void store8_tail(void* p, int dt, long long i, const float (&v)[8], int n) {
 #pragma unroll
   for (int u = 0; u < 8; ++u)
