@@ -474,8 +474,9 @@ SB_API int sb_cross_attention(const void* q, long long q_row, long long q_img, c
                               long long work_bytes, void* stream);
 
 /* Bytes of workspace that sb_cross_attention (backward = 0) or sb_cross_attention_backward
- * (backward = 1) needs for these sizes on the current device (0: work may be NULL). */
-SB_API int sb_cross_attention_work(int backward, int B, int H, int Hkv, int dh, int Tq, int Tk, long long* bytes);
+ * (backward = 1) needs for these sizes on the current device (0: work may be NULL); masked: with valid. */
+SB_API int sb_cross_attention_work(int backward, int masked, int B, int H, int Hkv, int dh, int Tq, int Tk,
+                                   long long* bytes);
 
 /* Gradients of sb_cross_attention: dq [B][Tq][H*dh], dk, dv [B][Tk][Hkv*dh] (every element is
  * written; keys that take no part get zeros) from dout and the forward pass's out and lse. Sums

@@ -108,7 +108,7 @@ PROTOTYPES = {
     "sb_box_dec": (_I, [_I, _P, _LL, _P, _P, _LL, _P, _LL, _I, _P, C.c_float, _P, _P, _P, _LL, _I, _P]),
     "sb_l2norm_rows": (_I, [_P, _LL, _I, _I, _P, _LL, _P]),
     "sb_cross_attention": (_I, [_P, _LL, _LL] * 3 + [_I] * 7 + [C.c_float, _P, _P, _LL, _P, _LL, _LL, _P, _P, _LL, _P]),
-    "sb_cross_attention_work": (_I, [_I] * 7 + [C.POINTER(_LL)]),
+    "sb_cross_attention_work": (_I, [_I] * 8 + [C.POINTER(_LL)]),
     "sb_cross_attention_backward": (_I, [_P, _LL, _LL] * 5 + [_P] + [_I] * 7 + [C.c_float, _P, _P, _LL]
                                     + [_P, _LL, _LL] * 3 + [_P, _LL, _P]),
     "sb_rope_axes": (_I, [_P, _LL, _LL, _I, _I, _I, _I, _I, _P, _I, _LL, _I, _P, _P, _I, _I, _I, _P, _LL, _LL, _P]),

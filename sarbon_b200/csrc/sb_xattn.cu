@@ -570,6 +570,26 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
   if (a.lse && c == 0) a.lse[rr] = sum != 0.f ? top + logf(sum) : -INFINITY;
 }
 
+// One CTA an item, from the end on: images are padded behind, cameras are off.
+__global__ void __launch_bounds__(1024) count_keys_kernel(KeyMask mask, int* counts) {
+  constexpr int kEach = 8;
+  const int b = blockIdx.x;
+  __shared__ int last;
+  if (threadIdx.x == 0) last = 0;
+  __syncthreads();
+  for (int end = mask.count(b); end > 0; end -= 1024 * kEach) {
+    int mine = 0;
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int j = end - 1 - u * 1024 - (int)threadIdx.x;
+      if (j >= 0 && mask.valid[b * mask.valid_img + j] != 0) mine = max(mine, j + 1);
+    }
+    if (mine > 0) atomicMax(&last, mine);
+    if (__syncthreads_or(mine > 0)) break;
+  }
+  if (threadIdx.x == 0) counts[b] = last;
+}
+
 // No keys at all: zero rows and L = -inf.
 __global__ void attend_none_kernel(OutView o, float* lse, int H, int Tq, int dh, long long n) {
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -686,6 +706,11 @@ bool xattn_tensor_map(CUtensorMap* map, const View& v, int dtype, int B, int T, 
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+cudaError_t count_keys(const KeyMask& mask, int B, int* counts, cudaStream_t st) {
+  count_keys_kernel<<<(unsigned)B, 1024, 0, st>>>(mask, counts);
+  return cudaGetLastError();
+}
+
 int xattn_error(int clear, int* flags) {
   const int zero = 0;
   if (cudaMemcpyFromSymbol(flags, g_xattn_error, sizeof(int)) != cudaSuccess) return -1;
@@ -717,7 +742,7 @@ int xattn_sms() {
 
 using namespace sb;
 
-extern "C" int sb_cross_attention_work(int backward, int B, int H, int Hkv, int dh, int Tq, int Tk, long long* bytes) {
+extern "C" int sb_cross_attention_work(int backward, int masked, int B, int H, int Hkv, int dh, int Tq, int Tk, long long* bytes) {
   if (!bytes || !xattn_sizes_ok(SB_F16, B, H, Hkv, dh, Tq, Tk))
     return record_error(SB_EINVAL, "sb_cross_attention_work: arguments");
   *bytes = 0;
@@ -725,11 +750,11 @@ extern "C" int sb_cross_attention_work(int backward, int B, int H, int Hkv, int 
   const int sms = xattn_sms();
   if (sms == 0) return record_error(SB_ECUDA, "sb_cross_attention_work: device");
   if (backward) {
-    *bytes = xattn_back_work(B, H, Hkv, dh, Tq, Tk, sms);
+    *bytes = counts_bytes(masked, B) + xattn_back_work(B, H, Hkv, dh, Tq, Tk, sms);
     return SB_OK;
   }
   const FwdPlan p = fwd_plan(B, H, Hkv, Tq, Tk, sms);
-  if (p.splits > 1) *bytes = (long long)p.splits * B * H * Tq * (dh + 1) * 4;
+  *bytes = counts_bytes(masked, B) + (p.splits > 1 ? (long long)p.splits * B * H * Tq * (dh + 1) * 4 : 0);
   return SB_OK;
 }
 
@@ -754,7 +779,8 @@ extern "C" int sb_cross_attention(const void* q, long long q_row, long long q_im
   const int sms = xattn_sms();
   if (sms == 0) return record_error(SB_ECUDA, "sb_cross_attention: device");
   const FwdPlan p = fwd_plan(B, H, Hkv, Tq, Tk, sms);
-  const long long need = p.splits > 1 ? (long long)p.splits * B * H * Tq * (dh + 1) * 4 : 0;
+  const long long counts = counts_bytes(valid != nullptr, B);
+  const long long need = counts + (p.splits > 1 ? (long long)p.splits * B * H * Tq * (dh + 1) * 4 : 0);
   if (need > 0 && (!work || work_bytes < need || (reinterpret_cast<uintptr_t>(work) & 15) != 0))
     return record_error(SB_EINVAL, "sb_cross_attention: workspace (sb_cross_attention_work bytes, 16-byte aligned)");
   if (p.units * p.splits > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_cross_attention: too many items");
@@ -769,7 +795,13 @@ extern "C" int sb_cross_attention(const void* q, long long q_row, long long q_im
   a.masked = lens || valid;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.all_rows = (long long)B * H * Tq;
-  a.part_o = static_cast<float*>(work);
+  if (valid) {
+    int* last = static_cast<int*>(work);
+    const cudaError_t e = count_keys(a.mask, B, last, st);
+    if (e != cudaSuccess) return record_error(SB_ECUDA, cudaGetErrorString(e));
+    a.mask.lens = last;
+  }
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(work) + counts);
   a.part_l = a.part_o + (long long)p.splits * a.all_rows * dh;
   CUtensorMap km, vm;
   const int box = p.few ? few_keys(dh) : KT;

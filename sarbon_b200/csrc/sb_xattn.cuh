@@ -207,6 +207,9 @@ bool xattn_tensor_map(CUtensorMap* map, const View& v, int dtype, int B, int T, 
 bool xattn_sizes_ok(int dtype, int B, int H, int Hkv, int dh, int Tq, int Tk);
 // 16-byte rows whose strides fit a tensor map
 bool xattn_view_ok(const void* p, long long row, long long img);
+// counts[b] = 1 + the last key of item b that takes part (0: none): keys behind it are never looked at.
+constexpr long long counts_bytes(int masked, int B) { return masked ? ((long long)B * 4 + 15) / 16 * 16 : 0; }
+cudaError_t count_keys(const KeyMask& mask, int B, int* counts, cudaStream_t st);
 // Few query rows an (item, key head): the key splits of its kernel, its launch (partial rows where splits
 // > 1), and the join of the partial rows.
 constexpr int kFewRows = 16;

@@ -679,16 +679,23 @@ extern "C" int sb_cross_attention_backward(const void* dout, long long do_row, l
   const int sms = xattn_sms();
   if (sms == 0) return record_error(SB_ECUDA, "sb_cross_attention_backward: device");
   const BackPlan p = back_plan(B, H, Hkv, dh, Tq, Tk, sms);
-  if (!work || work_bytes < p.bytes || (reinterpret_cast<uintptr_t>(work) & 15) != 0)
+  const long long counts = counts_bytes(valid != nullptr, B);
+  if (!work || work_bytes < counts + p.bytes || (reinterpret_cast<uintptr_t>(work) & 15) != 0)
     return record_error(SB_EINVAL,
                         "sb_cross_attention_backward: workspace (sb_cross_attention_work bytes, 16-byte aligned)");
   for (const SidePlan& s : p.side)
     if (s.units * s.splits > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_cross_attention_backward: too many items");
   if ((long long)B * (H + Hkv) > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_cross_attention_backward: too many items");
-  a.lse2 = static_cast<float*>(work);
+  if (valid) {
+    int* last = static_cast<int*>(work);
+    const cudaError_t e = count_keys(a.mask, B, last, st);
+    if (e != cudaSuccess) return record_error(SB_ECUDA, cudaGetErrorString(e));
+    a.mask.lens = last;
+  }
+  a.lse2 = reinterpret_cast<float*>(static_cast<char*>(work) + counts);
   a.delta = a.lse2 + p.rows;
   a.top = reinterpret_cast<unsigned*>(a.delta + p.rows);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(work) + (p.rows * 8 + (long long)B * Hkv * 8 + 15) / 16 * 16);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(work) + counts + (p.rows * 8 + (long long)B * Hkv * 8 + 15) / 16 * 16);
   if (dtype == SB_BF16)
     return dh == 32 ? launch_back<32, true>(a, p, st) : dh == 64 ? launch_back<64, true>(a, p, st)
                                                                  : launch_back<128, true>(a, p, st);

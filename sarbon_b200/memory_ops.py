@@ -182,7 +182,7 @@ def cross_attention(q, k, v, heads, kv_heads=None, lens=None, valid=None, scale=
         out, op = _new(q, qs, dtype)
     if b == 0 or tq == 0:
         return out
-    hold, work, size = _work("sb_cross_attention_work", index, 0, b, heads, kv_heads, dim, tq, tk)
+    hold, work, size = _work("sb_cross_attention_work", index, 0, valid is not None, b, heads, kv_heads, dim, tq, tk)
     _launch("sb_cross_attention", index, *qp, *kp, *vp, DTYPES[dtype], b, heads, kv_heads, dim, tq, tk, scale, *masks,
             *op, None if lse is None else lse.data_ptr(), work, size)
     return out
@@ -210,7 +210,7 @@ def cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=None, lens
     dv, dvp = _new(v, ks, dtype) if dv is None else (dv, _rows(dv, "dv", ks, dtype))
     if b == 0 or (tq == 0 and tk == 0):
         return dq, dk, dv
-    hold, work, size = _work("sb_cross_attention_work", index, 1, b, heads, kv_heads, dim, tq, tk)
+    hold, work, size = _work("sb_cross_attention_work", index, 1, valid is not None, b, heads, kv_heads, dim, tq, tk)
     _launch("sb_cross_attention_backward", index, *views, lse.data_ptr(), DTYPES[dtype], b, heads, kv_heads, dim, tq, tk,
             scale, *masks, *dqp, *dkp, *dvp, work, size)
     return dq, dk, dv

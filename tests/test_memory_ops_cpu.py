@@ -104,7 +104,7 @@ def test_library_refuses():
                 dict(q=C.c_void_p(8))):
         assert attention(**bad) == _lib.SB_EINVAL, bad
     assert attention(b=0) == _lib.SB_OK and attention(tq=0) == _lib.SB_OK
-    assert lib.sb_cross_attention_work(0, 1, 2, 1, 48, 4, 4, C.byref(n)) == _lib.SB_EINVAL
+    assert lib.sb_cross_attention_work(0, 0, 1, 2, 1, 48, 4, 4, C.byref(n)) == _lib.SB_EINVAL
     assert lib.sb_gated_norm_work(1, 1, 9000, C.byref(n)) == _lib.SB_EINVAL
     assert lib.sb_rope_axes(one, 64, 64, 0, 1, 1, 1, 64, one, 0, 0, 1, one, one, 33, 0, 0, one, 64, 64, None) == _lib.SB_EINVAL
     assert lib.sb_rope_axes(None, 64, 64, 0, 1, 1, 1, 64, one, 0, 0, 1, one, one, 32, 0, 0, one, 64, 64, None) == _lib.SB_EINVAL
