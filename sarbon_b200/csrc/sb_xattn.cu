@@ -125,9 +125,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int kvh = idx % a.Hkv, b = idx / a.Hkv;
   const bool two = pair * 256 + 128 < a.rows;  // two tiles of rows
   const int count = a.mask.count(b);
-  const int each = (a.key_tiles + a.splits - 1) / a.splits;
-  const int first = split * each;
-  const int n = max(0, min(min(first + each, a.key_tiles), (count + KT - 1) / KT) - first);
+  // the item's own key tiles, split evenly
+  const int all_tiles = (count + KT - 1) / KT, each = (all_tiles + a.splits - 1) / a.splits;
+  const int first = min(split * each, all_tiles), n = min(first + each, all_tiles) - first;
   const int KS = two ? C::K2 : C::K1, VS = two ? C::V2 : C::V1;
   uint8_t* k_ring = smem + (two ? 2 : 1) * C::QB;
   uint8_t* v_ring = k_ring + KS * C::SB;

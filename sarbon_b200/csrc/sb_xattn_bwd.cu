@@ -163,10 +163,10 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
   const int kvh = idx % a.Hkv, b = idx / a.Hkv;
   const int count = a.mask.count(b);
   const int q_tiles = (a.Tq + kStep - 1) / kStep;  // SIDE 1: steps a head
-  const int each = (a.steps + a.splits - 1) / a.splits, first = split * each;
-  // steps with anything to do: key tiles that begin before the item's end; all, if the held keys do
-  const int all = SIDE == 0 ? min(a.steps, (count + kStep - 1) / kStep) : tile * 128 < count ? a.steps : 0;
-  const int n = max(0, min(first + each, all) - first);
+  // steps with anything to do, split evenly: key tiles that begin before the item's end; all, if the held
+  // keys do
+  const int all = SIDE == 0 ? (count + kStep - 1) / kStep : tile * 128 < count ? a.steps : 0;
+  const int each = (all + a.splits - 1) / a.splits, first = min(split * each, all), n = min(first + each, all) - first;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
