@@ -300,11 +300,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kSoft + 3) {
     if (a.masked) {  // cleaner, its mask bytes two tiles ahead
+      const uint8_t* vrow = a.mask.row(b);
       uint32_t next[2][KT / 32];
+      if (vrow) {
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int x = 0; x < KT / 32; ++x) next[y][x] = a.mask.ask(b, (first + y) * KT + 32 * x, count);
+          for (int x = 0; x < KT / 32; ++x) next[y][x] = ask_keys(vrow, (first + y) * KT + 32 * x, count);
+      }
       Place vp(VS);
 #pragma unroll 2
       for (int i = 0; i < n; ++i, vp.next()) {
@@ -313,8 +316,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t w[KT / 32];
 #pragma unroll
         for (int x = 0; x < KT / 32; ++x) {
-          w[x] = a.mask.told(next[i & 1][x], j0 + 32 * x, count);
-          next[i & 1][x] = a.mask.ask(b, j0 + 2 * KT + 32 * x, count);
+          if (vrow) {
+            w[x] = told_keys(next[i & 1][x]);
+            next[i & 1][x] = ask_keys(vrow, j0 + 2 * KT + 32 * x, count);
+          } else {
+            w[x] = bits_below(j0 + 32 * x, count);
+          }
         }
         if (!warp_wait(&v_full[vp.st], vp.parity, abort_flag)) {
           if (lane == 0) give_up(SB_ERR_TIMEOUT_FULL);
@@ -348,12 +355,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t sl2 = pair2(sl, sl);
     const int jstep = two ? KT : 2 * KT;
     int j0 = (first + (two ? 0 : t)) * KT + hf * 64;
-    uint32_t b0 = a.mask.ask(b, j0, count), b1 = a.mask.ask(b, j0 + 32, count);
+    const uint8_t* vrow = a.mask.row(b);
+    uint32_t b0 = 0, b1 = 0;
+    if (vrow) {
+      b0 = ask_keys(vrow, j0, count);
+      b1 = ask_keys(vrow, j0 + 32, count);
+    }
     // A warp whose wait failed goes on to the next barrier with its partner, which then leaves too.
     for (int i = 0; i < mine; ++i, j0 += jstep) {
-      const uint32_t w0 = a.mask.told(b0, j0, count), w1 = a.mask.told(b1, j0 + 32, count);
-      b0 = a.mask.ask(b, j0 + jstep, count);
-      b1 = a.mask.ask(b, j0 + jstep + 32, count);
+      uint32_t w0 = 0xFFFFFFFFu, w1 = 0xFFFFFFFFu;
+      if (vrow) {
+        w0 = told_keys(b0);
+        w1 = told_keys(b1);
+        b0 = ask_keys(vrow, j0 + jstep, count);
+        b1 = ask_keys(vrow, j0 + jstep + 32, count);
+      } else if (j0 + 64 > count) {
+        w0 = bits_below(j0, count);
+        w1 = bits_below(j0 + 32, count);
+      }
       ok = ok && warp_wait(&s_full[t], i & 1, abort_flag);
       if (!some) {  // P of lanes without rows is never looked at
         if (!ok) break;

@@ -21,21 +21,22 @@ struct KeyMask {
   long long valid_img;
   int Tk;
   SB_DEV int count(int b) const { return lens ? min(max(lens[b], 0), Tk) : Tk; }
-  // word() in two steps, so that a tile's bytes are on their way while another tile is worked on
-  SB_DEV uint32_t ask(int b, int j0, int n) const {
-    const int j = j0 + (int)lane_id();
-    return valid && j < n ? valid[b * valid_img + j] : 1u;
-  }
-  SB_DEV uint32_t told(uint32_t byte, int j0, int n) const {
-    const int left = n - j0;
-    const uint32_t w = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
-    return valid ? w & __ballot_sync(0xFFFFFFFFu, byte != 0) : w;
-  }
-  // bit i of the result: key j0 + i takes part (whole warp; n = count(b))
-  SB_DEV uint32_t word(int b, int j0, int n) const {
-    return told(ask(b, j0, n), j0, n);
-  }
+  // the item's row of valid, kept in registers by what uses it in a loop
+  SB_DEV const uint8_t* row(int b) const { return valid ? valid + b * valid_img : nullptr; }
 };
+
+// Keys j0 .. j0 + 31 below n, as bits.
+SB_DEV uint32_t bits_below(int j0, int n) {
+  const int left = n - j0;
+  return left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
+}
+// A lane's byte of keys j0 .. j0 + 31 of row (KeyMask::row, not null) and, a tile later, the warp's
+// bits: the bytes are on their way while another tile is worked on.
+SB_DEV uint32_t ask_keys(const uint8_t* row, int j0, int n) {
+  const int j = j0 + (int)lane_id();
+  return j < n ? row[j] : 0u;
+}
+SB_DEV uint32_t told_keys(uint32_t byte) { return __ballot_sync(0xFFFFFFFFu, byte != 0); }
 
 // Arguments of the forward kernels.
 struct FwdArgs {

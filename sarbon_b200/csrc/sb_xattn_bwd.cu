@@ -286,19 +286,26 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
     }
   } else if (warp == kSoft + 3) {
     if (SIDE == 0 && a.masked) {  // cleaner: k's rows of keys that take no part, mask bytes two tiles ahead
+      const uint8_t* vrow = a.mask.row(b);
       uint32_t next[2][kStep / 32];
+      if (vrow) {
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int x = 0; x < kStep / 32; ++x) next[y][x] = a.mask.ask(b, (first + y) * kStep + 32 * x, count);
+          for (int x = 0; x < kStep / 32; ++x) next[y][x] = ask_keys(vrow, (first + y) * kStep + 32 * x, count);
+      }
 #pragma unroll 2
       for (int i = 0; i < n; ++i) {
         const int st = i % ST, j0 = (first + i) * kStep;
         uint32_t w[kStep / 32];
 #pragma unroll
         for (int x = 0; x < kStep / 32; ++x) {
-          w[x] = a.mask.told(next[i & 1][x], j0 + 32 * x, count);
-          next[i & 1][x] = a.mask.ask(b, j0 + 2 * kStep + 32 * x, count);
+          if (vrow) {
+            w[x] = told_keys(next[i & 1][x]);
+            next[i & 1][x] = ask_keys(vrow, j0 + 2 * kStep + 32 * x, count);
+          } else {
+            w[x] = bits_below(j0 + 32 * x, count);
+          }
         }
         if (!warp_wait(&full[st], (i / ST) & 1, abort_flag)) {
           if (lane == 0) give_up(SB_ERR_TIMEOUT_FULL);
@@ -378,15 +385,20 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
       next[1] = t < a.Tq ? a.delta[at] * f : 0.f;
     };
     if (SIDE == 1 && n > 0) fetch(0);
-    uint32_t byte = SIDE == 0 ? a.mask.ask(b, first * kStep + cg * 32, count) : 0u;
+    const uint8_t* vrow = SIDE == 0 ? a.mask.row(b) : nullptr;
+    uint32_t byte = vrow ? ask_keys(vrow, first * kStep + cg * 32, count) : 0u;
     bool ok = true;
     for (int i = 0; i < n; ++i) {
       uint32_t w = takes ? 0xFFFFFFFFu : 0u;
       const float* st = mine + (i & 1) * 64;
       if constexpr (SIDE == 0) {
         const int j0 = (first + i) * kStep + cg * 32;
-        w = a.mask.told(byte, j0, count);
-        byte = a.mask.ask(b, j0 + kStep, count);
+        if (vrow) {
+          w = told_keys(byte);
+          byte = ask_keys(vrow, j0 + kStep, count);
+        } else {
+          w = bits_below(j0, count);
+        }
       } else {
         float* put = mine + (i & 1) * 64;
         put[lane] = next[0];

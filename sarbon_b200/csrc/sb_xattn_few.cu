@@ -128,13 +128,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   const int krow = lane & 7, kc = lane >> 3;
   const int vrow = ((lane >> 3) & 1) * 8 + (lane & 7), vc = lane >> 4;
+  const uint8_t* valid = a.mask.row(b);
   uint32_t next[WORDS];
   auto ask = [&](int i) {
 #pragma unroll
-    for (int x = 0; x < WORDS; ++x)
-      next[x] = a.mask.ask(b, (first + warp + i * kWarps) * CK + 32 * x, count);
+    for (int x = 0; x < WORDS; ++x) next[x] = ask_keys(valid, (first + warp + i * kWarps) * CK + 32 * x, count);
   };
-  ask(0);
+  if (valid) ask(0);
   bool ok = true;
   for (int i = 0; i < mine; ++i) {
     const int st = i % kStages, j0 = (first + warp + i * kWarps) * CK;
@@ -142,11 +142,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     bool all = true;
 #pragma unroll
     for (int x = 0; x < WORDS; ++x) {
-      w[x] = a.mask.told(next[x], j0 + 32 * x, count);
+      w[x] = valid ? told_keys(next[x]) : bits_below(j0 + 32 * x, count);
       if (CK < 32) w[x] |= 0xFFFFFFFFu << (CK & 31);  // keys of the next chunk
       all = all && w[x] == 0xFFFFFFFFu;
     }
-    ask(i + 1);
+    if (valid) ask(i + 1);
     ok = __all_sync(0xFFFFFFFFu, bounded_wait(&full[warp][st], (i / kStages) & 1));
     if (!ok) break;
     uint8_t* stage = ring + st * C::STAGE;
