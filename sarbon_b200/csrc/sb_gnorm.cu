@@ -64,7 +64,7 @@ struct NormArgs {
 // Sum of a pair of values over the threads of a row; the two halves of the buffer alternate, so one
 // barrier a reduction is enough.
 struct RowSum {
-  float2* buf;  // [2][32], with four sums at once [2][16] of them
+  float2* buf;  // [2][32]; as floats, [2][64]: K sums of up to 64 / K warps
   int warps, half;
   SB_DEV float2 operator()(float a, float b) {
 #pragma unroll
@@ -171,26 +171,26 @@ SB_DEV void from_smem(const uint8_t* row, int dt, int c, bool on, float (&v)[8])
     for (int u = 0; u < 8; ++u) v[u] = 0.f;
   }
 }
-// Sums of K = 1, 2 or 4 values over a team, in every thread.  A warp halves the values with its lanes
-// (each half of the lanes goes on with half of the values), so K values take 5 or 6 shuffles, not 5 K.
-template <int K>
+// Sums of K = 1, 2, 4 or 8 values over a team, in every thread.  A warp halves the values with its
+// lanes (each half of the lanes goes on with half of the values), so eight values take 9 shuffles, not 40.
+// WARPS: as many as a team can have, each with STRIDE floats in the buffer, zero where there is no such
+// warp (a loop of known length); 0: the team's own number.
+template <int K, int WARPS = 0, int STRIDE = K>
 SB_DEV void team_sum(float (&v)[K], RowSum& sum) {
-  static_assert(K == 1 || K == 2 || K == 4, "values");
+  static_assert(K == 1 || K == 2 || K == 4 || K == 8, "values");
+  static_assert(WARPS * STRIDE <= 64 && STRIDE >= K, "half of the buffer");
   const int lane = threadIdx.x & 31;
-  float x;
-  if constexpr (K == 4) {
-    const bool up = lane & 16, odd = lane & 8;
-    const float k0 = up ? v[2] : v[0], k1 = up ? v[3] : v[1], s0 = up ? v[0] : v[2], s1 = up ? v[1] : v[3];
-    const float a0 = k0 + __shfl_xor_sync(0xFFFFFFFFu, s0, 16), a1 = k1 + __shfl_xor_sync(0xFFFFFFFFu, s1, 16);
-    x = (odd ? a1 : a0) + __shfl_xor_sync(0xFFFFFFFFu, odd ? a0 : a1, 8);
-  } else if constexpr (K == 2) {
-    const bool up = lane & 16;
-    x = (up ? v[1] : v[0]) + __shfl_xor_sync(0xFFFFFFFFu, up ? v[0] : v[1], 16);
-  } else {
-    x = v[0] + __shfl_xor_sync(0xFFFFFFFFu, v[0], 16);
-  }
+  int o = 16;
 #pragma unroll
-  for (int o = K == 4 ? 4 : 8; o; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
+  for (int n = K / 2; n; n >>= 1, o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int k = 0; k < n; ++k)
+      v[k] = (up ? v[k + n] : v[k]) + __shfl_xor_sync(0xFFFFFFFFu, up ? v[k] : v[k + n], o);
+  }
+  float x = v[0];
+#pragma unroll
+  for (o = 16 / K; o; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
   constexpr int per = 32 / K;  // lanes that hold the same value: value k in lanes k * per ..
   if (sum.warps == 1) {
 #pragma unroll
@@ -199,20 +199,33 @@ SB_DEV void team_sum(float (&v)[K], RowSum& sum) {
   }
   float* mine = reinterpret_cast<float*>(sum.buf) + sum.half * 64;
   sum.half ^= 1;
-  if (lane % per == 0) mine[(threadIdx.x >> 5) * K + lane / per] = x;
+  if (lane % per == 0) mine[(threadIdx.x >> 5) * STRIDE + lane / per] = x;
   __syncthreads();
+  if constexpr (K == 1) {
+    v[0] = 0.f;
+    const int warps = WARPS ? WARPS : sum.warps;
+#pragma unroll WARPS ? WARPS : 1
+    for (int i = 0; i < warps; ++i) v[0] += mine[i * STRIDE];
+  } else {
+    uint64_t t[K / 2];
 #pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = 0.f;
-  for (int i = 0; i < sum.warps; ++i) {
-    if constexpr (K == 4) {
-      const float4 t = reinterpret_cast<const float4*>(mine)[i];
-      v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
-    } else if constexpr (K == 2) {
-      const float2 t = reinterpret_cast<const float2*>(mine)[i];
-      v[0] += t.x; v[1] += t.y;
-    } else {
-      v[0] += mine[i];
+    for (int k = 0; k < K / 2; ++k) t[k] = 0;
+    const int warps = WARPS ? WARPS : sum.warps;
+#pragma unroll WARPS ? WARPS : 1
+    for (int i = 0; i < warps; ++i) {
+      if constexpr (K == 2) {
+        t[0] = add2(t[0], *reinterpret_cast<const uint64_t*>(mine + i * STRIDE));
+      } else {
+#pragma unroll
+        for (int k = 0; k < K; k += 4) {
+          const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(mine + i * STRIDE + k);
+          t[k / 2] = add2(t[k / 2], w.x);
+          t[k / 2 + 1] = add2(t[k / 2 + 1], w.y);
+        }
+      }
     }
+#pragma unroll
+    for (int k = 0; k < K / 2; ++k) split2(t[k], v[2 * k], v[2 * k + 1]);
   }
 }
 
@@ -429,14 +442,50 @@ __global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant_
   }
 }
 
-// R rows of a team at once: their reductions share barriers and overlap.  A row in shared memory has
-// room for all of the team's columns, zero past D, and a row past the team's last is zeroed before its
-// step, so the loop has no selects: lanes past D hold zeros in x, z, dy, dh and in scale x gate, which
-// makes every term they add zero but the squares around the mean (left out by `in`).
+// Pairs of fp32 values, two operations an instruction
+SB_DEV float both(uint64_t v) {
+  float lo, hi;
+  split2(v, lo, hi);
+  return lo + hi;
+}
+SB_DEV uint64_t twice(float v) { return pair2(v, v); }
+SB_DEV void pairs(const float (&v)[8], uint64_t (&p)[4]) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) p[u] = pair2(v[2 * u], v[2 * u + 1]);
+}
+template <int DT>
+SB_DEV void pairs_from(const uint8_t* row, int dt, int c, uint64_t (&p)[4]) {
+  float v[8];
+  from_smem<DT>(row, dt, c, v);
+  pairs(v, p);
+}
+SB_DEV void store_pairs(void* p, int dt, long long i, const uint64_t (&v)[4]) {
+  float f[8];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) split2(v[u], f[2 * u], f[2 * u + 1]);
+  store8(p, dt, i, f);
+}
+// The mean of four values: of equal ones exactly their value.
+SB_DEV float mean4(float a, float b, float c, float d) { return ((a + b) + (c + d)) * 0.25f; }
+
+// R rows of a team at once, in three reductions that their rows share:
+//   1. z - c and its square,  2. y - c', its square, e and e (y - c') with e = dh w_pre,
+//   3. e and e zhat with e = dn w_post  (RMS norm: the squares and the products alone).
+// Layer norm's c and c' are the mean of the row's first four values.  Such a mean is at most
+// sqrt(D) / 2 deviations away from the row's, so var = E (v - c)^2 - (E v - c)^2 loses at most a
+// factor D / 4 of fp32's precision where one value is all of the variance, and nothing in rows of
+// values alike, however large their mean: no pass for the mean comes first.  (With the means first,
+// it was six reductions a step, whose latency bounded the kernel: 387 us for 65,280 rows of 1024.)
+// With A = scale gate w_post and B = scale gate b_post (of a row's own gate: without it),
+// y = x + zhat A + B and dn w_post = dyt A.
+// A row in shared memory has room for all of the team's columns, zero past D, and a row past the
+// team's last is zeroed before its step, so the loop has no selects: lanes past D hold zeros in
+// x, z, dy, dh, A and B and subtract nothing from them, which makes every term they add zero.
 template <int XD, int ZD, bool LAYER, int R, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) gated_norm_back_kernel(const __grid_constant__ NormArgs a) {
   __shared__ __align__(16) float2 buf[64];
   __shared__ uint64_t bars[8 * kMaxStages];
+  __shared__ __align__(16) float first[2][4];  // A and B of the first four columns
   extern __shared__ __align__(16) uint8_t rows_smem[];
   const int xdt = XD < 0 ? a.xdt : XD, zdt = ZD < 0 ? a.zdt : ZD;
   const int warps = a.tpr >> 5;
@@ -452,6 +501,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) gated_norm_back_ker
     on[j] = c[j] < a.D;
     cw[j] = on[j] ? c[j] : 0;
   }
+  constexpr int kWarps = MAXT / 32, kStride = (LAYER ? 4 : 2) * R;
+  for (int i = threadIdx.x; i < 64; i += blockDim.x) buf[i] = make_float2(0.f, 0.f);
   if (me == 0)
     for (int i = 0; i < a.stages; ++i) mbar_init(&ring.full[i], 1);
   fence_mbar_init();
@@ -474,8 +525,9 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) gated_norm_back_ker
   // places in a row of a stage: z, gate, x, dy, dh
   const int zb = a.pitch * (zdt == SB_F32 ? 4 : 2), xb = a.pitch * (xdt == SB_F32 ? 4 : 2);
   const int xo = a.gate_is_row ? 2 * zb : zb, dyo = a.dh.p ? xo + xb : xo, dho = a.dy.p ? dyo + xb : dyo;
-  // scale x gate of the CTA's rows (scale alone where every row has its gate)
-  float sg[NV][8], acc[kSums][NV][8];
+  // A, B and w_pre in registers where a thread has one vector, else from the cache each time
+  float sg[NV][8];  // scale x gate of the CTA's rows (scale alone where every row has its gate)
+  uint64_t acc[kSums][NV][4], keep[3][4];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     weights8(a.scale, c[j], on[j], on[j] ? 1.f : 0.f, sg[j]);
@@ -488,10 +540,48 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) gated_norm_back_ker
 #pragma unroll
     for (int k = 0; k < kSums; ++k)
 #pragma unroll
-      for (int u = 0; u < 8; ++u) acc[k][j][u] = 0.f;
+      for (int u = 0; u < 4; ++u) acc[k][j][u] = 0;
   }
-  long long out = begin * a.D;
-  for (int i = 0; i < n; ++i, out += R * a.D, here.next(ring)) {
+  enum { kA, kB, kW };
+  auto column = [&](int which, int j, uint64_t(&v)[4]) {
+    float w[8];
+    weights8(which == kA ? a.post_w : which == kB ? a.post_b : a.pre_w, cw[j], true, which == kB ? 0.f : 1.f, w);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (which != kW) w[u] *= sg[j][u];
+    pairs(w, v);
+  };
+  auto take = [&](int which, int j, uint64_t(&v)[4]) {
+    if constexpr (NV == 1) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = keep[which][u];
+    } else {
+      column(which, j, v);
+    }
+  };
+  if constexpr (NV == 1) {
+    column(kA, 0, keep[kA]);
+    if (LAYER) column(kB, 0, keep[kB]);
+    column(kW, 0, keep[kW]);
+  }
+  if (LAYER) {
+    if (threadIdx.x == 0) {
+      uint64_t v[4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        take(k, 0, v);
+        split2(v[0], first[k][0], first[k][1]);
+        split2(v[1], first[k][2], first[k][3]);
+      }
+    }
+    __syncthreads();
+  }
+  // where the thread's columns of the step's first row go
+  const int xe = xdt == SB_F32 ? 4 : 2, ze = zdt == SB_F32 ? 4 : 2;
+  uint8_t* dx = static_cast<uint8_t*>(a.dx) + (begin * a.D + c[0]) * xe;
+  uint8_t* dz = static_cast<uint8_t*>(a.dz) + (begin * a.D + c[0]) * ze;
+  const intptr_t to_gates = reinterpret_cast<intptr_t>(a.dgate_rows) - reinterpret_cast<intptr_t>(a.dz);
+  for (int i = 0; i < n; ++i, dx += R * a.D * xe, dz += R * a.D * ze, here.next(ring)) {
     if (!team_all(bounded_wait(&ring.full[here.st], here.parity), warps)) {
       give_up(ring, here, filled - i, me);
       break;
@@ -502,160 +592,224 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) gated_norm_back_ker
       ++filled;
       there.next(ring);
     }
-    uint8_t* row = ring.base + here.st * a.stage_bytes;
+    uint8_t* stage = ring.base + here.st * a.stage_bytes;
     const bool odd = R > 1 && (i + 1) * R > rows;  // the last row of this step does not exist
     if (odd) {
       for (int o = 0; o < a.row_bytes; o += 16 * a.tpr)
-        if (o + 16 * me < a.row_bytes) *reinterpret_cast<uint4*>(row + a.row_bytes + o + 16 * me) = make_uint4(0, 0, 0, 0);
+        if (o + 16 * me < a.row_bytes) *reinterpret_cast<uint4*>(stage + a.row_bytes + o + 16 * me) = make_uint4(0, 0, 0, 0);
       team_all(true, warps);
     }
-    float zh[R][NV][8], d[R][NV][8], zr[R], shift[R];
+    uint64_t zh[R][NV][4];
+    float zr[R], zs[R], zc[R];  // zhat = (z - zc) zr + zs
 #pragma unroll
     for (int x = 0; x < R; ++x) {
       zr[x] = 1.f;
+      zs[x] = zc[x] = 0.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        from_smem<ZD>(row + x * a.row_bytes, zdt, c[j], zh[x][j]);
-        if (a.dy.p) {
-          from_smem<XD>(row + x * a.row_bytes + dyo, xdt, c[j], d[x][j]);
-        } else {
-#pragma unroll
-          for (int u = 0; u < 8; ++u) d[x][j][u] = 0.f;
-        }
-      }
+      for (int j = 0; j < NV; ++j) pairs_from<ZD>(stage + x * a.row_bytes, zdt, c[j], zh[x][j]);
     }
     if (a.post_w) {
-      stats8<LAYER>(zh, on, inv_d, a.eps, sum, zr, shift);
-      if (odd) zr[R - 1] = shift[R - 1] = 0.f;
+      float s[LAYER ? 2 * R : R];  // squares, then (layer norm) values
 #pragma unroll
-      for (int x = 0; x < R; ++x)
+      for (int x = 0; x < R; ++x) {
+        if (LAYER) {
+          float f[8];
+          from_smem<ZD>(stage + x * a.row_bytes, zdt, 0, f);
+          zc[x] = mean4(f[0], f[1], f[2], f[3]);
+        }
+        uint64_t q = 0, t = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const uint64_t off = twice(on[j] ? -zc[x] : 0.f);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint64_t& v = zh[x][j][u];
+            if (LAYER) {
+              v = add2(v, off);
+              t = add2(t, v);
+            }
+            q = fma2(v, v, q);
+          }
+        }
+        s[x] = both(q);
+        if (LAYER) s[R + x] = both(t);
+      }
+      team_sum<sizeof(s) / 4, kWarps, kStride>(s, sum);
+#pragma unroll
+      for (int x = 0; x < R; ++x) {
+        float var = s[x] * inv_d;
+        if (LAYER) {
+          const float m = s[R + x] * inv_d;
+          var = fmaf(-m, m, var);
+          if (var < 0.f) var = 0.f;  // (NaN stays)
+          zr[x] = rsqrtf(var + a.eps);
+          zs[x] = -m * zr[x];
+        } else {
+          zr[x] = rsqrtf(var + a.eps);
+        }
+        if (odd && x == R - 1) zr[x] = zs[x] = 0.f;
+        const uint64_t r2 = twice(zr[x]), s2 = twice(zs[x]);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int u = 0; u < 8; ++u) zh[x][j][u] = LAYER ? fmaf(zh[x][j][u], zr[x], shift[x]) : zh[x][j][u] * zr[x];
+          for (int u = 0; u < 4; ++u) zh[x][j][u] = LAYER ? fma2(zh[x][j][u], r2, s2) : mul2(zh[x][j][u], r2);
+      }
     }
+    uint64_t d[R][NV][4];
+    float rs[R], m1[R], m0[R];
     if (a.dh.p) {
-      float y[R][NV][8], dh[R][NV][8], rs[R];
+      constexpr int K = LAYER ? 4 : 2;  // squares, products of e, (layer norm) values, e
+      float s[K * R];
+      uint64_t dh[R][NV][4];
+#pragma unroll
+      for (int x = 0; x < R; ++x) {
+        const uint8_t* row = stage + x * a.row_bytes;
+        float cy = 0.f;
+        if (LAYER) {
+          float z8[8], x8[8], g8[8], y4[4];
+          from_smem<ZD>(row, zdt, 0, z8);
+          from_smem<XD>(row + xo, xdt, 0, x8);
+          if (a.gate_is_row) from_smem<ZD>(row + zb, zdt, 0, g8);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float t = fmaf(fmaf(z8[u] - zc[x], zr[x], zs[x]), first[0][u], first[1][u]);
+            y4[u] = a.gate_is_row ? fmaf(g8[u], t, x8[u]) : x8[u] + t;
+          }
+          cy = mean4(y4[0], y4[1], y4[2], y4[3]);
+        }
+        uint64_t q = 0, p = 0, t = 0, te = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const uint64_t off = twice(on[j] ? -cy : 0.f);
+          uint64_t A[4], B[4], W[4], g[4];
+          take(kA, j, A);
+          if (LAYER) take(kB, j, B);
+          take(kW, j, W);
+          if (a.gate_is_row) pairs_from<ZD>(row + zb, zdt, c[j], g);
+          pairs_from<XD>(row + xo, xdt, c[j], d[x][j]);  // x, then y - c', then yhat
+          pairs_from<ZD>(row + dho, zdt, c[j], dh[x][j]);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint64_t& y = d[x][j][u];
+            if (a.gate_is_row) y = fma2(g[u], LAYER ? fma2(zh[x][j][u], A[u], B[u]) : mul2(zh[x][j][u], A[u]), y);
+            else if (LAYER) y = add2(fma2(zh[x][j][u], A[u], B[u]), y);
+            else y = fma2(zh[x][j][u], A[u], y);
+            const uint64_t e = mul2(dh[x][j][u], W[u]);
+            if (LAYER) {
+              y = add2(y, off);
+              t = add2(t, y);
+              te = add2(te, e);
+            }
+            q = fma2(y, y, q);
+            p = fma2(e, y, p);
+          }
+        }
+        s[x] = both(q);
+        s[R + x] = both(p);
+        if (LAYER) {
+          s[2 * R + x] = both(t);
+          s[3 * R + x] = both(te);
+        }
+      }
+      team_sum<sizeof(s) / 4, kWarps, kStride>(s, sum);
+#pragma unroll
+      for (int x = 0; x < R; ++x) {
+        float var = s[x] * inv_d, shift = 0.f, p = s[R + x];  // p: sum of e yhat
+        if (LAYER) {
+          const float m = s[2 * R + x] * inv_d;
+          var = fmaf(-m, m, var);
+          if (var < 0.f) var = 0.f;
+          rs[x] = rsqrtf(var + a.eps);
+          shift = -m * rs[x];
+          p = rs[x] * fmaf(-m, s[3 * R + x], p);
+          m0[x] = -s[3 * R + x] * inv_d * rs[x];
+        } else {
+          rs[x] = rsqrtf(var + a.eps);
+          p *= rs[x];
+        }
+        m1[x] = -p * inv_d;
+        if (odd && x == R - 1) rs[x] = shift = m1[x] = m0[x] = 0.f;
+        const uint64_t r2 = twice(rs[x]), s2 = twice(shift);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          uint64_t W[4], dy[4];
+          take(kW, j, W);
+          if (a.dy.p) pairs_from<XD>(stage + x * a.row_bytes + dyo, xdt, c[j], dy);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint64_t& v = d[x][j][u];
+            const uint64_t dd = dh[x][j][u], y = LAYER ? fma2(v, r2, s2) : mul2(v, r2);
+            acc[2][j][u] = fma2(dd, y, acc[2][j][u]);
+            if (LAYER) acc[3][j][u] = add2(acc[3][j][u], dd);
+            v = fma2(y, twice(m1[x]), mul2(dd, W[u]));
+            if (LAYER) v = fma2(v, r2, twice(m0[x]));
+            else v = mul2(v, r2);
+            if (a.dy.p) v = add2(v, dy[u]);
+          }
+        }
+      }
+    } else {
 #pragma unroll
       for (int x = 0; x < R; ++x)
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          float n8[8];  // Npost(z)
-          if (a.post_w) {
-            float w[8];
-            weights8(a.post_w, cw[j], true, 1.f, w);
-#pragma unroll
-            for (int u = 0; u < 8; ++u) n8[u] = zh[x][j][u] * w[u];
-            if (LAYER && a.post_b) {
-              weights8(a.post_b, cw[j], true, 0.f, w);
-#pragma unroll
-              for (int u = 0; u < 8; ++u) n8[u] += w[u];
-            }
+          if (a.dy.p) {
+            pairs_from<XD>(stage + x * a.row_bytes + dyo, xdt, c[j], d[x][j]);
           } else {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) n8[u] = zh[x][j][u];
+            for (int u = 0; u < 4; ++u) d[x][j][u] = 0;
           }
-          if (a.gate_is_row) {
-            float g[8];
-            from_smem<ZD>(row + x * a.row_bytes + zb, zdt, c[j], g);
-#pragma unroll
-            for (int u = 0; u < 8; ++u) n8[u] *= g[u];
-          }
-          from_smem<XD>(row + x * a.row_bytes + xo, xdt, c[j], y[x][j]);
-#pragma unroll
-          for (int u = 0; u < 8; ++u) y[x][j][u] = fmaf(sg[j][u], n8[u], y[x][j][u]);
         }
-      stats8<LAYER>(y, on, inv_d, a.eps, sum, rs, shift);
-      if (odd) rs[R - 1] = shift[R - 1] = 0.f;
-      float e[LAYER ? 2 * R : R];  // sums of e yhat, then (layer norm) of e
+    }
+    float s[LAYER ? 2 * R : R];  // sums of e zhat, then (layer norm) of e
 #pragma unroll
-      for (int x = 0; x < (LAYER ? 2 * R : R); ++x) e[x] = 0.f;
+    for (int x = 0; x < R; ++x) {
+      const bool there_is = !(x == R - 1 && odd);
+      uint64_t p = 0, te = 0;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        float w[8];
-        weights8(a.pre_w, cw[j], true, 1.f, w);
-#pragma unroll
-        for (int x = 0; x < R; ++x) {
-          from_smem<ZD>(row + x * a.row_bytes + dho, zdt, c[j], dh[x][j]);
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            float& yy = y[x][j][u];
-            float& dd = dh[x][j][u];
-            yy = LAYER ? fmaf(yy, rs[x], shift[x]) : yy * rs[x];
-            acc[2][j][u] = fmaf(dd, yy, acc[2][j][u]);
-            if (LAYER) acc[3][j][u] += dd;
-            dd *= w[u];
-            e[x] = fmaf(dd, yy, e[x]);
-            if (LAYER) e[R + x] += dd;
-          }
-        }
-      }
-      team_sum(e, sum);
-#pragma unroll
-      for (int x = 0; x < R; ++x) {
-        const float m1 = -e[x] * inv_d, m0 = LAYER ? -e[R + x] * inv_d * rs[x] : 0.f;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            d[x][j][u] = fmaf(rs[x], fmaf(y[x][j][u], m1, dh[x][j][u]), d[x][j][u]);
-            if (LAYER) d[x][j][u] += m0;
-          }
-      }
-    }
-    float e[LAYER ? 2 * R : R];
-#pragma unroll
-    for (int x = 0; x < (LAYER ? 2 * R : R); ++x) e[x] = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float w[8];  // scale x gate x post_w
-      if (a.post_w) {
-        weights8(a.post_w, cw[j], true, 1.f, w);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) w[u] *= sg[j][u];
-      } else {
-#pragma unroll
-        for (int u = 0; u < 8; ++u) w[u] = sg[j][u];
-      }
-#pragma unroll
-      for (int x = 0; x < R; ++x) {
-        const bool there_is = on[j] && !(x == R - 1 && odd);
-        if (there_is) store8(a.dx, xdt, out + x * a.D + c[j], d[x][j]);
+        uint64_t A[4];
+        take(kA, j, A);
+        if (there_is && on[j]) store_pairs(dx, xdt, x * a.D + j * a.tpr * 8, d[x][j]);
         if (a.gate_is_row) {
-          float g[8];
-          from_smem<ZD>(row + x * a.row_bytes + zb, zdt, c[j], g);
-          if (a.dgate_rows && there_is) {
-            float o[8], dg[8];
-            weights8(LAYER ? a.post_b : nullptr, c[j], true, 0.f, o);
+          uint64_t g[4];
+          pairs_from<ZD>(stage + x * a.row_bytes + zb, zdt, c[j], g);
+          if (a.dgate_rows && there_is && on[j]) {
+            uint64_t B[4], dg[4];
+            if (LAYER) take(kB, j, B);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) dg[u] = d[x][j][u] * fmaf(zh[x][j][u], w[u], sg[j][u] * o[u]);
-            store8(a.dgate_rows, zdt, out + x * a.D + c[j], dg);
+            for (int u = 0; u < 4; ++u)
+              dg[u] = mul2(d[x][j][u], LAYER ? fma2(zh[x][j][u], A[u], B[u]) : mul2(zh[x][j][u], A[u]));
+            store_pairs(dz + to_gates, zdt, x * a.D + j * a.tpr * 8, dg);
           }
 #pragma unroll
-          for (int u = 0; u < 8; ++u) d[x][j][u] *= g[u];
+          for (int u = 0; u < 4; ++u) d[x][j][u] = mul2(d[x][j][u], g[u]);
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          float& dd = d[x][j][u];
-          acc[0][j][u] = fmaf(dd, zh[x][j][u], acc[0][j][u]);
-          if (LAYER) acc[1][j][u] += dd;
-          dd *= w[u];
-          e[x] = fmaf(dd, zh[x][j][u], e[x]);
-          if (LAYER) e[R + x] += dd;
+        for (int u = 0; u < 4; ++u) {
+          uint64_t& dd = d[x][j][u];
+          acc[0][j][u] = fma2(dd, zh[x][j][u], acc[0][j][u]);
+          if (LAYER) acc[1][j][u] = add2(acc[1][j][u], dd);
+          dd = mul2(dd, A[u]);
+          p = fma2(dd, zh[x][j][u], p);
+          if (LAYER) te = add2(te, dd);
         }
       }
+      s[x] = both(p);
+      if (LAYER) s[R + x] = both(te);
     }
     if (a.post_w) {
-      team_sum(e, sum);
+      team_sum<sizeof(s) / 4, kWarps, kStride>(s, sum);
 #pragma unroll
       for (int x = 0; x < R; ++x) {
-        const float m1 = -e[x] * inv_d * zr[x], m0 = LAYER ? -e[R + x] * inv_d * zr[x] : 0.f;
+        const uint64_t n1 = twice(-s[x] * inv_d * zr[x]), n0 = twice(LAYER ? -s[R + x] * inv_d * zr[x] : 0.f);
+        const uint64_t r2 = twice(zr[x]);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const float t = LAYER ? fmaf(zh[x][j][u], m1, m0) : zh[x][j][u] * m1;
-            d[x][j][u] = fmaf(d[x][j][u], zr[x], t);
+          for (int u = 0; u < 4; ++u) {
+            const uint64_t t = LAYER ? fma2(zh[x][j][u], n1, n0) : mul2(zh[x][j][u], n1);
+            d[x][j][u] = fma2(d[x][j][u], r2, t);
           }
       }
     }
@@ -663,7 +817,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) gated_norm_back_ker
     for (int x = 0; x < R; ++x)
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (on[j] && !(x == R - 1 && odd)) store8(a.dz, zdt, out + x * a.D + c[j], d[x][j]);
+        if (on[j] && !(x == R - 1 && odd)) store_pairs(dz, zdt, x * a.D + j * a.tpr * 8, d[x][j]);
   }
   if (!a.part) return;
   float* mine = a.part + (long long)blockIdx.x * kSums * a.D;
@@ -672,7 +826,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) gated_norm_back_ker
     for (int k = 0; k < kSums; ++k)
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (on[j]) store8(mine, SB_F32, (long long)k * a.D + c[j], acc[k][j]);
+        if (on[j]) store_pairs(mine, SB_F32, (long long)k * a.D + c[j], acc[k][j]);
     return;
   }
   // the CTA's warps one after the other, over the rings (every copy has been waited for)
@@ -684,7 +838,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) gated_norm_back_ker
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int u = 0; u < 8; ++u) fold[(sub * kSums + k) * width + c[j] + u] = acc[k][j][u];
+      for (int u = 0; u < 4; ++u)
+        reinterpret_cast<uint64_t*>(fold)[((sub * kSums + k) * width + c[j]) / 2 + u] = acc[k][j][u];
   __syncthreads();
   for (int i = threadIdx.x; i < kSums * a.D; i += blockDim.x) {
     const int k = i / a.D, col = i - k * a.D;
