@@ -620,7 +620,7 @@ __global__ void attend_none_kernel(OutView o, float* lse, int H, int Tq, int dh,
 }
 
 struct FwdPlan {
-  int pairs, splits, key_tiles;
+  int pairs, splits;
   long long units;
   bool few;
 };
@@ -635,20 +635,20 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int Tq, int Tk, int sms) {
   const long long tiles = ((long long)(H / Hkv) * Tq + 127) / 128;
   p.few = (long long)(H / Hkv) * Tq <= kFewRows;
   if (p.few) {
-    p.pairs = p.key_tiles = 1;
+    p.pairs = 1;
     p.units = (long long)B * Hkv;
     p.splits = few_splits(p.units, Tk, sms);
     return p;
   }
   p.pairs = (int)((tiles + 1) / 2);
-  p.key_tiles = (Tk + KT - 1) / KT;
+  const int key_tiles = (Tk + KT - 1) / KT;
   p.units = (long long)B * Hkv * p.pairs;
   const double twos = (double)B * Hkv * (tiles / 2), ones = (double)B * Hkv * (tiles % 2);
   p.splits = 1;
   double best = 1e300;
-  for (int s = 1; s <= std::min(kMost, p.key_tiles); ++s) {
-    const int each = (p.key_tiles + s - 1) / s;
-    if ((p.key_tiles + each - 1) / each != s) continue;  // some split would be empty
+  for (int s = 1; s <= std::min(kMost, key_tiles); ++s) {
+    const int each = (key_tiles + s - 1) / s;
+    if ((key_tiles + each - 1) / each != s) continue;  // some split would be empty
     const double t2 = each + kStart, t1 = 0.5 * each + kStart, longest = tiles > 1 ? t2 : t1;
     // SMs take CTAs as they come: the even share, and about half of a CTA's time until the last ends
     const double share = s * (twos * t2 + ones * t1) / sms;
@@ -809,7 +809,7 @@ extern "C" int sb_cross_attention(const void* q, long long q_row, long long q_im
   a.lse = lse;
   a.mask = {lens, static_cast<const uint8_t*>(valid), valid_img, Tk};
   a.B = B; a.H = H; a.Hkv = Hkv; a.group = H / Hkv; a.Tq = Tq; a.rows = a.group * Tq;
-  a.pairs = p.pairs; a.splits = p.splits; a.key_tiles = p.key_tiles;
+  a.pairs = p.pairs; a.splits = p.splits;
   a.k_item = k_img != 0; a.v_item = v_img != 0;
   a.masked = lens || valid;
   a.scale_log2 = scale * 1.4426950408889634f;

@@ -45,7 +45,7 @@ struct FwdArgs {
   float* lse;
   KeyMask mask;
   int B, H, Hkv, group, Tq, rows;  // rows = group * Tq of an (item, key head)
-  int pairs, splits, key_tiles;    // CTAs a (item, key head) and split; key tiles in all
+  int pairs, splits;               // CTAs a (item, key head) and split
   int k_item, v_item;              // 0: one memory for every item
   int masked;                      // lens or valid given: the cleaner runs
   float scale_log2;
@@ -207,8 +207,9 @@ SB_DEV uint32_t pack16(float lo, float hi) {
 }
 
 // ---------------------------------------------------------------- host
-// One [B][T][heads * dh] operand as a 4-D tensor map; its box is `rows` rows of one head of one item, and rows past T arrive as zeros.  img = 0 (one memory for
-// every item) makes the item dimension 1: kernels multiply the item by 0 then.
+// One [B][T][heads * dh] operand as a 4-D tensor map; its box is `rows` rows of one head of one item, and
+// rows past T arrive as zeros.  img = 0 (one memory for every item) makes the item dimension 1: kernels
+// multiply the item by 0 then.
 bool xattn_tensor_map(CUtensorMap* map, const View& v, int dtype, int B, int T, int heads, int dh, int rows);
 bool xattn_sizes_ok(int dtype, int B, int H, int Hkv, int dh, int Tq, int Tk);
 // 16-byte rows whose strides fit a tensor map

@@ -107,6 +107,16 @@ def _rows(t, what, shape, dtype, out=False):
     return t.data_ptr(), row, img
 
 
+def _apart(results, operands):
+    """Results that do not begin where an operand or another result does."""
+    seen = {t.data_ptr() for t in operands if t.numel()}
+    for t in results:
+        if t is not None and t.numel():
+            if t.data_ptr() in seen:
+                raise ValueError("results need their own memory")
+            seen.add(t.data_ptr())
+
+
 def _new(like, shape, dtype):
     """A contiguous tensor, (pointer, row stride, item stride); empty_like is the cheapest allocation."""
     t = torch.empty_like(like) if like.dtype == dtype and like.is_contiguous() and like.shape == shape else \
@@ -177,6 +187,7 @@ def cross_attention(q, k, v, heads, kv_heads=None, lens=None, valid=None, scale=
         _statistics(lse, b, heads, tq)
     if out is not None:
         op = _rows(out, "out", qs, dtype, out=True)
+        _apart((out,), (q, k, v))
     index = _ready(q, k, v, lens, valid, out, lse)
     if out is None:
         out, op = _new(q, qs, dtype)
@@ -194,7 +205,8 @@ def cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=None, lens
 
     The same sizes, masks and scale as forward.  dk and dv have one row for every item's state, also
     where k and v are shared by the items (sum them over the batch then); states that take no part
-    get zeros.  The sums have a fixed order: the same inputs give the same bits."""
+    get zeros.  The sums have a fixed order: the same inputs give the same bits.  dq, dk and
+    dv (allocated if None) must not share memory with an operand or each other."""
     kv_heads, b, tq, tk, dim, scale = _attention_sizes(q, k, heads, kv_heads, scale)
     dtype, qs, ks = q.dtype, (b, tq, heads * dim), (b, tk, kv_heads * dim)
     views = _rows(dout, "dout", qs, dtype) + _rows(q, "q", qs, dtype) + _rows(k, "k", ks, dtype) + \
@@ -204,6 +216,8 @@ def cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=None, lens
     for what, t, shape in (("dq", dq, qs), ("dk", dk, ks), ("dv", dv, ks)):
         if t is not None:
             _rows(t, what, shape, dtype, out=True)
+    if dq is not None or dk is not None or dv is not None:
+        _apart((dq, dk, dv), (dout, q, k, v, out))
     index = _ready(dout, q, k, v, out, lse, lens, valid, dq, dk, dv)
     dq, dqp = _new(q, qs, dtype) if dq is None else (dq, _rows(dq, "dq", qs, dtype))
     dk, dkp = _new(k, ks, dtype) if dk is None else (dk, _rows(dk, "dk", ks, dtype))

@@ -222,7 +222,7 @@ def test_cross_attention_empty_sizes():
     assert dq.shape == (2, 0, 64) and not dk.any() and not dv.any()
 
 
-def check_backward(grads, dout, q, k, v, heads, kv_heads, lens, valid, out16, scale=None):
+def check_backward(grads, dout, q, k, v, heads, kv_heads, lens, valid, out16, scale=None, sub_ds=None, sub_p=None):
     ref, lse, p, qd, kd, vd = formula(q, k, v, heads, kv_heads, lens, valid, scale)
     scale = scale or qd.shape[-1] ** -0.5
     g, o = heads_of(dout, heads, kv_heads), heads_of(out16, heads, kv_heads)
@@ -232,8 +232,9 @@ def check_backward(grads, dout, q, k, v, heads, kv_heads, lens, valid, out16, sc
     # dS is off by its rounding, by D from the rounded out, by P and by the fp32 products
     absd = (g.abs() * ref.abs()).sum(-1, keepdim=True)
     sub = 2.0 ** -25 if q.dtype == torch.float16 else 0.0  # fp16 values below 2^-14
-    ds_tol = u * ds.abs() + p * ((g * (o - ref)).abs().sum(-1, keepdim=True) + e * (g.abs() @ vd.abs().transpose(-1, -2) + absd)) + sub
-    p_tol = (u + e) * p + sub
+    ds_tol = u * ds.abs() + p * ((g * (o - ref)).abs().sum(-1, keepdim=True) + e * (g.abs() @ vd.abs().transpose(-1, -2) + absd)) + \
+        (sub if sub_ds is None else sub_ds)
+    p_tol = (u + e) * p + (sub if sub_p is None else sub_p)
     want = {"dq": (ds @ kd * scale, ds_tol @ kd.abs() * scale),
             "dk": ((ds.transpose(-1, -2) @ qd * scale).sum(2, keepdim=True),
                    (ds_tol.transpose(-1, -2) @ qd.abs() * scale).sum(2, keepdim=True)),
@@ -288,6 +289,26 @@ def test_cross_attention_backward_strides():
     assert grads[1] is dk and grads[2] is dv
     check_backward(grads, dout, q, k, v, heads, heads, None, None, out)
     assert (both[..., :8] == 3).all() and (both[..., -8:] == 3).all()
+
+
+@pytest.mark.parametrize("kv_heads", [1, 4])
+def test_cross_attention_backward_small_fp16(kv_heads):
+    """fp16 gradients of a long memory and a small loss: P and dS lie far below fp16's normal numbers,
+    and keep its precision all the same.  P is held times 2^14 and dS times a power of two that
+    keeps 2 max |dout_i| max |v_j| in 2^14 .. 2^15, so a subnormal step of 2^-24 there, half of
+    which a rounding may be off by, is this much smaller."""
+    import sarbon_b200 as sb
+    g = gen(21)
+    b, tq, tk, heads, dim = 1, 40, 1500, 4, 64
+    q = rand(g, b, tq, heads * dim, dtype=torch.float16)
+    k, v = (rand(g, b, tk, kv_heads * dim, dtype=torch.float16) for _ in range(2))
+    dout = rand(g, b, tq, heads * dim, by=2.0 ** -8).half()
+    ref, lse, *_ = formula(q, k, v, heads, kv_heads, None, None)
+    out, lse = rows_of(ref).half(), lse.flatten(1, 2).float().contiguous()
+    grads = sb.cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=kv_heads)
+    most = (heads_of(dout, heads, kv_heads).norm(dim=-1).max() * heads_of(v, kv_heads, kv_heads).norm(dim=-1).max()).item()
+    check_backward(grads, dout, q, k, v, heads, kv_heads, None, None, out, sub_ds=2.0 ** -25 * 2 * most / 2 ** 14,
+                   sub_p=2.0 ** -39)
 
 
 def test_cross_attention_gradient_against_differences():
@@ -478,6 +499,40 @@ def test_gated_norm_backward(case, missing):
         assert ((x - r).abs() <= tol).all(), (name, ((x - r).abs() / tol).max().item())
     again = sb.gated_norm_backward(dy, dh, **s)
     assert all(v is None or torch.equal(v, again[k]) for k, v in got.items())
+
+
+@pytest.mark.parametrize("t,d", [(70, 256), (33, 1024), (9, 4096)])
+@pytest.mark.parametrize("rows", ["offset", "outlier", "flat"])
+def test_gated_norm_backward_statistics(rows, t, d):
+    """Layer norms of rows whose mean is hundreds of deviations, whose variance is one value's (the first:
+    what the squares are taken around contains it), and whose z is one value throughout."""
+    import sarbon_b200 as sb
+    g = gen(d + len(rows))
+    s = norm_case(g, 2, t, d, torch.float32, torch.float32, "layer", None, True, True, True)
+    if rows == "offset":
+        s["x"], s["z"] = s["x"] + 512, s["z"] - 256
+        worse = 512.0  # roundings of values that large, measured in deviations
+    elif rows == "outlier":
+        s["x"][..., 0] += 4096
+        s["z"][..., 0] -= 4096
+        worse = d / 4.0  # E (v - c)^2 against its part (E v - c)^2
+    else:
+        s["z"][:] = 7.25
+        worse = 1.0
+    dy, dh = rand(g, 2, t, d), rand(g, 2, t, d)
+    got = sb.gated_norm_backward(dy, dh, **s)
+    w = wide(s, grad=True)
+    y, h = norm_formula(**w)
+    ((y * dy.double()).sum() + (h * dh.double()).sum()).backward()
+    for name, r in (("dx", w["x"].grad), ("dz", w["z"].grad), ("post_w", w["post"][0].grad), ("pre_w", w["pre"][0].grad)):
+        size = r.abs() + r.square().mean().sqrt() + (1 if name in ("dx", "dz") else math.sqrt(2 * t))
+        if rows == "flat" and name == "dz":
+            size = size * s["eps"] ** -0.5  # 1 / deviation is sqrt(1 / eps): every term of dz is that large
+        if rows == "flat" and name == "post_w":
+            assert not got[name].any()  # z - mean is exactly zero
+            continue
+        err = (got[name].double() - r).abs()
+        assert (err <= 16 * FP32 * (1 + worse) * size).all(), (name, (err / (16 * FP32 * (1 + worse) * size)).max().item())
 
 
 def test_gated_norm_views_and_offset_rows():

@@ -49,6 +49,19 @@ def test_cross_attention_backward_refuses():
             sb.cross_attention_backward(**{**good, **change})
 
 
+def test_results_over_inputs_are_refused():
+    """Attention reads rows after others are written: a result may not lie on an operand, nor on another."""
+    q, k = torch.zeros(2, 5, 128, **H16), torch.zeros(2, 5, 128, **H16)
+    for x in (q, k):
+        with pytest.raises(ValueError, match="own memory"):
+            attend(q=q, k=k, v=k, kv_heads=4, out=x)
+    lse, grad = torch.zeros(2, 4, 5), torch.zeros(2, 5, 128, **H16)
+    good = dict(dout=q, q=q, k=k, v=k, out=q, lse=lse, heads=4)
+    for change in (dict(dq=q), dict(dk=k), dict(dv=k), dict(dk=grad, dv=grad), dict(dq=grad, dv=grad)):
+        with pytest.raises(ValueError, match="own memory"):
+            sb.cross_attention_backward(**{**good, **change})
+
+
 def test_rope_refuses():
     x, pos = torch.zeros(2, 6, 64), torch.zeros(6, 3, dtype=torch.int32)
     freq, axis = sb.rope_table((4, 6, 6), device="cpu")
