@@ -3,9 +3,10 @@
 // (each norm optional, RMS or layer norm, fp32 statistics), and its gradients.
 //
 // Forward, per row v of D values: RMS norm v r w with r = (mean v^2 + eps)^-1/2; layer norm
-// (v - m) r w + b with r = (mean (v - m)^2 + eps)^-1/2 (the mean first, then the centred
-// squares: no cancellation).  Apart, the norms and the residual sum would read and write the
-// rows five times; here x and z are read and y and h written once, which bounds the kernel.
+// (v - m) r w + b with r = (mean (v - m)^2 + eps)^-1/2 (the mean first, then the centred squares, no
+// cancellation; the backward kernel for aligned rows takes both at once around values of the row).
+// Apart, the norms and the residual sum would read and write the rows five times; here x and z are
+// read and y and h written once, which bounds the kernel.
 //
 // Backward, with hats the normalised rows and e = d * w:
 //   dyt = dy + r_y (e - yhat mean(e yhat) [- mean(e)]),  e = dh * w_pre        -> dx = dyt
@@ -24,6 +25,11 @@
 // ahead, so what is in flight does not cost registers and the reductions' latency is hidden.
 // Element types are compile-time for the usual pairs.  Rows that are not 16-byte aligned or not a
 // multiple of eight columns take plain loads, one row ahead (the kernels named `_any`).
+//
+// Forward, 65,280 rows of 2048 bf16 columns, RMS: 200 us, 82 % of the copy rate.  Backward, 65,280 rows of
+// 1024, x fp32, z bf16, layer norms: 322 us, 57 %: 1100 instructions a warp and step of two rows, three
+// dependent reductions, and registers for twelve warps an SM (a warp issues every 7 clocks; four CTAs an SM
+// spill, 503 us of a run whose three took 384; a third stage of rows changes nothing).
 #include <algorithm>
 
 #include "sb_xattn.cuh"

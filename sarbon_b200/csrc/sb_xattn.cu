@@ -27,8 +27,14 @@
 //                 with the OR of "grew" is all that a tile costs them
 //   cleaner warp  with masks: zeroes V's rows of keys that take no part (0 x NaN is NaN), before
 //                 the product reads them
-// The exponentials (16 a clock and SM) are the floor of heads of few channels; the rest of a row's
-// arithmetic works on pairs.  A polynomial for part of them was slower: the issue slots are as scarce.
+// What bounds it is the chain of a tile: P stored, its product, the wait for it, the next P.  A wait costs
+// 100 to 400 clocks whatever its form (polls, suspended or with sleeps, measured alike), a tile of a stream
+// 2400 with the arithmetic and all but one of its products left out, 4400 with them; two streams overlap,
+// and TMEM has no room for a third or for two P.  2 x 16 heads of 128 channels (4 key heads), 4096
+// queries, 8160 keys: 550 us, 995 TFLOP/s, where the products alone would take 336 and the exponentials
+// (16 a clock and SM) 238.  16 x 8 heads of 32 channels, 300 queries, 28,900 of 42,840 keys: 863 us, of them
+// 215 for the 44 rows behind the second tile, which load two of an SM's four schedulers.  A polynomial for
+// part of the exponentials was slower: the issue slots are as scarce.
 // The key range is split over CTAs where the rows alone leave SMs idle: these write fp32 partial rows
 // with their L, and a second kernel joins them.  Up to 16 rows (single tokens) have a kernel of their
 // own, which reads K and V once at memory speed.
