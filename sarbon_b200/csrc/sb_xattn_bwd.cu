@@ -606,7 +606,10 @@ template <int DH, bool BF16>
 int launch_back(BackArgs& a, const BackPlan& p, cudaStream_t st) {
   constexpr int per = 256 / (DH / 8);
   const int most = std::max(a.Tq, BF16 ? 0 : a.Tk);
-  const dim3 grid((unsigned)(a.B * a.H + (BF16 ? 0 : a.B * a.Hkv)), (unsigned)std::min((most + per - 1) / per, 64));
+  // sixteen CTAs an SM over all heads (8 x 8 heads of 300 queries and up to 2040 keys: 5 us less than with
+  // 64 a head)
+  const int heads = a.B * a.H + (BF16 ? 0 : a.B * a.Hkv), each = std::max(1, 16 * xattn_sms() / heads);
+  const dim3 grid((unsigned)heads, (unsigned)std::min({(most + per - 1) / per, each, 64}));
   if (!BF16 && cudaMemsetAsync(a.top, 0, (size_t)a.B * a.Hkv * 8, st) != cudaSuccess)
     return record_error(SB_ECUDA, "sb_cross_attention_backward: memset");
   attend_back_rows_kernel<DH><<<grid, 256, 0, st>>>(a);
