@@ -10,8 +10,8 @@
 // A thread owns eight pairs of one token: it computes their sines and cosines once and applies
 // them to every head of its chunk, so that the trigonometry is paid once a token and the pass is
 // bound by reading and writing x.  The heads are split over blockIdx.y only where the tokens
-// alone would leave SMs idle.  2 x 65,280 tokens of 8 x 128 channels in bf16: 91 us, 90 % of the copy rate;
-// 3 x 8161 of 12 x 64 in fp32: 37 us, 63 % (one wave of CTAs, so starting and ending show).
+// alone would leave SMs idle.  2 x 65,280 tokens of 8 x 128 channels in bf16: 90 us, 91 % of the copy rate;
+// 3 x 8161 of 12 x 64 in fp32: 35 us, 66 % (one wave of CTAs, so starting and ending show).
 #include <algorithm>
 
 #include "sb_rows.cuh"
@@ -49,9 +49,10 @@ SB_DEV void turn_of(const RopeArgs& a, long long at, int p, float& sn, float& cs
 
 constexpr int kAhead = 2;
 
-// VEC: rows in vectors of eight, of type DT; otherwise element by element
+// VEC: rows in vectors of eight, of type DT; otherwise element by element.  Four blocks an SM: with
+// three, or the five that 48 registers allow, 5 to 50 % slower.
 template <bool VEC, int DT>
-__global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(256, 4) rope_kernel(const __grid_constant__ RopeArgs a) {
   const int dt = VEC ? DT : a.dt;
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= a.units) return;
@@ -181,9 +182,10 @@ extern "C" int sb_rope_axes(const void* x, long long x_row, long long x_img, int
   a.units = (long long)B * T * a.slots;
   const long long blocks = (a.units + 255) / 256;
   if (blocks > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_rope_axes: too many rows");
-  // split the heads until every SM has about eight blocks
+  // split the heads until every SM has its four blocks; more of them pay the trigonometry again (eight an SM:
+  // 41 against 38 us for 3 x 8161 tokens of 12 x 64 in fp16, as long for fp32)
   int parts = 1;
-  while (parts < H && parts < 32 && blocks * parts < 1184) ++parts;
+  while (parts < H && parts < 32 && blocks * parts < 592) ++parts;
   a.heads_per = (H + parts - 1) / parts;
   const dim3 grid((unsigned)blocks, (unsigned)((H + a.heads_per - 1) / a.heads_per));
   auto kernel = !vec               ? rope_kernel<false, 0>

@@ -28,7 +28,7 @@
 //
 // 2 x 16 heads of 128 channels (4 key heads), 2040 queries, 8160 keys: 1140 us, 599 TFLOP/s of the five
 // products' operations, 840 of the seven that are done; what is left is waits, as in the forward kernel.
-// 8 x 8 heads of 64 channels, 300 queries, up to 2040 keys: 139 us, of them 16 for the first kernel, 42 for
+// 8 x 8 heads of 64 channels, 300 queries, up to 2040 keys: 135 us, of them 12 for the first kernel, 42 for
 // dq and 84 for dk and dv, whose CTAs have three steps each: starting and ending take most of theirs.
 #include <algorithm>
 #include <cmath>
