@@ -26,7 +26,7 @@
 // Element types are compile-time for the usual pairs.  Rows that are not 16-byte aligned or not a
 // multiple of eight columns take plain loads, one row ahead (the kernels named `_any`).
 //
-// Forward, 65,280 rows of 2048 bf16 columns, RMS: 200 us, 82 % of the copy rate.  Backward, 65,280 rows of
+// Forward, 65,280 rows of 2048 bf16 columns, RMS: 199 us, 82 % of the copy rate.  Backward, 65,280 rows of
 // 1024, x fp32, z bf16, layer norms: 322 us, 57 %: 1100 instructions a warp and step of two rows, three
 // dependent reductions, and registers for twelve warps an SM (a warp issues every 7 clocks; four CTAs an SM
 // spill, 503 us of a run whose three took 384; a third stage of rows changes nothing).
@@ -338,7 +338,7 @@ SB_DEV void give_up(const Ring& ring, Place at, int left, int me) {
 // other, so that what depends on the columns alone (and an image's gate) stays in registers:
 // y = x + hat A + B with A = scale gate post_w, B = scale gate post_b.
 template <int XD, int ZD, bool LAYER, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT) gated_norm_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(MAXT, MAXT == 128 ? 4 : 1) gated_norm_kernel(const __grid_constant__ NormArgs a) {
   __shared__ __align__(16) float2 buf[64];
   __shared__ uint64_t bars[8 * kMaxStages];
   extern __shared__ __align__(16) uint8_t rows_smem[];
@@ -1237,9 +1237,16 @@ NormKernel pick(bool back, int xdt, int zdt, bool vec, int kind, bool layer) {
   return ring_kernel<-1, -1>(back, kind, layer);
 }
 
-// The ring of each team (as many rows as kRing bytes a CTA hold, two to eight) and a CTA's shared
-// memory, which the backward kernels' last sums share.
-constexpr int kRing = 46 * 1024;
+// CTAs an SM: as many as have 512 threads (backward, with its registers: 384), four (three) at least.  With
+// four CTAs whatever their size 65,280 rows of 1024 bf16 columns took 178 us instead of 121; with 640
+// threads, whose registers then spill, fp32 rows of 2048 take 306 us instead of 278.
+int ctas_of(const Plan& p, bool back) { return back ? std::max(3, 384 / p.threads) : std::max(4, 512 / p.threads); }
+
+// The ring of each team (as many rows as its part of an SM's bytes holds, two to eight) and a CTA's shared
+// memory, which the backward kernels' last sums share.  More rows ahead than these do not help CTA teams: 184 KB
+// of forward rings take as long, or longer (fp32 rows of 2048: 326 us instead of 278); warps, with more
+// rows of an SM's at once, gain (fp32 rows of 256: 61 instead of 66 us).
+int ring_bytes(const Plan& p, bool back) { return (back ? 138 : p.per > 1 ? 184 : 96) * 1024; }
 int ring_of(NormArgs& a, const Plan& p, bool back, bool& vec) {
   const int xs = dtype_bytes(a.xdt), zs = dtype_bytes(a.zdt);
   a.pitch = back ? p.tpr * 8 * (p.at_once == 2 || p.kind == 0 ? 1 : 2) : a.D;
@@ -1247,7 +1254,7 @@ int ring_of(NormArgs& a, const Plan& p, bool back, bool& vec) {
   a.copy_bytes = a.D * elem;
   a.row_bytes = a.pitch * elem;
   a.stage_bytes = a.row_bytes * p.at_once;
-  a.stages = std::max(2, std::min(kMaxStages, kRing / (p.per * a.stage_bytes)));
+  a.stages = std::max(2, std::min(kMaxStages, ring_bytes(p, back) / ctas_of(p, back) / (p.per * a.stage_bytes)));
   vec = vec && 2 * p.per * a.stage_bytes <= 200 * 1024;  // else the widest fp32 rows: no room for two
   const int ring = vec ? p.per * a.stages * a.stage_bytes : 0;
   const int fold = back && p.per > 1 ? p.per * kSums * p.tpr * 8 * 4 : 0;
@@ -1262,10 +1269,9 @@ cudaError_t launch_norm(NormKernel kernel, unsigned grid, int threads, int smem,
   return cudaGetLastError();
 }
 
-// CTAs a group of rows: about `kBackCtas` a SM over all groups, at least eight rows a warp or CTA
-constexpr int kBackCtas = 3, kNormCtas = 4;
+// CTAs a group of rows: about ctas_of an SM over all groups, at least eight rows a warp or CTA
 int chunks_of(int groups, long long group_rows, const Plan& p, int sms) {
-  const long long want = std::max(1, kBackCtas * sms / groups);
+  const long long want = std::max(1, ctas_of(p, true) * sms / groups);
   return (int)std::max(1ll, std::min(want, (group_rows + 8 * p.per - 1) / (8 * p.per)));
 }
 
@@ -1318,7 +1324,7 @@ extern "C" int sb_gated_norm(const void* x, long long x_row, long long x_img, in
   a.gate_is_row = gate && gate_row != 0;
   const int smem = ring_of(a, p, false, vec);
   const NormKernel kernel = pick(false, x_dtype, z_dtype, vec, p.kind, layer != 0);
-  const long long grid = std::min((a.rows + p.per - 1) / p.per, (long long)sms * kNormCtas);
+  const long long grid = std::min((a.rows + p.per - 1) / p.per, (long long)sms * ctas_of(p, false));
   const long long step = grid * p.per;
   a.step_b = step / T;
   a.step_t = (int)(step % T);
