@@ -222,7 +222,7 @@ def test_cross_attention_empty_sizes():
     assert dq.shape == (2, 0, 64) and not dk.any() and not dv.any()
 
 
-def check_backward(grads, dout, q, k, v, heads, kv_heads, lens, valid, out16, scale=None, sub_ds=None, sub_p=None):
+def check_backward(grads, dout, q, k, v, heads, kv_heads, lens, valid, out16, scale=None, sub_ds=None, sub_p=None, one_tile=False):
     ref, lse, p, qd, kd, vd = formula(q, k, v, heads, kv_heads, lens, valid, scale)
     scale = scale or qd.shape[-1] ** -0.5
     g, o = heads_of(dout, heads, kv_heads), heads_of(out16, heads, kv_heads)
@@ -232,7 +232,8 @@ def check_backward(grads, dout, q, k, v, heads, kv_heads, lens, valid, out16, sc
     # dS is off by its rounding, by D from the rounded out, by P and by the fp32 products
     absd = (g.abs() * ref.abs()).sum(-1, keepdim=True)
     sub = 2.0 ** -25 if q.dtype == torch.float16 else 0.0  # fp16 values below 2^-14
-    ds_tol = u * ds.abs() + p * ((g * (o - ref)).abs().sum(-1, keepdim=True) + e * (g.abs() @ vd.abs().transpose(-1, -2) + absd)) + \
+    from_out = 0 if one_tile else (g * (o - ref)).abs().sum(-1, keepdim=True)
+    ds_tol = u * ds.abs() + p * (from_out + e * (g.abs() @ vd.abs().transpose(-1, -2) + absd)) + \
         (sub if sub_ds is None else sub_ds)
     p_tol = (u + e) * p + (sub if sub_p is None else sub_p)
     want = {"dq": (ds @ kd * scale, ds_tol @ kd.abs() * scale),
@@ -289,6 +290,22 @@ def test_cross_attention_backward_strides():
     assert grads[1] is dk and grads[2] is dv
     check_backward(grads, dout, q, k, v, heads, heads, None, None, out)
     assert (both[..., :8] == 3).all() and (both[..., -8:] == 3).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tq,tk,heads,kv_heads,dim", [(300, 2, 3, 1, 32), (7, 20, 4, 4, 64), (140, 128, 2, 1, 128), (5, 400, 2, 2, 64)])
+def test_cross_attention_backward_few_keys(tq, tk, heads, kv_heads, dim, dtype):
+    """Items whose keys fit one tile: D is not left with the rounding of out."""
+    import sarbon_b200 as sb
+    g = gen(tq + tk)
+    b = 4
+    q, dout = (rand(g, b, tq, heads * dim, dtype=dtype) for _ in range(2))
+    k, v = (rand(g, b, tk, kv_heads * dim, dtype=dtype) for _ in range(2))
+    lens = torch.tensor([min(tk, 128), 1, 0, min(tk, 19)], device="cuda", dtype=torch.int32)
+    ref, lse, *_ = formula(q, k, v, heads, kv_heads, lens, None)
+    out, lse = rows_of(ref).to(dtype), lse.flatten(1, 2).float().contiguous()
+    grads = sb.cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=kv_heads, lens=lens)
+    check_backward(grads, dout, q, k, v, heads, kv_heads, lens, None, out, one_tile=True)
 
 
 @pytest.mark.parametrize("kv_heads", [1, 4])
