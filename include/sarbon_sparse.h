@@ -466,7 +466,8 @@ SB_API int sb_l2norm_rows(const void* x, long long ldx, int rows, int D, float* 
  * without keys gets a zero row.  lse (fp32 [B][H][Tq], NULL: none): natural log of the sum of the
  * exponentials, -inf without keys.  scale > 0.  work: sb_cross_attention_work bytes (16-byte
  * aligned), not shared by calls that may overlap.  Scores, statistics and sums are fp32; the
- * probabilities are rounded to dtype before they meet v. */
+ * probabilities are rounded to dtype before they meet v (SB_F16: times 2^7, so that those of 2^-31 of the
+ * row's largest still count). */
 SB_API int sb_cross_attention(const void* q, long long q_row, long long q_img, const void* k, long long k_row,
                               long long k_img, const void* v, long long v_row, long long v_img, int dtype, int B, int H,
                               int Hkv, int dh, int Tq, int Tk, float scale, const int* lens, const void* valid,

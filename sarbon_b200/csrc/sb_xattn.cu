@@ -22,9 +22,9 @@
 //                 streams with 128 channels, which the accumulators leave no room beside; one each
 //                 below); P = 2^(s scale log2 e - m), rounded to the operands' type, back to TMEM.  The
 //                 reference point m moves, and O is rescaled, only when a row's maximum grew by more
-//                 than 2^8 since the last time (P stays below 2^8, far from fp16's limit; m cancels in
-//                 O / l), so the two threads need each other's maximum only then: otherwise one barrier
-//                 with the OR of "grew" is all that a tile costs them
+//                 than 2^8 since the last time (P stays below 2^8, in fp16 times 2^7 below 2^15; m and the
+//                 factor cancel in O / l), so the two threads need each other's maximum only then:
+//                 otherwise one barrier with the OR of "grew" is all that a tile costs them
 //   cleaner warp  with masks: zeroes V's rows of keys that take no part (0 x NaN is NaN), before
 //                 the product reads them
 // What bounds it is the chain of a tile: P stored, its product, the wait for it, the next P.  A wait costs
@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int bar_id = 1 + t * 4 + quad;  // of the two warps of these rows
   float* tell = told + t * 128 + lr;
   const float sl = a.scale_log2;
+  constexpr float lift = kLift<BF16>;
   float m = -INFINITY, l = 0.f;
   bool ok = true;
 
@@ -357,7 +358,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async_smem();
       warp_arrive(&q_full[t]);
     }
-    const float slack = 8.f / sl;
     const uint64_t sl2 = pair2(sl, sl);
     const int jstep = two ? KT : 2 * KT;
     int j0 = (first + (two ? 0 : t)) * KT + hf * 64;
@@ -411,8 +411,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < 64; j += 2)
         mx[j / 2 & 3] = max3(mx[j / 2 & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
       float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-      // a new reference point: with the first tile, and where the maximum grew (or is NaN)
-      const bool grew = pair_or(bar_id, !ok || i == 0 || !(top <= m + slack));
+      // a new reference point: with the first tile, and where the maximum grew (or is NaN).  What is compared
+      // is the exponent that the row's largest P would get, so no score's rounding carries one past 2^15.
+      float ms = fmaf(-m, sl, lift);
+      const bool grew = pair_or(bar_id, !ok || i == 0 || !(fmaf(top, sl, ms) <= lift + 8.f));
       float c = 1.f;
       if (grew) {
         if (hf == 1) *tell = top;
@@ -425,10 +427,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (hf == 1) top = *tell;
         c = m == top ? 1.f : exp2_hw((m - top) * sl);
         m = top;
+        ms = fmaf(-m, sl, lift);
         l *= c;
       }
       // masked scores give 0; a row whose reference is still -inf has had no keys
-      const float ms = m == -INFINITY ? 0.f : -m * sl;
+      if (m == -INFINITY) ms = 0.f;
       const uint64_t ms2 = pair2(ms, ms);
       uint64_t sum[2] = {0, 0};
       // All exponentials before the last product is waited for, or the second half after the first has
@@ -511,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       m = top;
       l = l * w0 + l1 * w1;
     }
-    const float lse = l == 0.f ? -INFINITY : m * sl * 0.69314718055994531f + logf(l);
+    const float lse = l == 0.f ? -INFINITY : fmaf(m, sl, -lift) * 0.69314718055994531f + logf(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     w0 *= inv;
     w1 *= inv;

@@ -54,6 +54,14 @@ struct FwdArgs {
   long long all_rows;
 };
 
+// fp16 probabilities are held times 2^kLift: the reference point keeps them below 2^8, so fp16 has seven more
+// powers of two above, and what a long memory's many small ones add up to is not lost (42,839 keys at
+// 2^-25 of the one on top: 0 instead of 1.3e-3 without).  A value below 2^-14 is off by 2^-25, so Tk keys are
+// off by Tk 2^-32 of the row's sum at most, less than fp16's own half step up to two million of them.
+// The sum is taken of the same values, so the factor leaves with it.  bf16 has fp32's range.
+template <bool BF16>
+constexpr float kLift = BF16 ? 0.f : 7.f;
+
 // ---------------------------------------------------------------- tcgen05 forms
 // D[tmem] (+)= A[tmem] * B[smem]: A holds 16-bit pairs, k and k + 1 in a 32-bit column.
 SB_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accum) {

@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   for (int i = 0; i < DH / 8; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-  const float sl = a.scale_log2, slack = 8.f / sl;
+  constexpr float lift = kLift<BF16>;
+  const float sl = a.scale_log2;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   const int krow = lane & 7, kc = lane >> 3;
   const int vrow = ((lane >> 3) & 1) * 8 + (lane & 7), vc = lane >> 4;
@@ -192,11 +193,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       t1 = max3(t1, u1, u1);
     }
     // a new reference point with the first keys, and where a maximum grew by more than 2^8 (or is NaN)
-    if (__any_sync(0xFFFFFFFFu, !(t0 <= m0 + slack) || !(t1 <= m1 + slack))) {
+    // (what is compared is the exponent that a row's largest P would get)
+    float r0 = fmaf(-m0, sl, lift), r1 = fmaf(-m1, sl, lift);
+    if (__any_sync(0xFFFFFFFFu, !(fmaf(t0, sl, r0) <= lift + 8.f) || !(fmaf(t1, sl, r1) <= lift + 8.f))) {
       const float n0 = max3(m0, t0, t0), n1 = max3(m1, t1, t1);
       const float c0 = m0 == n0 ? 1.f : exp2_hw((m0 - n0) * sl), c1 = m1 == n1 ? 1.f : exp2_hw((m1 - n1) * sl);
       m0 = n0;
       m1 = n1;
+      r0 = fmaf(-m0, sl, lift);
+      r1 = fmaf(-m1, sl, lift);
       l0 *= c0;
       l1 *= c1;
 #pragma unroll
@@ -207,7 +212,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         o[x][3] *= c1;
       }
     }
-    const float r0 = m0 == -INFINITY ? 0.f : -m0 * sl, r1 = m1 == -INFINITY ? 0.f : -m1 * sl;
+    if (m0 == -INFINITY) r0 = 0.f;
+    if (m1 == -INFINITY) r1 = 0.f;
     uint32_t p[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -287,7 +293,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     const float inv = none ? 0.f : 1.f / l;
 #pragma unroll
     for (int u = 0; u < 8; ++u) f[u] = none ? 0.f : f[u] * inv;
-    const float lse = none ? -INFINITY : top * sl * 0.69314718055994531f + logf(l);
+    const float lse = none ? -INFINITY : fmaf(top, sl, -lift) * 0.69314718055994531f + logf(l);
     const int t = r / a.group, h = kvh * a.group + r - t * a.group;
     const long long rr = ((long long)b * a.H + h) * a.Tq + t;
     if (a.splits > 1) {

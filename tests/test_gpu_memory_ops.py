@@ -205,6 +205,52 @@ def test_cross_attention_large_scores(dtype):
     check_forward(out, lse, q, k, v, heads, heads, None, None, scale=1.0)
 
 
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("tq", [1, 16, 40, 300])
+@pytest.mark.parametrize("far", [25.0, 24.6, 30.0])
+def test_cross_attention_small_probabilities(tq, dim, far):
+    """One key on top of a long memory, the others 2^-far of it: their sum counts although each lies near or
+    below fp16's smallest number.  P is held times 2^7, where a value below 2^-14 is rounded by at most
+    2^-25, so each of them is off by at most 2^-32 of the top one (or u of itself)."""
+    import sarbon_b200 as sb
+    b, tk = 160, 8160
+    z = dict(device="cuda", dtype=torch.float16)
+    q, k, v = torch.zeros(b, tq, dim, **z), torch.zeros(b, tk, dim, **z), torch.ones(b, tk, dim, **z)
+    q[..., 0] = 1
+    k[:, 1:, 0] = -far  # scores in powers of two: the scale is log 2
+    v[:, 0] = 0
+    lse = torch.empty(b, 1, tq, device="cuda")
+    out = sb.cross_attention(q, k, v, 1, scale=math.log(2.0), lse=lse)
+    each = 2.0 ** k[0, 1, 0].double().item()
+    total = 1 + (tk - 1) * each
+    u, e = unit(torch.float16), FP32 + 2 * (dim + 2) * 2.0 ** -24 * far
+    want = (tk - 1) * each / total
+    tol = want * (2 * u + e) + (tk - 1) * 2.0 ** -32 + 2.0 ** -25
+    assert ((out.double() - want).abs() <= 1.02 * tol).all(), (out.double().min().item(), out.double().max().item(), want)
+    assert ((lse.double() - math.log(total)).abs() <= e).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tq", [1, 300])
+def test_cross_attention_huge_scores(tq, dtype):
+    """Scores of tens of millions, far apart and growing, with ties at the top: exact integers in fp32, and
+    probabilities of 1 / ties and 0."""
+    import sarbon_b200 as sb
+    b, tk, dim = 160, 1400, 64
+    z = dict(device="cuda", dtype=dtype)
+    q, k = torch.full((b, tq, dim), 128.0, **z), torch.zeros(b, tk, dim, **z)
+    v = rand(gen(8), b, tk, dim, dtype=dtype)
+    k[:] = (8192.0 - 64.0 * torch.arange(13, -1, -1, device="cuda").repeat_interleave(100))[:, None].to(dtype)
+    lse = torch.empty(b, 1, tq, device="cuda")
+    out = sb.cross_attention(q, k, v, 1, scale=math.log(2.0), lse=lse)
+    best = k[0, :, 0] == k[0, -1, 0]
+    want = v[:, best].double().mean(1, keepdim=True).expand(b, tq, dim)
+    tol = 2 * unit(dtype) * v[:, best].double().abs().mean(1, keepdim=True) + FP32 + 2.0 ** -25
+    assert ((out.double() - want).abs() <= 1.02 * tol).all()
+    score = math.log(2.0) * 64 * 128 * k[0, -1, 0].double().item()
+    assert ((lse.double() - score - math.log(best.sum().item())).abs() <= 2.0 ** -22 * score).all()
+
+
 def test_cross_attention_empty_sizes():
     import sarbon_b200 as sb
     z = dict(device="cuda", dtype=torch.float16)
