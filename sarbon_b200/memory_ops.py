@@ -18,7 +18,7 @@ caching allocator for each call, so calls on two streams or in two graphs share 
 
 Gradients are calls of their own (``cross_attention_backward``, ``rope_axes(inverse=True)``,
 ``gated_norm_backward``) that an ``autograd.Function`` or a hand-written step makes; the forward
-calls record no graph and refuse tensors that would need one.
+calls record no graph and refuse tensors that would need one, or that carry a forward-mode tangent.
 """
 from __future__ import annotations
 
@@ -26,6 +26,7 @@ import ctypes as C
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, lib
@@ -46,6 +47,11 @@ _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_devic
 
 def _ready(*tensors):
     """All tensors on one CUDA device and none that autograd would have to follow; its index."""
+    # a dual tensor does not require a gradient; looked for only inside a forward_ad.dual_level
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t, level=0).tangent is not None:
+                raise ValueError("no forward-mode tangent is followed: call on primals")
     index = tensors[0].get_device()
     grad = torch.is_grad_enabled()
     for t in tensors:

@@ -129,6 +129,26 @@ def test_autograd_inputs_are_refused():
         sb.cross_attention(q, q, q, 1)
 
 
+def test_forward_mode_inputs_are_refused():
+    """A dual tensor does not say that it requires a gradient; its tangent would be lost."""
+    import torch.autograd.forward_ad as fw
+    q = torch.zeros(1, 2, 64, **H16)
+    x, freq, axis = torch.zeros(1, 2, 64), *sb.rope_table((32,), device="cpu")
+    pos = torch.zeros(2, 1, dtype=torch.int32)
+    with fw.dual_level():
+        dual, dual32 = fw.make_dual(q, torch.ones_like(q)), fw.make_dual(x, torch.ones_like(x))
+        lse = torch.zeros(1, 1, 2)
+        for call in (lambda: sb.cross_attention(q, dual, q, 1), lambda: sb.cross_attention_backward(dual, q, q, q, q, lse, 1),
+                     lambda: sb.rope_axes(dual32, pos, 1, freq, axis), lambda: sb.gated_norm(x, x, scale=dual32[0, 0]),
+                     lambda: sb.gated_norm_backward(dual32, None, x, x)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            sb.cross_attention(dual, q, q, 1)
+        with pytest.raises(ValueError, match="CUDA"):  # none among these
+            sb.cross_attention(q, q, q, 1)
+
+
 def test_rope_table_and_grid():
     freq, axis = sb.rope_table((2, 0, 4), theta=100.0, device="cpu")
     assert axis.tolist() == [0, 0, 2, 2, 2, 2]
