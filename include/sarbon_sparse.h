@@ -460,7 +460,8 @@ SB_API int sb_l2norm_rows(const void* x, long long ldx, int rows, int D, float* 
 /* Attention of Tq queries to an encoder's Tk states, out = softmax(scale q k^T) v per head.
  * H query heads of dh = 32, 64 or 128 channels (head h = columns h*dh ..), Hkv key / value heads,
  * H % Hkv == 0, query head h reads key head h / (H / Hkv).  q, k, v, out have one dtype (SB_F16 or
- * SB_BF16), 16-byte aligned bases, row and img multiples of 8.  Key j of item b takes part when
+ * SB_BF16), 16-byte aligned bases, row and img multiples of 8, and for k and v a row other than 0
+ * where Tk > 1 (backward also for q and dout where Tq > 1).  Key j of item b takes part when
  * j < lens[b] (int32 [B], NULL: Tk; values outside [0, Tk] are clamped) and valid[b * valid_img + j]
  * != 0 (uint8, NULL: all).  Keys that do not take part may hold anything, NaN included.  A query
  * without keys gets a zero row.  lse (fp32 [B][H][Tq], NULL: none): natural log of the sum of the

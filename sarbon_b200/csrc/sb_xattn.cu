@@ -722,6 +722,9 @@ bool xattn_view_ok(const void* p, long long row, long long img) {
   return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && row >= 0 && img >= 0 && row % 8 == 0 && img % 8 == 0 &&
          row < (1ll << 38) && img < (1ll << 38);
 }
+bool xattn_map_ok(const void* p, long long row, long long img, int T) {
+  return xattn_view_ok(p, row, img) && (row > 0 || T == 1);
+}
 
 bool xattn_tensor_map(CUtensorMap* map, const View& v, int dtype, int B, int T, int heads, int dh, int rows) {
   PFN_encodeTiled enc = encode_fn();
@@ -729,10 +732,9 @@ bool xattn_tensor_map(CUtensorMap* map, const View& v, int dtype, int B, int T, 
   const bool one = v.img == 0;
   const cuuint64_t row = (cuuint64_t)v.row * 2, img = one ? 16 : (cuuint64_t)v.img * 2;
   cuuint64_t dims[4] = {(cuuint64_t)dh, (cuuint64_t)T, (cuuint64_t)heads, one ? 1u : (cuuint64_t)B};
-  cuuint64_t strides[3] = {row == 0 ? 16 : row, (cuuint64_t)dh * 2, img};
+  cuuint64_t strides[3] = {row == 0 ? 16 : row, (cuuint64_t)dh * 2, img};  // (a single row's is never used)
   cuuint32_t box[4] = {(cuuint32_t)std::min(dh, 64), (cuuint32_t)rows, 1u, 1u};
   cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
-  if (row == 0 && T > 1) return false;
   return enc(map, dtype == SB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
              const_cast<void*>(v.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
              dh < 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -800,8 +802,8 @@ extern "C" int sb_cross_attention(const void* q, long long q_row, long long q_im
     return record_error(SB_EINVAL, "sb_cross_attention: sizes (dh 32, 64 or 128, H a multiple of Hkv), dtype or scale");
   if (B == 0 || Tq == 0) return SB_OK;
   if (!xattn_view_ok(q, q_row, q_img) || !xattn_view_ok(out, o_row, o_img) ||
-      (Tk > 0 && (!xattn_view_ok(k, k_row, k_img) || !xattn_view_ok(v, v_row, v_img))))
-    return record_error(SB_EINVAL, "sb_cross_attention: rows (16-byte aligned, strides multiples of 8)");
+      (Tk > 0 && (!xattn_map_ok(k, k_row, k_img, Tk) || !xattn_map_ok(v, v_row, v_img, Tk))))
+    return record_error(SB_EINVAL, "sb_cross_attention: rows (16-byte aligned, strides multiples of 8, k's and v's not 0)");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (Tk == 0) {
     const long long n = (long long)B * Tq * H * dh;
@@ -828,6 +830,12 @@ extern "C" int sb_cross_attention(const void* q, long long q_row, long long q_im
   a.masked = lens || valid;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.all_rows = (long long)B * H * Tq;
+  // (before the first launch: a call that is refused has done nothing)
+  CUtensorMap km, vm;
+  const int box = p.few ? few_keys(dh) : KT;
+  if (!xattn_tensor_map(&km, {k, k_row, k_img}, dtype, B, Tk, Hkv, dh, box) ||
+      !xattn_tensor_map(&vm, {v, v_row, v_img}, dtype, B, Tk, Hkv, dh, box))
+    return record_error(SB_EINVAL, "sb_cross_attention: tensor map of k or v");
   if (valid) {
     int* last = static_cast<int*>(work);
     const cudaError_t e = count_keys(a.mask, B, last, st);
@@ -836,11 +844,6 @@ extern "C" int sb_cross_attention(const void* q, long long q_row, long long q_im
   }
   a.part_o = reinterpret_cast<float*>(static_cast<char*>(work) + counts);
   a.part_l = a.part_o + (long long)p.splits * a.all_rows * dh;
-  CUtensorMap km, vm;
-  const int box = p.few ? few_keys(dh) : KT;
-  if (!xattn_tensor_map(&km, {k, k_row, k_img}, dtype, B, Tk, Hkv, dh, box) ||
-      !xattn_tensor_map(&vm, {v, v_row, v_img}, dtype, B, Tk, Hkv, dh, box))
-    return record_error(SB_EINVAL, "sb_cross_attention: tensor map of k or v");
   const bool bf16 = dtype == SB_BF16;
   if (p.few) {
     cudaError_t e = few_launch(a, dh, bf16, km, vm, st);

@@ -220,8 +220,9 @@ SB_DEV uint32_t pack16(float lo, float hi) {
 // multiply the item by 0 then.
 bool xattn_tensor_map(CUtensorMap* map, const View& v, int dtype, int B, int T, int heads, int dh, int rows);
 bool xattn_sizes_ok(int dtype, int B, int H, int Hkv, int dh, int Tq, int Tk);
-// 16-byte rows whose strides fit a tensor map
+// 16-byte rows whose strides fit a tensor map; where one is made, several rows may not be one and the same
 bool xattn_view_ok(const void* p, long long row, long long img);
+bool xattn_map_ok(const void* p, long long row, long long img, int T);
 // counts[b] = 1 + the last key of item b that takes part (0: none): keys behind it are never looked at.
 constexpr long long counts_bytes(int masked, int B) { return masked ? ((long long)B * 4 + 15) / 16 * 16 : 0; }
 cudaError_t count_keys(const KeyMask& mask, int B, int* counts, cudaStream_t st);

@@ -627,7 +627,19 @@ cudaError_t launch_side(BackArgs a, const SidePlan& p, const CUtensorMap& y1, co
 }
 
 template <int DH, bool BF16>
-int launch_back(BackArgs& a, const BackPlan& p, cudaStream_t st) {
+int launch_back(BackArgs& a, const BackPlan& p, int* counts, cudaStream_t st) {
+  // all maps before the first launch: a call that is refused has done nothing
+  CUtensorMap km, vm, qm, dm;
+  if (!xattn_tensor_map(&km, a.k, a.dt, a.B, a.Tk, a.Hkv, DH, kStep) ||
+      !xattn_tensor_map(&vm, a.v, a.dt, a.B, a.Tk, a.Hkv, DH, kStep) ||
+      !xattn_tensor_map(&qm, a.q, a.dt, a.B, a.Tq, a.H, DH, kStep) ||
+      !xattn_tensor_map(&dm, a.dout, a.dt, a.B, a.Tq, a.H, DH, kStep))
+    return record_error(SB_EINVAL, "sb_cross_attention_backward: tensor map of k, v, q or dout");
+  if (a.mask.valid) {
+    const cudaError_t e = count_keys(a.mask, a.B, counts, st);
+    if (e != cudaSuccess) return record_error(SB_ECUDA, cudaGetErrorString(e));
+    a.mask.lens = counts;
+  }
   constexpr int per = 256 / (DH / 8);
   const int most = std::max(a.Tq, BF16 ? 0 : a.Tk);
   // sixteen CTAs an SM over all heads (8 x 8 heads of 300 queries and up to 2040 keys: 5 us less than with
@@ -637,20 +649,13 @@ int launch_back(BackArgs& a, const BackPlan& p, cudaStream_t st) {
   if (!BF16 && cudaMemsetAsync(a.top, 0, (size_t)a.B * a.Hkv * 8, st) != cudaSuccess)
     return record_error(SB_ECUDA, "sb_cross_attention_backward: memset");
   attend_back_rows_kernel<DH><<<grid, 256, 0, st>>>(a);
-  CUtensorMap y1, y2;
-  if (!xattn_tensor_map(&y1, a.k, a.dt, a.B, a.Tk, a.Hkv, DH, kStep) ||
-      !xattn_tensor_map(&y2, a.v, a.dt, a.B, a.Tk, a.Hkv, DH, kStep))
-    return record_error(SB_EINVAL, "sb_cross_attention_backward: tensor map of k or v");
   a.y1_item = a.k.img != 0;
   a.y2_item = a.v.img != 0;
-  cudaError_t e = launch_side<DH, BF16, 0>(a, p.side[0], y1, y2, st);
+  cudaError_t e = launch_side<DH, BF16, 0>(a, p.side[0], km, vm, st);
   if (e != cudaSuccess) return record_error(SB_ECUDA, cudaGetErrorString(e));
-  if (!xattn_tensor_map(&y1, a.q, a.dt, a.B, a.Tq, a.H, DH, kStep) ||
-      !xattn_tensor_map(&y2, a.dout, a.dt, a.B, a.Tq, a.H, DH, kStep))
-    return record_error(SB_EINVAL, "sb_cross_attention_backward: tensor map of q or dout");
   a.y1_item = a.q.img != 0;
   a.y2_item = a.dout.img != 0;
-  e = launch_side<DH, BF16, 1>(a, p.side[1], y1, y2, st);
+  e = launch_side<DH, BF16, 1>(a, p.side[1], qm, dm, st);
   return e == cudaSuccess ? SB_OK : record_error(SB_ECUDA, cudaGetErrorString(e));
 }
 
@@ -694,11 +699,12 @@ extern "C" int sb_cross_attention_backward(const void* dout, long long do_row, l
     return record_error(SB_EINVAL,
                         "sb_cross_attention_backward: sizes (dh 32, 64 or 128, H a multiple of Hkv), dtype or scale");
   if (B == 0 || (Tq == 0 && Tk == 0)) return SB_OK;
-  if ((Tq > 0 && (!lse || !xattn_view_ok(dout, do_row, do_img) || !xattn_view_ok(q, q_row, q_img) ||
+  if ((Tq > 0 && (!lse || !xattn_map_ok(dout, do_row, do_img, Tq) || !xattn_map_ok(q, q_row, q_img, Tq) ||
                   !xattn_view_ok(out, o_row, o_img) || !xattn_view_ok(dq, dq_row, dq_img))) ||
-      (Tk > 0 && (!xattn_view_ok(k, k_row, k_img) || !xattn_view_ok(v, v_row, v_img) ||
+      (Tk > 0 && (!xattn_map_ok(k, k_row, k_img, Tk) || !xattn_map_ok(v, v_row, v_img, Tk) ||
                   !xattn_view_ok(dk, dk_row, dk_img) || !xattn_view_ok(dv, dv_row, dv_img))))
-    return record_error(SB_EINVAL, "sb_cross_attention_backward: rows (16-byte aligned, strides multiples of 8) or lse");
+    return record_error(SB_EINVAL, "sb_cross_attention_backward: rows (16-byte aligned, strides multiples of 8, dout's, q's, "
+                                   "k's and v's not 0) or lse");
   BackArgs a{};
   a.q = {q, q_row, q_img}; a.k = {k, k_row, k_img}; a.v = {v, v_row, v_img};
   a.out = {out, o_row, o_img}; a.dout = {dout, do_row, do_img};
@@ -730,19 +736,14 @@ extern "C" int sb_cross_attention_backward(const void* dout, long long do_row, l
   for (const SidePlan& s : p.side)
     if (s.units * s.splits > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_cross_attention_backward: too many items");
   if ((long long)B * (H + Hkv) > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_cross_attention_backward: too many items");
-  if (valid) {
-    int* last = static_cast<int*>(work);
-    const cudaError_t e = count_keys(a.mask, B, last, st);
-    if (e != cudaSuccess) return record_error(SB_ECUDA, cudaGetErrorString(e));
-    a.mask.lens = last;
-  }
+  int* counts_at = static_cast<int*>(work);
   a.lse2 = reinterpret_cast<float*>(static_cast<char*>(work) + counts);
   a.delta = a.lse2 + p.rows;
   a.top = reinterpret_cast<unsigned*>(a.delta + p.rows);
   a.part = reinterpret_cast<float*>(static_cast<char*>(work) + counts + (p.rows * 8 + (long long)B * Hkv * 8 + 15) / 16 * 16);
   if (dtype == SB_BF16)
-    return dh == 32 ? launch_back<32, true>(a, p, st) : dh == 64 ? launch_back<64, true>(a, p, st)
-                                                                 : launch_back<128, true>(a, p, st);
-  return dh == 32 ? launch_back<32, false>(a, p, st) : dh == 64 ? launch_back<64, false>(a, p, st)
-                                                                : launch_back<128, false>(a, p, st);
+    return dh == 32 ? launch_back<32, true>(a, p, counts_at, st) : dh == 64 ? launch_back<64, true>(a, p, counts_at, st)
+                                                                 : launch_back<128, true>(a, p, counts_at, st);
+  return dh == 32 ? launch_back<32, false>(a, p, counts_at, st) : dh == 64 ? launch_back<64, false>(a, p, counts_at, st)
+                                                                : launch_back<128, false>(a, p, counts_at, st);
 }

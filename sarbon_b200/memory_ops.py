@@ -11,7 +11,8 @@ attends to the tokens of p8 / p16 / p32, of several frames or of images padded t
     x, h = gated_norm(x, proj(o), gate=gate, post=(w0, b0), pre=(w1, b1), kind="layer")
 
 Rows are ``[B, T, channels]`` with contiguous channels; slices of wider projections, sequence-first
-layouts and memories shared by all items (a batch stride of 0) are read as they are.  Every call
+layouts and memories shared by all items (a batch stride of 0) are read as they are; attention copies
+operands whose rows are one expanded row where its kernels cannot.  Every call
 launches kernels of ``libsarbon_sparse.so`` on the current CUDA stream of its tensors' device and can
 be captured in a CUDA graph after a first call outside capture.  Workspaces come from torch's
 caching allocator for each call, so calls on two streams or in two graphs share none.
@@ -113,6 +114,13 @@ def _rows(t, what, shape, dtype, out=False):
     return t.data_ptr(), row, img
 
 
+def _own_rows(t):
+    """t, or a copy where its rows are one and the same (a row stride of 0, which no tensor map has)."""
+    if t.dim() != 3 or t.stride(1) != 0 or t.shape[1] <= 1:
+        return t
+    return t[:1].contiguous().expand(t.shape) if t.stride(0) == 0 else t.contiguous()
+
+
 def _apart(results, operands):
     """Results that do not begin where an operand or another result does."""
     seen = {t.data_ptr() for t in operands if t.numel()}
@@ -187,6 +195,7 @@ def cross_attention(q, k, v, heads, kv_heads=None, lens=None, valid=None, scale=
     queries on many states (single tokens) are split over the states."""
     kv_heads, b, tq, tk, dim, scale = _attention_sizes(q, k, heads, kv_heads, scale)
     dtype, qs, ks = q.dtype, (b, tq, heads * dim), (b, tk, kv_heads * dim)
+    k, v = _own_rows(k), _own_rows(v)
     qp, kp, vp = _rows(q, "q", qs, dtype), _rows(k, "k", ks, dtype), _rows(v, "v", ks, dtype)
     masks = _masks(lens, valid, b, tk)
     if lse is not None:
@@ -215,6 +224,7 @@ def cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=None, lens
     dv (allocated if None) must not share memory with an operand or each other."""
     kv_heads, b, tq, tk, dim, scale = _attention_sizes(q, k, heads, kv_heads, scale)
     dtype, qs, ks = q.dtype, (b, tq, heads * dim), (b, tk, kv_heads * dim)
+    dout, q, k, v = _own_rows(dout), _own_rows(q), _own_rows(k), _own_rows(v)
     views = _rows(dout, "dout", qs, dtype) + _rows(q, "q", qs, dtype) + _rows(k, "k", ks, dtype) + \
         _rows(v, "v", ks, dtype) + _rows(out, "out", qs, dtype)
     masks = _masks(lens, valid, b, tk)

@@ -374,6 +374,24 @@ def test_cross_attention_backward_small_fp16(kv_heads):
                    sub_p=2.0 ** -39)
 
 
+@pytest.mark.parametrize("which", ["dout", "q", "k", "v", "all"])
+def test_cross_attention_rows_of_one(which):
+    """Operands whose rows are one and the same (row stride 0): the gradient of a sum over the queries, one
+    learned query for every place, one state for every key."""
+    import sarbon_b200 as sb
+    g = gen(12)
+    b, tq, tk, heads, kv_heads, dim = 2, 140, 200, 4, 2, 64
+    x = {n: rand(g, b, 1 if which in (n, "all") else t, h * dim, dtype=torch.bfloat16).expand(b, t, h * dim)
+         for n, t, h in (("dout", tq, heads), ("q", tq, heads), ("k", tk, kv_heads), ("v", tk, kv_heads))}
+    valid = torch.rand(b, tk, device="cuda", generator=g) < 0.7
+    dout, qkv = x.pop("dout"), list(x.values())
+    lse = torch.empty(b, heads, tq, device="cuda")
+    out = sb.cross_attention(*qkv, heads, kv_heads=kv_heads, valid=valid, lse=lse)
+    check_forward(out, lse, *qkv, heads, kv_heads, None, valid)
+    grads = sb.cross_attention_backward(dout, *qkv, out, lse, heads, kv_heads=kv_heads, valid=valid)
+    check_backward(grads, dout, *qkv, heads, kv_heads, None, valid, out)
+
+
 def test_cross_attention_gradient_against_differences():
     """<gradient, direction> against the central difference of the 64-bit formula, whose own error at
     step 1e-4 is of order 1e-8; the gradients carry roundings of u to each of their many terms."""

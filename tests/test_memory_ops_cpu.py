@@ -123,6 +123,27 @@ def test_library_refuses():
     assert lib.sb_rope_axes(None, 64, 64, 0, 1, 1, 1, 64, one, 0, 0, 1, one, one, 32, 0, 0, one, 64, 64, None) == _lib.SB_EINVAL
 
 
+def test_library_refuses_rows_of_one():
+    """A row stride of 0 where there are several rows is turned down before anything is launched, by the
+    operands that tensor maps describe: k, v and, backward, q and dout."""
+    lib, one = _lib.lib(), C.c_void_p(16)
+    rows = {n: (128, 1024) for n in ("dout", "q", "k", "v", "out")}
+
+    def call(back, **change):
+        r = {**rows, **change}
+        names = ["dout", "q", "k", "v", "out"] if back else ["q", "k", "v"]
+        a = [x for n in names for x in (one, *r[n])] + ([one] if back else [])
+        a += [0, 1, 2, 1, 64, 4, 4, 1.0, None, None, 0]
+        if back:
+            return lib.sb_cross_attention_backward(*a, *(one, 128, 1024) * 3, None, 0, None)
+        return lib.sb_cross_attention(*a, one, 128, 1024, None, None, 0, None)
+
+    for n in ("k", "v"):
+        assert call(False, **{n: (0, 1024)}) == _lib.SB_EINVAL, n
+    for n in ("dout", "q", "k", "v"):
+        assert call(True, **{n: (0, 1024)}) == _lib.SB_EINVAL, n
+
+
 def test_autograd_inputs_are_refused():
     q = torch.zeros(1, 2, 64, **H16, requires_grad=True)
     with pytest.raises(ValueError):
