@@ -19,9 +19,11 @@
 // global memory this costs 2 of 7 products and saves the atomics.
 //
 // fp16 gradients: P and dS may be far below fp16's smallest normal number (long memories, small
-// losses).  P is held as 2^14 P, and dS as F dS with F the power of two that the bound |dS| <= 2 P
-// max|dout_i| max|v_j| (norms over the item and key head, from a first kernel that also forms D)
-// keeps below 2^15; both factors leave at the end.  bf16 has fp32's range and needs neither.
+// losses).  P is held as 2^14 P, and dS as F dS with F the power of two that the bound |dS_i| <= 2 P_i
+// |dout_i| max|v_j| (norms from a first kernel that also forms D, the largest over the item and key head) keeps
+// below 2^15; both factors leave at the end.  For dq each row has its own F, so that one query with a
+// gradient 2^23 times the others' takes nothing from theirs; dk and dv add rows up and have one F of the largest
+// |dout_i| of an item and key head.  bf16 has fp32's range and needs neither.
 //
 // A range of steps may be split over CTAs (few rows against many): these write fp32 partial
 // results, which a last kernel adds in order.
@@ -55,6 +57,7 @@ struct BackArgs {
   float scale, scale_log2;
   float* lse2;   // [B][H][Tq] L log2 e, +inf for a row without keys
   float* delta;  // [B][H][Tq]
+  float* norm;   // [B][H][Tq] |dout_i| (fp16 only)
   unsigned* top;  // [B][Hkv][2] bits of max |dout_i|, max |v_j| (fp16 only)
   float* part;   // [splits][held rows of all][DH] (SIDE 1: dk, then dv)
   long long part_rows;
@@ -98,6 +101,7 @@ __global__ void __launch_bounds__(256) attend_back_rows_kernel(const __grid_cons
       const float l = a.lse[r];
       a.delta[r] = l == -INFINITY ? 0.f : d;
       a.lse2[r] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
+      if (a.dt == SB_F16) a.norm[r] = sqrtf(sq);
     }
   }
   if (a.dt != SB_F16) return;
@@ -369,17 +373,17 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
     // P is held as 2^lift P, dS as F dS with F = f 2^lift
     constexpr float lift = BF16 ? 0.f : 14.f;
     float f = 1.f;
+    const long long qrow = ((long long)b * a.H + h) * a.Tq + tq;  // SIDE 0: the held row
     if constexpr (!BF16) {
       const unsigned* top = a.top + (b * a.Hkv + kvh) * 2;
-      const float bound = __uint_as_float(top[0]) * __uint_as_float(top[1]);
+      const float bound = (SIDE == 1 ? __uint_as_float(top[0]) : live ? a.norm[qrow] : 0.f) * __uint_as_float(top[1]);
       if (bound > 0.f && bound < INFINITY) f = exp2f(-(float)(ilogbf(bound) + 1));
     }
     const float sl = a.scale_log2;
     float l2 = INFINITY, df = 0.f;
     if (SIDE == 0 && live) {
-      const long long r = ((long long)b * a.H + h) * a.Tq + tq;
-      l2 = a.lse2[r] - lift;
-      df = a.delta[r] * f;
+      l2 = a.lse2[qrow] - lift;
+      df = a.delta[qrow] * f;
     }
     float* mine = stat + warp * 128;  // [2][L, D][32]
     float next[2];
@@ -470,7 +474,7 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
         told[cg * 128] = sum;
         meet();
         df += ((told[0] + told[128]) + (told[256] + told[384])) * exp2f(-lift);
-        if (live && cg == 0) a.delta[((long long)b * a.H + h) * a.Tq + tq] = df / f;
+        if (live && cg == 0) a.delta[qrow] = df / f;
       }
 #pragma unroll
       for (int j = 0; j < 32; ++j) p[j] *= fmaf(__uint_as_float(s[j]), f, -(SIDE == 0 ? df : st[32 + j]));
@@ -505,7 +509,7 @@ __global__ void __launch_bounds__(Back<DH, SIDE>::THREADS, 1)
       const uint32_t from = tmem + lanes + C::ACC + (SIDE == 0 ? 0 : u * DH) + c0;
       const float by = SIDE == 1 && u == 1 ? exp2f(-lift) : a.scale * exp2f(-lift) / f;
       const OutView& o = SIDE == 0 ? a.dq : u == 0 ? a.dk : a.dv;
-      const long long prow = SIDE == 0 ? ((long long)b * a.H + h) * a.Tq + tq
+      const long long prow = SIDE == 0 ? qrow
                                        : (((long long)u * a.B + b) * a.Hkv + kvh) * a.Tk + x;
 #pragma unroll
       for (int c = 0; c < cols; c += 16) {
@@ -595,6 +599,8 @@ SidePlan side_plan(long long items, long long x_rows, long long steps, long long
   }
   return p;
 }
+// lse2, delta, norm and top
+long long stats_bytes(long long rows, long long items) { return (rows * 12 + items * 8 + 15) / 16 * 16; }
 BackPlan back_plan(int B, int H, int Hkv, int dh, int Tq, int Tk, int sms) {
   BackPlan p;
   const long long group = H / Hkv, items = (long long)B * Hkv;
@@ -604,7 +610,7 @@ BackPlan back_plan(int B, int H, int Hkv, int dh, int Tq, int Tk, int sms) {
   long long part = 0;  // the sides run one after the other and share it
   for (const SidePlan& s : p.side)
     if (s.splits > 1) part = std::max(part, (long long)s.splits * s.part_rows * dh * 4);
-  p.bytes = (p.rows * 8 + items * 8 + 15) / 16 * 16 + part;
+  p.bytes = stats_bytes(p.rows, items) + part;
   return p;
 }
 
@@ -739,8 +745,9 @@ extern "C" int sb_cross_attention_backward(const void* dout, long long do_row, l
   int* counts_at = static_cast<int*>(work);
   a.lse2 = reinterpret_cast<float*>(static_cast<char*>(work) + counts);
   a.delta = a.lse2 + p.rows;
-  a.top = reinterpret_cast<unsigned*>(a.delta + p.rows);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(work) + counts + (p.rows * 8 + (long long)B * Hkv * 8 + 15) / 16 * 16);
+  a.norm = a.delta + p.rows;
+  a.top = reinterpret_cast<unsigned*>(a.norm + p.rows);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(work) + counts + stats_bytes(p.rows, (long long)B * Hkv));
   if (dtype == SB_BF16)
     return dh == 32 ? launch_back<32, true>(a, p, counts_at, st) : dh == 64 ? launch_back<64, true>(a, p, counts_at, st)
                                                                  : launch_back<128, true>(a, p, counts_at, st);

@@ -392,6 +392,33 @@ def test_cross_attention_rows_of_one(which):
     check_backward(grads, dout, *qkv, heads, kv_heads, None, valid, out)
 
 
+@pytest.mark.parametrize("top", [2.0 ** 15, math.inf])
+def test_cross_attention_backward_rows_of_other_sizes(top):
+    """fp16: one query whose incoming gradient is 2^23 times the others', or not finite, leaves their dq
+    as precise as it is without it.  A row's dS is held times 2^14 and a power of two from the
+    row's own |dout_i| max |v_j|, so a step of 2^-24 there is as in the test above, row by row."""
+    import sarbon_b200 as sb
+    g = gen(22)
+    b, tq, tk, heads, kv_heads, dim = 1, 150, 4000, 2, 1, 64
+    q, k = rand(g, b, tq, heads * dim, by=2.0 ** -5).half(), rand(g, b, tk, dim, by=2.0 ** 5).half()
+    v, dout = rand(g, b, tk, dim).half(), rand(g, b, tq, heads * dim, by=2.0 ** -8).half()
+    dout[:, 5, 3] = top
+    ref, lse, p, qd, kd, vd = formula(q, k, v, heads, kv_heads, None, None)
+    out, lse = rows_of(ref).half(), lse.flatten(1, 2).float().contiguous()
+    dq = sb.cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=kv_heads)[0]
+    gd, od, u, e, scale = heads_of(dout, heads, kv_heads), heads_of(out, heads, kv_heads), unit(q.dtype), slack_of(qd, kd), dim ** -0.5
+    ds = p * (gd @ vd.transpose(-1, -2) - (gd * ref).sum(-1, keepdim=True))
+    most = gd.norm(dim=-1, keepdim=True) * vd.norm(dim=-1).max()
+    ds_tol = u * ds.abs() + 2.0 ** -25 * 2 * most / 2 ** 14 + \
+        p * ((gd * (od - ref)).abs().sum(-1, keepdim=True) + e * (gd.abs() @ vd.abs().transpose(-1, -2) + (gd * ref).abs().sum(-1, keepdim=True)))
+    want = rows_of(ds @ kd * scale)
+    tol = rows_of(ds_tol @ kd.abs() * scale) + u * want.abs() + 2.0 ** -25
+    rest = torch.arange(tq, device="cuda") != 5
+    err = (dq.double() - want).abs()[:, rest]
+    assert dq[:, rest].isfinite().all()
+    assert (err <= 1.02 * tol[:, rest]).all(), (err / tol[:, rest]).max().item()
+
+
 def test_cross_attention_gradient_against_differences():
     """<gradient, direction> against the central difference of the 64-bit formula, whose own error at
     step 1e-4 is of order 1e-8; the gradients carry roundings of u to each of their many terms."""
