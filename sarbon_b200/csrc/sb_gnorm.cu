@@ -4,7 +4,8 @@
 //
 // Forward, per row v of D values: RMS norm v r w with r = (mean v^2 + eps)^-1/2; layer norm
 // (v - m) r w + b with r = (mean (v - m)^2 + eps)^-1/2 (the mean first, then the centred squares, no
-// cancellation; the backward kernel for aligned rows takes both at once around values of the row).
+// cancellation; the backward kernel for aligned rows takes both at once around values of the row, and
+// again around its mean where those lie far from it).
 // Apart, the norms and the residual sum would read and write the rows five times; here x and z are
 // read and y and h written once, which bounds the kernel.
 //
@@ -471,17 +472,31 @@ SB_DEV void store_pairs(void* p, int dt, long long i, const uint64_t (&v)[4]) {
   for (int u = 0; u < 4; ++u) split2(v[u], f[2 * u], f[2 * u + 1]);
   store8(p, dt, i, f);
 }
+// Whether the squares of one of R rows were summed around a point more than four deviations from its mean
+// (`squares` and `values`: sums over the row's columns; the same in all of a team's threads).
+template <int R>
+SB_DEV bool far_off(const float* squares, const float* values, float inv_d) {
+  bool far = false;
+#pragma unroll
+  for (int x = 0; x < R; ++x) {
+    const float m = values[x] * inv_d;
+    far = far || 17.f * m * m > 16.f * (squares[x] * inv_d);
+  }
+  return far;
+}
 // The mean of four values: of equal ones exactly their value.
 SB_DEV float mean4(float a, float b, float c, float d) { return ((a + b) + (c + d)) * 0.25f; }
 
 // R rows of a team at once, in three reductions that their rows share:
 //   1. z - c and its square,  2. y - c', its square, e and e (y - c') with e = dh w_pre,
 //   3. e and e zhat with e = dn w_post  (RMS norm: the squares and the products alone).
-// Layer norm's c and c' are the mean of the row's first four values.  Such a mean is at most
-// sqrt(D) / 2 deviations away from the row's, so var = E (v - c)^2 - (E v - c)^2 loses at most a
-// factor D / 4 of fp32's precision where one value is all of the variance, and nothing in rows of
-// values alike, however large their mean: no pass for the mean comes first.  (With the means first,
-// it was six reductions a step, whose latency bounded the kernel: 387 us for 65,280 rows of 1024.)
+// Layer norm's c and c' are the mean of the row's first four values, so that no pass for the mean comes
+// first, and var = E (v - c)^2 - (E v - c)^2 loses nothing in rows of values alike, however large
+// their mean.  Where c is more than four deviations off (the first values are the row's outliers), the row's
+// mean takes its place and the sums are taken once more, a fourth reduction for those rows: what
+// cancels is at most 16 var of 17.  Asking costs all rows 3 % (65,280 rows of 1024: 322 -> 331 us; as a loop
+// over both blocks 25 %).  With the means first it was six reductions a step, whose latency bounded
+// the kernel: 387 us.
 // With A = scale gate w_post and B = scale gate b_post (of a row's own gate: without it),
 // y = x + zhat A + B and dn w_post = dyt A.
 // A row in shared memory has room for all of the team's columns, zero past D, and a row past the
@@ -641,6 +656,28 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) gated_norm_back_ker
         if (LAYER) s[R + x] = both(t);
       }
       team_sum<sizeof(s) / 4, kWarps, kStride>(s, sum);
+      if (LAYER && far_off<R>(s, s + R, inv_d)) {
+#pragma unroll
+        for (int x = 0; x < R; ++x) {
+          const float m = s[R + x] * inv_d;
+          zc[x] += m;
+          uint64_t q = 0, t = 0;
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            const uint64_t off = twice(on[j] ? -m : 0.f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              uint64_t& v = zh[x][j][u];
+              v = add2(v, off);
+              t = add2(t, v);
+              q = fma2(v, v, q);
+            }
+          }
+          s[x] = both(q);
+          s[R + x] = both(t);
+        }
+        team_sum<sizeof(s) / 4, kWarps, kStride>(s, sum);
+      }
 #pragma unroll
       for (int x = 0; x < R; ++x) {
         float var = s[x] * inv_d;
@@ -718,6 +755,34 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) gated_norm_back_ker
         }
       }
       team_sum<sizeof(s) / 4, kWarps, kStride>(s, sum);
+      if (LAYER && far_off<R>(s, s + 2 * R, inv_d)) {
+#pragma unroll
+        for (int x = 0; x < R; ++x) {
+          const float m = s[2 * R + x] * inv_d;
+          uint64_t q = 0, p = 0, t = 0, te = 0;
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            const uint64_t off = twice(on[j] ? -m : 0.f);
+            uint64_t W[4];
+            take(kW, j, W);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              uint64_t& y = d[x][j][u];
+              const uint64_t e = mul2(dh[x][j][u], W[u]);
+              y = add2(y, off);
+              t = add2(t, y);
+              te = add2(te, e);
+              q = fma2(y, y, q);
+              p = fma2(e, y, p);
+            }
+          }
+          s[x] = both(q);
+          s[R + x] = both(p);
+          s[2 * R + x] = both(t);
+          s[3 * R + x] = both(te);
+        }
+        team_sum<sizeof(s) / 4, kWarps, kStride>(s, sum);
+      }
 #pragma unroll
       for (int x = 0; x < R; ++x) {
         float var = s[x] * inv_d, shift = 0.f, p = s[R + x];  // p: sum of e yhat

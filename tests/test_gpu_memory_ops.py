@@ -643,6 +643,29 @@ def test_gated_norm_backward_statistics(rows, t, d):
         assert (err <= 16 * FP32 * (1 + worse) * size).all(), (name, (err / (16 * FP32 * (1 + worse) * size)).max().item())
 
 
+@pytest.mark.parametrize("d", [256, 1024, 2048, 4096, 8192])
+@pytest.mark.parametrize("norm", ["post", "pre"])
+def test_gated_norm_backward_deviation_of_outliers(norm, d):
+    """Layer norms whose first four values are nearly all of the variance: 1 / deviation, the factor of a row's
+    gradient, is as precise as a sum of D squares around a point of the row within four deviations of its
+    mean: at most 17 var is summed, by chains of at most 16 + 5 + 8 additions, half of that in the root."""
+    import sarbon_b200 as sb
+    g = gen(d)
+    b, t = 2, 20
+    w, dd = 1 + rand(g, d, by=0.2), rand(g, b, t, d)
+    far, near = rand(g, b, t, d), rand(g, b, t, d)
+    far[..., :4] += 4096
+    if norm == "post":
+        got = sb.gated_norm_backward(dd, None, near, far, post=w, kind="layer", eps=1e-6)["dz"]
+    else:
+        got = sb.gated_norm_backward(None, dd, far, near * 2.0 ** -10, pre=w, kind="layer", eps=1e-6)["dx"]
+    x = (far.double() if norm == "post" else far.double() + near.double() * 2.0 ** -10).requires_grad_(True)
+    torch.nn.functional.layer_norm(x, (d,), w.double(), None, 1e-6).backward(dd.double())
+    rest, want = got[..., 4:].double(), x.grad[..., 4:]
+    off = ((rest * want).sum(-1) / want.square().sum(-1) - 1).abs().max().item()
+    assert off <= 17 / 2 * 29 * 2.0 ** -24, off
+
+
 def test_gated_norm_views_and_offset_rows():
     """Slices, an image's gate as an expanded row, rows whose mean is far from zero."""
     import sarbon_b200 as sb
