@@ -131,6 +131,14 @@ def _apart(results, operands):
             seen.add(t.data_ptr())
 
 
+def _in_place(result, dtype, *operands):
+    """A result's rows may be an operand's rows; other rows may not begin where an operand does.  Rows as
+    _rows returns them, operands as (rows, type)."""
+    for rows, kind in operands:
+        if rows[0] == result[0] and result[0] and (rows != result or kind != dtype):
+            raise ValueError("results need their own memory or an operand's very rows")
+
+
 def _new(like, shape, dtype):
     """A contiguous tensor, (pointer, row stride, item stride); empty_like is the cheapest allocation."""
     t = torch.empty_like(like) if like.dtype == dtype and like.is_contiguous() and like.shape == shape else \
@@ -272,7 +280,8 @@ def rope_axes(x, pos, heads, freq, axis, layout="half", inverse=False, out=None)
     the gradient).  pos: int32 or fp32 [B, T, A], or [T, A] for all items; freq fp64 [R], axis int32 [R]
     (:func:`rope_table`; an axis outside pos's leaves its pair).  Pairs are channels (p, p + R) of a
     head ("half") or (2p, 2p + 1) ("pairs"); channels from 2R on stay as they are.  Angles are formed in
-    fp64, so positions in the millions keep their fraction of a turn.  out may be x itself."""
+    fp64, so positions in the millions keep their fraction of a turn.  out may be x itself (the
+    very rows) and otherwise shares no memory with it."""
     dtype = x.dtype
     if x.dim() != 3 or dtype not in DTYPES:
         raise ValueError("x: [B, T, heads * dim] of fp16, bf16 or fp32")
@@ -295,6 +304,7 @@ def rope_axes(x, pos, heads, freq, axis, layout="half", inverse=False, out=None)
     xp = _rows(x, "x", shape, dtype)
     if out is not None:
         op = _rows(out, "out", shape, dtype, out=True)
+        _in_place(op, dtype, (xp, dtype))
     index = _ready(x, pos, freq, axis, out)
     if out is None:
         out, op = _new(x, shape, dtype)
@@ -348,7 +358,8 @@ def gated_norm(x, z, gate=None, scale=None, post=None, pre=None, kind="rms", eps
     x (the residual) and z (the block's output): [B, T, D] rows; y has x's type and h z's.  post, pre: a
     norm's fp32 [D] weight or (weight, bias), None for no norm there (without pre, h is None).  kind:
     "rms" or "layer".  gate: z's type, [D], [B, D] (one an item) or [B, T, D].  scale: fp32 [D].  h comes
-    from y before its rounding.  y may be x and h may be z.  Returns (y, h)."""
+    from y before its rounding.  y may be x and h may be z (the very rows); otherwise y and h share
+    no memory with an operand or each other.  Returns (y, h)."""
     shape, xp, zp, gp, weights = _norm_inputs(x, z, gate, scale, post, pre, kind, eps)
     hp = (None, 0, 0)
     if y is not None:
@@ -357,6 +368,12 @@ def gated_norm(x, z, gate=None, scale=None, post=None, pre=None, kind="rms", eps
         if pre is None:
             raise ValueError("h needs the norm pre")
         hp = _rows(h, "h", shape, z.dtype, out=True)
+    if y is not None or h is not None:
+        on = (xp, x.dtype), (zp, z.dtype), (gp, z.dtype)
+        if y is not None:
+            _in_place(yp, x.dtype, *on)
+        if h is not None:
+            _in_place(hp, z.dtype, *on, *(((yp, None),) if y is not None else ()))
     index = _ready(x, z, gate, scale, *weights, y, h)
     if y is None:
         y, yp = _new(x, shape, x.dtype)

@@ -90,6 +90,30 @@ def test_gated_norm_refuses():
             sb.gated_norm_backward(**{"dy": None, "dh": None, **good, **change})
 
 
+def test_results_over_other_rows_are_refused():
+    """Row by row a result may take its operand's place, with the operand's rows; with other rows, or on another
+    result, one row's result would fall on another's operands."""
+    base = torch.zeros(2, 6, 128)
+    x, other = base[..., :64], base.view(2, 12, 64)[:, :6]
+    assert x.data_ptr() == other.data_ptr()
+    freq, axis = sb.rope_table((32,), device="cpu")
+    pos = torch.zeros(6, 1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="own memory"):
+        sb.rope_axes(x, pos, 1, freq, axis, out=other)
+    with pytest.raises(ValueError, match="CUDA"):
+        sb.rope_axes(x, pos, 1, freq, axis, out=x)
+    w, z, free = torch.ones(64), torch.zeros(2, 6, 64), torch.zeros(2, 6, 64)
+    for change in (dict(y=other), dict(z=x, h=other), dict(y=free, h=free)):
+        with pytest.raises(ValueError, match="own memory"):
+            sb.gated_norm(**{**dict(x=x, z=z, pre=w), **change})
+    with pytest.raises(ValueError, match="CUDA"):
+        sb.gated_norm(x, z, pre=w, y=x, h=z)
+    # another type's rows begin there: its elements lie elsewhere
+    half = z.view(torch.float16).view(2, 6, 128)[..., :64]
+    with pytest.raises(ValueError, match="own memory"):
+        sb.gated_norm(z, torch.zeros(2, 6, 64, **H16), pre=w, h=half)
+
+
 def test_strides_of_views():
     wide = torch.zeros(2, 5, 192)
     assert mo._rows(wide[..., 64:128], "x", (2, 5, 64), F32)[1:] == (192, 960)
