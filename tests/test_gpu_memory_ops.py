@@ -689,6 +689,72 @@ def test_gated_norm_views_and_offset_rows():
     assert got["dx"].shape == (b, 0, d) and not got["post_w"].any() and not got["scale"].any()
 
 
+@pytest.mark.parametrize("gate", ["image", "row"])
+@pytest.mark.parametrize("d,odd", [(64, 0), (255, 0), (520, 0), (520, 1), (1152, 0), (4096, 0)])
+def test_gated_norm_many_rows(d, odd, gate):
+    """Many rows a team, of several items: every stage of a ring is used again, gates change on the way, and in place
+    the next rows are on their way while one is written.  odd: rows that begin off 16 bytes."""
+    import sarbon_b200 as sb
+    g = gen(d + odd)
+    b, t = (3, 9001) if d < 4096 else (5, 1803)
+    s = norm_case(g, b, t, d, torch.float32, torch.bfloat16, "layer", gate, True, True, True)
+    if odd:
+        s["x"] = rand(g, b, t, d + 1, by=2.0)[..., 1:]
+    y, h = sb.gated_norm(**s)
+    again = dict(s, x=s["x"].clone(), z=s["z"].clone()) if not odd else \
+        dict(s, x=torch.cat([s["x"][..., :1], s["x"]], -1)[..., 1:], z=s["z"].clone())
+    y2, h2 = sb.gated_norm(**again, y=again["x"], h=again["z"])
+    assert torch.equal(y2, y) and torch.equal(h2, h)
+    for i in range(b):  # an item at a time
+        one = wide(dict(s, x=s["x"][i:i + 1], z=s["z"][i:i + 1], gate=s["gate"][i:i + 1]))
+        ry, rh = norm_formula(**one)
+        size = one["x"].abs() + (ry - one["x"]).abs() * 2 + 1
+        assert ((y[i:i + 1].double() - ry).abs() <= unit(y.dtype) * ry.abs() + FP32 * size + 2.0 ** -25).all()
+        spread = (ry.abs().mean(-1, keepdim=True) + size) * ry.var(-1, keepdim=True, unbiased=False).add(s["eps"]).rsqrt()
+        tol = unit(h.dtype) * rh.abs() + 2 * FP32 * (spread * one["pre"][0].abs() + 1) + 2.0 ** -25
+        assert ((h[i:i + 1].double() - rh).abs() <= tol).all()
+
+
+def grads_of(s, dy, dh):
+    """The gradients in fp64, by differentiation."""
+    w = wide(s, grad=True)
+    y, h = norm_formula(**w)
+    ((y * dy.double()).sum() + (h * dh.double()).sum()).backward()
+    want = dict(dx=w["x"].grad, dz=w["z"].grad, gate=w["gate"].grad, scale=w["scale"].grad)
+    for name in ("post", "pre"):
+        want[name + "_w"], want[name + "_b"] = (None if v is None else v.grad for v in w[name])
+    return want
+
+
+@pytest.mark.parametrize("b,t,d,kind,gate,odd", [
+    (3, 9001, 64, "layer", "image", 0), (3, 9001, 520, "rms", "row", 0), (3, 5001, 1152, "layer", "row", 0),
+    (3, 5001, 520, "layer", "image", 1), (5, 803, 4096, "rms", "image", 0), (700, 3, 256, "layer", "image", 0),
+    (300, 1, 96, "rms", "image", 0),
+    (2, 70, 96, "layer", "expanded", 0), (2, 3001, 768, "layer", "expanded", 0), (2, 3001, 100, "rms", "expanded", 0),
+])
+def test_gated_norm_backward_many_rows(b, t, d, kind, gate, odd):
+    """Rings used many times, teams whose rows are of several items, many items with a gate each, and a gate of each
+    item given as rows (stride 0), whose gradient has a value a row."""
+    import sarbon_b200 as sb
+    g = gen(b + t + d)
+    s = norm_case(g, b, t, d, torch.float32, torch.bfloat16, kind, "image" if gate == "expanded" else gate, True, True, True)
+    if gate == "expanded":
+        s["gate"] = s["gate"][:, None].expand(b, t, d)
+    if odd:
+        s["x"] = rand(g, b, t, d + 1, by=2.0)[..., 1:]
+    dy, dh = rand(g, b, t, d), rand(g, b, t, d, dtype=torch.bfloat16)
+    got, want = sb.gated_norm_backward(dy, dh, **s), grads_of(s, dy, dh)
+    for name, r in want.items():
+        if r is None:
+            assert got[name] is None
+            continue
+        assert got[name].shape == r.shape
+        x = got[name].double()
+        size = r.abs() + r.square().mean().sqrt() + (1 if name in ("dx", "dz") or r.dim() == 3 else math.sqrt(b * t))
+        tol = unit(got[name].dtype) * r.abs() + 16 * FP32 * size + 2.0 ** -25
+        assert ((x - r).abs() <= tol).all(), (name, ((x - r).abs() / tol).max().item())
+
+
 # ---------------------------------------------------------------- together
 def block(sb, g, heads, kv_heads, dim):
     """One block that reads a memory: positions, attention, gated residual and norms."""
