@@ -511,6 +511,23 @@ def test_rope_views():
     assert sb.rope_axes(x[:0], pos, 2, freq, axis).shape == (0, 105, 128)
 
 
+@pytest.mark.parametrize("dtype", TYPES + [torch.float32])
+@pytest.mark.parametrize("layout", ["half", "pairs"])
+@pytest.mark.parametrize("b,t,heads,dim,sections", [(2, 20000, 3, 64, (16, 16)), (1, 30001, 8, 128, (16, 24, 8)),
+                                                    (3, 16000, 5, 80, (4, 4, 8)), (1, 90000, 2, 20, (3, 4))])
+def test_rope_many_tokens(b, t, heads, dim, sections, layout, dtype):
+    """Enough tokens that a thread turns all of a token's heads, an odd number of them among them; also in place."""
+    import sarbon_b200 as sb
+    g = gen(t + heads)
+    freq, axis = sb.rope_table(sections)
+    pos = torch.randint(-50, 5_000_000, (b, t, len(sections)), device="cuda", generator=g, dtype=torch.int32)
+    x = rand(g, b, t, heads * dim, dtype=dtype)
+    out = sb.rope_axes(x, pos, heads, freq, axis, layout=layout)
+    check_rope(out, x, pos, heads, freq, axis, layout, False)
+    assert sb.rope_axes(x, pos, heads, freq, axis, layout=layout, out=x) is x
+    assert torch.equal(x, out)
+
+
 # ---------------------------------------------------------------- gated residual and norms
 def norm_formula(x, z, gate, scale, post, pre, kind, eps):
     def norm(v, w):
