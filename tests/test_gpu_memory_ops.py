@@ -419,6 +419,34 @@ def test_cross_attention_backward_rows_of_other_sizes(top):
     assert (err <= 1.02 * tol[:, rest]).all(), (err / tol[:, rest]).max().item()
 
 
+@pytest.mark.parametrize("kind", ["lens", "valid", "both", "queries"])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_cross_attention_backward_long_ragged(dim, kind):
+    """So many items that no range of steps is split: each CTA streams many tiles of keys (dq) or, with many
+    queries, of queries (dk, dv), and every stage of its ring is used many times."""
+    import sarbon_b200 as sb
+    g = gen(78 + dim)
+    b, tq, tk, heads, kv_heads = (160, 300, 3000, 2, 1) if kind != "queries" else (160, 1500, 200, 2, 1)
+    q, dout = (rand(g, b, tq, heads * dim, dtype=torch.bfloat16) for _ in range(2))
+    kv = rand(g, b, tk, 2 * dim, dtype=torch.bfloat16)
+    lens = valid = None
+    if kind != "valid":
+        lens = torch.randint(0, tk + 1, (b,), device="cuda", generator=g, dtype=torch.int32)
+    if kind != "lens":
+        valid = torch.rand(b, tk, device="cuda", generator=g) < 0.8
+    kv[~keep_of(b, tk, lens, valid)] = math.nan
+    k, v = kv[..., :dim], kv[..., dim:]
+    lse = torch.empty(b, heads, tq, device="cuda")
+    out = sb.cross_attention(q, k, v, heads, kv_heads=kv_heads, lens=lens, valid=valid, lse=lse)
+    grads = sb.cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=kv_heads, lens=lens, valid=valid)
+    for i in range(0, b, 20):  # twenty items at a time
+        at = slice(i, i + 20)
+        check_backward([x[at] for x in grads], dout[at], q[at], k[at], v[at], heads, kv_heads, None if lens is None else lens[at],
+                       None if valid is None else valid[at], out[at])
+    again = sb.cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=kv_heads, lens=lens, valid=valid)
+    assert all(torch.equal(x, y) for x, y in zip(grads, again))
+
+
 def test_cross_attention_gradient_against_differences():
     """<gradient, direction> against the central difference of the 64-bit formula, whose own error at
     step 1e-4 is of order 1e-8; the gradients carry roundings of u to each of their many terms."""
