@@ -14,7 +14,7 @@
 // 3 x 8161 of 12 x 64 in fp32: 35 us, 66 % (one wave of CTAs, so starting and ending show).
 #include <algorithm>
 
-#include "sb_rows.cuh"
+#include "sb_xattn.cuh"
 
 namespace sb {
 namespace {
@@ -184,8 +184,10 @@ extern "C" int sb_rope_axes(const void* x, long long x_row, long long x_img, int
   if (blocks > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_rope_axes: too many rows");
   // split the heads until every SM has its four blocks; more of them pay the trigonometry again (eight an SM:
   // 41 against 38 us for 3 x 8161 tokens of 12 x 64 in fp16, as long for fp32)
+  const int sms = xattn_sms();
+  if (sms == 0) return record_error(SB_ECUDA, "sb_rope_axes: device");
   int parts = 1;
-  while (parts < H && parts < 32 && blocks * parts < 592) ++parts;
+  while (parts < H && parts < 32 && blocks * parts < 4ll * sms) ++parts;
   a.heads_per = (H + parts - 1) / parts;
   const dim3 grid((unsigned)blocks, (unsigned)((H + a.heads_per - 1) / a.heads_per));
   auto kernel = !vec               ? rope_kernel<false, 0>
