@@ -54,7 +54,7 @@ struct NormArgs {
   float eps;
   int T, D, tpr, per;  // threads a row, rows a CTA takes at once (several: a warp each)
   long long rows;      // B * T
-  long long step_b;    // a team's step from row to row as (items, rows): no division in the loop
+  long long step_b;    // forward, any alignment: from row to row as (items, rows), no division in the loop
   int step_t;
   void *y, *h;         // forward
   long long y_row, y_img, h_row, h_img;
@@ -1463,8 +1463,6 @@ extern "C" int sb_gated_norm_backward(const void* dy, long long dy_row, long lon
                    cols_aligned(pre_b);
   const int smem = ring_of(a, p, true, vec);
   const NormKernel kernel = pick(true, x_dtype, z_dtype, vec, p.kind, layer != 0);
-  a.step_b = p.per / T;
-  a.step_t = p.per % T;
   if ((long long)groups * a.chunks > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_gated_norm_backward: too many items");
   cudaError_t e = launch_norm(kernel, (unsigned)(groups * a.chunks), p.threads, smem, a, (cudaStream_t)stream);
   if (e == cudaSuccess && sums) {

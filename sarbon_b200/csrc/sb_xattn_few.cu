@@ -366,7 +366,8 @@ cudaError_t join(const FwdArgs& a, cudaStream_t st) {
 
 int few_keys(int dh) { return 2048 / dh; }
 
-// About three CTAs a place (two an SM), so that ragged lengths even out, and at least 256 keys each.
+// About three CTAs a place (two an SM), so that ragged lengths even out, but a split for each 256 keys begun
+// at most.
 int few_splits(long long units, int Tk, int sms) {
   const long long want = (3ll * 2 * sms + units - 1) / units;
   return (int)std::max(1ll, std::min({want, ((long long)Tk + 255) / 256, 128ll}));
