@@ -800,6 +800,63 @@ def test_gated_norm_backward_many_rows(b, t, d, kind, gate, odd):
         assert ((x - r).abs() <= tol).all(), (name, ((x - r).abs() / tol).max().item())
 
 
+def far_apart(x):
+    """x's values as the items of one buffer whose second item begins past 2^31 elements."""
+    b, t, c = x.shape
+    step = (2 ** 31 // max(1, b - 1) // c + 1) * c
+    hold = torch.empty(step * (b - 1) + t * c, device="cuda", dtype=x.dtype)
+    y = hold.as_strided((b, t, c), (step, c, 1))
+    y.copy_(x)
+    return y
+
+
+@pytest.mark.parametrize("tq", [3, 140])
+def test_items_past_32_bits(tq):
+    """Items that lie more than 2^31 elements apart, in and out, give the bits of those that lie together."""
+    import sarbon_b200 as sb
+    g = gen(50)
+    b, tk, heads, dim = 2, 300, 2, 64
+    q, dout = (rand(g, b, tq, heads * dim, dtype=torch.float16) for _ in range(2))
+    k, v = (rand(g, b, tk, heads * dim, dtype=torch.float16) for _ in range(2))
+    valid = torch.rand(b, tk, device="cuda", generator=g) < 0.7
+    lse, lse2 = torch.empty(b, heads, tq, device="cuda"), torch.empty(b, heads, tq, device="cuda")
+    out = sb.cross_attention(q, k, v, heads, valid=valid, lse=lse)
+    grads = sb.cross_attention_backward(dout, q, k, v, out, lse, heads, valid=valid)
+    kf, of, vf = far_apart(k), far_apart(torch.zeros_like(out)), far_apart(valid[..., None])[..., 0]
+    sb.cross_attention(q, kf, v, heads, valid=vf, lse=lse2, out=of)
+    assert torch.equal(of, out) and torch.equal(lse2, lse)
+    df = far_apart(torch.zeros_like(k))
+    again = sb.cross_attention_backward(far_apart(dout), q, kf, v, of, lse, heads, valid=vf, dk=df)
+    assert all(torch.equal(x, y) for x, y in zip(grads, again))
+    freq, axis = sb.rope_table((16, 16))
+    pos = torch.randint(0, 99, (b, tk, 2), device="cuda", generator=g, dtype=torch.int32)
+    assert torch.equal(sb.rope_axes(kf, pos, heads, freq, axis, out=df), sb.rope_axes(k, pos, heads, freq, axis))
+    for d in (128, 127):
+        s = norm_case(g, b, tk, d, torch.float16, torch.float16, "layer", "row", True, True, True)
+        far = dict(s, x=far_apart(s["x"]), gate=far_apart(s["gate"]))
+        y, h = sb.gated_norm(**s)
+        y2, h2 = sb.gated_norm(**far, y=far_apart(torch.zeros_like(y)))
+        assert torch.equal(y2, y) and torch.equal(h2, h)
+        want, got = sb.gated_norm_backward(y, h, **s), sb.gated_norm_backward(far_apart(y), h, **far)
+        assert all(x is None or torch.equal(x, got[n]) for n, x in want.items())
+
+
+def test_shared_queries():
+    """Queries, and what comes back to them, that are one item's for all (a batch stride of 0)."""
+    import sarbon_b200 as sb
+    g = gen(51)
+    b, tq, tk, heads, kv_heads, dim = 3, 150, 200, 4, 2, 64
+    q, dout = (rand(g, 1, tq, heads * dim, dtype=torch.bfloat16).expand(b, -1, -1) for _ in range(2))
+    k, v = (rand(g, b, tk, kv_heads * dim, dtype=torch.bfloat16) for _ in range(2))
+    lse = torch.empty(b, heads, tq, device="cuda")
+    out = sb.cross_attention(q, k, v, heads, kv_heads=kv_heads, lse=lse)
+    check_forward(out, lse, q, k, v, heads, kv_heads, None, None)
+    few = sb.cross_attention(q[:, :3], k, v, heads, kv_heads=kv_heads)
+    check_forward(few, None, q[:, :3], k, v, heads, kv_heads, None, None)
+    grads = sb.cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=kv_heads)
+    check_backward(grads, dout, q, k, v, heads, kv_heads, None, None, out)
+
+
 # ---------------------------------------------------------------- together
 def block(sb, g, heads, kv_heads, dim):
     """One block that reads a memory: positions, attention, gated residual and norms."""
