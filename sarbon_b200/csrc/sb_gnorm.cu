@@ -27,8 +27,8 @@
 // Element types are compile-time for the usual pairs.  Rows that are not 16-byte aligned or not a
 // multiple of eight columns take plain loads, one row ahead (the kernels named `_any`).
 //
-// Forward, 65,280 rows of 2048 bf16 columns, RMS: 199 us, 82 % of the copy rate.  Backward, 65,280 rows of
-// 1024, x fp32, z bf16, layer norms: 322 us, 57 %: 1100 instructions a warp and step of two rows, three
+// Forward, 65,280 rows of 2048 bf16 columns, RMS: 196 us, 83 % of the copy rate.  Backward, 65,280 rows of
+// 1024, x fp32, z bf16, layer norms: 331 us, 56 %: 1100 instructions a warp and step of two rows, three
 // dependent reductions, and registers for twelve warps an SM (a warp issues every 7 clocks; four CTAs an SM
 // spill, 503 us of a run whose three took 384; a third stage of rows ahead took 426).
 #include <algorithm>
@@ -1302,16 +1302,15 @@ NormKernel pick(bool back, int xdt, int zdt, bool vec, int kind, bool layer) {
   return ring_kernel<-1, -1>(back, kind, layer);
 }
 
-// CTAs an SM: as many as have 512 threads (backward, with its registers: 384), four (three) at least.  With
-// four CTAs whatever their size 65,280 rows of 1024 bf16 columns took 178 us instead of 121; with 640
-// threads, whose registers then spill, fp32 rows of 2048 take 306 us instead of 278.
+// CTAs an SM: as many as have 512 threads (backward, with its registers: 384), four (three) at least.  65,280
+// rows of bf16, RMS: with four CTAs whatever their size 1024 columns take 154 us instead of 97; with 640
+// threads, whose registers then spill, 137, and 2048 columns 277 instead of 193.
 int ctas_of(const Plan& p, bool back) { return back ? std::max(3, 384 / p.threads) : std::max(4, 512 / p.threads); }
 
 // The ring of each team (as many rows as its part of an SM's bytes holds, two to eight) and a CTA's shared
-// memory, which the backward kernels' last sums share.  More rows ahead than these do not help CTA teams: 184 KB
-// of forward rings take as long, or longer (fp32 rows of 2048: 326 us instead of 278); warps, with more
-// rows of an SM's at once, gain (fp32 rows of 256: 61 instead of 66 us).
-int ring_bytes(const Plan& p, bool back) { return (back ? 138 : p.per > 1 ? 184 : 96) * 1024; }
+// memory, which the backward kernels' last sums share.  More rows ahead than these do not help: with 184 KB of
+// forward rings 65,280 rows of 256 to 2048 columns take as long, or up to 5 % longer.
+int ring_bytes(bool back) { return (back ? 138 : 96) * 1024; }
 int ring_of(NormArgs& a, const Plan& p, bool back, bool& vec) {
   const int xs = dtype_bytes(a.xdt), zs = dtype_bytes(a.zdt);
   a.pitch = back ? p.tpr * 8 * (p.at_once == 2 || p.kind == 0 ? 1 : 2) : a.D;
@@ -1319,7 +1318,7 @@ int ring_of(NormArgs& a, const Plan& p, bool back, bool& vec) {
   a.copy_bytes = a.D * elem;
   a.row_bytes = a.pitch * elem;
   a.stage_bytes = a.row_bytes * p.at_once;
-  a.stages = std::max(2, std::min(kMaxStages, ring_bytes(p, back) / ctas_of(p, back) / (p.per * a.stage_bytes)));
+  a.stages = std::max(2, std::min(kMaxStages, ring_bytes(back) / ctas_of(p, back) / (p.per * a.stage_bytes)));
   vec = vec && 2 * p.per * a.stage_bytes <= 200 * 1024;  // else the widest fp32 rows: no room for two
   const int ring = vec ? p.per * a.stages * a.stage_bytes : 0;
   const int fold = back && p.per > 1 ? p.per * kSums * p.tpr * 8 * 4 : 0;
