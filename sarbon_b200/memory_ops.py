@@ -49,7 +49,7 @@ _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_devic
 def _ready(*tensors):
     """All tensors on one CUDA device and none that autograd would have to follow; its index."""
     # a dual tensor does not require a gradient; looked for only inside a forward_ad.dual_level
-    if getattr(forward_ad, "_current_level", 0) >= 0:
+    if forward_ad._current_level >= 0:
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t, level=0).tangent is not None:
                 raise ValueError("no forward-mode tangent is followed: call on primals")
@@ -115,10 +115,17 @@ def _rows(t, what, shape, dtype, out=False):
 
 
 def _own_rows(t):
-    """t, or a copy where its rows are one and the same (a row stride of 0, which no tensor map has)."""
-    if t.dim() != 3 or t.stride(1) != 0 or t.shape[1] <= 1:
-        return t
+    """A copy of t, whose rows are one and the same (a row stride of 0, which no tensor map has)."""
     return t[:1].contiguous().expand(t.shape) if t.stride(0) == 0 else t.contiguous()
+
+
+def _mapped(t, what, shape, dtype):
+    """_rows of an operand that a tensor map describes, and what they lie in (t or a copy)."""
+    rows = _rows(t, what, shape, dtype)
+    if rows[1] == 0:
+        t = _own_rows(t)
+        rows = _rows(t, what, shape, dtype)
+    return rows, t
 
 
 def _apart(results, operands):
@@ -203,8 +210,7 @@ def cross_attention(q, k, v, heads, kv_heads=None, lens=None, valid=None, scale=
     queries on many states (single tokens) are split over the states."""
     kv_heads, b, tq, tk, dim, scale = _attention_sizes(q, k, heads, kv_heads, scale)
     dtype, qs, ks = q.dtype, (b, tq, heads * dim), (b, tk, kv_heads * dim)
-    k, v = _own_rows(k), _own_rows(v)
-    qp, kp, vp = _rows(q, "q", qs, dtype), _rows(k, "k", ks, dtype), _rows(v, "v", ks, dtype)
+    qp, (kp, k), (vp, v) = _rows(q, "q", qs, dtype), _mapped(k, "k", ks, dtype), _mapped(v, "v", ks, dtype)
     masks = _masks(lens, valid, b, tk)
     if lse is not None:
         _statistics(lse, b, heads, tq)
@@ -232,9 +238,9 @@ def cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=None, lens
     dv (allocated if None) must not share memory with an operand or each other."""
     kv_heads, b, tq, tk, dim, scale = _attention_sizes(q, k, heads, kv_heads, scale)
     dtype, qs, ks = q.dtype, (b, tq, heads * dim), (b, tk, kv_heads * dim)
-    dout, q, k, v = _own_rows(dout), _own_rows(q), _own_rows(k), _own_rows(v)
-    views = _rows(dout, "dout", qs, dtype) + _rows(q, "q", qs, dtype) + _rows(k, "k", ks, dtype) + \
-        _rows(v, "v", ks, dtype) + _rows(out, "out", qs, dtype)
+    (dp, dout), (qp, q), (kp, k), (vp, v) = _mapped(dout, "dout", qs, dtype), _mapped(q, "q", qs, dtype), \
+        _mapped(k, "k", ks, dtype), _mapped(v, "v", ks, dtype)
+    views = dp + qp + kp + vp + _rows(out, "out", qs, dtype)
     masks = _masks(lens, valid, b, tk)
     _statistics(lse, b, heads, tq)
     for what, t, shape in (("dq", dq, qs), ("dk", dk, ks), ("dv", dv, ks)):
