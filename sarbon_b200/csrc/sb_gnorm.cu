@@ -27,7 +27,7 @@
 // Element types are compile-time for the usual pairs.  Rows that are not 16-byte aligned or not a
 // multiple of eight columns take plain loads, one row ahead (the kernels named `_any`).
 //
-// Forward, 65,280 rows of 2048 bf16 columns, RMS: 196 us, 83 % of the copy rate.  Backward, 65,280 rows of
+// Forward, 65,280 rows of 2048 bf16 columns, RMS: 198 us, 83 % of the copy rate.  Backward, 65,280 rows of
 // 1024, x fp32, z bf16, layer norms: 331 us, 56 %: 1100 instructions a warp and step of two rows, three
 // dependent reductions, and registers for twelve warps an SM (a warp issues every 7 clocks; four CTAs an SM
 // spill, 503 us of a run whose three took 384; a third stage of rows ahead took 426).

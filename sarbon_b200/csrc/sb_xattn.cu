@@ -30,9 +30,9 @@
 // What bounds it is the chain of a tile: P stored, its product, the wait for it, the next P.  A wait costs
 // 100 to 400 clocks whatever its form (polls, suspended or with sleeps, measured alike), a tile of a stream
 // 2400 with the arithmetic and all but one of its products left out, 4400 with them; two streams overlap,
-// and TMEM has no room for a third or for two P.  2 x 16 heads of 128 channels (4 key heads), 4096
-// queries, 8160 keys: 550 us, 995 TFLOP/s, where the products alone would take 336 and the exponentials
-// (16 a clock and SM) 238.  16 x 8 heads of 32 channels, 300 queries, 28,900 of 42,840 keys: 863 us, of them
+// and with P beside the scores TMEM has no room for a third or for two P.  2 x 16 heads of 128 channels (4 key heads), 4096
+// queries, 8160 keys: 545 us, 1005 TFLOP/s, where the products alone would take 336 and the exponentials
+// (16 a clock and SM) 238.  16 x 8 heads of 32 channels, 300 queries, 28,900 of 42,840 keys: 842 us, of them
 // 215 for the 44 rows behind the second tile, which load two of an SM's four schedulers.  A polynomial for
 // part of the exponentials was slower: the issue slots are as scarce.
 // The key range is split over CTAs where the rows alone leave SMs idle: these write fp32 partial rows
@@ -435,8 +435,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t ms2 = pair2(ms, ms);
       uint64_t sum[2] = {0, 0};
       // All exponentials before the last product is waited for, or the second half after the first has
-      // gone to TMEM: 2 x 16 heads, 4096 queries, 8160 keys: 503 against 523 us with 64 channels, 515 against
-      // 525 with 128, but 496 against 489 with 32, whose products are short.
+      // gone to TMEM: 2 x 16 heads, 4096 queries, 8160 keys: 440 against 473 us with 64 channels, 493 against
+      // 503 with 128; with 32, whose products are short, 447 against 433 in bf16 (420 against 438 in fp16).
       constexpr bool kAll = DH >= 64;
       uint32_t pk[16], pl[16];
       probabilities<BF16>(s, sl2, ms2, sum, pk);

@@ -28,9 +28,9 @@
 // A range of steps may be split over CTAs (few rows against many): these write fp32 partial
 // results, which a last kernel adds in order.
 //
-// 2 x 16 heads of 128 channels (4 key heads), 2040 queries, 8160 keys: 1140 us, 599 TFLOP/s of the five
-// products' operations, 840 of the seven that are done; what is left is waits, as in the forward kernel.
-// 8 x 8 heads of 64 channels, 300 queries, up to 2040 keys: 135 us, of them 12 for the first kernel, 42 for
+// 2 x 16 heads of 128 channels (4 key heads), 2040 queries, 8160 keys: 1126 us, 606 TFLOP/s of the five
+// products' operations, 848 of the seven that are done; what is left is waits, as in the forward kernel.
+// 8 x 8 heads of 64 channels, 300 queries, up to 2040 keys: 136 us, of them 12 for the first kernel, 42 for
 // dq and 84 for dk and dv, whose CTAs have three steps each: starting and ending take most of theirs.
 #include <algorithm>
 #include <cmath>
