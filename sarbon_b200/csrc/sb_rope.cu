@@ -5,7 +5,8 @@
 // and by the opposite angle for the gradient (the rotation's transpose).  A camera's frame
 // numbers reach millions, where an fp32 product is off by a tenth of a radian, so the angle is
 // taken in fp64 as turns (pos * freq / 2 pi), its whole turns are dropped there, and only the
-// remainder in [-1/2, 1/2] goes to fp32 and to sincospi.
+// remainder in [-1/2, 1/2] goes to fp32 and to sincospi; what that rounds off, up to 1.6 2^-24 of an
+// angle, is added to first order.
 //
 // A thread owns eight pairs of one token: it computes their sines and cosines once and applies
 // them to every head of its chunk, so that the trigonometry is paid once a token and the pass is
@@ -42,8 +43,12 @@ SB_DEV void turn_of(const RopeArgs& a, long long at, int p, float& sn, float& cs
   const double where = a.pos_f32 ? (double)static_cast<const float*>(a.pos)[at + ax]
                                  : (double)static_cast<const int*>(a.pos)[at + ax];
   double turns = where * a.freq[p] * 0.15915494309189533576888;  // 1 / (2 pi)
-  turns -= rint(turns);
-  sincospif((float)(2.0 * turns), &sn, &cs);
+  turns = 2.0 * (turns - rint(turns));
+  const float near = (float)turns, rest = 3.14159265f * (float)(turns - (double)near);
+  sincospif(near, &sn, &cs);
+  const float s0 = sn;
+  sn = fmaf(cs, rest, sn);
+  cs = fmaf(-s0, rest, cs);
   if (a.inverse) sn = -sn;
 }
 

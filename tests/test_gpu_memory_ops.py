@@ -556,6 +556,23 @@ def test_rope_many_tokens(b, t, heads, dim, sections, layout, dtype):
     assert torch.equal(x, out)
 
 
+@pytest.mark.parametrize("dim", [2, 32])
+def test_rope_angles(dim):
+    """Sines and cosines themselves (pairs 0, 1), in fp32: one unit in the last place of the function (2^-24 below 1), half of
+    one for the correction of the angle's rounding, and 2^-53 of 8e5 turns, three roundings of them."""
+    import sarbon_b200 as sb
+    t, n = 200_000, dim // 2
+    x = torch.zeros(1, t, dim, device="cuda")
+    x[..., n:] = 1
+    freq = 1.0 / (1 + torch.arange(n, device="cuda", dtype=torch.float64))
+    axis = torch.zeros(n, device="cuda", dtype=torch.int32)
+    pos = torch.randint(-5_000_000, 5_000_000, (t, 1), device="cuda", generator=gen(4), dtype=torch.int32)
+    out = sb.rope_axes(x, pos, 1, freq, axis)[0].double()
+    angle = pos.double() * freq
+    want = torch.cat([-angle.sin(), angle.cos()], -1)
+    assert (out - want).abs().max().item() <= 1.5 * 2.0 ** -24 + 3 * 2.0 ** -53 * 5e6
+
+
 # ---------------------------------------------------------------- gated residual and norms
 def norm_formula(x, z, gate, scale, post, pre, kind, eps):
     def norm(v, w):
