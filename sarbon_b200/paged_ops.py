@@ -1,0 +1,285 @@
+"""A memory that a camera stream keeps between frames: its states in pages, read, extended and cut back.
+
+Where :func:`sarbon_b200.cross_attention` is given an encoder's whole memory with each call, a tracker
+that runs for days keeps one: every frame adds its tokens, a few query tokens attend to all that is
+there, and once there is more than the budget allows, the states that were looked at least go::
+
+    n = paged_write(k, v, k_pages, v_pages, table, lens, weight=weight, born=born, stamp=frame)
+    o = paged_attention(q, k_pages, v_pages, table, n, heads, kv_heads=kv_heads, weight=weight, decay=0.98)
+    paged_evict(k_pages, v_pages, table, n, weight, budget, born=born, since=oldest, weight_out=weight,
+                born_out=born, after=lens)
+
+``k_pages`` and ``v_pages`` are pools ``[P, page, kv_heads * dim]`` of fp16, bf16 or e4m3 (heads of 32, 64
+or 128 channels; any page size; pages and rows any multiple of 16 bytes apart, so keys and values may
+lie side by side).  ``table`` (int32 [B, N]) names the pages of an item's states: state j is row
+``j % page`` of page ``table[b, j // page]``.  A number outside [0, P) is no page: its states are neither
+written nor read and take no part.  Pages may be shared by items that only read them.  Lengths (int32 [B])
+outside [0, N * page] are clamped.
+
+``weight`` (fp32) and ``born`` (int32), ``[B, kv_heads, N * page]``, hold for each state and key head how much it was
+looked at and its stamp (a frame number, say).  Eviction decides for each key head by itself, so a row's heads may
+stem from different states afterwards; attention does not mind the order of states, and their positions are in
+the keys (:func:`sarbon_b200.rope_axes` before they are written).
+
+Every call launches kernels of ``libsarbon_sparse.so`` on the current CUDA stream of its tensors' device,
+takes its workspace from torch's allocator and can be captured in a CUDA graph after a first call outside
+capture.  No graph of gradients is recorded; tensors that would need one are refused.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .memory_ops import _HALVES, _INF, _apart, _launch, _new, _ready, _rows, _statistics, _work
+
+E4M3 = torch.float8_e4m3fn
+PAGE_DTYPES = {torch.float16: _lib.SB_F16, torch.bfloat16: _lib.SB_BF16, E4M3: _lib.SB_F8}
+
+
+def _pool(t, what, shape, dtype):
+    """(pointer, row stride, page stride) in elements of a pool [P, page, C]."""
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{what}: expected {tuple(shape)} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+    pages, page, width = shape
+    img, row, one = t.stride()
+    if one != 1 and width > 1:
+        raise ValueError(f"{what}: channels must be contiguous")
+    if page <= 1:
+        row = width
+    if pages <= 1:
+        img = page * row
+    return t.data_ptr(), row, img
+
+
+def _own_pool(pool, what, shape):
+    """A pool that is written: no row lies on another."""
+    _, row, img = pool
+    pages, page, width = shape
+    if (page > 1 and row < width) or (pages > 1 and img < row * (page - 1) + width and not
+                                      (img >= width and (page == 1 or row >= img * (pages - 1) + width))):
+        raise ValueError(f"{what}: rows overlap")
+
+
+def _memory(k_pages, v_pages, table, kv_heads, written=False):
+    """The arguments that every call has: (pools and table for the library, batch, page, entries, dim)."""
+    if k_pages.dim() != 3 or k_pages.dtype not in PAGE_DTYPES:
+        raise ValueError("k_pages, v_pages: [P, page, kv_heads * dim] pools of fp16, bf16 or e4m3")
+    shape, dtype = k_pages.shape, k_pages.dtype
+    pages, page, width = shape
+    if kv_heads < 1 or page < 1 or width % kv_heads or width // kv_heads not in (32, 64, 128):
+        raise ValueError("pools: pages of one state or more, key heads of 32, 64 or 128 channels")
+    kp, vp = _pool(k_pages, "k_pages", shape, dtype), _pool(v_pages, "v_pages", shape, dtype)
+    if written:
+        _own_pool(kp, "k_pages", shape)
+        _own_pool(vp, "v_pages", shape)
+        _apart((v_pages,), (k_pages,))
+    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table: int32 [B, N] with contiguous rows")
+    b, n = table.shape
+    if n * page >= 1 << 30:
+        raise ValueError("table: fewer than 2^30 states an item")
+    return (*kp, *vp, PAGE_DTYPES[dtype], pages, page, table.data_ptr(), table.stride(0) if b > 1 else n, n), b, page, n, \
+        width // kv_heads
+
+
+def _each(t, what, b):
+    """Pointer of an int32 [B]."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.shape != (b,) or (b > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what}: contiguous int32 [B]")
+    return t.data_ptr()
+
+
+def _account(t, what, shape, dtype):
+    """Pointer of weights or stamps."""
+    if t is None:
+        return None
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous {dtype} {tuple(shape)}")
+    return t.data_ptr()
+
+
+def _scales(k_scale, v_scale, dtype):
+    if not (0.0 < k_scale < _INF and 0.0 < v_scale < _INF):
+        raise ValueError("k_scale, v_scale: positive numbers")
+    if dtype != E4M3 and (k_scale != 1.0 or v_scale != 1.0):
+        raise ValueError("k_scale, v_scale: of e4m3 pages only")
+
+
+def _clear_of(results, operands):
+    """Contiguous results that share no memory with an operand or another result."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in operands if t is not None and t.numel()]
+    for t in results:
+        if t is not None and t.numel():
+            lo, hi = t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+            if any(lo < y and x < hi for x, y in spans):
+                raise ValueError("results need their own memory")
+            spans.append((lo, hi))
+
+
+# ---------------------------------------------------------------- attention
+def paged_attention(q, k_pages, v_pages, table, lens, heads, kv_heads=None, scale=None, causal=False, k_scale=1.0,
+                    v_scale=1.0, weight=None, decay=1.0, out=None, lse=None):
+    """softmax(scale q k^T) v per head of a few query tokens [B, Tq, heads * dim] (fp16 or bf16) over the
+    ``lens[b]`` states of each item's pages.
+
+    Query head h reads key head ``h // (heads // kv_heads)``.  causal: the queries are the last Tq of the
+    states, and query t sees those up to itself, the first ``lens[b] - Tq + 1 + t``.  A query without
+    states gets zeros.  Pages have q's type, or e4m3: a code c of a key then stands for ``c * k_scale``, of a value for
+    ``c * v_scale``.  scale: 1 / sqrt(dim) unless given.  Fills out (allocated if None) and, if given, lse (fp32
+    [B, heads, Tq], the log-sum-exp of the scaled scores, -inf without states).
+
+    weight (fp32 [B, kv_heads, N * page]), if given, is brought up to date: ``weight[b, h, j] = decay *
+    weight[b, h, j] +`` the probabilities that the queries of key head h gave to state j, for the ``lens[b]`` states;
+    sums have a fixed order.  This takes a workspace of 4 bytes a query row, key head and place.
+
+    Made for single tokens: the states are read once for every 16 query rows of a key head, and split
+    over the SMs where there are few rows; many queries want cross_attention."""
+    if q.dim() != 3 or q.dtype not in _HALVES:
+        raise ValueError("q: [B, T, heads * dim] rows of fp16 or bf16")
+    if kv_heads is None:
+        kv_heads = heads
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError("heads: a multiple of kv_heads")
+    memory, b, page, n, dim = _memory(k_pages, v_pages, table, kv_heads)
+    tq, dtype = q.shape[1], q.dtype
+    if k_pages.dtype not in (dtype, E4M3):
+        raise ValueError("pages: q's type or e4m3")
+    shape = (b, tq, heads * dim)
+    if scale is None:
+        scale = dim ** -0.5
+    if not 0.0 < scale < _INF or not 0.0 <= decay <= 1.0:
+        raise ValueError("scale: a positive number; decay: from 0 to 1")
+    _scales(k_scale, v_scale, k_pages.dtype)
+    qp, p_lens = _rows(q, "q", shape, dtype), _each(lens, "lens", b)
+    if p_lens is None:
+        raise ValueError("lens: contiguous int32 [B]")
+    p_weight = _account(weight, "weight", (b, kv_heads, n * page), torch.float32)
+    if lse is not None:
+        _statistics(lse, b, heads, tq)
+    if out is not None:
+        op = _rows(out, "out", shape, dtype, out=True)
+        _apart((out,), (q, k_pages, v_pages))
+    if weight is not None and lse is not None:
+        _clear_of((weight, lse), ())
+    index = _ready(q, k_pages, v_pages, table, lens, weight, out, lse)
+    if out is None:
+        out, op = _new(q, shape, dtype)
+    if b == 0 or tq == 0:
+        return out
+    hold, work, size = _work("sb_paged_attention_work", index, b, heads, kv_heads, dim, tq, page, n, weight is not None)
+    _launch("sb_paged_attention", index, *qp, _lib.SB_BF16 if dtype == torch.bfloat16 else _lib.SB_F16, *memory, p_lens, b,
+            heads, kv_heads, dim, tq, scale, k_scale, v_scale, causal, *op, None if lse is None else lse.data_ptr(), p_weight,
+            decay, work, size)
+    return out
+
+
+# ---------------------------------------------------------------- new states
+def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_scale=1.0, weight=None, born=None,
+                stamp=None, after=None, kv_heads=None):
+    """Writes new states k, v [B, T, kv_heads * dim] (fp16 or bf16) behind the ``at[b]`` that item b has, the first
+    ``count[b]`` (int32 [B]) of each or all T, and returns the new lengths (int32 [B]).
+
+    Pages have the states' type, or e4m3: the code nearest to ``x / k_scale`` (``v_scale``), at most 448 of
+    either sign.  The new states' weight becomes 0 and born their stamp (int32 [B, T], or [B] for all of an item's).  Places
+    behind an item's pages, on no page or from ``count[b]`` on keep what they hold.  An item's pages that are
+    written must be its own.  after (allocated if None) shares no memory with at.  kv_heads is that of weight
+    or born where they are given; without them the rows are taken as heads of 32 channels."""
+    if k.dim() != 3 or k.dtype not in _HALVES:
+        raise ValueError("k, v: [B, T, kv_heads * dim] rows of fp16 or bf16")
+    if (born is None) != (stamp is None):
+        raise ValueError("born and stamp: both or neither")
+    for t in (weight, born):
+        if t is not None:
+            if t.dim() != 3 or (kv_heads is not None and t.shape[1] != kv_heads):
+                raise ValueError("weight, born: [B, kv_heads, N * page]")
+            kv_heads = t.shape[1]
+    if kv_heads is None:
+        kv_heads = k.shape[2] // 32
+    memory, b, page, n, dim = _memory(k_pages, v_pages, table, kv_heads, written=True)
+    t, dtype = k.shape[1], k.dtype
+    if k_pages.dtype not in (dtype, E4M3):
+        raise ValueError("pages: the states' type or e4m3")
+    _scales(k_scale, v_scale, k_pages.dtype)
+    shape, places = (b, t, kv_heads * dim), (b, kv_heads, n * page)
+    kp, vp = _rows(k, "k", shape, dtype), _rows(v, "v", shape, dtype)
+    p_at, p_count = _each(at, "at", b), _each(count, "count", b)
+    if p_at is None:
+        raise ValueError("at: contiguous int32 [B]")
+    p_weight, p_born = _account(weight, "weight", places, torch.float32), _account(born, "born", places, torch.int32)
+    sp = (None, 0, 0)
+    if stamp is not None:
+        if stamp.dtype != torch.int32 or stamp.shape not in ((b,), (b, t)):
+            raise ValueError("stamp: int32 [B, T] or [B]")
+        s = stamp.stride()
+        sp = (stamp.data_ptr(), s[0], s[1] if stamp.dim() == 2 else 0)
+    _apart((k_pages, v_pages), (k, v))
+    p_after = _each(after, "after", b)
+    if after is not None:
+        _clear_of((after,), (at, count))
+    index = _ready(k, v, k_pages, v_pages, table, at, count, weight, born, stamp, after)
+    if after is None:
+        after = torch.empty_like(at)
+        p_after = after.data_ptr()
+    if b == 0:
+        return after
+    _launch("sb_paged_write", index, *kp, *vp, _lib.SB_BF16 if dtype == torch.bfloat16 else _lib.SB_F16, *memory, p_at,
+            p_count, b, t, kv_heads, dim, k_scale, v_scale, p_weight, p_born, *sp, p_after)
+    return after
+
+
+# ---------------------------------------------------------------- eviction
+def paged_evict(k_pages, v_pages, table, lens, weight, keep, born=None, since=None, weight_out=None, born_out=None,
+                after=None):
+    """Cuts every item's ``lens[b]`` states back to ``keep`` (a number, or int32 [B]), for each key head by itself.
+
+    Those with ``born >= since[b]`` (int32 [B]) stay before all others, then those of larger weight, of equal
+    ones the first; NaN is the least.  The i-th freed place below keep takes the i-th kept state from keep
+    on: keys, values, weight and stamp; nothing else moves.  Returns (after, weight, born): the new
+    lengths ``min(lens, keep)``, and weights and stamps [B, kv_heads, N * page] with 0 from the new length on
+    (born None without born).  after, weight_out and born_out (allocated if None) may be lens, weight and born
+    themselves and otherwise share no memory with them.  An item's pages must be its own; rows on
+    no page are not moved."""
+    if weight.dim() != 3:
+        raise ValueError("weight: [B, kv_heads, N * page]")
+    kv_heads = weight.shape[1]
+    memory, b, page, n, dim = _memory(k_pages, v_pages, table, kv_heads, written=True)
+    places = (b, kv_heads, n * page)
+    if since is not None and born is None:
+        raise ValueError("since needs born")
+    if born is None and born_out is not None:
+        raise ValueError("born_out needs born")
+    p_lens, p_since, p_after = _each(lens, "lens", b), _each(since, "since", b), _each(after, "after", b)
+    if p_lens is None:
+        raise ValueError("lens: contiguous int32 [B]")
+    p_keep, keep_all = None, 0
+    if isinstance(keep, torch.Tensor):
+        p_keep = _each(keep, "keep", b)
+    else:
+        keep_all = min(int(keep), 1 << 30)
+        if keep_all < 0 or keep_all != min(keep, 1 << 30):
+            raise ValueError("keep: a whole number from 0 on, or int32 [B]")
+    pw, pb = _account(weight, "weight", places, torch.float32), _account(born, "born", places, torch.int32)
+    pwo, pbo = _account(weight_out, "weight_out", places, torch.float32), _account(born_out, "born_out", places, torch.int32)
+    if weight_out is not None or born_out is not None or after is not None:
+        same = (pwo is not None and pwo == pw, pbo is not None and pbo == pb, p_after is not None and p_after == p_lens)
+        _clear_of((None if same[0] else weight_out, None if same[1] else born_out, None if same[2] else after),
+                  (weight, born, lens, since, keep if p_keep is not None else None))
+    index = _ready(k_pages, v_pages, table, lens, weight, born, since, keep if p_keep is not None else None, weight_out,
+                   born_out, after)
+    if after is None:
+        after = torch.empty_like(lens)
+        p_after = after.data_ptr()
+    if weight_out is None:
+        weight_out = torch.empty_like(weight)
+        pwo = weight_out.data_ptr()
+    if born_out is None and born is not None:
+        born_out = torch.empty_like(born)
+        pbo = born_out.data_ptr()
+    if b == 0:
+        return after, weight_out, born_out
+    hold, work, size = _work("sb_paged_evict_work", index, b, kv_heads, page, n)
+    _launch("sb_paged_evict", index, *memory, p_lens, p_keep, keep_all, p_since, b, kv_heads, dim, pw, pb, pwo, pbo, p_after,
+            work, size)
+    return after, weight_out, born_out

@@ -1,0 +1,140 @@
+"""Refusals of the paged memory's operators on the CPU: every wrong argument is turned down before anything
+reaches a kernel."""
+import ctypes as C
+
+import pytest
+import torch
+
+import sarbon_b200 as sb
+from sarbon_b200 import _lib
+
+H16 = dict(dtype=torch.float16)
+I32 = dict(dtype=torch.int32)
+E4M3 = torch.float8_e4m3fn
+
+
+def pools(p=6, page=4, width=128, dtype=torch.float16):
+    return torch.zeros(p, page, width, dtype=dtype), torch.zeros(p, page, width, dtype=dtype)
+
+
+K, V = pools()
+ATTEND = dict(q=torch.zeros(2, 1, 256, **H16), k_pages=K, v_pages=V, table=torch.zeros(2, 3, **I32),
+              lens=torch.zeros(2, **I32), heads=4, kv_heads=2)
+WRITE = dict(k=torch.zeros(2, 5, 128, **H16), v=torch.zeros(2, 5, 128, **H16), k_pages=K, v_pages=V,
+             table=torch.zeros(2, 3, **I32), at=torch.zeros(2, **I32), weight=torch.zeros(2, 2, 12),
+             born=torch.zeros(2, 2, 12, **I32), stamp=torch.zeros(2, 5, **I32))
+EVICT = dict(k_pages=K, v_pages=V, table=torch.zeros(2, 3, **I32), lens=torch.zeros(2, **I32), weight=torch.zeros(2, 2, 12),
+             keep=4, born=torch.zeros(2, 2, 12, **I32), since=torch.zeros(2, **I32))
+
+MEMORY = [
+    dict(k_pages=K.float(), v_pages=V.float()), dict(k_pages=K[0]), dict(v_pages=V[:5]), dict(v_pages=V.bfloat16()),
+    dict(k_pages=torch.zeros(6, 128, 4, **H16).transpose(1, 2)), dict(table=torch.zeros(2, 3, dtype=torch.int64)),
+    dict(table=torch.zeros(6, **I32)), dict(table=torch.zeros(3, 2, **I32).t()), dict(table=torch.zeros(3, 3, **I32)),
+    dict(k_pages=pools(width=96)[0], v_pages=pools(width=96)[1]), dict(k_pages=pools(page=0)[0], v_pages=pools(page=0)[1]),
+    dict(table=torch.zeros(2, 1, **I32).expand(2, 1 << 28)),
+    dict(),  # all well, but not on a GPU
+]
+
+
+@pytest.mark.parametrize("change", MEMORY + [
+    dict(q=torch.zeros(2, 1, 256)), dict(q=torch.zeros(2, 256, **H16)), dict(q=torch.zeros(2, 1, 256, dtype=torch.bfloat16)),
+    dict(q=torch.zeros(1, 1, 256, **H16)), dict(heads=3), dict(heads=8, kv_heads=3), dict(kv_heads=None), dict(heads=0),
+    dict(lens=None), dict(lens=torch.zeros(2, dtype=torch.int64)), dict(lens=torch.zeros(3, **I32)),
+    dict(lens=torch.zeros(4, **I32)[::2]), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")),
+    dict(decay=-0.1), dict(decay=1.1), dict(decay=float("nan")), dict(k_scale=2.0), dict(v_scale=0.5), dict(k_scale=0.0),
+    dict(weight=torch.zeros(2, 2, 11)), dict(weight=torch.zeros(2, 4, 12)), dict(weight=torch.zeros(2, 2, 12, **H16)),
+    dict(weight=torch.zeros(2, 12, 2).transpose(1, 2)), dict(lse=torch.zeros(2, 4, 2)), dict(out=torch.zeros(2, 1, 128, **H16)),
+    dict(out=ATTEND["q"]),
+])
+def test_attention_refuses(change):
+    with pytest.raises(ValueError):
+        sb.paged_attention(**{**ATTEND, **change})
+
+
+@pytest.mark.parametrize("change", MEMORY + [
+    dict(k=torch.zeros(2, 5, 128)), dict(k=torch.zeros(2, 5, 128, dtype=torch.bfloat16)), dict(v=torch.zeros(2, 4, 128, **H16)),
+    dict(k=torch.zeros(2, 5, 64, **H16), v=torch.zeros(2, 5, 64, **H16)), dict(at=None), dict(at=torch.zeros(2)),
+    dict(count=torch.zeros(3, **I32)), dict(count=torch.zeros(2, dtype=torch.int64)), dict(weight=torch.zeros(2, 12)),
+    dict(weight=torch.zeros(2, 2, 13)), dict(born=torch.zeros(2, 2, 12)), dict(born=torch.zeros(2, 1, 12, **I32)),
+    dict(stamp=None), dict(born=None), dict(stamp=torch.zeros(2, 4, **I32)), dict(stamp=torch.zeros(5, **I32)),
+    dict(stamp=torch.zeros(2, 5)), dict(k_scale=2.0), dict(after=torch.zeros(3, **I32)), dict(after=WRITE["at"]),
+    dict(kv_heads=4), dict(v_pages=K), dict(k=K[:2, :, :].expand(2, 4, 128), v=V[:2], stamp=torch.zeros(2, **I32)),
+    dict(k_pages=torch.zeros(1, 4, 128, **H16).expand(6, 4, 128)), dict(v_pages=torch.zeros(6, 1, 128, **H16).expand(6, 4, 128)),
+])
+def test_write_refuses(change):
+    with pytest.raises(ValueError):
+        sb.paged_write(**{**WRITE, **change})
+
+
+@pytest.mark.parametrize("change", MEMORY + [
+    dict(weight=torch.zeros(2, 24)), dict(weight=torch.zeros(2, 2, 13)), dict(weight=torch.zeros(2, 3, 12)), dict(lens=None),
+    dict(lens=torch.zeros(2)), dict(keep=-1), dict(keep=1.5), dict(keep=torch.zeros(2)), dict(keep=torch.zeros(3, **I32)),
+    dict(born=None), dict(since=torch.zeros(3, **I32)), dict(born=torch.zeros(2, 2, 12)),
+    dict(weight_out=torch.zeros(2, 2, 11)), dict(born=None, since=None, born_out=EVICT["born"]), dict(after=torch.zeros(1, **I32)),
+    dict(weight_out=EVICT["born"].view(torch.float32)), dict(after=EVICT["since"]), dict(v_pages=K),
+    dict(k_pages=torch.zeros(1, 4, 128, **H16).expand(6, 4, 128)),
+])
+def test_evict_refuses(change):
+    with pytest.raises(ValueError):
+        sb.paged_evict(**{**EVICT, **change})
+
+
+def test_results_that_lie_on_others():
+    """Results may be their operands themselves in eviction, but lie on nothing in part."""
+    room = torch.zeros(2 * 2 * 12 + 4)
+    weight, beside = room[:48].view(2, 2, 12), room[4:].view(2, 2, 12)
+    with pytest.raises(ValueError, match="own memory"):
+        sb.paged_evict(**{**EVICT, "weight": weight, "weight_out": beside})
+    with pytest.raises(ValueError, match="CUDA"):
+        sb.paged_evict(**{**EVICT, "weight": weight, "weight_out": weight, "born_out": EVICT["born"], "after": EVICT["lens"]})
+    ints = torch.zeros(3, **I32)
+    with pytest.raises(ValueError, match="own memory"):
+        sb.paged_evict(**{**EVICT, "lens": ints[:2], "after": ints[1:]})
+
+
+def test_autograd_inputs_are_refused():
+    with pytest.raises(ValueError):
+        sb.paged_attention(**{**ATTEND, "q": torch.zeros(2, 1, 256, **H16, requires_grad=True)})
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+        sb.paged_attention(**{**ATTEND, "q": fw.make_dual(ATTEND["q"], torch.ones_like(ATTEND["q"]))})
+
+
+def test_library_refuses():
+    """The C entries turn down what the wrappers never pass, before any device call."""
+    lib, n, one, two = _lib.lib(), C.c_longlong(0), C.c_void_p(16), C.c_void_p(32)
+
+    def attention(q=one, row=64, qt=0, pt=0, kp=one, kr=64, p=4, page=4, table=one, tr=2, nn=2, lens=one, b=1, h=2, hkv=1, dh=32,
+                  tq=1, scale=1.0, ks=1.0, weight=None, decay=1.0, work=None, size=0):
+        return lib.sb_paged_attention(q, row, 64, qt, kp, kr, 256, two, kr, 256, pt, p, page, table, tr, nn, lens, b, h, hkv, dh, tq,
+                                      scale, ks, 1.0, 0, one, row, 64, None, weight, decay, work, size, None)
+
+    for bad in (dict(qt=1), dict(qt=2), dict(pt=3), dict(pt=1), dict(dh=48), dict(h=3, hkv=2), dict(hkv=0), dict(tq=-1), dict(b=-1),
+                dict(page=0), dict(p=-1), dict(nn=-1), dict(page=1 << 20, nn=1 << 10), dict(scale=0.0), dict(scale=float("nan")),
+                dict(ks=2.0), dict(pt=2, ks=0.0), dict(pt=2, scale=1e30, ks=1e30), dict(weight=one, decay=2.0), dict(q=None),
+                dict(q=C.c_void_p(8)), dict(row=60), dict(kr=60), dict(kr=-8), dict(kp=None), dict(kp=C.c_void_p(8)),
+                dict(table=None), dict(tr=-1), dict(lens=None)):
+        assert attention(**bad) == _lib.SB_EINVAL, bad
+    assert attention(b=0) == _lib.SB_OK and attention(tq=0) == _lib.SB_OK
+    assert lib.sb_paged_attention_work(1, 2, 1, 48, 1, 4, 2, 0, C.byref(n)) == _lib.SB_EINVAL
+    assert lib.sb_paged_attention_work(1, 2, 1, 32, 1, 0, 2, 0, C.byref(n)) == _lib.SB_EINVAL
+    assert lib.sb_paged_evict_work(1, 0, 4, 2, C.byref(n)) == _lib.SB_EINVAL
+    assert lib.sb_paged_evict_work(3, 2, 4, 2, C.byref(n)) == _lib.SB_OK and n.value > 0
+
+    def write(k=one, pt=0, dt=0, kp=one, ks=1.0, at=one, after=one, b=1, t=1, dh=32, kr=32, pr=32):
+        return lib.sb_paged_write(k, kr, 32, one, kr, 32, dt, kp, pr, 128, two, pr, 128, pt, 4, 4, one, 2, 2, at, None, b, t, 1, dh, ks,
+                                  1.0, None, None, None, 0, 0, after, None)
+
+    for bad in (dict(k=None), dict(dt=1), dict(pt=3), dict(kp=None), dict(kp=C.c_void_p(8)), dict(ks=2.0), dict(pt=2, ks=-1.0),
+                dict(at=None), dict(after=None), dict(b=-1), dict(t=-1), dict(dh=16), dict(kr=-1), dict(pr=20)):
+        assert write(**bad) == _lib.SB_EINVAL, bad
+    assert write(b=0) == _lib.SB_OK
+
+    def evict(kp=one, pt=0, lens=one, weight=one, since=None, born=None, born_out=None, work=one, size=1 << 20, b=1, dh=32):
+        return lib.sb_paged_evict(kp, 32, 128, two, 32, 128, pt, 4, 4, one, 2, 2, lens, None, 2, since, b, 1, dh, weight, born, weight,
+                                  born_out, one, work, size, None)
+
+    for bad in (dict(kp=None), dict(pt=1), dict(lens=None), dict(weight=None), dict(since=one), dict(born=one), dict(born_out=one),
+                dict(work=None), dict(work=C.c_void_p(8)), dict(size=4), dict(b=-1), dict(dh=16)):
+        assert evict(**bad) == _lib.SB_EINVAL, bad
+    assert evict(b=0) == _lib.SB_OK
