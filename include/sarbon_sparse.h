@@ -541,6 +541,15 @@ SB_API int sb_gated_norm_backward(const void* dy, long long dy_row, long long dy
  * Lengths outside [0, N * page] are clamped.  Each call launches on `stream`, allocates nothing and may be
  * captured in a CUDA graph after a first call outside capture on the device.  SB_F8 pools hold e4m3 codes: c
  * stands for c * scale (scales are 1 for the other types). */
+typedef struct {
+  void *k, *v;
+  long long k_row, k_page, v_row, v_page;
+  const int* table;
+  long long table_row;
+  int dtype; /* SB_F16, SB_BF16 or SB_F8 */
+  int P, page, N;
+  int B, Hkv, dh;
+} sb_paged_memory;
 
 /* Attention of Tq query tokens, [B][Tq][H*dh] rows of SB_F16 or SB_BF16 (16-byte aligned, strides multiples of 8), to
  * the first lens[b] states of each item: out = softmax(scale q k^T) v per head, query head h on key head
@@ -550,35 +559,30 @@ SB_API int sb_gated_norm_backward(const void* dy, long long dy_row, long long dy
  * probabilities of a key head's queries, for the states below lens[b]; fixed order.  work:
  * sb_paged_attention_work bytes (16-byte aligned), not shared by calls that may overlap.  Scores, statistics,
  * probabilities and sums are fp32; probabilities meet v as two 16-bit parts. */
-SB_API int sb_paged_attention(const void* q, long long q_row, long long q_img, int q_dtype, const void* k_pages,
-                              long long k_row, long long k_page, const void* v_pages, long long v_row,
-                              long long v_page, int page_dtype, int P, int page, const int* table, long long table_row,
-                              int N, const int* lens, int B, int H, int Hkv, int dh, int Tq, float scale, float k_scale,
-                              float v_scale, int causal, void* out, long long o_row, long long o_img, float* lse,
-                              float* weight, float decay, void* work, long long work_bytes, void* stream);
+SB_API int sb_paged_attention(const sb_paged_memory* memory, const void* q, long long q_row, long long q_img, int q_dtype,
+                              const int* lens, int H, int Tq, float scale, float k_scale, float v_scale, int causal,
+                              void* out, long long o_row, long long o_img, float* lse, float* weight, float decay,
+                              void* work, long long work_bytes, void* stream);
 
 /* Bytes of workspace that sb_paged_attention needs on the current device (account: with weight). */
-SB_API int sb_paged_attention_work(int B, int H, int Hkv, int dh, int Tq, int page, int N, int account, long long* bytes);
+SB_API int sb_paged_attention_work(int B, int H, int Hkv, int dh, int Tq, int page_dtype, int page, int N, int account,
+                                   long long* bytes);
 
 /* New states: row t < count[b] (NULL: T) of k, v [B][T][Hkv*dh] (SB_F16 or SB_BF16, any strides) goes to
  * position at[b] + t of item b; pools of the same type, or SB_F8: the code nearest to x / scale, at most 448
  * of either sign.  weight there becomes 0, born stamp[b * stamp_img + t * stamp_row] (each may be NULL).
  * after [B] gets the new lengths and shares no memory with at. */
-SB_API int sb_paged_write(const void* k, long long k_row, long long k_img, const void* v, long long v_row, long long v_img,
-                          int dtype, void* k_pages, long long kp_row, long long kp_page, void* v_pages,
-                          long long vp_row, long long vp_page, int page_dtype, int P, int page, const int* table,
-                          long long table_row, int N, const int* at, const int* count, int B, int T, int Hkv, int dh,
-                          float k_scale, float v_scale, float* weight, int* born, const int* stamp,
-                          long long stamp_img, long long stamp_row, int* after, void* stream);
+SB_API int sb_paged_write(const sb_paged_memory* memory, const void* k, long long k_row, long long k_img, const void* v,
+                          long long v_row, long long v_img, int dtype, const int* at, const int* count, int T,
+                          float k_scale, float v_scale, float* weight, int* born, const int* stamp, long long stamp_img,
+                          long long stamp_row, int* after, void* stream);
 
 /* Eviction: of the lens[b] states of each item and key head the keep[b] (keep NULL: keep_all) first by (born >=
  * since[b], weight descending, index) stay (NaN is the least; since NULL: weight alone).  The i-th freed place
  * below keep takes the i-th kept state from keep on.  weight_out and born_out get the weights and stamps
  * that stay, 0 from the new length on; after [B] the new lengths.  They may be weight, born and lens themselves.
  * work: sb_paged_evict_work bytes, as above. */
-SB_API int sb_paged_evict(void* k_pages, long long k_row, long long k_page, void* v_pages, long long v_row,
-                          long long v_page, int page_dtype, int P, int page, const int* table, long long table_row, int N,
-                          const int* lens, const int* keep, int keep_all, const int* since, int B, int Hkv, int dh,
+SB_API int sb_paged_evict(const sb_paged_memory* memory, const int* lens, const int* keep, int keep_all, const int* since,
                           const float* weight, const int* born, float* weight_out, int* born_out, int* after, void* work,
                           long long work_bytes, void* stream);
 SB_API int sb_paged_evict_work(int B, int Hkv, int page, int N, long long* bytes);

@@ -23,15 +23,16 @@ namespace sb {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kRing = 24 * 1024;  // bytes a warp
-
 struct PagedArgs {
   const void* q;
   long long q_row, q_img;  // elements
   Pool k, v;
   PageTable pages;
   const int* lens;
-  int B, H, Hkv, group, Tq, rows, blocks, splits;  // rows = group * Tq of an (item, key head), blocks of 16
+  int B, H, Hkv, group, Tq, rows, blocks;  // rows = group * Tq of an (item, key head), blocks of 16
+  int shares;                              // CTAs that share the chunks of all units; 0: a CTA a unit
+  int ends;                                // CTAs an (item, key head) of the last kernel; 0: none
+  int chunk;                               // states
   int q_bf16, causal;
   float scale_log2, v_scale;  // scale * k_scale * log2(e)
   OutView o;
@@ -39,31 +40,115 @@ struct PagedArgs {
   float* weight;
   float decay;
   float* scores;  // [B * Hkv][cap][rows], log2 units
-  float* part_o;  // [splits][B * H * Tq][dh]
-  float* part_l;  // [splits][B * H * Tq], log2 of the sum
-  float* log_sum;  // [B * H * Tq], log2
-  long long all_rows;
+  float* part_o;  // [slots][part_rows][dh]
+  float* part_l;  // [slots][part_rows], log2 of the sum
+  int part_rows;  // min(rows, 16)
+  SB_DEV int chunks(int b) const { return (pages.clamp(lens[b]) + chunk - 1) / chunk; }
+  SB_DEV int units() const { return Hkv * blocks; }  // of an item
 };
 
-template <int DH, int PT>
+// How the chunks of all units, one unit after the other, are shared: CTA i gets `each` of them from i * each on.  What
+// CTA i finds of unit u goes to slot i + u: along the chunks i or u grows from one piece to the next.
+struct Shares {
+  long long total, each;
+  int item;            // the item that position `at` lies in (B: none)
+  long long before;    // chunks of one unit of every item before it
+};
+constexpr long long kLeast = 16;  // chunks a CTA, four a warp
+
+// Looks up the shares and position `at` of the chunks, with all `THREADS` of the CTA; item >= 0: that item instead.
+template <int THREADS>
+SB_DEV Shares look_up(const PagedArgs& a, long long cta, int item, long long (&room)[THREADS / 32 + 2], int& found) {
+  const int lane = lane_id(), warp = warp_id();
+  long long sum = 0, before = 0;
+  for (int b = threadIdx.x; b < a.B; b += THREADS) {
+    const int n = a.chunks(b);
+    sum += n;
+    if (b < item) before += n;
+  }
+#pragma unroll
+  for (int x = 16; x; x >>= 1) {
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+    before += __shfl_xor_sync(0xFFFFFFFFu, before, x);
+  }
+  Shares s;
+  s.total = s.before = 0;
+  __syncthreads();
+  if (lane == 0) room[warp] = sum;
+  __syncthreads();
+  for (int w = 0; w < THREADS / 32; ++w) s.total += room[w];
+  s.total *= a.units();
+  s.each = max((s.total + a.shares - 1) / a.shares, kLeast);
+  s.item = item;
+  if (item >= 0) {
+    __syncthreads();
+    if (lane == 0) room[warp] = before;
+    __syncthreads();
+    for (int w = 0; w < THREADS / 32; ++w) s.before += room[w];
+    return s;
+  }
+  s.item = a.B;
+  if (cta * s.each >= s.total) return s;
+  const long long at = cta * s.each / a.units();
+  for (int b0 = 0; b0 < a.B; b0 += THREADS) {  // ends with the tile of items that holds it
+    const int b = b0 + (int)threadIdx.x;
+    const int n = b < a.B ? a.chunks(b) : 0;
+    long long upto = n;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const long long u = __shfl_up_sync(0xFFFFFFFFu, upto, x);
+      if (lane >= x) upto += u;
+    }
+    __syncthreads();
+    if (lane == 31) room[warp] = upto;
+    if (threadIdx.x == 0) found = -1;
+    __syncthreads();
+    long long base = s.before, all = 0;
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) base += room[w];
+      all += room[w];
+    }
+    const long long from = base + upto - n;
+    if (from <= at && at < from + n) {
+      found = b;
+      room[THREADS / 32] = from;
+    }
+    __syncthreads();
+    if (found >= 0) {
+      s.item = found;
+      s.before = room[THREADS / 32];
+      break;
+    }
+    s.before += all;
+  }
+  return s;
+}
+
+template <int DH, int PT, int NB>
 struct Paged {
   static constexpr bool E4M3 = PT == SB_F8, BF16 = PT == SB_BF16;
   static constexpr int RB = DH * (E4M3 ? 1 : 2);                // bytes a state and head
-  static constexpr int CK = 4096 / RB < 64 ? 4096 / RB : 64;    // states a chunk
+  // Two CTAs an SM, 24 KB a warp on their way.  e4m3 is bound by issuing instructions more than by memory: three CTAs.
+  static constexpr int OCC = E4M3 && NB == 1 ? 3 : 2;
+  static constexpr int kRing = OCC == 3 ? 16 * 1024 : 24 * 1024;  // bytes a warp
+  static constexpr int CK = 4096 / RB < 64 ? 4096 / RB : 64;      // states a chunk
   static constexpr int HALF = CK * RB, STAGE = 2 * HALF, STAGES = kRing / STAGE;
   static constexpr int LANES = RB / 16, AT_ONCE = 32 / LANES;   // lanes a row, rows a copy
-  static constexpr int PITCH = DH + 4;                          // floats a row of the warps' outputs
   static constexpr int SMEM = kWarps * kRing;
-  static_assert(kWarps * 16 * PITCH * 4 <= SMEM && STAGES >= 3, "ring");
-  // byte of 16-byte chunk c of a row: eight rows of a chunk fall in distinct banks
-  SB_DEV static uint32_t at(int row, int c) {
-    const int x = RB >= 128 ? row & 7 : RB == 64 ? (row >> 1) & 3 : (row >> 2) & 1;
-    return row * RB + ((c ^ x) << 4);
+  static_assert(8 * NB * DH * 4 <= STAGE && STAGES >= 2, "ring");
+  // Byte of 16-byte chunk c of a row: eight rows of a chunk fall in distinct banks.  Bits of the row are bits of
+  // what its chunks are turned by, so rows x + l that share none are l's place, turned by x's.
+  SB_DEV static constexpr uint32_t turn(int row) {
+    return (RB >= 128 ? row & 7 : RB == 64 ? (row >> 1) & 3 : (row >> 2) & 1) << 4;
   }
+  SB_DEV static uint32_t at(int row, int c) { return row * RB + (c << 4 ^ turn(row)); }
 };
 
-SB_DEV void copy16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+// What states that take no part are read from.
+__device__ uint4 g_zeros[16];
+
+SB_DEV void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 SB_DEV void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -112,49 +197,89 @@ struct Row {
   SB_DEV Row(const PagedArgs& a, int kvh, int r) : t(r / a.group), h(kvh * a.group + r - t * a.group) {}
 };
 
+// Where a warp is among the chunks: item, unit of the item, chunk of the unit.
+struct Cursor {
+  int b, unit, c, n, count;
+  SB_DEV void item(const PagedArgs& a) {
+    count = a.pages.clamp(a.lens[b]);
+    n = (count + a.chunk - 1) / a.chunk;
+  }
+  // `by` chunks on, of which there are as many
+  SB_DEV void advance(const PagedArgs& a, int by) {
+    c += by;
+    while (c >= n) {
+      c -= n;
+      if (++unit == a.units()) {
+        unit = 0;
+        do {
+          ++b;
+          item(a);
+        } while (n == 0);
+      }
+    }
+  }
+};
+
 // NB: column tiles of eight query rows
 template <int DH, int PT, int NB>
-__global__ void __launch_bounds__(kWarps * 32, 2) paged_attend_kernel(const __grid_constant__ PagedArgs a) {
-  using C = Paged<DH, PT>;
+__global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_attend_kernel(const __grid_constant__ PagedArgs a) {
+  using C = Paged<DH, PT, NB>;
   constexpr bool E4M3 = C::E4M3, BF16 = C::BF16;
   constexpr int CK = C::CK, KT = CK / 16, KS = DH / 16, R = CK > 32 ? 2 : 1;
   constexpr float lift = kLift<BF16>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ longlong2 place[kWarps][CK];       // where a chunk's rows lie in the pools; -1: nowhere
+  __shared__ ulonglong2 place[kWarps][CK];      // addresses of a chunk's rows of K and V
   __shared__ uint64_t there[kWarps][C::STAGES];  // a stage's rows that take part, as bits
   __shared__ float2 ml[kWarps][16];
   __shared__ float fin[16];
+  __shared__ long long room[kWarps + 2];
+  __shared__ int area[kWarps], found;
   const int warp = warp_id(), lane = lane_id();
   const int g = lane >> 2, tig = lane & 3;
-  int idx = blockIdx.x;
-  const int block = idx % a.blocks;
-  idx /= a.blocks;
-  const int split = idx % a.splits;
-  idx /= a.splits;
-  const int kvh = idx % a.Hkv, b = idx / a.Hkv, unit = idx;
-  const int r0 = block * 16, rows = min(16, a.rows - r0);
-  const int count = a.pages.clamp(a.lens[b]);
-  // the item's own states are split evenly, in whole chunks
-  const int chunks = (count + CK - 1) / CK, each = (chunks + a.splits - 1) / a.splits;
-  const int first = min(split * each, chunks), n = min(first + each, chunks) - first;
-  const int mine = n > warp ? (n - warp + kWarps - 1) / kWarps : 0;  // chunks first + warp, + kWarps ...
-  uint8_t* const ring = smem + warp * kRing;
+
+  // this CTA's chunks: `left` from cursor `at` on
+  Cursor at;
+  long long left;
+  if (a.shares) {
+    const Shares s = look_up<kWarps * 32>(a, blockIdx.x, -1, room, found);
+    if (s.item == a.B) return;
+    at.b = s.item;
+    at.item(a);
+    const long long in = blockIdx.x * s.each - s.before * a.units();
+    at.unit = (int)(in / at.n);
+    at.c = (int)(in - (long long)at.unit * at.n);
+    left = min(s.each, s.total - blockIdx.x * s.each);
+  } else {
+    at.b = blockIdx.x / a.units();
+    at.unit = blockIdx.x - at.b * a.units();
+    at.c = 0;
+    at.item(a);
+    left = at.n;
+  }
+  const int mine = left > warp ? (int)((left - warp + kWarps - 1) / kWarps) : 0;  // chunks warp, warp + kWarps, ... of them
+  uint8_t* const ring = smem + warp * C::kRing;
   const uint32_t ring_at = smem_u32(ring);
-  const uint8_t* const kp = a.k.p + (long long)kvh * C::RB;
-  const uint8_t* const vp = a.v.p + (long long)kvh * C::RB;
 
   // table entries of the next chunk to be copied, asked for a chunk ahead
-  int entry[R];
+  Cursor ahead = at;
+  if (mine > 0 && warp > 0) ahead.advance(a, warp);
+  int entry[R], asked = 0, head = 0;
   uint32_t within[R];
-  auto ask = [&](int i) {
+  auto ask = [&] {
+    if (asked < mine) {
+      if (asked) ahead.advance(a, kWarps);
+      head = ahead.unit / a.blocks;
 #pragma unroll
-    for (int x = 0; x < R; ++x) {
-      const int r = lane + 32 * x, j = (first + warp + i * kWarps) * CK + r;
-      entry[x] = -1;
-      within[x] = 0;
-      if (r < CK && i < mine && j < count) entry[x] = a.pages.entry(b, (uint32_t)j, within[x]);
+      for (int x = 0; x < R; ++x) {
+        const int r = lane + 32 * x, j = ahead.c * CK + r;
+        entry[x] = -1;
+        within[x] = 0;
+        if (r < CK && j < ahead.count) entry[x] = a.pages.entry(ahead.b, (uint32_t)j, within[x]);
+      }
     }
+    ++asked;
   };
+  const uint32_t own16 = lane % C::LANES * 16, own_at = ring_at + C::at(lane / C::LANES, lane % C::LANES);
   auto copy = [&](int i) {  // the warp's chunk i, whose entries are there
     if (i < mine) {
       const int st = i % C::STAGES;
@@ -162,35 +287,42 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attend_kernel(const __gr
 #pragma unroll
       for (int x = 0; x < R; ++x) {
         const bool ok = a.pages.has(entry[x]);
-        const long long w = within[x], e = entry[x];
+        const uint64_t none = reinterpret_cast<uint64_t>(g_zeros);
         if (lane + 32 * x < CK)
-          place[warp][lane + 32 * x] = ok ? make_longlong2(e * a.k.page + w * a.k.row, e * a.v.page + w * a.v.row)
-                                          : make_longlong2(-1, -1);
+          place[warp][lane + 32 * x] =
+              make_ulonglong2(ok ? a.k.row_at(entry[x], within[x]) + head * C::RB : none,
+                              ok ? a.v.row_at(entry[x], within[x]) + head * C::RB : none);
         bits |= (uint64_t)__ballot_sync(0xFFFFFFFFu, ok) << (32 * x);
       }
       if (lane == 0) there[warp][st] = bits;
       __syncwarp();
-      const int c = lane % C::LANES;
-      const uint32_t dst = ring_at + st * C::STAGE;
+      const uint32_t dst = own_at + st * C::STAGE;
 #pragma unroll
-      for (int x = 0; x < CK / C::AT_ONCE; ++x) {
-        const int r = x * C::AT_ONCE + lane / C::LANES;
-        const longlong2 from = place[warp][r];
-        const bool ok = from.x >= 0;
-        const uint32_t to = dst + C::at(r, c);
-        copy16(to, ok ? kp + from.x + c * 16 : static_cast<const uint8_t*>(a.q), ok);
-        copy16(to + C::HALF, ok ? vp + from.y + c * 16 : static_cast<const uint8_t*>(a.q), ok);
+      for (int x = 0; x < CK; x += C::AT_ONCE) {
+        const ulonglong2 from = place[warp][x + lane / C::LANES];
+        const uint32_t to = (dst ^ C::turn(x)) + x * C::RB;
+        copy16(to, reinterpret_cast<const void*>(from.x + own16));
+        copy16(to + C::HALF, reinterpret_cast<const void*>(from.y + own16));
       }
     }
     copies_done();
   };
-  ask(0);
+  ask();
 #pragma unroll 1
   for (int i = 0; i < C::STAGES; ++i) {
     copy(i);
-    ask(i + 1);
+    ask();
     __syncwarp();  // place is written again
   }
+
+  int i = 0;  // the warp's chunk
+  long long done = 0;
+  do {  // a piece: this CTA's chunks of a unit
+    const int b = at.b, kvh = at.unit / a.blocks, block = at.unit - kvh * a.blocks, count = at.count;
+    const int r0 = block * 16, rows = min(16, a.rows - r0);
+    const int piece = (int)min((long long)at.n - at.c, left - done);
+    const bool whole = piece == at.n;
+    const int i_end = done + piece > warp ? (int)((done + piece - warp + kWarps - 1) / kWarps) : 0;
 
   // Q as the second operand: rows g (+ 8), channels 16 ks + 2 tig (+ 8), or for e4m3 16 ks + 4 tig (+ 2).  e4m3 is
   // multiplied as fp16: bf16 rows are then brought to at most 2^14 by a power of two, and what falls
@@ -246,12 +378,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attend_kernel(const __gr
 #pragma unroll
     for (int x = 0; x < KS; ++x) o[x][y][0] = o[x][y][1] = o[x][y][2] = o[x][y][3] = 0.f;
   }
-  float* const scores = a.scores ? a.scores + (long long)unit * a.pages.cap * a.rows + r0 : nullptr;
+  float* const scores = a.scores ? a.scores + ((long long)b * a.Hkv + kvh) * a.pages.cap * a.rows + r0 : nullptr;
+  const int chunk0 = at.c - (int)done;  // of the unit: chunk0 + warp + i * kWarps
 
-  for (int i = 0; i < mine; ++i) {
+  const int i_first = i;
+  for (; i < i_end; ++i) {
     copies_wait<C::STAGES - 1>();
     __syncwarp();
-    const int st = i % C::STAGES, j0 = (first + warp + i * kWarps) * CK;
+    const int st = i % C::STAGES, j0 = (chunk0 + warp + i * kWarps) * CK;
     const uint32_t kb = ring_at + st * C::STAGE, vb = kb + C::HALF;
     const uint64_t bits = there[warp][st];
     const bool mixed = j0 + CK > seen_by_all;  // (or the last chunk)
@@ -301,16 +435,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attend_kernel(const __gr
         }
     }
     if (scores) {
+      float* to8 = scores + (long long)(j0 + g) * a.rows + 2 * tig;  // of every eighth state
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int j = j0 + kt * 16 + g + 8 * x;
-          if (j < count) {
+        for (int x = 0; x < 2; ++x, to8 += 8 * a.rows) {
+          if (j0 + kt * 16 + 8 * x + g < count) {
 #pragma unroll
             for (int y = 0; y < NB; ++y) {
               const int r = 8 * y + 2 * tig;
-              float* to = scores + (long long)j * a.rows + r;
+              float* to = to8 + 8 * y;
               const float u = s[kt][y][2 * x] * factor[y][0], w = s[kt][y][2 * x + 1] * factor[y][1];
               if (a.rows % 2 == 0) {
                 if (r < rows) *reinterpret_cast<float2*>(to) = make_float2(u, w);
@@ -468,29 +602,35 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attend_kernel(const __gr
         }
     }
     __syncwarp();  // every lane has read the stage
-    copy(i + C::STAGES);
-    ask(i + C::STAGES + 1);
-    __syncwarp();
+    if (i + 1 < i_end) {
+      copy(i + C::STAGES);
+      ask();
+      __syncwarp();
+    }
   }
-  copies_wait<0>();
 #pragma unroll
   for (int y = 0; y < NB; ++y)
 #pragma unroll
     for (int z = 0; z < 2; ++z)
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) l[y][z] += __shfl_xor_sync(0xFFFFFFFFu, l[y][z], x);
-  // the warps' outputs meet in shared memory, rows [warp][8 NB][PITCH], over the rings; maxima as exponents of 2
-  __syncthreads();
-  float* all_o = reinterpret_cast<float*>(smem);
+  // the warps' outputs meet in shared memory: rows of DH floats in the stage that a warp has just read (and fills
+  // again afterwards), groups of eight floats turned so that no two lanes meet in a bank; maxima as exponents of 2
+  const bool some = i > i_first;
+  const int last = some ? warp * C::kRing + (i - 1) % C::STAGES * C::STAGE : -1;
+  if (some) {
+    float* own = reinterpret_cast<float*>(smem + last);
 #pragma unroll
-  for (int x = 0; x < KS; ++x)
+    for (int x = 0; x < KS; ++x)
 #pragma unroll
-    for (int y = 0; y < NB; ++y)
+      for (int y = 0; y < NB; ++y)
 #pragma unroll
-      for (int z = 0; z < 4; ++z) {
-        const int c = E4M3 ? x * 16 + 2 * g + (z >> 1) : x * 16 + g + 8 * (z >> 1);
-        all_o[(warp * 8 * NB + 8 * y + 2 * tig + (z & 1)) * C::PITCH + c] = o[x][y][z];
-      }
+        for (int z = 0; z < 4; ++z) {
+          const int c = E4M3 ? x * 16 + 2 * g + (z >> 1) : x * 16 + g + 8 * (z >> 1);
+          own[(8 * y + 2 * tig + (z & 1)) * DH + (c ^ tig << 3)] = o[x][y][z];
+        }
+  }
+  if (lane == 0) area[warp] = last;
   if (g == 0) {
 #pragma unroll
     for (int y = 0; y < NB; ++y)
@@ -499,17 +639,19 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attend_kernel(const __gr
         ml[warp][8 * y + 2 * tig + z] = make_float2(m[y][z] == -INFINITY ? -INFINITY : m[y][z] * factor[y][z], l[y][z]);
   }
   __syncthreads();
+  const long long slot = a.shares ? (long long)blockIdx.x + (long long)b * a.units() + at.unit : 0;
   constexpr int per = DH / 8;
-  for (int i = threadIdx.x; i < rows * per; i += kWarps * 32) {
-    const int r = i / per, c = (i - r * per) * 8;
+  for (int e = threadIdx.x; e < rows * per; e += kWarps * 32) {
+    const int r = e / per, c = (e - r * per) * 8;
     float top = -INFINITY, sum = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = max3(top, ml[w][r].x, ml[w][r].x);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
+      if (area[w] < 0) continue;
       const float mw = ml[w][r].x, k = mw == top ? 1.f : exp2_hw(mw - top);
       sum = fmaf(k, ml[w][r].y, sum);
-      const float4* src = reinterpret_cast<const float4*>(all_o + (w * 8 * NB + r) * C::PITCH + c);
+      const float4* src = reinterpret_cast<const float4*>(smem + area[w]) + (r * DH + (c ^ (r >> 1 & 3) << 3)) / 4;
       const float4 x = src[0], y = src[1];
       const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
@@ -521,22 +663,20 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attend_kernel(const __gr
     for (int u = 0; u < 8; ++u) f[u] = none ? 0.f : f[u] * inv;
     const float log_sum = none ? -INFINITY : top - lift + log2f(sum);
     const Row w(a, kvh, r0 + r);
-    const long long rr = ((long long)b * a.H + w.h) * a.Tq + w.t;
-    if (a.splits > 1) {
-      if (!none) store8(a.part_o, SB_F32, (split * a.all_rows + rr) * DH + c, f);
-      if (c == 0) a.part_l[split * a.all_rows + rr] = log_sum;
+    if (a.shares && !whole) {
+      store8(a.part_o, SB_F32, (slot * a.part_rows + r) * DH + c, f);
     } else {
       store8(a.o.p, a.q_bf16 ? SB_BF16 : SB_F16, b * a.o.img + w.t * a.o.row + (long long)w.h * DH + c, f);
-      if (c == 0) {
-        if (a.lse) a.lse[rr] = log_sum * 0.69314718055994531f;
-        if (a.log_sum) a.log_sum[rr] = log_sum;
-        fin[r] = log_sum;
-      }
+      if (c == 0 && a.lse) a.lse[((long long)b * a.H + w.h) * a.Tq + w.t] = log_sum * 0.69314718055994531f;
+    }
+    if (c == 0) {
+      if (a.ends > 0) a.part_l[(a.shares ? slot : (long long)b * a.units() + at.unit) * a.part_rows + r] = log_sum;
+      fin[r] = log_sum;
     }
   }
-  if (a.weight && a.splits == 1 && a.blocks == 1) {  // all of the scores and sums are this CTA's own
-    __syncthreads();
-    float* weight = a.weight + (long long)unit * a.pages.cap;
+  __syncthreads();
+  if (a.weight && a.ends == 0) {  // all of the scores and sums are this CTA's own
+    float* weight = a.weight + ((long long)b * a.Hkv + kvh) * a.pages.cap;
     for (int j = threadIdx.x; j < count; j += kWarps * 32) {
       float w = 0.f;
       for (int r = 0; r < rows; ++r)
@@ -544,105 +684,197 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attend_kernel(const __gr
       weight[j] = fmaf(a.decay, weight[j], w);
     }
   }
+    if (some) {
+      copy(i - 1 + C::STAGES);
+      ask();
+      __syncwarp();
+    }
+    done += piece;
+    if (done < left) at.advance(a, piece);
+  } while (done < left);
+  copies_wait<0>();
 }
 
-// Joins the splits' rows: out = sum_s 2^(L_s - L) O_s, L = log2 sum_s 2^L_s.  A warp takes a row: its lanes
-// find the largest L_s, then take eight channels each of several splits at once.  A split without states
-// (L_s = -inf) has not written its O_s.
+// What is left after the last piece, a CTA a part of an (item, key head): its share of the rows is joined from the
+// unit's pieces,
+//   out = sum_s 2^(L_s - L) O_s,  L = log2 sum_s 2^L_s,
+// and its share of the states gets its account, weight = decay weight + sum over the rows of 2^(score - L).  Every CTA
+// finds L of the rows by itself, 16 at a time.  A unit in one piece has its rows already, one without states gets
+// zeros.
+constexpr int kEndThreads = 256, kEndOcc = 4, kEndEach = 4;  // threads, CTAs an SM, states a thread at once
+
 template <int DH>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a) {
-  constexpr int per = DH / 8, lanes = 32 / per;  // threads of a split's row, splits at once
-  const int lane = lane_id();
-  const long long rr = (long long)blockIdx.x * 4 + warp_id();
-  if (rr >= a.all_rows) return;
-  float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 32) {
-    const float u = a.part_l[s * a.all_rows + rr];
-    top = max3(top, u, u);
-  }
+__global__ void __launch_bounds__(kEndThreads, kEndOcc) paged_end_kernel(const __grid_constant__ PagedArgs a) {
+  constexpr int per = DH / 8, at_once = kEndThreads / per;  // threads of a piece's row, pieces at once
+  __shared__ float fin[16];
+  __shared__ float part[at_once][DH + 4];
+  __shared__ long long room[kEndThreads / 32 + 2];
+  __shared__ int found;
+  const int warp = warp_id(), lane = lane_id();
+  const int p = blockIdx.x % a.ends, head = blockIdx.x / a.ends;
+  const int b = head / a.Hkv, kvh = head - b * a.Hkv;
+  const int count = a.pages.clamp(a.lens[b]), n = a.chunks(b);
+  // this CTA's states
+  const int share = (count + a.ends - 1) / a.ends, j_first = min(p * share, count), j_end = min(j_first + share, count);
+  // pieces of a unit: slots first .. first + pieces - 1
+  Shares s{};
+  if (a.shares) s = look_up<kEndThreads>(a, 0, b, room, found);
+  grid_dep_wait();
+  for (int block = 0; block < a.blocks; ++block) {
+    const int r0 = block * 16, rows = min(16, a.rows - r0), unit = kvh * a.blocks + block;
+    long long first = (long long)b * a.units() + unit;
+    int pieces = 1;
+    if (a.shares) {
+      const long long from = s.before * a.units() + (long long)unit * n;
+      pieces = n == 0 ? 0 : (int)((from + n - 1) / s.each - from / s.each) + 1;
+      first += from / s.each;
+    }
+    __syncthreads();
+    for (int r = warp; r < rows; r += kEndThreads / 32) {
+      float top = -INFINITY, sum = 0.f;
+      for (int x = lane; x < pieces; x += 32) {
+        const float u = a.part_l[(first + x) * a.part_rows + r], t = max3(top, u, u);
+        if (t != -INFINITY) sum = sum * (top == t ? 1.f : exp2_hw(top - t)) + (u == t ? 1.f : exp2_hw(u - t));
+        top = t;
+      }
 #pragma unroll
-  for (int x = 16; x; x >>= 1) {
-    const float u = __shfl_xor_sync(0xFFFFFFFFu, top, x);
-    top = max3(top, u, u);
-  }
-  const int c = lane % per * 8, s0 = lane / per;
-  float f[9] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // channels, sum of weights
-#pragma unroll 4
-  for (int s = s0; s < a.splits; s += lanes) {
-    const float ls = a.part_l[s * a.all_rows + rr];
-    if (ls == -INFINITY) continue;
-    const float w = exp2_hw(ls - top);
-    float v[8];
-    unpack8(load_raw8(a.part_o, SB_F32, (s * a.all_rows + rr) * DH + c), SB_F32, v);
+      for (int x = 16; x; x >>= 1) {
+        const float u = __shfl_xor_sync(0xFFFFFFFFu, top, x), y = __shfl_xor_sync(0xFFFFFFFFu, sum, x), t = max3(top, u, u);
+        if (t != -INFINITY) sum = sum * (top == t ? 1.f : exp2_hw(top - t)) + y * (u == t ? 1.f : exp2_hw(u - t));
+        top = t;
+      }
+      if (lane == 0) fin[r] = top == -INFINITY ? -INFINITY : top + log2f(sum);
+    }
+    __syncthreads();
+    if (pieces != 1) {
+      for (int r = (p + a.ends - r0 % a.ends) % a.ends; r < rows; r += a.ends) {  // rows p, p + ends, ... of all
+        const float l = fin[r];
+        const int c = threadIdx.x % per * 8;
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+        for (int x = threadIdx.x / per; x < pieces; x += at_once) {
+          const float ls = a.part_l[(first + x) * a.part_rows + r];
+          if (ls == -INFINITY) continue;
+          const float k = exp2_hw(ls - l);
+          float v[8];
+          unpack8(load_raw8(a.part_o, SB_F32, ((first + x) * a.part_rows + r) * DH + c), SB_F32, v);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) f[u] = fmaf(w, v[u], f[u]);
-    f[8] += w;
-  }
+          for (int u = 0; u < 8; ++u) f[u] = fmaf(k, v[u], f[u]);
+        }
+        float4* to = reinterpret_cast<float4*>(&part[threadIdx.x / per][c]);
+        to[0] = make_float4(f[0], f[1], f[2], f[3]);
+        to[1] = make_float4(f[4], f[5], f[6], f[7]);
+        __syncthreads();
+        if (threadIdx.x < DH / 2) {  // two channels a thread
+          float x = 0.f, y = 0.f;
+          const int some = min(at_once, pieces);
+          for (int z = 0; z < some; ++z) {
+            x += part[z][2 * threadIdx.x];
+            y += part[z][2 * threadIdx.x + 1];
+          }
+          const Row q(a, kvh, r0 + r);
+          uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o.p) + b * a.o.img + q.t * a.o.row + (long long)q.h * DH);
+          o[threadIdx.x] = pack_pair(x, y, a.q_bf16 ? SB_BF16 : SB_F16);
+          if (threadIdx.x == 0 && a.lse) a.lse[((long long)b * a.H + q.h) * a.Tq + q.t] = l * 0.69314718055994531f;
+        }
+        __syncthreads();
+      }
+    }
+    if (!a.weight) continue;
+    float* const weight = a.weight + (long long)head * a.pages.cap;
+    const float* const scores = a.scores + (long long)head * a.pages.cap * a.rows + r0;
+    const bool vec = a.rows % 4 == 0;
+    for (int j = j_first + (int)threadIdx.x; j < j_end; j += kEndThreads * kEndEach) {
+      float w[kEndEach];
 #pragma unroll
-  for (int x = per; x < 32; x <<= 1)
+      for (int x = 0; x < kEndEach; ++x) w[x] = j + x * kEndThreads < j_end ? weight[j + x * kEndThreads] : 0.f;
+      if (block == 0)
 #pragma unroll
-    for (int u = 0; u < 9; ++u) f[u] += __shfl_xor_sync(0xFFFFFFFFu, f[u], x);
-  if (s0 != 0) return;
-  const float inv = f[8] != 0.f ? 1.f / f[8] : 0.f;
-  float v[8];
+        for (int x = 0; x < kEndEach; ++x) w[x] *= a.decay;
+      if (vec) {
+        for (int r = 0; r < rows; r += 4) {
+          float4 v[kEndEach];
 #pragma unroll
-  for (int u = 0; u < 8; ++u) v[u] = f[u] * inv;
-  const int t = (int)(rr % a.Tq), h = (int)(rr / a.Tq % a.H);
-  const long long b = rr / a.Tq / a.H;
-  store8(a.o.p, a.q_bf16 ? SB_BF16 : SB_F16, b * a.o.img + t * a.o.row + (long long)h * DH + c, v);
-  if (c == 0) {
-    const float log_sum = f[8] != 0.f ? top + log2f(f[8]) : -INFINITY;
-    if (a.lse) a.lse[rr] = log_sum * 0.69314718055994531f;
-    if (a.log_sum) a.log_sum[rr] = log_sum;
+          for (int x = 0; x < kEndEach; ++x)
+            if (j + x * kEndThreads < j_end)
+              v[x] = *reinterpret_cast<const float4*>(scores + (long long)(j + x * kEndThreads) * a.rows + r);
+          const float l[4] = {fin[r], fin[r + 1], fin[r + 2], fin[r + 3]};
+#pragma unroll
+          for (int x = 0; x < kEndEach; ++x) {
+            const float u[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) w[x] += l[y] == -INFINITY ? 0.f : exp2_hw(u[y] - l[y]);
+          }
+        }
+      } else {
+        for (int r = 0; r < rows; ++r) {
+          float v[kEndEach];
+#pragma unroll
+          for (int x = 0; x < kEndEach; ++x)
+            if (j + x * kEndThreads < j_end) v[x] = scores[(long long)(j + x * kEndThreads) * a.rows + r];
+          const float l = fin[r];
+#pragma unroll
+          for (int x = 0; x < kEndEach; ++x) w[x] += l == -INFINITY ? 0.f : exp2_hw(v[x] - l);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kEndEach; ++x)
+        if (j + x * kEndThreads < j_end) weight[j + x * kEndThreads] = w[x];
+    }
   }
 }
 
-// weight = decay weight + sum over the rows of 2^(score - L): a thread a state.
-__global__ void __launch_bounds__(256) paged_account_kernel(const __grid_constant__ PagedArgs a) {
-  const int parts = (a.pages.cap + 255) / 256;
-  const int unit = blockIdx.x / parts, j = (blockIdx.x - unit * parts) * 256 + threadIdx.x;
-  const int b = unit / a.Hkv, kvh = unit - b * a.Hkv;
-  if (j >= a.pages.clamp(a.lens[b])) return;
-  const float* s = a.scores + ((long long)unit * a.pages.cap + j) * a.rows;
-  float w = 0.f;
-  for (int r = 0; r < a.rows; ++r) {
-    const Row q(a, kvh, r);
-    const float l = a.log_sum[((long long)b * a.H + q.h) * a.Tq + q.t];
-    if (l != -INFINITY) w += exp2_hw(s[r] - l);
-  }
-  float* to = a.weight + (long long)unit * a.pages.cap + j;
-  *to = fmaf(a.decay, *to, w);
+template <int DH, int PT>
+void shape_of(int rows, int& chunk, int& occ) {
+  chunk = rows <= 8 ? Paged<DH, PT, 1>::CK : Paged<DH, PT, 2>::CK;
+  occ = rows <= 8 ? Paged<DH, PT, 1>::OCC : Paged<DH, PT, 2>::OCC;
+}
+template <int DH>
+void shape_of(int pt, int rows, int& chunk, int& occ) {
+  return pt == SB_F8     ? shape_of<DH, SB_F8>(rows, chunk, occ)
+         : pt == SB_BF16 ? shape_of<DH, SB_BF16>(rows, chunk, occ) : shape_of<DH, SB_F16>(rows, chunk, occ);
 }
 
 struct PagedPlan {
-  int rows, blocks, splits;
-  bool apart;  // the account by a kernel of its own
-  long long units, scores, part_o, part_l, sums;  // floats of the workspace
-  long long bytes() const { return (scores + part_o + part_l + sums) * 4; }
+  int rows, blocks, shares, ends, chunk, part_rows;
+  long long units, scores, part_o, part_l;  // floats of the workspace
+  long long bytes() const { return (scores + part_o + part_l) * 4; }
 };
 
-PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int cap, bool account, int sms) {
+// A CTA a unit where a unit is small (256 KB of places: a few us, and the call is one kernel) or the units alone
+// fill the SMs eight times; else as many CTAs as are resident at once share all chunks evenly, whatever the
+// items' lengths, and a second kernel joins the pieces.
+PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int pt, int cap, bool account, int sms) {
   PagedPlan p{};
+  int occ;
   p.rows = H / Hkv * Tq;
+  if (dh == 32) shape_of<32>(pt, p.rows, p.chunk, occ);
+  else if (dh == 64) shape_of<64>(pt, p.rows, p.chunk, occ);
+  else shape_of<128>(pt, p.rows, p.chunk, occ);
   p.blocks = (p.rows + 15) / 16;
+  p.part_rows = std::min(p.rows, 16);
   p.units = (long long)B * Hkv * p.blocks;
-  p.splits = few_splits(p.units, cap, sms);
-  p.apart = account && (p.splits > 1 || p.blocks > 1);
-  const long long all = (long long)B * H * Tq;
+  const bool apart = 2ll * cap * dh * page_dtype_bytes(pt) > 256 * 1024 && p.units < 8ll * occ * sms;
+  p.shares = apart ? occ * sms : 0;
+  account = account && cap > 0;
+  // one wave of the last kernel's CTAs, each with 256 places or a row
+  const long long heads = (long long)B * Hkv, wave = ((long long)kEndOcc * sms + heads - 1) / std::max(heads, 1ll);
+  if (account && (apart || p.blocks > 1)) p.ends = (int)std::min(wave, ((long long)cap + 255) / 256);
+  else if (apart) p.ends = (int)std::min(wave, (long long)p.rows);
   auto even = [](long long n) { return (n + 3) / 4 * 4; };
   p.scores = account ? even((long long)B * Hkv * cap * p.rows) : 0;
-  p.part_o = p.splits > 1 ? p.splits * all * dh : 0;
-  p.part_l = p.splits > 1 ? even(p.splits * all) : 0;
-  p.sums = p.apart ? even(all) : 0;
+  const long long slots = p.units + p.shares;
+  p.part_o = apart ? slots * p.part_rows * dh : 0;
+  p.part_l = p.ends > 0 ? even(slots * p.part_rows) : 0;
   return p;
 }
 
 template <int DH, int PT, int NB>
 cudaError_t launch(const PagedArgs& a, long long ctas, cudaStream_t st) {
   static bool ready[64];
-  const cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&paged_attend_kernel<DH, PT, NB>), Paged<DH, PT>::SMEM, ready);
+  const cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&paged_attend_kernel<DH, PT, NB>), Paged<DH, PT, NB>::SMEM, ready);
   if (e != cudaSuccess) return e;
-  paged_attend_kernel<DH, PT, NB><<<(unsigned)ctas, kWarps * 32, Paged<DH, PT>::SMEM, st>>>(a);
+  paged_attend_kernel<DH, PT, NB><<<(unsigned)ctas, kWarps * 32, Paged<DH, PT, NB>::SMEM, st>>>(a);
   return cudaGetLastError();
 }
 template <int DH, int PT>
@@ -650,12 +882,10 @@ cudaError_t launch(const PagedArgs& a, long long ctas, cudaStream_t st) {
   return a.rows <= 8 ? launch<DH, PT, 1>(a, ctas, st) : launch<DH, PT, 2>(a, ctas, st);
 }
 template <int DH>
-cudaError_t launch(const PagedArgs& a, int pt, long long ctas, cudaStream_t st) {
+cudaError_t launch(const PagedArgs& a, int pt, long long ctas, long long ends, cudaStream_t st) {
   const cudaError_t e = pt == SB_F8     ? launch<DH, SB_F8>(a, ctas, st)
                         : pt == SB_BF16 ? launch<DH, SB_BF16>(a, ctas, st) : launch<DH, SB_F16>(a, ctas, st);
-  if (e != cudaSuccess || a.splits == 1) return e;
-  paged_join_kernel<DH><<<(unsigned)((a.all_rows + 3) / 4), 128, 0, st>>>(a);
-  return cudaGetLastError();
+  return e != cudaSuccess || ends == 0 ? e : launch_after(paged_end_kernel<DH>, ends, kEndThreads, 0, st, a);
 }
 
 bool paged_attention_sizes_ok(int B, int H, int Hkv, int dh, int Tq, int P, int page, int N) {
@@ -668,50 +898,47 @@ bool paged_attention_sizes_ok(int B, int H, int Hkv, int dh, int Tq, int P, int 
 
 using namespace sb;
 
-extern "C" int sb_paged_attention_work(int B, int H, int Hkv, int dh, int Tq, int page, int N, int account, long long* bytes) {
-  if (!bytes || !paged_attention_sizes_ok(B, H, Hkv, dh, Tq, 0, page, N))
+extern "C" int sb_paged_attention_work(int B, int H, int Hkv, int dh, int Tq, int page_dtype, int page, int N, int account,
+                                       long long* bytes) {
+  if (!bytes || !paged_attention_sizes_ok(B, H, Hkv, dh, Tq, 0, page, N) || !page_dtype_ok(page_dtype))
     return record_error(SB_EINVAL, "sb_paged_attention_work: arguments");
   *bytes = 0;
   if (B == 0 || Tq == 0) return SB_OK;
   const int sms = xattn_sms();
   if (sms == 0) return record_error(SB_ECUDA, "sb_paged_attention_work: device");
-  *bytes = paged_plan(B, H, Hkv, dh, Tq, N * page, account != 0, sms).bytes();
+  *bytes = paged_plan(B, H, Hkv, dh, Tq, page_dtype, N * page, account != 0, sms).bytes();
   return SB_OK;
 }
 
-extern "C" int sb_paged_attention(const void* q, long long q_row, long long q_img, int q_dtype, const void* k_pages,
-                                  long long k_row, long long k_page, const void* v_pages, long long v_row,
-                                  long long v_page, int page_dtype, int P, int page, const int* table, long long table_row,
-                                  int N, const int* lens, int B, int H, int Hkv, int dh, int Tq, float scale, float k_scale,
-                                  float v_scale, int causal, void* out, long long o_row, long long o_img, float* lse,
-                                  float* weight, float decay, void* work, long long work_bytes, void* stream) {
-  if (!paged_attention_sizes_ok(B, H, Hkv, dh, Tq, P, page, N) || (q_dtype != SB_F16 && q_dtype != SB_BF16) ||
-      (page_dtype != q_dtype && page_dtype != SB_F8))
+extern "C" int sb_paged_attention(const sb_paged_memory* memory, const void* q, long long q_row, long long q_img, int q_dtype,
+                                  const int* lens, int H, int Tq, float scale, float k_scale, float v_scale, int causal,
+                                  void* out, long long o_row, long long o_img, float* lse, float* weight, float decay,
+                                  void* work, long long work_bytes, void* stream) {
+  const sb_paged_memory* const m = memory;
+  if (!paged_memory_ok(m) || !paged_attention_sizes_ok(m->B, H, m->Hkv, m->dh, Tq, m->P, m->page, m->N) ||
+      (q_dtype != SB_F16 && q_dtype != SB_BF16) || (m->dtype != q_dtype && m->dtype != SB_F8))
     return record_error(SB_EINVAL, "sb_paged_attention: sizes (dh 32, 64 or 128, H a multiple of Hkv) or dtypes");
-  if (!(scale > 0.f) || !std::isfinite(scale) || !(k_scale > 0.f) || !std::isfinite(k_scale) || !(v_scale > 0.f) ||
-      !std::isfinite(v_scale) || !std::isfinite(scale * k_scale) || (page_dtype != SB_F8 && (k_scale != 1.f || v_scale != 1.f)))
+  if (!(scale > 0.f) || !scales_ok(m, k_scale, v_scale) || !std::isfinite(scale * k_scale))
     return record_error(SB_EINVAL, "sb_paged_attention: scale, or scales of pages that are not e4m3");
   if (weight && !(decay >= 0.f && decay <= 1.f)) return record_error(SB_EINVAL, "sb_paged_attention: decay from 0 to 1");
-  if (B == 0 || Tq == 0) return SB_OK;
-  const int es = page_dtype_bytes(page_dtype);
-  const bool some = P > 0 && N > 0;  // states there may be
-  if (!lens || (N > 0 && (!table || table_row < 0)) || !xattn_view_ok(q, q_row, q_img) || !xattn_view_ok(out, o_row, o_img) ||
-      (some && (!pool_ok(k_pages, k_row, k_page, es) || !pool_ok(v_pages, v_row, v_page, es))))
+  if (m->B == 0 || Tq == 0) return SB_OK;
+  if (!lens || !xattn_view_ok(q, q_row, q_img) || !xattn_view_ok(out, o_row, o_img) || !paged_pools_ok(m))
     return record_error(SB_EINVAL, "sb_paged_attention: rows (16-byte aligned, strides multiples of 16 bytes) or null argument");
   const int sms = xattn_sms();
   if (sms == 0) return record_error(SB_ECUDA, "sb_paged_attention: device");
-  const PagedPlan p = paged_plan(B, H, Hkv, dh, Tq, N * page, weight != nullptr, sms);
+  PagedArgs a{};
+  a.pages = page_table(m);
+  const PagedPlan p = paged_plan(m->B, H, m->Hkv, m->dh, Tq, m->dtype, a.pages.cap, weight != nullptr, sms);
   if (p.bytes() > 0 && (!work || work_bytes < p.bytes() || (reinterpret_cast<uintptr_t>(work) & 15) != 0))
     return record_error(SB_EINVAL, "sb_paged_attention: workspace (sb_paged_attention_work bytes, 16-byte aligned)");
-  const long long ctas = p.units * p.splits, parts = (N * (long long)page + 255) / 256 * B * Hkv;
-  if (ctas > 0x7FFFFFFFll || parts > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_paged_attention: too many items");
-  PagedArgs a{};
+  const long long ctas = p.shares ? p.shares : p.units, ends = (long long)p.ends * m->B * m->Hkv;
+  if (ctas > 0x7FFFFFFFll || ends > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_paged_attention: too many items");
   a.q = q; a.q_row = q_row; a.q_img = q_img;
-  a.k = pool_of(k_pages, k_row, k_page, es);
-  a.v = pool_of(v_pages, v_row, v_page, es);
-  a.pages = page_table(table, table_row, P, page, N);
+  a.k = k_pool(m);
+  a.v = v_pool(m);
   a.lens = lens;
-  a.B = B; a.H = H; a.Hkv = Hkv; a.group = H / Hkv; a.Tq = Tq; a.rows = p.rows; a.blocks = p.blocks; a.splits = p.splits;
+  a.B = m->B; a.H = H; a.Hkv = m->Hkv; a.group = H / m->Hkv; a.Tq = Tq;
+  a.rows = p.rows; a.blocks = p.blocks; a.shares = p.shares; a.ends = p.ends; a.chunk = p.chunk; a.part_rows = p.part_rows;
   a.q_bf16 = q_dtype == SB_BF16; a.causal = causal != 0;
   a.scale_log2 = scale * k_scale * 1.4426950408889634f;
   a.v_scale = v_scale;
@@ -719,18 +946,12 @@ extern "C" int sb_paged_attention(const void* q, long long q_row, long long q_im
   a.lse = lse;
   a.weight = p.scores > 0 ? weight : nullptr;  // (no places: no account)
   a.decay = decay;
-  a.all_rows = (long long)B * H * Tq;
   float* w = static_cast<float*>(work);
   a.scores = p.scores > 0 ? w : nullptr;
   a.part_o = w + p.scores;
   a.part_l = a.part_o + p.part_o;
-  a.log_sum = p.sums > 0 ? a.part_l + p.part_l : nullptr;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = dh == 32   ? launch<32>(a, page_dtype, ctas, st)
-                  : dh == 64 ? launch<64>(a, page_dtype, ctas, st) : launch<128>(a, page_dtype, ctas, st);
-  if (e == cudaSuccess && p.apart && parts > 0) {
-    paged_account_kernel<<<(unsigned)parts, 256, 0, st>>>(a);
-    e = cudaGetLastError();
-  }
+  const cudaError_t e = m->dh == 32   ? launch<32>(a, m->dtype, ctas, ends, st)
+                        : m->dh == 64 ? launch<64>(a, m->dtype, ctas, ends, st) : launch<128>(a, m->dtype, ctas, ends, st);
   return e == cudaSuccess ? SB_OK : record_error(SB_ECUDA, cudaGetErrorString(e));
 }

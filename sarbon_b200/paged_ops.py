@@ -27,12 +27,15 @@ capture.  No graph of gradients is recorded; tensors that would need one are ref
 """
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from . import _lib
 from .memory_ops import _HALVES, _INF, _apart, _launch, _new, _ready, _rows, _statistics, _work
 
 E4M3 = torch.float8_e4m3fn
+_MEMORY = struct.Struct("@PPqqqqPqiiiiiii4x")  # sb_paged_memory
 PAGE_DTYPES = {torch.float16: _lib.SB_F16, torch.bfloat16: _lib.SB_BF16, E4M3: _lib.SB_F8}
 
 
@@ -61,7 +64,7 @@ def _own_pool(pool, what, shape):
 
 
 def _memory(k_pages, v_pages, table, kv_heads, written=False):
-    """The arguments that every call has: (pools and table for the library, batch, page, entries, dim)."""
+    """The memory of a call: (sb_paged_memory, batch, page, entries, dim)."""
     if k_pages.dim() != 3 or k_pages.dtype not in PAGE_DTYPES:
         raise ValueError("k_pages, v_pages: [P, page, kv_heads * dim] pools of fp16, bf16 or e4m3")
     shape, dtype = k_pages.shape, k_pages.dtype
@@ -78,8 +81,9 @@ def _memory(k_pages, v_pages, table, kv_heads, written=False):
     b, n = table.shape
     if n * page >= 1 << 30:
         raise ValueError("table: fewer than 2^30 states an item")
-    return (*kp, *vp, PAGE_DTYPES[dtype], pages, page, table.data_ptr(), table.stride(0) if b > 1 else n, n), b, page, n, \
-        width // kv_heads
+    dim = width // kv_heads
+    return _MEMORY.pack(kp[0], vp[0], kp[1], kp[2], vp[1], vp[2], table.data_ptr(), table.stride(0) if b > 1 else n,
+                        PAGE_DTYPES[dtype], pages, page, n, b, kv_heads, dim), b, page, n, dim
 
 
 def _each(t, what, b):
@@ -168,10 +172,10 @@ def paged_attention(q, k_pages, v_pages, table, lens, heads, kv_heads=None, scal
         out, op = _new(q, shape, dtype)
     if b == 0 or tq == 0:
         return out
-    hold, work, size = _work("sb_paged_attention_work", index, b, heads, kv_heads, dim, tq, page, n, weight is not None)
-    _launch("sb_paged_attention", index, *qp, _lib.SB_BF16 if dtype == torch.bfloat16 else _lib.SB_F16, *memory, p_lens, b,
-            heads, kv_heads, dim, tq, scale, k_scale, v_scale, causal, *op, None if lse is None else lse.data_ptr(), p_weight,
-            decay, work, size)
+    hold, work, size = _work("sb_paged_attention_work", index, b, heads, kv_heads, dim, tq, PAGE_DTYPES[k_pages.dtype], page, n,
+                             weight is not None)
+    _launch("sb_paged_attention", index, memory, *qp, PAGE_DTYPES[dtype], p_lens, heads, tq, scale, k_scale, v_scale, causal, *op,
+            None if lse is None else lse.data_ptr(), p_weight, decay, work, size)
     return out
 
 
@@ -224,8 +228,8 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
         p_after = after.data_ptr()
     if b == 0:
         return after
-    _launch("sb_paged_write", index, *kp, *vp, _lib.SB_BF16 if dtype == torch.bfloat16 else _lib.SB_F16, *memory, p_at,
-            p_count, b, t, kv_heads, dim, k_scale, v_scale, p_weight, p_born, *sp, p_after)
+    _launch("sb_paged_write", index, memory, *kp, *vp, PAGE_DTYPES[dtype], p_at, p_count, t, k_scale, v_scale, p_weight, p_born,
+            *sp, p_after)
     return after
 
 
@@ -280,6 +284,5 @@ def paged_evict(k_pages, v_pages, table, lens, weight, keep, born=None, since=No
     if b == 0:
         return after, weight_out, born_out
     hold, work, size = _work("sb_paged_evict_work", index, b, kv_heads, page, n)
-    _launch("sb_paged_evict", index, *memory, p_lens, p_keep, keep_all, p_since, b, kv_heads, dim, pw, pb, pwo, pbo, p_after,
-            work, size)
+    _launch("sb_paged_evict", index, memory, p_lens, p_keep, keep_all, p_since, pw, pb, pwo, pbo, p_after, work, size)
     return after, weight_out, born_out

@@ -102,39 +102,41 @@ def test_autograd_inputs_are_refused():
 
 def test_library_refuses():
     """The C entries turn down what the wrappers never pass, before any device call."""
-    lib, n, one, two = _lib.lib(), C.c_longlong(0), C.c_void_p(16), C.c_void_p(32)
+    from sarbon_b200.paged_ops import _MEMORY
+    lib, n, one = _lib.lib(), C.c_longlong(0), C.c_void_p(16)
 
-    def attention(q=one, row=64, qt=0, pt=0, kp=one, kr=64, p=4, page=4, table=one, tr=2, nn=2, lens=one, b=1, h=2, hkv=1, dh=32,
-                  tq=1, scale=1.0, ks=1.0, weight=None, decay=1.0, work=None, size=0):
-        return lib.sb_paged_attention(q, row, 64, qt, kp, kr, 256, two, kr, 256, pt, p, page, table, tr, nn, lens, b, h, hkv, dh, tq,
-                                      scale, ks, 1.0, 0, one, row, 64, None, weight, decay, work, size, None)
+    def memory(kp=16, vp=32, kr=64, pt=0, p=4, page=4, table=16, tr=2, nn=2, b=1, hkv=1, dh=32):
+        return _MEMORY.pack(kp, vp, kr, 256, kr, 256, table, tr, pt, p, page, nn, b, hkv, dh)
 
-    for bad in (dict(qt=1), dict(qt=2), dict(pt=3), dict(pt=1), dict(dh=48), dict(h=3, hkv=2), dict(hkv=0), dict(tq=-1), dict(b=-1),
-                dict(page=0), dict(p=-1), dict(nn=-1), dict(page=1 << 20, nn=1 << 10), dict(scale=0.0), dict(scale=float("nan")),
-                dict(ks=2.0), dict(pt=2, ks=0.0), dict(pt=2, scale=1e30, ks=1e30), dict(weight=one, decay=2.0), dict(q=None),
-                dict(q=C.c_void_p(8)), dict(row=60), dict(kr=60), dict(kr=-8), dict(kp=None), dict(kp=C.c_void_p(8)),
-                dict(table=None), dict(tr=-1), dict(lens=None)):
+    wrong = [dict(pt=1), dict(dh=48), dict(hkv=0), dict(b=-1), dict(page=0), dict(p=-1), dict(nn=-1), dict(page=1 << 20, nn=1 << 10),
+             dict(kr=60), dict(kr=-8), dict(kp=0), dict(vp=0), dict(kp=8), dict(table=0), dict(tr=-1), None]
+
+    def attention(m=memory(), q=one, row=64, qt=0, lens=one, h=2, tq=1, scale=1.0, ks=1.0, weight=None, decay=1.0, work=None, size=0):
+        return lib.sb_paged_attention(m, q, row, 64, qt, lens, h, tq, scale, ks, 1.0, 0, one, row, 64, None, weight, decay, work, size, None)
+
+    def write(m=memory(), k=one, dt=0, ks=1.0, at=one, after=one, t=1, kr=32):
+        return lib.sb_paged_write(m, k, kr, 32, one, kr, 32, dt, at, None, t, ks, 1.0, None, None, None, 0, 0, after, None)
+
+    def evict(m=memory(), lens=one, weight=one, since=None, born=None, born_out=None, work=one, size=1 << 20):
+        return lib.sb_paged_evict(m, lens, None, 2, since, weight, born, weight, born_out, one, work, size, None)
+
+    e4m3 = memory(pt=_lib.SB_F8)
+    for call in (attention, write, evict):
+        for change in wrong:
+            assert call(m=None if change is None else memory(**change)) == _lib.SB_EINVAL, (call, change)
+        assert call(m=memory(b=0)) == _lib.SB_OK
+    for bad in (dict(qt=1), dict(qt=2), dict(qt=3), dict(h=0), dict(m=memory(hkv=2), h=3), dict(tq=-1), dict(scale=0.0),
+                dict(scale=float("nan")), dict(ks=2.0), dict(m=e4m3, ks=0.0), dict(m=e4m3, scale=1e30, ks=1e30),
+                dict(weight=one, decay=2.0), dict(q=None), dict(q=C.c_void_p(8)), dict(row=60), dict(lens=None)):
         assert attention(**bad) == _lib.SB_EINVAL, bad
-    assert attention(b=0) == _lib.SB_OK and attention(tq=0) == _lib.SB_OK
-    assert lib.sb_paged_attention_work(1, 2, 1, 48, 1, 4, 2, 0, C.byref(n)) == _lib.SB_EINVAL
-    assert lib.sb_paged_attention_work(1, 2, 1, 32, 1, 0, 2, 0, C.byref(n)) == _lib.SB_EINVAL
-    assert lib.sb_paged_evict_work(1, 0, 4, 2, C.byref(n)) == _lib.SB_EINVAL
-    assert lib.sb_paged_evict_work(3, 2, 4, 2, C.byref(n)) == _lib.SB_OK and n.value > 0
-
-    def write(k=one, pt=0, dt=0, kp=one, ks=1.0, at=one, after=one, b=1, t=1, dh=32, kr=32, pr=32):
-        return lib.sb_paged_write(k, kr, 32, one, kr, 32, dt, kp, pr, 128, two, pr, 128, pt, 4, 4, one, 2, 2, at, None, b, t, 1, dh, ks,
-                                  1.0, None, None, None, 0, 0, after, None)
-
-    for bad in (dict(k=None), dict(dt=1), dict(pt=3), dict(kp=None), dict(kp=C.c_void_p(8)), dict(ks=2.0), dict(pt=2, ks=-1.0),
-                dict(at=None), dict(after=None), dict(b=-1), dict(t=-1), dict(dh=16), dict(kr=-1), dict(pr=20)):
+    assert attention(tq=0) == _lib.SB_OK
+    for bad in (dict(k=None), dict(dt=1), dict(dt=3), dict(ks=2.0), dict(m=e4m3, ks=-1.0), dict(at=None), dict(after=None), dict(t=-1),
+                dict(kr=-1)):
         assert write(**bad) == _lib.SB_EINVAL, bad
-    assert write(b=0) == _lib.SB_OK
-
-    def evict(kp=one, pt=0, lens=one, weight=one, since=None, born=None, born_out=None, work=one, size=1 << 20, b=1, dh=32):
-        return lib.sb_paged_evict(kp, 32, 128, two, 32, 128, pt, 4, 4, one, 2, 2, lens, None, 2, since, b, 1, dh, weight, born, weight,
-                                  born_out, one, work, size, None)
-
-    for bad in (dict(kp=None), dict(pt=1), dict(lens=None), dict(weight=None), dict(since=one), dict(born=one), dict(born_out=one),
-                dict(work=None), dict(work=C.c_void_p(8)), dict(size=4), dict(b=-1), dict(dh=16)):
+    for bad in (dict(lens=None), dict(weight=None), dict(since=one), dict(born=one), dict(born_out=one), dict(work=None),
+                dict(work=C.c_void_p(8))):
         assert evict(**bad) == _lib.SB_EINVAL, bad
-    assert evict(b=0) == _lib.SB_OK
+    assert lib.sb_paged_attention_work(1, 2, 1, 48, 1, 0, 4, 2, 0, C.byref(n)) == _lib.SB_EINVAL
+    assert lib.sb_paged_attention_work(1, 2, 1, 32, 1, 0, 0, 2, 0, C.byref(n)) == _lib.SB_EINVAL
+    assert lib.sb_paged_attention_work(1, 2, 1, 32, 1, 1, 4, 2, 0, C.byref(n)) == _lib.SB_EINVAL
+    assert lib.sb_paged_evict_work(1, 0, 4, 2, C.byref(n)) == _lib.SB_EINVAL
