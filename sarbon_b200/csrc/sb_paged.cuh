@@ -51,6 +51,16 @@ SB_DEV uint32_t peer_word(const void* p, uint32_t rank) {
   return v;
 }
 
+// 16 bytes of it (at a multiple of 16).
+SB_DEV uint4 peer_words(const void* p, uint32_t rank) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(mapa_shared(smem_u32(p), rank))
+               : "memory");
+  return v;
+}
+
 // A launch whose CTAs may start while the kernel before them on the stream ends; they call grid_dep_wait() before they
 // read what it wrote.  cluster: CTAs that share their memory (1: none).
 template <class Args>

@@ -39,12 +39,16 @@ struct PagedArgs {
   float* lse;
   float* weight;
   float decay;
-  float* scores;  // [B * Hkv][cap][rows], log2 units
+  float* scores;  // [B * Hkv][blocks][places][score_rows], log2 units
+  int places, score_rows;  // cap and a block's rows, up to a multiple of 4 and a power of two
   float* part_o;  // [slots][part_rows][dh]
   float* part_l;  // [slots][part_rows], log2 of the sum
   int part_rows;  // min(rows, 16)
   SB_DEV int chunks(int b) const { return (pages.clamp(lens[b]) + chunk - 1) / chunk; }
   SB_DEV int units() const { return Hkv * blocks; }  // of an item
+  SB_DEV float* plane(int head, int block) const {
+    return scores + ((long long)head * blocks + block) * places * score_rows;
+  }
 };
 
 // How the chunks of all units, one unit after the other, are shared: CTA i gets `each` of them from i * each on.  What
@@ -378,7 +382,7 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_att
 #pragma unroll
     for (int x = 0; x < KS; ++x) o[x][y][0] = o[x][y][1] = o[x][y][2] = o[x][y][3] = 0.f;
   }
-  float* const scores = a.scores ? a.scores + ((long long)b * a.Hkv + kvh) * a.pages.cap * a.rows + r0 : nullptr;
+  float* const scores = a.scores ? a.plane(b * a.Hkv + kvh, block) : nullptr;
   const int chunk0 = at.c - (int)done;  // of the unit: chunk0 + warp + i * kWarps
 
   const int i_first = i;
@@ -435,22 +439,19 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_att
         }
     }
     if (scores) {
-      float* to8 = scores + (long long)(j0 + g) * a.rows + 2 * tig;  // of every eighth state
+      float* to8 = scores + (long long)(j0 + g) * a.score_rows + 2 * tig;  // of every eighth state
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int x = 0; x < 2; ++x, to8 += 8 * a.rows) {
+        for (int x = 0; x < 2; ++x, to8 += 8 * a.score_rows) {
           if (j0 + kt * 16 + 8 * x + g < count) {
 #pragma unroll
             for (int y = 0; y < NB; ++y) {
-              const int r = 8 * y + 2 * tig;
-              float* to = to8 + 8 * y;
               const float u = s[kt][y][2 * x] * factor[y][0], w = s[kt][y][2 * x + 1] * factor[y][1];
-              if (a.rows % 2 == 0) {
-                if (r < rows) *reinterpret_cast<float2*>(to) = make_float2(u, w);
-              } else {
-                if (r < rows) to[0] = u;
-                if (r + 1 < rows) to[1] = w;
+              if (a.score_rows == 1) {
+                if (tig == 0 && y == 0) *to8 = u;
+              } else if (8 * y + 2 * tig < rows) {  // (the row after an odd last one is room of its own)
+                *reinterpret_cast<float2*>(to8 + 8 * y) = make_float2(u, w);
               }
             }
           }
@@ -680,7 +681,7 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_att
     for (int j = threadIdx.x; j < count; j += kWarps * 32) {
       float w = 0.f;
       for (int r = 0; r < rows; ++r)
-        if (fin[r] != -INFINITY) w += exp2_hw(scores[(long long)j * a.rows + r] - fin[r]);
+        if (fin[r] != -INFINITY) w += exp2_hw(scores[(long long)j * a.score_rows + r] - fin[r]);
       weight[j] = fmaf(a.decay, weight[j], w);
     }
   }
@@ -703,6 +704,45 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_att
 // zeros.
 constexpr int kEndThreads = 256, kEndOcc = 4, kEndEach = 4;  // threads, CTAs an SM, states a thread at once
 
+// The account of states j_first (a multiple of 4) .. j_end - 1 from a plane of scores, ROWS a state: neighbouring threads
+// take neighbouring 16 bytes, four at once, and those of a state add up among themselves.
+template <int ROWS>
+SB_DEV void account(const float4* scores, const float* fin, float* weight, float decay, int j_first, int j_end) {
+  constexpr int lanes = ROWS > 4 ? ROWS / 4 : 1, states = ROWS < 4 ? 4 / ROWS : 1;  // threads a state, states a thread
+  constexpr int step = kEndThreads / lanes * states;
+  const int quad = threadIdx.x % lanes * 4, j_mine = j_first + (int)threadIdx.x / lanes * states;
+  float l[4];
+#pragma unroll
+  for (int y = 0; y < 4; ++y) l[y] = fin[ROWS < 4 ? y % ROWS : quad + y];
+  for (int j0 = j_first; j0 < j_end; j0 += step * kEndEach) {  // (all threads take part in the sums)
+    float4 v[kEndEach];
+    float w[kEndEach][states];
+#pragma unroll
+    for (int x = 0; x < kEndEach; ++x) {
+      const int j = j_mine + (j0 - j_first) + x * step;
+      v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j < j_end) v[x] = scores[(long long)j * ROWS / 4 + (ROWS > 4 ? (int)threadIdx.x % lanes : 0)];
+#pragma unroll
+      for (int z = 0; z < states; ++z) w[x][z] = j + z < j_end && quad == 0 ? weight[j + z] : 0.f;
+    }
+#pragma unroll
+    for (int x = 0; x < kEndEach; ++x) {
+      const int j = j_mine + (j0 - j_first) + x * step;
+      const float u[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+      float sum[states];
+#pragma unroll
+      for (int z = 0; z < states; ++z) sum[z] = 0.f;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) sum[y / (4 / states)] += l[y] == -INFINITY ? 0.f : exp2_hw(u[y] - l[y]);
+#pragma unroll
+      for (int z = 1; z < lanes; z <<= 1) sum[0] += __shfl_xor_sync(0xFFFFFFFFu, sum[0], z);
+#pragma unroll
+      for (int z = 0; z < states; ++z)
+        if (j + z < j_end && quad == 0) weight[j + z] = fmaf(decay, w[x][z], sum[z]);
+    }
+  }
+}
+
 template <int DH>
 __global__ void __launch_bounds__(kEndThreads, kEndOcc) paged_end_kernel(const __grid_constant__ PagedArgs a) {
   constexpr int per = DH / 8, at_once = kEndThreads / per;  // threads of a piece's row, pieces at once
@@ -715,7 +755,7 @@ __global__ void __launch_bounds__(kEndThreads, kEndOcc) paged_end_kernel(const _
   const int b = head / a.Hkv, kvh = head - b * a.Hkv;
   const int count = a.pages.clamp(a.lens[b]), n = a.chunks(b);
   // this CTA's states
-  const int share = (count + a.ends - 1) / a.ends, j_first = min(p * share, count), j_end = min(j_first + share, count);
+  const int share = ((count + a.ends - 1) / a.ends + 3) / 4 * 4, j_first = p * share, j_end = min(j_first + share, count);
   // pieces of a unit: slots first .. first + pieces - 1
   Shares s{};
   if (a.shares) s = look_up<kEndThreads>(a, 0, b, room, found);
@@ -730,7 +770,11 @@ __global__ void __launch_bounds__(kEndThreads, kEndOcc) paged_end_kernel(const _
       first += from / s.each;
     }
     __syncthreads();
-    for (int r = warp; r < rows; r += kEndThreads / 32) {
+    for (int r = warp; r < 16; r += kEndThreads / 32) {
+      if (r >= rows) {
+        if (lane == 0) fin[r] = -INFINITY;
+        continue;
+      }
       float top = -INFINITY, sum = 0.f;
       for (int x = lane; x < pieces; x += 32) {
         const float u = a.part_l[(first + x) * a.part_rows + r], t = max3(top, u, u);
@@ -782,45 +826,13 @@ __global__ void __launch_bounds__(kEndThreads, kEndOcc) paged_end_kernel(const _
     }
     if (!a.weight) continue;
     float* const weight = a.weight + (long long)head * a.pages.cap;
-    const float* const scores = a.scores + (long long)head * a.pages.cap * a.rows + r0;
-    const bool vec = a.rows % 4 == 0;
-    for (int j = j_first + (int)threadIdx.x; j < j_end; j += kEndThreads * kEndEach) {
-      float w[kEndEach];
-#pragma unroll
-      for (int x = 0; x < kEndEach; ++x) w[x] = j + x * kEndThreads < j_end ? weight[j + x * kEndThreads] : 0.f;
-      if (block == 0)
-#pragma unroll
-        for (int x = 0; x < kEndEach; ++x) w[x] *= a.decay;
-      if (vec) {
-        for (int r = 0; r < rows; r += 4) {
-          float4 v[kEndEach];
-#pragma unroll
-          for (int x = 0; x < kEndEach; ++x)
-            if (j + x * kEndThreads < j_end)
-              v[x] = *reinterpret_cast<const float4*>(scores + (long long)(j + x * kEndThreads) * a.rows + r);
-          const float l[4] = {fin[r], fin[r + 1], fin[r + 2], fin[r + 3]};
-#pragma unroll
-          for (int x = 0; x < kEndEach; ++x) {
-            const float u[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
-#pragma unroll
-            for (int y = 0; y < 4; ++y) w[x] += l[y] == -INFINITY ? 0.f : exp2_hw(u[y] - l[y]);
-          }
-        }
-      } else {
-        for (int r = 0; r < rows; ++r) {
-          float v[kEndEach];
-#pragma unroll
-          for (int x = 0; x < kEndEach; ++x)
-            if (j + x * kEndThreads < j_end) v[x] = scores[(long long)(j + x * kEndThreads) * a.rows + r];
-          const float l = fin[r];
-#pragma unroll
-          for (int x = 0; x < kEndEach; ++x) w[x] += l == -INFINITY ? 0.f : exp2_hw(v[x] - l);
-        }
-      }
-#pragma unroll
-      for (int x = 0; x < kEndEach; ++x)
-        if (j + x * kEndThreads < j_end) weight[j + x * kEndThreads] = w[x];
-    }
+    const float4* const scores = reinterpret_cast<const float4*>(a.plane(head, block));
+    const float decay = block == 0 ? a.decay : 1.f;
+    if (a.score_rows == 1) account<1>(scores, fin, weight, decay, j_first, j_end);
+    else if (a.score_rows == 2) account<2>(scores, fin, weight, decay, j_first, j_end);
+    else if (a.score_rows == 4) account<4>(scores, fin, weight, decay, j_first, j_end);
+    else if (a.score_rows == 8) account<8>(scores, fin, weight, decay, j_first, j_end);
+    else account<16>(scores, fin, weight, decay, j_first, j_end);
   }
 }
 
@@ -836,7 +848,7 @@ void shape_of(int pt, int rows, int& chunk, int& occ) {
 }
 
 struct PagedPlan {
-  int rows, blocks, shares, ends, chunk, part_rows;
+  int rows, blocks, shares, ends, chunk, part_rows, places, score_rows;
   long long units, scores, part_o, part_l;  // floats of the workspace
   long long bytes() const { return (scores + part_o + part_l) * 4; }
 };
@@ -862,7 +874,9 @@ PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int pt, int cap, boo
   if (account && (apart || p.blocks > 1)) p.ends = (int)std::min(wave, ((long long)cap + 255) / 256);
   else if (apart) p.ends = (int)std::min(wave, (long long)p.rows);
   auto even = [](long long n) { return (n + 3) / 4 * 4; };
-  p.scores = account ? even((long long)B * Hkv * cap * p.rows) : 0;
+  p.places = (cap + 3) / 4 * 4;
+  for (p.score_rows = 1; p.score_rows < p.part_rows;) p.score_rows *= 2;
+  p.scores = account ? (long long)B * Hkv * p.blocks * p.places * p.score_rows : 0;
   const long long slots = p.units + p.shares;
   p.part_o = apart ? slots * p.part_rows * dh : 0;
   p.part_l = p.ends > 0 ? even(slots * p.part_rows) : 0;
@@ -939,6 +953,7 @@ extern "C" int sb_paged_attention(const sb_paged_memory* memory, const void* q, 
   a.lens = lens;
   a.B = m->B; a.H = H; a.Hkv = m->Hkv; a.group = H / m->Hkv; a.Tq = Tq;
   a.rows = p.rows; a.blocks = p.blocks; a.shares = p.shares; a.ends = p.ends; a.chunk = p.chunk; a.part_rows = p.part_rows;
+  a.places = p.places; a.score_rows = p.score_rows;
   a.q_bf16 = q_dtype == SB_BF16; a.causal = causal != 0;
   a.scale_log2 = scale * k_scale * 1.4426950408889634f;
   a.v_scale = v_scale;

@@ -11,7 +11,7 @@ namespace {
 // ---------------------------------------------------------------- write
 // Row (b, t), t < count[b], goes to position at[b] + t of item b.  Copies, bound by memory: a warp takes the
 // rows of a group (their pages are looked up once, by a lane a row) and keeps four vectors of K and four of V a lane
-// in flight (two where 32 bytes become 16 of e4m3).  e4m3 pages get the code of x / scale, a true division, or
+// in flight.  e4m3 pages get the code of x / scale, a true division, or
 // where both scales are powers of two the product with their reciprocals, which is the quotient.
 struct WriteArgs {
   const void *k, *v;
@@ -25,7 +25,7 @@ struct WriteArgs {
   float k_scale, v_scale;
   float* weight;
   int *born, *after;
-  FastDiv vecs;  // 16-byte vectors a row of the pool
+  FastDiv vecs;  // vectors of eight elements a row
   int group;     // rows a warp
   long long rows, row_blocks, marks;  // marks: what else is written, one a thread
   SB_DEV int start(int b) const { return pages.clamp(at[b]); }
@@ -34,44 +34,25 @@ struct WriteArgs {
 
 constexpr int kWriteWarps = 8;
 
-// The 16 bytes of a pool's vector from row element i on: eight values, or sixteen as e4m3.
-template <bool E4M3>
-struct Vec {
-  Raw8 r[E4M3 ? 2 : 1];
-};
-template <bool E4M3, bool ALIGNED>
-SB_DEV Vec<E4M3> load_vec(const void* p, int dt, long long i) {
-  Vec<E4M3> v;
-#pragma unroll
-  for (int x = 0; x < (E4M3 ? 2 : 1); ++x)
-    v.r[x] = ALIGNED ? load_raw8(p, dt, i + 8 * x) : load_raw8_tail(p, dt, i + 8 * x, 8);
-  return v;
-}
-// MODE 0: as they are; 1: e4m3 of x * scale; 2: e4m3 of x / scale
+// Eight elements as a pool holds them.  MODE 0: as they are; 1: e4m3 of x * scale; 2: e4m3 of x / scale
 template <int MODE>
-SB_DEV uint4 pool_vec(const Vec<(MODE > 0)>& v, int dt, float scale) {
+SB_DEV void put_vec(uint64_t to, const Raw8& r, int dt, float scale) {
   if constexpr (MODE == 0) {
-    return v.r[0].lo;
+    *reinterpret_cast<uint4*>(to) = r.lo;
   } else {
-    uint32_t w[4];
+    float f[8];
+    unpack8(r, dt, f);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      float f[8];
-      unpack8(v.r[x], dt, f);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) f[u] = MODE == 1 ? f[u] * scale : __fdiv_rn(f[u], scale);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        w[2 * x + u] = (uint32_t)e4m3x2_of(f[4 * u], f[4 * u + 1]) | (uint32_t)e4m3x2_of(f[4 * u + 2], f[4 * u + 3]) << 16;
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    for (int u = 0; u < 8; ++u) f[u] = MODE == 1 ? f[u] * scale : __fdiv_rn(f[u], scale);
+    *reinterpret_cast<uint2*>(to) =
+        make_uint2((uint32_t)e4m3x2_of(f[0], f[1]) | (uint32_t)e4m3x2_of(f[2], f[3]) << 16,
+                   (uint32_t)e4m3x2_of(f[4], f[5]) | (uint32_t)e4m3x2_of(f[6], f[7]) << 16);
   }
 }
 
 template <int MODE, bool ALIGNED>
-__global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __grid_constant__ WriteArgs a) {
-  constexpr bool E4M3 = MODE > 0;
-  constexpr int kAhead = E4M3 ? 2 : 4;
+__global__ void __launch_bounds__(kWriteWarps * 32, MODE == 2 ? 2 : 4) paged_write_kernel(const __grid_constant__ WriteArgs a) {
+  constexpr int kAhead = 4, bytes = MODE ? 8 : 16;  // vectors of K and V at once, bytes of one in the pool
   if (blockIdx.x >= a.row_blocks) {  // new lengths, then weights and stamps, neighbours along t
     long long i = (blockIdx.x - a.row_blocks) * (kWriteWarps * 32) + threadIdx.x;
     if (i >= a.marks) return;
@@ -108,31 +89,30 @@ __global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __g
   }
   __syncwarp();
   const int total = rows * (int)a.vecs.d;
-  constexpr int per = E4M3 ? 16 : 8;
   for (int i0 = lane; i0 < total; i0 += 32 * kAhead) {
-    Vec<E4M3> k[kAhead], v[kAhead];
+    Raw8 k[kAhead], v[kAhead];
     ulonglong2 where[kAhead];
-    int c[kAhead];
 #pragma unroll
     for (int x = 0; x < kAhead; ++x) {
       const int i = i0 + 32 * x;
       where[x] = make_ulonglong2(0, 0);
       if (i < total) {
-        const int r = (int)a.vecs.div((uint32_t)i);
-        c[x] = i - r * (int)a.vecs.d;
+        const int r = (int)a.vecs.div((uint32_t)i), c = i - r * (int)a.vecs.d;
         where[x] = to[warp][r];
         if (where[x].x) {
+          where[x].x += c * bytes;
+          where[x].y += c * bytes;
           const longlong2 s = from[warp][r];
-          k[x] = load_vec<E4M3, ALIGNED>(a.k, a.dt, s.x + c[x] * per);
-          v[x] = load_vec<E4M3, ALIGNED>(a.v, a.dt, s.y + c[x] * per);
+          k[x] = ALIGNED ? load_raw8(a.k, a.dt, s.x + c * 8) : load_raw8_tail(a.k, a.dt, s.x + c * 8, 8);
+          v[x] = ALIGNED ? load_raw8(a.v, a.dt, s.y + c * 8) : load_raw8_tail(a.v, a.dt, s.y + c * 8, 8);
         }
       }
     }
 #pragma unroll
     for (int x = 0; x < kAhead; ++x)
       if (where[x].x) {
-        *reinterpret_cast<uint4*>(where[x].x + c[x] * 16) = pool_vec<MODE>(k[x], a.dt, a.k_scale);
-        *reinterpret_cast<uint4*>(where[x].y + c[x] * 16) = pool_vec<MODE>(v[x], a.dt, a.v_scale);
+        put_vec<MODE>(where[x].x, k[x], a.dt, a.k_scale);
+        put_vec<MODE>(where[x].y, v[x], a.dt, a.v_scale);
       }
   }
 }
@@ -163,13 +143,6 @@ struct EvictArgs {
 };
 
 constexpr int kSelect = 512, kSelectWarps = kSelect / 32, kBins = 2048, kMostCtas = 8;
-constexpr int kSelectRoom = 92 * 1024;  // shared memory for weights and bits, two CTAs an SM
-// words of 32 states of a CTA, one of `ctas`
-inline int select_words(int cap, int ctas) {
-  const int words = (cap + 31) / 32, warps = kSelectWarps * ctas;
-  return (words + warps - 1) / warps * kSelectWarps;
-}
-inline long long select_bytes(int cap, int ctas) { return select_words(cap, ctas) * (32ll * 4 + 8); }
 
 // Integers in the order of the weights; NaN is the least, both zeros are one.
 SB_DEV uint32_t ordered(float w) {
@@ -178,246 +151,392 @@ SB_DEV uint32_t ordered(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sums over the warps before this one and over all, of the CTA.  `room`: 33 ints; begins and ends with a barrier.
-SB_DEV int warps_before(int v, int* room, int& total) {
+// What the CTAs of an (item, key head) tell each other; bins and counts are never written twice.
+struct Told {
+  int bins[3][kBins];
+  int counts[4][2];
+  int room[2][kSelectWarps], found[2];
+};
+SB_DEV void all_sync(int ctas) {
+  if (ctas > 1) cluster_sync();
+  else __syncthreads();
+}
+
+// Sums of two numbers over the threads before this one and over all, of all CTAs; the c-th such sum.
+SB_DEV void before_and_all(int (&v)[2], int (&total)[2], Told& told, int c, int ctas, uint32_t rank) {
   const int lane = lane_id(), warp = warp_id();
+  int s[2] = {v[0], v[1]};
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int u = __shfl_up_sync(0xFFFFFFFFu, s[y], x);
+      if (lane >= x) s[y] += u;
+    }
   __syncthreads();
-  if (lane == 0) room[warp] = v;
+  if (lane == 31) {
+    told.room[0][warp] = s[0];
+    told.room[1][warp] = s[1];
+  }
   __syncthreads();
-  int w = lane < kSelectWarps ? room[lane] : 0, s = w;
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    int before = s[y] - v[y], all = 0;
+    for (int w = 0; w < kSelectWarps; ++w) {
+      const int t = told.room[y][w];
+      if (w < warp) before += t;
+      all += t;
+    }
+    v[y] = before;
+    total[y] = all;
+  }
+  if (ctas > 1) {
+    if (threadIdx.x == 0) {
+      told.counts[c][0] = total[0];
+      told.counts[c][1] = total[1];
+    }
+    cluster_sync();
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      int all = 0;
+      for (uint32_t r = 0; r < (uint32_t)ctas; ++r) {
+        const int t = (int)peer_word(&told.counts[c][y], r);
+        if (r < rank) v[y] += t;
+        all += t;
+      }
+      total[y] = all;
+    }
+  }
+}
+
+// The bin of a pass, counted from the top, that holds the need-th number; need becomes its place in the bin, same how
+// many the bin holds.
+SB_DEV int find_bin(Told& told, int pass, int& need, int& same, int ctas) {
+  const int lane = lane_id(), warp = warp_id(), first = kBins - 4 - 4 * (int)threadIdx.x;  // four bins a thread
+  all_sync(ctas);
+  int c[4] = {0, 0, 0, 0};
+  for (uint32_t r = 0; r < (uint32_t)ctas; ++r) {
+    const uint4 u = ctas > 1 ? peer_words(&told.bins[pass][first], r) : *reinterpret_cast<const uint4*>(&told.bins[pass][first]);
+    c[0] += (int)u.w;
+    c[1] += (int)u.z;
+    c[2] += (int)u.y;
+    c[3] += (int)u.x;
+  }
+  const int four = c[0] + c[1] + c[2] + c[3];
+  int s = four;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) {
     const int u = __shfl_up_sync(0xFFFFFFFFu, s, x);
     if (lane >= x) s += u;
   }
-  total = __shfl_sync(0xFFFFFFFFu, s, 31);
-  const int before = __shfl_sync(0xFFFFFFFFu, s - w, warp);
-  return before;
-}
-// The same over the warps of all CTAs of the cluster; `mine`: an int of its own for each call.
-SB_DEV int warps_before_all(int v, int* room, int* mine, int ctas, uint32_t rank, int& total) {
-  int before = warps_before(v, room, total);
-  if (ctas > 1) {
-    if (threadIdx.x == 0) *mine = total;
-    cluster_sync();
-    int all = 0;
-    for (uint32_t r = 0; r < (uint32_t)ctas; ++r) {
-      const int t = (int)peer_word(mine, r);
-      if (r < rank) before += t;
-      all += t;
+  __syncthreads();
+  if (lane == 31) told.room[0][warp] = s;
+  __syncthreads();
+  int above = s - four;
+  for (int w = 0; w < warp; ++w) above += told.room[0][w];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    if (above < need && need <= above + c[x]) {
+      told.found[0] = first + 3 - x;
+      told.found[1] = above;
+      told.room[1][0] = c[x];
     }
-    total = all;
+    above += c[x];
   }
-  return before;
+  __syncthreads();
+  const int bin = told.found[0];
+  need -= told.found[1];
+  same = told.room[1][0];
+  return bin;
+}
+// A pass's bits of a key, and those of the passes before it.
+SB_DEV int bin_of(uint32_t key, int pass) { return pass == 0 ? key >> 21 : pass == 1 ? key >> 10 & 2047u : key & 1023u; }
+SB_DEV uint32_t prefix_of(uint32_t key, int pass) { return pass == 0 ? 0u : pass == 1 ? key & 0xFFE00000u : key & 0xFFFFFC00u; }
+SB_DEV uint32_t as_prefix(int bin, int pass) { return (uint32_t)bin << (pass == 0 ? 21 : pass == 1 ? 10 : 0); }
+
+// What both selections end with: the pairs' weights and stamps, zeros from the new length on.
+SB_DEV void finish(const EvictArgs& a, long long unit, int moves, int left, const int* to, const int* from, int ctas, uint32_t rank) {
+  const long long at = unit * a.pages.cap;
+  all_sync(ctas);
+  for (int i = (int)rank * kSelect + (int)threadIdx.x; i < moves; i += ctas * kSelect) {
+    const int d = to[i], s = from[i];
+    a.weight_out[at + d] = a.weight[at + s];
+    if (a.born) a.born_out[at + d] = a.born[at + s];
+  }
+  all_sync(ctas);  // where the results lie on the operands: read before they are cleared
+  for (int j = left + (int)rank * kSelect + (int)threadIdx.x; j < a.pages.cap; j += ctas * kSelect) {
+    a.weight_out[at + j] = 0.f;
+    if (a.born) a.born_out[at + j] = 0;
+  }
+  if (threadIdx.x == 0 && rank == 0) a.moves[unit] = moves;
+  if (ctas > 1) cluster_sync();  // no CTA ends while another reads what it told
+}
+// An item within its budget: as it is.
+SB_DEV void keep_all_of(const EvictArgs& a, long long unit, int len, int ctas, uint32_t rank) {
+  const long long at = unit * a.pages.cap;
+  for (int j = (int)rank * kSelect + (int)threadIdx.x; j < len; j += ctas * kSelect) {
+    if (a.weight_out != a.weight) a.weight_out[at + j] = a.weight[at + j];
+    if (a.born_out != a.born) a.born_out[at + j] = a.born[at + j];
+  }
 }
 
-// A warp's states lie behind one another, so that places come out in order; kAtOnce times 32 at a time.
-// HELD: the weights and bits are in shared memory.
-template <bool HELD>
-__global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_constant__ EvictArgs a) {
-  constexpr int kAtOnce = 8;
-  extern __shared__ __align__(16) uint32_t held[];  // the CTA's ordered weights; words of protected states and of those that stay
-  __shared__ int bins[kBins], sums[kBins];
-  __shared__ int room[33], totals[4], found[2];
-  const int warp = warp_id(), lane = lane_id(), cap = a.pages.cap, ctas = a.ctas;
-  const uint32_t rank = ctas > 1 ? cluster_ctarank() : 0u;
-  const long long unit = blockIdx.x / ctas;
-  const int b = (int)(unit / a.Hkv);
-  const int len = a.pages.clamp(a.lens[b]), keep = a.budget(b), left = min(len, keep);
-  const float* weight = a.weight + unit * cap;
-  float* weight_out = a.weight_out + unit * cap;
-  const int* born = a.born ? a.born + unit * cap : nullptr;
-  int* born_out = a.born ? a.born_out + unit * cap : nullptr;
-  const bool guard = born && a.since;
-  const int since = guard ? a.since[b] : 0;
-  int* to = a.to + unit * a.half;
-  int* from = a.from + unit * a.half;
-  const int warps = kSelectWarps * ctas, words = (len + 31) / 32, steps = (words + warps - 1) / warps;
-  const int w_first = min(((int)rank * kSelectWarps + warp) * steps, words), w_end = min(w_first + steps, words);
-  // words of this CTA, from its first on; in memory, of the unit
-  const int base = HELD ? (int)rank * kSelectWarps * steps : 0, all_words = (cap + 31) / 32;
-  uint32_t* guarded = HELD ? held + kSelectWarps * steps * 32 : a.bits + unit * 2 * all_words;
-  uint32_t* stay = HELD ? guarded + kSelectWarps * steps : guarded + all_words;
-  int moves = 0;
-  auto cta_sync = [&] {
-    if (ctas > 1) cluster_sync();
-    else __syncthreads();
-  };
+// Selection with the CTA's ordered weights in shared memory: a thread has a run of states, an odd number of fours, so that
+// neighbours' 16-byte reads fall in distinct banks, and their bits (protected, staying) in registers; no pass
+// needs a word with another thread but the counts.
+constexpr int kMostFours = 9;                                 // states a thread: 36; two CTAs an SM
+constexpr int kHeldRoom = kSelect * kMostFours * 4 * 4 + kSelect * kMostFours * 4 / 8 + 16;
+inline int held_fours(int cap, int ctas) { return ((cap + ctas * kSelect * 4 - 1) / (ctas * kSelect * 4)) | 1; }
 
-  if (len > keep) {
-    // what the passes look at: the ordered weight of state j (below len, else 0) and the bits of its word
-    auto key_of = [&](int w) {
-      const int j = w * 32 + lane;
-      return HELD ? held[(w - base) * 32 + lane] : j < len ? ordered(weight[j]) : 0u;
-    };
-    int n = 0;
-    for (int w0 = w_first; w0 < w_end; w0 += kAtOnce) {
+__global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_constant__ EvictArgs a) {
+  extern __shared__ __align__(16) uint32_t held[];  // weights of the CTA's states, then bits of the protected ones
+  __shared__ __align__(16) Told told;
+  const int warp = warp_id(), lane = lane_id(), ctas = a.ctas;
+  const uint32_t rank = ctas > 1 ? cluster_ctarank() : 0u;
+  const long long unit = blockIdx.x / ctas, at = unit * a.pages.cap;
+  const int b = (int)(unit / a.Hkv);
+  const int len = a.pages.clamp(a.lens[b]), keep = a.budget(b);
+  int* const to = a.to + unit * a.half;
+  int* const from = a.from + unit * a.half;
+  int moves = 0;
+  if (len <= keep) {
+    keep_all_of(a, unit, len, ctas, rank);
+  } else {
+    const bool guard = a.born && a.since;
+    const int since = guard ? a.since[b] : 0;
+    const int fours = ((len + ctas * kSelect * 4 - 1) / (ctas * kSelect * 4)) | 1, run = fours * 4, mine = kSelect * run;
+    const int j_cta = (int)rank * mine, here = min(max(len - j_cta, 0), mine);  // the CTA's states
+    uint32_t* const bits = held + mine;
+    for (int x = threadIdx.x; x < 3 * kBins; x += kSelect) told.bins[0][x] = 0;
+    int all[2], n[2] = {0, 0};
+    constexpr int kAtOnce = 8;
+    for (int w0 = warp * 32; w0 < here; w0 += kAtOnce * kSelect) {
       float f[kAtOnce];
       int s[kAtOnce];
 #pragma unroll
       for (int x = 0; x < kAtOnce; ++x) {
+        const int j = w0 + x * kSelect + lane;
+        f[x] = j < here ? a.weight[at + j_cta + j] : 0.f;
+        s[x] = a.born && j < here ? a.born[at + j_cta + j] : 0;
+      }
+#pragma unroll
+      for (int x = 0; x < kAtOnce; ++x) {
+        const int w = w0 + x * kSelect, j = w + lane;
+        if (w < here) {
+          const uint32_t word = __ballot_sync(0xFFFFFFFFu, guard && j < here && s[x] >= since);
+          held[j] = ordered(f[x]);
+          if (lane == 0) {
+            bits[w >> 5] = word;
+            n[0] += __popc(word);
+          }
+          if (j_cta + j < keep && j < here) {  // as if all of these stayed
+            if (a.weight_out != a.weight) a.weight_out[at + j_cta + j] = f[x];
+            if (a.born_out != a.born) a.born_out[at + j_cta + j] = s[x];
+          }
+        }
+      }
+    }
+    before_and_all(n, all, told, 0, ctas, rank);
+    // the states among which weights decide: the protected ones where they alone are too many, else the others
+    const bool inner = all[0] >= keep;
+    int need = inner ? keep : keep - all[0], same = 0;
+    uint32_t last = 0xFFFFFFFFu;  // the ordered weight of the last state that stays; `need` of that weight do
+    // this thread's run
+    const int j_run = (int)threadIdx.x * run, states = min(max(here - j_run, 0), run);
+    const uint64_t valid = states > 0 ? ~0ull >> (64 - states) : 0ull;
+    uint64_t safe = 0;
+    if (states > 0) {
+      const int w = j_run >> 5, w_last = (here - 1) >> 5, o = j_run & 31;
+      const uint64_t lo = bits[w] | (w + 1 <= w_last ? (uint64_t)bits[w + 1] << 32 : 0ull);
+      safe = lo >> o;
+      if (o && w + 2 <= w_last) safe |= (uint64_t)bits[w + 2] << (64 - o);
+      safe &= valid;
+    }
+    const uint64_t who = inner ? safe : valid & ~safe;
+    const uint4* const keys = reinterpret_cast<const uint4*>(held + j_run);
+    const int my_fours = (states + 3) / 4;
+    if (need > 0) {
+      last = 0;
+      for (int pass = 0; pass < 3; ++pass) {
+        // (many states may have one weight, new ones 0: runs of a bin are counted before they are added)
+        int bin = -1, count = 0;
+        for (int i = 0; i < my_fours; ++i) {
+          const uint4 k = keys[i];
+          const uint32_t key[4] = {k.x, k.y, k.z, k.w}, nibble = (uint32_t)(who >> (4 * i));
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if ((nibble >> y & 1u) && prefix_of(key[y], pass) == last) {
+              const int x = bin_of(key[y], pass);
+              if (x != bin) {
+                if (count) atomicAdd(&told.bins[pass][bin], count);
+                bin = x;
+                count = 0;
+              }
+              ++count;
+            }
+        }
+        if (count) atomicAdd(&told.bins[pass][bin], count);
+        last |= as_prefix(find_bin(told, pass, need, same, ctas), pass);
+      }
+    }
+    uint64_t more = 0, tied = 0;
+    for (int i = 0; i < my_fours; ++i) {
+      const uint4 k = keys[i];
+      const uint32_t g = (uint32_t)(k.x > last) | (uint32_t)(k.y > last) << 1 | (uint32_t)(k.z > last) << 2 | (uint32_t)(k.w > last) << 3;
+      const uint32_t t = (uint32_t)(k.x == last) | (uint32_t)(k.y == last) << 1 | (uint32_t)(k.z == last) << 2 | (uint32_t)(k.w == last) << 3;
+      more |= (uint64_t)g << (4 * i);
+      tied |= (uint64_t)t << (4 * i);
+    }
+    more &= who;
+    tied &= need > 0 ? who : 0ull;
+    if (same > need) {  // more states have the last weight than may stay: the first of them do
+      int ties[2] = {__popcll(tied), 0}, total[2];
+      before_and_all(ties, total, told, 1, ctas, rank);
+      for (int extra = ties[0] + __popcll(tied) - max(need, ties[0]); extra > 0; --extra) tied &= ~(1ull << (63 - __clzll(tied)));
+    }
+    const uint64_t stays = more | tied | (inner ? 0ull : safe);
+    const int low_n = min(max(keep - j_cta - j_run, 0), states);  // states of the run below keep
+    const uint64_t low = low_n > 0 ? ~0ull >> (64 - low_n) : 0ull;
+    uint64_t free = low & ~stays, move = stays & ~low;
+    int put[2] = {__popcll(free), __popcll(move)}, total[2];
+    before_and_all(put, total, told, 2, ctas, rank);
+    moves = total[1];
+    for (; free; free &= free - 1) to[put[0]++] = j_cta + j_run + __ffsll(free) - 1;
+    for (; move; move &= move - 1) from[put[1]++] = j_cta + j_run + __ffsll(move) - 1;
+  }
+  finish(a, unit, moves, min(len, keep), to, from, ctas, rank);
+}
+
+// The same for longer ones, from memory: a warp's states lie behind one another, 32 at a time, their bits in memory too.
+__global__ void __launch_bounds__(kSelect, 2) evict_select_long_kernel(const __grid_constant__ EvictArgs a) {
+  __shared__ __align__(16) Told told;
+  const int warp = warp_id(), lane = lane_id(), ctas = a.ctas;
+  const uint32_t rank = ctas > 1 ? cluster_ctarank() : 0u;
+  const long long unit = blockIdx.x / ctas, at = unit * a.pages.cap;
+  const int b = (int)(unit / a.Hkv);
+  const int len = a.pages.clamp(a.lens[b]), keep = a.budget(b);
+  int* const to = a.to + unit * a.half;
+  int* const from = a.from + unit * a.half;
+  int moves = 0;
+  if (len <= keep) {
+    keep_all_of(a, unit, len, ctas, rank);
+  } else {
+    constexpr int kAtOnce = 8;
+    const bool guard = a.born && a.since;
+    const int since = guard ? a.since[b] : 0;
+    const int warps = kSelectWarps * ctas, words = (len + 31) / 32, steps = (words + warps - 1) / warps;
+    const int w_first = min(((int)rank * kSelectWarps + warp) * steps, words), w_end = min(w_first + steps, words);
+    uint32_t* const guarded = a.bits + unit * 2 * ((a.pages.cap + 31) / 32);
+    uint32_t* const stay = guarded + (a.pages.cap + 31) / 32;
+    auto key_of = [&](int w) { return w < w_end && w * 32 + lane < len ? ordered(a.weight[at + w * 32 + lane]) : 0u; };
+    for (int x = threadIdx.x; x < 3 * kBins; x += kSelect) told.bins[0][x] = 0;
+    int all[2], n[2] = {0, 0};
+    for (int w0 = w_first; w0 < w_end; w0 += kAtOnce) {
+      int s[kAtOnce];
+#pragma unroll
+      for (int x = 0; x < kAtOnce; ++x) {
         const int j = (w0 + x) * 32 + lane;
-        const bool in = w0 + x < w_end && j < len;
-        f[x] = HELD && in ? weight[j] : 0.f;
-        s[x] = guard && in ? born[j] : 0;
+        s[x] = a.born && w0 + x < w_end && j < len ? a.born[at + j] : 0;
       }
 #pragma unroll
       for (int x = 0; x < kAtOnce; ++x) {
         const int j = (w0 + x) * 32 + lane;
         if (w0 + x < w_end) {
           const uint32_t word = __ballot_sync(0xFFFFFFFFu, guard && j < len && s[x] >= since);
-          if (HELD) held[(w0 + x - base) * 32 + lane] = ordered(f[x]);
-          if (lane == 0) guarded[w0 + x - base] = word;
-          n += __popc(word);
+          if (lane == 0) {
+            guarded[w0 + x] = word;
+            n[0] += __popc(word);
+          }
+          if (j < keep) {  // as if all of these stayed
+            if (a.weight_out != a.weight) a.weight_out[at + j] = a.weight[at + j];
+            if (a.born_out != a.born) a.born_out[at + j] = s[x];
+          }
         }
       }
     }
-    int all;
-    warps_before_all(n, room, &totals[0], ctas, rank, all);
-    // the states among which weights decide: the protected ones where they alone are too many, else the others
-    const bool inner = all >= keep;
+    before_and_all(n, all, told, 0, ctas, rank);
+    const bool inner = all[0] >= keep;
     const uint32_t flip = inner ? 0u : 0xFFFFFFFFu;
-    int need = inner ? keep : keep - all, same = 0;
-    uint32_t last = 0xFFFFFFFFu;  // the ordered weight of the last state that stays; `need` of that weight do
+    int need = inner ? keep : keep - all[0], same = 0;
+    uint32_t last = 0xFFFFFFFFu;
+    auto class_of = [&](int w) { return w < w_end ? (guarded[w] ^ flip) & bits_below(w * 32, len) : 0u; };
     if (need > 0) {
       last = 0;
       for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
-        for (int x = threadIdx.x; x < kBins; x += kSelect) bins[x] = 0;
-        __syncthreads();
         for (int w0 = w_first; w0 < w_end; w0 += kAtOnce) {
           uint32_t key[kAtOnce], who[kAtOnce];
 #pragma unroll
           for (int x = 0; x < kAtOnce; ++x) {
-            const int w = w0 + x;
-            key[x] = w < w_end ? key_of(w) : 0u;
-            who[x] = w < w_end ? (guarded[w - base] ^ flip) & bits_below(w * 32, len) : 0u;
+            key[x] = key_of(w0 + x);
+            who[x] = class_of(w0 + x);
           }
 #pragma unroll
           for (int x = 0; x < kAtOnce; ++x) {
-            const bool mine = (who[x] >> lane & 1u) && (key[x] & mask) == last;
+            const bool mine = (who[x] >> lane & 1u) && prefix_of(key[x], pass) == last;
             const uint32_t some = __ballot_sync(0xFFFFFFFFu, mine);
             if (some == 0) continue;
-            const int bin = key[x] >> shift & (pass == 2 ? 1023 : 2047);
-            // many states of one weight (new ones have 0): one count for the warp
+            const int bin = bin_of(key[x], pass);
             const int one = __shfl_sync(0xFFFFFFFFu, bin, __ffs(some) - 1);
             if (__all_sync(0xFFFFFFFFu, !mine || bin == one)) {
-              if (lane == 0) atomicAdd(&bins[one], __popc(some));
+              if (lane == 0) atomicAdd(&told.bins[pass][one], __popc(some));
             } else if (mine) {
-              atomicAdd(&bins[bin], 1);
+              atomicAdd(&told.bins[pass][bin], 1);
             }
           }
         }
-        cta_sync();
-        // four bins a thread, from the top
-        const int top = kBins - 1 - 4 * (int)threadIdx.x;
-        int c[4], four = 0;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          c[x] = 0;
-          if (ctas > 1)
-            for (uint32_t r = 0; r < (uint32_t)ctas; ++r) c[x] += (int)peer_word(&bins[top - x], r);
-          else c[x] = bins[top - x];
-          sums[top - x] = c[x];
-          four += c[x];
-        }
-        if (ctas > 1) cluster_sync();  // bins are written again
-        int s = four, total;
-#pragma unroll
-        for (int x = 1; x < 32; x <<= 1) {
-          const int u = __shfl_up_sync(0xFFFFFFFFu, s, x);
-          if (lane >= x) s += u;
-        }
-        int above = warps_before(__shfl_sync(0xFFFFFFFFu, s, 31), room, total) + s - four;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if (above < need && need <= above + c[x]) {
-            found[0] = top - x;
-            found[1] = above;
-          }
-          above += c[x];
-        }
-        __syncthreads();
-        last |= (uint32_t)found[0] << shift;
-        need -= found[1];
-        same = sums[found[0]];
-        __syncthreads();  // sums and found are written again
+        last |= as_prefix(find_bin(told, pass, need, same, ctas), pass);
       }
     }
-    // where more states have the last weight than may stay, the first of them do
     const bool some = need > 0, choose = same > need;
     int ties = 0;
     if (choose) {
-      n = 0;
+      int t[2] = {0, 0}, total[2];
       for (int w = w_first; w < w_end; ++w) {
-        const uint32_t who = (guarded[w - base] ^ flip) & bits_below(w * 32, len);
-        n += __popc(__ballot_sync(0xFFFFFFFFu, key_of(w) == last) & who);
+        const uint32_t tied = __ballot_sync(0xFFFFFFFFu, key_of(w) == last) & class_of(w);
+        if (lane == 0) t[0] += __popc(tied);
       }
-      int total;
-      ties = warps_before_all(n, room, &totals[1], ctas, rank, total);
+      before_and_all(t, total, told, 1, ctas, rank);
+      ties = __shfl_sync(0xFFFFFFFFu, t[0], 0);
     }
-    int free = 0, move = 0;
+    int put[2] = {0, 0}, total[2];
     for (int w0 = w_first; w0 < w_end; w0 += kAtOnce) {
-      uint32_t key[kAtOnce], g[kAtOnce];
+      uint32_t key[kAtOnce];
 #pragma unroll
-      for (int x = 0; x < kAtOnce; ++x) {
-        const int w = w0 + x;
-        key[x] = w < w_end ? key_of(w) : 0u;
-        g[x] = w < w_end ? guarded[w - base] : 0u;
-      }
+      for (int x = 0; x < kAtOnce; ++x) key[x] = key_of(w0 + x);
 #pragma unroll
       for (int x = 0; x < kAtOnce; ++x) {
         const int w = w0 + x;
         if (w < w_end) {
-          const uint32_t here = bits_below(w * 32, len), low = bits_below(w * 32, keep), who = (g[x] ^ flip) & here;
+          const uint32_t here = bits_below(w * 32, len), low = bits_below(w * 32, keep), who = class_of(w);
           const uint32_t more = __ballot_sync(0xFFFFFFFFu, key[x] > last) & who;
-          uint32_t tied = some ? __ballot_sync(0xFFFFFFFFu, key[x] == last) & who : 0u;
+          const uint32_t tied = __ballot_sync(0xFFFFFFFFu, key[x] == last) & (some ? who : 0u);
           uint32_t first = tied;
           if (choose) {
             first = __ballot_sync(0xFFFFFFFFu, (tied >> lane & 1u) && ties + __popc(tied & ((1u << lane) - 1u)) < need);
             ties += __popc(tied);
           }
-          const uint32_t stays = more | first | (inner ? 0u : g[x] & here);
-          if (lane == 0) stay[w - base] = stays;
-          free += __popc(~stays & low & here);
-          move += __popc(stays & ~low);
+          const uint32_t stays = more | first | (inner ? 0u : guarded[w] & here);
+          __syncwarp();
+          if (lane == 0) {
+            stay[w] = stays;
+            put[0] += __popc(~stays & low & here);
+            put[1] += __popc(stays & ~low);
+          }
         }
       }
     }
-    int total;
-    int at_free = warps_before_all(free, room, &totals[2], ctas, rank, total);
-    int at_move = warps_before_all(move, room, &totals[3], ctas, rank, moves);
+    before_and_all(put, total, told, 2, ctas, rank);
+    moves = total[1];
+    int at_free = __shfl_sync(0xFFFFFFFFu, put[0], 0), at_move = __shfl_sync(0xFFFFFFFFu, put[1], 0);
     for (int w = w_first; w < w_end; ++w) {
-      const int j = w * 32 + lane;
-      const uint32_t s = stay[w - base], low = bits_below(w * 32, keep), below = (1u << lane) - 1u;
+      const uint32_t s = stay[w], low = bits_below(w * 32, keep), below = (1u << lane) - 1u;
       const uint32_t f = ~s & low & bits_below(w * 32, len), m = s & ~low;
-      if (f >> lane & 1u) to[at_free + __popc(f & below)] = j;
-      if (m >> lane & 1u) from[at_move + __popc(m & below)] = j;
-      if (weight_out != weight && (s & low) >> lane & 1u) weight_out[j] = weight[j];
-      if (born_out != born && (s & low) >> lane & 1u) born_out[j] = born[j];
+      if (f >> lane & 1u) to[at_free + __popc(f & below)] = w * 32 + lane;
+      if (m >> lane & 1u) from[at_move + __popc(m & below)] = w * 32 + lane;
       at_free += __popc(f);
       at_move += __popc(m);
     }
-    cta_sync();
-    for (int i = (int)rank * kSelect + threadIdx.x; i < moves; i += ctas * kSelect) {
-      const int d = to[i], s = from[i];
-      weight_out[d] = weight[s];
-      if (born) born_out[d] = born[s];
-    }
-    cta_sync();  // where the results lie on the operands: read before they are cleared
-  } else {
-    for (int j = (int)rank * kSelect + threadIdx.x; j < len; j += ctas * kSelect) {
-      if (weight_out != weight) weight_out[j] = weight[j];
-      if (born_out != born) born_out[j] = born[j];
-    }
   }
-  for (int j = left + (int)rank * kSelect + threadIdx.x; j < cap; j += ctas * kSelect) {
-    weight_out[j] = 0.f;
-    if (born) born_out[j] = 0;
-  }
-  if (threadIdx.x == 0 && rank == 0) a.moves[unit] = moves;
-  if (ctas > 1) cluster_sync();  // no CTA ends while another reads its counts
+  finish(a, unit, moves, min(len, keep), to, from, ctas, rank);
 }
 
 // Rows of the pairs: a warp takes 32 pairs, a lane looks up where a pair's rows lie, then all copy them, 16 bytes a lane,
@@ -492,10 +611,9 @@ EvictPlan evict_plan(int B, int Hkv, int cap, int sms) {
   p.half = std::max(1, cap / 2);  // at most min(keep, len - keep) states move
   p.words = (cap + 31) / 32;
   p.ctas = 1;
-  while (p.ctas < kMostCtas &&
-         ((2 * units * p.ctas <= 2 * sms && cap / p.ctas > 2048) || select_bytes(cap, p.ctas) > kSelectRoom))
+  while (p.ctas < kMostCtas && ((2 * units * p.ctas <= 2 * sms && cap / p.ctas > 2048) || held_fours(cap, p.ctas) > kMostFours))
     p.ctas *= 2;
-  p.held = select_bytes(cap, p.ctas) <= kSelectRoom;
+  p.held = held_fours(cap, p.ctas) <= kMostFours;
   p.parts = (int)std::max(1ll, std::min(((long long)p.half + kMoveWarps * 32 - 1) / (kMoveWarps * 32), (16ll * sms + units - 1) / units));
   p.lists = 2 * units * p.half;
   p.moves = units;
@@ -503,12 +621,13 @@ EvictPlan evict_plan(int B, int Hkv, int cap, int sms) {
   return p;
 }
 
-template <bool HELD>
-cudaError_t evict_select(const EvictArgs& a, long long units, cudaStream_t st) {
+cudaError_t evict_select(const EvictArgs& a, bool held, long long units, cudaStream_t st) {
+  if (!held) return launch_after(evict_select_long_kernel, units * a.ctas, kSelect, 0, st, a, a.ctas, false);
   static bool ready[64];
-  const size_t room = HELD ? (size_t)select_bytes(a.pages.cap, a.ctas) : 0;
-  const cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&evict_select_kernel<HELD>), kSelectRoom, ready);
-  return e != cudaSuccess ? e : launch_after(evict_select_kernel<HELD>, units * a.ctas, kSelect, room, st, a, a.ctas, false);
+  const cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&evict_select_kernel), kHeldRoom, ready);
+  if (e != cudaSuccess) return e;
+  const int states = kSelect * 4 * held_fours(a.pages.cap, a.ctas);
+  return launch_after(evict_select_kernel, units * a.ctas, kSelect, (size_t)states * 4 + states / 8, st, a, a.ctas, false);
 }
 
 }  // namespace
@@ -541,7 +660,7 @@ extern "C" int sb_paged_write(const sb_paged_memory* memory, const void* k, long
   a.k_scale = k_scale; a.v_scale = v_scale;
   a.weight = weight; a.born = born; a.after = after;
   const bool e4m3 = m->dtype == SB_F8;
-  const int vecs = m->Hkv * m->dh * (e4m3 ? 1 : 2) / 16;
+  const int vecs = m->Hkv * m->dh / 8;
   a.vecs = fast_div((uint32_t)vecs);
   a.group = std::min(32, std::max(1, 128 / vecs));
   a.rows = some ? (long long)m->B * T : 0;
@@ -607,7 +726,7 @@ extern "C" int sb_paged_evict(const sb_paged_memory* memory, const int* lens, co
   a.moves = a.from + units * p.half;
   a.bits = reinterpret_cast<uint32_t*>(a.moves + units);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = p.held ? evict_select<true>(a, units, st) : evict_select<false>(a, units, st);
+  cudaError_t e = evict_select(a, p.held, units, st);
   if (e == cudaSuccess) {
     auto move = a.row_bytes == 32   ? evict_move_kernel<2>
                 : a.row_bytes == 64 ? evict_move_kernel<4> : a.row_bytes == 128 ? evict_move_kernel<8> : evict_move_kernel<16>;

@@ -476,9 +476,9 @@ def test_evict_lengths_and_pages_outside():
     check_eviction(k, v, table, ints(95, 90, 2 ** 31 - 1, 80, -4), weight, 40, born, None)
 
 
-@pytest.mark.parametrize("cap", [48800, 48960, 140000])
+@pytest.mark.parametrize("cap", [18400, 18560, 48960, 147360, 147520, 300000])
 def test_evict_long(cap):
-    """Lengths that just fit shared memory, just do not, and far longer ones, against a sort."""
+    """One CTA to eight an item and head, places that just fit their shared memory, just do not, and far more, against a sort."""
     import sarbon_b200 as sb
     g = gen(cap)
     b, kv_heads, page = 2, 2, 160
