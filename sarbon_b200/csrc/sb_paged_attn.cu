@@ -151,8 +151,16 @@ struct Paged {
 // What states that take no part are read from.
 __device__ uint4 g_zeros[16];
 
-SB_DEV void copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// K and V that are read once pass through the L2 as what goes first: scores written meanwhile are still there for the
+// account (64 x 8160 states in bf16: 176 -> 171 us), and nothing else is driven out.
+SB_DEV uint64_t passing(bool once) {
+  uint64_t p;
+  if (once) asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  else asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+SB_DEV void copy16(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
 }
 SB_DEV void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -189,10 +197,14 @@ SB_DEV uint32_t transposed(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-// Two e4m3 codes as two fp16 values (exact)
-SB_DEV uint32_t widen(uint32_t codes) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
-  return (uint32_t)h.x | (uint32_t)h.y << 16;
+// Four e4m3 codes as two pairs of fp16 values (exact)
+SB_DEV void widen(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "mov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
 }
 
 // Query row r of an (item, key head): token r / group, head r % group.
@@ -283,6 +295,7 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_att
     }
     ++asked;
   };
+  const uint64_t policy = passing(a.blocks == 1);
   const uint32_t own16 = lane % C::LANES * 16, own_at = ring_at + C::at(lane / C::LANES, lane % C::LANES);
   auto copy = [&](int i) {  // the warp's chunk i, whose entries are there
     if (i < mine) {
@@ -305,8 +318,8 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_att
       for (int x = 0; x < CK; x += C::AT_ONCE) {
         const ulonglong2 from = place[warp][x + lane / C::LANES];
         const uint32_t to = (dst ^ C::turn(x)) + x * C::RB;
-        copy16(to, reinterpret_cast<const void*>(from.x + own16));
-        copy16(to + C::HALF, reinterpret_cast<const void*>(from.y + own16));
+        copy16(to, reinterpret_cast<const void*>(from.x + own16), policy);
+        copy16(to + C::HALF, reinterpret_cast<const void*>(from.y + own16), policy);
       }
     }
     copies_done();
@@ -408,8 +421,9 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_att
           ldsm4(kb + C::at(row, 2 * p + (lane >> 4)), f);
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
-            const uint32_t w[4] = {widen(f[2 * z] & 0xFFFFu), widen(f[2 * z + 1] & 0xFFFFu), widen(f[2 * z] >> 16),
-                                   widen(f[2 * z + 1] >> 16)};
+            uint32_t w[4];
+            widen(f[2 * z], w[0], w[2]);
+            widen(f[2 * z + 1], w[1], w[3]);
 #pragma unroll
             for (int y = 0; y < NB; ++y) mma16816<false>(s[kt][y], w, q[2 * p + z][y][0], q[2 * p + z][y][1]);
           }
@@ -550,8 +564,9 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_att
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
               // a register: channels 2g, 2g + 1 of a state, then of the next
-              const uint32_t u = __byte_perm(f[2 * z], 0, 0x3120), v = __byte_perm(f[2 * z + 1], 0, 0x3120);
-              const uint32_t w[4] = {widen(u & 0xFFFFu), widen(u >> 16), widen(v & 0xFFFFu), widen(v >> 16)};
+              uint32_t w[4];
+              widen(__byte_perm(f[2 * z], 0, 0x3120), w[0], w[1]);
+              widen(__byte_perm(f[2 * z + 1], 0, 0x3120), w[2], w[3]);
 #pragma unroll
               for (int y = 0; y < NB; ++y) {
                 mma16816<false>(o[2 * p + z][y], w, hi[y][0], hi[y][1]);

@@ -16,7 +16,6 @@ namespace {
 struct WriteArgs {
   const void *k, *v;
   long long k_row, k_img, v_row, v_img;  // elements
-  int dt;
   Pool kp, vp;
   PageTable pages;
   const int *at, *count, *stamp;
@@ -35,22 +34,36 @@ struct WriteArgs {
 constexpr int kWriteWarps = 8;
 
 // Eight elements as a pool holds them.  MODE 0: as they are; 1: e4m3 of x * scale; 2: e4m3 of x / scale
-template <int MODE>
-SB_DEV void put_vec(uint64_t to, const Raw8& r, int dt, float scale) {
+template <int MODE, bool BF16>
+SB_DEV void put_vec(uint64_t to, const uint4& r, float scale) {
   if constexpr (MODE == 0) {
-    *reinterpret_cast<uint4*>(to) = r.lo;
+    *reinterpret_cast<uint4*>(to) = r;
   } else {
-    float f[8];
-    unpack8(r, dt, f);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    uint32_t c[4];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) f[u] = MODE == 1 ? f[u] * scale : __fdiv_rn(f[u], scale);
-    *reinterpret_cast<uint2*>(to) =
-        make_uint2((uint32_t)e4m3x2_of(f[0], f[1]) | (uint32_t)e4m3x2_of(f[2], f[3]) << 16,
-                   (uint32_t)e4m3x2_of(f[4], f[5]) | (uint32_t)e4m3x2_of(f[6], f[7]) << 16);
+    for (int u = 0; u < 4; ++u) {
+      const float2 f = pair_of(w[u], BF16 ? SB_BF16 : SB_F16);
+      c[u] = MODE == 1 ? e4m3x2_of(f.x * scale, f.y * scale) : e4m3x2_of(__fdiv_rn(f.x, scale), __fdiv_rn(f.y, scale));
+    }
+    *reinterpret_cast<uint2*>(to) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+  }
+}
+// Eight 16-bit elements from element i on.
+template <bool ALIGNED>
+SB_DEV uint4 load_vec(const void* p, long long i) {
+  const uint16_t* q = static_cast<const uint16_t*>(p) + i;
+  if constexpr (ALIGNED) {
+    return *reinterpret_cast<const uint4*>(q);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w[u] = (uint32_t)q[2 * u] | (uint32_t)q[2 * u + 1] << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
-template <int MODE, bool ALIGNED>
+template <int MODE, bool ALIGNED, bool BF16>
 __global__ void __launch_bounds__(kWriteWarps * 32, MODE == 2 ? 2 : 4) paged_write_kernel(const __grid_constant__ WriteArgs a) {
   constexpr int kAhead = 4, bytes = MODE ? 8 : 16;  // vectors of K and V at once, bytes of one in the pool
   if (blockIdx.x >= a.row_blocks) {  // new lengths, then weights and stamps, neighbours along t
@@ -90,7 +103,7 @@ __global__ void __launch_bounds__(kWriteWarps * 32, MODE == 2 ? 2 : 4) paged_wri
   __syncwarp();
   const int total = rows * (int)a.vecs.d;
   for (int i0 = lane; i0 < total; i0 += 32 * kAhead) {
-    Raw8 k[kAhead], v[kAhead];
+    uint4 k[kAhead], v[kAhead];
     ulonglong2 where[kAhead];
 #pragma unroll
     for (int x = 0; x < kAhead; ++x) {
@@ -103,16 +116,16 @@ __global__ void __launch_bounds__(kWriteWarps * 32, MODE == 2 ? 2 : 4) paged_wri
           where[x].x += c * bytes;
           where[x].y += c * bytes;
           const longlong2 s = from[warp][r];
-          k[x] = ALIGNED ? load_raw8(a.k, a.dt, s.x + c * 8) : load_raw8_tail(a.k, a.dt, s.x + c * 8, 8);
-          v[x] = ALIGNED ? load_raw8(a.v, a.dt, s.y + c * 8) : load_raw8_tail(a.v, a.dt, s.y + c * 8, 8);
+          k[x] = load_vec<ALIGNED>(a.k, s.x + c * 8);
+          v[x] = load_vec<ALIGNED>(a.v, s.y + c * 8);
         }
       }
     }
 #pragma unroll
     for (int x = 0; x < kAhead; ++x)
       if (where[x].x) {
-        put_vec<MODE>(where[x].x, k[x], a.dt, a.k_scale);
-        put_vec<MODE>(where[x].y, v[x], a.dt, a.v_scale);
+        put_vec<MODE, BF16>(where[x].x, k[x], a.k_scale);
+        put_vec<MODE, BF16>(where[x].y, v[x], a.v_scale);
       }
   }
 }
@@ -556,17 +569,21 @@ __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const __gri
   const long long c = (long long)h * a.row_bytes + lane % LANES * 16;
   const int *to = a.to + unit * a.half, *from = a.from + unit * a.half;
   constexpr int AT_ONCE = 32 / LANES;
-  for (int i0 = (part * kMoveWarps + warp) * 32; i0 < moves; i0 += a.parts * kMoveWarps * 32) {
+  const int stride = a.parts * kMoveWarps * 32;
+  int i0 = (part * kMoveWarps + warp) * 32, d = i0 + lane < moves ? to[i0 + lane] : -1, s = d < 0 ? 0 : from[i0 + lane];
+  for (; i0 < moves; i0 += stride) {
     ulonglong2 p = make_ulonglong2(0, 0), q = p;
-    if (i0 + lane < moves) {
+    if (d >= 0) {
       uint32_t dr, sr;
-      const int d = to[i0 + lane], s = from[i0 + lane];
       const int dp = a.pages.entry(b, (uint32_t)d, dr), sp = a.pages.entry(b, (uint32_t)s, sr);
       if (a.pages.has(dp) && a.pages.has(sp)) {
         p = make_ulonglong2(a.k.row_at(sp, sr), a.v.row_at(sp, sr));
         q = make_ulonglong2(a.k.row_at(dp, dr), a.v.row_at(dp, dr));
       }
     }
+    const int next = i0 + stride + lane;  // the next pair's places, on their way meanwhile
+    d = next < moves ? to[next] : -1;
+    s = d < 0 ? 0 : from[next];
     __syncwarp();
     source[warp][lane] = p;
     target[warp][lane] = q;
@@ -651,7 +668,6 @@ extern "C" int sb_paged_write(const sb_paged_memory* memory, const void* k, long
   WriteArgs a{};
   a.k = k; a.k_row = k_row; a.k_img = k_img;
   a.v = v; a.v_row = v_row; a.v_img = v_img;
-  a.dt = dtype;
   a.kp = k_pool(m);
   a.vp = v_pool(m);
   a.pages = page_table(m);
@@ -679,9 +695,12 @@ extern "C" int sb_paged_write(const sb_paged_memory* memory, const void* k, long
     a.k_scale = 1.f / k_scale;
     a.v_scale = 1.f / v_scale;
   }
-  auto kernel = !e4m3  ? (vec ? paged_write_kernel<0, true> : paged_write_kernel<0, false>)
-                : exact ? (vec ? paged_write_kernel<1, true> : paged_write_kernel<1, false>)
-                        : (vec ? paged_write_kernel<2, true> : paged_write_kernel<2, false>);
+  const bool bf16 = dtype == SB_BF16;
+  auto kernel = !e4m3   ? (vec ? paged_write_kernel<0, true, false> : paged_write_kernel<0, false, false>)
+                : exact ? (bf16 ? (vec ? paged_write_kernel<1, true, true> : paged_write_kernel<1, false, true>)
+                                : (vec ? paged_write_kernel<1, true, false> : paged_write_kernel<1, false, false>))
+                        : (bf16 ? (vec ? paged_write_kernel<2, true, true> : paged_write_kernel<2, false, true>)
+                                : (vec ? paged_write_kernel<2, true, false> : paged_write_kernel<2, false, false>));
   kernel<<<(unsigned)blocks, kWriteWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(a);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SB_OK : record_error(SB_ECUDA, cudaGetErrorString(e));

@@ -39,51 +39,44 @@ _MEMORY = struct.Struct("@PPqqqqPqiiiiiii4x")  # sb_paged_memory
 PAGE_DTYPES = {torch.float16: _lib.SB_F16, torch.bfloat16: _lib.SB_BF16, E4M3: _lib.SB_F8}
 
 
-def _pool(t, what, shape, dtype):
-    """(pointer, row stride, page stride) in elements of a pool [P, page, C]."""
-    if t.shape != shape or t.dtype != dtype:
-        raise ValueError(f"{what}: expected {tuple(shape)} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
-    pages, page, width = shape
-    img, row, one = t.stride()
-    if one != 1 and width > 1:
-        raise ValueError(f"{what}: channels must be contiguous")
-    if page <= 1:
-        row = width
-    if pages <= 1:
-        img = page * row
-    return t.data_ptr(), row, img
-
-
-def _own_pool(pool, what, shape):
-    """A pool that is written: no row lies on another."""
-    _, row, img = pool
-    pages, page, width = shape
-    if (page > 1 and row < width) or (pages > 1 and img < row * (page - 1) + width and not
-                                      (img >= width and (page == 1 or row >= img * (pages - 1) + width))):
-        raise ValueError(f"{what}: rows overlap")
+def _overlap(row, img, pages, page, width):
+    """Whether rows of a pool with these strides lie on one another."""
+    return (page > 1 and row < width) or (pages > 1 and img < row * (page - 1) + width and not
+                                          (img >= width and (page == 1 or row >= img * (pages - 1) + width)))
 
 
 def _memory(k_pages, v_pages, table, kv_heads, written=False):
     """The memory of a call: (sb_paged_memory, batch, page, entries, dim)."""
-    if k_pages.dim() != 3 or k_pages.dtype not in PAGE_DTYPES:
-        raise ValueError("k_pages, v_pages: [P, page, kv_heads * dim] pools of fp16, bf16 or e4m3")
     shape, dtype = k_pages.shape, k_pages.dtype
+    code = PAGE_DTYPES.get(dtype)
+    if len(shape) != 3 or code is None or v_pages.shape != shape or v_pages.dtype != dtype:
+        raise ValueError("k_pages, v_pages: [P, page, kv_heads * dim] pools of one shape and type, fp16, bf16 or e4m3")
     pages, page, width = shape
-    if kv_heads < 1 or page < 1 or width % kv_heads or width // kv_heads not in (32, 64, 128):
+    dim = width // kv_heads if kv_heads >= 1 else 0
+    if page < 1 or dim not in (32, 64, 128) or dim * kv_heads != width:
         raise ValueError("pools: pages of one state or more, key heads of 32, 64 or 128 channels")
-    kp, vp = _pool(k_pages, "k_pages", shape, dtype), _pool(v_pages, "v_pages", shape, dtype)
+    (k_img, k_row, k_one), (v_img, v_row, v_one) = k_pages.stride(), v_pages.stride()
+    if k_one != 1 or v_one != 1:
+        raise ValueError("pools: channels must be contiguous")
+    # the stride of a dimension of one element is arbitrary and never used
+    if page == 1:
+        k_row = v_row = width
+    if pages <= 1:
+        k_img, v_img = page * k_row, page * v_row
+    k, v = k_pages.data_ptr(), v_pages.data_ptr()
     if written:
-        _own_pool(kp, "k_pages", shape)
-        _own_pool(vp, "v_pages", shape)
-        _apart((v_pages,), (k_pages,))
-    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
+        if _overlap(k_row, k_img, *shape) or _overlap(v_row, v_img, *shape):
+            raise ValueError("pools: rows overlap")
+        if k == v and pages:
+            raise ValueError("results need their own memory")
+    at, step = table.shape, table.stride()
+    if len(at) != 2 or table.dtype != torch.int32 or (at[1] > 1 and step[1] != 1):
         raise ValueError("table: int32 [B, N] with contiguous rows")
-    b, n = table.shape
+    b, n = at
     if n * page >= 1 << 30:
         raise ValueError("table: fewer than 2^30 states an item")
-    dim = width // kv_heads
-    return _MEMORY.pack(kp[0], vp[0], kp[1], kp[2], vp[1], vp[2], table.data_ptr(), table.stride(0) if b > 1 else n,
-                        PAGE_DTYPES[dtype], pages, page, n, b, kv_heads, dim), b, page, n, dim
+    return _MEMORY.pack(k, v, k_row, k_img, v_row, v_img, table.data_ptr(), step[0] if b > 1 else n, code, pages, page, n, b,
+                        kv_heads, dim), b, page, n, dim
 
 
 def _each(t, what, b):
@@ -218,7 +211,8 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
             raise ValueError("stamp: int32 [B, T] or [B]")
         s = stamp.stride()
         sp = (stamp.data_ptr(), s[0], s[1] if stamp.dim() == 2 else 0)
-    _apart((k_pages, v_pages), (k, v))
+    if kp[0] and (kp[0] in (k_pages.data_ptr(), v_pages.data_ptr()) or vp[0] in (k_pages.data_ptr(), v_pages.data_ptr())):
+        raise ValueError("results need their own memory")
     p_after = _each(after, "after", b)
     if after is not None:
         _clear_of((after,), (at, count))
