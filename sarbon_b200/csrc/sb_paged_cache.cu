@@ -163,20 +163,24 @@ SB_DEV uint32_t ordered(float w) {
   const uint32_t u = w == 0.f ? 0u : __float_as_uint(w);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+// A pass's bits of a key, and those of the passes before it.
+SB_DEV int bin_of(uint32_t key, int pass) { return pass == 0 ? key >> 21 : pass == 1 ? key >> 10 & 2047u : key & 1023u; }
+SB_DEV uint32_t prefix_of(uint32_t key, int pass) { return pass == 0 ? 0u : pass == 1 ? key & 0xFFE00000u : key & 0xFFFFFC00u; }
+SB_DEV uint32_t as_prefix(int bin, int pass) { return (uint32_t)bin << (pass == 0 ? 21 : pass == 1 ? 10 : 0); }
 
 // What the CTAs of an (item, key head) tell each other; bins and counts are never written twice.
 struct Told {
-  int bins[3][kBins];
-  int counts[4][2];
-  int room[2][kSelectWarps], found[2];
+  int bins[4][kBins];  // the first pass's of the protected and of the others, the second's, the third's
+  int counts[3][2];
+  int room[2][kSelectWarps], found[3];
 };
 SB_DEV void all_sync(int ctas) {
   if (ctas > 1) cluster_sync();
   else __syncthreads();
 }
 
-// Sums of two numbers over the threads before this one and over all, of all CTAs; the c-th such sum.
-SB_DEV void before_and_all(int (&v)[2], int (&total)[2], Told& told, int c, int ctas, uint32_t rank) {
+// Sums of two numbers over the threads before this one and over all of the CTA.
+SB_DEV void before_and_all(int (&v)[2], int (&total)[2], Told& told) {
   const int lane = lane_id(), warp = warp_id();
   int s[2] = {v[0], v[1]};
 #pragma unroll
@@ -203,6 +207,10 @@ SB_DEV void before_and_all(int (&v)[2], int (&total)[2], Told& told, int c, int 
     v[y] = before;
     total[y] = all;
   }
+}
+// The same over all CTAs; the c-th such sum.
+SB_DEV void before_and_all(int (&v)[2], int (&total)[2], Told& told, int c, int ctas, uint32_t rank) {
+  before_and_all(v, total, told);
   if (ctas > 1) {
     if (threadIdx.x == 0) {
       told.counts[c][0] = total[0];
@@ -222,21 +230,25 @@ SB_DEV void before_and_all(int (&v)[2], int (&total)[2], Told& told, int c, int 
   }
 }
 
-// The bin of a pass, counted from the top, that holds the need-th number; need becomes its place in the bin, same how
-// many the bin holds.
-SB_DEV int find_bin(Told& told, int pass, int& need, int& same, int ctas) {
-  const int lane = lane_id(), warp = warp_id(), first = kBins - 4 - 4 * (int)threadIdx.x;  // four bins a thread
-  all_sync(ctas);
-  int c[4] = {0, 0, 0, 0};
+// The bin of all CTAs' bins, which they have told, that holds the need-th number from the top; need becomes its place in
+// the bin, same how many the bin holds.
+SB_DEV int find_bin(Told& told, const int* bins, int& need, int& same, int ctas) {
+  constexpr int each = kBins / kSelect;  // bins a thread
+  static_assert(each == 4, "16 bytes");
+  const int lane = lane_id(), warp = warp_id(), first = kBins - each * (1 + (int)threadIdx.x);
+  int c[each], sum = 0;
+#pragma unroll
+  for (int x = 0; x < each; ++x) c[x] = 0;
   for (uint32_t r = 0; r < (uint32_t)ctas; ++r) {
-    const uint4 u = ctas > 1 ? peer_words(&told.bins[pass][first], r) : *reinterpret_cast<const uint4*>(&told.bins[pass][first]);
+    const uint4 u = ctas > 1 ? peer_words(bins + first, r) : *reinterpret_cast<const uint4*>(bins + first);
     c[0] += (int)u.w;
     c[1] += (int)u.z;
     c[2] += (int)u.y;
     c[3] += (int)u.x;
   }
-  const int four = c[0] + c[1] + c[2] + c[3];
-  int s = four;
+#pragma unroll
+  for (int x = 0; x < each; ++x) sum += c[x];
+  int s = sum;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) {
     const int u = __shfl_up_sync(0xFFFFFFFFu, s, x);
@@ -245,60 +257,55 @@ SB_DEV int find_bin(Told& told, int pass, int& need, int& same, int ctas) {
   __syncthreads();
   if (lane == 31) told.room[0][warp] = s;
   __syncthreads();
-  int above = s - four;
+  int above = s - sum;
   for (int w = 0; w < warp; ++w) above += told.room[0][w];
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
+  for (int x = 0; x < each; ++x) {
     if (above < need && need <= above + c[x]) {
-      told.found[0] = first + 3 - x;
+      told.found[0] = first + each - 1 - x;
       told.found[1] = above;
-      told.room[1][0] = c[x];
+      told.found[2] = c[x];
     }
     above += c[x];
   }
   __syncthreads();
-  const int bin = told.found[0];
   need -= told.found[1];
-  same = told.room[1][0];
-  return bin;
+  same = told.found[2];
+  return told.found[0];
 }
-// A pass's bits of a key, and those of the passes before it.
-SB_DEV int bin_of(uint32_t key, int pass) { return pass == 0 ? key >> 21 : pass == 1 ? key >> 10 & 2047u : key & 1023u; }
-SB_DEV uint32_t prefix_of(uint32_t key, int pass) { return pass == 0 ? 0u : pass == 1 ? key & 0xFFE00000u : key & 0xFFFFFC00u; }
-SB_DEV uint32_t as_prefix(int bin, int pass) { return (uint32_t)bin << (pass == 0 ? 21 : pass == 1 ? 10 : 0); }
 
-// What both selections end with: the pairs' weights and stamps, zeros from the new length on.
-SB_DEV void finish(const EvictArgs& a, long long unit, int moves, int left, const int* to, const int* from, int ctas, uint32_t rank) {
-  const long long at = unit * a.pages.cap;
-  all_sync(ctas);
-  for (int i = (int)rank * kSelect + (int)threadIdx.x; i < moves; i += ctas * kSelect) {
-    const int d = to[i], s = from[i];
-    a.weight_out[at + d] = a.weight[at + s];
-    if (a.born) a.born_out[at + d] = a.born[at + s];
-  }
-  all_sync(ctas);  // where the results lie on the operands: read before they are cleared
-  for (int j = left + (int)rank * kSelect + (int)threadIdx.x; j < a.pages.cap; j += ctas * kSelect) {
-    a.weight_out[at + j] = 0.f;
-    if (a.born) a.born_out[at + j] = 0;
-  }
-  if (threadIdx.x == 0 && rank == 0) a.moves[unit] = moves;
-  if (ctas > 1) cluster_sync();  // no CTA ends while another reads what it told
-}
-// An item within its budget: as it is.
-SB_DEV void keep_all_of(const EvictArgs& a, long long unit, int len, int ctas, uint32_t rank) {
-  const long long at = unit * a.pages.cap;
+// An item within its budget stays as it is.  Places from the new length on are cleared here where the results lie in
+// memory of their own; where they lie on the operands, those of states that go are, and the second
+// kernel clears those of states that move once it has read them.
+SB_DEV void keep_all_of(const EvictArgs& a, long long at, int len, int ctas, uint32_t rank) {
   for (int j = (int)rank * kSelect + (int)threadIdx.x; j < len; j += ctas * kSelect) {
     if (a.weight_out != a.weight) a.weight_out[at + j] = a.weight[at + j];
     if (a.born_out != a.born) a.born_out[at + j] = a.born[at + j];
   }
 }
+SB_DEV void finish(const EvictArgs& a, long long unit, int moves, int len, int left, int ctas, uint32_t rank) {
+  const long long at = unit * a.pages.cap;
+  const int w_from = a.weight_out != a.weight ? left : len, b_from = a.born_out != a.born ? left : len;
+  for (int j = left + (int)rank * kSelect + (int)threadIdx.x; j < a.pages.cap; j += ctas * kSelect) {
+    if (j >= w_from) a.weight_out[at + j] = 0.f;
+    if (a.born && j >= b_from) a.born_out[at + j] = 0;
+  }
+  if (threadIdx.x == 0 && rank == 0) a.moves[unit] = moves;
+  if (ctas > 1) cluster_sync();  // no CTA ends while another reads what it told
+}
+// A state that goes from its place, which nothing fills.
+SB_DEV void clear_own(const EvictArgs& a, long long at) {
+  if (a.weight_out == a.weight) a.weight_out[at] = 0.f;
+  if (a.born && a.born_out == a.born) a.born_out[at] = 0;
+}
 
 // Selection with the CTA's ordered weights in shared memory: a thread has a run of states, an odd number of fours, so that
 // neighbours' 16-byte reads fall in distinct banks, and their bits (protected, staying) in registers; no pass
-// needs a word with another thread but the counts.
-constexpr int kMostFours = 9;                                 // states a thread: 36; two CTAs an SM
-constexpr int kHeldRoom = kSelect * kMostFours * 4 * 4 + kSelect * kMostFours * 4 / 8 + 16;
+// needs a word with another thread but the counts.  (1024 threads, one CTA an SM, took half as long again for clusters of
+// eight: not all of them find their SMs at once.)
+constexpr int kMostFours = 9;  // states a thread: 36; 107 KB of shared memory, two CTAs an SM
 inline int held_fours(int cap, int ctas) { return ((cap + ctas * kSelect * 4 - 1) / (ctas * kSelect * 4)) | 1; }
+inline int held_bytes(int fours) { return kSelect * 4 * fours * 4 + kSelect * 4 * fours / 8; }
 
 __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_constant__ EvictArgs a) {
   extern __shared__ __align__(16) uint32_t held[];  // weights of the CTA's states, then bits of the protected ones
@@ -308,19 +315,17 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
   const long long unit = blockIdx.x / ctas, at = unit * a.pages.cap;
   const int b = (int)(unit / a.Hkv);
   const int len = a.pages.clamp(a.lens[b]), keep = a.budget(b);
-  int* const to = a.to + unit * a.half;
-  int* const from = a.from + unit * a.half;
   int moves = 0;
   if (len <= keep) {
-    keep_all_of(a, unit, len, ctas, rank);
+    keep_all_of(a, at, len, ctas, rank);
   } else {
     const bool guard = a.born && a.since;
     const int since = guard ? a.since[b] : 0;
     const int fours = ((len + ctas * kSelect * 4 - 1) / (ctas * kSelect * 4)) | 1, run = fours * 4, mine = kSelect * run;
     const int j_cta = (int)rank * mine, here = min(max(len - j_cta, 0), mine);  // the CTA's states
     uint32_t* const bits = held + mine;
-    for (int x = threadIdx.x; x < 3 * kBins; x += kSelect) told.bins[0][x] = 0;
-    int all[2], n[2] = {0, 0};
+    for (int x = threadIdx.x; x < 4 * kBins; x += kSelect) told.bins[0][x] = 0;
+    int n[2] = {0, 0}, all[2];
     constexpr int kAtOnce = 8;
     for (int w0 = warp * 32; w0 < here; w0 += kAtOnce * kSelect) {
       float f[kAtOnce];
@@ -348,13 +353,10 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
         }
       }
     }
-    before_and_all(n, all, told, 0, ctas, rank);
-    // the states among which weights decide: the protected ones where they alone are too many, else the others
-    const bool inner = all[0] >= keep;
-    int need = inner ? keep : keep - all[0], same = 0;
-    uint32_t last = 0xFFFFFFFFu;  // the ordered weight of the last state that stays; `need` of that weight do
+    before_and_all(n, all, told);
+    if (threadIdx.x == 0) told.counts[0][0] = all[0];
     // this thread's run
-    const int j_run = (int)threadIdx.x * run, states = min(max(here - j_run, 0), run);
+    const int j_run = (int)threadIdx.x * run, states = min(max(here - j_run, 0), run), my_fours = (states + 3) / 4;
     const uint64_t valid = states > 0 ? ~0ull >> (64 - states) : 0ull;
     uint64_t safe = 0;
     if (states > 0) {
@@ -364,13 +366,40 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
       if (o && w + 2 <= w_last) safe |= (uint64_t)bits[w + 2] << (64 - o);
       safe &= valid;
     }
-    const uint64_t who = inner ? safe : valid & ~safe;
     const uint4* const keys = reinterpret_cast<const uint4*>(held + j_run);
-    const int my_fours = (states + 3) / 4;
+    {  // the first pass for both classes, before it is known which of them weights decide among
+      // (many states may have one weight, new ones 0: runs of a bin are counted before they are added)
+      int bin = -1, count = 0;
+      for (int i = 0; i < my_fours; ++i) {
+        const uint4 k = keys[i];
+        const uint32_t key[4] = {k.x, k.y, k.z, k.w}, is = (uint32_t)(valid >> (4 * i)), other = (uint32_t)(~safe >> (4 * i));
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (is >> y & 1u) {
+            const int x = bin_of(key[y], 0) + (other >> y & 1u ? kBins : 0);
+            if (x != bin) {
+              if (count) atomicAdd(&told.bins[0][bin], count);
+              bin = x;
+              count = 0;
+            }
+            ++count;
+          }
+      }
+      if (count) atomicAdd(&told.bins[0][bin], count);
+    }
+    all_sync(ctas);
+    if (ctas > 1) {
+      all[0] = 0;
+      for (uint32_t r = 0; r < (uint32_t)ctas; ++r) all[0] += (int)peer_word(&told.counts[0][0], r);
+    }
+    // the states among which weights decide: the protected ones where they alone are too many, else the others
+    const bool inner = all[0] >= keep;
+    const uint64_t who = inner ? safe : valid & ~safe;
+    int need = inner ? keep : keep - all[0], same = 0;
+    uint32_t last = 0xFFFFFFFFu;  // the ordered weight of the last state that stays; `need` of that weight do
     if (need > 0) {
-      last = 0;
-      for (int pass = 0; pass < 3; ++pass) {
-        // (many states may have one weight, new ones 0: runs of a bin are counted before they are added)
+      last = as_prefix(find_bin(told, told.bins[inner ? 0 : 1], need, same, ctas), 0);
+      for (int pass = 1; pass < 3; ++pass) {
         int bin = -1, count = 0;
         for (int i = 0; i < my_fours; ++i) {
           const uint4 k = keys[i];
@@ -380,15 +409,16 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
             if ((nibble >> y & 1u) && prefix_of(key[y], pass) == last) {
               const int x = bin_of(key[y], pass);
               if (x != bin) {
-                if (count) atomicAdd(&told.bins[pass][bin], count);
+                if (count) atomicAdd(&told.bins[1 + pass][bin], count);
                 bin = x;
                 count = 0;
               }
               ++count;
             }
         }
-        if (count) atomicAdd(&told.bins[pass][bin], count);
-        last |= as_prefix(find_bin(told, pass, need, same, ctas), pass);
+        if (count) atomicAdd(&told.bins[1 + pass][bin], count);
+        all_sync(ctas);
+        last |= as_prefix(find_bin(told, told.bins[1 + pass], need, same, ctas), pass);
       }
     }
     uint64_t more = 0, tied = 0;
@@ -413,10 +443,14 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
     int put[2] = {__popcll(free), __popcll(move)}, total[2];
     before_and_all(put, total, told, 2, ctas, rank);
     moves = total[1];
+    int* const to = a.to + unit * a.half;
+    int* const from = a.from + unit * a.half;
     for (; free; free &= free - 1) to[put[0]++] = j_cta + j_run + __ffsll(free) - 1;
     for (; move; move &= move - 1) from[put[1]++] = j_cta + j_run + __ffsll(move) - 1;
+    if (a.weight_out == a.weight || (a.born && a.born_out == a.born))
+      for (uint64_t gone = valid & ~low & ~stays; gone; gone &= gone - 1) clear_own(a, at + j_cta + j_run + __ffsll(gone) - 1);
   }
-  finish(a, unit, moves, min(len, keep), to, from, ctas, rank);
+  finish(a, unit, moves, len, min(len, keep), ctas, rank);
 }
 
 // The same for longer ones, from memory: a warp's states lie behind one another, 32 at a time, their bits in memory too.
@@ -427,21 +461,19 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_long_kernel(const __g
   const long long unit = blockIdx.x / ctas, at = unit * a.pages.cap;
   const int b = (int)(unit / a.Hkv);
   const int len = a.pages.clamp(a.lens[b]), keep = a.budget(b);
-  int* const to = a.to + unit * a.half;
-  int* const from = a.from + unit * a.half;
   int moves = 0;
   if (len <= keep) {
-    keep_all_of(a, unit, len, ctas, rank);
+    keep_all_of(a, at, len, ctas, rank);
   } else {
     constexpr int kAtOnce = 8;
     const bool guard = a.born && a.since;
     const int since = guard ? a.since[b] : 0;
     const int warps = kSelectWarps * ctas, words = (len + 31) / 32, steps = (words + warps - 1) / warps;
-    const int w_first = min(((int)rank * kSelectWarps + warp) * steps, words), w_end = min(w_first + steps, words);
+    const int w_first = min(((int)rank * (kSelectWarps) + warp) * steps, words), w_end = min(w_first + steps, words);
     uint32_t* const guarded = a.bits + unit * 2 * ((a.pages.cap + 31) / 32);
     uint32_t* const stay = guarded + (a.pages.cap + 31) / 32;
     auto key_of = [&](int w) { return w < w_end && w * 32 + lane < len ? ordered(a.weight[at + w * 32 + lane]) : 0u; };
-    for (int x = threadIdx.x; x < 3 * kBins; x += kSelect) told.bins[0][x] = 0;
+    for (int x = threadIdx.x; x < 4 * kBins; x += kSelect) told.bins[0][x] = 0;
     int all[2], n[2] = {0, 0};
     for (int w0 = w_first; w0 < w_end; w0 += kAtOnce) {
       int s[kAtOnce];
@@ -496,7 +528,8 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_long_kernel(const __g
             }
           }
         }
-        last |= as_prefix(find_bin(told, pass, need, same, ctas), pass);
+        all_sync(ctas);
+        last |= as_prefix(find_bin(told, told.bins[pass], need, same, ctas), pass);
       }
     }
     const bool some = need > 0, choose = same > need;
@@ -528,7 +561,6 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_long_kernel(const __g
             ties += __popc(tied);
           }
           const uint32_t stays = more | first | (inner ? 0u : guarded[w] & here);
-          __syncwarp();
           if (lane == 0) {
             stay[w] = stays;
             put[0] += __popc(~stays & low & here);
@@ -539,21 +571,24 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_long_kernel(const __g
     }
     before_and_all(put, total, told, 2, ctas, rank);
     moves = total[1];
+    int* const to = a.to + unit * a.half;
+    int* const from = a.from + unit * a.half;
     int at_free = __shfl_sync(0xFFFFFFFFu, put[0], 0), at_move = __shfl_sync(0xFFFFFFFFu, put[1], 0);
     for (int w = w_first; w < w_end; ++w) {
-      const uint32_t s = stay[w], low = bits_below(w * 32, keep), below = (1u << lane) - 1u;
-      const uint32_t f = ~s & low & bits_below(w * 32, len), m = s & ~low;
+      const uint32_t s = stay[w], low = bits_below(w * 32, keep), here = bits_below(w * 32, len), below = (1u << lane) - 1u;
+      const uint32_t f = ~s & low & here, m = s & ~low;
       if (f >> lane & 1u) to[at_free + __popc(f & below)] = w * 32 + lane;
       if (m >> lane & 1u) from[at_move + __popc(m & below)] = w * 32 + lane;
+      if ((here & ~low & ~s) >> lane & 1u) clear_own(a, at + w * 32 + lane);
       at_free += __popc(f);
       at_move += __popc(m);
     }
   }
-  finish(a, unit, moves, min(len, keep), to, from, ctas, rank);
+  finish(a, unit, moves, len, min(len, keep), ctas, rank);
 }
 
-// Rows of the pairs: a warp takes 32 pairs, a lane looks up where a pair's rows lie, then all copy them, 16 bytes a lane,
-// four loads of K and four of V in flight.  And the new lengths, which may lie on the old ones: nothing but the
+// Rows, weights and stamps of the pairs: a warp takes 32 pairs, a lane looks up where a pair's rows lie, then all copy
+// them, 16 bytes a lane, four loads of K and four of V in flight.  And the new lengths, which may lie on the old ones: nothing but the
 // thread that writes an item's reads it here.
 constexpr int kMoveWarps = 4, kMoveAhead = 4;
 template <int LANES>
@@ -574,6 +609,10 @@ __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const __gri
   for (; i0 < moves; i0 += stride) {
     ulonglong2 p = make_ulonglong2(0, 0), q = p;
     if (d >= 0) {
+      const long long w = unit * a.pages.cap;
+      a.weight_out[w + d] = a.weight[w + s];
+      if (a.born) a.born_out[w + d] = a.born[w + s];
+      clear_own(a, w + s);
       uint32_t dr, sr;
       const int dp = a.pages.entry(b, (uint32_t)d, dr), sp = a.pages.entry(b, (uint32_t)s, sr);
       if (a.pages.has(dp) && a.pages.has(sp)) {
@@ -641,10 +680,10 @@ EvictPlan evict_plan(int B, int Hkv, int cap, int sms) {
 cudaError_t evict_select(const EvictArgs& a, bool held, long long units, cudaStream_t st) {
   if (!held) return launch_after(evict_select_long_kernel, units * a.ctas, kSelect, 0, st, a, a.ctas, false);
   static bool ready[64];
-  const cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&evict_select_kernel), kHeldRoom, ready);
+  const cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&evict_select_kernel), held_bytes(kMostFours), ready);
   if (e != cudaSuccess) return e;
-  const int states = kSelect * 4 * held_fours(a.pages.cap, a.ctas);
-  return launch_after(evict_select_kernel, units * a.ctas, kSelect, (size_t)states * 4 + states / 8, st, a, a.ctas, false);
+  return launch_after(evict_select_kernel, units * a.ctas, kSelect, (size_t)held_bytes(held_fours(a.pages.cap, a.ctas)), st, a,
+                      a.ctas, false);
 }
 
 }  // namespace
