@@ -585,7 +585,7 @@ SB_API int sb_paged_write(const sb_paged_memory* memory, const void* k, long lon
 SB_API int sb_paged_evict(const sb_paged_memory* memory, const int* lens, const int* keep, int keep_all, const int* since,
                           const float* weight, const int* born, float* weight_out, int* born_out, int* after, void* work,
                           long long work_bytes, void* stream);
-SB_API int sb_paged_evict_work(int B, int Hkv, int page, int N, long long* bytes);
+SB_API int sb_paged_evict_work(int B, int Hkv, int page, int N, int in_place, long long* bytes); /* in_place: after is lens */
 
 /* Counters (fused_engine.py:92,239) and sticky device errors (synchronises). */
 SB_API int sb_stats(sb_engine* e, void* stream, sb_stats_t* out);

@@ -123,7 +123,7 @@ PROTOTYPES = {
     "sb_paged_attention_work": (_I, [_I] * 9 + [C.POINTER(_LL)]),
     "sb_paged_write": (_I, [C.c_char_p] + [_P, _LL, _LL] * 2 + [_I, _P, _P, _I] + [C.c_float] * 2 + [_P, _P, _P, _LL, _LL, _P, _P]),
     "sb_paged_evict": (_I, [C.c_char_p, _P, _P, _I] + [_P] * 7 + [_LL, _P]),
-    "sb_paged_evict_work": (_I, [_I] * 4 + [C.POINTER(_LL)]),
+    "sb_paged_evict_work": (_I, [_I] * 5 + [C.POINTER(_LL)]),
     "sb_stats": (_I, [_P, _P, C.POINTER(Stats)]),
     "sb_last_launch_count": (_I, [_P]),
     "sb_destroy": (_I, [_P]),

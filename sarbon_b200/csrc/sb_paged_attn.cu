@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_att
 #pragma unroll
     for (int x = 0; x < KS; ++x) o[x][y][0] = o[x][y][1] = o[x][y][2] = o[x][y][3] = 0.f;
   }
-  float* const scores = a.scores ? a.plane(b * a.Hkv + kvh, block) : nullptr;
+  float* const scores = a.scores ? a.plane(b * a.Hkv + kvh, block) : a.weight ? reinterpret_cast<float*>(smem + C::SMEM) : nullptr;
   const int chunk0 = at.c - (int)done;  // of the unit: chunk0 + warp + i * kWarps
 
   const int i_first = i;
@@ -862,8 +862,11 @@ void shape_of(int pt, int rows, int& chunk, int& occ) {
          : pt == SB_BF16 ? shape_of<DH, SB_BF16>(rows, chunk, occ) : shape_of<DH, SB_F16>(rows, chunk, occ);
 }
 
+constexpr int kHeldScores = 1536;  // 6 KB: as many CTAs an SM as without
+
 struct PagedPlan {
   int rows, blocks, shares, ends, chunk, part_rows, places, score_rows;
+  bool held;  // scores in shared memory
   long long units, scores, part_o, part_l;  // floats of the workspace
   long long bytes() const { return (scores + part_o + part_l) * 4; }
 };
@@ -891,7 +894,8 @@ PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int pt, int cap, boo
   auto even = [](long long n) { return (n + 3) / 4 * 4; };
   p.places = (cap + 3) / 4 * 4;
   for (p.score_rows = 1; p.score_rows < p.part_rows;) p.score_rows *= 2;
-  p.scores = account ? (long long)B * Hkv * p.blocks * p.places * p.score_rows : 0;
+  p.held = account && p.ends == 0 && p.places * p.score_rows <= kHeldScores;
+  p.scores = account && !p.held ? (long long)B * Hkv * p.blocks * p.places * p.score_rows : 0;
   const long long slots = p.units + p.shares;
   p.part_o = apart ? slots * p.part_rows * dh : 0;
   p.part_l = p.ends > 0 ? even(slots * p.part_rows) : 0;
@@ -901,9 +905,10 @@ PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int pt, int cap, boo
 template <int DH, int PT, int NB>
 cudaError_t launch(const PagedArgs& a, long long ctas, cudaStream_t st) {
   static bool ready[64];
-  const cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&paged_attend_kernel<DH, PT, NB>), Paged<DH, PT, NB>::SMEM, ready);
+  constexpr int room = Paged<DH, PT, NB>::SMEM, most = room + kHeldScores * 4;
+  const cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&paged_attend_kernel<DH, PT, NB>), most, ready);
   if (e != cudaSuccess) return e;
-  paged_attend_kernel<DH, PT, NB><<<(unsigned)ctas, kWarps * 32, Paged<DH, PT, NB>::SMEM, st>>>(a);
+  paged_attend_kernel<DH, PT, NB><<<(unsigned)ctas, kWarps * 32, a.weight && !a.scores ? most : room, st>>>(a);
   return cudaGetLastError();
 }
 template <int DH, int PT>
@@ -974,7 +979,7 @@ extern "C" int sb_paged_attention(const sb_paged_memory* memory, const void* q, 
   a.v_scale = v_scale;
   a.o = {out, o_row, o_img};
   a.lse = lse;
-  a.weight = p.scores > 0 ? weight : nullptr;  // (no places: no account)
+  a.weight = p.scores > 0 || p.held ? weight : nullptr;  // (no places: no account)
   a.decay = decay;
   float* w = static_cast<float*>(work);
   a.scores = p.scores > 0 ? w : nullptr;

@@ -149,7 +149,7 @@ struct EvictArgs {
   const int* born;
   int* born_out;
   int* after;
-  int B, Hkv, row_bytes, half, parts, ctas;
+  int B, Hkv, row_bytes, half, parts, ctas;  // parts: CTAs a unit of the second kernel; 0: none, the first does it all
   int *to, *from, *moves;  // workspace: [units][half], [units][half], [units]
   uint32_t* bits;          // [units][2][cap / 32]: states that are protected, that stay, where shared memory has no room
   SB_DEV int budget(int b) const { return pages.clamp(keep ? keep[b] : keep_all); }
@@ -290,13 +290,71 @@ SB_DEV void finish(const EvictArgs& a, long long unit, int moves, int len, int l
     if (j >= w_from) a.weight_out[at + j] = 0.f;
     if (a.born && j >= b_from) a.born_out[at + j] = 0;
   }
-  if (threadIdx.x == 0 && rank == 0) a.moves[unit] = moves;
+  if (a.parts && threadIdx.x == 0 && rank == 0) a.moves[unit] = moves;
   if (ctas > 1) cluster_sync();  // no CTA ends while another reads what it told
 }
 // A state that goes from its place, which nothing fills.
 SB_DEV void clear_own(const EvictArgs& a, long long at) {
   if (a.weight_out == a.weight) a.weight_out[at] = 0.f;
   if (a.born && a.born_out == a.born) a.born_out[at] = 0;
+}
+
+// Rows, weights and stamps of the pairs: a warp takes 32 of them from i0 on, then those `stride` on; a lane looks up where
+// a pair's rows lie, then all copy them, 16 bytes a lane, four loads of K and four of V in flight.
+constexpr int kMoveWarps = 4, kMoveAhead = 4;
+struct Pairs {
+  ulonglong2 source[32], target[32];  // addresses of K and V; 0: nowhere
+};
+template <int LANES>
+SB_DEV void move_pairs(const EvictArgs& a, long long unit, const int* to, const int* from, int moves, int i0, int stride, Pairs& pairs) {
+  constexpr int AT_ONCE = 32 / LANES;
+  const int lane = lane_id(), b = (int)(unit / a.Hkv), h = (int)(unit - (long long)b * a.Hkv);
+  const long long c = (long long)h * a.row_bytes + lane % LANES * 16, at = unit * a.pages.cap;
+  int d = i0 + lane < moves ? to[i0 + lane] : -1, s = d < 0 ? 0 : from[i0 + lane];
+  for (; i0 < moves; i0 += stride) {
+    ulonglong2 p = make_ulonglong2(0, 0), q = p;
+    if (d >= 0) {
+      a.weight_out[at + d] = a.weight[at + s];
+      if (a.born) a.born_out[at + d] = a.born[at + s];
+      clear_own(a, at + s);
+      uint32_t dr, sr;
+      const int dp = a.pages.entry(b, (uint32_t)d, dr), sp = a.pages.entry(b, (uint32_t)s, sr);
+      if (a.pages.has(dp) && a.pages.has(sp)) {
+        p = make_ulonglong2(a.k.row_at(sp, sr), a.v.row_at(sp, sr));
+        q = make_ulonglong2(a.k.row_at(dp, dr), a.v.row_at(dp, dr));
+      }
+    }
+    const int next = i0 + stride + lane;  // the next pair's places, on their way meanwhile
+    d = next < moves ? to[next] : -1;
+    s = d < 0 ? 0 : from[next];
+    __syncwarp();
+    pairs.source[lane] = p;
+    pairs.target[lane] = q;
+    __syncwarp();
+#pragma unroll
+    for (int x0 = 0; x0 < LANES; x0 += kMoveAhead) {
+      if (i0 + x0 * AT_ONCE >= moves) break;
+      uint4 k[kMoveAhead], v[kMoveAhead];
+#pragma unroll
+      for (int x = 0; x < kMoveAhead; ++x)
+        if (x0 + x < LANES) {
+          const ulonglong2 from_row = pairs.source[(x0 + x) * AT_ONCE + lane / LANES];
+          if (from_row.x) {
+            k[x] = *reinterpret_cast<const uint4*>(from_row.x + c);
+            v[x] = *reinterpret_cast<const uint4*>(from_row.y + c);
+          }
+        }
+#pragma unroll
+      for (int x = 0; x < kMoveAhead; ++x)
+        if (x0 + x < LANES) {
+          const ulonglong2 to_row = pairs.target[(x0 + x) * AT_ONCE + lane / LANES];
+          if (to_row.x) {
+            *reinterpret_cast<uint4*>(to_row.x + c) = k[x];
+            *reinterpret_cast<uint4*>(to_row.y + c) = v[x];
+          }
+        }
+    }
+  }
 }
 
 // Selection with the CTA's ordered weights in shared memory: a thread has a run of states, an odd number of fours, so that
@@ -306,6 +364,9 @@ SB_DEV void clear_own(const EvictArgs& a, long long at) {
 constexpr int kMostFours = 9;  // states a thread: 36; 107 KB of shared memory, two CTAs an SM
 inline int held_fours(int cap, int ctas) { return ((cap + ctas * kSelect * 4 - 1) / (ctas * kSelect * 4)) | 1; }
 inline int held_bytes(int fours) { return kSelect * 4 * fours * 4 + kSelect * 4 * fours / 8; }
+// A memory of up to this many places is evicted from by one kernel: at most half of them move, 512 KB a CTA.
+constexpr int kOneKernel = 2048;
+static_assert(sizeof(Told) >= kSelectWarps * sizeof(Pairs), "room for the pairs");
 
 __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_constant__ EvictArgs a) {
   extern __shared__ __align__(16) uint32_t held[];  // weights of the CTA's states, then bits of the protected ones
@@ -443,13 +504,23 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
     int put[2] = {__popcll(free), __popcll(move)}, total[2];
     before_and_all(put, total, told, 2, ctas, rank);
     moves = total[1];
-    int* const to = a.to + unit * a.half;
-    int* const from = a.from + unit * a.half;
+    // one kernel: the pairs in shared memory, behind the bits
+    int* const to = a.parts ? a.to + unit * a.half : reinterpret_cast<int*>(bits + mine / 32);
+    int* const from = a.parts ? a.from + unit * a.half : to + a.half;
     for (; free; free &= free - 1) to[put[0]++] = j_cta + j_run + __ffsll(free) - 1;
     for (; move; move &= move - 1) from[put[1]++] = j_cta + j_run + __ffsll(move) - 1;
     if (a.weight_out == a.weight || (a.born && a.born_out == a.born))
       for (uint64_t gone = valid & ~low & ~stays; gone; gone &= gone - 1) clear_own(a, at + j_cta + j_run + __ffsll(gone) - 1);
+    if (a.parts == 0) {
+      __syncthreads();
+      Pairs& pairs = reinterpret_cast<Pairs*>(&told)[warp];  // (the counts are not looked at again)
+      if (a.row_bytes == 32) move_pairs<2>(a, unit, to, from, moves, warp * 32, kSelect, pairs);
+      else if (a.row_bytes == 64) move_pairs<4>(a, unit, to, from, moves, warp * 32, kSelect, pairs);
+      else if (a.row_bytes == 128) move_pairs<8>(a, unit, to, from, moves, warp * 32, kSelect, pairs);
+      else move_pairs<16>(a, unit, to, from, moves, warp * 32, kSelect, pairs);
+    }
   }
+  if (a.parts == 0 && threadIdx.x == 0 && unit % a.Hkv == 0) a.after[b] = min(len, keep);
   finish(a, unit, moves, len, min(len, keep), ctas, rank);
 }
 
@@ -587,70 +658,20 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_long_kernel(const __g
   finish(a, unit, moves, len, min(len, keep), ctas, rank);
 }
 
-// Rows, weights and stamps of the pairs: a warp takes 32 pairs, a lane looks up where a pair's rows lie, then all copy
-// them, 16 bytes a lane, four loads of K and four of V in flight.  And the new lengths, which may lie on the old ones: nothing but the
-// thread that writes an item's reads it here.
-constexpr int kMoveWarps = 4, kMoveAhead = 4;
+// The pairs of longer memories, and the new lengths, which may lie on the old ones: nothing but the thread that writes
+// an item's reads it here.
 template <int LANES>
 __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const __grid_constant__ EvictArgs a) {
-  __shared__ ulonglong2 source[kMoveWarps][32], target[kMoveWarps][32];  // addresses of K and V; 0: nowhere
-  const int warp = warp_id(), lane = lane_id();
-  const int part = blockIdx.x % a.parts;
+  __shared__ Pairs pairs[kMoveWarps];
+  const int part = blockIdx.x % a.parts, warp = warp_id();
   const long long unit = blockIdx.x / a.parts;
-  const int b = (int)(unit / a.Hkv), h = (int)(unit - (long long)b * a.Hkv);
   grid_dep_wait();
-  if (h == 0 && part == 0 && threadIdx.x == 0) a.after[b] = min(a.pages.clamp(a.lens[b]), a.budget(b));
-  const int moves = a.moves[unit];
-  const long long c = (long long)h * a.row_bytes + lane % LANES * 16;
-  const int *to = a.to + unit * a.half, *from = a.from + unit * a.half;
-  constexpr int AT_ONCE = 32 / LANES;
-  const int stride = a.parts * kMoveWarps * 32;
-  int i0 = (part * kMoveWarps + warp) * 32, d = i0 + lane < moves ? to[i0 + lane] : -1, s = d < 0 ? 0 : from[i0 + lane];
-  for (; i0 < moves; i0 += stride) {
-    ulonglong2 p = make_ulonglong2(0, 0), q = p;
-    if (d >= 0) {
-      const long long w = unit * a.pages.cap;
-      a.weight_out[w + d] = a.weight[w + s];
-      if (a.born) a.born_out[w + d] = a.born[w + s];
-      clear_own(a, w + s);
-      uint32_t dr, sr;
-      const int dp = a.pages.entry(b, (uint32_t)d, dr), sp = a.pages.entry(b, (uint32_t)s, sr);
-      if (a.pages.has(dp) && a.pages.has(sp)) {
-        p = make_ulonglong2(a.k.row_at(sp, sr), a.v.row_at(sp, sr));
-        q = make_ulonglong2(a.k.row_at(dp, dr), a.v.row_at(dp, dr));
-      }
-    }
-    const int next = i0 + stride + lane;  // the next pair's places, on their way meanwhile
-    d = next < moves ? to[next] : -1;
-    s = d < 0 ? 0 : from[next];
-    __syncwarp();
-    source[warp][lane] = p;
-    target[warp][lane] = q;
-    __syncwarp();
-#pragma unroll
-    for (int x0 = 0; x0 < LANES; x0 += kMoveAhead) {
-      if (i0 + x0 * AT_ONCE >= moves) break;
-      uint4 k[kMoveAhead], v[kMoveAhead];
-#pragma unroll
-      for (int x = 0; x < kMoveAhead; ++x)
-        if (x0 + x < LANES) {
-          const ulonglong2 at = source[warp][(x0 + x) * AT_ONCE + lane / LANES];
-          if (at.x) {
-            k[x] = *reinterpret_cast<const uint4*>(at.x + c);
-            v[x] = *reinterpret_cast<const uint4*>(at.y + c);
-          }
-        }
-#pragma unroll
-      for (int x = 0; x < kMoveAhead; ++x)
-        if (x0 + x < LANES) {
-          const ulonglong2 at = target[warp][(x0 + x) * AT_ONCE + lane / LANES];
-          if (at.x) {
-            *reinterpret_cast<uint4*>(at.x + c) = k[x];
-            *reinterpret_cast<uint4*>(at.y + c) = v[x];
-          }
-        }
-    }
+  if (part == 0 && threadIdx.x == 0 && unit % a.Hkv == 0) {
+    const int b = (int)(unit / a.Hkv);
+    a.after[b] = min(a.pages.clamp(a.lens[b]), a.budget(b));
   }
+  move_pairs<LANES>(a, unit, a.to + unit * a.half, a.from + unit * a.half, a.moves[unit], (part * kMoveWarps + warp) * 32,
+                    a.parts * kMoveWarps * 32, pairs[warp]);
 }
 
 struct EvictPlan {
@@ -660,8 +681,9 @@ struct EvictPlan {
   long long bytes() const { return (lists + moves + bits) * 4; }
 };
 // CTAs an (item, key head): doubled while all are resident at once (two an SM) and each still has 2048 places, or until
-// the weights fit shared memory.
-EvictPlan evict_plan(int B, int Hkv, int cap, int sms) {
+// the weights fit shared memory.  apart: the new lengths do not lie on the old ones, which one kernel's CTAs read at
+// any time.
+EvictPlan evict_plan(int B, int Hkv, int cap, bool apart, int sms) {
   const long long units = (long long)B * Hkv;
   EvictPlan p{};
   p.half = std::max(1, cap / 2);  // at most min(keep, len - keep) states move
@@ -670,6 +692,7 @@ EvictPlan evict_plan(int B, int Hkv, int cap, int sms) {
   while (p.ctas < kMostCtas && ((2 * units * p.ctas <= 2 * sms && cap / p.ctas > 2048) || held_fours(cap, p.ctas) > kMostFours))
     p.ctas *= 2;
   p.held = held_fours(cap, p.ctas) <= kMostFours;
+  if (cap <= kOneKernel && apart) return p;
   p.parts = (int)std::max(1ll, std::min(((long long)p.half + kMoveWarps * 32 - 1) / (kMoveWarps * 32), (16ll * sms + units - 1) / units));
   p.lists = 2 * units * p.half;
   p.moves = units;
@@ -682,8 +705,8 @@ cudaError_t evict_select(const EvictArgs& a, bool held, long long units, cudaStr
   static bool ready[64];
   const cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&evict_select_kernel), held_bytes(kMostFours), ready);
   if (e != cudaSuccess) return e;
-  return launch_after(evict_select_kernel, units * a.ctas, kSelect, (size_t)held_bytes(held_fours(a.pages.cap, a.ctas)), st, a,
-                      a.ctas, false);
+  const int room = held_bytes(held_fours(a.pages.cap, a.ctas)) + (a.parts ? 0 : 2 * a.half * 4);
+  return launch_after(evict_select_kernel, units * a.ctas, kSelect, (size_t)room, st, a, a.ctas, false);
 }
 
 }  // namespace
@@ -745,13 +768,13 @@ extern "C" int sb_paged_write(const sb_paged_memory* memory, const void* k, long
   return e == cudaSuccess ? SB_OK : record_error(SB_ECUDA, cudaGetErrorString(e));
 }
 
-extern "C" int sb_paged_evict_work(int B, int Hkv, int page, int N, long long* bytes) {
+extern "C" int sb_paged_evict_work(int B, int Hkv, int page, int N, int in_place, long long* bytes) {
   if (!bytes || !paged_sizes_ok(B, Hkv, 32, 0, page, N)) return record_error(SB_EINVAL, "sb_paged_evict_work: arguments");
   *bytes = 0;
   if (B == 0) return SB_OK;
   const int sms = xattn_sms();
   if (sms == 0) return record_error(SB_ECUDA, "sb_paged_evict_work: device");
-  *bytes = evict_plan(B, Hkv, N * page, sms).bytes();
+  *bytes = evict_plan(B, Hkv, N * page, !in_place, sms).bytes();
   return SB_OK;
 }
 
@@ -763,13 +786,13 @@ extern "C" int sb_paged_evict(const sb_paged_memory* memory, const int* lens, co
   if (m->B == 0) return SB_OK;
   if (!lens || !after || (m->N > 0 && (!weight || !weight_out)) || (since && !born) || (!born) != (!born_out) || !paged_pools_ok(m))
     return record_error(SB_EINVAL, "sb_paged_evict: rows (16-byte aligned, strides multiples of 16 bytes) or null argument");
-  if (!work || (reinterpret_cast<uintptr_t>(work) & 15) != 0)
+  EvictArgs a{};
+  a.pages = page_table(m);
+  if ((a.pages.cap > kOneKernel || after == lens) && (!work || (reinterpret_cast<uintptr_t>(work) & 15) != 0))
     return record_error(SB_EINVAL, "sb_paged_evict: workspace (sb_paged_evict_work bytes, 16-byte aligned)");
   const int sms = xattn_sms();
   if (sms == 0) return record_error(SB_ECUDA, "sb_paged_evict: device");
-  EvictArgs a{};
-  a.pages = page_table(m);
-  const EvictPlan p = evict_plan(m->B, m->Hkv, a.pages.cap, sms);
+  const EvictPlan p = evict_plan(m->B, m->Hkv, a.pages.cap, after != lens, sms);
   if (work_bytes < p.bytes()) return record_error(SB_EINVAL, "sb_paged_evict: workspace (sb_paged_evict_work bytes, 16-byte aligned)");
   a.k = k_pool(m);
   a.v = v_pool(m);
@@ -785,7 +808,7 @@ extern "C" int sb_paged_evict(const sb_paged_memory* memory, const int* lens, co
   a.bits = reinterpret_cast<uint32_t*>(a.moves + units);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = evict_select(a, p.held, units, st);
-  if (e == cudaSuccess) {
+  if (e == cudaSuccess && p.parts) {
     auto move = a.row_bytes == 32   ? evict_move_kernel<2>
                 : a.row_bytes == 64 ? evict_move_kernel<4> : a.row_bytes == 128 ? evict_move_kernel<8> : evict_move_kernel<16>;
     e = launch_after(move, units * a.parts, kMoveWarps * 32, 0, st, a);

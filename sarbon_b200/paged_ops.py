@@ -30,9 +30,10 @@ from __future__ import annotations
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
-from .memory_ops import _HALVES, _INF, _apart, _launch, _new, _ready, _rows, _statistics, _work
+from .memory_ops import _INF, _apart, _launch, _new, _ready, _rows, _statistics, _work
 
 E4M3 = torch.float8_e4m3fn
 _MEMORY = struct.Struct("@PPqqqqPqiiiiiii4x")  # sb_paged_memory
@@ -81,8 +82,6 @@ def _memory(k_pages, v_pages, table, kv_heads, written=False):
 
 def _each(t, what, b):
     """Pointer of an int32 [B]."""
-    if t is None:
-        return None
     if t.dtype != torch.int32 or t.shape != (b,) or (b > 1 and t.stride(0) != 1):
         raise ValueError(f"{what}: contiguous int32 [B]")
     return t.data_ptr()
@@ -90,11 +89,29 @@ def _each(t, what, b):
 
 def _account(t, what, shape, dtype):
     """Pointer of weights or stamps."""
-    if t is None:
-        return None
     if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
         raise ValueError(f"{what}: contiguous {dtype} {tuple(shape)}")
     return t.data_ptr()
+
+
+def _one_device(floats, others):
+    """memory_ops._ready for a call of many tensors, of which only `floats` could need a gradient."""
+    if forward_ad._current_level >= 0:
+        return _ready(*floats, *others)
+    index = floats[0].get_device()
+    if index < 0:
+        raise ValueError("tensors of one CUDA device")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError("tensors of one CUDA device")
+    grad = torch.is_grad_enabled()
+    for t in floats:
+        if t is not None:
+            if t.get_device() != index or not t.is_cuda:
+                raise ValueError("tensors of one CUDA device")
+            if grad and t.requires_grad:
+                raise ValueError("no autograd graph is recorded: call under torch.no_grad() or from an autograd.Function")
+    return index
 
 
 def _scales(k_scale, v_scale, dtype):
@@ -133,42 +150,47 @@ def paged_attention(q, k_pages, v_pages, table, lens, heads, kv_heads=None, scal
 
     Made for single tokens: the states are read once for every 16 query rows of a key head, and split
     over the SMs where there are few rows; many queries want cross_attention."""
-    if q.dim() != 3 or q.dtype not in _HALVES:
+    dtype, page_dtype = q.dtype, k_pages.dtype
+    if q.dim() != 3 or (dtype != torch.bfloat16 and dtype != torch.float16):
         raise ValueError("q: [B, T, heads * dim] rows of fp16 or bf16")
     if kv_heads is None:
         kv_heads = heads
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError("heads: a multiple of kv_heads")
     memory, b, page, n, dim = _memory(k_pages, v_pages, table, kv_heads)
-    tq, dtype = q.shape[1], q.dtype
-    if k_pages.dtype not in (dtype, E4M3):
+    if page_dtype != dtype and page_dtype != E4M3:
         raise ValueError("pages: q's type or e4m3")
+    tq = q.shape[1]
     shape = (b, tq, heads * dim)
     if scale is None:
         scale = dim ** -0.5
     if not 0.0 < scale < _INF or not 0.0 <= decay <= 1.0:
         raise ValueError("scale: a positive number; decay: from 0 to 1")
-    _scales(k_scale, v_scale, k_pages.dtype)
-    qp, p_lens = _rows(q, "q", shape, dtype), _each(lens, "lens", b)
-    if p_lens is None:
+    if k_scale != 1.0 or v_scale != 1.0:
+        _scales(k_scale, v_scale, page_dtype)
+    if lens is None:
         raise ValueError("lens: contiguous int32 [B]")
-    p_weight = _account(weight, "weight", (b, kv_heads, n * page), torch.float32)
+    qp, p_lens = _rows(q, "q", shape, dtype), _each(lens, "lens", b)
+    p_weight = p_lse = None
+    if weight is not None:
+        p_weight = _account(weight, "weight", (b, kv_heads, n * page), torch.float32)
     if lse is not None:
         _statistics(lse, b, heads, tq)
+        p_lse = lse.data_ptr()
+        if weight is not None:
+            _clear_of((weight, lse), ())
     if out is not None:
         op = _rows(out, "out", shape, dtype, out=True)
         _apart((out,), (q, k_pages, v_pages))
-    if weight is not None and lse is not None:
-        _clear_of((weight, lse), ())
-    index = _ready(q, k_pages, v_pages, table, lens, weight, out, lse)
+    index = _one_device((q, k_pages, v_pages, weight, out, lse), (table, lens))
     if out is None:
         out, op = _new(q, shape, dtype)
     if b == 0 or tq == 0:
         return out
-    hold, work, size = _work("sb_paged_attention_work", index, b, heads, kv_heads, dim, tq, PAGE_DTYPES[k_pages.dtype], page, n,
-                             weight is not None)
+    hold, work, size = _work("sb_paged_attention_work", index, b, heads, kv_heads, dim, tq, PAGE_DTYPES[page_dtype], page, n,
+                             p_weight is not None)
     _launch("sb_paged_attention", index, memory, *qp, PAGE_DTYPES[dtype], p_lens, heads, tq, scale, k_scale, v_scale, causal, *op,
-            None if lse is None else lse.data_ptr(), p_weight, decay, work, size)
+            p_lse, p_weight, decay, work, size)
     return out
 
 
@@ -183,40 +205,44 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
     behind an item's pages, on no page or from ``count[b]`` on keep what they hold.  An item's pages that are
     written must be its own.  after (allocated if None) shares no memory with at.  kv_heads is that of weight
     or born where they are given; without them the rows are taken as heads of 32 channels."""
-    if k.dim() != 3 or k.dtype not in _HALVES:
+    dtype, page_dtype, rows = k.dtype, k_pages.dtype, k.shape
+    if len(rows) != 3 or (dtype != torch.bfloat16 and dtype != torch.float16):
         raise ValueError("k, v: [B, T, kv_heads * dim] rows of fp16 or bf16")
     if (born is None) != (stamp is None):
         raise ValueError("born and stamp: both or neither")
-    for t in (weight, born):
-        if t is not None:
-            if t.dim() != 3 or (kv_heads is not None and t.shape[1] != kv_heads):
-                raise ValueError("weight, born: [B, kv_heads, N * page]")
-            kv_heads = t.shape[1]
     if kv_heads is None:
-        kv_heads = k.shape[2] // 32
+        like = weight if weight is not None else born
+        if like is not None and like.dim() != 3:
+            raise ValueError("weight, born: [B, kv_heads, N * page]")
+        kv_heads = rows[2] // 32 if like is None else like.shape[1]
     memory, b, page, n, dim = _memory(k_pages, v_pages, table, kv_heads, written=True)
-    t, dtype = k.shape[1], k.dtype
-    if k_pages.dtype not in (dtype, E4M3):
+    if page_dtype != dtype and page_dtype != E4M3:
         raise ValueError("pages: the states' type or e4m3")
-    _scales(k_scale, v_scale, k_pages.dtype)
-    shape, places = (b, t, kv_heads * dim), (b, kv_heads, n * page)
+    if k_scale != 1.0 or v_scale != 1.0:
+        _scales(k_scale, v_scale, page_dtype)
+    t = rows[1]
+    shape = (b, t, kv_heads * dim)
     kp, vp = _rows(k, "k", shape, dtype), _rows(v, "v", shape, dtype)
-    p_at, p_count = _each(at, "at", b), _each(count, "count", b)
-    if p_at is None:
-        raise ValueError("at: contiguous int32 [B]")
-    p_weight, p_born = _account(weight, "weight", places, torch.float32), _account(born, "born", places, torch.int32)
-    sp = (None, 0, 0)
-    if stamp is not None:
-        if stamp.dtype != torch.int32 or stamp.shape not in ((b,), (b, t)):
-            raise ValueError("stamp: int32 [B, T] or [B]")
-        s = stamp.stride()
-        sp = (stamp.data_ptr(), s[0], s[1] if stamp.dim() == 2 else 0)
-    if kp[0] and (kp[0] in (k_pages.data_ptr(), v_pages.data_ptr()) or vp[0] in (k_pages.data_ptr(), v_pages.data_ptr())):
+    pools = k_pages.data_ptr(), v_pages.data_ptr()
+    if (kp[0] in pools or vp[0] in pools) and kp[0]:
         raise ValueError("results need their own memory")
-    p_after = _each(after, "after", b)
+    if at is None:
+        raise ValueError("at: contiguous int32 [B]")
+    p_at, p_count, p_weight, p_born, sp = _each(at, "at", b), None, None, None, _NO_STAMP
+    if count is not None:
+        p_count = _each(count, "count", b)
+    if weight is not None:
+        p_weight = _account(weight, "weight", (b, kv_heads, n * page), torch.float32)
+    if born is not None:
+        p_born = _account(born, "born", (b, kv_heads, n * page), torch.int32)
+        if stamp.dtype != torch.int32 or stamp.shape not in ((b, t), (b,)):
+            raise ValueError("stamp: int32 [B, T] or [B]")
+        step = stamp.stride()
+        sp = stamp.data_ptr(), step[0], step[1] if len(step) == 2 else 0
     if after is not None:
+        p_after = _each(after, "after", b)
         _clear_of((after,), (at, count))
-    index = _ready(k, v, k_pages, v_pages, table, at, count, weight, born, stamp, after)
+    index = _one_device((k, v, k_pages, v_pages, weight), (table, at, count, born, stamp, after))
     if after is None:
         after = torch.empty_like(at)
         p_after = after.data_ptr()
@@ -225,6 +251,9 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
     _launch("sb_paged_write", index, memory, *kp, *vp, PAGE_DTYPES[dtype], p_at, p_count, t, k_scale, v_scale, p_weight, p_born,
             *sp, p_after)
     return after
+
+
+_NO_STAMP = (None, 0, 0)
 
 
 # ---------------------------------------------------------------- eviction
@@ -239,44 +268,54 @@ def paged_evict(k_pages, v_pages, table, lens, weight, keep, born=None, since=No
     (born None without born).  after, weight_out and born_out (allocated if None) may be lens, weight and born
     themselves and otherwise share no memory with them.  An item's pages must be its own; rows on
     no page are not moved."""
-    if weight.dim() != 3:
+    places = weight.shape
+    if len(places) != 3:
         raise ValueError("weight: [B, kv_heads, N * page]")
-    kv_heads = weight.shape[1]
+    kv_heads = places[1]
     memory, b, page, n, dim = _memory(k_pages, v_pages, table, kv_heads, written=True)
-    places = (b, kv_heads, n * page)
-    if since is not None and born is None:
-        raise ValueError("since needs born")
-    if born is None and born_out is not None:
-        raise ValueError("born_out needs born")
-    p_lens, p_since, p_after = _each(lens, "lens", b), _each(since, "since", b), _each(after, "after", b)
-    if p_lens is None:
-        raise ValueError("lens: contiguous int32 [B]")
-    p_keep, keep_all = None, 0
+    if places != (b, kv_heads, n * page) or lens is None:
+        raise ValueError("weight: [B, kv_heads, N * page]; lens: contiguous int32 [B]")
+    pw, p_lens = _account(weight, "weight", places, torch.float32), _each(lens, "lens", b)
+    pb = p_since = p_keep = None
+    if born is not None:
+        pb = _account(born, "born", places, torch.int32)
+    elif since is not None or born_out is not None:
+        raise ValueError("since and born_out need born")
+    if since is not None:
+        p_since = _each(since, "since", b)
+    keep_all = 0
     if isinstance(keep, torch.Tensor):
         p_keep = _each(keep, "keep", b)
     else:
         keep_all = min(int(keep), 1 << 30)
         if keep_all < 0 or keep_all != min(keep, 1 << 30):
             raise ValueError("keep: a whole number from 0 on, or int32 [B]")
-    pw, pb = _account(weight, "weight", places, torch.float32), _account(born, "born", places, torch.int32)
-    pwo, pbo = _account(weight_out, "weight_out", places, torch.float32), _account(born_out, "born_out", places, torch.int32)
+    pwo = pbo = p_after = None
     if weight_out is not None or born_out is not None or after is not None:
-        same = (pwo is not None and pwo == pw, pbo is not None and pbo == pb, p_after is not None and p_after == p_lens)
-        _clear_of((None if same[0] else weight_out, None if same[1] else born_out, None if same[2] else after),
-                  (weight, born, lens, since, keep if p_keep is not None else None))
-    index = _ready(k_pages, v_pages, table, lens, weight, born, since, keep if p_keep is not None else None, weight_out,
-                   born_out, after)
+        own = []
+        if weight_out is not None:
+            pwo = _account(weight_out, "weight_out", places, torch.float32)
+            own.append(weight_out if pwo != pw else None)
+        if born_out is not None:
+            pbo = _account(born_out, "born_out", places, torch.int32)
+            own.append(born_out if pbo != pb else None)
+        if after is not None:
+            p_after = _each(after, "after", b)
+            own.append(after if p_after != p_lens else None)
+        _clear_of(own, (weight, born, lens, since, keep if p_keep is not None else None))
+    index = _one_device((k_pages, v_pages, weight, weight_out),
+                        (table, lens, born, since, keep if p_keep is not None else None, born_out, after))
     if after is None:
         after = torch.empty_like(lens)
         p_after = after.data_ptr()
     if weight_out is None:
         weight_out = torch.empty_like(weight)
         pwo = weight_out.data_ptr()
-    if born_out is None and born is not None:
+    if pb is not None and born_out is None:
         born_out = torch.empty_like(born)
         pbo = born_out.data_ptr()
     if b == 0:
         return after, weight_out, born_out
-    hold, work, size = _work("sb_paged_evict_work", index, b, kv_heads, page, n)
+    hold, work, size = _work("sb_paged_evict_work", index, b, kv_heads, page, n, p_after == p_lens)
     _launch("sb_paged_evict", index, memory, p_lens, p_keep, keep_all, p_since, pw, pb, pwo, pbo, p_after, work, size)
     return after, weight_out, born_out

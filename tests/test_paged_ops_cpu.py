@@ -133,10 +133,10 @@ def test_library_refuses():
     for bad in (dict(k=None), dict(dt=1), dict(dt=3), dict(ks=2.0), dict(m=e4m3, ks=-1.0), dict(at=None), dict(after=None), dict(t=-1),
                 dict(kr=-1)):
         assert write(**bad) == _lib.SB_EINVAL, bad
-    for bad in (dict(lens=None), dict(weight=None), dict(since=one), dict(born=one), dict(born_out=one), dict(work=None),
-                dict(work=C.c_void_p(8))):
+    for bad in (dict(lens=None), dict(weight=None), dict(since=one), dict(born=one), dict(born_out=one), dict(m=memory(page=4096), work=None),
+                dict(m=memory(page=4096), work=C.c_void_p(8))):
         assert evict(**bad) == _lib.SB_EINVAL, bad
     assert lib.sb_paged_attention_work(1, 2, 1, 48, 1, 0, 4, 2, 0, C.byref(n)) == _lib.SB_EINVAL
     assert lib.sb_paged_attention_work(1, 2, 1, 32, 1, 0, 0, 2, 0, C.byref(n)) == _lib.SB_EINVAL
     assert lib.sb_paged_attention_work(1, 2, 1, 32, 1, 1, 4, 2, 0, C.byref(n)) == _lib.SB_EINVAL
-    assert lib.sb_paged_evict_work(1, 0, 4, 2, C.byref(n)) == _lib.SB_EINVAL
+    assert lib.sb_paged_evict_work(1, 0, 4, 2, 0, C.byref(n)) == _lib.SB_EINVAL
