@@ -208,24 +208,27 @@ SB_DEV void before_and_all(int (&v)[2], int (&total)[2], Told& told) {
     total[y] = all;
   }
 }
-// The same over all CTAs; the c-th such sum.
-SB_DEV void before_and_all(int (&v)[2], int (&total)[2], Told& told, int c, int ctas, uint32_t rank) {
+// The same over all CTAs; the c-th such sum.  base: what the CTAs before this one have.
+SB_DEV void before_and_all(int (&v)[2], int (&total)[2], int (&base)[2], Told& told, int c, int ctas, uint32_t rank) {
   before_and_all(v, total, told);
+  base[0] = base[1] = 0;
   if (ctas > 1) {
     if (threadIdx.x == 0) {
       told.counts[c][0] = total[0];
       told.counts[c][1] = total[1];
     }
     cluster_sync();
+    const uint32_t lane = lane_id();
+    int t[2] = {0, 0};  // (a lane a CTA: one trip to the others)
+    if (lane < (uint32_t)ctas) {
+      t[0] = (int)peer_word(&told.counts[c][0], lane);
+      t[1] = (int)peer_word(&told.counts[c][1], lane);
+    }
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
-      int all = 0;
-      for (uint32_t r = 0; r < (uint32_t)ctas; ++r) {
-        const int t = (int)peer_word(&told.counts[c][y], r);
-        if (r < rank) v[y] += t;
-        all += t;
-      }
-      total[y] = all;
+      base[y] = __reduce_add_sync(0xFFFFFFFFu, lane < rank ? t[y] : 0);
+      total[y] = __reduce_add_sync(0xFFFFFFFFu, t[y]);
+      v[y] += base[y];
     }
   }
 }
@@ -239,12 +242,21 @@ SB_DEV int find_bin(Told& told, const int* bins, int& need, int& same, int ctas)
   int c[each], sum = 0;
 #pragma unroll
   for (int x = 0; x < each; ++x) c[x] = 0;
-  for (uint32_t r = 0; r < (uint32_t)ctas; ++r) {
-    const uint4 u = ctas > 1 ? peer_words(bins + first, r) : *reinterpret_cast<const uint4*>(bins + first);
-    c[0] += (int)u.w;
-    c[1] += (int)u.z;
-    c[2] += (int)u.y;
-    c[3] += (int)u.x;
+  for (int r0 = 0; r0 < ctas; r0 += 4) {  // four asked for before one is looked at
+    uint4 u[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      u[r] = make_uint4(0, 0, 0, 0);
+      if (r0 + r < ctas)
+        u[r] = ctas > 1 ? peer_words(bins + first, (uint32_t)(r0 + r)) : *reinterpret_cast<const uint4*>(bins + first);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      c[0] += (int)u[r].w;
+      c[1] += (int)u[r].z;
+      c[2] += (int)u[r].y;
+      c[3] += (int)u[r].x;
+    }
   }
 #pragma unroll
   for (int x = 0; x < each; ++x) sum += c[x];
@@ -310,27 +322,45 @@ SB_DEV void move_pairs(const EvictArgs& a, long long unit, const int* to, const 
   constexpr int AT_ONCE = 32 / LANES;
   const int lane = lane_id(), b = (int)(unit / a.Hkv), h = (int)(unit - (long long)b * a.Hkv);
   const long long c = (long long)h * a.row_bytes + lane % LANES * 16, at = unit * a.pages.cap;
-  int d = i0 + lane < moves ? to[i0 + lane] : -1, s = d < 0 ? 0 : from[i0 + lane];
+  // a lane's pair: its places, the pages and rows they are on, weight and stamp; asked for two rounds and one ahead
+  int d = -1, s = 0, dp = -1, sp = -1, r = 0;
+  uint32_t dr = 0, sr = 0;
+  float w = 0.f;
+  auto places = [&](int i) {
+    d = i < moves ? to[i] : -1;
+    s = d < 0 ? 0 : from[i];
+  };
+  auto look_up = [&] {
+    if (d >= 0) {
+      dp = a.pages.entry(b, (uint32_t)d, dr);
+      sp = a.pages.entry(b, (uint32_t)s, sr);
+      w = a.weight[at + s];
+      if (a.born) r = a.born[at + s];
+    }
+  };
+  places(i0 + lane);
+  look_up();
+  int d_now = d, s_now = s;
+  places(i0 + stride + lane);
   for (; i0 < moves; i0 += stride) {
     ulonglong2 p = make_ulonglong2(0, 0), q = p;
-    if (d >= 0) {
-      a.weight_out[at + d] = a.weight[at + s];
-      if (a.born) a.born_out[at + d] = a.born[at + s];
-      clear_own(a, at + s);
-      uint32_t dr, sr;
-      const int dp = a.pages.entry(b, (uint32_t)d, dr), sp = a.pages.entry(b, (uint32_t)s, sr);
+    if (d_now >= 0) {
       if (a.pages.has(dp) && a.pages.has(sp)) {
         p = make_ulonglong2(a.k.row_at(sp, sr), a.v.row_at(sp, sr));
         q = make_ulonglong2(a.k.row_at(dp, dr), a.v.row_at(dp, dr));
       }
+      a.weight_out[at + d_now] = w;
+      if (a.born) a.born_out[at + d_now] = r;
+      clear_own(a, at + s_now);
     }
-    const int next = i0 + stride + lane;  // the next pair's places, on their way meanwhile
-    d = next < moves ? to[next] : -1;
-    s = d < 0 ? 0 : from[next];
     __syncwarp();
     pairs.source[lane] = p;
     pairs.target[lane] = q;
     __syncwarp();
+    look_up();
+    d_now = d;
+    s_now = s;
+    places(i0 + 2 * stride + lane);
 #pragma unroll
     for (int x0 = 0; x0 < LANES; x0 += kMoveAhead) {
       if (i0 + x0 * AT_ONCE >= moves) break;
@@ -450,8 +480,7 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
     }
     all_sync(ctas);
     if (ctas > 1) {
-      all[0] = 0;
-      for (uint32_t r = 0; r < (uint32_t)ctas; ++r) all[0] += (int)peer_word(&told.counts[0][0], r);
+      all[0] = __reduce_add_sync(0xFFFFFFFFu, lane < ctas ? (int)peer_word(&told.counts[0][0], (uint32_t)lane) : 0);
     }
     // the states among which weights decide: the protected ones where they alone are too many, else the others
     const bool inner = all[0] >= keep;
@@ -493,22 +522,37 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
     more &= who;
     tied &= need > 0 ? who : 0ull;
     if (same > need) {  // more states have the last weight than may stay: the first of them do
-      int ties[2] = {__popcll(tied), 0}, total[2];
-      before_and_all(ties, total, told, 1, ctas, rank);
+      int ties[2] = {__popcll(tied), 0}, total[2], base[2];
+      before_and_all(ties, total, base, told, 1, ctas, rank);
       for (int extra = ties[0] + __popcll(tied) - max(need, ties[0]); extra > 0; --extra) tied &= ~(1ull << (63 - __clzll(tied)));
     }
     const uint64_t stays = more | tied | (inner ? 0ull : safe);
     const int low_n = min(max(keep - j_cta - j_run, 0), states);  // states of the run below keep
     const uint64_t low = low_n > 0 ? ~0ull >> (64 - low_n) : 0ull;
     uint64_t free = low & ~stays, move = stays & ~low;
-    int put[2] = {__popcll(free), __popcll(move)}, total[2];
-    before_and_all(put, total, told, 2, ctas, rank);
+    int put[2] = {__popcll(free), __popcll(move)}, total[2], base[2];
+    before_and_all(put, total, base, told, 2, ctas, rank);
     moves = total[1];
     // one kernel: the pairs in shared memory, behind the bits
     int* const to = a.parts ? a.to + unit * a.half : reinterpret_cast<int*>(bits + mine / 32);
     int* const from = a.parts ? a.from + unit * a.half : to + a.half;
-    for (; free; free &= free - 1) to[put[0]++] = j_cta + j_run + __ffsll(free) - 1;
-    for (; move; move &= move - 1) from[put[1]++] = j_cta + j_run + __ffsll(move) - 1;
+    if (a.parts) {
+      // through shared memory, over the weights, from both ends, and out in whole lines
+      int* const list = reinterpret_cast<int*>(held);
+      int f = put[0] - base[0], m = mine - 1 - (put[1] - base[1]);
+      for (; free; free &= free - 1) list[f++] = j_cta + j_run + __ffsll(free) - 1;
+      for (; move; move &= move - 1) list[m--] = j_cta + j_run + __ffsll(move) - 1;
+      if (threadIdx.x == kSelect - 1) {  // how many of each this CTA has
+        told.found[0] = f;
+        told.found[1] = mine - 1 - m;
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < told.found[0]; i += kSelect) to[base[0] + i] = list[i];
+      for (int i = threadIdx.x; i < told.found[1]; i += kSelect) from[base[1] + i] = list[mine - 1 - i];
+    } else {
+      for (; free; free &= free - 1) to[put[0]++] = j_cta + j_run + __ffsll(free) - 1;
+      for (; move; move &= move - 1) from[put[1]++] = j_cta + j_run + __ffsll(move) - 1;
+    }
     if (a.weight_out == a.weight || (a.born && a.born_out == a.born))
       for (uint64_t gone = valid & ~low & ~stays; gone; gone &= gone - 1) clear_own(a, at + j_cta + j_run + __ffsll(gone) - 1);
     if (a.parts == 0) {
@@ -569,7 +613,8 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_long_kernel(const __g
         }
       }
     }
-    before_and_all(n, all, told, 0, ctas, rank);
+    int base[2];
+    before_and_all(n, all, base, told, 0, ctas, rank);
     const bool inner = all[0] >= keep;
     const uint32_t flip = inner ? 0u : 0xFFFFFFFFu;
     int need = inner ? keep : keep - all[0], same = 0;
@@ -611,7 +656,7 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_long_kernel(const __g
         const uint32_t tied = __ballot_sync(0xFFFFFFFFu, key_of(w) == last) & class_of(w);
         if (lane == 0) t[0] += __popc(tied);
       }
-      before_and_all(t, total, told, 1, ctas, rank);
+      before_and_all(t, total, base, told, 1, ctas, rank);
       ties = __shfl_sync(0xFFFFFFFFu, t[0], 0);
     }
     int put[2] = {0, 0}, total[2];
@@ -640,7 +685,7 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_long_kernel(const __g
         }
       }
     }
-    before_and_all(put, total, told, 2, ctas, rank);
+    before_and_all(put, total, base, told, 2, ctas, rank);
     moves = total[1];
     int* const to = a.to + unit * a.half;
     int* const from = a.from + unit * a.half;
