@@ -569,8 +569,8 @@ SB_API int sb_paged_attention_work(int B, int H, int Hkv, int dh, int Tq, int pa
                                    long long* bytes);
 
 /* New states: row t < count[b] (NULL: T) of k, v [B][T][Hkv*dh] (SB_F16 or SB_BF16, any strides) goes to
- * position at[b] + t of item b; pools of the same type, or SB_F8: the code nearest to x / scale, at most 448
- * of either sign.  weight there becomes 0, born stamp[b * stamp_img + t * stamp_row] (each may be NULL).
+ * position at[b] + t of item b; pools of the same type, or SB_F8: the code nearest to the fp32 quotient
+ * x / scale, at most 448 of either sign.  weight there becomes 0, born stamp[b * stamp_img + t * stamp_row] (each may be NULL).
  * after [B] gets the new lengths and shares no memory with at. */
 SB_API int sb_paged_write(const sb_paged_memory* memory, const void* k, long long k_row, long long k_img, const void* v,
                           long long v_row, long long v_img, int dtype, const int* at, const int* count, int T,

@@ -952,7 +952,7 @@ extern "C" int sb_paged_attention(const sb_paged_memory* memory, const void* q, 
   if (!paged_memory_ok(m) || !paged_attention_sizes_ok(m->B, H, m->Hkv, m->dh, Tq, m->P, m->page, m->N) ||
       (q_dtype != SB_F16 && q_dtype != SB_BF16) || (m->dtype != q_dtype && m->dtype != SB_F8))
     return record_error(SB_EINVAL, "sb_paged_attention: sizes (dh 32, 64 or 128, H a multiple of Hkv) or dtypes");
-  if (!(scale > 0.f) || !scales_ok(m, k_scale, v_scale) || !std::isfinite(scale * k_scale))
+  if (!(scale > 0.f) || !scales_ok(m, k_scale, v_scale) || !std::isnormal(scale * k_scale))
     return record_error(SB_EINVAL, "sb_paged_attention: scale, or scales of pages that are not e4m3");
   if (weight && !(decay >= 0.f && decay <= 1.f)) return record_error(SB_EINVAL, "sb_paged_attention: decay from 0 to 1");
   if (m->B == 0 || Tq == 0) return SB_OK;

@@ -125,7 +125,8 @@ TYPES = [(torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16), (torc
     (1, 1, 1, 1, 1, 32, 1), (2, 1, 240, 8, 8, 32, 20), (3, 1, 63, 4, 2, 64, 7), (2, 1, 17, 6, 2, 128, 16), (2, 3, 300, 9, 3, 64, 1),
     (4, 1, 1030, 16, 2, 128, 64), (1, 5, 2040, 8, 1, 32, 60), (2, 17, 129, 4, 2, 128, 128), (1, 1, 9001, 5, 1, 64, 13),
     (1, 2, 42840, 8, 4, 128, 240), (64, 1, 700, 4, 4, 32, 100), (3, 1, 4097, 32, 1, 128, 48), (1, 33, 515, 2, 1, 64, 5),
-    (160, 1, 1300, 4, 2, 128, 17),
+    (160, 1, 1300, 4, 2, 128, 17), (2, 9, 5000, 8, 2, 64, 33), (3, 3, 9000, 3, 1, 128, 7), (1, 1, 30000, 3, 1, 32, 64),
+    (300, 1, 1100, 2, 1, 128, 50), (2, 1, 384, 4, 1, 64, 8), (2, 1, 388, 4, 1, 64, 4),
 ])
 def test_attention(b, tq, n, heads, kv_heads, dim, page, qt, pt):
     import sarbon_b200 as sb
@@ -257,6 +258,20 @@ def test_attention_strides_and_shared_pages():
     assert same_bits(out[..., heads * dim:], keep[..., heads * dim:])
     turned = k.transpose(0, 1).contiguous().transpose(0, 1)  # the same row of all pages together
     assert same_bits(out[..., :heads * dim], sb.paged_attention(q, turned, v, table, lens, heads, kv_heads=kv_heads))
+
+
+def test_attention_uneven_items():
+    """CTAs share the states of items of very unequal lengths, empty ones among and behind them."""
+    import sarbon_b200 as sb
+    g = gen(12)
+    b, n, heads, kv_heads, dim = 9, 20000, 6, 2, 64
+    k, v, table = pages_of(g, b, n, 100, kv_heads * dim, torch.float16)
+    q = rand(g, b, 2, heads * dim, dtype=torch.float16)
+    for lens in (ints(0, 0, 20000, 1, 0, 33, 12345, 0, 0), ints(*[0] * 8, 17), ints(*[0] * 9), ints(20000, *[0] * 8), ints(*range(500, 509))):
+        lse, weight = torch.empty(b, heads, 2, device="cuda"), rand(g, b, kv_heads, n).abs()
+        before = weight.clone()
+        out = sb.paged_attention(q, k, v, table, lens, heads, kv_heads=kv_heads, causal=True, lse=lse, weight=weight, decay=0.5)
+        check_attention(out, lse, weight, q, k, v, table, lens, heads, kv_heads, before=before, decay=0.5, causal=True)
 
 
 def test_nothing_there():
@@ -474,6 +489,25 @@ def test_evict_lengths_and_pages_outside():
     born = torch.zeros(5, 1, 90, dtype=torch.int32, device="cuda")
     table[1, 2], table[1, 7], table[2, 8], table[3] = -1, k.shape[0], 2 ** 31 - 1, -9
     check_eviction(k, v, table, ints(95, 90, 2 ** 31 - 1, 80, -4), weight, 40, born, None)
+
+
+@pytest.mark.parametrize("n", [900, 30000, 160000])
+def test_evict_partly_in_place(n):
+    """One kernel, clusters and long memories; each result on its operand or apart."""
+    import sarbon_b200 as sb
+    g = gen(n)
+    b, kv_heads, page, keep = 2, 2, 50, n * 2 // 3
+    k, v, table = pages_of(g, b, n, page, kv_heads * 32, E4M3)
+    weight = torch.randint(0, 500, (b, kv_heads, n), device="cuda", generator=g).float()
+    born = torch.randint(0, 99, weight.shape, dtype=torch.int32, device="cuda", generator=g)
+    lens, since, results = ints(n - 1, n // 2), ints(50, 3), []
+    for here in range(8):
+        kk, vv, w, r, m = k.clone(), v.clone(), weight.clone(), born.clone(), lens.clone()
+        own = dict(weight_out=w if here & 1 else None, born_out=r if here & 2 else None, after=m if here & 4 else None)
+        results.append(sb.paged_evict(kk, vv, table, m, w, keep, born=r, since=since, **own) + (kk, vv))
+    assert results[0][0].tolist() == [keep, n // 2]
+    for other in results[1:]:
+        assert all(same_bits(x, y) for x, y in zip(results[0], other))
 
 
 @pytest.mark.parametrize("cap", [18400, 18560, 48960, 147360, 147520, 300000])
