@@ -41,8 +41,8 @@ struct PagedArgs {
   float decay;
   float* scores;  // [B * Hkv][blocks][places][score_rows], log2 units
   int places, score_rows;  // cap and a block's rows, up to a multiple of 4 and a power of two
-  float* part_o;  // [slots][part_rows][dh]
-  float* part_l;  // [slots][part_rows], log2 of the sum
+  float* part_l;  // [units + shares][part_rows], log2 of the sum: what CTA i finds of unit u at i + u
+  float* part_o;  // [2 shares][part_rows][dh]: a CTA's piece of a unit that began before, of one that goes on behind
   int part_rows;  // min(rows, 16)
   SB_DEV int chunks(int b) const { return (pages.clamp(lens[b]) + chunk - 1) / chunk; }
   SB_DEV int units() const { return Hkv * blocks; }  // of an item
@@ -51,8 +51,8 @@ struct PagedArgs {
   }
 };
 
-// How the chunks of all units, one unit after the other, are shared: CTA i gets `each` of them from i * each on.  What
-// CTA i finds of unit u goes to slot i + u: along the chunks i or u grows from one piece to the next.
+// How the chunks of all units, one unit after the other, are shared: CTA i gets `each` of them from i * each on.
+// (Along the chunks i or u grows from one piece to the next, so i + u is a place of its own.)
 struct Shares {
   long long total, each;
   int item;            // the item that position `at` lies in (B: none)
@@ -238,7 +238,8 @@ struct Cursor {
 
 // NB: column tiles of eight query rows
 template <int DH, int PT, int NB>
-__global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_attend_kernel(const __grid_constant__ PagedArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
+    paged_attend_kernel(const __grid_constant__ PagedArgs a) {
   using C = Paged<DH, PT, NB>;
   constexpr bool E4M3 = C::E4M3, BF16 = C::BF16;
   constexpr int CK = C::CK, KT = CK / 16, KS = DH / 16, R = CK > 32 ? 2 : 1;
@@ -341,365 +342,367 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC) paged_att
     const bool whole = piece == at.n;
     const int i_end = done + piece > warp ? (int)((done + piece - warp + kWarps - 1) / kWarps) : 0;
 
-  // Q as the second operand: rows g (+ 8), channels 16 ks + 2 tig (+ 8), or for e4m3 16 ks + 4 tig (+ 2).  e4m3 is
-  // multiplied as fp16: bf16 rows are then brought to at most 2^14 by a power of two, and what falls
-  // below fp16's 2^-24 is less than 2^-37 of the row's largest.
-  uint32_t q[KS][NB][2];
-  float factor[NB][2];  // of rows 2 tig, 2 tig + 1 (+ 8): scores times it are exponents of 2
-  int limit[NB][2];     // states that those rows see
+    // Q as the second operand: rows g (+ 8), channels 16 ks + 2 tig (+ 8), or for e4m3 16 ks + 4 tig (+ 2).  e4m3 is
+    // multiplied as fp16: bf16 rows are then brought to at most 2^14 by a power of two, and what falls
+    // below fp16's 2^-24 is less than 2^-37 of the row's largest.
+    uint32_t q[KS][NB][2];
+    float factor[NB][2];  // of rows 2 tig, 2 tig + 1 (+ 8): scores times it are exponents of 2
+    int limit[NB][2];     // states that those rows see
 #pragma unroll
-  for (int y = 0; y < NB; ++y) {
-    const bool has = g + 8 * y < rows;
-    const Row w(a, kvh, has ? r0 + g + 8 * y : 0);
-    const uint16_t* p = static_cast<const uint16_t*>(a.q) + b * a.q_img + w.t * a.q_row + (long long)w.h * DH;
+    for (int y = 0; y < NB; ++y) {
+      const bool has = g + 8 * y < rows;
+      const Row w(a, kvh, has ? r0 + g + 8 * y : 0);
+      const uint16_t* p = static_cast<const uint16_t*>(a.q) + b * a.q_img + w.t * a.q_row + (long long)w.h * DH;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int c = E4M3 ? ks * 16 + 4 * tig : ks * 16 + 2 * tig;
-      q[ks][y][0] = has ? *reinterpret_cast<const uint32_t*>(p + c) : 0u;
-      q[ks][y][1] = has ? *reinterpret_cast<const uint32_t*>(p + c + (E4M3 ? 2 : 8)) : 0u;
-    }
-    int up = 0;
-    if (E4M3 && a.q_bf16) {
-      uint32_t top = 0;
+      for (int ks = 0; ks < KS; ++ks) {
+        const int c = E4M3 ? ks * 16 + 4 * tig : ks * 16 + 2 * tig;
+        q[ks][y][0] = has ? *reinterpret_cast<const uint32_t*>(p + c) : 0u;
+        q[ks][y][1] = has ? *reinterpret_cast<const uint32_t*>(p + c + (E4M3 ? 2 : 8)) : 0u;
+      }
+      int up = 0;
+      if (E4M3 && a.q_bf16) {
+        uint32_t top = 0;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) top = max(top, max(q[ks][y][x] & 0x7FFFu, q[ks][y][x] >> 16 & 0x7FFFu));
-      top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-      top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-      const int e = (int)(top >> 7);  // the largest's exponent, biased by 127
-      up = e == 0 || e == 255 ? 0 : min(max(140 - e, -126), 126);
-      const float by = __uint_as_float((uint32_t)(127 + up) << 23);
+          for (int x = 0; x < 2; ++x) top = max(top, max(q[ks][y][x] & 0x7FFFu, q[ks][y][x] >> 16 & 0x7FFFu));
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        const int e = (int)(top >> 7);  // the largest's exponent, biased by 127
+        up = e == 0 || e == 255 ? 0 : min(max(140 - e, -126), 126);
+        const float by = __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float2 f = pair_of(q[ks][y][x], SB_BF16);
-          q[ks][y][x] = pack_pair(f.x * by, f.y * by, SB_F16);
-        }
-    }
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int down = __shfl_sync(0xFFFFFFFFu, up, (2 * tig + x) * 4), r = r0 + 8 * y + 2 * tig + x;
-      factor[y][x] = a.scale_log2 * __uint_as_float((uint32_t)(127 - down) << 23);
-      limit[y][x] = a.causal && r < a.rows ? max(count - a.Tq + 1 + r / a.group, 0) : count;
-    }
-  }
-  const int seen_by_all = a.causal ? max(count - a.Tq + 1 + r0 / a.group, 0) : count;
-
-  float o[KS][NB][4], m[NB][2], l[NB][2];
-#pragma unroll
-  for (int y = 0; y < NB; ++y) {
-    m[y][0] = m[y][1] = -INFINITY;
-    l[y][0] = l[y][1] = 0.f;
-#pragma unroll
-    for (int x = 0; x < KS; ++x) o[x][y][0] = o[x][y][1] = o[x][y][2] = o[x][y][3] = 0.f;
-  }
-  float* const scores = a.scores ? a.plane(b * a.Hkv + kvh, block) : a.weight ? reinterpret_cast<float*>(smem + C::SMEM) : nullptr;
-  const int chunk0 = at.c - (int)done;  // of the unit: chunk0 + warp + i * kWarps
-
-  const int i_first = i;
-  for (; i < i_end; ++i) {
-    copies_wait<C::STAGES - 1>();
-    __syncwarp();
-    const int st = i % C::STAGES, j0 = (chunk0 + warp + i * kWarps) * CK;
-    const uint32_t kb = ring_at + st * C::STAGE, vb = kb + C::HALF;
-    const uint64_t bits = there[warp][st];
-    const bool mixed = j0 + CK > seen_by_all;  // (or the last chunk)
-    const bool all = bits == (~0ull >> (64 - CK)) && !mixed;
-
-    float s[KT][NB][4];
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-      for (int y = 0; y < NB; ++y) s[kt][y][0] = s[kt][y][1] = s[kt][y][2] = s[kt][y][3] = 0.f;
-      const int row = kt * 16 + (lane >> 3 & 1) * 8 + (lane & 7);
-      if constexpr (E4M3) {
-#pragma unroll
-        for (int p = 0; p < KS / 2; ++p) {
-          uint32_t f[4];
-          ldsm4(kb + C::at(row, 2 * p + (lane >> 4)), f);
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            uint32_t w[4];
-            widen(f[2 * z], w[0], w[2]);
-            widen(f[2 * z + 1], w[1], w[3]);
-#pragma unroll
-            for (int y = 0; y < NB; ++y) mma16816<false>(s[kt][y], w, q[2 * p + z][y][0], q[2 * p + z][y][1]);
+          for (int x = 0; x < 2; ++x) {
+            const float2 f = pair_of(q[ks][y][x], SB_BF16);
+            q[ks][y][x] = pack_pair(f.x * by, f.y * by, SB_F16);
           }
-        }
-      } else {
+      }
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          uint32_t f[4];
-          ldsm4(kb + C::at(row, 2 * ks + (lane >> 4)), f);
-#pragma unroll
-          for (int y = 0; y < NB; ++y) mma16816<BF16>(s[kt][y], f, q[ks][y][0], q[ks][y][1]);
-        }
+      for (int x = 0; x < 2; ++x) {
+        const int down = __shfl_sync(0xFFFFFFFFu, up, (2 * tig + x) * 4), r = r0 + 8 * y + 2 * tig + x;
+        factor[y][x] = a.scale_log2 * __uint_as_float((uint32_t)(127 - down) << 23);
+        limit[y][x] = a.causal && r < a.rows ? max(count - a.Tq + 1 + r / a.group, 0) : count;
       }
     }
-    if (!all) {
+    const int seen_by_all = a.causal ? max(count - a.Tq + 1 + r0 / a.group, 0) : count;
+
+    float o[KS][NB][4], m[NB][2], l[NB][2];
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
+    for (int y = 0; y < NB; ++y) {
+      m[y][0] = m[y][1] = -INFINITY;
+      l[y][0] = l[y][1] = 0.f;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int k = kt * 16 + g + 8 * x;
-          const bool in = bits >> k & 1u;
-#pragma unroll
-          for (int y = 0; y < NB; ++y)
-#pragma unroll
-            for (int z = 0; z < 2; ++z)
-              if (!in || j0 + k >= limit[y][z]) s[kt][y][2 * x + z] = -INFINITY;
-        }
+      for (int x = 0; x < KS; ++x) o[x][y][0] = o[x][y][1] = o[x][y][2] = o[x][y][3] = 0.f;
     }
-    if (scores) {
-      float* to8 = scores + (long long)(j0 + g) * a.score_rows + 2 * tig;  // of every eighth state
+    float* const scores = a.scores   ? a.plane(b * a.Hkv + kvh, block)
+                          : a.weight ? reinterpret_cast<float*>(smem + C::SMEM) : nullptr;
+    const int chunk0 = at.c - (int)done;  // of the unit: chunk0 + warp + i * kWarps
+
+    const int i_first = i;
+    for (; i < i_end; ++i) {
+      copies_wait<C::STAGES - 1>();
+      __syncwarp();
+      const int st = i % C::STAGES, j0 = (chunk0 + warp + i * kWarps) * CK;
+      const uint32_t kb = ring_at + st * C::STAGE, vb = kb + C::HALF;
+      const uint64_t bits = there[warp][st];
+      const bool mixed = j0 + CK > seen_by_all;  // (or the last chunk)
+      const bool all = bits == (~0ull >> (64 - CK)) && !mixed;
+
+      float s[KT][NB][4];
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
+      for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x, to8 += 8 * a.score_rows) {
-          if (j0 + kt * 16 + 8 * x + g < count) {
+        for (int y = 0; y < NB; ++y) s[kt][y][0] = s[kt][y][1] = s[kt][y][2] = s[kt][y][3] = 0.f;
+        const int row = kt * 16 + (lane >> 3 & 1) * 8 + (lane & 7);
+        if constexpr (E4M3) {
 #pragma unroll
-            for (int y = 0; y < NB; ++y) {
-              const float u = s[kt][y][2 * x] * factor[y][0], w = s[kt][y][2 * x + 1] * factor[y][1];
-              if (a.score_rows == 1) {
-                if (tig == 0 && y == 0) *to8 = u;
-              } else if (8 * y + 2 * tig < rows) {  // (the row after an odd last one is room of its own)
-                *reinterpret_cast<float2*>(to8 + 8 * y) = make_float2(u, w);
+          for (int p = 0; p < KS / 2; ++p) {
+            uint32_t f[4];
+            ldsm4(kb + C::at(row, 2 * p + (lane >> 4)), f);
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              uint32_t w[4];
+              widen(f[2 * z], w[0], w[2]);
+              widen(f[2 * z + 1], w[1], w[3]);
+#pragma unroll
+              for (int y = 0; y < NB; ++y) mma16816<false>(s[kt][y], w, q[2 * p + z][y][0], q[2 * p + z][y][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t f[4];
+            ldsm4(kb + C::at(row, 2 * ks + (lane >> 4)), f);
+#pragma unroll
+            for (int y = 0; y < NB; ++y) mma16816<BF16>(s[kt][y], f, q[ks][y][0], q[ks][y][1]);
+          }
+        }
+      }
+      if (!all) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int k = kt * 16 + g + 8 * x;
+            const bool in = bits >> k & 1u;
+#pragma unroll
+            for (int y = 0; y < NB; ++y)
+#pragma unroll
+              for (int z = 0; z < 2; ++z)
+                if (!in || j0 + k >= limit[y][z]) s[kt][y][2 * x + z] = -INFINITY;
+          }
+      }
+      if (scores) {
+        float* to8 = scores + (long long)(j0 + g) * a.score_rows + 2 * tig;  // of every eighth state
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x, to8 += 8 * a.score_rows) {
+            if (j0 + kt * 16 + 8 * x + g < count) {
+#pragma unroll
+              for (int y = 0; y < NB; ++y) {
+                const float u = s[kt][y][2 * x] * factor[y][0], w = s[kt][y][2 * x + 1] * factor[y][1];
+                if (a.score_rows == 1) {
+                  if (tig == 0 && y == 0) *to8 = u;
+                } else if (8 * y + 2 * tig < rows) {  // (the row after an odd last one is room of its own)
+                  *reinterpret_cast<float2*>(to8 + 8 * y) = make_float2(u, w);
+                }
               }
             }
           }
-        }
-    }
-    // a new reference point with the first states, and where a maximum grew by more than 2^8 (or is NaN)
-    bool grew = false;
-    float base[NB][2];
-#pragma unroll
-    for (int y = 0; y < NB; ++y)
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        float top = s[0][y][z];
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) top = max3(top, s[kt][y][z], s[kt][y][2 + z]);
-        base[y][z] = fmaf(-m[y][z], factor[y][z], lift);
-        grew = grew || !(fmaf(top, factor[y][z], base[y][z]) <= lift + 8.f);
       }
-    if (__any_sync(0xFFFFFFFFu, grew)) {
+      // a new reference point with the first states, and where a maximum grew by more than 2^8 (or is NaN)
+      bool grew = false;
+      float base[NB][2];
 #pragma unroll
       for (int y = 0; y < NB; ++y)
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          float top = m[y][z];
+          float top = s[0][y][z];
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt) top = max3(top, s[kt][y][z], s[kt][y][2 + z]);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) {
-            const float u = __shfl_xor_sync(0xFFFFFFFFu, top, x);
-            top = max3(top, u, u);
-          }
-          const float c = m[y][z] == top ? 1.f : exp2_hw((m[y][z] - top) * factor[y][z]);
-          m[y][z] = top;
-          base[y][z] = fmaf(-top, factor[y][z], lift);
-          l[y][z] *= c;
-#pragma unroll
-          for (int x = 0; x < KS; ++x) {
-            o[x][y][z] *= c;
-            o[x][y][2 + z] *= c;
-          }
+          base[y][z] = fmaf(-m[y][z], factor[y][z], lift);
+          grew = grew || !(fmaf(top, factor[y][z], base[y][z]) <= lift + 8.f);
         }
-    }
-#pragma unroll
-    for (int y = 0; y < NB; ++y)
-#pragma unroll
-      for (int z = 0; z < 2; ++z)
-        if (m[y][z] == -INFINITY) base[y][z] = 0.f;
-    // probabilities in place of the scores
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int y = 0; y < NB; ++y)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float p = exp2_hw(fmaf(s[kt][y][x], factor[y][x & 1], base[y][x & 1]));
-          s[kt][y][x] = p;
-          l[y][x & 1] += p;
-        }
-    // a causal call's last states are seen by some rows only; where one's V is no number, 0 x V is not 0
-    bool odd = false;
-    if (a.causal && mixed) {
-      for (int x = lane; x < C::HALF / 16; x += 32) {
-        const uint4 w = *reinterpret_cast<const uint4*>(ring + st * C::STAGE + C::HALF + x * 16);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          if constexpr (E4M3) odd = odd || (__vcmpeq4(u[z] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0);
-          else {
-            constexpr uint32_t e = BF16 ? 0x7F807F80u : 0x7C007C00u;
-            odd = odd || (__vcmpeq2(u[z] & e, e) != 0);
-          }
-        }
-      }
-      odd = __any_sync(0xFFFFFFFFu, odd);
-    }
-    if (!odd) {
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        uint32_t hi[NB][2], lo[NB][2];
+      if (__any_sync(0xFFFFFFFFu, grew)) {
 #pragma unroll
         for (int y = 0; y < NB; ++y)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float u = s[kt][y][2 * x], w = s[kt][y][2 * x + 1];
-            const uint32_t h = pack16<BF16>(u, w);
-            const float2 f = pair_of(h, BF16 ? SB_BF16 : SB_F16);
-            hi[y][x] = transposed(h);
-            lo[y][x] = transposed(pack16<BF16>(u - f.x, w - f.y));
-          }
-        if constexpr (E4M3) {
-          const int row = kt * 16 + (lane >> 3 & 1) * 8 + (lane & 7);
+          for (int z = 0; z < 2; ++z) {
+            float top = m[y][z];
 #pragma unroll
-          for (int p = 0; p < KS / 2; ++p) {
-            uint32_t f[4];
-            ldsm4_t(vb + C::at(row, 2 * p + (lane >> 4)), f);
+            for (int kt = 0; kt < KT; ++kt) top = max3(top, s[kt][y][z], s[kt][y][2 + z]);
 #pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              // a register: channels 2g, 2g + 1 of a state, then of the next
-              uint32_t w[4];
-              widen(__byte_perm(f[2 * z], 0, 0x3120), w[0], w[1]);
-              widen(__byte_perm(f[2 * z + 1], 0, 0x3120), w[2], w[3]);
+            for (int x = 4; x < 32; x <<= 1) {
+              const float u = __shfl_xor_sync(0xFFFFFFFFu, top, x);
+              top = max3(top, u, u);
+            }
+            const float c = m[y][z] == top ? 1.f : exp2_hw((m[y][z] - top) * factor[y][z]);
+            m[y][z] = top;
+            base[y][z] = fmaf(-top, factor[y][z], lift);
+            l[y][z] *= c;
 #pragma unroll
-              for (int y = 0; y < NB; ++y) {
-                mma16816<false>(o[2 * p + z][y], w, hi[y][0], hi[y][1]);
-                mma16816<false>(o[2 * p + z][y], w, lo[y][0], lo[y][1]);
-              }
+            for (int x = 0; x < KS; ++x) {
+              o[x][y][z] *= c;
+              o[x][y][2 + z] *= c;
             }
           }
-        } else {
-          const int row = kt * 16 + (lane >> 4) * 8 + (lane & 7);
-#pragma unroll
-          for (int x = 0; x < KS; ++x) {
-            uint32_t f[4];
-            ldsm4_t(vb + C::at(row, 2 * x + (lane >> 3 & 1)), f);
-#pragma unroll
-            for (int y = 0; y < NB; ++y) {
-              mma16816<BF16>(o[x][y], f, hi[y][0], hi[y][1]);
-              mma16816<BF16>(o[x][y], f, lo[y][0], lo[y][1]);
-            }
-          }
-        }
       }
-    } else {  // state by state, rows that do not see it left alone
-      const uint8_t* v = ring + st * C::STAGE + C::HALF;
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll 1
-        for (int k = 0; k < 16; ++k) {
-          const int row = kt * 16 + k;
-          float p[NB][2];
-#pragma unroll
-          for (int y = 0; y < NB; ++y)
-#pragma unroll
-            for (int z = 0; z < 2; ++z)
-              p[y][z] = __shfl_sync(0xFFFFFFFFu, k < 8 ? s[kt][y][z] : s[kt][y][2 + z], (k & 7) * 4 + tig);
-#pragma unroll
-          for (int x = 0; x < KS; ++x)
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              const int c = E4M3 ? x * 16 + 2 * g + w : x * 16 + g + 8 * w;
-              float f;
-              if constexpr (E4M3) f = float2_of_e4m3x2(v[C::at(row, c >> 4) + (c & 15)]).x;
-              else f = one_of(v + C::at(row, c >> 3), PT, c & 7);
-#pragma unroll
-              for (int y = 0; y < NB; ++y)
-#pragma unroll
-                for (int z = 0; z < 2; ++z)
-                  if (j0 + row < limit[y][z]) o[x][y][2 * w + z] = fmaf(p[y][z], f, o[x][y][2 * w + z]);
-            }
-        }
-    }
-    __syncwarp();  // every lane has read the stage
-    if (i + 1 < i_end) {
-      copy(i + C::STAGES);
-      ask();
-      __syncwarp();
-    }
-  }
-#pragma unroll
-  for (int y = 0; y < NB; ++y)
-#pragma unroll
-    for (int z = 0; z < 2; ++z)
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) l[y][z] += __shfl_xor_sync(0xFFFFFFFFu, l[y][z], x);
-  // the warps' outputs meet in shared memory: rows of DH floats in the stage that a warp has just read (and fills
-  // again afterwards), groups of eight floats turned so that no two lanes meet in a bank; maxima as exponents of 2
-  const bool some = i > i_first;
-  const int last = some ? warp * C::kRing + (i - 1) % C::STAGES * C::STAGE : -1;
-  if (some) {
-    float* own = reinterpret_cast<float*>(smem + last);
-#pragma unroll
-    for (int x = 0; x < KS; ++x)
 #pragma unroll
       for (int y = 0; y < NB; ++y)
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const int c = E4M3 ? x * 16 + 2 * g + (z >> 1) : x * 16 + g + 8 * (z >> 1);
-          own[(8 * y + 2 * tig + (z & 1)) * DH + (c ^ tig << 3)] = o[x][y][z];
+        for (int z = 0; z < 2; ++z)
+          if (m[y][z] == -INFINITY) base[y][z] = 0.f;
+      // probabilities in place of the scores
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int y = 0; y < NB; ++y)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float p = exp2_hw(fmaf(s[kt][y][x], factor[y][x & 1], base[y][x & 1]));
+            s[kt][y][x] = p;
+            l[y][x & 1] += p;
+          }
+      // a causal call's last states are seen by some rows only; where one's V is no number, 0 x V is not 0
+      bool odd = false;
+      if (a.causal && mixed) {
+        for (int x = lane; x < C::HALF / 16; x += 32) {
+          const uint4 w = *reinterpret_cast<const uint4*>(ring + st * C::STAGE + C::HALF + x * 16);
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            if constexpr (E4M3) odd = odd || (__vcmpeq4(u[z] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0);
+            else {
+              constexpr uint32_t e = BF16 ? 0x7F807F80u : 0x7C007C00u;
+              odd = odd || (__vcmpeq2(u[z] & e, e) != 0);
+            }
+          }
         }
-  }
-  if (lane == 0) area[warp] = last;
-  if (g == 0) {
+        odd = __any_sync(0xFFFFFFFFu, odd);
+      }
+      if (!odd) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          uint32_t hi[NB][2], lo[NB][2];
+#pragma unroll
+          for (int y = 0; y < NB; ++y)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float u = s[kt][y][2 * x], w = s[kt][y][2 * x + 1];
+              const uint32_t h = pack16<BF16>(u, w);
+              const float2 f = pair_of(h, BF16 ? SB_BF16 : SB_F16);
+              hi[y][x] = transposed(h);
+              lo[y][x] = transposed(pack16<BF16>(u - f.x, w - f.y));
+            }
+          if constexpr (E4M3) {
+            const int row = kt * 16 + (lane >> 3 & 1) * 8 + (lane & 7);
+#pragma unroll
+            for (int p = 0; p < KS / 2; ++p) {
+              uint32_t f[4];
+              ldsm4_t(vb + C::at(row, 2 * p + (lane >> 4)), f);
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                // a register: channels 2g, 2g + 1 of a state, then of the next
+                uint32_t w[4];
+                widen(__byte_perm(f[2 * z], 0, 0x3120), w[0], w[1]);
+                widen(__byte_perm(f[2 * z + 1], 0, 0x3120), w[2], w[3]);
+#pragma unroll
+                for (int y = 0; y < NB; ++y) {
+                  mma16816<false>(o[2 * p + z][y], w, hi[y][0], hi[y][1]);
+                  mma16816<false>(o[2 * p + z][y], w, lo[y][0], lo[y][1]);
+                }
+              }
+            }
+          } else {
+            const int row = kt * 16 + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+            for (int x = 0; x < KS; ++x) {
+              uint32_t f[4];
+              ldsm4_t(vb + C::at(row, 2 * x + (lane >> 3 & 1)), f);
+#pragma unroll
+              for (int y = 0; y < NB; ++y) {
+                mma16816<BF16>(o[x][y], f, hi[y][0], hi[y][1]);
+                mma16816<BF16>(o[x][y], f, lo[y][0], lo[y][1]);
+              }
+            }
+          }
+        }
+      } else {  // state by state, rows that do not see it left alone
+        const uint8_t* v = ring + st * C::STAGE + C::HALF;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll 1
+          for (int k = 0; k < 16; ++k) {
+            const int row = kt * 16 + k;
+            float p[NB][2];
+#pragma unroll
+            for (int y = 0; y < NB; ++y)
+#pragma unroll
+              for (int z = 0; z < 2; ++z)
+                p[y][z] = __shfl_sync(0xFFFFFFFFu, k < 8 ? s[kt][y][z] : s[kt][y][2 + z], (k & 7) * 4 + tig);
+#pragma unroll
+            for (int x = 0; x < KS; ++x)
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                const int c = E4M3 ? x * 16 + 2 * g + w : x * 16 + g + 8 * w;
+                float f;
+                if constexpr (E4M3) f = float2_of_e4m3x2(v[C::at(row, c >> 4) + (c & 15)]).x;
+                else f = one_of(v + C::at(row, c >> 3), PT, c & 7);
+#pragma unroll
+                for (int y = 0; y < NB; ++y)
+#pragma unroll
+                  for (int z = 0; z < 2; ++z)
+                    if (j0 + row < limit[y][z]) o[x][y][2 * w + z] = fmaf(p[y][z], f, o[x][y][2 * w + z]);
+              }
+          }
+      }
+      __syncwarp();  // every lane has read the stage
+      if (i + 1 < i_end) {
+        copy(i + C::STAGES);
+        ask();
+        __syncwarp();
+      }
+    }
 #pragma unroll
     for (int y = 0; y < NB; ++y)
 #pragma unroll
       for (int z = 0; z < 2; ++z)
-        ml[warp][8 * y + 2 * tig + z] = make_float2(m[y][z] == -INFINITY ? -INFINITY : m[y][z] * factor[y][z], l[y][z]);
-  }
-  __syncthreads();
-  const long long slot = a.shares ? (long long)blockIdx.x + (long long)b * a.units() + at.unit : 0;
-  constexpr int per = DH / 8;
-  for (int e = threadIdx.x; e < rows * per; e += kWarps * 32) {
-    const int r = e / per, c = (e - r * per) * 8;
-    float top = -INFINITY, sum = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = max3(top, ml[w][r].x, ml[w][r].x);
+        for (int x = 4; x < 32; x <<= 1) l[y][z] += __shfl_xor_sync(0xFFFFFFFFu, l[y][z], x);
+    // the warps' outputs meet in shared memory: rows of DH floats in the stage that a warp has just read (and fills
+    // again afterwards), groups of eight floats turned so that no two lanes meet in a bank; maxima as exponents of 2
+    const bool some = i > i_first;
+    const int last = some ? warp * C::kRing + (i - 1) % C::STAGES * C::STAGE : -1;
+    if (some) {
+      float* own = reinterpret_cast<float*>(smem + last);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (area[w] < 0) continue;
-      const float mw = ml[w][r].x, k = mw == top ? 1.f : exp2_hw(mw - top);
-      sum = fmaf(k, ml[w][r].y, sum);
-      const float4* src = reinterpret_cast<const float4*>(smem + area[w]) + (r * DH + (c ^ (r >> 1 & 3) << 3)) / 4;
-      const float4 x = src[0], y = src[1];
-      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      for (int x = 0; x < KS; ++x)
 #pragma unroll
-      for (int u = 0; u < 8; ++u) f[u] = fmaf(k, v[u], f[u]);
-    }
-    const bool none = top == -INFINITY;  // no states
-    const float inv = none ? 0.f : a.v_scale / sum;
+        for (int y = 0; y < NB; ++y)
 #pragma unroll
-    for (int u = 0; u < 8; ++u) f[u] = none ? 0.f : f[u] * inv;
-    const float log_sum = none ? -INFINITY : top - lift + log2f(sum);
-    const Row w(a, kvh, r0 + r);
-    if (a.shares && !whole) {
-      store8(a.part_o, SB_F32, (slot * a.part_rows + r) * DH + c, f);
-    } else {
-      store8(a.o.p, a.q_bf16 ? SB_BF16 : SB_F16, b * a.o.img + w.t * a.o.row + (long long)w.h * DH + c, f);
-      if (c == 0 && a.lse) a.lse[((long long)b * a.H + w.h) * a.Tq + w.t] = log_sum * 0.69314718055994531f;
+          for (int z = 0; z < 4; ++z) {
+            const int c = E4M3 ? x * 16 + 2 * g + (z >> 1) : x * 16 + g + 8 * (z >> 1);
+            own[(8 * y + 2 * tig + (z & 1)) * DH + (c ^ tig << 3)] = o[x][y][z];
+          }
     }
-    if (c == 0) {
-      if (a.ends > 0) a.part_l[(a.shares ? slot : (long long)b * a.units() + at.unit) * a.part_rows + r] = log_sum;
-      fin[r] = log_sum;
+    if (lane == 0) area[warp] = last;
+    if (g == 0) {
+#pragma unroll
+      for (int y = 0; y < NB; ++y)
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+          ml[warp][8 * y + 2 * tig + z] = make_float2(m[y][z] == -INFINITY ? -INFINITY : m[y][z] * factor[y][z], l[y][z]);
     }
-  }
-  __syncthreads();
-  if (a.weight && a.ends == 0) {  // all of the scores and sums are this CTA's own
-    float* weight = a.weight + ((long long)b * a.Hkv + kvh) * a.pages.cap;
-    for (int j = threadIdx.x; j < count; j += kWarps * 32) {
-      float w = 0.f;
-      for (int r = 0; r < rows; ++r)
-        if (fin[r] != -INFINITY) w += exp2_hw(scores[(long long)j * a.score_rows + r] - fin[r]);
-      weight[j] = fmaf(a.decay, weight[j], w);
+    __syncthreads();
+    const long long slot = a.shares ? (long long)blockIdx.x + (long long)b * a.units() + at.unit : 0;
+    constexpr int per = DH / 8;
+    for (int e = threadIdx.x; e < rows * per; e += kWarps * 32) {
+      const int r = e / per, c = (e - r * per) * 8;
+      float top = -INFINITY, sum = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = max3(top, ml[w][r].x, ml[w][r].x);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (area[w] < 0) continue;
+        const float mw = ml[w][r].x, k = mw == top ? 1.f : exp2_hw(mw - top);
+        sum = fmaf(k, ml[w][r].y, sum);
+        const float4* src = reinterpret_cast<const float4*>(smem + area[w]) + (r * DH + (c ^ (r >> 1 & 3) << 3)) / 4;
+        const float4 x = src[0], y = src[1];
+        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int u = 0; u < 8; ++u) f[u] = fmaf(k, v[u], f[u]);
+      }
+      const bool none = top == -INFINITY;  // no states
+      const float inv = none ? 0.f : a.v_scale / sum;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) f[u] = none ? 0.f : f[u] * inv;
+      const float log_sum = none ? -INFINITY : top - lift + log2f(sum);
+      const Row w(a, kvh, r0 + r);
+      if (a.shares && !whole) {
+        const long long place = 2ll * blockIdx.x + (at.c == 0);
+        store8(a.part_o, SB_F32, (place * a.part_rows + r) * DH + c, f);
+      } else {
+        store8(a.o.p, a.q_bf16 ? SB_BF16 : SB_F16, b * a.o.img + w.t * a.o.row + (long long)w.h * DH + c, f);
+        if (c == 0 && a.lse) a.lse[((long long)b * a.H + w.h) * a.Tq + w.t] = log_sum * 0.69314718055994531f;
+      }
+      if (c == 0) {
+        if (a.ends > 0) a.part_l[(a.shares ? slot : (long long)b * a.units() + at.unit) * a.part_rows + r] = log_sum;
+        fin[r] = log_sum;
+      }
     }
-  }
+    __syncthreads();
+    if (a.weight && a.ends == 0) {  // all of the scores and sums are this CTA's own
+      float* weight = a.weight + ((long long)b * a.Hkv + kvh) * a.pages.cap;
+      for (int j = threadIdx.x; j < count; j += kWarps * 32) {
+        float w = 0.f;
+        for (int r = 0; r < rows; ++r)
+          if (fin[r] != -INFINITY) w += exp2_hw(scores[(long long)j * a.score_rows + r] - fin[r]);
+        weight[j] = fmaf(a.decay, weight[j], w);
+      }
+    }
     if (some) {
       copy(i - 1 + C::STAGES);
       ask();
@@ -777,12 +780,13 @@ __global__ void __launch_bounds__(kEndThreads, kEndOcc) paged_end_kernel(const _
   grid_dep_wait();
   for (int block = 0; block < a.blocks; ++block) {
     const int r0 = block * 16, rows = min(16, a.rows - r0), unit = kvh * a.blocks + block;
-    long long first = (long long)b * a.units() + unit;
+    long long first = (long long)b * a.units() + unit, cta = 0;
     int pieces = 1;
     if (a.shares) {
       const long long from = s.before * a.units() + (long long)unit * n;
-      pieces = n == 0 ? 0 : (int)((from + n - 1) / s.each - from / s.each) + 1;
-      first += from / s.each;
+      cta = from / s.each;
+      pieces = n == 0 ? 0 : (int)((from + n - 1) / s.each - cta) + 1;
+      first += cta;
     }
     __syncthreads();
     for (int r = warp; r < 16; r += kEndThreads / 32) {
@@ -816,7 +820,8 @@ __global__ void __launch_bounds__(kEndThreads, kEndOcc) paged_end_kernel(const _
           if (ls == -INFINITY) continue;
           const float k = exp2_hw(ls - l);
           float v[8];
-          unpack8(load_raw8(a.part_o, SB_F32, ((first + x) * a.part_rows + r) * DH + c), SB_F32, v);
+          const long long place = 2 * (cta + x) + (x == 0);  // the first of them goes on behind its CTA
+          unpack8(load_raw8(a.part_o, SB_F32, (place * a.part_rows + r) * DH + c), SB_F32, v);
 #pragma unroll
           for (int u = 0; u < 8; ++u) f[u] = fmaf(k, v[u], f[u]);
         }
@@ -832,8 +837,8 @@ __global__ void __launch_bounds__(kEndThreads, kEndOcc) paged_end_kernel(const _
             y += part[z][2 * threadIdx.x + 1];
           }
           const Row q(a, kvh, r0 + r);
-          uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o.p) + b * a.o.img + q.t * a.o.row + (long long)q.h * DH);
-          o[threadIdx.x] = pack_pair(x, y, a.q_bf16 ? SB_BF16 : SB_F16);
+          uint16_t* o = static_cast<uint16_t*>(a.o.p) + b * a.o.img + q.t * a.o.row + (long long)q.h * DH;
+          reinterpret_cast<uint32_t*>(o)[threadIdx.x] = pack_pair(x, y, a.q_bf16 ? SB_BF16 : SB_F16);
           if (threadIdx.x == 0 && a.lse) a.lse[((long long)b * a.H + q.h) * a.Tq + q.t] = l * 0.69314718055994531f;
         }
         __syncthreads();
@@ -871,9 +876,12 @@ struct PagedPlan {
   long long bytes() const { return (scores + part_o + part_l) * 4; }
 };
 
-// A CTA a unit where a unit is small (256 KB of places: a few us, and the call is one kernel) or the units alone
-// fill the SMs eight times; else as many CTAs as are resident at once share all chunks evenly, whatever the
-// items' lengths, and a second kernel joins the pieces.
+// Either a CTA a unit, and one kernel; or as many CTAs as are resident at once share all chunks evenly, whatever the
+// items' lengths, and a second kernel joins the pieces.  What they take is estimated from the places (lengths are
+// on the device): a CTA a unit about 3 us to start and end and its share of the rate of all resident ones, in waves;
+// shared chunks about 18 us for both kernels and the rate of all.  Measured, us in kernels, apart and shared: 2 x 8
+// units of 1000, 2000, 4000 states of 32 channels 12 and 20, 21 and 18, 40 and 18; 1 x 4 of 512, 1024 of 128 14 and
+// 15, 25 and 14; 64 x 4 of 1024, 2048, 8160 of 128 30 and 38, 54 and 54, 203 and 171; 640 x 4 of 1000 of 64 142 and 127.
 PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int pt, int cap, bool account, int sms) {
   PagedPlan p{};
   int occ;
@@ -884,11 +892,13 @@ PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int pt, int cap, boo
   p.blocks = (p.rows + 15) / 16;
   p.part_rows = std::min(p.rows, 16);
   p.units = (long long)B * Hkv * p.blocks;
-  const bool apart = 2ll * cap * dh * page_dtype_bytes(pt) > 256 * 1024 && p.units < 8ll * occ * sms;
-  p.shares = apart ? occ * sms : 0;
+  const long long resident = (long long)occ * sms, waves = (p.units + resident - 1) / resident;
+  const double unit_us = 2.0 * cap * dh * page_dtype_bytes(pt) / 6.2e6;  // at the rate of all
+  const bool apart = waves * (3.0 + resident * unit_us) > 18.0 + p.units * unit_us;
+  p.shares = apart ? (int)resident : 0;
   account = account && cap > 0;
   // one wave of the last kernel's CTAs, each with 256 places or a row
-  const long long heads = (long long)B * Hkv, wave = ((long long)kEndOcc * sms + heads - 1) / std::max(heads, 1ll);
+  const long long heads = (long long)B * Hkv, wave = std::max(1ll, (long long)kEndOcc * sms / std::max(heads, 1ll));
   if (account && (apart || p.blocks > 1)) p.ends = (int)std::min(wave, ((long long)cap + 255) / 256);
   else if (apart) p.ends = (int)std::min(wave, (long long)p.rows);
   auto even = [](long long n) { return (n + 3) / 4 * 4; };
@@ -896,9 +906,8 @@ PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int pt, int cap, boo
   for (p.score_rows = 1; p.score_rows < p.part_rows;) p.score_rows *= 2;
   p.held = account && p.ends == 0 && p.places * p.score_rows <= kHeldScores;
   p.scores = account && !p.held ? (long long)B * Hkv * p.blocks * p.places * p.score_rows : 0;
-  const long long slots = p.units + p.shares;
-  p.part_o = apart ? slots * p.part_rows * dh : 0;
-  p.part_l = p.ends > 0 ? even(slots * p.part_rows) : 0;
+  p.part_l = p.ends > 0 ? even((p.units + p.shares) * p.part_rows) : 0;
+  p.part_o = 2ll * p.shares * p.part_rows * dh;
   return p;
 }
 
@@ -983,8 +992,8 @@ extern "C" int sb_paged_attention(const sb_paged_memory* memory, const void* q, 
   a.decay = decay;
   float* w = static_cast<float*>(work);
   a.scores = p.scores > 0 ? w : nullptr;
-  a.part_o = w + p.scores;
-  a.part_l = a.part_o + p.part_o;
+  a.part_l = w + p.scores;
+  a.part_o = a.part_l + p.part_l;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = m->dh == 32   ? launch<32>(a, m->dtype, ctas, ends, st)
                         : m->dh == 64 ? launch<64>(a, m->dtype, ctas, ends, st) : launch<128>(a, m->dtype, ctas, ends, st);

@@ -64,7 +64,8 @@ SB_DEV uint4 load_vec(const void* p, long long i) {
 }
 
 template <int MODE, bool ALIGNED, bool BF16>
-__global__ void __launch_bounds__(kWriteWarps * 32, MODE == 2 ? 2 : 4) paged_write_kernel(const __grid_constant__ WriteArgs a) {
+__global__ void __launch_bounds__(kWriteWarps * 32, MODE == 2 ? 2 : 4)
+    paged_write_kernel(const __grid_constant__ WriteArgs a) {
   constexpr int kAhead = 4, bytes = MODE ? 8 : 16;  // vectors of K and V at once, bytes of one in the pool
   if (blockIdx.x >= a.row_blocks) {  // new lengths, then weights and stamps, neighbours along t
     long long i = (blockIdx.x - a.row_blocks) * (kWriteWarps * 32) + threadIdx.x;
@@ -165,7 +166,9 @@ SB_DEV uint32_t ordered(float w) {
 }
 // A pass's bits of a key, and those of the passes before it.
 SB_DEV int bin_of(uint32_t key, int pass) { return pass == 0 ? key >> 21 : pass == 1 ? key >> 10 & 2047u : key & 1023u; }
-SB_DEV uint32_t prefix_of(uint32_t key, int pass) { return pass == 0 ? 0u : pass == 1 ? key & 0xFFE00000u : key & 0xFFFFFC00u; }
+SB_DEV uint32_t prefix_of(uint32_t key, int pass) {
+  return pass == 0 ? 0u : pass == 1 ? key & 0xFFE00000u : key & 0xFFFFFC00u;
+}
 SB_DEV uint32_t as_prefix(int bin, int pass) { return (uint32_t)bin << (pass == 0 ? 21 : pass == 1 ? 10 : 0); }
 
 // What the CTAs of an (item, key head) tell each other; bins and counts are never written twice.
@@ -318,7 +321,8 @@ struct Pairs {
   ulonglong2 source[32], target[32];  // addresses of K and V; 0: nowhere
 };
 template <int LANES>
-SB_DEV void move_pairs(const EvictArgs& a, long long unit, const int* to, const int* from, int moves, int i0, int stride, Pairs& pairs) {
+SB_DEV void move_pairs(const EvictArgs& a, long long unit, const int* to, const int* from, int moves, int i0, int stride,
+                       Pairs& pairs) {
   constexpr int AT_ONCE = 32 / LANES;
   const int lane = lane_id(), b = (int)(unit / a.Hkv), h = (int)(unit - (long long)b * a.Hkv);
   const long long c = (long long)h * a.row_bytes + lane % LANES * 16, at = unit * a.pages.cap;
@@ -395,7 +399,7 @@ constexpr int kMostFours = 9;  // states a thread: 36; 107 KB of shared memory, 
 inline int held_fours(int cap, int ctas) { return ((cap + ctas * kSelect * 4 - 1) / (ctas * kSelect * 4)) | 1; }
 inline int held_bytes(int fours) { return kSelect * 4 * fours * 4 + kSelect * 4 * fours / 8; }
 // A memory of up to this many places is evicted from by one kernel: at most half of them move, 512 KB a CTA.
-constexpr int kOneKernel = 2048;
+constexpr int kFewPlaces = 2048;
 static_assert(sizeof(Told) >= kSelectWarps * sizeof(Pairs), "room for the pairs");
 
 __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_constant__ EvictArgs a) {
@@ -415,7 +419,7 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
     const int fours = ((len + ctas * kSelect * 4 - 1) / (ctas * kSelect * 4)) | 1, run = fours * 4, mine = kSelect * run;
     const int j_cta = (int)rank * mine, here = min(max(len - j_cta, 0), mine);  // the CTA's states
     uint32_t* const bits = held + mine;
-    for (int x = threadIdx.x; x < 4 * kBins; x += kSelect) told.bins[0][x] = 0;
+    for (int x = threadIdx.x; x < kBins; x += kSelect) reinterpret_cast<uint4*>(told.bins)[x] = make_uint4(0, 0, 0, 0);
     int n[2] = {0, 0}, all[2];
     constexpr int kAtOnce = 8;
     for (int w0 = warp * 32; w0 < here; w0 += kAtOnce * kSelect) {
@@ -514,17 +518,20 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
     uint64_t more = 0, tied = 0;
     for (int i = 0; i < my_fours; ++i) {
       const uint4 k = keys[i];
-      const uint32_t g = (uint32_t)(k.x > last) | (uint32_t)(k.y > last) << 1 | (uint32_t)(k.z > last) << 2 | (uint32_t)(k.w > last) << 3;
-      const uint32_t t = (uint32_t)(k.x == last) | (uint32_t)(k.y == last) << 1 | (uint32_t)(k.z == last) << 2 | (uint32_t)(k.w == last) << 3;
-      more |= (uint64_t)g << (4 * i);
-      tied |= (uint64_t)t << (4 * i);
+      const uint32_t key[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        more |= (uint64_t)(key[y] > last) << (4 * i + y);
+        tied |= (uint64_t)(key[y] == last) << (4 * i + y);
+      }
     }
     more &= who;
     tied &= need > 0 ? who : 0ull;
     if (same > need) {  // more states have the last weight than may stay: the first of them do
       int ties[2] = {__popcll(tied), 0}, total[2], base[2];
       before_and_all(ties, total, base, told, 1, ctas, rank);
-      for (int extra = ties[0] + __popcll(tied) - max(need, ties[0]); extra > 0; --extra) tied &= ~(1ull << (63 - __clzll(tied)));
+      for (int extra = ties[0] + __popcll(tied) - max(need, ties[0]); extra > 0; --extra)
+        tied &= ~(1ull << (63 - __clzll(tied)));
     }
     const uint64_t stays = more | tied | (inner ? 0ull : safe);
     const int low_n = min(max(keep - j_cta - j_run, 0), states);  // states of the run below keep
@@ -554,7 +561,8 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
       for (; move; move &= move - 1) from[put[1]++] = j_cta + j_run + __ffsll(move) - 1;
     }
     if (a.weight_out == a.weight || (a.born && a.born_out == a.born))
-      for (uint64_t gone = valid & ~low & ~stays; gone; gone &= gone - 1) clear_own(a, at + j_cta + j_run + __ffsll(gone) - 1);
+      for (uint64_t gone = valid & ~low & ~stays; gone; gone &= gone - 1)
+        clear_own(a, at + j_cta + j_run + __ffsll(gone) - 1);
     if (a.parts == 0) {
       __syncthreads();
       Pairs& pairs = reinterpret_cast<Pairs*>(&told)[warp];  // (the counts are not looked at again)
@@ -588,7 +596,7 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_long_kernel(const __g
     uint32_t* const guarded = a.bits + unit * 2 * ((a.pages.cap + 31) / 32);
     uint32_t* const stay = guarded + (a.pages.cap + 31) / 32;
     auto key_of = [&](int w) { return w < w_end && w * 32 + lane < len ? ordered(a.weight[at + w * 32 + lane]) : 0u; };
-    for (int x = threadIdx.x; x < 4 * kBins; x += kSelect) told.bins[0][x] = 0;
+    for (int x = threadIdx.x; x < kBins; x += kSelect) reinterpret_cast<uint4*>(told.bins)[x] = make_uint4(0, 0, 0, 0);
     int all[2], n[2] = {0, 0};
     for (int w0 = w_first; w0 < w_end; w0 += kAtOnce) {
       int s[kAtOnce];
@@ -725,20 +733,25 @@ struct EvictPlan {
   long long lists, moves, bits;  // ints
   long long bytes() const { return (lists + moves + bits) * 4; }
 };
-// CTAs an (item, key head): doubled while all are resident at once (two an SM) and each still has 2048 places, or until
-// the weights fit shared memory.  apart: the new lengths do not lie on the old ones, which one kernel's CTAs read at
-// any time.
+// CTAs an (item, key head): doubled while all are resident at once (two an SM) and the states that a CTA is relieved of
+// take longer than telling one more what it counted, or until the weights fit shared memory.  Measured, us of the first
+// kernel with 1, 2, 4, 8: 128 units of 18,360 places 35, 26, 39, 72; 4 units of 16,000 22.5, 18.6, 16.8, 17.8; of 8000
+// -, 15.4, 13.2, -; of 4000 11.1, 11.2, 12.9, 17.8.
+// One kernel where there are few places (us in kernels, one and two: 256 units of 1000 places 13.7 and 18.3, of 2000 16.4
+// and 19.2, of 8000 39.5 and 33), unless the new lengths lie on the old ones, which its CTAs read at any time.
 EvictPlan evict_plan(int B, int Hkv, int cap, bool apart, int sms) {
   const long long units = (long long)B * Hkv;
   EvictPlan p{};
   p.half = std::max(1, cap / 2);  // at most min(keep, len - keep) states move
   p.words = (cap + 31) / 32;
   p.ctas = 1;
-  while (p.ctas < kMostCtas && ((2 * units * p.ctas <= 2 * sms && cap / p.ctas > 2048) || held_fours(cap, p.ctas) > kMostFours))
+  while (p.ctas < kMostCtas &&
+         ((units * p.ctas <= sms && cap > 1024 * p.ctas * p.ctas) || held_fours(cap, p.ctas) > kMostFours))
     p.ctas *= 2;
   p.held = held_fours(cap, p.ctas) <= kMostFours;
-  if (cap <= kOneKernel && apart) return p;
-  p.parts = (int)std::max(1ll, std::min(((long long)p.half + kMoveWarps * 32 - 1) / (kMoveWarps * 32), (16ll * sms + units - 1) / units));
+  if (cap <= kFewPlaces && apart) return p;
+  constexpr int each = kMoveWarps * 32;
+  p.parts = (int)std::max(1ll, std::min(((long long)p.half + each - 1) / each, (16ll * sms + units - 1) / units));
   p.lists = 2 * units * p.half;
   p.moves = units;
   p.bits = p.held ? 0 : 2 * units * p.words;
@@ -797,7 +810,8 @@ extern "C" int sb_paged_write(const sb_paged_memory* memory, const void* k, long
   };
   const bool vec = aligned(k, k_row, k_img) && aligned(v, v_row, v_img);
   int bits;
-  const bool exact = std::frexp(k_scale, &bits) == 0.5f && std::abs(bits) < 120 && std::frexp(v_scale, &bits) == 0.5f && std::abs(bits) < 120;
+  auto power = [&](float x) { return std::frexp(x, &bits) == 0.5f && std::abs(bits) < 120; };
+  const bool exact = power(k_scale) && power(v_scale);
   if (exact) {
     a.k_scale = 1.f / k_scale;
     a.v_scale = 1.f / v_scale;
@@ -829,16 +843,17 @@ extern "C" int sb_paged_evict(const sb_paged_memory* memory, const int* lens, co
   const sb_paged_memory* const m = memory;
   if (!paged_memory_ok(m)) return record_error(SB_EINVAL, "sb_paged_evict: sizes (dh 32, 64 or 128) or dtype");
   if (m->B == 0) return SB_OK;
-  if (!lens || !after || (m->N > 0 && (!weight || !weight_out)) || (since && !born) || (!born) != (!born_out) || !paged_pools_ok(m))
+  if (!lens || !after || (m->N > 0 && (!weight || !weight_out)) || (since && !born) || (!born) != (!born_out) ||
+      !paged_pools_ok(m))
     return record_error(SB_EINVAL, "sb_paged_evict: rows (16-byte aligned, strides multiples of 16 bytes) or null argument");
   EvictArgs a{};
   a.pages = page_table(m);
-  if ((a.pages.cap > kOneKernel || after == lens) && (!work || (reinterpret_cast<uintptr_t>(work) & 15) != 0))
+  if ((a.pages.cap > kFewPlaces || after == lens) && (!work || (reinterpret_cast<uintptr_t>(work) & 15) != 0))
     return record_error(SB_EINVAL, "sb_paged_evict: workspace (sb_paged_evict_work bytes, 16-byte aligned)");
   const int sms = xattn_sms();
   if (sms == 0) return record_error(SB_ECUDA, "sb_paged_evict: device");
   const EvictPlan p = evict_plan(m->B, m->Hkv, a.pages.cap, after != lens, sms);
-  if (work_bytes < p.bytes()) return record_error(SB_EINVAL, "sb_paged_evict: workspace (sb_paged_evict_work bytes, 16-byte aligned)");
+  if (work_bytes < p.bytes()) return record_error(SB_EINVAL, "sb_paged_evict: workspace (sb_paged_evict_work bytes)");
   a.k = k_pool(m);
   a.v = v_pool(m);
   a.lens = lens; a.keep = keep; a.keep_all = keep_all; a.since = since;
@@ -854,8 +869,9 @@ extern "C" int sb_paged_evict(const sb_paged_memory* memory, const int* lens, co
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = evict_select(a, p.held, units, st);
   if (e == cudaSuccess && p.parts) {
-    auto move = a.row_bytes == 32   ? evict_move_kernel<2>
-                : a.row_bytes == 64 ? evict_move_kernel<4> : a.row_bytes == 128 ? evict_move_kernel<8> : evict_move_kernel<16>;
+    auto move = a.row_bytes == 32    ? evict_move_kernel<2>
+                : a.row_bytes == 64  ? evict_move_kernel<4>
+                : a.row_bytes == 128 ? evict_move_kernel<8> : evict_move_kernel<16>;
     e = launch_after(move, units * a.parts, kMoveWarps * 32, 0, st, a);
   }
   return e == cudaSuccess ? SB_OK : record_error(SB_ECUDA, cudaGetErrorString(e));

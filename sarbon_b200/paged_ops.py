@@ -203,8 +203,9 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
     Pages have the states' type, or e4m3: the code nearest to the fp32 quotient ``x / k_scale`` (``v_scale``), at
     most 448 of either sign.  The new states' weight becomes 0 and born their stamp (int32 [B, T], or [B] for
     all of an item's).  States behind an item's pages are dropped, rows on no page are not written, and what
-    lies from ``count[b]`` on is left alone.  An item's pages that are written must be its own.  after (allocated if None) shares no memory with at.  kv_heads is that of weight
-    or born where they are given; without them the rows are taken as heads of 32 channels."""
+    lies from ``count[b]`` on is left alone.  An item's pages that are written must be its own.  after
+    (allocated if None) shares no memory with at.  kv_heads is that of weight or born where they are given;
+    without them the rows are taken as heads of 32 channels."""
     dtype, page_dtype, rows = k.dtype, k_pages.dtype, k.shape
     if len(rows) != 3 or (dtype != torch.bfloat16 and dtype != torch.float16):
         raise ValueError("k, v: [B, T, kv_heads * dim] rows of fp16 or bf16")
