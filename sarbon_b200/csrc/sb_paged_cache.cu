@@ -745,11 +745,14 @@ EvictPlan evict_plan(int B, int Hkv, int cap, bool apart, int sms) {
   p.half = std::max(1, cap / 2);  // at most min(keep, len - keep) states move
   p.words = (cap + 31) / 32;
   p.ctas = 1;
+  if (cap <= kFewPlaces && apart) {  // (its pairs lie in one CTA's shared memory)
+    p.held = true;
+    return p;
+  }
   while (p.ctas < kMostCtas &&
          ((units * p.ctas <= sms && cap > 1024 * p.ctas * p.ctas) || held_fours(cap, p.ctas) > kMostFours))
     p.ctas *= 2;
   p.held = held_fours(cap, p.ctas) <= kMostFours;
-  if (cap <= kFewPlaces && apart) return p;
   constexpr int each = kMoveWarps * 32;
   p.parts = (int)std::max(1ll, std::min(((long long)p.half + each - 1) / each, (16ll * sms + units - 1) / units));
   p.lists = 2 * units * p.half;

@@ -451,6 +451,7 @@ def check_eviction(k, v, table, lens, weight, keep, born, since, **how):
 @pytest.mark.parametrize("b,n,kv_heads,dim,page,keep", [
     (1, 2, 1, 32, 1, 1), (2, 1, 2, 64, 4, 0), (3, 241, 4, 128, 16, 240), (2, 500, 3, 64, 7, 250), (2, 1025, 1, 128, 60, 1),
     (1, 2100, 2, 32, 100, 1024), (2, 33, 2, 64, 33, 32), (1, 4000, 1, 128, 250, 3999), (2, 64, 1, 64, 3, 64), (1, 70, 1, 32, 5, 1000),
+    (2, 1100, 2, 32, 60, 950), (1, 1412, 3, 32, 240, 1256), (1, 2018, 1, 128, 1, 1009), (3, 2018, 1, 32, 256, 2000),
 ])
 def test_evict(b, n, kv_heads, dim, page, keep, pt):
     g = gen(n + keep)
