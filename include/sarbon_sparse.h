@@ -551,18 +551,27 @@ typedef struct {
   int B, Hkv, dh;
 } sb_paged_memory;
 
-/* Attention of Tq query tokens, [B][Tq][H*dh] rows of SB_F16 or SB_BF16 (16-byte aligned, strides multiples of 8), to
- * the first lens[b] states of each item: out = softmax(scale q k^T) v per head, query head h on key head
- * h / (H / Hkv).  causal != 0: query t sees the first lens[b] - Tq + 1 + t.  Pages: q_dtype or SB_F8.  States
- * on no page take no part; a query without states gets zeros.  lse (fp32 [B][H][Tq], NULL: none): natural log of
- * the sum of the exponentials, -inf without states.  weight (NULL: none): decay * weight + the sum of the
- * probabilities of a key head's queries, for the states below lens[b]; fixed order.  work:
+/* Attention of Tq query tokens q, [B][Tq][H*dh] rows of SB_F16 or SB_BF16 (16-byte aligned, strides multiples of 8,
+ * element (b, t, c) at q[b * q_img + t * q_row + c]; out alike), to the first lens[b] states of each item: out =
+ * softmax(scale q k^T) v per head, query head h on key head h / (H / Hkv).  causal != 0: query t sees the first lens[b] -
+ * Tq + 1 + t.  Pages: q_dtype or SB_F8.  States on no page take no part; a query without states gets zeros.  lse (fp32
+ * [B][H][Tq], NULL: none): natural log of the sum of the exponentials, -inf without states.  weight (NULL: none): decay *
+ * weight + the sum of the probabilities of a key head's queries, for the states below lens[b]; fixed order.  work:
  * sb_paged_attention_work bytes (16-byte aligned), not shared by calls that may overlap.  Scores, statistics,
  * probabilities and sums are fp32; probabilities meet v as two 16-bit parts. */
-SB_API int sb_paged_attention(const sb_paged_memory* memory, const void* q, long long q_row, long long q_img, int q_dtype,
-                              const int* lens, int H, int Tq, float scale, float k_scale, float v_scale, int causal,
-                              void* out, long long o_row, long long o_img, float* lse, float* weight, float decay,
-                              void* work, long long work_bytes, void* stream);
+typedef struct {
+  sb_paged_memory memory;
+  const void* q;
+  void* out;
+  long long q_row, q_img, out_row, out_img;
+  const int* lens;
+  float *lse, *weight;
+  void* work;
+  long long work_bytes;
+  int q_dtype, H, Tq, causal;
+  float scale, k_scale, v_scale, decay;
+} sb_paged_attend;
+SB_API int sb_paged_attention(const sb_paged_attend* call, void* stream);
 
 /* Bytes of workspace that sb_paged_attention needs on the current device (account: with weight). */
 SB_API int sb_paged_attention_work(int B, int H, int Hkv, int dh, int Tq, int page_dtype, int page, int N, int account,
@@ -570,22 +579,42 @@ SB_API int sb_paged_attention_work(int B, int H, int Hkv, int dh, int Tq, int pa
 
 /* New states: row t < count[b] (NULL: T) of k, v [B][T][Hkv*dh] (SB_F16 or SB_BF16, any strides) goes to
  * position at[b] + t of item b; pools of the same type, or SB_F8: the code nearest to the fp32 quotient
- * x / scale, at most 448 of either sign.  weight there becomes 0, born stamp[b * stamp_img + t * stamp_row] (each may be NULL).
- * after [B] gets the new lengths and shares no memory with at. */
-SB_API int sb_paged_write(const sb_paged_memory* memory, const void* k, long long k_row, long long k_img, const void* v,
-                          long long v_row, long long v_img, int dtype, const int* at, const int* count, int T,
-                          float k_scale, float v_scale, float* weight, int* born, const int* stamp, long long stamp_img,
-                          long long stamp_row, int* after, void* stream);
+ * x / scale, at most 448 of either sign.  weight there becomes 0, born stamp[b * stamp_img + t * stamp_row] (each
+ * may be NULL).  after [B] gets the new lengths and shares no memory with at. */
+typedef struct {
+  sb_paged_memory memory;
+  const void *k, *v;
+  long long k_row, k_img, v_row, v_img;
+  const int *at, *count;
+  float* weight;
+  int* born;
+  const int* stamp;
+  long long stamp_img, stamp_row;
+  int* after;
+  int dtype, T;
+  float k_scale, v_scale;
+} sb_paged_append;
+SB_API int sb_paged_write(const sb_paged_append* call, void* stream);
 
 /* Eviction: of the lens[b] states of each item and key head the keep[b] (keep NULL: keep_all) first by (born >=
  * since[b], weight descending, index) stay (NaN is the least; since NULL: weight alone).  The i-th freed place
  * below keep takes the i-th kept state from keep on.  weight_out and born_out get the weights and stamps
  * that stay, 0 from the new length on; after [B] the new lengths.  They may be weight, born and lens themselves.
  * work: sb_paged_evict_work bytes, as above. */
-SB_API int sb_paged_evict(const sb_paged_memory* memory, const int* lens, const int* keep, int keep_all, const int* since,
-                          const float* weight, const int* born, float* weight_out, int* born_out, int* after, void* work,
-                          long long work_bytes, void* stream);
-SB_API int sb_paged_evict_work(int B, int Hkv, int page, int N, int in_place, long long* bytes); /* in_place: after is lens */
+typedef struct {
+  sb_paged_memory memory;
+  const int *lens, *keep, *since;
+  const float* weight;
+  const int* born;
+  float* weight_out;
+  int *born_out, *after;
+  void* work;
+  long long work_bytes;
+  int keep_all;
+} sb_paged_cut;
+SB_API int sb_paged_evict(const sb_paged_cut* call, void* stream);
+/* in_place: after is lens */
+SB_API int sb_paged_evict_work(int B, int Hkv, int page, int N, int in_place, long long* bytes);
 
 /* Counters (fused_engine.py:92,239) and sticky device errors (synchronises). */
 SB_API int sb_stats(sb_engine* e, void* stream, sb_stats_t* out);

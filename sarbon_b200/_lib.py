@@ -117,12 +117,11 @@ PROTOTYPES = {
     "sb_gated_norm_work": (_I, [_I, _I, _I, C.POINTER(_LL)]),
     "sb_gated_norm_backward": (_I, [_P, _LL, _LL] * 2 + [_P, _LL, _LL, _I] * 2 + [_P, _LL, _LL] + [_P] * 5
                                + [_I, C.c_float, _I, _I, _I] + [_P] * 4 + [_I] + [_P] * 5 + [_LL, _P]),
-    # (sb_paged_memory by pointer; paged_ops packs it as bytes)
-    "sb_paged_attention": (_I, [C.c_char_p, _P, _LL, _LL, _I, _P, _I, _I] + [C.c_float] * 3 + [_I, _P, _LL, _LL, _P, _P, C.c_float,
-                                _P, _LL, _P]),
+    # (structs by pointer; paged_ops packs them as bytes)
+    "sb_paged_attention": (_I, [C.c_char_p, _P]),
     "sb_paged_attention_work": (_I, [_I] * 9 + [C.POINTER(_LL)]),
-    "sb_paged_write": (_I, [C.c_char_p] + [_P, _LL, _LL] * 2 + [_I, _P, _P, _I] + [C.c_float] * 2 + [_P, _P, _P, _LL, _LL, _P, _P]),
-    "sb_paged_evict": (_I, [C.c_char_p, _P, _P, _I] + [_P] * 7 + [_LL, _P]),
+    "sb_paged_write": (_I, [C.c_char_p, _P]),
+    "sb_paged_evict": (_I, [C.c_char_p, _P]),
     "sb_paged_evict_work": (_I, [_I] * 5 + [C.POINTER(_LL)]),
     "sb_stats": (_I, [_P, _P, C.POINTER(Stats)]),
     "sb_last_launch_count": (_I, [_P]),

@@ -953,44 +953,44 @@ extern "C" int sb_paged_attention_work(int B, int H, int Hkv, int dh, int Tq, in
   return SB_OK;
 }
 
-extern "C" int sb_paged_attention(const sb_paged_memory* memory, const void* q, long long q_row, long long q_img, int q_dtype,
-                                  const int* lens, int H, int Tq, float scale, float k_scale, float v_scale, int causal,
-                                  void* out, long long o_row, long long o_img, float* lse, float* weight, float decay,
-                                  void* work, long long work_bytes, void* stream) {
-  const sb_paged_memory* const m = memory;
+extern "C" int sb_paged_attention(const sb_paged_attend* call, void* stream) {
+  if (!call) return record_error(SB_EINVAL, "sb_paged_attention: null argument");
+  const sb_paged_attend& c = *call;
+  const sb_paged_memory* const m = &c.memory;
+  const int H = c.H, Tq = c.Tq;
   if (!paged_memory_ok(m) || !paged_attention_sizes_ok(m->B, H, m->Hkv, m->dh, Tq, m->P, m->page, m->N) ||
-      (q_dtype != SB_F16 && q_dtype != SB_BF16) || (m->dtype != q_dtype && m->dtype != SB_F8))
+      (c.q_dtype != SB_F16 && c.q_dtype != SB_BF16) || (m->dtype != c.q_dtype && m->dtype != SB_F8))
     return record_error(SB_EINVAL, "sb_paged_attention: sizes (dh 32, 64 or 128, H a multiple of Hkv) or dtypes");
-  if (!(scale > 0.f) || !scales_ok(m, k_scale, v_scale) || !std::isnormal(scale * k_scale))
+  if (!(c.scale > 0.f) || !scales_ok(m, c.k_scale, c.v_scale) || !std::isnormal(c.scale * c.k_scale))
     return record_error(SB_EINVAL, "sb_paged_attention: scale, or scales of pages that are not e4m3");
-  if (weight && !(decay >= 0.f && decay <= 1.f)) return record_error(SB_EINVAL, "sb_paged_attention: decay from 0 to 1");
+  if (c.weight && !(c.decay >= 0.f && c.decay <= 1.f)) return record_error(SB_EINVAL, "sb_paged_attention: decay from 0 to 1");
   if (m->B == 0 || Tq == 0) return SB_OK;
-  if (!lens || !xattn_view_ok(q, q_row, q_img) || !xattn_view_ok(out, o_row, o_img) || !paged_pools_ok(m))
+  if (!c.lens || !xattn_view_ok(c.q, c.q_row, c.q_img) || !xattn_view_ok(c.out, c.out_row, c.out_img) || !paged_pools_ok(m))
     return record_error(SB_EINVAL, "sb_paged_attention: rows (16-byte aligned, strides multiples of 16 bytes) or null argument");
   const int sms = xattn_sms();
   if (sms == 0) return record_error(SB_ECUDA, "sb_paged_attention: device");
   PagedArgs a{};
   a.pages = page_table(m);
-  const PagedPlan p = paged_plan(m->B, H, m->Hkv, m->dh, Tq, m->dtype, a.pages.cap, weight != nullptr, sms);
-  if (p.bytes() > 0 && (!work || work_bytes < p.bytes() || (reinterpret_cast<uintptr_t>(work) & 15) != 0))
+  const PagedPlan p = paged_plan(m->B, H, m->Hkv, m->dh, Tq, m->dtype, a.pages.cap, c.weight != nullptr, sms);
+  if (p.bytes() > 0 && (!c.work || c.work_bytes < p.bytes() || (reinterpret_cast<uintptr_t>(c.work) & 15) != 0))
     return record_error(SB_EINVAL, "sb_paged_attention: workspace (sb_paged_attention_work bytes, 16-byte aligned)");
   const long long ctas = p.shares ? p.shares : p.units, ends = (long long)p.ends * m->B * m->Hkv;
   if (ctas > 0x7FFFFFFFll || ends > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_paged_attention: too many items");
-  a.q = q; a.q_row = q_row; a.q_img = q_img;
+  a.q = c.q; a.q_row = c.q_row; a.q_img = c.q_img;
   a.k = k_pool(m);
   a.v = v_pool(m);
-  a.lens = lens;
+  a.lens = c.lens;
   a.B = m->B; a.H = H; a.Hkv = m->Hkv; a.group = H / m->Hkv; a.Tq = Tq;
   a.rows = p.rows; a.blocks = p.blocks; a.shares = p.shares; a.ends = p.ends; a.chunk = p.chunk; a.part_rows = p.part_rows;
   a.places = p.places; a.score_rows = p.score_rows;
-  a.q_bf16 = q_dtype == SB_BF16; a.causal = causal != 0;
-  a.scale_log2 = scale * k_scale * 1.4426950408889634f;
-  a.v_scale = v_scale;
-  a.o = {out, o_row, o_img};
-  a.lse = lse;
-  a.weight = p.scores > 0 || p.held ? weight : nullptr;  // (no places: no account)
-  a.decay = decay;
-  float* w = static_cast<float*>(work);
+  a.q_bf16 = c.q_dtype == SB_BF16; a.causal = c.causal != 0;
+  a.scale_log2 = c.scale * c.k_scale * 1.4426950408889634f;
+  a.v_scale = c.v_scale;
+  a.o = {c.out, c.out_row, c.out_img};
+  a.lse = c.lse;
+  a.weight = p.scores > 0 || p.held ? c.weight : nullptr;  // (no places: no account)
+  a.decay = c.decay;
+  float* w = static_cast<float*>(c.work);
   a.scores = p.scores > 0 ? w : nullptr;
   a.part_l = w + p.scores;
   a.part_o = a.part_l + p.part_l;

@@ -775,18 +775,21 @@ cudaError_t evict_select(const EvictArgs& a, bool held, long long units, cudaStr
 
 using namespace sb;
 
-extern "C" int sb_paged_write(const sb_paged_memory* memory, const void* k, long long k_row, long long k_img, const void* v,
-                              long long v_row, long long v_img, int dtype, const int* at, const int* count, int T,
-                              float k_scale, float v_scale, float* weight, int* born, const int* stamp, long long stamp_img,
-                              long long stamp_row, int* after, void* stream) {
-  const sb_paged_memory* const m = memory;
+extern "C" int sb_paged_write(const sb_paged_append* call, void* stream) {
+  if (!call) return record_error(SB_EINVAL, "sb_paged_write: null argument");
+  const sb_paged_append& c = *call;
+  const sb_paged_memory* const m = &c.memory;
+  const void *const k = c.k, *const v = c.v;
+  const long long k_row = c.k_row, k_img = c.k_img, v_row = c.v_row, v_img = c.v_img;
+  const int T = c.T, dtype = c.dtype;
+  const float k_scale = c.k_scale, v_scale = c.v_scale;
   if (!paged_memory_ok(m) || T < 0 || T >= (1 << 30) || (dtype != SB_F16 && dtype != SB_BF16) ||
       (m->dtype != dtype && m->dtype != SB_F8))
     return record_error(SB_EINVAL, "sb_paged_write: sizes (dh 32, 64 or 128) or dtypes");
   if (!scales_ok(m, k_scale, v_scale)) return record_error(SB_EINVAL, "sb_paged_write: scales, or scales of pages that are not e4m3");
   if (m->B == 0) return SB_OK;
   const bool some = T > 0 && m->P > 0 && m->N > 0;
-  if (!at || !after || !paged_pools_ok(m) || (some && (!k || !v || k_row < 0 || k_img < 0 || v_row < 0 || v_img < 0)))
+  if (!c.at || !c.after || !paged_pools_ok(m) || (some && (!k || !v || k_row < 0 || k_img < 0 || v_row < 0 || v_img < 0)))
     return record_error(SB_EINVAL, "sb_paged_write: rows (pools 16-byte aligned, strides multiples of 16 bytes) or null argument");
   WriteArgs a{};
   a.k = k; a.k_row = k_row; a.k_img = k_img;
@@ -794,10 +797,10 @@ extern "C" int sb_paged_write(const sb_paged_memory* memory, const void* k, long
   a.kp = k_pool(m);
   a.vp = v_pool(m);
   a.pages = page_table(m);
-  a.at = at; a.count = count; a.stamp = stamp; a.stamp_img = stamp_img; a.stamp_row = stamp_row;
+  a.at = c.at; a.count = c.count; a.stamp = c.stamp; a.stamp_img = c.stamp_img; a.stamp_row = c.stamp_row;
   a.B = m->B; a.T = T; a.Hkv = m->Hkv;
   a.k_scale = k_scale; a.v_scale = v_scale;
-  a.weight = weight; a.born = born; a.after = after;
+  a.weight = c.weight; a.born = c.born; a.after = c.after;
   const bool e4m3 = m->dtype == SB_F8;
   const int vecs = m->Hkv * m->dh / 8;
   a.vecs = fast_div((uint32_t)vecs);
@@ -805,7 +808,7 @@ extern "C" int sb_paged_write(const sb_paged_memory* memory, const void* k, long
   a.rows = some ? (long long)m->B * T : 0;
   const long long warps = (a.rows + a.group - 1) / a.group;
   a.row_blocks = (warps + kWriteWarps - 1) / kWriteWarps;
-  a.marks = m->B + (T > 0 && m->N > 0 && (weight || born) ? (long long)m->B * m->Hkv * T : 0);
+  a.marks = m->B + (T > 0 && m->N > 0 && (c.weight || c.born) ? (long long)m->B * m->Hkv * T : 0);
   const long long blocks = a.row_blocks + (a.marks + kWriteWarps * 32 - 1) / (kWriteWarps * 32);
   if (blocks > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_paged_write: too many rows");
   auto aligned = [](const void* p, long long row, long long img) {
@@ -840,32 +843,32 @@ extern "C" int sb_paged_evict_work(int B, int Hkv, int page, int N, int in_place
   return SB_OK;
 }
 
-extern "C" int sb_paged_evict(const sb_paged_memory* memory, const int* lens, const int* keep, int keep_all, const int* since,
-                              const float* weight, const int* born, float* weight_out, int* born_out, int* after, void* work,
-                              long long work_bytes, void* stream) {
-  const sb_paged_memory* const m = memory;
+extern "C" int sb_paged_evict(const sb_paged_cut* call, void* stream) {
+  if (!call) return record_error(SB_EINVAL, "sb_paged_evict: null argument");
+  const sb_paged_cut& c = *call;
+  const sb_paged_memory* const m = &c.memory;
   if (!paged_memory_ok(m)) return record_error(SB_EINVAL, "sb_paged_evict: sizes (dh 32, 64 or 128) or dtype");
   if (m->B == 0) return SB_OK;
-  if (!lens || !after || (m->N > 0 && (!weight || !weight_out)) || (since && !born) || (!born) != (!born_out) ||
+  if (!c.lens || !c.after || (m->N > 0 && (!c.weight || !c.weight_out)) || (c.since && !c.born) || (!c.born) != (!c.born_out) ||
       !paged_pools_ok(m))
     return record_error(SB_EINVAL, "sb_paged_evict: rows (16-byte aligned, strides multiples of 16 bytes) or null argument");
   EvictArgs a{};
   a.pages = page_table(m);
-  if ((a.pages.cap > kFewPlaces || after == lens) && (!work || (reinterpret_cast<uintptr_t>(work) & 15) != 0))
+  if ((a.pages.cap > kFewPlaces || c.after == c.lens) && (!c.work || (reinterpret_cast<uintptr_t>(c.work) & 15) != 0))
     return record_error(SB_EINVAL, "sb_paged_evict: workspace (sb_paged_evict_work bytes, 16-byte aligned)");
   const int sms = xattn_sms();
   if (sms == 0) return record_error(SB_ECUDA, "sb_paged_evict: device");
-  const EvictPlan p = evict_plan(m->B, m->Hkv, a.pages.cap, after != lens, sms);
-  if (work_bytes < p.bytes()) return record_error(SB_EINVAL, "sb_paged_evict: workspace (sb_paged_evict_work bytes)");
+  const EvictPlan p = evict_plan(m->B, m->Hkv, a.pages.cap, c.after != c.lens, sms);
+  if (c.work_bytes < p.bytes()) return record_error(SB_EINVAL, "sb_paged_evict: workspace (sb_paged_evict_work bytes)");
   a.k = k_pool(m);
   a.v = v_pool(m);
-  a.lens = lens; a.keep = keep; a.keep_all = keep_all; a.since = since;
-  a.weight = weight; a.weight_out = weight_out; a.born = born; a.born_out = born_out; a.after = after;
+  a.lens = c.lens; a.keep = c.keep; a.keep_all = c.keep_all; a.since = c.since;
+  a.weight = c.weight; a.weight_out = c.weight_out; a.born = c.born; a.born_out = c.born_out; a.after = c.after;
   a.B = m->B; a.Hkv = m->Hkv; a.row_bytes = m->dh * page_dtype_bytes(m->dtype); a.half = p.half;
   a.ctas = p.ctas; a.parts = p.parts;
   const long long units = (long long)m->B * m->Hkv;
   if (units * std::max(p.ctas, p.parts) > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_paged_evict: too many items");
-  a.to = static_cast<int*>(work);
+  a.to = static_cast<int*>(c.work);
   a.from = a.to + units * p.half;
   a.moves = a.from + units * p.half;
   a.bits = reinterpret_cast<uint32_t*>(a.moves + units);

@@ -33,11 +33,34 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
-from .memory_ops import _INF, _apart, _launch, _new, _ready, _rows, _statistics, _work
+from ._lib import check, lib
+from .memory_ops import _apart, _device, _new, _raw_stream, _ready, _rows, _statistics, _work
 
 E4M3 = torch.float8_e4m3fn
-_MEMORY = struct.Struct("@PPqqqqPqiiiiiii4x")  # sb_paged_memory
+_MOST = 3.4e38  # of fp32
+# sb_paged_attend, sb_paged_append, sb_paged_cut, each from its sb_paged_memory on: a call's host time is what a small call
+# costs, and a struct packed at once costs less of it than as many arguments
+_MEMORY = "@PPqqqqPqiiiiiii4x"
+_ATTEND = struct.Struct(_MEMORY + "PPqqqqPPPPqiiiiffff")
+_APPEND = struct.Struct(_MEMORY + "PPqqqqPPPPPqqPiiff")
+_CUT = struct.Struct(_MEMORY + "PPPPPPPPPqi4x")
 PAGE_DTYPES = {torch.float16: _lib.SB_F16, torch.bfloat16: _lib.SB_BF16, E4M3: _lib.SB_F8}
+
+
+# library calls made through this module
+CALLS = [0]
+
+
+def _call(name, index, packed):
+    CALLS[0] += 1
+    entry = getattr(lib(), name)
+    if index == _device():
+        status = entry(packed, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(packed, _raw_stream(index))
+    if status:
+        check(status, name)
 
 
 def _overlap(row, img, pages, page, width):
@@ -47,7 +70,7 @@ def _overlap(row, img, pages, page, width):
 
 
 def _memory(k_pages, v_pages, table, kv_heads, written=False):
-    """The memory of a call: (sb_paged_memory, batch, page, entries, dim)."""
+    """The memory of a call: (the fields of sb_paged_memory, batch, page, entries, dim)."""
     shape, dtype = k_pages.shape, k_pages.dtype
     code = PAGE_DTYPES.get(dtype)
     if len(shape) != 3 or code is None or v_pages.shape != shape or v_pages.dtype != dtype:
@@ -76,8 +99,8 @@ def _memory(k_pages, v_pages, table, kv_heads, written=False):
     b, n = at
     if n * page >= 1 << 30:
         raise ValueError("table: fewer than 2^30 states an item")
-    return _MEMORY.pack(k, v, k_row, k_img, v_row, v_img, table.data_ptr(), step[0] if b > 1 else n, code, pages, page, n, b,
-                        kv_heads, dim), b, page, n, dim
+    return (k, v, k_row, k_img, v_row, v_img, table.data_ptr(), step[0] if b > 1 else n, code, pages, page, n, b, kv_heads, dim), \
+        b, page, n, dim
 
 
 def _each(t, what, b):
@@ -115,7 +138,7 @@ def _one_device(floats, others):
 
 
 def _scales(k_scale, v_scale, dtype):
-    if not (0.0 < k_scale < _INF and 0.0 < v_scale < _INF):
+    if not (0.0 < k_scale < _MOST and 0.0 < v_scale < _MOST):
         raise ValueError("k_scale, v_scale: positive numbers")
     if dtype != E4M3 and (k_scale != 1.0 or v_scale != 1.0):
         raise ValueError("k_scale, v_scale: of e4m3 pages only")
@@ -164,14 +187,14 @@ def paged_attention(q, k_pages, v_pages, table, lens, heads, kv_heads=None, scal
     shape = (b, tq, heads * dim)
     if scale is None:
         scale = dim ** -0.5
-    if not 0.0 < scale < _INF or not 0.0 <= decay <= 1.0:
+    if not 0.0 < scale < _MOST or not 0.0 <= decay <= 1.0:
         raise ValueError("scale: a positive number; decay: from 0 to 1")
     if k_scale != 1.0 or v_scale != 1.0:
         _scales(k_scale, v_scale, page_dtype)
     if lens is None:
         raise ValueError("lens: contiguous int32 [B]")
     qp, p_lens = _rows(q, "q", shape, dtype), _each(lens, "lens", b)
-    p_weight = p_lse = None
+    p_weight = p_lse = 0
     if weight is not None:
         p_weight = _account(weight, "weight", (b, kv_heads, n * page), torch.float32)
     if lse is not None:
@@ -188,9 +211,10 @@ def paged_attention(q, k_pages, v_pages, table, lens, heads, kv_heads=None, scal
     if b == 0 or tq == 0:
         return out
     hold, work, size = _work("sb_paged_attention_work", index, b, heads, kv_heads, dim, tq, PAGE_DTYPES[page_dtype], page, n,
-                             p_weight is not None)
-    _launch("sb_paged_attention", index, memory, *qp, PAGE_DTYPES[dtype], p_lens, heads, tq, scale, k_scale, v_scale, causal, *op,
-            p_lse, p_weight, decay, work, size)
+                             weight is not None)
+    _call("sb_paged_attention", index, _ATTEND.pack(*memory, qp[0], op[0], qp[1], qp[2], op[1], op[2], p_lens, p_lse, p_weight,
+                                                    work or 0, size, PAGE_DTYPES[dtype], heads, tq, causal, scale, k_scale,
+                                                    v_scale, decay))
     return out
 
 
@@ -229,7 +253,7 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
         raise ValueError("results need their own memory")
     if at is None:
         raise ValueError("at: contiguous int32 [B]")
-    p_at, p_count, p_weight, p_born, sp = _each(at, "at", b), None, None, None, _NO_STAMP
+    p_at, p_count, p_weight, p_born, sp = _each(at, "at", b), 0, 0, 0, _NO_STAMP
     if count is not None:
         p_count = _each(count, "count", b)
     if weight is not None:
@@ -249,12 +273,12 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
         p_after = after.data_ptr()
     if b == 0:
         return after
-    _launch("sb_paged_write", index, memory, *kp, *vp, PAGE_DTYPES[dtype], p_at, p_count, t, k_scale, v_scale, p_weight, p_born,
-            *sp, p_after)
+    _call("sb_paged_write", index, _APPEND.pack(*memory, kp[0], vp[0], kp[1], kp[2], vp[1], vp[2], p_at, p_count, p_weight, p_born,
+                                                *sp, p_after, PAGE_DTYPES[dtype], t, k_scale, v_scale))
     return after
 
 
-_NO_STAMP = (None, 0, 0)
+_NO_STAMP = (0, 0, 0)
 
 
 # ---------------------------------------------------------------- eviction
@@ -277,7 +301,7 @@ def paged_evict(k_pages, v_pages, table, lens, weight, keep, born=None, since=No
     if places != (b, kv_heads, n * page) or lens is None:
         raise ValueError("weight: [B, kv_heads, N * page]; lens: contiguous int32 [B]")
     pw, p_lens = _account(weight, "weight", places, torch.float32), _each(lens, "lens", b)
-    pb = p_since = p_keep = None
+    pb = p_since = p_keep = 0
     if born is not None:
         pb = _account(born, "born", places, torch.int32)
     elif since is not None or born_out is not None:
@@ -291,7 +315,7 @@ def paged_evict(k_pages, v_pages, table, lens, weight, keep, born=None, since=No
         keep_all = min(int(keep), 1 << 30)
         if keep_all < 0 or keep_all != min(keep, 1 << 30):
             raise ValueError("keep: a whole number from 0 on, or int32 [B]")
-    pwo = pbo = p_after = None
+    pwo = pbo = p_after = 0
     if weight_out is not None or born_out is not None or after is not None:
         own = []
         if weight_out is not None:
@@ -303,20 +327,20 @@ def paged_evict(k_pages, v_pages, table, lens, weight, keep, born=None, since=No
         if after is not None:
             p_after = _each(after, "after", b)
             own.append(after if p_after != p_lens else None)
-        _clear_of(own, (weight, born, lens, since, keep if p_keep is not None else None))
+        _clear_of(own, (weight, born, lens, since, keep if p_keep else None))
     index = _one_device((k_pages, v_pages, weight, weight_out),
-                        (table, lens, born, since, keep if p_keep is not None else None, born_out, after))
+                        (table, lens, born, since, keep if p_keep else None, born_out, after))
     if after is None:
         after = torch.empty_like(lens)
         p_after = after.data_ptr()
     if weight_out is None:
         weight_out = torch.empty_like(weight)
         pwo = weight_out.data_ptr()
-    if pb is not None and born_out is None:
+    if born is not None and born_out is None:
         born_out = torch.empty_like(born)
         pbo = born_out.data_ptr()
     if b == 0:
         return after, weight_out, born_out
     hold, work, size = _work("sb_paged_evict_work", index, b, kv_heads, page, n, p_after == p_lens)
-    _launch("sb_paged_evict", index, memory, p_lens, p_keep, keep_all, p_since, pw, pb, pwo, pbo, p_after, work, size)
+    _call("sb_paged_evict", index, _CUT.pack(*memory, p_lens, p_keep, p_since, pw, pb, pwo, pbo, p_after, work or 0, size, keep_all))
     return after, weight_out, born_out

@@ -40,8 +40,8 @@ MEMORY = [
     dict(q=torch.zeros(2, 1, 256)), dict(q=torch.zeros(2, 256, **H16)), dict(q=torch.zeros(2, 1, 256, dtype=torch.bfloat16)),
     dict(q=torch.zeros(1, 1, 256, **H16)), dict(heads=3), dict(heads=8, kv_heads=3), dict(kv_heads=None), dict(heads=0),
     dict(lens=None), dict(lens=torch.zeros(2, dtype=torch.int64)), dict(lens=torch.zeros(3, **I32)),
-    dict(lens=torch.zeros(4, **I32)[::2]), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")),
-    dict(decay=-0.1), dict(decay=1.1), dict(decay=float("nan")), dict(k_scale=2.0), dict(v_scale=0.5), dict(k_scale=0.0),
+    dict(lens=torch.zeros(4, **I32)[::2]), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=1e39),
+    dict(k_scale=float("nan")), dict(v_scale=1e39), dict(decay=-0.1), dict(decay=1.1), dict(decay=float("nan")), dict(k_scale=2.0), dict(v_scale=0.5), dict(k_scale=0.0),
     dict(weight=torch.zeros(2, 2, 11)), dict(weight=torch.zeros(2, 4, 12)), dict(weight=torch.zeros(2, 2, 12, **H16)),
     dict(weight=torch.zeros(2, 12, 2).transpose(1, 2)), dict(lse=torch.zeros(2, 4, 2)), dict(out=torch.zeros(2, 1, 128, **H16)),
     dict(out=ATTEND["q"]),
@@ -102,40 +102,42 @@ def test_autograd_inputs_are_refused():
 
 def test_library_refuses():
     """The C entries turn down what the wrappers never pass, before any device call."""
-    from sarbon_b200.paged_ops import _MEMORY
-    lib, n, one = _lib.lib(), C.c_longlong(0), C.c_void_p(16)
+    from sarbon_b200.paged_ops import _APPEND, _ATTEND, _CUT
+    lib, n = _lib.lib(), C.c_longlong(0)
 
     def memory(kp=16, vp=32, kr=64, pt=0, p=4, page=4, table=16, tr=2, nn=2, b=1, hkv=1, dh=32):
-        return _MEMORY.pack(kp, vp, kr, 256, kr, 256, table, tr, pt, p, page, nn, b, hkv, dh)
+        return kp, vp, kr, 256, kr, 256, table, tr, pt, p, page, nn, b, hkv, dh
 
     wrong = [dict(pt=1), dict(dh=48), dict(hkv=0), dict(b=-1), dict(page=0), dict(p=-1), dict(nn=-1), dict(page=1 << 20, nn=1 << 10),
-             dict(kr=60), dict(kr=-8), dict(kp=0), dict(vp=0), dict(kp=8), dict(table=0), dict(tr=-1), None]
+             dict(kr=60), dict(kr=-8), dict(kp=0), dict(vp=0), dict(kp=8), dict(table=0), dict(tr=-1)]
 
-    def attention(m=memory(), q=one, row=64, qt=0, lens=one, h=2, tq=1, scale=1.0, ks=1.0, weight=None, decay=1.0, work=None, size=0):
-        return lib.sb_paged_attention(m, q, row, 64, qt, lens, h, tq, scale, ks, 1.0, 0, one, row, 64, None, weight, decay, work, size, None)
+    def attention(m=memory(), q=16, row=64, qt=0, lens=16, h=2, tq=1, scale=1.0, ks=1.0, weight=0, decay=1.0, work=0, size=0):
+        return lib.sb_paged_attention(_ATTEND.pack(*m, q, 16, row, 64, row, 64, lens, 0, weight, work, size, qt, h, tq, 0, scale, ks, 1.0,
+                                                   decay), None)
 
-    def write(m=memory(), k=one, dt=0, ks=1.0, at=one, after=one, t=1, kr=32):
-        return lib.sb_paged_write(m, k, kr, 32, one, kr, 32, dt, at, None, t, ks, 1.0, None, None, None, 0, 0, after, None)
+    def write(m=memory(), k=16, dt=0, ks=1.0, at=16, after=16, t=1, kr=32):
+        return lib.sb_paged_write(_APPEND.pack(*m, k, 16, kr, 32, kr, 32, at, 0, 0, 0, 0, 0, 0, after, dt, t, ks, 1.0), None)
 
-    def evict(m=memory(), lens=one, weight=one, since=None, born=None, born_out=None, work=one, size=1 << 20):
-        return lib.sb_paged_evict(m, lens, None, 2, since, weight, born, weight, born_out, one, work, size, None)
+    def evict(m=memory(), lens=16, weight=16, since=0, born=0, born_out=0, work=16, size=1 << 20):
+        return lib.sb_paged_evict(_CUT.pack(*m, lens, 0, since, weight, born, weight, born_out, 32, work, size, 2), None)
 
     e4m3 = memory(pt=_lib.SB_F8)
     for call in (attention, write, evict):
         for change in wrong:
-            assert call(m=None if change is None else memory(**change)) == _lib.SB_EINVAL, (call, change)
+            assert call(m=memory(**change)) == _lib.SB_EINVAL, (call, change)
         assert call(m=memory(b=0)) == _lib.SB_OK
     for bad in (dict(qt=1), dict(qt=2), dict(qt=3), dict(h=0), dict(m=memory(hkv=2), h=3), dict(tq=-1), dict(scale=0.0),
                 dict(scale=float("nan")), dict(ks=2.0), dict(m=e4m3, ks=0.0), dict(m=e4m3, scale=1e30, ks=1e30),
-                dict(weight=one, decay=2.0), dict(q=None), dict(q=C.c_void_p(8)), dict(row=60), dict(lens=None)):
+                dict(weight=16, decay=2.0), dict(q=0), dict(q=8), dict(row=60), dict(lens=0)):
         assert attention(**bad) == _lib.SB_EINVAL, bad
     assert attention(tq=0) == _lib.SB_OK
-    for bad in (dict(k=None), dict(dt=1), dict(dt=3), dict(ks=2.0), dict(m=e4m3, ks=-1.0), dict(at=None), dict(after=None), dict(t=-1),
+    for bad in (dict(k=0), dict(dt=1), dict(dt=3), dict(ks=2.0), dict(m=e4m3, ks=-1.0), dict(at=0), dict(after=0), dict(t=-1),
                 dict(kr=-1)):
         assert write(**bad) == _lib.SB_EINVAL, bad
-    for bad in (dict(lens=None), dict(weight=None), dict(since=one), dict(born=one), dict(born_out=one), dict(m=memory(page=4096), work=None),
-                dict(m=memory(page=4096), work=C.c_void_p(8))):
+    for bad in (dict(lens=0), dict(weight=0), dict(since=16), dict(born=16), dict(born_out=16), dict(m=memory(page=4096), work=0),
+                dict(m=memory(page=4096), work=8)):
         assert evict(**bad) == _lib.SB_EINVAL, bad
+    assert all(f(None, None) == _lib.SB_EINVAL for f in (lib.sb_paged_attention, lib.sb_paged_write, lib.sb_paged_evict))
     assert lib.sb_paged_attention_work(1, 2, 1, 48, 1, 0, 4, 2, 0, C.byref(n)) == _lib.SB_EINVAL
     assert lib.sb_paged_attention_work(1, 2, 1, 32, 1, 0, 0, 2, 0, C.byref(n)) == _lib.SB_EINVAL
     assert lib.sb_paged_attention_work(1, 2, 1, 32, 1, 1, 4, 2, 0, C.byref(n)) == _lib.SB_EINVAL
