@@ -11,7 +11,8 @@ namespace {
 // ---------------------------------------------------------------- write
 // Row (b, t), t < count[b], goes to position at[b] + t of item b.  Copies, bound by memory: a warp takes the
 // rows of a group (their pages are looked up once, by a lane a row) and keeps four vectors of K and four of V a lane
-// in flight.  e4m3 pages get the code of x / scale, a true division, or
+// in flight: 16 x 2040 ragged rows of 8 x 128 channels of K and of V in bf16 37 us, 224 MB, 93 % of the copy rate; 8 x
+// 8160 of 8 x 64 from fp16 to e4m3 35.5 us, 205 MB, 88 % (57 with divisions).  e4m3 pages get the code of x / scale, a true division, or
 // where both scales are powers of two the product with their reciprocals, which is the quotient.
 struct WriteArgs {
   const void *k, *v;
@@ -140,6 +141,10 @@ __global__ void __launch_bounds__(kWriteWarps * 32, MODE == 2 ? 2 : 4)
 // selection (11, 11 and 10 bits; each CTA counts its own states in shared memory and all add up the others'
 // counts) and pairs places with states; the second moves the rows.  The weights, as integers of the same
 // order, are kept in shared memory where they fit.
+//
+// What bounds it: the chain of passes, each with an exchange of counts.  16 x 8 units of 18,360 states, 2040 of them to
+// go, rows of 256 bytes: 26 us for the selection, 13.5 for the rows (82 MB, 93 % of the copy rate); 2 x 8 of 130,560, half
+// of them, rows of 64 bytes: 50 and 40 (150 MB in pieces of 64 bytes: 58 %).
 struct EvictArgs {
   Pool k, v;
   PageTable pages;

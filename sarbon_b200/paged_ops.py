@@ -38,6 +38,7 @@ from .memory_ops import _apart, _device, _new, _raw_stream, _ready, _rows, _stat
 
 E4M3 = torch.float8_e4m3fn
 _MOST = 3.4e38  # of fp32
+_INT, _FLOAT, _HALF, _BRAIN = torch.int32, torch.float32, torch.float16, torch.bfloat16
 # sb_paged_attend, sb_paged_append, sb_paged_cut, each from its sb_paged_memory on: a call's host time is what a small call
 # costs, and a struct packed at once costs less of it than as many arguments
 _MEMORY = "@PPqqqqPqiiiiiii4x"
@@ -89,14 +90,16 @@ def _memory(k_pages, v_pages, table, kv_heads, written=False):
         k_img, v_img = page * k_row, page * v_row
     k, v = k_pages.data_ptr(), v_pages.data_ptr()
     if written:
-        if _overlap(k_row, k_img, *shape) or _overlap(v_row, v_img, *shape):
+        if not (k_row >= width <= v_row and k_img >= k_row * page and v_img >= v_row * page) and \
+                (_overlap(k_row, k_img, *shape) or _overlap(v_row, v_img, *shape)):
             raise ValueError("pools: rows overlap")
         if k == v and pages:
             raise ValueError("results need their own memory")
-    at, step = table.shape, table.stride()
-    if len(at) != 2 or table.dtype != torch.int32 or (at[1] > 1 and step[1] != 1):
+    if table.dtype != _INT or table.dim() != 2:
         raise ValueError("table: int32 [B, N] with contiguous rows")
-    b, n = at
+    (b, n), step = table.shape, table.stride()
+    if step[1] != 1 and n > 1:
+        raise ValueError("table: int32 [B, N] with contiguous rows")
     if n * page >= 1 << 30:
         raise ValueError("table: fewer than 2^30 states an item")
     return (k, v, k_row, k_img, v_row, v_img, table.data_ptr(), step[0] if b > 1 else n, code, pages, page, n, b, kv_heads, dim), \
@@ -105,7 +108,7 @@ def _memory(k_pages, v_pages, table, kv_heads, written=False):
 
 def _each(t, what, b):
     """Pointer of an int32 [B]."""
-    if t.dtype != torch.int32 or t.shape != (b,) or (b > 1 and t.stride(0) != 1):
+    if t.dtype != _INT or t.shape != (b,) or not t.is_contiguous():
         raise ValueError(f"{what}: contiguous int32 [B]")
     return t.data_ptr()
 
@@ -122,8 +125,6 @@ def _one_device(floats, others):
     if forward_ad._current_level >= 0:
         return _ready(*floats, *others)
     index = floats[0].get_device()
-    if index < 0:
-        raise ValueError("tensors of one CUDA device")
     for t in others:
         if t is not None and t.get_device() != index:
             raise ValueError("tensors of one CUDA device")
@@ -174,7 +175,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, heads, kv_heads=None, scal
     Made for single tokens: the states are read once for every 16 query rows of a key head, and split
     over the SMs where there are few rows; many queries want cross_attention."""
     dtype, page_dtype = q.dtype, k_pages.dtype
-    if q.dim() != 3 or (dtype != torch.bfloat16 and dtype != torch.float16):
+    if q.dim() != 3 or (dtype != _BRAIN and dtype != _HALF):
         raise ValueError("q: [B, T, heads * dim] rows of fp16 or bf16")
     if kv_heads is None:
         kv_heads = heads
@@ -196,7 +197,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, heads, kv_heads=None, scal
     qp, p_lens = _rows(q, "q", shape, dtype), _each(lens, "lens", b)
     p_weight = p_lse = 0
     if weight is not None:
-        p_weight = _account(weight, "weight", (b, kv_heads, n * page), torch.float32)
+        p_weight = _account(weight, "weight", (b, kv_heads, n * page), _FLOAT)
     if lse is not None:
         _statistics(lse, b, heads, tq)
         p_lse = lse.data_ptr()
@@ -231,7 +232,7 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
     (allocated if None) shares no memory with at.  kv_heads is that of weight or born where they are given;
     without them the rows are taken as heads of 32 channels."""
     dtype, page_dtype, rows = k.dtype, k_pages.dtype, k.shape
-    if len(rows) != 3 or (dtype != torch.bfloat16 and dtype != torch.float16):
+    if len(rows) != 3 or (dtype != _BRAIN and dtype != _HALF):
         raise ValueError("k, v: [B, T, kv_heads * dim] rows of fp16 or bf16")
     if (born is None) != (stamp is None):
         raise ValueError("born and stamp: both or neither")
@@ -257,10 +258,10 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
     if count is not None:
         p_count = _each(count, "count", b)
     if weight is not None:
-        p_weight = _account(weight, "weight", (b, kv_heads, n * page), torch.float32)
+        p_weight = _account(weight, "weight", (b, kv_heads, n * page), _FLOAT)
     if born is not None:
-        p_born = _account(born, "born", (b, kv_heads, n * page), torch.int32)
-        if stamp.dtype != torch.int32 or stamp.shape not in ((b, t), (b,)):
+        p_born = _account(born, "born", (b, kv_heads, n * page), _INT)
+        if stamp.dtype != _INT or stamp.shape not in ((b, t), (b,)):
             raise ValueError("stamp: int32 [B, T] or [B]")
         step = stamp.stride()
         sp = stamp.data_ptr(), step[0], step[1] if len(step) == 2 else 0
@@ -300,10 +301,10 @@ def paged_evict(k_pages, v_pages, table, lens, weight, keep, born=None, since=No
     memory, b, page, n, dim = _memory(k_pages, v_pages, table, kv_heads, written=True)
     if places != (b, kv_heads, n * page) or lens is None:
         raise ValueError("weight: [B, kv_heads, N * page]; lens: contiguous int32 [B]")
-    pw, p_lens = _account(weight, "weight", places, torch.float32), _each(lens, "lens", b)
+    pw, p_lens = _account(weight, "weight", places, _FLOAT), _each(lens, "lens", b)
     pb = p_since = p_keep = 0
     if born is not None:
-        pb = _account(born, "born", places, torch.int32)
+        pb = _account(born, "born", places, _INT)
     elif since is not None or born_out is not None:
         raise ValueError("since and born_out need born")
     if since is not None:
@@ -319,10 +320,10 @@ def paged_evict(k_pages, v_pages, table, lens, weight, keep, born=None, since=No
     if weight_out is not None or born_out is not None or after is not None:
         own = []
         if weight_out is not None:
-            pwo = _account(weight_out, "weight_out", places, torch.float32)
+            pwo = _account(weight_out, "weight_out", places, _FLOAT)
             own.append(weight_out if pwo != pw else None)
         if born_out is not None:
-            pbo = _account(born_out, "born_out", places, torch.int32)
+            pbo = _account(born_out, "born_out", places, _INT)
             own.append(born_out if pbo != pb else None)
         if after is not None:
             p_after = _each(after, "after", b)
