@@ -100,8 +100,8 @@ def _memory(k_pages, v_pages, table, kv_heads, written=False):
     (b, n), step = table.shape, table.stride()
     if step[1] != 1 and n > 1:
         raise ValueError("table: int32 [B, N] with contiguous rows")
-    if n * page >= 1 << 30:
-        raise ValueError("table: fewer than 2^30 states an item")
+    if n * page >= 1 << 30 or pages >= 1 << 31:
+        raise ValueError("fewer than 2^30 states an item, 2^31 pages")
     return (k, v, k_row, k_img, v_row, v_img, table.data_ptr(), step[0] if b > 1 else n, code, pages, page, n, b, kv_heads, dim), \
         b, page, n, dim
 

@@ -328,6 +328,34 @@ def test_pools_beyond_32_bit_offsets():
     torch.cuda.empty_cache()
 
 
+def test_accounts_beyond_32_bit_offsets():
+    """Weights and stamps of more than 2^31 places in all: the last item's."""
+    import sarbon_b200 as sb
+    g = gen(6)
+    b, page, n = 5, 1 << 20, 512
+    k, v = (rand(g, 2, page, 32, dtype=torch.float16) for _ in range(2))
+    table = torch.full((b, n), -1, dtype=torch.int32, device="cuda")
+    table[:, 0] = torch.arange(b, device="cuda") % 2
+    q = rand(g, b, 1, 32, dtype=torch.float16)
+    lens = ints(3, 0, 7, 1, 900)
+    weight = torch.ones(b, 1, n * page, device="cuda")
+    out = sb.paged_attention(q, k, v, table, lens, 1, weight=weight, decay=0.5)
+    few = slice(0, 1000)
+    check_attention(out, None, weight[..., few].contiguous(), q, k[:, few], v[:, few], table[:, :1], lens, 1, 1,
+                    before=torch.ones(b, 1, 1000, device="cuda"), decay=0.5)
+    best = torch.sort(weight[4, 0, :900], descending=True, stable=True)
+    after, _, _ = sb.paged_evict(k, v, table, lens, weight, 100, weight_out=weight)
+    assert after.tolist() == [3, 0, 7, 1, 100]
+    assert same_bits(weight[4, 0, :100].sort(descending=True).values, best.values[:100]) and not weight[4, 0, 100:1000].any()
+    assert not weight[4, 0, -1000:].any() and not weight[1].any()
+    new = rand(g, b, 2, 32, dtype=torch.float16)
+    weight[4, 0, 100:102] = 5.0
+    assert sb.paged_write(new, new, k, v, table, after, weight=weight).tolist() == [5, 2, 9, 3, 102]
+    assert not weight[4, 0, 100:102].any() and same_bits(k[0, 100:102], new[4])
+    del weight
+    torch.cuda.empty_cache()
+
+
 # ---------------------------------------------------------------- new states
 def codes(x, scale):
     # (by a tensor: torch multiplies by the reciprocal of a number, which is not the quotient)

@@ -32,6 +32,7 @@ MEMORY = [
     dict(table=torch.zeros(6, **I32)), dict(table=torch.zeros(3, 2, **I32).t()), dict(table=torch.zeros(3, 3, **I32)),
     dict(k_pages=pools(width=96)[0], v_pages=pools(width=96)[1]), dict(k_pages=pools(page=0)[0], v_pages=pools(page=0)[1]),
     dict(table=torch.zeros(2, 1, **I32).expand(2, 1 << 28)),
+    dict(k_pages=torch.zeros(1, 4, 128, **H16).expand(1 << 31, 4, 128), v_pages=torch.ones(1, 4, 128, **H16).expand(1 << 31, 4, 128)),
     dict(),  # all well, but not on a GPU
 ]
 
