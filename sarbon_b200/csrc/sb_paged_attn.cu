@@ -71,6 +71,29 @@ constexpr long long kLeast = 16;  // chunks a CTA, four a warp
 template <int THREADS>
 SB_DEV Shares look_up(const PagedArgs& a, long long cta, int item, long long (&room)[THREADS / 32 + 2], int& found) {
   const int lane = lane_id(), warp = warp_id();
+  Shares s;
+  if (a.B <= 32) {  // each warp for itself: a lane an item, no barrier (fewer than 2^27 chunks an item)
+    const uint32_t n = lane < a.B ? (uint32_t)a.chunks(lane) : 0u;
+    s.total = (long long)__reduce_add_sync(0xFFFFFFFFu, n) * a.units();
+    s.each = max((s.total + a.shares - 1) / a.shares, kLeast);
+    if (item >= 0) {
+      s.item = item;
+      s.before = __reduce_add_sync(0xFFFFFFFFu, lane < item ? n : 0u);
+      return s;
+    }
+    uint32_t upto = n;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, upto, x);
+      if (lane >= x) upto += u;
+    }
+    const long long at = cta * s.each < s.total ? cta * s.each / a.units() : -1;
+    const uint32_t here = __ballot_sync(0xFFFFFFFFu, (long long)(upto - n) <= at && at < (long long)upto);
+    const int lane_of = here ? __ffs(here) - 1 : 0;
+    s.item = here ? lane_of : a.B;
+    s.before = __shfl_sync(0xFFFFFFFFu, upto - n, lane_of);
+    return s;
+  }
   long long sum = 0, before = 0;
   for (int b = threadIdx.x; b < a.B; b += THREADS) {
     const int n = a.chunks(b);
@@ -82,7 +105,6 @@ SB_DEV Shares look_up(const PagedArgs& a, long long cta, int item, long long (&r
     sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
     before += __shfl_xor_sync(0xFFFFFFFFu, before, x);
   }
-  Shares s;
   s.total = s.before = 0;
   __syncthreads();
   if (lane == 0) room[warp] = sum;
