@@ -37,7 +37,8 @@ struct PagedArgs {
   PageTable pages;
   const int* lens;
   int B, H, Hkv, group, Tq, rows, blocks;  // rows = group * Tq of an (item, key head), blocks of 16
-  int shares;                              // CTAs that share the chunks of all units; 0: a CTA a unit
+  int shares;                              // CTAs that share the chunks of all units; 0: CTAs of a unit's own
+  int cluster;                             // of them, then: 1 to 8
   int ends;                                // CTAs an (item, key head) of the last kernel; 0: none
   int chunk;                               // states
   int q_bf16, causal;
@@ -265,6 +266,56 @@ struct Cursor {
   }
 };
 
+constexpr int kHeldScores = 1536;  // floats: 6 KB, as many CTAs an SM as without
+
+// The rows of a unit from those of its cluster's CTAs, out = sum_s 2^(L_s - L) O_s, CTA by CTA every cluster-th of them, and
+// L of all into fin.  A group of lanes takes a row's eight channels, a lane a CTA.
+template <int DH>
+SB_DEV void join_cluster(const PagedArgs& a, int b, int kvh, int unit, int r0, int rows, const float* own, const float* own_l,
+                         float* fin) {
+  constexpr int per = DH / 8;
+  const int n = a.cluster, rank = (int)cluster_ctarank(), lane = lane_id(), s = lane % n;
+  auto sums_of = [&](int r, float& l, float& all) {  // L of this lane's CTA and of the cluster, for row r
+    l = __uint_as_float(peer_word(own_l + r, (uint32_t)s));
+    float top = l;
+    for (int x = 1; x < n; x <<= 1) {
+      const float u = __shfl_xor_sync(0xFFFFFFFFu, top, x);
+      top = max3(top, u, u);
+    }
+    float sum = l == top ? 1.f : exp2_hw(l - top);
+    for (int x = 1; x < n; x <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+    all = top == -INFINITY ? -INFINITY : top + log2f(sum);
+  };
+  for (int r = threadIdx.x / n; r < 16; r += kWarps * 32 / n) {  // (16 rows: whole warps)
+    float l, all;
+    sums_of(min(r, rows - 1), l, all);
+    if (s == 0 && r < rows) {
+      fin[r] = all;
+      if (rank == 0 && a.ends > 0) a.part_l[((long long)b * a.units() + unit) * a.part_rows + r] = all;
+    }
+  }
+  const int mine = rows > rank ? (rows - rank + n - 1) / n : 0, work = mine * per;
+  for (int e0 = 0; e0 < work; e0 += kWarps * 32 / n) {
+    const int e = e0 + (int)threadIdx.x / n, at = min(e, work - 1), r = rank + at / per * n, c = at % per * 8;
+    float l, all;
+    sums_of(r, l, all);
+    const uint4 x = peer_words(own + r * DH + c, (uint32_t)s), y = peer_words(own + r * DH + c + 4, (uint32_t)s);
+    const uint32_t v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    const float k = l == -INFINITY ? 0.f : exp2_hw(l - all);
+    float f[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      f[u] = k * __uint_as_float(v[u]);
+      for (int z = 1; z < n; z <<= 1) f[u] += __shfl_xor_sync(0xFFFFFFFFu, f[u], z);
+    }
+    if (s == 0 && e < work) {
+      const Row w(a, kvh, r0 + r);
+      store8(a.o.p, a.q_bf16 ? SB_BF16 : SB_F16, b * a.o.img + w.t * a.o.row + (long long)w.h * DH + c, f);
+      if (c == 0 && a.lse) a.lse[((long long)b * a.H + w.h) * a.Tq + w.t] = all * 0.69314718055994531f;
+    }
+  }
+}
+
 // NB: column tiles of eight query rows
 template <int DH, int PT, int NB>
 __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
@@ -277,7 +328,7 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
   __shared__ ulonglong2 place[kWarps][CK];      // addresses of a chunk's rows of K and V
   __shared__ uint64_t there[kWarps][C::STAGES];  // a stage's rows that take part, as bits
   __shared__ float2 ml[kWarps][16];
-  __shared__ float fin[16];
+  __shared__ float fin[16], found_l[16];
   __shared__ long long room[kWarps + 2];
   __shared__ int area[kWarps], found;
   const int warp = warp_id(), lane = lane_id();
@@ -296,11 +347,13 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
     at.c = (int)(in - (long long)at.unit * at.n);
     left = min(s.each, s.total - blockIdx.x * s.each);
   } else {
-    at.b = blockIdx.x / a.units();
-    at.unit = blockIdx.x - at.b * a.units();
-    at.c = 0;
+    const int unit = blockIdx.x / a.cluster, rank = blockIdx.x - unit * a.cluster;  // (a cluster's CTAs lie side by side)
+    at.b = unit / a.units();
+    at.unit = unit - at.b * a.units();
     at.item(a);
-    left = at.n;
+    const int each = (at.n + a.cluster - 1) / a.cluster;
+    at.c = min(rank * each, at.n);
+    left = min(each, at.n - at.c);
   }
   const int mine = left > warp ? (int)((left - warp + kWarps - 1) / kWarps) : 0;  // chunks warp, warp + kWarps, ... of them
   uint8_t* const ring = smem + warp * C::kRing;
@@ -361,6 +414,10 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
     ask();
     __syncwarp();  // place is written again
   }
+
+  // behind the rings: this CTA's states' scores, where they are held, and its rows of a cluster
+  float* const held = reinterpret_cast<float*>(smem + C::SMEM);
+  float* const rows_of_cluster = held + kHeldScores;
 
   int i = 0;  // the warp's chunk
   long long done = 0;
@@ -426,7 +483,7 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
       for (int x = 0; x < KS; ++x) o[x][y][0] = o[x][y][1] = o[x][y][2] = o[x][y][3] = 0.f;
     }
     float* const scores = a.scores   ? a.plane(b * a.Hkv + kvh, block)
-                          : a.weight ? reinterpret_cast<float*>(smem + C::SMEM) : nullptr;
+                          : a.weight ? held - (long long)at.c * CK * a.score_rows : nullptr;
     const int chunk0 = at.c - (int)done;  // of the unit: chunk0 + warp + i * kWarps
 
     const int i_first = i;
@@ -710,6 +767,11 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
       for (int u = 0; u < 8; ++u) f[u] = none ? 0.f : f[u] * inv;
       const float log_sum = none ? -INFINITY : top - lift + log2f(sum);
       const Row w(a, kvh, r0 + r);
+      if (a.cluster > 1) {
+        store8(rows_of_cluster, SB_F32, r * DH + c, f);
+        if (c == 0) found_l[r] = log_sum;
+        continue;
+      }
       if (a.shares && !whole) {
         const long long place = 2ll * blockIdx.x + (at.c == 0);
         store8(a.part_o, SB_F32, (place * a.part_rows + r) * DH + c, f);
@@ -722,10 +784,16 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
         fin[r] = log_sum;
       }
     }
+    if (a.cluster > 1) {  // (one piece a CTA)
+      __syncwarp();
+      cluster_sync();
+      join_cluster<DH>(a, b, kvh, at.unit, r0, rows, rows_of_cluster, found_l, fin);
+    }
     __syncthreads();
-    if (a.weight && a.ends == 0) {  // all of the scores and sums are this CTA's own
+    if (a.weight && a.ends == 0) {  // the scores are this CTA's own, and all of the sums are here
       float* weight = a.weight + ((long long)b * a.Hkv + kvh) * a.pages.cap;
-      for (int j = threadIdx.x; j < count; j += kWarps * 32) {
+      const int j_end = min(count, (at.c + piece) * CK);
+      for (int j = at.c * CK + (int)threadIdx.x; j < j_end; j += kWarps * 32) {
         float w = 0.f;
         for (int r = 0; r < rows; ++r)
           if (fin[r] != -INFINITY) w += exp2_hw(scores[(long long)j * a.score_rows + r] - fin[r]);
@@ -741,6 +809,8 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
     if (done < left) at.advance(a, piece);
   } while (done < left);
   copies_wait<0>();
+  __syncwarp();
+  if (a.cluster > 1) cluster_sync();  // no CTA ends while another reads its rows
 }
 
 // What is left after the last piece, a CTA a part of an (item, key head): its share of the rows is joined from the
@@ -896,21 +966,20 @@ void shape_of(int pt, int rows, int& chunk, int& occ) {
          : pt == SB_BF16 ? shape_of<DH, SB_BF16>(rows, chunk, occ) : shape_of<DH, SB_F16>(rows, chunk, occ);
 }
 
-constexpr int kHeldScores = 1536;  // 6 KB: as many CTAs an SM as without
-
 struct PagedPlan {
-  int rows, blocks, shares, ends, chunk, part_rows, places, score_rows;
+  int rows, blocks, shares, cluster, ends, chunk, part_rows, places, score_rows;
   bool held;  // scores in shared memory
   long long units, scores, part_o, part_l;  // floats of the workspace
   long long bytes() const { return (scores + part_o + part_l) * 4; }
 };
 
-// Either a CTA a unit, and one kernel; or as many CTAs as are resident at once share all chunks evenly, whatever the
-// items' lengths, and a second kernel joins the pieces.  What they take is estimated from the places (lengths are
-// on the device): a CTA a unit about 3 us to start and end and its share of the rate of all resident ones, in waves;
-// shared chunks about 18 us for both kernels and the rate of all.  Measured, us in kernels, apart and shared: 2 x 8
-// units of 1000, 2000, 4000 states of 32 channels 12 and 20, 21 and 18, 40 and 18; 1 x 4 of 512, 1024 of 128 14 and
-// 15, 25 and 14; 64 x 4 of 1024, 2048, 8160 of 128 30 and 38, 54 and 54, 203 and 171; 640 x 4 of 1000 of 64 142 and 127.
+// Either a CTA or a cluster of up to eight a unit, and one kernel; or as many CTAs as are resident at once share all chunks
+// evenly, whatever the items' lengths, and a second kernel joins the pieces.  What they take is estimated from
+// the places (lengths are on the device): a CTA of a unit about 3 us to start and end (5 in a cluster) and 6 ns and 35 ps a
+// byte for a state; shared chunks 14 us for both kernels and the rate of all.  Measured, us in kernels, for a CTA a unit, the
+// cluster taken, and shared chunks: 2 x 8 units of 1000, 2000, 4000, 8000 states of 32 channels 12, 8, 20; 21, 9, 18;
+// 40, 12, 18; 83, 16, 19; 1 x 4 of 512, 1024, 2048, 4096 of 128 14, 8, 15; 25, 10, 14; 47, 12, 14; -, 18, 14; 64 x 4 of
+// 1024, 2048, 8160 30, -, 38; 54, -, 54; 203, -, 171; 640 x 4 of 1000 of 64 142, -, 127.
 PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int pt, int cap, bool account, int sms) {
   PagedPlan p{};
   int occ;
@@ -921,10 +990,21 @@ PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int pt, int cap, boo
   p.blocks = (p.rows + 15) / 16;
   p.part_rows = std::min(p.rows, 16);
   p.units = (long long)B * Hkv * p.blocks;
-  const long long resident = (long long)occ * sms, waves = (p.units + resident - 1) / resident;
+  const long long resident = (long long)occ * sms;
   const double unit_us = 2.0 * cap * dh * page_dtype_bytes(pt) / 6.2e6;  // at the rate of all
-  const bool apart = waves * (3.0 + resident * unit_us) > 18.0 + p.units * unit_us;
+  const double state_us = 0.006 + 35e-6 * 2.0 * dh * page_dtype_bytes(pt);
+  double best = 1e300;
+  for (int c = 1; c <= 8; c *= 2) {
+    if (c > 1 && cap < c * kWarps * p.chunk) break;  // a chunk a warp
+    const double us = (double)((p.units * c + resident - 1) / resident) * ((c > 1 ? 5.0 : 3.0) + cap * state_us / c);
+    if (us < best) {
+      best = us;
+      p.cluster = c;
+    }
+  }
+  const bool apart = best > 14.0 + p.units * unit_us;
   p.shares = apart ? (int)resident : 0;
+  if (apart) p.cluster = 1;
   account = account && cap > 0;
   // one wave of the last kernel's CTAs, each with 256 places or a row
   const long long heads = (long long)B * Hkv, wave = std::max(1ll, (long long)kEndOcc * sms / std::max(heads, 1ll));
@@ -933,7 +1013,8 @@ PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int pt, int cap, boo
   auto even = [](long long n) { return (n + 3) / 4 * 4; };
   p.places = (cap + 3) / 4 * 4;
   for (p.score_rows = 1; p.score_rows < p.part_rows;) p.score_rows *= 2;
-  p.held = account && p.ends == 0 && p.places * p.score_rows <= kHeldScores;
+  const int chunks = (cap + p.chunk - 1) / p.chunk, most = (chunks + p.cluster - 1) / p.cluster * p.chunk;  // of a CTA
+  p.held = account && p.ends == 0 && (p.cluster > 1 ? most : p.places) * p.score_rows <= kHeldScores;
   p.scores = account && !p.held ? (long long)B * Hkv * p.blocks * p.places * p.score_rows : 0;
   p.part_l = p.ends > 0 ? even((p.units + p.shares) * p.part_rows) : 0;
   p.part_o = 2ll * p.shares * p.part_rows * dh;
@@ -943,11 +1024,12 @@ PagedPlan paged_plan(int B, int H, int Hkv, int dh, int Tq, int pt, int cap, boo
 template <int DH, int PT, int NB>
 cudaError_t launch(const PagedArgs& a, long long ctas, cudaStream_t st) {
   static bool ready[64];
-  constexpr int room = Paged<DH, PT, NB>::SMEM, most = room + kHeldScores * 4;
-  const cudaError_t e = xattn_smem(reinterpret_cast<const void*>(&paged_attend_kernel<DH, PT, NB>), most, ready);
+  constexpr int room = Paged<DH, PT, NB>::SMEM, scores = kHeldScores * 4, rows = 8 * NB * DH * 4;
+  auto* const kernel = paged_attend_kernel<DH, PT, NB>;
+  const cudaError_t e = xattn_smem(reinterpret_cast<const void*>(kernel), room + scores + rows, ready);
   if (e != cudaSuccess) return e;
-  paged_attend_kernel<DH, PT, NB><<<(unsigned)ctas, kWarps * 32, a.weight && !a.scores ? most : room, st>>>(a);
-  return cudaGetLastError();
+  const int bytes = room + (a.cluster > 1 ? scores + rows : a.weight && !a.scores ? scores : 0);
+  return launch_after(kernel, ctas, kWarps * 32, (size_t)bytes, st, a, a.cluster, false);
 }
 template <int DH, int PT>
 cudaError_t launch(const PagedArgs& a, long long ctas, cudaStream_t st) {
@@ -1003,14 +1085,14 @@ extern "C" int sb_paged_attention(const sb_paged_attend* call, void* stream) {
   const PagedPlan p = paged_plan(m->B, H, m->Hkv, m->dh, Tq, m->dtype, a.pages.cap, c.weight != nullptr, sms);
   if (p.bytes() > 0 && (!c.work || c.work_bytes < p.bytes() || (reinterpret_cast<uintptr_t>(c.work) & 15) != 0))
     return record_error(SB_EINVAL, "sb_paged_attention: workspace (sb_paged_attention_work bytes, 16-byte aligned)");
-  const long long ctas = p.shares ? p.shares : p.units, ends = (long long)p.ends * m->B * m->Hkv;
+  const long long ctas = p.shares ? p.shares : p.units * p.cluster, ends = (long long)p.ends * m->B * m->Hkv;
   if (ctas > 0x7FFFFFFFll || ends > 0x7FFFFFFFll) return record_error(SB_EINVAL, "sb_paged_attention: too many items");
   a.q = c.q; a.q_row = c.q_row; a.q_img = c.q_img;
   a.k = k_pool(m);
   a.v = v_pool(m);
   a.lens = c.lens;
   a.B = m->B; a.H = H; a.Hkv = m->Hkv; a.group = H / m->Hkv; a.Tq = Tq;
-  a.rows = p.rows; a.blocks = p.blocks; a.shares = p.shares; a.ends = p.ends; a.chunk = p.chunk; a.part_rows = p.part_rows;
+  a.rows = p.rows; a.blocks = p.blocks; a.shares = p.shares; a.cluster = p.cluster; a.ends = p.ends; a.chunk = p.chunk; a.part_rows = p.part_rows;
   a.places = p.places; a.score_rows = p.score_rows;
   a.q_bf16 = c.q_dtype == SB_BF16; a.causal = c.causal != 0;
   a.scale_log2 = c.scale * c.k_scale * 1.4426950408889634f;

@@ -183,6 +183,7 @@ struct Told {
   int room[2][kSelectWarps], found[3];
 };
 SB_DEV void all_sync(int ctas) {
+  __syncwarp();
   if (ctas > 1) cluster_sync();
   else __syncthreads();
 }
@@ -225,7 +226,7 @@ SB_DEV void before_and_all(int (&v)[2], int (&total)[2], int (&base)[2], Told& t
       told.counts[c][0] = total[0];
       told.counts[c][1] = total[1];
     }
-    cluster_sync();
+    all_sync(ctas);
     const uint32_t lane = lane_id();
     int t[2] = {0, 0};  // (a lane a CTA: one trip to the others)
     if (lane < (uint32_t)ctas) {
@@ -311,7 +312,7 @@ SB_DEV void finish(const EvictArgs& a, long long unit, int moves, int len, int l
     if (a.born && j >= b_from) a.born_out[at + j] = 0;
   }
   if (a.parts && threadIdx.x == 0 && rank == 0) a.moves[unit] = moves;
-  if (ctas > 1) cluster_sync();  // no CTA ends while another reads what it told
+  if (ctas > 1) all_sync(ctas);  // no CTA ends while another reads what it told
 }
 // A state that goes from its place, which nothing fills.
 SB_DEV void clear_own(const EvictArgs& a, long long at) {
