@@ -13,14 +13,16 @@
 // product more, and the tensor pipe has room for it.
 //
 // As many CTAs as are resident share the chunks of all (item, key head)s evenly, whatever their lengths, and a second
-// kernel joins the fp32 partial rows; small calls take a CTA an (item, key head) and no second kernel.  The account
-// needs L, which is there only after the last piece, so the scores are kept (fp32) and the second kernel reads them
-// back: 8 bytes a state and row beside 4 dim bytes of K and V, most of them from the L2.
+// kernel joins the fp32 partial rows; smaller calls take a CTA or a cluster of them an (item, key head), joined through
+// the cluster's shared memory, and no second kernel.  The account needs L, which is there only after the last piece, so
+// the scores are kept (fp32) and the second kernel, or the CTA itself, reads them back: 8 bytes a state and row
+// beside 4 dim bytes of K and V, most of them from the L2.
 //
-// 64 x 1 token on 8160 ragged states of 4 key heads of 128, 16 query heads, with the account: bf16 164 us (961 MB with the
-// scores: 5.9 TB/s, 90 % of the copy rate), e4m3 100 (issuing instructions; 76 % with two kernels' ends).  One stream of
-// 130,560 states 56 (267 MB, 73 %: 7 of them the second kernel).  16 x 8 causal tokens on 42,840 of 4 heads of 64: 175; the
-// scores of 16 rows a state, written and read, are 350 MB beside 601 of K and V.
+// 64 x 1 token on 8160 ragged states of 4 key heads of 128, 16 query heads, with the account: bf16 165 to 172 us (157 for
+// 961 MB with the scores, 6.1 TB/s, 94 % of the copy rate; 11 the second kernel), e4m3 97 to 100 (84 for 495 MB, 90 %, and
+// 41 % of the issue slots).  One stream of 130,560 states 56 (47 for 267 MB: start and end; 7 the second kernel).  16 x 8
+// causal tokens on 42,840 of 4 heads of 64: 173 to 180; the scores of 16 rows a state, written and read, are 350 MB
+// beside 601 of K and V.
 #include <algorithm>
 #include <cmath>
 
@@ -30,6 +32,7 @@ namespace sb {
 namespace {
 
 constexpr int kWarps = 4;
+
 struct PagedArgs {
   const void* q;
   long long q_row, q_img;  // elements
@@ -162,7 +165,8 @@ template <int DH, int PT, int NB>
 struct Paged {
   static constexpr bool E4M3 = PT == SB_F8, BF16 = PT == SB_BF16;
   static constexpr int RB = DH * (E4M3 ? 1 : 2);                // bytes a state and head
-  // Two CTAs an SM, 24 KB a warp on their way.  e4m3 is bound by issuing instructions more than by memory: three CTAs.
+  // Two CTAs an SM, 24 KB a warp on their way.  e4m3 waits for instructions more than for memory: three CTAs (83 us
+  // for the 64 x 8160 states above, 92 with two).
   static constexpr int OCC = E4M3 && NB == 1 ? 3 : 2;
   static constexpr int kRing = OCC == 3 ? 16 * 1024 : 24 * 1024;  // bytes a warp
   static constexpr int CK = 4096 / RB < 64 ? 4096 / RB : 64;      // states a chunk
@@ -196,31 +200,6 @@ SB_DEV void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory");
 template <int N>
 SB_DEV void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <bool BF16>
-SB_DEV void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-SB_DEV void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-SB_DEV void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
 // An 8 x 8 matrix of 16-bit values, a pair of a row a thread, turned around.
 SB_DEV uint32_t transposed(uint32_t a) {
   uint32_t d;
@@ -1031,6 +1010,8 @@ cudaError_t launch(const PagedArgs& a, long long ctas, cudaStream_t st) {
   const int bytes = room + (a.cluster > 1 ? scores + rows : a.weight && !a.scores ? scores : 0);
   return launch_after(kernel, ctas, kWarps * 32, (size_t)bytes, st, a, a.cluster, false);
 }
+// One column tile for up to eight rows: e4m3 above 83 us and with two tiles 116, fp16 heads of 32 158 and 162, bf16 heads of
+// 128, which wait for memory alone, 156 and 152.
 template <int DH, int PT>
 cudaError_t launch(const PagedArgs& a, long long ctas, cudaStream_t st) {
   return a.rows <= 8 ? launch<DH, PT, 1>(a, ctas, st) : launch<DH, PT, 2>(a, ctas, st);
