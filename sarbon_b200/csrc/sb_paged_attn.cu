@@ -24,6 +24,7 @@
 // causal tokens on 42,840 of 4 heads of 64: 173 to 180; the scores of 16 rows a state, written and read, are 350 MB
 // beside 601 of K and V.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "sb_paged.cuh"
@@ -434,7 +435,7 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
         top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
         top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
         const int e = (int)(top >> 7);  // the largest's exponent, biased by 127
-        up = e == 0 || e == 255 ? 0 : min(max(140 - e, -126), 126);
+        up = e == 255 ? 0 : min(max(140 - e, -126), 126);
         const float by = __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
@@ -447,7 +448,8 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int down = __shfl_sync(0xFFFFFFFFu, up, (2 * tig + x) * 4), r = r0 + 8 * y + 2 * tig + x;
-        factor[y][x] = a.scale_log2 * __uint_as_float((uint32_t)(127 - down) << 23);
+        // (neither 0 nor infinite: -inf, which states that take no part score, has to stay so, and 0 too)
+        factor[y][x] = fminf(fmaxf(a.scale_log2 * __uint_as_float((uint32_t)(127 - down) << 23), FLT_MIN), FLT_MAX);
         limit[y][x] = a.causal && r < a.rows ? max(count - a.Tq + 1 + r / a.group, 0) : count;
       }
     }
@@ -1053,7 +1055,7 @@ extern "C" int sb_paged_attention(const sb_paged_attend* call, void* stream) {
   if (!paged_memory_ok(m) || !paged_attention_sizes_ok(m->B, H, m->Hkv, m->dh, Tq, m->P, m->page, m->N) ||
       (c.q_dtype != SB_F16 && c.q_dtype != SB_BF16) || (m->dtype != c.q_dtype && m->dtype != SB_F8))
     return record_error(SB_EINVAL, "sb_paged_attention: sizes (dh 32, 64 or 128, H a multiple of Hkv) or dtypes");
-  if (!(c.scale > 0.f) || !scales_ok(m, c.k_scale, c.v_scale) || !std::isnormal(c.scale * c.k_scale))
+  if (!(c.scale > 0.f) || !scales_ok(m, c.k_scale, c.v_scale) || !std::isnormal(c.scale * c.k_scale * 1.4426950408889634f))
     return record_error(SB_EINVAL, "sb_paged_attention: scale, or scales of pages that are not e4m3");
   if (c.weight && !(c.decay >= 0.f && c.decay <= 1.f)) return record_error(SB_EINVAL, "sb_paged_attention: decay from 0 to 1");
   if (m->B == 0 || Tq == 0) return SB_OK;

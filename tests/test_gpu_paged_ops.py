@@ -233,6 +233,24 @@ def test_attention_bf16_queries_of_any_size_on_e4m3():
         check_attention(out, lse, None, q[at], k, v, table[at], lens[at], 2, 1, scale=scale)
 
 
+@pytest.mark.parametrize("size,scale", [(2.0 ** -126, 2.0 ** -40), (2.0 ** -120, 0.1), (2.0 ** -131, 2.0 ** 126), (2.0 ** 126, 2.0 ** -126), (1.0, 2.0 ** -120)])
+@pytest.mark.parametrize("qt", [torch.float16, torch.bfloat16])
+def test_attention_sizes_near_the_types_ends(qt, size, scale):
+    """Queries and scales of any size leave states that take no part without weight, and scores of next to nothing
+    share evenly."""
+    import sarbon_b200 as sb
+    g, b, n, heads, kv_heads = gen(21), 2, 100, 4, 2
+    k, v, table = pages_of(g, b, n, 16, kv_heads * 64, E4M3)
+    lens = ints(37, n)
+    q = (rand(g, b, 2, heads * 64) * size).clamp(-torch.finfo(qt).max, torch.finfo(qt).max).to(qt)
+    if qt == torch.float16 and size > 1:
+        scale = 2.0 ** -16
+    weight, lse = torch.zeros(b, kv_heads, table.shape[1] * 16, device="cuda"), torch.empty(b, heads, 2, device="cuda")
+    out = sb.paged_attention(q, k, v, table, lens, heads, kv_heads, scale=scale, causal=True, weight=weight, lse=lse)
+    check_attention(out, lse, weight, q, k, v, table, lens, heads, kv_heads, scale=scale, causal=True,
+                    before=torch.zeros_like(weight))
+
+
 def test_attention_strides_and_shared_pages():
     """Keys and values side by side, pages inside wider rows, queries of a projection, a table that is part of a larger one,
     pages that several items and several places of one item share, pages in no order in memory."""

@@ -128,7 +128,7 @@ def test_library_refuses():
             assert call(m=memory(**change)) == _lib.SB_EINVAL, (call, change)
         assert call(m=memory(b=0)) == _lib.SB_OK
     for bad in (dict(qt=1), dict(qt=2), dict(qt=3), dict(h=0), dict(m=memory(hkv=2), h=3), dict(tq=-1), dict(scale=0.0),
-                dict(scale=float("nan")), dict(ks=2.0), dict(m=e4m3, ks=0.0), dict(m=e4m3, scale=1e30, ks=1e30),
+                dict(scale=float("nan")), dict(ks=2.0), dict(m=e4m3, ks=0.0), dict(m=e4m3, scale=1e30, ks=1e30), dict(scale=3e38),
                 dict(weight=16, decay=2.0), dict(q=0), dict(q=8), dict(row=60), dict(lens=0)):
         assert attention(**bad) == _lib.SB_EINVAL, bad
     assert attention(tq=0) == _lib.SB_OK
