@@ -1,4 +1,5 @@
-"""Build ``libsarbon_sparse.so`` (the C ABI in ``include/sarbon_sparse.h``) for sm_100a.
+"""Build ``libsarbon_sparse.so`` (the C ABI in ``include/sarbon_sparse.h``) for sm_100a, and ``_paged_calls.so``, the
+Python module through which the paged memory's calls reach it.
 
 The library is built in-tree next to this file so that it travels with the source
 tree; object files go to ``sarbon_b200/_build``.  Usage::
@@ -18,6 +19,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libsarbon_sparse.so"
+CALLS_SOURCE, CALLS_LIB = CSRC / "sb_paged_calls.cpp", PKG / "_paged_calls.so"
 SOURCES = ["sb_engine.cu", "sb_gate.cu", "sb_conv_tc.cu", "sb_conv_simt.cu", "sb_noalloc.cu", "sb_cells.cu", "sb_boxes.cu",
            "sb_prep.cu", "sb_deform.cu", "sb_gemm.cu", "sb_detops.cu", "sb_attn.cu", "sb_xattn.cu", "sb_xattn_few.cu", "sb_xattn_bwd.cu",
            "sb_rope.cu", "sb_gnorm.cu", "sb_paged_attn.cu", "sb_paged_cache.cu"]
@@ -44,8 +46,38 @@ def _compile(src: str, extra) -> Path:
     return out
 
 
+def _run(what, cmd):
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{what} failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+
+
+def build_calls(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the Python module against the installed torch."""
+    import sysconfig
+
+    import torch
+    header = PKG.parent / "include" / "sarbon_sparse.h"
+    root = Path(torch.__file__).resolve().parent
+    newest = max(p.stat().st_mtime for p in (CALLS_SOURCE, header, root / "version.py"))
+    if CALLS_LIB.exists() and not force and CALLS_LIB.stat().st_mtime > newest:
+        return CALLS_LIB
+    cuda = Path(nvcc()).resolve().parents[1]
+    found = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"],
+             cuda / "include"]
+    tmp = CALLS_LIB.with_suffix(".so.tmp")
+    _run("g++", ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{header.parent}",
+                 *(x for p in found for x in ("-isystem", str(p))), str(CALLS_SOURCE), "-o", str(tmp), f"-L{root / 'lib'}", "-lc10",
+                 "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"])
+    os.replace(tmp, CALLS_LIB)
+    if verbose:
+        print(f"built {CALLS_LIB}")
+    return CALLS_LIB
+
+
 def build(force: bool = False, extra=(), verbose: bool = False) -> Path:
-    """Compile every CUDA source for sm_100a and link the shared library."""
+    """Compile every CUDA source for sm_100a and link the shared library; then the Python module."""
+    build_calls(force, verbose)
     srcs = [CSRC / s for s in SOURCES] + list(CSRC.glob("*.cuh")) + [PKG.parent / "include" / "sarbon_sparse.h"]
     if LIB.exists() and not force:
         newest = max(p.stat().st_mtime for p in srcs)

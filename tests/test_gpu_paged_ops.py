@@ -653,3 +653,50 @@ def test_captured_steps_and_streams():
     torch.cuda.synchronize()
     for a, b in zip(plain, held):
         assert all(same_bits(a[x], b[x]) for x in ("k", "v", "weight", "born", "lens", "out"))
+
+
+def test_calls_from_either_side(monkeypatch):
+    """The native side of a call and the Python side do the same; what the native side leaves alone is done all the same, and a
+    status of the library's is an error on both."""
+    import sarbon_b200 as sb
+    from sarbon_b200 import paged_ops
+    sides = [paged_ops._load()]
+
+    class Nothing:
+        attend = append = cut = staticmethod(lambda *a: None)
+
+    sides.append(Nothing)
+    for pt in (torch.float16, E4M3):
+        got = []
+        for side in sides:
+            monkeypatch.setattr(paged_ops, "_native", side)
+            s, f = stream(41, pt), ints(0, 0, 0)
+            was = paged_ops.CALLS[0]
+            for _ in range(3):
+                step(sb, s, f)
+                f.add_(1)
+            assert paged_ops.CALLS[0] == was + 9
+            n = sb.paged_write(s["new_k"], s["new_v"], s["k"], s["v"], s["table"], s["lens"], k_scale=s["scale"], v_scale=s["scale"])
+            out = sb.paged_attention(torch.nn.Parameter(s["q"], requires_grad=False), s["k"], s["v"], s["table"], n, 4, 2)
+            got.append([s[x] for x in ("k", "v", "out", "lens", "n", "weight", "born")] + [n, out] +
+                       list(sb.paged_evict(s["k"], s["v"], s["table"], n, s["weight"], ints(100, 0, 150), born=s["born"], since=f)))
+            assert sb.paged_evict(s["k"], s["v"], s["table"], n, s["weight"], 9)[2] is None
+            with pytest.raises(ValueError):
+                sb.paged_attention(s["q"], s["k"], s["v"], s["table"], n, 4, kv_heads=3)
+            with pytest.raises(ValueError):
+                sb.paged_attention(s["q"].clone().requires_grad_(), s["k"], s["v"], s["table"], n, 4, kv_heads=2)
+            with pytest.raises(ValueError):
+                sb.paged_attention(s["q"], s["k"], s["v"], s["table"], n.cpu(), 4, kv_heads=2)
+            off = torch.empty(s["q"].numel() + 1, dtype=torch.float16, device="cuda")[1:].view(s["q"].shape)
+            with pytest.raises(RuntimeError, match="aligned"):
+                sb.paged_attention(off, s["k"], s["v"], s["table"], n, 4, kv_heads=2)
+        assert all(same_bits(x, y) for x, y in zip(*got))
+
+    class Own(torch.Tensor):
+        pass
+
+    monkeypatch.setattr(paged_ops, "_native", sides[0])
+    s = stream(42)
+    whole = sb.paged_attention(s["q"], s["k"], s["v"], s["table"], s["lens"], 4, 2)
+    assert same_bits(whole, sb.paged_attention(s["q"].as_subclass(Own), s["k"], s["v"], s["table"], s["lens"], 4, 2))
+    assert sb.paged_attention(s["q"][:0], s["k"], s["v"], s["table"][:0], s["lens"][:0], 4, 2).shape == (0, 2, 256)
