@@ -179,6 +179,7 @@ SB_DEV uint32_t as_prefix(int bin, int pass) { return (uint32_t)bin << (pass == 
 // What the CTAs of an (item, key head) tell each other; bins and counts are never written twice.
 struct Told {
   int bins[4][kBins];  // the first pass's of the protected and of the others, the second's, the third's
+  int groups[4][kBins / 32];  // their sums by 32
   int counts[3][2];
   int room[2][kSelectWarps], found[3];
 };
@@ -206,15 +207,10 @@ SB_DEV void before_and_all(int (&v)[2], int (&total)[2], Told& told) {
   }
   __syncthreads();
 #pragma unroll
-  for (int y = 0; y < 2; ++y) {
-    int before = s[y] - v[y], all = 0;
-    for (int w = 0; w < kSelectWarps; ++w) {
-      const int t = told.room[y][w];
-      if (w < warp) before += t;
-      all += t;
-    }
-    v[y] = before;
-    total[y] = all;
+  for (int y = 0; y < 2; ++y) {  // (a lane a warp)
+    const int t = lane < kSelectWarps ? told.room[y][lane] : 0;
+    v[y] = s[y] - v[y] + __reduce_add_sync(0xFFFFFFFFu, lane < warp ? t : 0);
+    total[y] = __reduce_add_sync(0xFFFFFFFFu, t);
   }
 }
 // The same over all CTAs; the c-th such sum.  base: what the CTAs before this one have.
@@ -242,52 +238,106 @@ SB_DEV void before_and_all(int (&v)[2], int (&total)[2], int (&base)[2], Told& t
   }
 }
 
-// The bin of all CTAs' bins, which they have told, that holds the need-th number from the top; need becomes its place in
-// the bin, same how many the bin holds.
-SB_DEV int find_bin(Told& told, const int* bins, int& need, int& same, int ctas) {
-  constexpr int each = kBins / kSelect;  // bins a thread
-  static_assert(each == 4, "16 bytes");
-  const int lane = lane_id(), warp = warp_id(), first = kBins - each * (1 + (int)threadIdx.x);
-  int c[each], sum = 0;
-#pragma unroll
-  for (int x = 0; x < each; ++x) c[x] = 0;
-  for (int r0 = 0; r0 < ctas; r0 += 4) {  // four asked for before one is looked at
-    uint4 u[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      u[r] = make_uint4(0, 0, 0, 0);
-      if (r0 + r < ctas)
-        u[r] = ctas > 1 ? peer_words(bins + first, (uint32_t)(r0 + r)) : *reinterpret_cast<const uint4*>(bins + first);
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      c[0] += (int)u[r].w;
-      c[1] += (int)u[r].z;
-      c[2] += (int)u[r].y;
-      c[3] += (int)u[r].x;
-    }
+// Inclusive sums over lanes of `width`, in order.
+SB_DEV int scan_of(int v, int width) {
+  for (int x = 1; x < width; x <<= 1) {
+    const int u = __shfl_up_sync(0xFFFFFFFFu, v, x, width);
+    if ((lane_id() & (width - 1)) >= x) v += u;
   }
+  return v;
+}
+// Where among four numbers a lane, of which `above` lie before, the need-th is: x, what lies before it and it; -1: not here.
+struct Found {
+  int x, above, same;
+};
+SB_DEV Found find_in(const int (&c)[4], int above, int need) {
+  Found f{-1, 0, 0};
 #pragma unroll
-  for (int x = 0; x < each; ++x) sum += c[x];
-  int s = sum;
-#pragma unroll
-  for (int x = 1; x < 32; x <<= 1) {
-    const int u = __shfl_up_sync(0xFFFFFFFFu, s, x);
-    if (lane >= x) s += u;
-  }
-  __syncthreads();
-  if (lane == 31) told.room[0][warp] = s;
-  __syncthreads();
-  int above = s - sum;
-  for (int w = 0; w < warp; ++w) above += told.room[0][w];
-#pragma unroll
-  for (int x = 0; x < each; ++x) {
-    if (above < need && need <= above + c[x]) {
-      told.found[0] = first + each - 1 - x;
-      told.found[1] = above;
-      told.found[2] = c[x];
-    }
+  for (int x = 0; x < 4; ++x) {
+    if (above < need && need <= above + c[x]) f = {x, above, c[x]};
     above += c[x];
+  }
+  return f;
+}
+
+// What the CTAs of a cluster tell: the sums of their bins by 32.
+SB_DEV void tell_groups(Told& told, int which) {
+  const uint4 u = reinterpret_cast<const uint4*>(told.bins[which])[threadIdx.x];
+  int sum = (int)(u.x + u.y + u.z + u.w);
+#pragma unroll
+  for (int x = 1; x < 8; x <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+  if (lane_id() % 8 == 0) told.groups[which][threadIdx.x / 8] = sum;
+}
+
+// After a pass over a CTA's states.
+SB_DEV void counted(Told& told, int which, int ctas) {
+  if (ctas > 1) {
+    __syncthreads();
+    tell_groups(told, which);
+  }
+  all_sync(ctas);
+}
+
+// The bin of all CTAs' bins, which they have told, that holds the need-th number from the top; need becomes its place in
+// the bin, same how many the bin holds.  In a cluster one warp looks at the groups of all CTAs and then at the bins
+// of one group (for eight CTAs 0.9 us, where all threads looked at all bins 2.7).
+SB_DEV int find_bin(Told& told, int which, int& need, int& same, int ctas) {
+  static_assert(kBins == 4 * kSelect && kBins / 32 == 64, "four bins a thread, four groups a lane of 16");
+  const int lane = lane_id(), warp = warp_id();
+  auto add = [](int (&c)[4], const uint4& u) {  // from the top
+    c[0] += (int)u.w;
+    c[1] += (int)u.z;
+    c[2] += (int)u.y;
+    c[3] += (int)u.x;
+  };
+  int c[4] = {0, 0, 0, 0};
+  if (ctas > 1) {
+    if (warp == 0) {
+#pragma unroll
+      for (int r = 0; r < kMostCtas; r += 2)
+        if (r + lane / 16 < ctas) add(c, peer_words(&told.groups[which][60 - lane % 16 * 4], (uint32_t)(r + lane / 16)));
+#pragma unroll
+      for (int x = 0; x < 4; ++x) c[x] += __shfl_xor_sync(0xFFFFFFFFu, c[x], 16);
+      int sum = c[0] + c[1] + c[2] + c[3];
+      const Found g = find_in(c, scan_of(sum, 16) - sum, need);
+      const int holds = max(__ffs(__ballot_sync(0xFFFFFFFFu, g.x >= 0)) - 1, 0);
+      const int group = 63 - __shfl_sync(0xFFFFFFFFu, lane % 16 * 4 + g.x, holds), above = __shfl_sync(0xFFFFFFFFu, g.above, holds);
+      const int first = group * 32 + 28 - lane % 8 * 4;
+      c[0] = c[1] = c[2] = c[3] = 0;
+#pragma unroll
+      for (int r = 0; r < kMostCtas; r += 4)
+        if (r + lane / 8 < ctas) add(c, peer_words(&told.bins[which][first], (uint32_t)(r + lane / 8)));
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        c[x] += __shfl_xor_sync(0xFFFFFFFFu, c[x], 8);
+        c[x] += __shfl_xor_sync(0xFFFFFFFFu, c[x], 16);
+      }
+      sum = c[0] + c[1] + c[2] + c[3];
+      const Found f = find_in(c, above + scan_of(sum, 8) - sum, need);
+      if (lane < 8 && f.x >= 0) {
+        told.found[0] = first + 3 - f.x;
+        told.found[1] = f.above;
+        told.found[2] = f.same;
+      }
+    }
+  } else {
+    const int first = kBins - 4 * (1 + (int)threadIdx.x);
+    add(c, *reinterpret_cast<const uint4*>(&told.bins[which][first]));
+    const int sum = c[0] + c[1] + c[2] + c[3], of_warp = __reduce_add_sync(0xFFFFFFFFu, sum);
+    if (lane == 0) told.room[0][warp] = of_warp;  // (all_sync came after what it held before was read)
+    __syncthreads();
+    // every warp finds the warp whose bins hold it, and that warp the bin
+    const int t = lane < kSelectWarps ? told.room[0][lane] : 0, upto = scan_of(t, 32);
+    const uint32_t holds = __ballot_sync(0xFFFFFFFFu, upto - t < need && need <= upto);
+    const int above = __shfl_sync(0xFFFFFFFFu, upto - t, max(__ffs(holds) - 1, 0));
+    if (holds >> warp & 1u) {
+      const Found f = find_in(c, above + scan_of(sum, 32) - sum, need);
+      if (f.x >= 0) {
+        told.found[0] = first + 3 - f.x;
+        told.found[1] = f.above;
+        told.found[2] = f.same;
+      }
+    }
   }
   __syncthreads();
   need -= told.found[1];
@@ -397,19 +447,28 @@ SB_DEV void move_pairs(const EvictArgs& a, long long unit, const int* to, const 
   }
 }
 
+// To shared memory, asynchronously: `bytes` of 16, zeros behind them; 0: a word.
+SB_DEV void copy_in(const void* to, const void* from, int bytes) {
+  if (bytes)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(bytes) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+SB_DEV void copies_in() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // Selection with the CTA's ordered weights in shared memory: a thread has a run of states, an odd number of fours, so that
 // neighbours' 16-byte reads fall in distinct banks, and their bits (protected, staying) in registers; no pass
 // needs a word with another thread but the counts.  (1024 threads, one CTA an SM, took half as long again for clusters of
 // eight: not all of them find their SMs at once.)
-constexpr int kMostFours = 9;  // states a thread: 36; 107 KB of shared memory, two CTAs an SM
+constexpr int kMostFours = 9;  // states a thread: 36; 109 KB of shared memory, two CTAs an SM
 inline int held_fours(int cap, int ctas) { return ((cap + ctas * kSelect * 4 - 1) / (ctas * kSelect * 4)) | 1; }
-inline int held_bytes(int fours) { return kSelect * 4 * fours * 4 + kSelect * 4 * fours / 8; }
+inline int held_bytes(int fours) { return kSelect * 4 * fours * 4 + kSelect * fours; }
 // A memory of up to this many places is evicted from by one kernel: at most half of them move, 512 KB a CTA.
 constexpr int kFewPlaces = 2048;
 static_assert(sizeof(Told) >= kSelectWarps * sizeof(Pairs), "room for the pairs");
 
 __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_constant__ EvictArgs a) {
-  extern __shared__ __align__(16) uint32_t held[];  // weights of the CTA's states, then bits of the protected ones
+  extern __shared__ __align__(16) uint32_t held[];  // weights of the CTA's states, then bits of the protected ones, a byte four
   __shared__ __align__(16) Told told;
   const int warp = warp_id(), lane = lane_id(), ctas = a.ctas;
   const uint32_t rank = ctas > 1 ? cluster_ctarank() : 0u;
@@ -424,49 +483,98 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
     const int since = guard ? a.since[b] : 0;
     const int fours = ((len + ctas * kSelect * 4 - 1) / (ctas * kSelect * 4)) | 1, run = fours * 4, mine = kSelect * run;
     const int j_cta = (int)rank * mine, here = min(max(len - j_cta, 0), mine);  // the CTA's states
-    uint32_t* const bits = held + mine;
+    uint8_t* const nibbles = reinterpret_cast<uint8_t*>(held + mine);
+    // weights arrive in shared memory by themselves, sixteen bytes at once where they lie so, while stamps are looked at
+    const float* const from_w = a.weight + at + j_cta;
+    float* const to_w = a.weight_out + at + j_cta;
+    const int* const from_b = a.born + at + j_cta;
+    int* const to_b = a.born_out + at + j_cta;
+    const bool copied = a.weight_out != a.weight, copied_b = a.born_out != a.born;
+    const uintptr_t all_at = reinterpret_cast<uintptr_t>(from_w) | reinterpret_cast<uintptr_t>(to_w) |
+                             (a.born ? reinterpret_cast<uintptr_t>(from_b) | reinterpret_cast<uintptr_t>(to_b) : 0);
+    const bool wide = (all_at & 15) == 0;
+    const int step = wide ? 4 : 1, kept = min(keep - j_cta, here);  // as if all of those below keep stayed
+    for (int j = (int)threadIdx.x * step; j < here; j += kSelect * step) copy_in(held + j, from_w + j, wide ? min(16, (here - j) * 4) : 0);
     for (int x = threadIdx.x; x < kBins; x += kSelect) reinterpret_cast<uint4*>(told.bins)[x] = make_uint4(0, 0, 0, 0);
-    int n[2] = {0, 0}, all[2];
-    constexpr int kAtOnce = 8;
-    for (int w0 = warp * 32; w0 < here; w0 += kAtOnce * kSelect) {
-      float f[kAtOnce];
-      int s[kAtOnce];
+    if (!a.born) {
+      for (int x = threadIdx.x; x * 16 < here; x += kSelect) reinterpret_cast<uint32_t*>(nibbles)[x] = 0;
+    } else if (wide) {
+      int4 s[kMostFours];
 #pragma unroll
-      for (int x = 0; x < kAtOnce; ++x) {
-        const int j = w0 + x * kSelect + lane;
-        f[x] = j < here ? a.weight[at + j_cta + j] : 0.f;
-        s[x] = a.born && j < here ? a.born[at + j_cta + j] : 0;
+      for (int x = 0; x < kMostFours; ++x) {
+        const int j = ((int)threadIdx.x + x * kSelect) * 4;
+        s[x] = make_int4(0, 0, 0, 0);
+        if (j + 3 < here) {
+          s[x] = *reinterpret_cast<const int4*>(from_b + j);
+        } else if (j < here) {
+          s[x].x = from_b[j];
+          if (j + 1 < here) s[x].y = from_b[j + 1];
+          if (j + 2 < here) s[x].z = from_b[j + 2];
+        }
       }
 #pragma unroll
-      for (int x = 0; x < kAtOnce; ++x) {
-        const int w = w0 + x * kSelect, j = w + lane;
-        if (w < here) {
-          const uint32_t word = __ballot_sync(0xFFFFFFFFu, guard && j < here && s[x] >= since);
-          held[j] = ordered(f[x]);
-          if (lane == 0) {
-            bits[w >> 5] = word;
-            n[0] += __popc(word);
-          }
-          if (j_cta + j < keep && j < here) {  // as if all of these stayed
-            if (a.weight_out != a.weight) a.weight_out[at + j_cta + j] = f[x];
-            if (a.born_out != a.born) a.born_out[at + j_cta + j] = s[x];
-          }
+      for (int x = 0; x < kMostFours; ++x) {
+        const int j = ((int)threadIdx.x + x * kSelect) * 4;
+        if (j >= here) break;
+        const int low = copied_b ? kept - j : 0;
+        nibbles[j >> 2] = guard ? (s[x].x >= since) | (s[x].y >= since) << 1 | (s[x].z >= since) << 2 | (s[x].w >= since) << 3 : 0;
+        if (low >= 4) {
+          *reinterpret_cast<int4*>(to_b + j) = s[x];
+        } else {
+          if (low > 0) to_b[j] = s[x].x;
+          if (low > 1) to_b[j + 1] = s[x].y;
+          if (low > 2) to_b[j + 2] = s[x].z;
+        }
+      }
+    } else {
+      constexpr int kAtOnce = 8;
+      for (int j0 = warp * 32; j0 < here; j0 += kAtOnce * kSelect) {
+        int s[kAtOnce];
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
+          const int j = j0 + x * kSelect + lane;
+          s[x] = j < here ? from_b[j] : 0;
+        }
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
+          const int j = j0 + x * kSelect + lane;
+          if (j0 + x * kSelect >= here) break;
+          const uint32_t word = __ballot_sync(0xFFFFFFFFu, guard && s[x] >= since);
+          if (lane % 4 == 0) nibbles[j >> 2] = word >> lane & 15u;
+          if (copied_b && j < kept) to_b[j] = s[x];
         }
       }
     }
-    before_and_all(n, all, told);
-    if (threadIdx.x == 0) told.counts[0][0] = all[0];
-    // this thread's run
+    copies_in();
+    for (int j = (int)threadIdx.x * step; j < here; j += kSelect * step) {  // what this thread has copied
+      const int low = copied ? kept - j : 0;
+      if (wide) {
+        uint4 u = *reinterpret_cast<const uint4*>(held + j);
+        if (low >= 4) {
+          *reinterpret_cast<uint4*>(to_w + j) = u;
+        } else {
+          if (low > 0) to_w[j] = __uint_as_float(u.x);
+          if (low > 1) to_w[j + 1] = __uint_as_float(u.y);
+          if (low > 2) to_w[j + 2] = __uint_as_float(u.z);
+        }
+        u = make_uint4(ordered(__uint_as_float(u.x)), ordered(__uint_as_float(u.y)), ordered(__uint_as_float(u.z)),
+                       ordered(__uint_as_float(u.w)));
+        *reinterpret_cast<uint4*>(held + j) = u;
+      } else {
+        const float f = __uint_as_float(held[j]);
+        if (low > 0) to_w[j] = f;
+        held[j] = ordered(f);
+      }
+    }
+    __syncthreads();
+    // this thread's run, its protected states, and those of all
     const int j_run = (int)threadIdx.x * run, states = min(max(here - j_run, 0), run), my_fours = (states + 3) / 4;
     const uint64_t valid = states > 0 ? ~0ull >> (64 - states) : 0ull;
     uint64_t safe = 0;
-    if (states > 0) {
-      const int w = j_run >> 5, w_last = (here - 1) >> 5, o = j_run & 31;
-      const uint64_t lo = bits[w] | (w + 1 <= w_last ? (uint64_t)bits[w + 1] << 32 : 0ull);
-      safe = lo >> o;
-      if (o && w + 2 <= w_last) safe |= (uint64_t)bits[w + 2] << (64 - o);
-      safe &= valid;
-    }
+    for (int i = 0; i < my_fours; ++i) safe |= (uint64_t)nibbles[(j_run >> 2) + i] << (4 * i);
+    safe &= valid;
+    const int n = __reduce_add_sync(0xFFFFFFFFu, __popcll(safe));
+    if (lane == 0) told.room[1][warp] = n;
     const uint4* const keys = reinterpret_cast<const uint4*>(held + j_run);
     {  // the first pass for both classes, before it is known which of them weights decide among
       // (many states may have one weight, new ones 0: runs of a bin are counted before they are added)
@@ -488,17 +596,22 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
       }
       if (count) atomicAdd(&told.bins[0][bin], count);
     }
-    all_sync(ctas);
+    __syncthreads();
+    int protect = __reduce_add_sync(0xFFFFFFFFu, lane < kSelectWarps ? told.room[1][lane] : 0);
     if (ctas > 1) {
-      all[0] = __reduce_add_sync(0xFFFFFFFFu, lane < ctas ? (int)peer_word(&told.counts[0][0], (uint32_t)lane) : 0);
+      if (threadIdx.x == 0) told.counts[0][0] = protect;
+      tell_groups(told, 0);
+      tell_groups(told, 1);
+      all_sync(ctas);
+      protect = __reduce_add_sync(0xFFFFFFFFu, lane < ctas ? (int)peer_word(&told.counts[0][0], (uint32_t)lane) : 0);
     }
     // the states among which weights decide: the protected ones where they alone are too many, else the others
-    const bool inner = all[0] >= keep;
+    const bool inner = protect >= keep;
     const uint64_t who = inner ? safe : valid & ~safe;
-    int need = inner ? keep : keep - all[0], same = 0;
+    int need = inner ? keep : keep - protect, same = 0;
     uint32_t last = 0xFFFFFFFFu;  // the ordered weight of the last state that stays; `need` of that weight do
     if (need > 0) {
-      last = as_prefix(find_bin(told, told.bins[inner ? 0 : 1], need, same, ctas), 0);
+      last = as_prefix(find_bin(told, inner ? 0 : 1, need, same, ctas), 0);
       for (int pass = 1; pass < 3; ++pass) {
         int bin = -1, count = 0;
         for (int i = 0; i < my_fours; ++i) {
@@ -517,8 +630,8 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
             }
         }
         if (count) atomicAdd(&told.bins[1 + pass][bin], count);
-        all_sync(ctas);
-        last |= as_prefix(find_bin(told, told.bins[1 + pass], need, same, ctas), pass);
+        counted(told, 1 + pass, ctas);
+        last |= as_prefix(find_bin(told, 1 + pass, need, same, ctas), pass);
       }
     }
     uint64_t more = 0, tied = 0;
@@ -546,8 +659,8 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
     int put[2] = {__popcll(free), __popcll(move)}, total[2], base[2];
     before_and_all(put, total, base, told, 2, ctas, rank);
     moves = total[1];
-    // one kernel: the pairs in shared memory, behind the bits
-    int* const to = a.parts ? a.to + unit * a.half : reinterpret_cast<int*>(bits + mine / 32);
+    // one kernel: the pairs in shared memory, behind the nibbles
+    int* const to = a.parts ? a.to + unit * a.half : reinterpret_cast<int*>(held + mine + mine / 16);
     int* const from = a.parts ? a.from + unit * a.half : to + a.half;
     if (a.parts) {
       // through shared memory, over the weights, from both ends, and out in whole lines
@@ -658,8 +771,8 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_long_kernel(const __g
             }
           }
         }
-        all_sync(ctas);
-        last |= as_prefix(find_bin(told, told.bins[pass], need, same, ctas), pass);
+        counted(told, pass, ctas);
+        last |= as_prefix(find_bin(told, pass, need, same, ctas), pass);
       }
     }
     const bool some = need > 0, choose = same > need;
