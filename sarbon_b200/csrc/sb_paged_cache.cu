@@ -460,7 +460,7 @@ SB_DEV void copies_in() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // neighbours' 16-byte reads fall in distinct banks, and their bits (protected, staying) in registers; no pass
 // needs a word with another thread but the counts.  (1024 threads, one CTA an SM, took half as long again for clusters of
 // eight: not all of them find their SMs at once.)
-constexpr int kMostFours = 9;  // states a thread: 36; 109 KB of shared memory, two CTAs an SM
+constexpr int kMostFours = 15, kFoursOfTwo = 9;  // states a thread: 60; up to 36 (109 KB of shared memory) two CTAs an SM
 inline int held_fours(int cap, int ctas) { return ((cap + ctas * kSelect * 4 - 1) / (ctas * kSelect * 4)) | 1; }
 inline int held_bytes(int fours) { return kSelect * 4 * fours * 4 + kSelect * fours; }
 // A memory of up to this many places is evicted from by one kernel: at most half of them move, 512 KB a CTA.
@@ -499,31 +499,34 @@ __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_c
     if (!a.born) {
       for (int x = threadIdx.x; x * 16 < here; x += kSelect) reinterpret_cast<uint32_t*>(nibbles)[x] = 0;
     } else if (wide) {
-      int4 s[kMostFours];
+      constexpr int kAtOnce = kFoursOfTwo;
+      for (int j0 = (int)threadIdx.x * 4; j0 < here; j0 += kAtOnce * kSelect * 4) {
+        int4 s[kAtOnce];
 #pragma unroll
-      for (int x = 0; x < kMostFours; ++x) {
-        const int j = ((int)threadIdx.x + x * kSelect) * 4;
-        s[x] = make_int4(0, 0, 0, 0);
-        if (j + 3 < here) {
-          s[x] = *reinterpret_cast<const int4*>(from_b + j);
-        } else if (j < here) {
-          s[x].x = from_b[j];
-          if (j + 1 < here) s[x].y = from_b[j + 1];
-          if (j + 2 < here) s[x].z = from_b[j + 2];
+        for (int x = 0; x < kAtOnce; ++x) {
+          const int j = j0 + x * kSelect * 4;
+          s[x] = make_int4(0, 0, 0, 0);
+          if (j + 3 < here) {
+            s[x] = *reinterpret_cast<const int4*>(from_b + j);
+          } else if (j < here) {
+            s[x].x = from_b[j];
+            if (j + 1 < here) s[x].y = from_b[j + 1];
+            if (j + 2 < here) s[x].z = from_b[j + 2];
+          }
         }
-      }
 #pragma unroll
-      for (int x = 0; x < kMostFours; ++x) {
-        const int j = ((int)threadIdx.x + x * kSelect) * 4;
-        if (j >= here) break;
-        const int low = copied_b ? kept - j : 0;
-        nibbles[j >> 2] = guard ? (s[x].x >= since) | (s[x].y >= since) << 1 | (s[x].z >= since) << 2 | (s[x].w >= since) << 3 : 0;
-        if (low >= 4) {
-          *reinterpret_cast<int4*>(to_b + j) = s[x];
-        } else {
-          if (low > 0) to_b[j] = s[x].x;
-          if (low > 1) to_b[j + 1] = s[x].y;
-          if (low > 2) to_b[j + 2] = s[x].z;
+        for (int x = 0; x < kAtOnce; ++x) {
+          const int j = j0 + x * kSelect * 4;
+          if (j >= here) break;
+          const int low = copied_b ? kept - j : 0;
+          nibbles[j >> 2] = guard ? (s[x].x >= since) | (s[x].y >= since) << 1 | (s[x].z >= since) << 2 | (s[x].w >= since) << 3 : 0;
+          if (low >= 4) {
+            *reinterpret_cast<int4*>(to_b + j) = s[x];
+          } else {
+            if (low > 0) to_b[j] = s[x].x;
+            if (low > 1) to_b[j + 1] = s[x].y;
+            if (low > 2) to_b[j + 2] = s[x].z;
+          }
         }
       }
     } else {
@@ -852,10 +855,40 @@ struct EvictPlan {
   long long lists, moves, bits;  // ints
   long long bytes() const { return (lists + moves + bits) * 4; }
 };
-// CTAs an (item, key head): doubled while all are resident at once (two an SM) and the states that a CTA is relieved of
-// take longer than telling one more what it counted, or until the weights fit shared memory.  Measured, us of the first
-// kernel with 1, 2, 4, 8: 128 units of 18,360 places 35, 26, 39, 72; 4 units of 16,000 22.5, 18.6, 16.8, 17.8; of 8000
-// -, 15.4, 13.2, -; of 4000 11.1, 11.2, 12.9, 17.8.
+// Clusters of `ctas` that find an SM for each of their CTAs at once (the SMs come in groups, and not all divide evenly).
+int clusters_at_once(int ctas, int sms) {
+  static int of[64][kMostCtas + 1];
+  int dev = 0;
+  if (ctas == 1 || cudaGetDevice(&dev) != cudaSuccess) return sms / ctas;
+  int& known = of[dev & 63][ctas];
+  if (known == 0) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kSelect);
+    cfg.dynamicSmemBytes = (size_t)held_bytes(kMostFours);  // no room for another
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)ctas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    static bool ready[64];
+    if (xattn_smem(reinterpret_cast<const void*>(&evict_select_kernel), held_bytes(kMostFours), ready) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, evict_select_kernel, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = std::max(1, sms / ctas * 7 / 8);
+    }
+    known = n;
+  }
+  return known;
+}
+
+// CTAs an (item, key head): those with the least estimated time.  A CTA takes about 4.8 us and, by how its weights spread over
+// the bins, 1.8 to 2.9 for each four states of a thread, 1.2 to 1.5 times that where it shares its SM; one of a cluster of
+// c 8.3 + 0.17 c.  Measured, us of the first kernel with 1, 2, 4, 6, 8: 4 units of 4000 places 10.1, 10.6, 11.0, 11.2, 11.3; of
+// 8000 13.6, 13.7, 10.9, 11.1, 11.4; of 16,000 20.5, 17.1, 14.3, 14.6, 11.5; 64 of 8000 13.9, 14.2, 13.7, 23.5, 26.9; 128 of
+// 18,360, whose weights spread, 34.3, 24.0, 37, 42.6, 71; 16 of 130,560, alike, -, -, -, 34.7, 41.7.
 // One kernel where there are few places (us in kernels, one and two: 256 units of 1000 places 13.7 and 18.3, of 2000 16.4
 // and 19.2, of 8000 39.5 and 33), unless the new lengths lie on the old ones, which its CTAs read at any time.
 EvictPlan evict_plan(int B, int Hkv, int cap, bool apart, int sms) {
@@ -868,10 +901,20 @@ EvictPlan evict_plan(int B, int Hkv, int cap, bool apart, int sms) {
     p.held = true;
     return p;
   }
-  while (p.ctas < kMostCtas &&
-         ((units * p.ctas <= sms && cap > 1024 * p.ctas * p.ctas) || held_fours(cap, p.ctas) > kMostFours))
-    p.ctas *= 2;
-  p.held = held_fours(cap, p.ctas) <= kMostFours;
+  p.held = held_fours(cap, kMostCtas) <= kMostFours;
+  if (!p.held) p.ctas = kMostCtas;
+  double best = 1e300;
+  for (int c = 1; p.held && c <= kMostCtas; ++c) {
+    const int fours = held_fours(cap, c);
+    if (fours > kMostFours) continue;
+    const long long room = clusters_at_once(c, sms), resident = fours <= kFoursOfTwo ? 2 * room : room;
+    const double us = (double)((units + resident - 1) / resident) *
+                      ((c > 1 ? 8.3 + 0.17 * c : 4.8) + 2.7 * fours * (units > room ? 1.4 : 1.0));
+    if (us < best) {
+      best = us;
+      p.ctas = c;
+    }
+  }
   constexpr int each = kMoveWarps * 32;
   p.parts = (int)std::max(1ll, std::min(((long long)p.half + each - 1) / each, (16ll * sms + units - 1) / units));
   p.lists = 2 * units * p.half;

@@ -557,7 +557,7 @@ def test_evict_partly_in_place(n):
         assert all(same_bits(x, y) for x, y in zip(results[0], other))
 
 
-@pytest.mark.parametrize("cap", [18400, 18560, 48960, 147360, 147520, 300000])
+@pytest.mark.parametrize("cap", [18400, 18560, 48960, 147360, 147520, 245760, 245776, 300000])
 def test_evict_long(cap):
     """One CTA to eight an item and head, places that just fit their shared memory, just do not, and far more, against a sort."""
     import sarbon_b200 as sb
