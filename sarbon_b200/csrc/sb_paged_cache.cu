@@ -143,8 +143,8 @@ __global__ void __launch_bounds__(kWriteWarps * 32, MODE == 2 ? 2 : 4)
 // order, are kept in shared memory where they fit.
 //
 // What bounds it: the chain of passes, each with an exchange of counts.  16 x 8 units of 18,360 states, 2040 of them to
-// go, rows of 256 bytes: 26 us for the selection, 13.5 for the rows (82 MB, 93 % of the copy rate); 2 x 8 of 130,560, half
-// of them, rows of 64 bytes: 50 and 40 (150 MB in pieces of 64 bytes: 58 %).
+// go, rows of 256 bytes: 24 us for the selection, 13.5 for the rows (82 MB, 93 % of the copy rate); 2 x 8 of 130,560, half
+// of them, rows of 64 bytes: 34.7 and 40 (150 MB in pieces of 64 bytes: 58 %).
 struct EvictArgs {
   Pool k, v;
   PageTable pages;
@@ -463,8 +463,8 @@ SB_DEV void copies_in() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 constexpr int kMostFours = 15, kFoursOfTwo = 9;  // states a thread: 60; up to 36 (109 KB of shared memory) two CTAs an SM
 inline int held_fours(int cap, int ctas) { return ((cap + ctas * kSelect * 4 - 1) / (ctas * kSelect * 4)) | 1; }
 inline int held_bytes(int fours) { return kSelect * 4 * fours * 4 + kSelect * fours; }
-// A memory of up to this many places is evicted from by one kernel: at most half of them move, 512 KB a CTA.
-constexpr int kFewPlaces = 2048;
+// A memory of up to this many places is evicted from by one kernel: at most half of them move, 1 MB a CTA.
+constexpr int kFewPlaces = 4096;
 static_assert(sizeof(Told) >= kSelectWarps * sizeof(Pairs), "room for the pairs");
 
 __global__ void __launch_bounds__(kSelect, 2) evict_select_kernel(const __grid_constant__ EvictArgs a) {
@@ -889,8 +889,9 @@ int clusters_at_once(int ctas, int sms) {
 // c 8.3 + 0.17 c.  Measured, us of the first kernel with 1, 2, 4, 6, 8: 4 units of 4000 places 10.1, 10.6, 11.0, 11.2, 11.3; of
 // 8000 13.6, 13.7, 10.9, 11.1, 11.4; of 16,000 20.5, 17.1, 14.3, 14.6, 11.5; 64 of 8000 13.9, 14.2, 13.7, 23.5, 26.9; 128 of
 // 18,360, whose weights spread, 34.3, 24.0, 37, 42.6, 71; 16 of 130,560, alike, -, -, -, 34.7, 41.7.
-// One kernel where there are few places (us in kernels, one and two: 256 units of 1000 places 13.7 and 18.3, of 2000 16.4
-// and 19.2, of 8000 39.5 and 33), unless the new lengths lie on the old ones, which its CTAs read at any time.
+// One kernel where there are few places (us in kernels, one and two: 256 units of 1000 places 12.1 and 16.7, of 2000 14.0
+// and 20.5, of 4000 22.0 and 26.4, of 8000 45.8 and 45.2; 4 units 10.2 and 11.8, 10.7 and 12.3, 14.2 and 15.3, 20.1 and
+// 15.5), unless the new lengths lie on the old ones, which its CTAs read at any time.
 EvictPlan evict_plan(int B, int Hkv, int cap, bool apart, int sms) {
   const long long units = (long long)B * Hkv;
   EvictPlan p{};

@@ -538,7 +538,7 @@ def test_evict_lengths_and_pages_outside():
     check_eviction(k, v, table, ints(95, 90, 2 ** 31 - 1, 80, -4), weight, 40, born, None)
 
 
-@pytest.mark.parametrize("n", [900, 30000, 160000])
+@pytest.mark.parametrize("n", [900, 2100, 4050, 4100, 30000, 160000])
 def test_evict_partly_in_place(n):
     """One kernel, clusters and long memories; each result on its operand or apart."""
     import sarbon_b200 as sb
