@@ -700,3 +700,42 @@ def test_calls_from_either_side(monkeypatch):
     whole = sb.paged_attention(s["q"], s["k"], s["v"], s["table"], s["lens"], 4, 2)
     assert same_bits(whole, sb.paged_attention(s["q"].as_subclass(Own), s["k"], s["v"], s["table"], s["lens"], 4, 2))
     assert sb.paged_attention(s["q"][:0], s["k"], s["v"], s["table"][:0], s["lens"][:0], 4, 2).shape == (0, 2, 256)
+
+
+FIRST_IN_A_CAPTURE = """
+import torch
+import test_gpu_paged_ops as t
+import sarbon_b200 as sb
+
+def case(n, dim, pt, heads):
+    g = t.gen(n)
+    k, v, table = t.pages_of(g, 2, n, 40, 2 * dim, pt)
+    weight = t.rand(g, 2, 2, table.shape[1] * 40).abs()
+    q, lens = t.rand(g, 2, 1, heads * dim, dtype=torch.float16), t.ints(n, n - 5)
+    return lambda: (sb.paged_attention(q, k, v, table, lens, heads, 2, weight=weight.clone()),) + \\
+        sb.paged_evict(k.view(k.shape), v, table, lens, weight, n // 2)[:2]
+
+case(100, 32, torch.float16, 2)()
+for n, dim, pt, heads in ((90, 64, t.E4M3, 20), (3000, 128, torch.float16, 4), (9000, 32, t.E4M3, 2), (70000, 64, torch.float16, 4)):
+    run = case(n, dim, pt, heads)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = run()
+    graph.replay()
+    torch.cuda.synchronize()
+    ref = case(n, dim, pt, heads)()
+    assert all(t.same_bits(a, b) for a, b in zip(got, ref)), n
+print("fine")
+"""
+
+
+def test_first_calls_of_a_size_inside_a_capture():
+    """A process whose first call was a small one captures other types and sizes at once."""
+    import pathlib
+    import subprocess
+    import sys
+    here = pathlib.Path(__file__).resolve().parent
+    r = subprocess.run([sys.executable, "-c", f"import sys; sys.path[:0] = [{str(here)!r}, {str(here.parent)!r}]\n" + FIRST_IN_A_CAPTURE],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
