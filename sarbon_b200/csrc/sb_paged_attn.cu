@@ -285,7 +285,8 @@ SB_DEV void join_cluster(const PagedArgs& a, int b, int kvh, int unit, int r0, i
     float f[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      f[u] = k * __uint_as_float(v[u]);
+      const float x = __uint_as_float(v[u]);
+      f[u] = fabsf(x) == INFINITY ? x : k * x;  // (however small its share)
       for (int z = 1; z < n; z <<= 1) f[u] += __shfl_xor_sync(0xFFFFFFFFu, f[u], z);
     }
     if (s == 0 && e < work) {
@@ -294,6 +295,39 @@ SB_DEV void join_cluster(const PagedArgs& a, int b, int kvh, int unit, int r0, i
       if (c == 0 && a.lse) a.lse[((long long)b * a.H + w.h) * a.Tq + w.t] = all * 0.69314718055994531f;
     }
   }
+}
+
+// A 16-bit value that is infinite is lost where a probability is multiplied in two parts (inf - inf where they differ in
+// sign, 0 x inf where the second is 0).  So a row's channels c .. c + 7 that came out as no number, `lost` as bits, are asked
+// here what states j0 .. j1 - 1 make of them: bits 0 .. 7 where one has +inf, 8 .. 15 -inf, 16 .. 23 no number (NaN, or an infinite
+// value of a state whose score is -inf).  A share that rounds to 0 is taken for what it stands for.  Looked at only
+// then, so that the loop over the states knows nothing of it.
+template <int DH, bool BF16>
+__device__ __noinline__ uint32_t odd_values(const PagedArgs& a, int b, int kvh, int t, int h, int c, uint32_t lost, int j0,
+                                            int j1) {
+  constexpr int type = BF16 ? SB_BF16 : SB_F16;
+  const uint16_t* const q = static_cast<const uint16_t*>(a.q) + b * a.q_img + t * a.q_row + (long long)h * DH;
+  uint32_t odd = 0;
+  for (int j = j0; j < j1; ++j) {
+    uint32_t row;
+    const int p = a.pages.entry(b, (uint32_t)j, row);
+    if (!a.pages.has(p)) continue;
+    float v[8];
+    unpack8(load_raw8(reinterpret_cast<const void*>(a.v.row_at(p, row)), type, kvh * DH + c), type, v);
+    uint32_t here = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      here |= (v[u] == INFINITY ? 1u : v[u] == -INFINITY ? 1u << 8 : v[u] != v[u] ? 1u << 16 : 0u) << u;
+    if (here & 0xFFFFu) {
+      const void* const k = reinterpret_cast<const void*>(a.k.row_at(p, row));
+      float s = 0.f;
+      for (int x = 0; x < DH; ++x) s = fmaf(one_of(q, type, x), one_of(k, type, kvh * DH + x), s);
+      if (s == -INFINITY) here = ((here | here >> 8 | here >> 16) & 0xFFu) << 16;
+    }
+    odd |= here;
+    if (((odd >> 16 | (odd & odd >> 8)) & lost) == lost) break;  // none of them can be anything else
+  }
+  return odd;
 }
 
 // NB: column tiles of eight query rows
@@ -748,6 +782,19 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
       for (int u = 0; u < 8; ++u) f[u] = none ? 0.f : f[u] * inv;
       const float log_sum = none ? -INFINITY : top - lift + log2f(sum);
       const Row w(a, kvh, r0 + r);
+      if constexpr (!E4M3) {  // (e4m3 has no infinities)
+        uint32_t lost = 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) lost |= (uint32_t)(f[u] != f[u]) << u;
+        if (lost && sum == sum) {
+          const int seen = a.causal ? max(count - a.Tq + 1 + w.t, 0) : count;
+          const uint32_t odd = odd_values<DH, BF16>(a, b, kvh, w.t, w.h, c, lost, at.c * CK, min(seen, (at.c + piece) * CK));
+          lost &= (odd ^ odd >> 8) & ~(odd >> 16);  // of one sign
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (lost >> u & 1u) f[u] = odd >> u & 1u ? INFINITY : -INFINITY;
+        }
+      }
       if (a.cluster > 1) {
         store8(rows_of_cluster, SB_F32, r * DH + c, f);
         if (c == 0) found_l[r] = log_sum;
@@ -903,7 +950,7 @@ __global__ void __launch_bounds__(kEndThreads, kEndOcc) paged_end_kernel(const _
           const long long place = 2 * (cta + x) + (x == 0);  // the first of them goes on behind its CTA
           unpack8(load_raw8(a.part_o, SB_F32, (place * a.part_rows + r) * DH + c), SB_F32, v);
 #pragma unroll
-          for (int u = 0; u < 8; ++u) f[u] = fmaf(k, v[u], f[u]);
+          for (int u = 0; u < 8; ++u) f[u] = fmaf(fabsf(v[u]) == INFINITY ? 1.f : k, v[u], f[u]);  // (however small its share)
         }
         float4* to = reinterpret_cast<float4*>(&part[threadIdx.x / per][c]);
         to[0] = make_float4(f[0], f[1], f[2], f[3]);

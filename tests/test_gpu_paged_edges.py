@@ -1,0 +1,103 @@
+"""The paged memory's operators where values, lengths or places end.
+
+Bounds are those of ``test_gpu_paged_ops``, whose formulas in 64 bits are used."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged_ops import formula, gen, ints, pages_of, rand, rows_of, same_bits, unit
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU tests need CUDA")
+
+
+def put(pool, table, item, state, channels, value):
+    """One state's channels in its page."""
+    page = pool.shape[1]
+    pool[int(table[item, state // page]), state % page, channels] = value
+
+
+# a CTA a key head, a cluster, shared chunks; more rows than 8 and 16
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("b,tq,n,heads,kv_heads,dim,page", [
+    (2, 1, 240, 8, 4, 32, 20), (2, 1, 1, 2, 1, 64, 4), (2, 3, 1500, 4, 1, 128, 50), (1, 1, 2048, 4, 4, 128, 60), (2, 2, 9001, 4, 2, 64, 13),
+    (64, 1, 4100, 4, 2, 128, 64), (2, 9, 700, 4, 2, 64, 60), (2, 20, 6000, 2, 1, 32, 100),
+])
+def test_attention_infinite_values(b, tq, n, heads, kv_heads, dim, page, dtype):
+    """A channel that holds +inf in a state with weight is +inf, with -inf too or NaN it is NaN, wherever the state lies; channels
+    beside it and rows that do not see it are as without."""
+    import sarbon_b200 as sb
+    g = gen(n + dim)
+    k, v, table = pages_of(g, b, n, page, kv_heads * dim, dtype)
+    q = rand(g, b, tq, heads * dim, dtype=dtype)
+    lens = torch.tensor([n - (i * 5) % max(1, n // 3) for i in range(b)], dtype=torch.int32, device="cuda")
+    for i, m in enumerate(lens.tolist()):
+        for x in range(12):  # +inf in states all over, -inf, both, NaN beside it
+            put(v, table, i, (x * 7919 + i) % m, x, math.inf)
+            put(v, table, i, (x * 6007 + i) % m, dim - 1 - x, -math.inf)
+        put(v, table, i, 0, 13, math.inf)
+        put(v, table, i, m - 1, 13, math.inf)
+        put(v, table, i, m // 2, 14, math.inf)
+        put(v, table, i, m - 1, 14, -math.inf if m > 1 else math.inf)
+        put(v, table, i, m // 3, 15, math.nan)
+        put(v, table, i, m - 1, 15, math.inf if m > 1 else math.nan)
+    weight = rand(g, b, kv_heads, table.shape[1] * page).abs()
+    for causal in (False, True):
+        lse, account = torch.empty(b, heads, tq, device="cuda"), weight.clone()
+        out = sb.paged_attention(q, k, v, table, lens, heads, kv_heads=kv_heads, causal=causal, weight=account, lse=lse)
+        assert same_bits(out, sb.paged_attention(q, k, v, table, lens, heads, kv_heads=kv_heads, causal=causal))
+        clean = v.masked_fill(~v.isfinite(), 0.0)
+        ref, ref_lse, p, absolute, whole, e = formula(q, k, clean, table, lens, heads, kv_heads, causal=causal)
+        takes = (p > 0).double()
+        values = v[table.long()].flatten(1, 2).unflatten(-1, (kv_heads, -1)).transpose(1, 2)
+        plus, minus, nan = (takes @ x.double() > 0 for x in (values == math.inf, values == -math.inf, values.isnan()))
+        ref = ref.masked_fill(plus, math.inf).masked_fill(minus, -math.inf).masked_fill(nan | (plus & minus), math.nan)
+        tol = unit(dtype) * ref.abs() + (unit(dtype) ** 2 + e) * absolute + 2.0 ** -32 * whole + 2.0 ** -25
+        tol, ref = rows_of(tol, b, tq), rows_of(ref, b, tq)
+        got, odd = out.double(), ~ref.isfinite()
+        assert torch.equal(got.isnan(), ref.isnan())
+        assert torch.equal((got == math.inf) | (got == -math.inf), ref.isinf()) and torch.equal(got[ref.isinf()], ref[ref.isinf()])
+        assert ((got - ref).abs()[~odd] <= 1.02 * tol[~odd]).all()
+        seen = ref_lse.view(b, heads, tq) > -math.inf
+        assert torch.equal(lse > -math.inf, seen) and account.isfinite().all()
+        again = weight.clone()  # the account and the log-sum-exp know nothing of values
+        plain = torch.empty_like(lse)
+        sb.paged_attention(q, k, clean, table, lens, heads, kv_heads=kv_heads, causal=causal, weight=again, lse=plain)
+        assert same_bits(lse, plain) and same_bits(account, again)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [200, 1900, 9000])
+def test_attention_infinite_values_of_little_weight(n, dtype):
+    """States whose share is far below the 16-bit types' smallest step, in the first, a middle and the last place."""
+    import sarbon_b200 as sb
+    g = gen(n)
+    dim, page = 64, 40
+    k, v, table = pages_of(g, 1, n, page, dim, dtype, by=0.1)
+    q = rand(g, 1, 1, dim, dtype=dtype)
+    far = (-45.0 * math.sqrt(dim) / q.float().pow(2).sum() * q.float()).to(dtype)[0, 0]  # a share of about e^-45
+    for x, j in enumerate((0, n // 2, n - 1)):
+        put(k, table, 0, j, slice(None), far)
+        put(v, table, 0, j, x, math.inf)
+        put(v, table, 0, j, 5 + x, -math.inf)
+    out = sb.paged_attention(q, k, v, table, ints(n), 1)[0, 0].float()
+    assert (out[:3] == math.inf).all() and (out[5:8] == -math.inf).all() and out[8:].isfinite().all() and out[3:5].isfinite().all()
+
+
+def test_attention_infinite_keys_and_values():
+    """A state whose score is -inf has no share: 0 times its infinite value is no number."""
+    import sarbon_b200 as sb
+    g = gen(3)
+    k, v, table = pages_of(g, 1, 60, 20, 32, torch.float16)
+    q = rand(g, 1, 1, 32, dtype=torch.float16).abs()
+    put(k, table, 0, 7, 2, -math.inf)
+    put(v, table, 0, 7, 4, math.inf)
+    put(v, table, 0, 8, 5, math.inf)
+    out = sb.paged_attention(q, k, v, table, ints(60), 1)[0, 0].float()
+    assert out[4].isnan() and out[5] == math.inf and out.isfinite().sum() == 30
