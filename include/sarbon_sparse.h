@@ -556,9 +556,9 @@ typedef struct {
  * softmax(scale q k^T) v per head, query head h on key head h / (H / Hkv).  causal != 0: query t sees the first lens[b] -
  * Tq + 1 + t.  Pages: q_dtype or SB_F8.  States on no page take no part; a query without states gets zeros.  lse (fp32
  * [B][H][Tq], NULL: none): natural log of the sum of the exponentials, -inf without states.  weight (NULL: none): decay *
- * weight + the sum of the probabilities of a key head's queries, for the states below lens[b]; fixed order.  work:
- * sb_paged_attention_work bytes (16-byte aligned), not shared by calls that may overlap.  Scores, statistics,
- * probabilities and sums are fp32; probabilities meet v as two 16-bit parts. */
+ * weight + the sum of the probabilities of a key head's queries, for the states below lens[b] (decay * weight where Tq is
+ * 0); fixed order.  work: sb_paged_attention_work bytes (16-byte aligned), not shared by calls that may overlap.  Scores,
+ * statistics, probabilities and sums are fp32; probabilities meet v as two 16-bit parts. */
 typedef struct {
   sb_paged_memory memory;
   const void* q;

@@ -983,6 +983,13 @@ __global__ void __launch_bounds__(kEndThreads, kEndOcc) paged_end_kernel(const _
   }
 }
 
+// The account of a call without queries, `ends` CTAs an (item, key head): decay times the weight of the states that are there.
+__global__ void __launch_bounds__(kEndThreads) paged_age_kernel(const __grid_constant__ PagedArgs a) {
+  const int part = blockIdx.x % a.ends, head = blockIdx.x / a.ends, count = a.pages.clamp(a.lens[head / a.Hkv]);
+  float* const weight = a.weight + (long long)head * a.pages.cap;
+  for (int j = part * kEndThreads + (int)threadIdx.x; j < count; j += a.ends * kEndThreads) weight[j] *= a.decay;
+}
+
 template <int DH, int PT>
 void shape_of(int rows, int& chunk, int& occ) {
   chunk = rows <= 8 ? Paged<DH, PT, 1>::CK : Paged<DH, PT, 2>::CK;
@@ -1105,7 +1112,16 @@ extern "C" int sb_paged_attention(const sb_paged_attend* call, void* stream) {
   if (!(c.scale > 0.f) || !scales_ok(m, c.k_scale, c.v_scale) || !std::isnormal(c.scale * c.k_scale * 1.4426950408889634f))
     return record_error(SB_EINVAL, "sb_paged_attention: scale, or scales of pages that are not e4m3");
   if (c.weight && !(c.decay >= 0.f && c.decay <= 1.f)) return record_error(SB_EINVAL, "sb_paged_attention: decay from 0 to 1");
-  if (m->B == 0 || Tq == 0) return SB_OK;
+  if (m->B == 0 || (Tq == 0 && (!c.weight || m->N == 0))) return SB_OK;
+  if (Tq == 0 && c.lens) {
+    PagedArgs a{};
+    a.pages = page_table(m);
+    a.lens = c.lens; a.Hkv = m->Hkv; a.weight = c.weight; a.decay = c.decay;
+    const long long heads = (long long)m->B * m->Hkv;
+    a.ends = (int)std::min((a.pages.cap + kEndThreads - 1ll) / kEndThreads, std::max(1ll, 2048 / heads));
+    const cudaError_t e = launch_after(paged_age_kernel, heads * a.ends, kEndThreads, 0, static_cast<cudaStream_t>(stream), a, 1, false);
+    return e == cudaSuccess ? SB_OK : record_error(SB_ECUDA, cudaGetErrorString(e));
+  }
   if (!c.lens || !xattn_view_ok(c.q, c.q_row, c.q_img) || !xattn_view_ok(c.out, c.out_row, c.out_img) || !paged_pools_ok(m))
     return record_error(SB_EINVAL, "sb_paged_attention: rows (16-byte aligned, strides multiples of 16 bytes) or null argument");
   const int sms = xattn_sms();

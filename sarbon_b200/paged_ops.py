@@ -188,7 +188,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, heads, kv_heads=None, scal
 
     weight (fp32 [B, kv_heads, N * page]), if given, is brought up to date: ``weight[b, h, j] = decay *
     weight[b, h, j] +`` the probabilities that the queries of key head h gave to state j, for the ``lens[b]`` states;
-    sums have a fixed order.  This takes a workspace of 4 bytes a query row, key head and place.
+    sums have a fixed order.  Without queries (Tq 0) that is ``decay`` times it.  This takes a workspace of 4 bytes a query row, key head and place.
 
     Made for single tokens: the states are read once for every 16 query rows of a key head, and split
     over the SMs where there are few rows; many queries want cross_attention."""
@@ -233,7 +233,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, heads, kv_heads=None, scal
     index = _one_device((q, k_pages, v_pages, weight, out, lse), (table, lens))
     if out is None:
         out, op = _new(q, shape, dtype)
-    if b == 0 or tq == 0:
+    if b == 0 or (tq == 0 and (weight is None or n == 0)):
         return out
     hold, work, size = _work("sb_paged_attention_work", index, b, heads, kv_heads, dim, tq, PAGE_DTYPES[page_dtype], page, n,
                              weight is not None)

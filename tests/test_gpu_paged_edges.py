@@ -101,3 +101,28 @@ def test_attention_infinite_keys_and_values():
     put(v, table, 0, 8, 5, math.inf)
     out = sb.paged_attention(q, k, v, table, ints(60), 1)[0, 0].float()
     assert out[4].isnan() and out[5] == math.inf and out.isfinite().sum() == 30
+
+
+@pytest.mark.parametrize("page,n", [(16, 3), (100, 400)])
+def test_attention_without_queries_ages_the_account(page, n):
+    """No query gives a state anything: its weight is decay times what it was, of the states that are there."""
+    import sarbon_b200 as sb
+    g = gen(page)
+    k, v, _ = pages_of(g, 1, 10, page, 128, torch.float16)
+    table = torch.zeros(4, n, dtype=torch.int32, device="cuda")
+    cap = n * page
+    before = rand(g, 4, 2, cap)
+    lens = ints(0, 5, cap - 3, cap + 9)
+    ref = torch.where(torch.arange(cap, device="cuda") < lens[:, None, None], before * 0.75, before)
+    q = torch.empty(4, 0, 256, dtype=torch.float16, device="cuda")
+    lse = torch.empty(4, 4, 0, device="cuda")
+    weight = before.clone()
+    assert sb.paged_attention(q, k, v, table, lens, 4, kv_heads=2, weight=weight, decay=0.75, lse=lse).shape == q.shape
+    assert same_bits(weight, ref)
+    graph, weight = torch.cuda.CUDAGraph(), before.clone()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        sb.paged_attention(q, k, v, table, lens, 4, kv_heads=2, weight=weight, decay=0.5)
+    graph.replay()
+    graph.replay()
+    assert same_bits(weight, torch.where(torch.arange(cap, device="cuda") < lens[:, None, None], before * 0.5 * 0.5, before))
