@@ -1012,7 +1012,8 @@ extern "C" int sb_paged_evict(const sb_paged_cut* call, void* stream) {
   const sb_paged_memory* const m = &c.memory;
   if (!paged_memory_ok(m)) return record_error(SB_EINVAL, "sb_paged_evict: sizes (dh 32, 64 or 128) or dtype");
   if (m->B == 0) return SB_OK;
-  if (!c.lens || !c.after || (m->N > 0 && (!c.weight || !c.weight_out)) || (c.since && !c.born) || (!c.born) != (!c.born_out) ||
+  // (without places an account is an empty tensor, whose address is null)
+  if (!c.lens || !c.after || (m->N > 0 && (!c.weight || !c.weight_out || (c.since && !c.born))) || (!c.born) != (!c.born_out) ||
       !paged_pools_ok(m))
     return record_error(SB_EINVAL, "sb_paged_evict: rows (16-byte aligned, strides multiples of 16 bytes) or null argument");
   EvictArgs a{};

@@ -126,3 +126,19 @@ def test_attention_without_queries_ages_the_account(page, n):
     graph.replay()
     graph.replay()
     assert same_bits(weight, torch.where(torch.arange(cap, device="cuda") < lens[:, None, None], before * 0.5 * 0.5, before))
+
+
+def test_memories_without_places():
+    """Tables without entries: nothing to write, to look at or to move, with stamps and in place too."""
+    import sarbon_b200 as sb
+    k = torch.ones(3, 8, 64, device="cuda", dtype=torch.float16)
+    v = k.clone()
+    table, new = torch.zeros(2, 0, dtype=torch.int32, device="cuda"), torch.zeros(2, 3, 64, device="cuda", dtype=torch.float16)
+    weight, born = torch.zeros(2, 1, 0, device="cuda"), torch.zeros(2, 1, 0, dtype=torch.int32, device="cuda")
+    lens = ints(4, 0)
+    assert sb.paged_write(new, new, k, v, table, lens, weight=weight, born=born, stamp=ints(1, 2)).tolist() == [0, 0]
+    assert not sb.paged_attention(new, k, v, table, lens, 1, weight=weight, decay=0.5).any()
+    after, w, r = sb.paged_evict(k, v, table, lens, weight, 3, born=born, since=ints(1, 1))
+    assert after.tolist() == [0, 0] and w.shape == weight.shape and r.shape == born.shape
+    sb.paged_evict(k, v, table, lens, weight, 3, born=born, since=ints(1, 1), weight_out=weight, born_out=born, after=lens)
+    assert lens.tolist() == [0, 0] and (k == 1).all() and (v == 1).all()
