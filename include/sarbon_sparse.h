@@ -539,8 +539,10 @@ SB_API int sb_gated_norm_backward(const void* dy, long long dy_row, long long dy
  * aligned).  State j of item b is row j % page of page table[b * table_row + j / page] (int32 [B][N], N * page
  * < 2^30); an entry outside [0, P) is no page.  weight (fp32) and born (int32) are [B][Hkv][N * page].
  * Lengths outside [0, N * page] are clamped.  Each call launches on `stream`, allocates nothing and may be
- * captured in a CUDA graph after a first call outside capture on the device.  SB_F8 pools hold e4m3 codes: c
- * stands for c * scale (scales are 1 for the other types). */
+ * captured in a CUDA graph after a first call outside capture on the device.  What a call writes shares no memory with
+ * what it reads or else writes, but where it is said that a result may be an operand (not checked here); rows of keys
+ * and values may lie between one another.  SB_F8 pools hold e4m3 codes: c stands for c * scale (scales are 1 for the
+ * other types). */
 typedef struct {
   void *k, *v;
   long long k_row, k_page, v_row, v_page;
@@ -580,7 +582,7 @@ SB_API int sb_paged_attention_work(int B, int H, int Hkv, int dh, int Tq, int pa
 /* New states: row t < count[b] (NULL: T) of k, v [B][T][Hkv*dh] (SB_F16 or SB_BF16, any strides) goes to
  * position at[b] + t of item b; pools of the same type, or SB_F8: the code nearest to the fp32 quotient
  * x / scale, at most 448 of either sign.  weight there becomes 0, born stamp[b * stamp_img + t * stamp_row] (each
- * may be NULL).  after [B] gets the new lengths and shares no memory with at. */
+ * may be NULL).  after [B] gets the new lengths. */
 typedef struct {
   sb_paged_memory memory;
   const void *k, *v;

@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 
 #include "sarbon_sparse.h"
 
@@ -103,9 +104,7 @@ bool read_memory(Reader& r, Maybe k, Maybe v, Maybe table, int64_t kv_heads, boo
     k_img = page * k_row;
     v_img = page * v_row;
   }
-  if (written && !r.need(k_row >= width && v_row >= width && k_img >= k_row * page && v_img >= v_row * page &&
-                         (k->data_ptr() != v->data_ptr() || pages == 0)))
-    return false;
+  if (written && !r.need(k_row >= width && v_row >= width && k_img >= k_row * page && v_img >= v_row * page)) return false;
   if (!r.need(table->scalar_type() == at::kInt && table->dim() == 2)) return false;
   const int64_t b = table->size(0), n = table->size(1);
   if (!r.need((table->stride(1) == 1 || n <= 1) && page < kPlaces && n < kPlaces && n * page < kPlaces &&
@@ -142,13 +141,96 @@ void* read_account(Reader& r, Maybe t, int64_t b, int64_t heads, int64_t n, c10:
     return nullptr;
   return t->data_ptr();
 }
-// Whether contiguous tensors share memory
-bool meet(Maybe a, Maybe b) {
-  if (!a || !b || a->numel() == 0 || b->numel() == 0) return false;
-  const auto x = reinterpret_cast<uintptr_t>(a->data_ptr()), y = reinterpret_cast<uintptr_t>(b->data_ptr());
-  return x < y + b->nbytes() && y < x + a->nbytes();
+// A tensor's memory: bytes of its contiguous runs, and how often each step (in bytes, rising) goes on from the first.
+struct Steps {
+  int64_t run, step[8], more[8];
+  int n = 0;
+};
+// (at most four dimensions: those of what a call takes have been looked at)
+Steps steps_of(const Tensor& t) {
+  Steps s;
+  const int64_t size = (int64_t)t.element_size();
+  const auto sizes = t.sizes(), strides = t.strides();
+  s.run = size;
+  for (size_t d = 0; d < sizes.size() && s.n < 4; ++d) {
+    if (sizes[d] <= 1 || strides[d] == 0) continue;
+    int at = s.n++;
+    for (; at > 0 && s.step[at - 1] > strides[d] * size; --at) {
+      s.step[at] = s.step[at - 1];
+      s.more[at] = s.more[at - 1];
+    }
+    s.step[at] = strides[d] * size;
+    s.more[at] = sizes[d] - 1;
+  }
+  int dense = 0;
+  for (; dense < s.n && s.step[dense] == s.run; ++dense) s.run *= s.more[dense] + 1;
+  int n = 0;
+  for (int i = dense; i < s.n; ++i) {
+    if (n > 0 && s.step[n - 1] == s.step[i]) {
+      s.more[n - 1] += s.more[i];
+    } else {
+      s.step[n] = s.step[i];
+      s.more[n++] = s.more[i];
+    }
+  }
+  s.n = n;
+  return s;
 }
-bool same_start(Maybe a, Maybe b) { return a->numel() > 0 && b->numel() > 0 && a->data_ptr() == b->data_ptr(); }
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b != 0 && a < 0); }
+// Whether two tensors, whose first to last bytes overlap, share memory: _meet of paged_ops.py.
+bool meet(const Tensor& a, const Tensor& b) {
+  const Steps s = steps_of(a), t = steps_of(b);
+  int64_t step[2], g = 0;
+  int kinds = 0;
+  for (const Steps* x : {&s, &t})
+    for (int i = 0; i < x->n; ++i) {
+      g = std::gcd(g, x->step[i]);
+      bool known = false;
+      for (int y = 0; y < std::min(kinds, 2); ++y) known = known || step[y] == x->step[i];
+      if (known) continue;
+      if (kinds < 2) step[kinds] = x->step[i];
+      ++kinds;
+    }
+  if (kinds == 0) return true;
+  const int64_t apart = static_cast<char*>(b.data_ptr()) - static_cast<char*>(a.data_ptr());
+  const int64_t at = apart - floor_div(apart, g) * g;
+  if (s.run <= at && at <= g - t.run) return false;
+  if (kinds > 2) return true;
+  auto more = [](const Steps& x, int64_t step) {
+    for (int i = 0; i < x.n; ++i)
+      if (x.step[i] == step) return x.more[i];
+    return int64_t{0};
+  };
+  // a run of b begins apart + x outer + y inner behind one of a: they meet between -t.run and s.run
+  const int64_t inner = kinds == 2 ? std::min(step[0], step[1]) : step[0], outer = kinds == 2 ? std::max(step[0], step[1]) : inner;
+  const int64_t y0 = -more(s, inner), y1 = more(t, inner);
+  int64_t x0 = kinds == 2 ? -more(s, outer) : 0, x1 = kinds == 2 ? more(t, outer) : 0;
+  x0 = std::max(x0, floor_div(-t.run - y1 * inner - apart, outer) + 1);
+  x1 = std::min(x1, -floor_div(apart + y0 * inner - s.run, outer) - 1);
+  if (x1 - x0 > 64) return true;
+  for (int64_t x = x0; x <= x1; ++x) {
+    const int64_t d = apart + x * outer;
+    if (std::max(y0, floor_div(-t.run - d, inner) + 1) <= std::min(y1, -floor_div(d - s.run, inner) - 1)) return true;
+  }
+  return false;
+}
+// Results that share no memory with an operand or another result: the first `results` of the tensors.
+template <int N>
+void own_memory(Reader& r, const Maybe (&t)[N], int results) {
+  if (!r.ok) return;
+  uintptr_t lo[N], hi[N];
+  for (int i = 0; i < N; ++i) {
+    lo[i] = hi[i] = 0;
+    if (!t[i] || t[i]->numel() == 0) continue;
+    const auto sizes = t[i]->sizes(), strides = t[i]->strides();
+    int64_t last = 0;
+    for (size_t d = 0; d < sizes.size(); ++d) last += (sizes[d] - 1) * strides[d];
+    lo[i] = reinterpret_cast<uintptr_t>(t[i]->data_ptr());
+    hi[i] = lo[i] + (uintptr_t)(last + 1) * t[i]->element_size();
+    for (int x = 0; x < std::min(i, results); ++x)
+      if (lo[x] < hi[i] && lo[i] < hi[x] && !r.need(!meet(*t[x], *t[i]))) return;
+  }
+}
 
 void read_scales(Reader& r, double k, double v, int code) {
   r.need(0.0 < k && k < kMost && 0.0 < v && v < kMost && (code == SB_F8 || (k == 1.0 && v == 1.0)));
@@ -211,11 +293,9 @@ PyObject* attend_of(PyObject* const* a, bool look) {
   void* const p_weight = read_account(r, weight, b, kv_heads, places, at::kFloat);
   void* const p_lse = read_account(r, lse, b, heads, tq, at::kFloat);
   Rows o{nullptr, width, tq * width};
-  if (out) {
-    o = read_rows(r, out, b, tq, width, q->scalar_type(), true);
-    r.need(!same_start(out, q) && !same_start(out, k) && !same_start(out, v));
-  }
-  r.need(!meet(weight, lse) && b > 0 && tq > 0 && tq < 1ll << 31);
+  if (out) o = read_rows(r, out, b, tq, width, q->scalar_type(), true);
+  r.need(b > 0 && tq > 0 && tq < 1ll << 31);
+  own_memory(r, {out, lse, weight, q, k, v, table, lens}, 3);
   if (!r.ok || !r.on_current_device()) Py_RETURN_NONE;
   if (look) Py_RETURN_TRUE;
   Work w;
@@ -266,8 +346,6 @@ PyObject* append_of(PyObject* const* a, bool look) {
   r.need((code == SB_F16 || code == SB_BF16) && (page_code == code || page_code == SB_F8) && t < kPlaces);
   read_scales(r, k_scale, v_scale, page_code);
   const Rows kr = read_rows(r, k, b, t, kv_heads * c.memory.dh, dtype), vr = read_rows(r, v, b, t, kv_heads * c.memory.dh, dtype);
-  r.need(!kr.p || (kr.p != c.memory.k && kr.p != c.memory.v));
-  r.need(!vr.p || (vr.p != c.memory.k && vr.p != c.memory.v));
   c.at = read_each(r, at, b);
   c.count = read_each(r, count, b);
   c.weight = static_cast<float*>(read_account(r, weight, b, kv_heads, places, at::kFloat));
@@ -281,7 +359,8 @@ PyObject* append_of(PyObject* const* a, bool look) {
     c.stamp_row = shape.size() == 2 ? stamp->stride(1) : 0;
   }
   c.after = read_each(r, after, b);
-  r.need(!meet(after, at) && !meet(after, count) && b > 0);
+  r.need(b > 0);
+  own_memory(r, {kp, vp, weight, born, after, k, v, table, at, count, stamp}, 5);
   if (!r.ok || !r.on_current_device()) Py_RETURN_NONE;
   if (look) Py_RETURN_TRUE;
   Tensor made;
@@ -323,14 +402,11 @@ PyObject* cut_of(PyObject* const* a, bool look) {
   c.born_out = static_cast<int*>(read_account(r, born_out, b, kv_heads, places, at::kInt));
   c.after = read_each(r, after, b);
   if (!r.ok) Py_RETURN_NONE;
-  // results of their own share no memory with an operand or one another
-  const Maybe own[3] = {weight_out && c.weight_out != c.weight ? weight_out : nullptr,
-                        born_out && c.born_out != c.born ? born_out : nullptr, after && c.after != c.lens ? after : nullptr};
-  const Maybe operands[5] = {weight, born, lens, since, keep};
-  for (int x = 0; x < 3; ++x) {
-    for (const Maybe o : operands) r.need(!meet(own[x], o));
-    for (int y = 0; y < x; ++y) r.need(!meet(own[x], own[y]));
-  }
+  // results that are an operand itself are no operands; lens may be since or keep too
+  const void* const here = c.after == c.lens ? c.after : nullptr;
+  own_memory(r, {kp, vp, weight_out, born_out, after, table, c.weight_out == c.weight ? nullptr : weight,
+                 c.born_out == c.born ? nullptr : born, c.lens == here ? nullptr : lens, c.since == here ? nullptr : since,
+                 c.keep == here ? nullptr : keep}, 5);
   r.need(b > 0);
   if (!r.ok || !r.on_current_device()) Py_RETURN_NONE;
   if (look) Py_RETURN_TRUE;

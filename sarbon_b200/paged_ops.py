@@ -14,7 +14,8 @@ or 128 channels; any page size; pages and rows any multiple of 16 bytes apart, s
 lie side by side).  ``table`` (int32 [B, N]) names the pages of an item's states: state j is row
 ``j % page`` of page ``table[b, j // page]``.  A number outside [0, P) is no page: its states are neither
 written nor read and take no part.  Pages may be shared by items that only read them.  Lengths (int32 [B])
-outside [0, N * page] are clamped.
+outside [0, N * page] are clamped.  What a call writes shares no memory with what it reads or else writes; rows may lie
+between one another, as keys and values side by side do.
 
 ``weight`` (fp32) and ``born`` (int32), ``[B, kv_heads, N * page]``, hold for each state and key head how much it was
 looked at and its stamp (a frame number, say).  Eviction decides for each key head by itself, so a row's heads may
@@ -28,6 +29,7 @@ capture.  No graph of gradients is recorded; tensors that would need one are ref
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 
 import torch
@@ -35,7 +37,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, lib
-from .memory_ops import _apart, _device, _new, _raw_stream, _ready, _rows, _statistics, _work
+from .memory_ops import _device, _new, _raw_stream, _ready, _rows, _statistics, _work
 
 E4M3 = torch.float8_e4m3fn
 _MOST = 3.4e38  # of fp32
@@ -111,8 +113,6 @@ def _memory(k_pages, v_pages, table, kv_heads, written=False):
         if not (k_row >= width <= v_row and k_img >= k_row * page and v_img >= v_row * page) and \
                 (_overlap(k_row, k_img, *shape) or _overlap(v_row, v_img, *shape)):
             raise ValueError("pools: rows overlap")
-        if k == v and pages:
-            raise ValueError("results need their own memory")
     if table.dtype != _INT or table.dim() != 2:
         raise ValueError("table: int32 [B, N] with contiguous rows")
     (b, n), step = table.shape, table.stride()
@@ -163,15 +163,62 @@ def _scales(k_scale, v_scale, dtype):
         raise ValueError("k_scale, v_scale: of e4m3 pages only")
 
 
-def _clear_of(results, operands):
-    """Contiguous results that share no memory with an operand or another result."""
-    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in operands if t is not None and t.numel()]
-    for t in results:
-        if t is not None and t.numel():
-            lo, hi = t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
-            if any(lo < y and x < hi for x, y in spans):
+def _steps(t):
+    """A tensor's memory: bytes of its contiguous runs, and how often each step (in bytes) goes on from the first."""
+    size = run = t.element_size()
+    steps = {}
+    for step, n in sorted(zip(t.stride(), t.shape)):
+        if n > 1 and step:
+            step *= size
+            if step == run and not steps:
+                run *= n
+            else:
+                steps[step] = steps.get(step, 0) + n - 1
+    return run, steps
+
+
+def _meet(a, b):
+    """Whether two tensors, whose first to last bytes overlap, share memory.  Rows that lie between the other's, of up to two
+    different strides in all, are told apart; others only where a common divisor of their strides has room for both."""
+    (run, mine), (width, its) = _steps(a), _steps(b)
+    apart, steps = b.data_ptr() - a.data_ptr(), sorted(mine.keys() | its.keys())
+    if not steps:
+        return True
+    g = math.gcd(*steps)
+    if run <= apart % g <= g - width:
+        return False
+    if len(steps) > 2:
+        return True
+    # a run of b begins apart + x outer + y inner behind one of a: they meet between -width and run
+    inner, outer = steps[0], steps[-1]
+    y0, y1 = -mine.get(inner, 0), its.get(inner, 0)
+    x0, x1 = (-mine.get(outer, 0), its.get(outer, 0)) if outer != inner else (0, 0)
+    x0 = max(x0, (-width - y1 * inner - apart) // outer + 1)
+    x1 = min(x1, -((apart + y0 * inner - run) // outer) - 1)
+    if x1 - x0 > 64:
+        return True
+    for d in range(apart + x0 * outer, apart + x1 * outer + 1, outer):
+        if max(y0, (-width - d) // inner + 1) <= min(y1, -((d - run) // inner) - 1):
+            return True
+    return False
+
+
+def _own_memory(results, operands):
+    """Results that share no memory with an operand or another result."""
+    spans = []
+    for group in results, operands:
+        for t in group:
+            if t is not None and t.numel():
+                lo = t.data_ptr()
+                last = sum((n - 1) * step for n, step in zip(t.shape, t.stride()))
+                spans.append((lo, lo + (last + 1) * t.element_size(), group is results, t))
+    spans.sort(key=lambda x: x[0])
+    for i, (lo, hi, result, t) in enumerate(spans):
+        for other in spans[i + 1:]:
+            if other[0] >= hi:
+                break
+            if (result or other[2]) and _meet(t, other[3]):
                 raise ValueError("results need their own memory")
-            spans.append((lo, hi))
 
 
 # ---------------------------------------------------------------- attention
@@ -225,11 +272,9 @@ def paged_attention(q, k_pages, v_pages, table, lens, heads, kv_heads=None, scal
     if lse is not None:
         _statistics(lse, b, heads, tq)
         p_lse = lse.data_ptr()
-        if weight is not None:
-            _clear_of((weight, lse), ())
     if out is not None:
         op = _rows(out, "out", shape, dtype, out=True)
-        _apart((out,), (q, k_pages, v_pages))
+    _own_memory((out, lse, weight), (q, k_pages, v_pages, table, lens))
     index = _one_device((q, k_pages, v_pages, weight, out, lse), (table, lens))
     if out is None:
         out, op = _new(q, shape, dtype)
@@ -253,7 +298,7 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
     most 448 of either sign.  The new states' weight becomes 0 and born their stamp (int32 [B, T], or [B] for
     all of an item's).  States behind an item's pages are dropped, rows on no page are not written, and what
     lies from ``count[b]`` on is left alone.  An item's pages that are written must be its own.  after
-    (allocated if None) shares no memory with at.  kv_heads is that of weight or born where they are given;
+    is allocated if None.  kv_heads is that of weight or born where they are given;
     without them the rows are taken as heads of 32 channels."""
     if k.is_cuda and forward_ad._current_level < 0:
         done = (_native or _load()).append(k, v, k_pages, v_pages, table, at, count, k_scale, v_scale, weight, born, stamp,
@@ -279,9 +324,6 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
     t = rows[1]
     shape = (b, t, kv_heads * dim)
     kp, vp = _rows(k, "k", shape, dtype), _rows(v, "v", shape, dtype)
-    pools = k_pages.data_ptr(), v_pages.data_ptr()
-    if (kp[0] in pools or vp[0] in pools) and kp[0]:
-        raise ValueError("results need their own memory")
     if at is None:
         raise ValueError("at: contiguous int32 [B]")
     p_at, p_count, p_weight, p_born, sp = _each(at, "at", b), 0, 0, 0, _NO_STAMP
@@ -297,7 +339,7 @@ def paged_write(k, v, k_pages, v_pages, table, at, count=None, k_scale=1.0, v_sc
         sp = stamp.data_ptr(), step[0], step[1] if len(step) == 2 else 0
     if after is not None:
         p_after = _each(after, "after", b)
-        _clear_of((after,), (at, count))
+    _own_memory((k_pages, v_pages, weight, born, after), (k, v, table, at, count, stamp))
     index = _one_device((k, v, k_pages, v_pages, weight), (table, at, count, born, stamp, after))
     if after is None:
         after = torch.empty_like(at)
@@ -352,18 +394,20 @@ def paged_evict(k_pages, v_pages, table, lens, weight, keep, born=None, since=No
         if keep_all < 0 or keep_all != min(keep, 1 << 30):
             raise ValueError("keep: a whole number from 0 on, or int32 [B]")
     pwo = pbo = p_after = 0
-    if weight_out is not None or born_out is not None or after is not None:
-        own = []
-        if weight_out is not None:
-            pwo = _account(weight_out, "weight_out", places, _FLOAT)
-            own.append(weight_out if pwo != pw else None)
-        if born_out is not None:
-            pbo = _account(born_out, "born_out", places, _INT)
-            own.append(born_out if pbo != pb else None)
-        if after is not None:
-            p_after = _each(after, "after", b)
-            own.append(after if p_after != p_lens else None)
-        _clear_of(own, (weight, born, lens, since, keep if p_keep else None))
+    operands = [table]
+    if weight_out is not None:
+        pwo = _account(weight_out, "weight_out", places, _FLOAT)
+    if weight_out is None or pwo != pw:
+        operands.append(weight)
+    if born_out is not None:
+        pbo = _account(born_out, "born_out", places, _INT)
+    if born_out is None or pbo != pb:
+        operands.append(born)
+    if after is not None:
+        p_after = _each(after, "after", b)
+    here = p_after if p_after == p_lens else 0  # (lens may be since or keep too)
+    operands += [t for t, p in ((lens, p_lens), (since, p_since), (keep if p_keep else None, p_keep)) if p != here]
+    _own_memory((k_pages, v_pages, weight_out, born_out, after), operands)
     index = _one_device((k_pages, v_pages, weight, weight_out),
                         (table, lens, born, since, keep if p_keep else None, born_out, after))
     if after is None:
