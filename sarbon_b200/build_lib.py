@@ -1,5 +1,6 @@
-"""Build ``libsarbon_sparse.so`` (the C ABI in ``include/sarbon_sparse.h``) for sm_100a, and ``_paged_calls.so``, the
-Python module through which the paged memory's calls reach it.
+"""Build ``libsarbon_sparse.so`` (the C ABI in ``include/sarbon_sparse.h``) for sm_100a, and ``_paged_calls``, the
+Python module through which the paged memory's calls reach it with little host time.  The library needs neither Python nor
+torch; where the module cannot be built, the Python side makes its calls.
 
 The library is built in-tree next to this file so that it travels with the source
 tree; object files go to ``sarbon_b200/_build``.  Usage::
@@ -12,6 +13,8 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -19,7 +22,9 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libsarbon_sparse.so"
-CALLS_SOURCE, CALLS_LIB = CSRC / "sb_paged_calls.cpp", PKG / "_paged_calls.so"
+# (named for its interpreter: no other one looks at it)
+CALLS_SOURCE, CALLS_LIB = CSRC / "sb_paged_calls.cpp", PKG / f"_paged_calls{sysconfig.get_config_var('EXT_SUFFIX')}"
+CALLS_FOR = OBJ / "paged_calls_built_for.txt"  # the torch that it was built against
 SOURCES = ["sb_engine.cu", "sb_gate.cu", "sb_conv_tc.cu", "sb_conv_simt.cu", "sb_noalloc.cu", "sb_cells.cu", "sb_boxes.cu",
            "sb_prep.cu", "sb_deform.cu", "sb_gemm.cu", "sb_detops.cu", "sb_attn.cu", "sb_xattn.cu", "sb_xattn_few.cu", "sb_xattn_bwd.cu",
            "sb_rope.cu", "sb_gnorm.cu", "sb_paged_attn.cu", "sb_paged_cache.cu"]
@@ -54,30 +59,44 @@ def _run(what, cmd):
 
 def build_calls(force: bool = False, verbose: bool = False) -> Path:
     """Compile the Python module against the installed torch."""
-    import sysconfig
-
     import torch
     header = PKG.parent / "include" / "sarbon_sparse.h"
     root = Path(torch.__file__).resolve().parent
-    newest = max(p.stat().st_mtime for p in (CALLS_SOURCE, header, root / "version.py"))
-    if CALLS_LIB.exists() and not force and CALLS_LIB.stat().st_mtime > newest:
+    newest = max(p.stat().st_mtime for p in (CALLS_SOURCE, header))
+    if not force and CALLS_LIB.exists() and CALLS_LIB.stat().st_mtime > newest and CALLS_FOR.exists() and \
+            CALLS_FOR.read_text() == torch.__version__:
         return CALLS_LIB
     cuda = Path(nvcc()).resolve().parents[1]
     found = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"],
              cuda / "include"]
     tmp = CALLS_LIB.with_suffix(".so.tmp")
     _run("g++", ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{header.parent}",
-                 *(x for p in found for x in ("-isystem", str(p))), str(CALLS_SOURCE), "-o", str(tmp), f"-L{root / 'lib'}", "-lc10",
-                 "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"])
+                 f'-DSB_BUILT_FOR="{torch.__version__}"', *(x for p in found for x in ("-isystem", str(p))), str(CALLS_SOURCE),
+                 "-o", str(tmp), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"])
     os.replace(tmp, CALLS_LIB)
+    OBJ.mkdir(exist_ok=True)
+    CALLS_FOR.write_text(torch.__version__)
     if verbose:
         print(f"built {CALLS_LIB}")
     return CALLS_LIB
 
 
 def build(force: bool = False, extra=(), verbose: bool = False) -> Path:
-    """Compile every CUDA source for sm_100a and link the shared library; then the Python module."""
-    build_calls(force, verbose)
+    """Build the shared library, then the Python module, without which all goes on."""
+    lib = build_library(force, extra, verbose)
+    for old in PKG.glob("_paged_calls*.so"):
+        if old != CALLS_LIB:  # another interpreter's, or of no interpreter's name, against other declarations
+            old.unlink()
+    try:
+        build_calls(force, verbose)
+    except (RuntimeError, OSError, ImportError) as e:
+        CALLS_LIB.unlink(missing_ok=True)  # what is there was built for something else
+        warnings.warn(f"_paged_calls was not built, small calls of the paged memory take longer on the host: {e}", RuntimeWarning)
+    return lib
+
+
+def build_library(force: bool = False, extra=(), verbose: bool = False) -> Path:
+    """Compile every CUDA source for sm_100a and link the shared library."""
     srcs = [CSRC / s for s in SOURCES] + list(CSRC.glob("*.cuh")) + [PKG.parent / "include" / "sarbon_sparse.h"]
     if LIB.exists() and not force:
         newest = max(p.stat().st_mtime for p in srcs)

@@ -493,4 +493,12 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_paged_calls", "The paged memory
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__paged_calls() { return PyModule_Create(&g_module); }
+// built_for: the version of torch, of whose tensors' layout the reads above know.
+PyMODINIT_FUNC PyInit__paged_calls() {
+  PyObject* const m = PyModule_Create(&g_module);
+  if (m && PyModule_AddStringConstant(m, "built_for", SB_BUILT_FOR) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

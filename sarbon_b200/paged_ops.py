@@ -31,6 +31,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+import warnings
 
 import torch
 from torch.autograd import forward_ad
@@ -57,15 +58,26 @@ CALLS = [0]
 _native = None
 
 
+class _PythonSide:
+    """In place of the native module: every call is left to the Python side."""
+    attend = append = cut = staticmethod(lambda *arguments: None)
+
+
 def _load():
     """The module that makes plainly right calls with little host time.  Measured, us a call with one token, with the checks
-    below and there: attention 11.8 and 8.2 (5.0 of them the host's), writing 13.5 and 5.4, evicting 14.8 and 10.3."""
+    below and there: attention 11.8 and 8.2 (5.0 of them the host's), writing 13.5 and 5.4, evicting 14.8 and 10.3.  Without
+    it, or where it was built for another torch, all calls are made from here."""
     global _native
     so = lib()
     try:
         from . import _paged_calls
+        if _paged_calls.built_for != torch.__version__:
+            raise ImportError(f"built for torch {_paged_calls.built_for}")
     except ImportError as e:
-        raise _lib.SarbonLibraryError(f"cannot load _paged_calls.so: {e}; build it with `python -m sarbon_b200.build_lib`") from e
+        warnings.warn(f"_paged_calls is not used ({e}), small calls take longer on the host; it is built by "
+                      "`python -m sarbon_b200.build_lib`", RuntimeWarning, stacklevel=3)
+        _native = _PythonSide
+        return _native
     _paged_calls.setup(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
         so.sb_paged_attention, so.sb_paged_attention_work, so.sb_paged_write, so.sb_paged_evict, so.sb_paged_evict_work)), check)
     _native = _paged_calls
