@@ -602,6 +602,8 @@ SB_API int sb_paged_write(const sb_paged_append* call, void* stream);
  * since[b], weight descending, index) stay (NaN is the least; since NULL: weight alone).  The i-th freed place
  * below keep takes the i-th kept state from keep on.  weight_out and born_out get the weights and stamps
  * that stay, 0 from the new length on; after [B] the new lengths.  They may be weight, born and lens themselves.
+ * Weights and stamps alone decide: each of the lens[b] states of an item that has more than keep[b] needs a page.  (A
+ * row is moved only where both places have one; weights and stamps move all the same.)
  * work: sb_paged_evict_work bytes, as above. */
 typedef struct {
   sb_paged_memory memory;

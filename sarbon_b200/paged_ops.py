@@ -13,8 +13,8 @@ there, and once there is more than the budget allows, the states that were looke
 or 128 channels; any page size; pages and rows any multiple of 16 bytes apart, so keys and values may
 lie side by side).  ``table`` (int32 [B, N]) names the pages of an item's states: state j is row
 ``j % page`` of page ``table[b, j // page]``.  A number outside [0, P) is no page: its states are neither
-written nor read and take no part.  Pages may be shared by items that only read them.  Lengths (int32 [B])
-outside [0, N * page] are clamped.  What a call writes shares no memory with what it reads or else writes; rows may lie
+written nor read and take no part in attention (eviction does not ask for a page, see there).  Pages may be shared by items
+that only read them.  Lengths (int32 [B]) outside [0, N * page] are clamped.  What a call writes shares no memory with what it reads or else writes; rows may lie
 between one another, as keys and values side by side do.
 
 ``weight`` (fp32) and ``born`` (int32), ``[B, kv_heads, N * page]``, hold for each state and key head how much it was
@@ -376,8 +376,11 @@ def paged_evict(k_pages, v_pages, table, lens, weight, keep, born=None, since=No
     on: keys, values, weight and stamp; nothing else moves.  Returns (after, weight, born): the new
     lengths ``min(lens, keep)``, and weights and stamps [B, kv_heads, N * page] with 0 from the new length on
     (born None without born).  after, weight_out and born_out (allocated if None) may be lens, weight and born
-    themselves and otherwise share no memory with them.  An item's pages must be its own; rows on
-    no page are not moved."""
+    themselves and otherwise share no memory with them.  An item's pages must be its own.
+
+    Weights and stamps alone decide, also among states on no page.  So each of the ``lens[b]`` states of an item that has
+    more than keep needs a page: a row is moved only where both places have one, and where one of them has none, the
+    weight and stamp that move to a place are no longer those of the row that lies there."""
     if weight.is_cuda and forward_ad._current_level < 0:
         done = (_native or _load()).cut(k_pages, v_pages, table, lens, weight, keep, born, since, weight_out, born_out, after)
         if done is not None:

@@ -142,3 +142,45 @@ def test_memories_without_places():
     assert after.tolist() == [0, 0] and w.shape == weight.shape and r.shape == born.shape
     sb.paged_evict(k, v, table, lens, weight, 3, born=born, since=ints(1, 1), weight_out=weight, born_out=born, after=lens)
     assert lens.tolist() == [0, 0] and (k == 1).all() and (v == 1).all()
+
+
+@pytest.mark.parametrize("n,keep,kv_heads,page", [(241, 240, 4, 16), (3000, 1100, 2, 7), (4090, 2000, 1, 64), (9000, 8000, 3, 60), (70000, 20000, 2, 240)])
+def test_evicted_states_leave_nothing_behind(n, keep, kv_heads, page):
+    """Each row carries the number of its state: afterwards a place's row, weight and stamp are one state's, no state is there
+    twice, and none that went.  Entries from the last state's page on are no pages."""
+    import sarbon_b200 as sb
+    g = gen(n)
+    b, dim = 3, 32
+    lens = ints(n, n - 1, keep + 1)
+    k, v, table = pages_of(g, b, n + 3 * page, page, kv_heads * dim, torch.float16)
+    cap = table.shape[1] * page
+    table.masked_fill_(torch.arange(table.shape[1], device="cuda") * page >= lens[:, None], -1)
+    state = torch.arange(cap, device="cuda")
+    number = torch.stack([state % 1024, state // 1024]).half()  # exact in fp16
+    for pool, sign in ((k, 1), (v, -1)):
+        rows = pool.view(-1, page, kv_heads, dim)
+        for i in range(b):
+            ok = table[i] >= 0
+            some = number.view(2, -1, page)[:, ok].permute(1, 2, 0)
+            rows[table[i][ok].long(), :, :, :2] = sign * some[:, :, None]
+            rows[table[i][ok].long(), :, :, 2] = torch.arange(kv_heads, device="cuda").half()
+    weight = torch.rand(b, kv_heads, cap, device="cuda", generator=g)
+    born = torch.randint(0, 1000, weight.shape, dtype=torch.int32, device="cuda", generator=g)
+    since = ints(990, 0, 500)
+    after, w, r = sb.paged_evict(k, v, table, lens, weight, keep, born=born, since=since)
+    assert after.tolist() == [keep] * b
+    for i in range(b):
+        for pool, sign in ((k, 1), (v, -1)):
+            rows = pool.view(-1, page, kv_heads, dim)[table[i][: -(-keep // page)].long()].flatten(0, 1)[:keep]
+            was = (sign * (rows[..., 0].double() + 1024 * rows[..., 1].double())).long().t()
+            assert (rows[..., 2].t() == torch.arange(kv_heads, device="cuda")[:, None]).all()
+            assert torch.equal(w[i, :, :keep], weight[i].gather(1, was)) and torch.equal(r[i, :, :keep], born[i].gather(1, was))
+            assert (was < lens[i]).all() and (was.sort(-1).values.diff(dim=-1) > 0).all()
+            stays = torch.zeros(kv_heads, cap, dtype=torch.bool, device="cuda").scatter_(1, was, True)
+            guarded = born[i] >= since[i]
+            gone = ~stays & (state < lens[i])
+            # none that went is before one that stays
+            for h in range(kv_heads):
+                if gone[h].any():
+                    best = (guarded[h].double() * 2 + weight[i, h].double())
+                    assert best[gone[h]].max() <= best[stays[h]].min()
