@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_paged_ops import formula, gen, ints, pages_of, rand, rows_of, same_bits, unit
+from test_gpu_paged_ops import E4M3, check_attention, formula, gen, ints, pages_of, rand, rows_of, same_bits, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -184,3 +184,23 @@ def test_evicted_states_leave_nothing_behind(n, keep, kv_heads, page):
                 if gone[h].any():
                     best = (guarded[h].double() * 2 + weight[i, h].double())
                     assert best[gone[h]].max() <= best[stays[h]].min()
+
+
+@pytest.mark.parametrize("qt,n", [(torch.bfloat16, 3000), (torch.float16, 3000), (torch.bfloat16, 20000), (torch.bfloat16, 200)])
+def test_attention_ramps_on_e4m3(qt, n):
+    """Scores that rise over one item's e4m3 states and fall over the other's: the running maximum grows with every chunk."""
+    import sarbon_b200 as sb
+    g = gen(n)
+    b, heads, dim, page = 2, 4, 64, 50
+    k, v, table = pages_of(g, b, n, page, dim, E4M3)
+    q = rand(g, b, 1, heads * dim, by=0.5).abs().to(qt)
+    ramp = torch.linspace(-12, 12, table.shape[1] * page, device="cuda")[:, None]
+    for i, r in enumerate((ramp, -ramp)):
+        rows = (rand(g, table.shape[1] * page, dim) * 0.1 + r).to(E4M3).view(-1, page, dim)
+        k.view(torch.uint8)[table[i].long()] = rows.view(torch.uint8)
+    lens = ints(n, n)
+    scores = (q.double().view(b, heads, dim) @ k.float()[table.long()].flatten(1, 2)[:, :n].double().transpose(1, 2)).argmax(-1)
+    assert (scores[0] > n * 0.9).all() and (scores[1] < n * 0.1).all()
+    lse, weight = torch.empty(b, heads, 1, device="cuda"), torch.zeros(b, 1, table.shape[1] * page, device="cuda")
+    out = sb.paged_attention(q, k, v, table, lens, heads, kv_heads=1, scale=0.25, k_scale=0.5, lse=lse, weight=weight)
+    check_attention(out, lse, weight, q, k, v, table, lens, heads, 1, before=torch.zeros_like(weight), scale=0.25, k_scale=0.5)
