@@ -19,8 +19,8 @@
 // beside 4 dim bytes of K and V, most of them from the L2.
 //
 // 64 x 1 token on 8160 ragged states of 4 key heads of 128, 16 query heads, with the account: bf16 165 to 172 us (157 for
-// 961 MB with the scores, 6.1 TB/s, 94 % of the copy rate; 11 the second kernel), e4m3 97 to 100 (84 for 495 MB, 90 %, and
-// 41 % of the issue slots).  One stream of 130,560 states 56 (47 for 267 MB: start and end; 7 the second kernel).  16 x 8
+// 961 MB with the scores, 6.1 TB/s, 94 % of the copy rate; 11 the second kernel), e4m3 97 to 100 (84 for 495 MB, 90 %; 11 the
+// second kernel and its launch).  One stream of 130,560 states 56 (47 for 267 MB: start and end; 7 the second kernel).  16 x 8
 // causal tokens on 42,840 of 4 heads of 64: 173 to 180; the scores of 16 rows a state, written and read, are 350 MB
 // beside 601 of K and V.
 #include <algorithm>
@@ -166,8 +166,8 @@ template <int DH, int PT, int NB>
 struct Paged {
   static constexpr bool E4M3 = PT == SB_F8, BF16 = PT == SB_BF16;
   static constexpr int RB = DH * (E4M3 ? 1 : 2);                // bytes a state and head
-  // Two CTAs an SM, 24 KB a warp on their way.  e4m3 waits for instructions more than for memory: three CTAs (83 us
-  // for the 64 x 8160 states above, 92 with two).
+  // Two CTAs an SM, 24 KB a warp on their way.  e4m3 has twice the instructions a byte (41 % of the issue slots): three
+  // CTAs (83 us for the 64 x 8160 states above, 92 with two).
   static constexpr int OCC = E4M3 && NB == 1 ? 3 : 2;
   static constexpr int kRing = OCC == 3 ? 16 * 1024 : 24 * 1024;  // bytes a warp
   static constexpr int CK = 4096 / RB < 64 ? 4096 / RB : 64;      // states a chunk

@@ -144,7 +144,9 @@ __global__ void __launch_bounds__(kWriteWarps * 32, MODE == 2 ? 2 : 4)
 //
 // What bounds it: the chain of passes, each with an exchange of counts.  16 x 8 units of 18,360 states, 2040 of them to
 // go, rows of 256 bytes: 24 us for the selection, 13.5 for the rows (82 MB, 93 % of the copy rate); 2 x 8 of 130,560, half
-// of them, rows of 64 bytes: 34.7 and 40 (150 MB in pieces of 64 bytes: 58 %).
+// of them, rows of 64 bytes: 34.7 and 40 (150 MB in pieces of 64 bytes: 58 %).  Each pass looks at all keys again, though after
+// the first only one bin's matter, and a few hundred places take the bins and barriers of many: 8.8 us for 241.  At 64
+// registers (two CTAs an SM) the selection spills 100 bytes a thread, as many with four stamps' loads at once as with nine.
 struct EvictArgs {
   Pool k, v;
   PageTable pages;

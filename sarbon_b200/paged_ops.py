@@ -247,10 +247,13 @@ def paged_attention(q, k_pages, v_pages, table, lens, heads, kv_heads=None, scal
 
     weight (fp32 [B, kv_heads, N * page]), if given, is brought up to date: ``weight[b, h, j] = decay *
     weight[b, h, j] +`` the probabilities that the queries of key head h gave to state j, for the ``lens[b]`` states;
-    sums have a fixed order.  Without queries (Tq 0) that is ``decay`` times it.  This takes a workspace of 4 bytes a query row, key head and place.
+    sums have a fixed order.  Without queries (Tq 0) that is ``decay`` times it.  This takes a workspace of 4 bytes for each
+    key head, place of the table (``N * page``, whatever the lengths) and query row, rows of a key head up to 16 counted as 1, 2,
+    4, 8 or 16, more as a multiple of 16; none where a few hundred places' scores stay in shared memory.
 
-    Made for single tokens: the states are read once for every 16 query rows of a key head, and split
-    over the SMs where there are few rows; many queries want cross_attention."""
+    Made for single tokens: the states are read once for every 16 query rows of a key head (``Tq * heads // kv_heads``), and
+    split over the SMs where there are few rows.  So 300 queries read them 19 times; cross_attention reads them once, but
+    wants the memory in one piece and of q's type."""
     if q.is_cuda and forward_ad._current_level < 0:
         done = (_native or _load()).attend(q, k_pages, v_pages, table, lens, heads, kv_heads, scale, causal, k_scale, v_scale,
                                            weight, decay, out, lse)
