@@ -14,8 +14,8 @@ or 128 channels; any page size; pages and rows any multiple of 16 bytes apart, s
 lie side by side).  ``table`` (int32 [B, N]) names the pages of an item's states: state j is row
 ``j % page`` of page ``table[b, j // page]``.  A number outside [0, P) is no page: its states are neither
 written nor read and take no part in attention (eviction does not ask for a page, see there).  Pages may be shared by items
-that only read them.  Lengths (int32 [B]) outside [0, N * page] are clamped.  What a call writes shares no memory with what it reads or else writes; rows may lie
-between one another, as keys and values side by side do.
+that only read them.  Lengths (int32 [B]) outside [0, N * page] are clamped.  What a call writes shares no memory with what
+it reads or else writes; rows may lie between one another, as keys and values side by side do.
 
 ``weight`` (fp32) and ``born`` (int32), ``[B, kv_heads, N * page]``, hold for each state and key head how much it was
 looked at and its stamp (a frame number, say).  Eviction decides for each key head by itself, so a row's heads may
