@@ -408,7 +408,7 @@ def paged_evict(k_pages, v_pages, table, lens, weight, keep, born=None, since=No
     if isinstance(keep, torch.Tensor):
         p_keep = _each(keep, "keep", b)
     else:
-        keep_all = min(int(keep), 1 << 30)
+        keep_all = min(int(keep), 1 << 30) if 0 <= keep < math.inf else -1
         if keep_all < 0 or keep_all != min(keep, 1 << 30):
             raise ValueError("keep: a whole number from 0 on, or int32 [B]")
     pwo = pbo = p_after = 0
