@@ -359,6 +359,9 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
   constexpr bool E4M3 = C::E4M3, BF16 = C::BF16;
   constexpr int CK = C::CK, KT = CK / 16, KS = DH / 16, R = CK > 32 ? 2 : 1;
   constexpr float lift = kLift<BF16>;
+  // bf16 values reach fp32's end, and a sum of them beyond it (p up to 2^8 a state): P meets V 2^40 times smaller, which is
+  // exact down to p = 2^-86 and leaves room for 2^30 states
+  constexpr float room_for = BF16 ? 0x1p-40f : 1.f;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ ulonglong2 place[kWarps][CK];      // addresses of a chunk's rows of K and V
   __shared__ uint64_t there[kWarps][C::STAGES];  // a stage's rows that take part, as bits
@@ -673,7 +676,7 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
           for (int y = 0; y < NB; ++y)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const float u = s[kt][y][2 * x], w = s[kt][y][2 * x + 1];
+              const float u = s[kt][y][2 * x] * room_for, w = s[kt][y][2 * x + 1] * room_for;
               const uint32_t h = pack16<BF16>(u, w);
               const float2 f = pair_of(h, BF16 ? SB_BF16 : SB_F16);
               hi[y][x] = transposed(h);
@@ -724,7 +727,7 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
             for (int y = 0; y < NB; ++y)
 #pragma unroll
               for (int z = 0; z < 2; ++z)
-                p[y][z] = __shfl_sync(0xFFFFFFFFu, k < 8 ? s[kt][y][z] : s[kt][y][2 + z], (k & 7) * 4 + tig);
+                p[y][z] = room_for * __shfl_sync(0xFFFFFFFFu, k < 8 ? s[kt][y][z] : s[kt][y][2 + z], (k & 7) * 4 + tig);
 #pragma unroll
             for (int x = 0; x < KS; ++x)
 #pragma unroll
@@ -798,7 +801,7 @@ __global__ void __launch_bounds__(kWarps * 32, Paged<DH, PT, NB>::OCC)
         for (int u = 0; u < 8; ++u) f[u] = fmaf(k, v[u], f[u]);
       }
       const bool none = top == -INFINITY;  // no states
-      const float inv = none ? 0.f : a.v_scale / sum;
+      const float inv = none ? 0.f : a.v_scale / room_for / sum;
 #pragma unroll
       for (int u = 0; u < 8; ++u) f[u] = none ? 0.f : f[u] * inv;
       const float log_sum = none ? -INFINITY : top - lift + log2f(sum);

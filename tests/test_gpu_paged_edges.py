@@ -73,6 +73,29 @@ def test_attention_infinite_values(b, tq, n, heads, kv_heads, dim, page, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("b,tq,n,heads,kv_heads,dim,page", [(2, 1, 240, 8, 4, 32, 20), (1, 1, 2048, 4, 4, 128, 60), (2, 9, 9001, 4, 2, 64, 13)])
+def test_attention_values_of_the_largest_size(b, tq, n, heads, kv_heads, dim, page, dtype):
+    """Sums over states stay in fp32's range: values at the type's largest, of one sign and of both, give what lies among them."""
+    import sarbon_b200 as sb
+    g = gen(n)
+    top = torch.finfo(dtype).max
+    k, v, table = pages_of(g, b, n, page, kv_heads * dim, dtype)
+    v.copy_(torch.where(torch.rand(v.shape, device="cuda", generator=g) < 0.5, top, -top))
+    v[..., ::3] = top
+    v[..., 1::9] = -top
+    q = rand(g, b, tq, heads * dim, dtype=dtype)
+    lens = torch.tensor([n - 3 * i for i in range(b)], dtype=torch.int32, device="cuda")
+    for causal in (False, True):
+        put(v, table, 0, n - 1, 3, math.inf)  # (a causal call's odd states too)
+        out = sb.paged_attention(q, k, v, table, lens, heads, kv_heads=kv_heads, causal=causal)
+        ref, _, _, absolute, whole, e = formula(q, k, v, table, lens, heads, kv_heads, causal=causal)
+        tol = unit(dtype) * ref.abs() + (unit(dtype) ** 2 + e) * absolute + 2.0 ** -32 * whole
+        tol, ref = rows_of(tol, b, tq), rows_of(ref, b, tq)
+        known = ~ref.isnan()
+        assert ((out.double() - ref).abs()[known] <= 1.02 * tol[known]).all() and (out.float()[~known] == math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("n", [200, 1900, 9000])
 def test_attention_infinite_values_of_little_weight(n, dtype):
     """States whose share is far below the 16-bit types' smallest step, in the first, a middle and the last place."""
